@@ -1,5 +1,5 @@
-"""ctypes binding of the C ABI in `include/attnres_hip.h`, and the loader of
-the eager autograd nodes.
+"""ctypes binding of the C ABI in `include/attnres_hip.h` and
+`include/attnres_layers_hip.h`, and the loader of the eager autograd nodes.
 
 The shared library `_lib/libattnres_hip.so` is built in-tree from
 `csrc/attnres_hip.hip` by `build_native.py` (hipcc, gfx950), and so is
@@ -91,6 +91,32 @@ SIGNATURES = {
                                                _c_void_p]),
 }
 
+# The layers' entry points (attnres_layers_hip.h), likewise.
+LAYER_SIGNATURES = {
+    "attnres_hip_layer_norm_forward": (ctypes.c_int, [
+        _c_void_p, _i64, _i64, _i64, ctypes.c_int, _c_void_p, _c_void_p, ctypes.c_int, _f32, _c_void_p, _c_void_p,
+        _c_void_p]),
+    "attnres_hip_layer_norm_workspace_elems": (_i64, [_i64, _i64]),
+    "attnres_hip_layer_norm_backward": (ctypes.c_int, [
+        _c_void_p, _c_void_p, _i64, _i64, _i64, ctypes.c_int, _c_void_p, ctypes.c_int, _c_void_p, _c_void_p,
+        _c_void_p, _c_void_p, _c_void_p, _i64, _c_void_p]),
+    "attnres_hip_embedding_forward": (ctypes.c_int, [
+        _c_void_p, ctypes.c_int, _i64, _i64, _c_void_p, _i64, _i64, ctypes.c_int, _c_void_p, _f32, _c_void_p,
+        ctypes.c_int, _c_void_p]),
+    "attnres_hip_embedding_workspace_bytes": (_i64, [_i64, _i64, _i64, _i64]),
+    "attnres_hip_embedding_backward": (ctypes.c_int, [
+        _c_void_p, ctypes.c_int, _c_void_p, ctypes.c_int, _i64, _i64, _i64, _i64, ctypes.c_int, _f32, _c_void_p,
+        _c_void_p, _i64, _c_void_p, _i64, _c_void_p]),
+    "attnres_hip_loss_saved_bytes": (_i64, [_i64]),
+    "attnres_hip_loss_workspace_bytes": (_i64, [_i64, _i64, _i64, ctypes.c_int, ctypes.c_int]),
+    "attnres_hip_loss_forward": (ctypes.c_int, [
+        _c_void_p, _i64, _c_void_p, _i64, _c_void_p, ctypes.c_int, _i64, _i64, _i64, ctypes.c_int, _i64, ctypes.c_int,
+        _c_void_p, _c_void_p, _c_void_p, _i64, _c_void_p]),
+    "attnres_hip_loss_backward": (ctypes.c_int, [
+        _c_void_p, _i64, _c_void_p, _i64, _i64, _i64, _i64, ctypes.c_int, ctypes.c_int, _c_void_p, _c_void_p,
+        _c_void_p, _c_void_p, _c_void_p, _i64, _c_void_p]),
+}
+
 _lock = threading.Lock()
 _library: ctypes.CDLL | None = None
 
@@ -111,7 +137,7 @@ def load() -> ctypes.CDLL:
                 library = ctypes.CDLL(str(path))
             except OSError as error:
                 raise RuntimeError(f"attnres HIP extension failed to load: {error}") from error
-            for name, (restype, argtypes) in SIGNATURES.items():
+            for name, (restype, argtypes) in (*SIGNATURES.items(), *LAYER_SIGNATURES.items()):
                 function = getattr(library, name)
                 function.restype = restype
                 function.argtypes = argtypes
@@ -158,4 +184,4 @@ def check(status: int, what: str) -> None:
     raise RuntimeError(f"{what}: {message} (status {status})")
 
 
-__all__ = ["AUTOGRAD_PATH", "LIBRARY_PATH", "SIGNATURES", "check", "load", "load_autograd"]
+__all__ = ["AUTOGRAD_PATH", "LAYER_SIGNATURES", "LIBRARY_PATH", "SIGNATURES", "check", "load", "load_autograd"]

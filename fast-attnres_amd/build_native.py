@@ -13,10 +13,13 @@ library:
   whose part 2 is scheduled with LLVM's iterative-minreg strategy, and once
   more for the (64, 4) token-block and whole-row key-resident backwards,
   scheduled with the max-ilp strategy;
+* `csrc/attnres_norm.hip`, `attnres_embedding.hip`, `attnres_loss.hip`: the
+  layers around the reads (`include/attnres_layers_hip.h`);
 
 and, against PyTorch's headers and libraries, the eager autograd nodes
-`csrc/attnres_autograd.cpp` -> `attnres/_lib/_autograd.so` (host C++, no
-device code; linked to the library above with an `$ORIGIN` run path).
+`csrc/attnres_autograd.cpp` and `csrc/attnres_layers_autograd.cpp` ->
+`attnres/_lib/_autograd.so` (host C++, no device code; linked to the library
+above with an `$ORIGIN` run path).
 
 Packed-FP32 VALU ops are disabled (``-target-feature -packed-fp32-ops``); the
 compiler still emits ordinary FP32 FMAs, v_dot2_f32_bf16 and the gfx950 BF16
@@ -52,8 +55,10 @@ GEOMETRIES = ((16, 1), (32, 1), (32, 2), (32, 3), (32, 4), (64, 3), (64, 4), (64
 # launch_fwd)
 SPLIT_GEOMETRIES = {(64, 8): ["-mllvm", "-amdgpu-sched-strategy=iterative-minreg"]}
 FLAGS = ["-O3", "-std=c++17", "-fPIC", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
-AUTOGRAD_SOURCE = CSRC / "attnres_autograd.cpp"
-AUTOGRAD_OBJECT = BUILD_DIR / "attnres_autograd.o"
+AUTOGRAD_SOURCES = (CSRC / "attnres_autograd.cpp", CSRC / "attnres_layers_autograd.cpp")
+AUTOGRAD_OBJECTS = tuple(BUILD_DIR / f"{source.stem}.o" for source in AUTOGRAD_SOURCES)
+# the layers around the reads, one unit each
+LAYER_UNITS = ("attnres_norm", "attnres_embedding", "attnres_loss")
 AUTOGRAD_OUTPUT = HERE / "attnres" / "_lib" / "_autograd.so"
 ROCM_INCLUDE = Path(os.environ.get("ROCM_PATH", "/opt/rocm")) / "include"
 
@@ -68,6 +73,7 @@ def hipcc() -> str:
 def compile_commands() -> list[tuple[list[str], Path]]:
     """(hipcc command, object path) for every translation unit."""
     units = [(CSRC / "attnres_hip.hip", [], BUILD_DIR / "attnres_hip.o")]
+    units += [(CSRC / f"{stem}.hip", [], BUILD_DIR / f"{stem}.o") for stem in LAYER_UNITS]
     for lanes, chunks in GEOMETRIES:
         defines = [f"-DATTNRES_LANES={lanes}", f"-DATTNRES_CHUNKS={chunks}"]
         stem = f"attnres_kernels_g{lanes}_c{chunks}"
@@ -131,10 +137,11 @@ def build(verbose: bool = False, jobs: int | None = None) -> Path:
     OUTPUT.parent.mkdir(parents=True, exist_ok=True)
     commands = compile_commands()
     compile_flags, link_flags = _torch_flags()
-    autograd = [cxx(), *compile_flags, "-c", str(AUTOGRAD_SOURCE), "-o", str(AUTOGRAD_OBJECT)]
-    workers = jobs or min(len(commands) + 1, os.cpu_count() or 1, 16)
+    autograd = [[cxx(), *compile_flags, "-c", str(source), "-o", str(obj)]
+                for source, obj in zip(AUTOGRAD_SOURCES, AUTOGRAD_OBJECTS)]
+    workers = jobs or min(len(commands) + len(autograd), os.cpu_count() or 1, 16)
     with ThreadPoolExecutor(max_workers=workers) as pool:
-        futures = [pool.submit(_run, autograd, verbose)]  # the longest unit (PyTorch headers) first
+        futures = [pool.submit(_run, cmd, verbose) for cmd in autograd]  # the longest units (PyTorch headers) first
         futures += [pool.submit(_run, cmd, verbose) for cmd, _ in commands]
         for future in futures:
             future.result()
@@ -143,7 +150,7 @@ def build(verbose: bool = False, jobs: int | None = None) -> Path:
           *[str(obj) for _, obj in commands], "-o", str(temporary)], verbose)
     os.replace(temporary, OUTPUT)
     temporary = AUTOGRAD_OUTPUT.with_suffix(".so.tmp")
-    _run([cxx(), "-shared", str(AUTOGRAD_OBJECT), "-o", str(temporary), f"-L{OUTPUT.parent}", "-lattnres_hip",
+    _run([cxx(), "-shared", *[str(obj) for obj in AUTOGRAD_OBJECTS], "-o", str(temporary), f"-L{OUTPUT.parent}", "-lattnres_hip",
           "-Wl,-rpath,$ORIGIN", *link_flags], verbose)
     os.replace(temporary, AUTOGRAD_OUTPUT)
     return OUTPUT

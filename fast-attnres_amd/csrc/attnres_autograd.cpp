@@ -38,25 +38,11 @@
 #include <optional>
 #include <vector>
 
-#include "attnres_hip.h"
+#include "attnres_nodes.h"
+
+using namespace attnres_nodes;
 
 namespace {
-
-using torch::Tensor;
-using torch::autograd::AutogradContext;
-using torch::autograd::variable_list;
-
-// A failing status raises as the Python binding does: ValueError for argument
-// errors, RuntimeError otherwise, with the library's own message.
-void check(int status, const char* what) {
-  if (status == ATTNRES_OK) return;
-  const char* message = attnres_hip_last_error();
-  if (status == ATTNRES_ERR_SHAPE || status == ATTNRES_ERR_STRIDE || status == ATTNRES_ERR_SCALAR ||
-      status == ATTNRES_ERR_WORKSPACE) {
-    TORCH_CHECK_VALUE(false, what, ": ", message);
-  }
-  TORCH_CHECK(false, what, ": ", message, " (status ", status, ")");
-}
 
 // Pooled saved state: out_refine [N, D] int8 at byte 0 (when saved), then
 // from the 16-byte aligned offset `head` logit [N, S], 1/rms [N, S] (`block`
@@ -85,10 +71,6 @@ StatePointers pool_pointers(const Tensor& pool, const PoolLayout& layout, bool s
   return {save ? reinterpret_cast<int8_t*>(base) : nullptr, logit, logit + layout.block, logit + 2 * layout.block};
 }
 
-hipStream_t current_stream(const Tensor& tensor) {
-  return c10::hip::getCurrentHIPStream(tensor.device().index()).stream();
-}
-
 Tensor bf16_empty(at::IntArrayRef shape, const Tensor& like) {
   return torch::empty(shape, like.options().dtype(torch::kBFloat16));
 }
@@ -97,26 +79,6 @@ Tensor dq_workspace(int64_t tokens, int64_t width, int64_t rank, const Tensor& l
   const int64_t elems = attnres_hip_dq_workspace_elems(tokens, width, rank);
   TORCH_CHECK_VALUE(elems >= 0, "attnres backward: shape outside the supported envelope");
   return torch::empty({elems}, like.options().dtype(torch::kFloat32));
-}
-
-// Element stride between consecutive rows of tensor[..., D] flattened to
-// [rows, D], or nothing when the rows are not evenly spaced or a row is not
-// unit-stride (the Python `row_stride`, after fla_full_sources.py:164-178).
-std::optional<int64_t> row_stride(const Tensor& tensor) {
-  const int64_t last = tensor.dim() - 1;
-  if (tensor.size(last) > 1 && tensor.stride(last) != 1) return std::nullopt;
-  std::optional<int64_t> stride;
-  int64_t rows = 1;
-  for (int64_t d = last - 1; d >= 0; --d) {
-    if (tensor.size(d) == 1) continue;
-    if (!stride) {
-      stride = tensor.stride(d);
-    } else if (tensor.stride(d) != rows * *stride) {
-      return std::nullopt;
-    }
-    rows *= tensor.size(d);
-  }
-  return stride.value_or(0);
 }
 
 // Row pointers and strides of a source list; sources whose rows are not
@@ -143,8 +105,6 @@ SourceTable source_table(at::TensorList sources) {
   }
   return table;
 }
-
-int64_t rows_of(const Tensor& tensor) { return tensor.dim() > 1 ? tensor.numel() / tensor.size(-1) : 1; }
 
 // Packed values [S, ..., D] as rows [S, N, D]: a view where the batch axes
 // collapse to one row stride (as torch's reshape does), a copy otherwise, and
@@ -821,4 +781,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("bank_push_sum", &bank_push_sum, "partial sum of a block, stored in a slot; returns it and the new token");
   m.def("bank_read", &bank_read, "read of leading slots and a tail slot (-1: none)");
   m.def("pool_layout", &layout_of, "(head, block, size) of the pooled saved state");
+  bind_layers(m);
 }

@@ -22,6 +22,7 @@
 #include <type_traits>
 
 #include "attnres_internal.h"
+#include "attnres_layers.h"
 
 // The dq workspace of attnres_hip_packed_backward_noalloc: device memory the
 // library holds for the life of the process, one copy per GPU (4 MiB each).
@@ -339,6 +340,19 @@ int check_recompute(bool recompute, int64_t S, int64_t D, int64_t R, const char*
 int64_t workspace_elems(int64_t N, int64_t D, int64_t R) { return (max_grid_rows(N, D) + 1) * R; }
 
 }  // namespace
+
+// For the entry points of the layers (attnres_layers.h): one error message per
+// thread, whichever unit's call failed.
+int layer_error(int code, const char* fmt, ...) {
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(g_error, sizeof(g_error), fmt, ap);
+  va_end(ap);
+  return code;
+}
+
+int layer_launch_status(const char* what) { return launch_status(what); }
+
 }  // namespace attnres_hip
 
 using namespace attnres_hip;

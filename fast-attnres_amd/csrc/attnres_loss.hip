@@ -1,0 +1,1041 @@
+// attnres_loss.hip - softmax cross entropy of logits = H W^T over a vocabulary, for gfx950.
+//
+//   l[n, v] = <H_n, W_v>,  lse_n = log sum_v exp(l[n, v]),  loss_n = lse_n - l[n, t_n]
+//   P[n, v] = g_n (exp(l[n, v] - lse_n) - [v = t_n]),  dH = P W,  dW = P^T H
+//
+// Bound by the matrix cores: four products of 2 N V D operations (the logits in
+// the forward, again in the backward, and two gradient products), 8 N V D in all, against
+// O(V D + N D) bytes.  The logits are never stored: the forward keeps a running (maximum, sum of
+// exponentials) per row and tile of 256 columns, the backward forms P for one piece of the
+// vocabulary at a time.
+//
+// Rows whose target is ignored are left out before anything is multiplied: the rows that count are
+// packed together (in order, the row length padded with zeros to whole tiles), so ignored
+// rows cost nothing and what they hold (NaN, infinities) reaches nothing.
+//
+// Operands are 16 bits wide.  BF16 and FP16 inputs are multiplied as they are.  FP32
+// inputs are scaled by a power of two to just under 2^15 and written as the sum of two FP16 numbers, hi +
+// lo (24 bits together for all within 2^-14 of the largest), and a product is
+// hi hi + hi lo + lo hi: what is left out, lo lo, is below 2^-24 of the product, like FP32's own
+// rounding.  Three FP16 products run at 16 / 3 times the rate of FP32 matrix instructions.
+// P is rounded to the operands' type (BF16), or, for FP16 and FP32 inputs, scaled by
+// 2^14 and written as one or two FP16 numbers, so that probabilities down to 2^-28 are normal numbers.
+
+#include "attnres_layers.h"
+
+#include <algorithm>
+
+namespace attnres_hip {
+namespace layers {
+namespace {
+
+constexpr int kTile = 256;     // rows and columns of a workgroup's tile
+constexpr int kDepth = 64;     // of a tile's operands in LDS
+constexpr int kThreads = 512;  // 8 wavefronts of 128 x 64 outputs
+constexpr int kOperand = kTile * kDepth;  // elements of one operand's stage
+constexpr float kProbabilityScale = 16384.0f;
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+
+#define ATTNRES_LDS __attribute__((address_space(3)))
+#define ATTNRES_GLOBAL __attribute__((address_space(1)))
+
+inline int64_t round_up(int64_t x, int64_t to) { return (x + to - 1) / to * to; }
+
+// What the forward leaves for the backward: a header, then per packed row the (maximum,
+// 1 / sum of exponentials above it) of its logits, its source row and its target, and per
+// source row its packed one (or -1).
+struct Header {
+  int32_t count;      // packed rows
+  float scale[2];     // of H and W (FP32 inputs; else 1)
+  uint32_t amax[2];   // their largest finite magnitudes, as bits
+};
+
+struct Saved {
+  Header* header;
+  f32x2* stats;
+  int32_t* index;
+  int32_t* packed;
+  int32_t* target;
+};
+
+constexpr int64_t kHeaderBytes = 256;
+inline int64_t saved_bytes(int64_t rows) { return kHeaderBytes + 20 * rows; }
+inline Saved saved_views(void* base, int64_t rows) {
+  char* at = static_cast<char*>(base) + kHeaderBytes;
+  return {static_cast<Header*>(base), reinterpret_cast<f32x2*>(at), reinterpret_cast<int32_t*>(at + 8 * rows),
+          reinterpret_cast<int32_t*>(at + 12 * rows), reinterpret_cast<int32_t*>(at + 16 * rows)};
+}
+
+// ------------------------------------------------------------- matrix product
+// out[b][a] = sum_k A[a][k] B[b][k] over a tile of 256 x 256: A's index is the contiguous
+// one of the output.  An operand lies either as rows of k (ROWS: the row is contiguous in k) or as
+// columns (row k holds all of the operand's entries).  Both go to LDS as they lie, 16 bytes
+// per lane straight from memory; a column operand's fragments are transposed on the way
+// from LDS (ds_read_b64_tr_b16).  16-byte slots are permuted within an LDS row so that the lanes of
+// a fragment read meet every bank once: slot = chunk ^ (row % 8) for rows of k (128 bytes), chunk ^
+// 4 (k % 4) for columns (512 bytes).
+
+struct Operand {
+  const uint16_t* part[2];  // hi, lo
+  int64_t ld;
+  int64_t entries;          // readable entries (rows: clamped row; columns: multiple of 8)
+  int64_t depth;            // readable k of a column operand
+};
+
+struct Product {
+  Operand a, b;
+  const int32_t* count;  // live packed rows
+  int64_t depth;         // k of the whole product (a multiple of 64), of all splits
+  int depth_is_count;    // depth: the packed rows
+  int tiles_a, tiles_b, splits;
+};
+
+template <bool ROWS>
+struct Loader {
+  uint32_t offset[4];  // bytes from the stage's origin; columns: of the chunk alone
+  int row[4];          // columns: k of the load
+  uint32_t slot;       // LDS byte of this wavefront's first load
+  __device__ __forceinline__ void init(const Operand& o, int64_t entry0, int wave, int lane) {
+    slot = static_cast<uint32_t>(wave) * 4096;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if constexpr (ROWS) {
+        const int r = (wave * 4 + j) * 8 + lane / 8;
+        const int64_t left = o.entries - 1 - entry0;
+        const int64_t at = r < left ? r : left;
+        offset[j] = static_cast<uint32_t>((at * o.ld + ((lane % 8) ^ (lane / 8)) * 8) * 2);
+      } else {
+        row[j] = (wave * 4 + j) * 2 + lane / 32;
+        const int chunk = (lane % 32) ^ ((row[j] & 3) << 2);
+        const int64_t left = o.entries - 8 - entry0;
+        const int64_t at = chunk * 8 < left ? chunk * 8 : left;
+        offset[j] = static_cast<uint32_t>(at * 2);
+      }
+    }
+  }
+  // one 1-KB load of the stage at k0 into `lds`
+  __device__ __forceinline__ void load(const Operand& o, const uint16_t* origin, int64_t k0, uint16_t* lds, int j) const {
+    const char* base = reinterpret_cast<const char*>(origin);
+    uint32_t at = offset[j];
+    if constexpr (ROWS) {
+      base += k0 * 2;
+    } else {
+      base += k0 * o.ld * 2;
+      const int64_t left = o.depth - 1 - k0;
+      at += static_cast<uint32_t>((row[j] < left ? row[j] : left) * o.ld * 2);
+    }
+    __builtin_amdgcn_global_load_lds(reinterpret_cast<const ATTNRES_GLOBAL uint32_t*>(reinterpret_cast<uintptr_t>(base + at)),
+                                     (ATTNRES_LDS uint32_t*)(reinterpret_cast<char*>(lds) + slot + j * 1024), 16, 0, 0);
+  }
+};
+
+// Fragment r (32 entries) of the 16 k's at `step`: lane l holds entry l % 32, k = 8 (l / 32) + 0..7.
+template <bool ROWS>
+__device__ __forceinline__ s16x8 fragment(const uint16_t* lds, int entry, int step, int lane) {
+  if constexpr (ROWS) {
+    const int row = entry + lane % 32;
+    const int slot = (step * 2 + lane / 32) ^ (lane & 7);
+    return *reinterpret_cast<const s16x8*>(lds + row * kDepth + slot * 8);
+  } else {
+    // 16 lanes read 4 k's of 16 entries and get one entry's 4 k's each
+    const int group = lane / 16, j = lane % 16;
+    const int column = entry + (group % 2) * 16 + (j % 4) * 4;
+    const int k = step * 16 + (group / 2) * 8 + j / 4;
+    const uint16_t* at = lds + k * kTile + ((column / 8) ^ ((j / 4) << 2)) * 8 + column % 8;
+    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((ATTNRES_LDS s16x4*)at);
+    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((ATTNRES_LDS s16x4*)(at + 4 * kTile));
+    return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+  }
+}
+
+template <class T>
+__device__ __forceinline__ f32x16 mfma(s16x8 a, s16x8 b, f32x16 c) {
+  if constexpr (std::is_same_v<T, Bf16>) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  } else {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  }
+}
+
+struct TileAt {
+  int a, b, split;
+};
+
+// Workgroup to tile: workgroups go round the 8 XCDs in turn, so each XCD takes one contiguous part of
+// the tiles' order, in which 8 tiles of B by all of A's follow each other: the 32 tiles that run on an
+// XCD at a time share 8 + 4 operand stripes in its L2.
+__device__ __forceinline__ TileAt tile_at(const Product& p) {
+  const int total = p.tiles_a * p.tiles_b * p.splits;
+  const int id = blockIdx.x;
+  const int q = total / 8, r = total % 8, xcd = id % 8, i = id / 8;
+  int at = xcd < r ? xcd * (q + 1) + i : r * (q + 1) + (xcd - r) * q + i;
+  const int split = at / (p.tiles_a * p.tiles_b);
+  at -= split * p.tiles_a * p.tiles_b;
+  constexpr int kGroup = 8;
+  const int group = at / (kGroup * p.tiles_a);
+  const int size = min(kGroup, p.tiles_b - group * kGroup);
+  at -= group * kGroup * p.tiles_a;
+  return {at / size, group * kGroup + at % size, split};
+}
+
+using Accumulators = f32x16[4][2];  // [32 entries of A][32 entries of B]; lane l, register i: entry
+                                    // 8 (i / 4) + 4 (l / 32) + i % 4 of A, l % 32 of B
+
+// The sum of a tile over its split's k's; SEGMENTS 3: hi hi + hi lo + lo hi.
+template <class T, int SEGMENTS, bool A_ROWS, bool B_ROWS>
+__device__ __forceinline__ void multiply(const Product& p, const TileAt& tile, uint16_t* lds, Accumulators& acc) {
+  const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) acc[i][j] = f32x16{};
+  }
+  const int64_t depth = p.depth_is_count ? (static_cast<int64_t>(*p.count) + kDepth - 1) / kDepth * kDepth : p.depth;
+  const int stages_all = static_cast<int>(depth / kDepth);
+  const int first = static_cast<int>(static_cast<int64_t>(stages_all) * tile.split / p.splits);
+  const int stages = static_cast<int>(static_cast<int64_t>(stages_all) * (tile.split + 1) / p.splits) - first;
+  if (stages == 0) return;
+  const int64_t a0 = static_cast<int64_t>(tile.a) * kTile, b0 = static_cast<int64_t>(tile.b) * kTile;
+  Loader<A_ROWS> load_a;
+  Loader<B_ROWS> load_b;
+  load_a.init(p.a, a0, wave, lane);
+  load_b.init(p.b, b0, wave, lane);
+  const int64_t origin_a = A_ROWS ? a0 * p.a.ld : a0, origin_b = B_ROWS ? b0 * p.b.ld : b0;
+  int segment = 0, stage = 0;  // of the next load
+  const auto load_stage = [&](int buffer) {
+    uint16_t* to = lds + buffer * 2 * kOperand;
+    const int64_t k0 = static_cast<int64_t>(first + stage) * kDepth;
+    const uint16_t* a = p.a.part[SEGMENTS == 3 && segment == 2] + origin_a;
+    const uint16_t* b = p.b.part[SEGMENTS == 3 && segment == 1] + origin_b;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      load_a.load(p.a, a, k0, to, j);
+      load_b.load(p.b, b, k0, to + kOperand, j);
+    }
+    if (++stage == stages) stage = 0, ++segment;
+  };
+  load_stage(0);
+  const int total = stages * SEGMENTS;
+  const int wa = (wave % 2) * 128, wb = (wave / 2) * 64;
+  for (int s = 0; s < total; ++s) {
+    // the stage has landed (a barrier alone does not wait for loads into LDS), and the other
+    // buffer is no longer read
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (s + 1 < total) load_stage((s + 1) & 1);
+    const uint16_t* from = lds + (s & 1) * 2 * kOperand;
+#pragma unroll
+    for (int step = 0; step < kDepth / 16; ++step) {
+      s16x8 a[4], b[2];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) a[i] = fragment<A_ROWS>(from, wa + i * 32, step, lane);
+#pragma unroll
+      for (int j = 0; j < 2; ++j) b[j] = fragment<B_ROWS>(from + kOperand, wb + j * 32, step, lane);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) acc[i][j] = mfma<T>(a[i], b[j], acc[i][j]);
+      }
+    }
+  }
+  __syncthreads();  // LDS is free for the epilogue
+}
+
+// -------------------------------------------------------------------- logits
+
+// Joins two (maximum, sum of exponentials above it).  A side without entries is (-inf, 0);
+// a NaN sum stays NaN.
+__device__ __forceinline__ f32x2 join(f32x2 x, f32x2 y) {
+  const float top = fmaxf(x.x, y.x);
+  if (top == -__builtin_inff()) return f32x2{top, x.y + y.y};
+  return f32x2{top, x.y * __expf(x.x - top) + y.y * __expf(y.x - top)};
+}
+
+// A logit from the product of scaled operands: by the two powers of two in turn, the smaller
+// first, so that neither step leaves FP32 where the logit itself does not.
+struct Unscale {
+  float first = 1.0f, second = 1.0f;
+  bool any;
+  __device__ __forceinline__ explicit Unscale(const Header* header) : any(header != nullptr) {
+    if (!any) return;
+    const float h = 1.0f / header->scale[0], w = 1.0f / header->scale[1];
+    first = fminf(h, w);
+    second = fmaxf(h, w);
+  }
+  __device__ __forceinline__ float operator()(float x) const { return any ? x * first * second : x; }
+};
+
+struct LogitArgs {
+  Product product;  // A: W (vocabulary), B: H (packed rows)
+  const Header* header;
+  const int32_t* target;
+  int64_t vocab;
+  int64_t first;      // of the piece's columns
+  int64_t row_tiles;  // packed rows, padded
+  // forward
+  f32x2* sums;          // [tiles][row_tiles] (maximum, sum of exponentials above it)
+  float* target_logit;  // [row_tiles]
+  // backward
+  const f32x2* stats;
+  const float* row_scale;  // [row_tiles] upstream gradient per packed row, scaled; 0 past the last
+  uint16_t* p[2];          // [row_tiles][p_ld]
+  int64_t p_ld;
+};
+
+// Forward: (maximum, sum) of a tile's 256 logits per row, and the target's logit.
+template <class T, int SEGMENTS>
+__global__ void __launch_bounds__(kThreads) attnres_loss_logits_kernel(LogitArgs g) {
+  __shared__ __align__(16) uint16_t lds[4 * kOperand];
+  const TileAt tile = tile_at(g.product);
+  const int count = *g.product.count;
+  if (tile.b * kTile >= count) return;
+  Accumulators acc;
+  multiply<T, SEGMENTS, true, true>(g.product, tile, lds, acc);
+  const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
+  const Unscale unscale(SEGMENTS == 3 ? g.header : nullptr);
+  const int64_t v0 = static_cast<int64_t>(tile.a) * kTile + (wave % 2) * 128;
+  const int limit = static_cast<int>(g.vocab - v0 < 128 ? g.vocab - v0 : 128);
+  f32x2* meet = reinterpret_cast<f32x2*>(lds);  // [2][256]
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const int column = (wave / 2) * 64 + j * 32 + lane % 32;
+    const int row = tile.b * kTile + column;
+    const int64_t from_v0 = row < count ? g.target[row] - v0 : -1;
+    const int rel = from_v0 >= 0 && from_v0 < 128 ? static_cast<int>(from_v0) : -1;
+    float top = -__builtin_inff();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const int v = i * 32 + 8 * (e / 4) + 4 * (lane / 32) + e % 4;
+        const float l = v < limit ? unscale(acc[i][j][e]) : -__builtin_inff();
+        acc[i][j][e] = l;
+        top = fmaxf(top, l);
+        if (v == rel) g.target_logit[row] = l;
+      }
+    }
+    top = fmaxf(top, __shfl_xor(top, 32, 64));
+    const float from = top == -__builtin_inff() ? 0.0f : top;  // nothing but NaN, or nothing at all
+    float sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) sum += __expf(acc[i][j][e] - from);
+    }
+    sum += __shfl_xor(sum, 32, 64);
+    if (lane < 32) meet[(wave % 2) * kTile + column] = f32x2{top, sum};
+  }
+  __syncthreads();
+  if (threadIdx.x < kTile) {
+    g.sums[static_cast<int64_t>(tile.a) * g.row_tiles + tile.b * kTile + threadIdx.x] =
+        join(meet[threadIdx.x], meet[kTile + threadIdx.x]);
+  }
+}
+
+// 16-byte slot of a staged output row of 512 bytes: a permutation per row, so that 32 lanes
+// writing one chunk of 32 rows meet 32 different slots.
+__device__ __forceinline__ int staged(int row, int chunk) { return row * 32 + (chunk ^ (row & 31)); }
+
+// Backward: P of a tile, rounded to the operands' type.
+template <class T, int SEGMENTS>
+__global__ void __launch_bounds__(kThreads) attnres_loss_probability_kernel(LogitArgs g) {
+  __shared__ __align__(16) uint16_t lds[4 * kOperand];
+  const TileAt tile = tile_at(g.product);
+  const int count = *g.product.count;
+  if (tile.b * kTile >= count) return;
+  Accumulators acc;
+  multiply<T, SEGMENTS, true, true>(g.product, tile, lds, acc);
+  const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
+  const Unscale unscale(SEGMENTS == 3 ? g.header : nullptr);
+  const int64_t v0 = g.first + static_cast<int64_t>(tile.a) * kTile + (wave % 2) * 128;
+  const int limit = static_cast<int>(g.vocab - v0 < 128 ? g.vocab - v0 : 128);
+  constexpr int kParts = SEGMENTS == 3 ? 2 : 1;
+#pragma unroll
+  for (int part = 0; part < kParts; ++part) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int column = (wave / 2) * 64 + j * 32 + lane % 32;
+      const int row = tile.b * kTile + column;
+      const bool live = row < count;
+      const int64_t from_v0 = live ? g.target[row] - v0 : -1;
+      const int rel = from_v0 >= 0 && from_v0 < 128 ? static_cast<int>(from_v0) : -1;
+      const f32x2 stats = live ? g.stats[row] : f32x2{0.0f, 0.0f};
+      const float by = live ? g.row_scale[row] : 0.0f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          uint32_t packed[2];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int v = i * 32 + 8 * q + 4 * (lane / 32) + e;
+            if (part == 0) {
+              float x = __expf(unscale(acc[i][j][4 * q + e]) - stats.x) * stats.y;
+              if (v == rel) x -= 1.0f;
+              acc[i][j][4 * q + e] = live && v < limit ? x * by : 0.0f;
+            }
+          }
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            packed[e] = pack2<T>(acc[i][j][4 * q + 2 * e], acc[i][j][4 * q + 2 * e + 1]);
+            if (kParts == 2 && part == 0) {  // what the first part leaves
+              acc[i][j][4 * q + 2 * e] -= to_f32(T{static_cast<uint16_t>(packed[e] & 0xffffu)});
+              acc[i][j][4 * q + 2 * e + 1] -= to_f32(T{static_cast<uint16_t>(packed[e] >> 16)});
+            }
+          }
+          const int chunk = (wave % 2) * 16 + i * 4 + q;
+          *reinterpret_cast<uint64_t*>(lds + staged(column, chunk) * 8 + (lane / 32) * 4) =
+              static_cast<uint64_t>(packed[1]) << 32 | packed[0];
+        }
+      }
+    }
+    __syncthreads();
+    for (int k = threadIdx.x; k < kTile * 32; k += kThreads) {
+      const int column = k / 32, chunk = k % 32;
+      *reinterpret_cast<u32x4*>(g.p[part] + (static_cast<int64_t>(tile.b) * kTile + column) * g.p_ld + tile.a * kTile + chunk * 8) =
+          *reinterpret_cast<const u32x4*>(lds + staged(column, chunk) * 8);
+    }
+    if (part + 1 < kParts) __syncthreads();
+  }
+}
+
+// ----------------------------------------------------------- gradient products
+
+struct GradientArgs {
+  Product product;
+  const float* alpha;  // two factors of the output; nullptr: 1
+  void* out;           // [splits][columns][ld]
+  int64_t ld;
+  int64_t split_stride;
+  int64_t entries_a;   // valid contiguous entries
+  int64_t entries_b;
+  int add;             // FP32: add to what is there
+  int live_only;       // entries of B past the packed rows are not needed
+};
+
+// dH (A: W by columns, B: P by rows) and dW (A: H by columns, B: P by columns).  OUT float:
+// FP32 partial sums or an FP32 gradient; else the 16-bit gradient itself.
+template <class T, class OUT, int SEGMENTS, bool B_ROWS>
+__global__ void __launch_bounds__(kThreads) attnres_loss_gradient_kernel(GradientArgs g) {
+  __shared__ __align__(16) uint16_t lds[4 * kOperand];
+  const TileAt tile = tile_at(g.product);
+  if (g.live_only && tile.b * kTile >= *g.product.count) return;
+  Accumulators acc;
+  multiply<T, SEGMENTS, false, B_ROWS>(g.product, tile, lds, acc);
+  const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
+  const float by = g.alpha != nullptr ? g.alpha[0] : 1.0f, unscale = g.alpha != nullptr ? g.alpha[1] : 1.0f;
+  OUT* out = static_cast<OUT*>(g.out) + tile.split * g.split_stride;
+  const int64_t a0 = static_cast<int64_t>(tile.a) * kTile, b0 = static_cast<int64_t>(tile.b) * kTile;
+  constexpr bool kWide = std::is_same_v<OUT, float>;
+  constexpr int kRounds = kWide ? 2 : 1;    // 512-byte rows: 128 FP32 or 256 16-bit outputs
+  constexpr int kChunk = kWide ? 4 : 8;     // outputs per 16 bytes
+#pragma unroll
+  for (int round = 0; round < kRounds; ++round) {
+    if (!kWide || wave % 2 == round) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int column = (wave / 2) * 64 + j * 32 + lane % 32;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            float x[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] = acc[i][j][4 * q + e] * by * unscale;
+            if constexpr (kWide) {
+              const int chunk = i * 8 + q * 2 + lane / 32;
+              *reinterpret_cast<f32x4*>(lds + staged(column, chunk) * 8) = f32x4{x[0], x[1], x[2], x[3]};
+            } else {
+              const int chunk = (wave % 2) * 16 + i * 4 + q;
+              *reinterpret_cast<uint64_t*>(lds + staged(column, chunk) * 8 + (lane / 32) * 4) =
+                  static_cast<uint64_t>(pack2<OUT>(x[2], x[3])) << 32 | pack2<OUT>(x[0], x[1]);
+            }
+          }
+        }
+      }
+    }
+    __syncthreads();
+    for (int k = threadIdx.x; k < kTile * 32; k += kThreads) {
+      const int column = k / 32, chunk = k % 32;
+      const int64_t a = a0 + round * 128 + chunk * kChunk, b = b0 + column;
+      if (b >= g.entries_b || a >= g.entries_a) continue;
+      OUT* to = out + b * g.ld + a;
+      const uint16_t* from = lds + staged(column, chunk) * 8;
+      if constexpr (kWide) {
+        f32x4 x = *reinterpret_cast<const f32x4*>(from);
+        if (a + kChunk <= g.entries_a) {
+          if (g.add) x += reinterpret_cast<const Raw32*>(to)->v;
+          reinterpret_cast<Raw32*>(to)->v = x;
+        } else {
+          for (int e = 0; a + e < g.entries_a; ++e) to[e] = g.add ? to[e] + x[e] : x[e];
+        }
+      } else {
+        const u32x4 x = *reinterpret_cast<const u32x4*>(from);
+        if (a + kChunk <= g.entries_a) {
+          reinterpret_cast<Raw16*>(to)->v = x;
+        } else {
+          for (int e = 0; a + e < g.entries_a; ++e) to[e].bits = from[e];
+        }
+      }
+    }
+    if (round + 1 < kRounds) __syncthreads();
+  }
+}
+
+// ------------------------------------------------------------------ small passes
+
+// One workgroup: the rows whose target counts, in order.  A target outside the
+// vocabulary is marked -1 (the row's loss and gradients become NaN).
+constexpr int kScanThreads = 1024;
+
+__global__ void __launch_bounds__(kScanThreads) attnres_loss_rows_kernel(const void* targets, int target_bytes, int64_t rows, int64_t vocab,
+                                                                         int64_t ignore_index, Saved s) {
+  __shared__ int waves[kScanThreads / 64];
+  const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
+  int base = 0;
+  for (int64_t r0 = 0; r0 < rows; r0 += kScanThreads) {
+    const int64_t row = r0 + threadIdx.x;
+    int64_t target = ignore_index;
+    if (row < rows) {
+      target = target_bytes == 8 ? static_cast<const int64_t*>(targets)[row] : static_cast<const int32_t*>(targets)[row];
+    }
+    const bool counts = row < rows && target != ignore_index;
+    const uint64_t ballot = __ballot(counts);
+    if (lane == 0) waves[wave] = __popcll(ballot);
+    __syncthreads();
+    int before = base, all = 0;
+    for (int w = 0; w < kScanThreads / 64; ++w) {
+      before += w < wave ? waves[w] : 0;
+      all += waves[w];
+    }
+    const int at = before + __popcll(ballot & ((uint64_t{1} << lane) - 1));
+    if (row < rows) s.packed[row] = counts ? at : -1;
+    if (counts) {
+      s.index[at] = static_cast<int32_t>(row);
+      s.target[at] = target >= 0 && target < vocab ? static_cast<int32_t>(target) : -1;
+    }
+    base += all;
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) {
+    s.header->count = base;
+    s.header->scale[0] = s.header->scale[1] = 1.0f;
+    s.header->amax[0] = s.header->amax[1] = 0;
+  }
+}
+
+// Largest finite magnitude of the rows (an integer maximum of the bits: the same in any order).
+__global__ void __launch_bounds__(kBlock) attnres_loss_amax_kernel(const float* __restrict__ x, int64_t stride, int64_t rows, int width,
+                                                                   const int32_t* index, const int32_t* count, uint32_t* amax) {
+  __shared__ uint32_t waves[kBlock / 64];
+  const int64_t live = count != nullptr ? *count : rows;
+  uint32_t top = 0;
+  for (int64_t r = blockIdx.x; r < live; r += gridDim.x) {
+    const float* row = x + (index != nullptr ? index[r] : r) * stride;
+    for (int c = threadIdx.x * kVec; c < width; c += kBlock * kVec) {
+      float v[kVec];
+      load_chunk(row, c, width, v);
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) {
+        const uint32_t bits = __float_as_uint(v[e]) & 0x7fffffffu;
+        if (bits < 0x7f800000u && bits > top) top = bits;
+      }
+    }
+  }
+#pragma unroll
+  for (int step = 32; step > 0; step >>= 1) top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), step, 64)));
+  if (threadIdx.x % 64 == 0) waves[threadIdx.x / 64] = top;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < kBlock / 64; ++w) top = max(top, waves[w]);
+    atomicMax(amax, top);
+  }
+}
+
+// The power of two that takes the largest magnitude into [2^14, 2^15), within 2^-110..2^110.
+__device__ __forceinline__ float split_scale(uint32_t amax) {
+  if (amax == 0) return 1.0f;
+  const int exponent = static_cast<int>(amax >> 23) - 127;
+  const int shift = min(110, max(-110, 14 - exponent));
+  return __uint_as_float(static_cast<uint32_t>(127 + shift) << 23);
+}
+
+// Rows to operands: [rows_out][width_out] zero-padded, as they are (X 16 bits) or as hi and
+// lo (X float).  index/count: the rows that count.
+template <class X>
+__global__ void __launch_bounds__(kBlock) attnres_loss_pack_kernel(const X* __restrict__ x, int64_t stride, int64_t rows, int width,
+                                                                   const int32_t* index, const int32_t* count, int64_t rows_out,
+                                                                   int width_out, Header* header, int which, bool keep_scale,
+                                                                   uint16_t* __restrict__ hi, uint16_t* __restrict__ lo) {
+  const int64_t live = count != nullptr ? *count : rows;
+  float scale = 1.0f;
+  if constexpr (std::is_same_v<X, float>) {
+    scale = split_scale(header->amax[which]);
+    if (keep_scale && blockIdx.x == 0 && threadIdx.x == 0) header->scale[which] = scale;
+  }
+  const int chunks = width_out / kVec;
+  const int64_t all = rows_out * chunks;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * kBlock + threadIdx.x; i < all; i += static_cast<int64_t>(gridDim.x) * kBlock) {
+    const int64_t r = i / chunks;
+    const int c = static_cast<int>(i - r * chunks) * kVec;
+    u32x4 h = {0, 0, 0, 0}, l = {0, 0, 0, 0};
+    if (r < live && c < width) {
+      const X* row = x + (index != nullptr ? index[r] : r) * stride;
+      float v[kVec];
+      load_chunk(row, c, width, v);
+      if constexpr (std::is_same_v<X, float>) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float a = v[2 * e] * scale, b = v[2 * e + 1] * scale;
+          h[e] = pack2<F16>(a, b);
+          l[e] = pack2<F16>(a - to_f32(F16{static_cast<uint16_t>(h[e] & 0xffffu)}),
+                            b - to_f32(F16{static_cast<uint16_t>(h[e] >> 16)}));
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) h[e] = pack2<X>(v[2 * e], v[2 * e + 1]);
+      }
+    }
+    *reinterpret_cast<u32x4*>(hi + i * kVec) = h;
+    if constexpr (std::is_same_v<X, float>) *reinterpret_cast<u32x4*>(lo + i * kVec) = l;
+  }
+}
+
+// Per row of the input: its log-sum from the tiles' sums, and its loss.  64 rows by 4 parts
+// of the tiles per workgroup.
+__global__ void __launch_bounds__(kBlock) attnres_loss_reduce_kernel(const f32x2* __restrict__ sums, int tiles, int64_t row_tiles,
+                                                                     const float* __restrict__ target_logit, int64_t rows, Saved s,
+                                                                     float* __restrict__ loss) {
+  __shared__ f32x2 part[4][64];
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * 64 + threadIdx.x % 64;
+  const int which = threadIdx.x / 64;
+  const int at = row < rows ? s.packed[row] : -1;
+  f32x2 total = {-__builtin_inff(), 0.0f};
+  if (at >= 0) {
+#pragma unroll 8
+    for (int t = which; t < tiles; t += 4) total = join(total, sums[static_cast<int64_t>(t) * row_tiles + at]);
+  }
+  part[which][threadIdx.x % 64] = total;
+  __syncthreads();
+  if (which != 0 || row >= rows) return;
+  if (at < 0) {
+    loss[row] = 0.0f;
+    return;
+  }
+  for (int k = 1; k < 4; ++k) total = join(total, part[k][threadIdx.x]);
+  const bool known = s.target[at] >= 0;
+  s.stats[at] = f32x2{total.x, known ? 1.0f / total.y : __builtin_nanf("")};
+  // the logarithm of the sum by itself: at a probability of one it is the whole loss
+  loss[row] = known ? logf(total.y) + (total.x - target_logit[at]) : __builtin_nanf("");
+}
+
+__global__ void __launch_bounds__(kScanThreads) attnres_loss_total_kernel(const float* __restrict__ loss, int64_t rows, const Header* header,
+                                                                          int mean, float* __restrict__ out) {
+  __shared__ float waves[kScanThreads / 64];
+  float sum = 0.0f;
+#pragma unroll 8
+  for (int64_t r = threadIdx.x; r < rows; r += kScanThreads) sum += loss[r];
+  sum = group_sum<64>(sum);
+  if (threadIdx.x % 64 == 0) waves[threadIdx.x / 64] = sum;
+  __syncthreads();
+  if (threadIdx.x != 0) return;
+  sum = 0.0f;
+  for (int w = 0; w < kScanThreads / 64; ++w) sum += waves[w];
+  out[0] = mean ? sum / static_cast<float>(header->count) : sum;
+}
+
+// Factors of the backward: per packed row its upstream gradient over the largest one's power of two (one
+// row's factor is at most 1), times the scale of P; and what the outputs are multiplied by.
+__global__ void __launch_bounds__(kScanThreads) attnres_loss_factors_kernel(const float* __restrict__ grad_loss, int reduction, Saved s,
+                                                                            int64_t row_tiles, float p_scale, float* row_scale,
+                                                                            float* alpha) {
+  __shared__ uint32_t waves[kScanThreads / 64];
+  const int count = s.header->count;
+  float outer = count > 0 ? 1.0f : 0.0f;  // nothing counts: zero gradients
+  if (count > 0 && reduction == ATTNRES_REDUCE_NONE) {
+    uint32_t top = 0;
+    for (int r = threadIdx.x; r < count; r += kScanThreads) {
+      const uint32_t bits = __float_as_uint(grad_loss[s.index[r]]) & 0x7fffffffu;
+      if (bits < 0x7f800000u && bits > top) top = bits;
+    }
+#pragma unroll
+    for (int step = 32; step > 0; step >>= 1) top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), step, 64)));
+    if (threadIdx.x % 64 == 0) waves[threadIdx.x / 64] = top;
+    __syncthreads();
+    top = 0;
+    for (int w = 0; w < kScanThreads / 64; ++w) top = max(top, waves[w]);
+    if (top != 0) outer = __uint_as_float(static_cast<uint32_t>(min(227, max(27, static_cast<int>(top >> 23) + 1))) << 23);
+  } else if (count > 0) {
+    outer = reduction == ATTNRES_REDUCE_MEAN ? grad_loss[0] / static_cast<float>(count) : grad_loss[0];
+  }
+  for (int64_t r = threadIdx.x; r < row_tiles; r += kScanThreads) {
+    float by = 0.0f;
+    if (r < count) by = reduction == ATTNRES_REDUCE_NONE ? grad_loss[s.index[r]] / outer * p_scale : p_scale;
+    row_scale[r] = by;
+  }
+  if (threadIdx.x == 0) {
+    // of dH = P W and dW = P^T H; two factors each, as their product may leave FP32 where the gradient does not
+    alpha[0] = alpha[2] = outer / p_scale;
+    alpha[1] = 1.0f / s.header->scale[1];
+    alpha[3] = 1.0f / s.header->scale[0];
+  }
+}
+
+// out[r] = both alpha's times the sum of the splits' partial rows; packed: of the row's packed one, zeros
+// where it has none.
+template <class OUT>
+__global__ void __launch_bounds__(kBlock) attnres_loss_join_kernel(const float* __restrict__ partial, int splits, int64_t split_stride,
+                                                                   int64_t ld, const int32_t* packed, int64_t rows, int width,
+                                                                   const float* __restrict__ alpha, OUT* __restrict__ out) {
+  const float by = alpha[0], unscale = alpha[1];
+  const int chunks = (width + kVec - 1) / kVec;
+  const int64_t all = rows * chunks;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * kBlock + threadIdx.x; i < all; i += static_cast<int64_t>(gridDim.x) * kBlock) {
+    const int64_t r = i / chunks;
+    const int c = static_cast<int>(i - r * chunks) * kVec;
+    const int64_t at = packed != nullptr ? packed[r] : r;
+    float sum[kVec] = {};
+    if (at >= 0) {
+#pragma unroll 4
+      for (int k = 0; k < splits; ++k) {
+        float x[kVec];
+        load8(partial + k * split_stride + at * ld + c, x);  // rows are padded to whole chunks
+#pragma unroll
+        for (int e = 0; e < kVec; ++e) sum[e] += x[e];
+      }
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) sum[e] = sum[e] * by * unscale;
+    }
+    store_chunk(out + r * width, c, width, sum);
+  }
+}
+
+// ---------------------------------------------------------------------- host
+
+constexpr int64_t kMaxRows = int64_t{1} << 24;
+constexpr int64_t kMaxVocab = int64_t{1} << 24;
+constexpr int64_t kMaxStride = int64_t{1} << 22;  // of W multiplied in place: 256 rows stay within 32-bit offsets
+constexpr int64_t kPieceBytes = int64_t{512} << 20;  // of P at a time
+constexpr int kUnits = 256;                          // compute units, one workgroup each
+
+// How many parts the depth is cut into so that the workgroups fill the chip: the number with the fullest last
+// round, the smaller at a tie; a part keeps at least 8 stages.
+int choose_splits(int64_t tiles, int64_t depth) {
+  int best = 1;
+  double best_fill = 0.0;
+  for (int s = 1; s <= 32; ++s) {
+    if (s > 1 && depth / kDepth / s < 8) break;
+    const int64_t work = tiles * s, rounds = (work + kUnits - 1) / kUnits;
+    const double fill = static_cast<double>(work) / static_cast<double>(rounds * kUnits) - 0.01 * s;
+    if (fill > best_fill + 1e-9) best = s, best_fill = fill;
+  }
+  return best;
+}
+
+struct LossPlan {
+  bool split, pack_weight;
+  int64_t rows_pad, width_pad, vocab_pad, piece;
+  int64_t hidden[2], weight[2], sums, target_logit, losses;  // offsets
+  int64_t row_scale, alpha, p[2], dh, dw;
+  int splits_h, splits_w;
+  int64_t bytes;
+};
+
+LossPlan loss_plan(int64_t rows, int64_t vocab, int64_t width, int dtype, bool backward) {
+  LossPlan p{};
+  p.split = dtype == ATTNRES_F32;
+  p.pack_weight = p.split || width % kDepth != 0;
+  p.rows_pad = round_up(std::max<int64_t>(rows, 1), kTile);
+  p.width_pad = round_up(width, kDepth);
+  p.vocab_pad = round_up(vocab, kTile);
+  const int parts = p.split ? 2 : 1;
+  int64_t at = 0;
+  const auto take = [&](int64_t bytes) {
+    const int64_t from = at;
+    at += round_up(bytes, 256);
+    return from;
+  };
+  for (int k = 0; k < parts; ++k) p.hidden[k] = take(2 * p.rows_pad * p.width_pad);
+  if (p.pack_weight) {
+    for (int k = 0; k < parts; ++k) p.weight[k] = take(2 * vocab * p.width_pad);
+  }
+  if (!backward) {
+    p.sums = take(8 * (p.vocab_pad / kTile) * p.rows_pad);
+    p.target_logit = take(4 * p.rows_pad);
+    p.losses = take(4 * rows);
+  } else {
+    p.row_scale = take(4 * p.rows_pad);
+    p.alpha = take(16);
+    p.piece = std::min(p.vocab_pad, std::max<int64_t>(kPieceBytes / (2 * parts * p.rows_pad) / kTile, 1) * kTile);
+    const int64_t pieces = (p.vocab_pad + p.piece - 1) / p.piece;
+    p.piece = round_up((p.vocab_pad + pieces - 1) / pieces, kTile);
+    for (int k = 0; k < parts; ++k) p.p[k] = take(2 * p.rows_pad * p.piece);
+    const int64_t tiles_d = (width + kTile - 1) / kTile;
+    p.splits_h = choose_splits(tiles_d * (p.rows_pad / kTile), p.piece);
+    p.dh = take(4 * p.splits_h * p.rows_pad * p.width_pad);
+    p.splits_w = choose_splits(tiles_d * (p.piece / kTile), p.rows_pad);
+    if (p.splits_w > 1) p.dw = take(4 * p.splits_w * p.piece * p.width_pad);
+  }
+  p.bytes = at;
+  return p;
+}
+
+unsigned stride_grid(int64_t items) { return static_cast<unsigned>(std::min<int64_t>((items + kBlock - 1) / kBlock, 8192)); }
+
+struct Call {
+  const void* hidden;
+  int64_t hidden_stride;
+  const void* weight;
+  int64_t weight_stride;
+  int64_t rows, vocab, width;
+  LossPlan plan;
+  Saved saved;
+  char* workspace;
+  hipStream_t stream;
+  template <class X>
+  X* at(int64_t offset) const { return reinterpret_cast<X*>(workspace + offset); }
+};
+
+// The operands of both directions: H's rows that count, packed, and W as it is or packed.
+template <class X>
+void prepare_operands(const Call& c, bool find_scales, Operand* h, Operand* w) {
+  const LossPlan& p = c.plan;
+  constexpr bool kSplit = std::is_same_v<X, float>;
+  const X* hidden = static_cast<const X*>(c.hidden);
+  const X* weight = static_cast<const X*>(c.weight);
+  Header* header = c.saved.header;
+  if constexpr (kSplit) {
+    if (find_scales) {
+      const unsigned grid_h = static_cast<unsigned>(std::min<int64_t>(c.rows, 1024));
+      hipLaunchKernelGGL(attnres_loss_amax_kernel, dim3(grid_h), dim3(kBlock), 0, c.stream, hidden, c.hidden_stride, c.rows,
+                         static_cast<int>(c.width), c.saved.index, &header->count, &header->amax[0]);
+      const unsigned grid_w = static_cast<unsigned>(std::min<int64_t>(c.vocab, 2048));
+      hipLaunchKernelGGL(attnres_loss_amax_kernel, dim3(grid_w), dim3(kBlock), 0, c.stream, weight, c.weight_stride, c.vocab,
+                         static_cast<int>(c.width), static_cast<const int32_t*>(nullptr), static_cast<const int32_t*>(nullptr),
+                         &header->amax[1]);
+    }
+  }
+  uint16_t* packed[2] = {c.at<uint16_t>(p.hidden[0]), kSplit ? c.at<uint16_t>(p.hidden[1]) : nullptr};
+  hipLaunchKernelGGL((attnres_loss_pack_kernel<X>), dim3(stride_grid(p.rows_pad * p.width_pad / kVec)), dim3(kBlock), 0, c.stream,
+                     hidden, c.hidden_stride, c.rows, static_cast<int>(c.width), c.saved.index, &header->count, p.rows_pad,
+                     static_cast<int>(p.width_pad), header, 0, find_scales, packed[0], packed[1]);
+  *h = {{packed[0], packed[1]}, p.width_pad, p.rows_pad, 0};
+  if (p.pack_weight) {
+    uint16_t* to[2] = {c.at<uint16_t>(p.weight[0]), kSplit ? c.at<uint16_t>(p.weight[1]) : nullptr};
+    hipLaunchKernelGGL((attnres_loss_pack_kernel<X>), dim3(stride_grid(c.vocab * p.width_pad / kVec)), dim3(kBlock), 0, c.stream,
+                       weight, c.weight_stride, c.vocab, static_cast<int>(c.width), static_cast<const int32_t*>(nullptr),
+                       static_cast<const int32_t*>(nullptr), c.vocab, static_cast<int>(p.width_pad), header, 1, find_scales, to[0], to[1]);
+    *w = {{to[0], to[1]}, p.width_pad, c.vocab, 0};
+  } else {
+    *w = {{reinterpret_cast<const uint16_t*>(weight), nullptr}, c.weight_stride, c.vocab, 0};
+  }
+}
+
+// X: the inputs' type; T: the operands'.
+template <class X, class T, int SEGMENTS>
+void loss_forward(const Call& c, const void* targets, int target_bytes, int64_t ignore_index, int reduction, float* loss) {
+  const LossPlan& p = c.plan;
+  hipLaunchKernelGGL(attnres_loss_rows_kernel, dim3(1), dim3(kScanThreads), 0, c.stream, targets, target_bytes, c.rows, c.vocab,
+                     ignore_index, c.saved);
+  if (c.rows > 0) {
+    LogitArgs g{};
+    prepare_operands<X>(c, true, &g.product.b, &g.product.a);
+    g.product.count = &c.saved.header->count;
+    g.product.depth = p.width_pad;
+    g.product.tiles_a = static_cast<int>(p.vocab_pad / kTile);
+    g.product.tiles_b = static_cast<int>(p.rows_pad / kTile);
+    g.product.splits = 1;
+    g.header = c.saved.header;
+    g.target = c.saved.target;
+    g.vocab = c.vocab;
+    g.row_tiles = p.rows_pad;
+    g.sums = c.at<f32x2>(p.sums);
+    g.target_logit = c.at<float>(p.target_logit);
+    hipLaunchKernelGGL((attnres_loss_logits_kernel<T, SEGMENTS>), dim3(g.product.tiles_a * g.product.tiles_b), dim3(kThreads), 0,
+                       c.stream, g);
+    float* losses = reduction == ATTNRES_REDUCE_NONE ? loss : c.at<float>(p.losses);
+    hipLaunchKernelGGL(attnres_loss_reduce_kernel, dim3(static_cast<unsigned>((c.rows + 63) / 64)), dim3(kBlock), 0, c.stream, g.sums,
+                       g.product.tiles_a, p.rows_pad, g.target_logit, c.rows, c.saved, losses);
+  }
+  if (reduction != ATTNRES_REDUCE_NONE) {
+    hipLaunchKernelGGL(attnres_loss_total_kernel, dim3(1), dim3(kScanThreads), 0, c.stream, c.at<const float>(p.losses), c.rows,
+                       c.saved.header, reduction == ATTNRES_REDUCE_MEAN ? 1 : 0, loss);
+  }
+}
+
+template <class X, class T, int SEGMENTS>
+void loss_backward(const Call& c, int reduction, const float* grad_loss, void* grad_hidden, void* grad_weight) {
+  const LossPlan& p = c.plan;
+  constexpr int kParts = SEGMENTS == 3 ? 2 : 1;
+  Operand h{}, w{};
+  prepare_operands<X>(c, false, &h, &w);
+  const float p_scale = std::is_same_v<T, Bf16> ? 1.0f : kProbabilityScale;
+  float* alpha = c.at<float>(p.alpha);
+  float* row_scale = c.at<float>(p.row_scale);
+  hipLaunchKernelGGL(attnres_loss_factors_kernel, dim3(1), dim3(kScanThreads), 0, c.stream, grad_loss, reduction, c.saved,
+                     p.rows_pad, p_scale, row_scale, alpha);
+  const int32_t* count = &c.saved.header->count;
+  const int tiles_d = static_cast<int>((c.width + kTile - 1) / kTile), tiles_n = static_cast<int>(p.rows_pad / kTile);
+  Operand probability{{c.at<const uint16_t>(p.p[0]), kParts == 2 ? c.at<const uint16_t>(p.p[1]) : nullptr}, p.piece, 0, 0};
+  for (int64_t v0 = 0; v0 < c.vocab; v0 += p.piece) {
+    const int64_t columns = std::min(p.piece, c.vocab - v0);
+    const int tiles_v = static_cast<int>((columns + kTile - 1) / kTile);
+    Operand piece = w;
+    for (int k = 0; k < kParts; ++k) piece.part[k] = w.part[k] + v0 * w.ld;
+    piece.entries = columns;
+    LogitArgs g{};
+    g.product = {piece, h, count, p.width_pad, 0, tiles_v, tiles_n, 1};
+    g.header = c.saved.header;
+    g.target = c.saved.target;
+    g.vocab = c.vocab;
+    g.first = v0;
+    g.row_tiles = p.rows_pad;
+    g.stats = c.saved.stats;
+    g.row_scale = row_scale;
+    for (int k = 0; k < kParts; ++k) g.p[k] = c.at<uint16_t>(p.p[k]);
+    g.p_ld = p.piece;
+    hipLaunchKernelGGL((attnres_loss_probability_kernel<T, SEGMENTS>), dim3(tiles_v * tiles_n), dim3(kThreads), 0, c.stream, g);
+    if (grad_weight != nullptr) {
+      Operand a = h, b = probability;
+      a.entries = p.width_pad;
+      a.depth = b.depth = p.rows_pad;
+      b.entries = p.piece;
+      GradientArgs e{};
+      e.product = {a, b, count, 0, 1, tiles_d, tiles_v, p.splits_w};
+      e.entries_a = c.width;
+      e.entries_b = columns;
+      const dim3 grid(tiles_d * tiles_v * p.splits_w);
+      X* out = static_cast<X*>(grad_weight) + v0 * c.width;
+      if (p.splits_w == 1) {
+        e.alpha = alpha + 2;
+        e.out = out;
+        e.ld = c.width;
+        hipLaunchKernelGGL((attnres_loss_gradient_kernel<T, X, SEGMENTS, false>), grid, dim3(kThreads), 0, c.stream, e);
+      } else {
+        e.out = c.at<float>(p.dw);
+        e.ld = p.width_pad;
+        e.entries_a = p.width_pad;
+        e.split_stride = p.piece * p.width_pad;
+        hipLaunchKernelGGL((attnres_loss_gradient_kernel<T, float, SEGMENTS, false>), grid, dim3(kThreads), 0, c.stream, e);
+        hipLaunchKernelGGL((attnres_loss_join_kernel<X>), dim3(stride_grid(columns * ((c.width + kVec - 1) / kVec))), dim3(kBlock), 0,
+                           c.stream, c.at<const float>(p.dw), p.splits_w, e.split_stride, p.width_pad,
+                           static_cast<const int32_t*>(nullptr), columns, static_cast<int>(c.width), alpha + 2, out);
+      }
+    }
+    if (grad_hidden != nullptr) {
+      Operand a = piece, b = probability;
+      a.entries = p.pack_weight ? p.width_pad : c.width;
+      a.depth = columns;
+      b.entries = p.rows_pad;
+      GradientArgs e{};
+      e.product = {a, b, count, round_up(columns, kDepth), 0, tiles_d, tiles_n, p.splits_h};
+      e.out = c.at<float>(p.dh);
+      e.ld = p.width_pad;
+      e.split_stride = p.rows_pad * p.width_pad;
+      e.entries_a = p.width_pad;
+      e.entries_b = p.rows_pad;
+      e.add = v0 > 0 ? 1 : 0;
+      e.live_only = 1;
+      hipLaunchKernelGGL((attnres_loss_gradient_kernel<T, float, SEGMENTS, true>), dim3(tiles_d * tiles_n * p.splits_h),
+                         dim3(kThreads), 0, c.stream, e);
+    }
+  }
+  if (grad_hidden != nullptr && c.rows > 0) {
+    hipLaunchKernelGGL((attnres_loss_join_kernel<X>), dim3(stride_grid(c.rows * ((c.width + kVec - 1) / kVec))), dim3(kBlock), 0,
+                       c.stream, c.at<const float>(p.dh), p.splits_h, p.rows_pad * p.width_pad, p.width_pad, c.saved.packed, c.rows,
+                       static_cast<int>(c.width), alpha, static_cast<X*>(grad_hidden));
+  }
+}
+
+// Workgroups of the logits' launch.
+bool fits_grid(int64_t rows, int64_t vocab) {
+  return (rows + kTile - 1) / kTile * ((vocab + kTile - 1) / kTile) <= int64_t{1} << 30;
+}
+
+int check_loss(const void* hidden, int64_t hidden_stride, const void* weight, int64_t weight_stride, int64_t rows, int64_t vocab,
+               int64_t width, int dtype, int reduction) {
+  if (rows < 0 || rows > kMaxRows) return layer_error(ATTNRES_ERR_SHAPE, "rows=%lld outside 0..2^24", (long long)rows);
+  if (vocab < 1 || vocab > kMaxVocab) return layer_error(ATTNRES_ERR_SHAPE, "vocab=%lld outside 1..2^24", (long long)vocab);
+  if (width < 1 || width > ATTNRES_MAX_WIDTH) {
+    return layer_error(ATTNRES_ERR_SHAPE, "width=%lld outside 1..%d", (long long)width, ATTNRES_MAX_WIDTH);
+  }
+  if (!dtype_known(dtype)) return layer_error(ATTNRES_ERR_SHAPE, "unknown dtype %d", dtype);
+  if (reduction < ATTNRES_REDUCE_NONE || reduction > ATTNRES_REDUCE_MEAN) {
+    return layer_error(ATTNRES_ERR_SCALAR, "unknown reduction %d", reduction);
+  }
+  if (!fits_grid(rows, vocab)) return layer_error(ATTNRES_ERR_SHAPE, "rows x vocab outside 2^46");
+  if (hidden_stride < 0 || weight_stride < 0) return layer_error(ATTNRES_ERR_STRIDE, "negative row stride");
+  if ((rows > 0 && hidden == nullptr) || weight == nullptr) return layer_error(ATTNRES_ERR_NULL_POINTER, "hidden or weight is NULL");
+  if (dtype != ATTNRES_F32 && width % kDepth == 0 &&
+      ((reinterpret_cast<uintptr_t>(weight) & 15u) != 0 || weight_stride % 8 != 0 || weight_stride < width ||
+       weight_stride > kMaxStride)) {
+    return layer_error(ATTNRES_ERR_STRIDE, "weight rows must start at multiples of 16 bytes, at most %lld elements apart",
+                       (long long)kMaxStride);
+  }
+  return ATTNRES_OK;
+}
+
+}  // namespace
+}  // namespace layers
+}  // namespace attnres_hip
+
+using namespace attnres_hip;
+using namespace attnres_hip::layers;
+
+extern "C" {
+
+int64_t attnres_hip_loss_saved_bytes(int64_t rows) { return rows < 0 || rows > kMaxRows ? -1 : saved_bytes(rows); }
+
+int64_t attnres_hip_loss_workspace_bytes(int64_t rows, int64_t vocab, int64_t width, int dtype, int backward) {
+  if (rows < 0 || rows > kMaxRows || vocab < 1 || vocab > kMaxVocab || width < 1 || width > ATTNRES_MAX_WIDTH || !dtype_known(dtype) ||
+      !fits_grid(rows, vocab)) {
+    return -1;
+  }
+  return loss_plan(rows, vocab, width, dtype, backward != 0).bytes;
+}
+
+int attnres_hip_loss_forward(const void* hidden, int64_t hidden_stride, const void* weight, int64_t weight_stride,
+                             const void* targets, int target_bytes, int64_t rows, int64_t vocab, int64_t width, int dtype,
+                             int64_t ignore_index, int reduction, float* loss, void* saved, void* workspace,
+                             int64_t workspace_bytes, void* stream) {
+  if (const int status = check_loss(hidden, hidden_stride, weight, weight_stride, rows, vocab, width, dtype, reduction)) return status;
+  if (target_bytes != 4 && target_bytes != 8) return layer_error(ATTNRES_ERR_SHAPE, "targets must be int32 or int64");
+  if (loss == nullptr || saved == nullptr || (rows > 0 && targets == nullptr)) {
+    return layer_error(ATTNRES_ERR_NULL_POINTER, "targets, loss or saved is NULL");
+  }
+  const Call c{hidden, hidden_stride, weight, weight_stride, rows, vocab, width, loss_plan(rows, vocab, width, dtype, false),
+               saved_views(saved, rows), static_cast<char*>(workspace), static_cast<hipStream_t>(stream)};
+  if (workspace == nullptr || workspace_bytes < c.plan.bytes) {
+    return layer_error(ATTNRES_ERR_WORKSPACE, "workspace of %lld bytes, %lld needed", (long long)workspace_bytes,
+                       (long long)c.plan.bytes);
+  }
+  if (dtype == ATTNRES_BF16) loss_forward<Bf16, Bf16, 1>(c, targets, target_bytes, ignore_index, reduction, loss);
+  else if (dtype == ATTNRES_F16) loss_forward<F16, F16, 1>(c, targets, target_bytes, ignore_index, reduction, loss);
+  else loss_forward<float, F16, 3>(c, targets, target_bytes, ignore_index, reduction, loss);
+  return layer_launch_status("loss forward");
+}
+
+int attnres_hip_loss_backward(const void* hidden, int64_t hidden_stride, const void* weight, int64_t weight_stride, int64_t rows,
+                              int64_t vocab, int64_t width, int dtype, int reduction, const void* saved, const float* grad_loss,
+                              void* grad_hidden, void* grad_weight, void* workspace, int64_t workspace_bytes, void* stream) {
+  if (const int status = check_loss(hidden, hidden_stride, weight, weight_stride, rows, vocab, width, dtype, reduction)) return status;
+  if (saved == nullptr || grad_loss == nullptr) return layer_error(ATTNRES_ERR_NULL_POINTER, "saved or grad_loss is NULL");
+  const Call c{hidden, hidden_stride, weight, weight_stride, rows, vocab, width, loss_plan(rows, vocab, width, dtype, true),
+               saved_views(const_cast<void*>(saved), rows), static_cast<char*>(workspace), static_cast<hipStream_t>(stream)};
+  if (workspace == nullptr || workspace_bytes < c.plan.bytes) {
+    return layer_error(ATTNRES_ERR_WORKSPACE, "workspace of %lld bytes, %lld needed", (long long)workspace_bytes,
+                       (long long)c.plan.bytes);
+  }
+  if (grad_hidden == nullptr && grad_weight == nullptr) return ATTNRES_OK;
+  if (dtype == ATTNRES_BF16) loss_backward<Bf16, Bf16, 1>(c, reduction, grad_loss, grad_hidden, grad_weight);
+  else if (dtype == ATTNRES_F16) loss_backward<F16, F16, 1>(c, reduction, grad_loss, grad_hidden, grad_weight);
+  else loss_backward<float, F16, 3>(c, reduction, grad_loss, grad_hidden, grad_weight);
+  return layer_launch_status("loss backward");
+}
+
+}  // extern "C"
