@@ -214,12 +214,12 @@ Tensor embedding(const Tensor& tokens, const Tensor& weight, const OptionalTenso
 
 // -------------------------------------------------------------------- loss
 
-// The vocabulary's rows as the kernels take them: 16-bit rows of whole 64-element steps are
+// The vocabulary's rows as the kernels take them: 16-bit rows of whole 32-element steps are
 // multiplied where they lie and have to start at multiples of 16 bytes; a copy does.
 Rows weight_rows(const Tensor& weight) {
   Rows rows = rows_view(weight);
   if (weight.size(0) == 1 && rows.stride < weight.size(1)) rows.stride = weight.size(1);
-  const bool in_place = weight.scalar_type() != at::kFloat && weight.size(1) % 64 == 0;
+  const bool in_place = weight.scalar_type() != at::kFloat && weight.size(1) % 32 == 0;
   if (in_place && (reinterpret_cast<uintptr_t>(rows.tensor.data_ptr()) % 16 != 0 || rows.stride % 8 != 0 ||
                    rows.stride < weight.size(1) || rows.stride > (int64_t{1} << 22))) {
     Tensor copy = torch::empty(weight.sizes(), weight.options().memory_format(at::MemoryFormat::Contiguous));

@@ -30,8 +30,10 @@ namespace layers {
 namespace {
 
 constexpr int kTile = 256;     // rows and columns of a workgroup's tile
-constexpr int kDepth = 64;     // of a tile's operands in LDS
-constexpr int kThreads = 512;  // 8 wavefronts of 128 x 64 outputs
+constexpr int kDepth = 32;     // of a stage of a tile's operands in LDS
+constexpr int kStages = 4;     // in LDS: one that is multiplied, three on their way
+constexpr int kThreads = 256;  // 4 wavefronts of 128 x 128 outputs, one per SIMD
+constexpr int kLoads = 4;      // per wavefront, operand and stage: 1 KB each
 constexpr int kOperand = kTile * kDepth;  // elements of one operand's stage
 constexpr float kProbabilityScale = 16384.0f;
 
@@ -77,7 +79,7 @@ inline Saved saved_views(void* base, int64_t rows) {
 // columns (row k holds all of the operand's entries).  Both go to LDS as they lie, 16 bytes
 // per lane straight from memory; a column operand's fragments are transposed on the way
 // from LDS (ds_read_b64_tr_b16).  16-byte slots are permuted within an LDS row so that the lanes of
-// a fragment read meet every bank once: slot = chunk ^ (row % 8) for rows of k (128 bytes), chunk ^
+// a fragment read meet every bank once: slot = chunk ^ (row / 2 % 4) for rows of k (64 bytes), chunk ^
 // 4 (k % 4) for columns (512 bytes).
 
 struct Operand {
@@ -97,49 +99,52 @@ struct Product {
 
 template <bool ROWS>
 struct Loader {
-  uint32_t offset[4];  // bytes from the stage's origin; columns: of the chunk alone
-  int row[4];          // columns: k of the load
-  uint32_t slot;       // LDS byte of this wavefront's first load
+  uint32_t offset[kLoads];  // bytes from the stage's origin; columns: of the chunk alone
+  uint32_t slot;            // LDS byte of this wavefront's first load
+  int row;                  // columns: k of the first load
   __device__ __forceinline__ void init(const Operand& o, int64_t entry0, int wave, int lane) {
-    slot = static_cast<uint32_t>(wave) * 4096;
+    slot = static_cast<uint32_t>(wave) * (kLoads * 1024);
+    row = wave * kLoads * 2 + lane / 32;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    for (int j = 0; j < kLoads; ++j) {
       if constexpr (ROWS) {
-        const int r = (wave * 4 + j) * 8 + lane / 8;
+        const int r = (wave * kLoads + j) * 16 + lane / 4;
         const int64_t left = o.entries - 1 - entry0;
         const int64_t at = r < left ? r : left;
-        offset[j] = static_cast<uint32_t>((at * o.ld + ((lane % 8) ^ (lane / 8)) * 8) * 2);
+        offset[j] = static_cast<uint32_t>((at * o.ld + ((lane % 4) ^ (lane / 8 % 4)) * 8) * 2);
       } else {
-        row[j] = (wave * 4 + j) * 2 + lane / 32;
-        const int chunk = (lane % 32) ^ ((row[j] & 3) << 2);
+        const int chunk = (lane % 32) ^ (((row + j * 2) & 3) << 2);
         const int64_t left = o.entries - 8 - entry0;
         const int64_t at = chunk * 8 < left ? chunk * 8 : left;
         offset[j] = static_cast<uint32_t>(at * 2);
       }
     }
   }
-  // one 1-KB load of the stage at k0 into `lds`
-  __device__ __forceinline__ void load(const Operand& o, const uint16_t* origin, int64_t k0, uint16_t* lds, int j) const {
-    const char* base = reinterpret_cast<const char*>(origin);
+  // The j-th 1-KB load of a stage into LDS byte `lds`; base: the stage's origin (scalar), left: k's
+  // of the stage that a column operand holds, less one.  Written out, since the compiler makes transposing LDS reads
+  // wait for every load into LDS that it knows of; what has to have landed is waited for in landed().
+  // The address registers are read when the load is issued, and nothing comes back in registers.
+  __device__ __forceinline__ void load(const Operand& o, const char* base, int left, uint32_t lds, int j) const {
     uint32_t at = offset[j];
-    if constexpr (ROWS) {
-      base += k0 * 2;
-    } else {
-      base += k0 * o.ld * 2;
-      const int64_t left = o.depth - 1 - k0;
-      at += static_cast<uint32_t>((row[j] < left ? row[j] : left) * o.ld * 2);
-    }
-    __builtin_amdgcn_global_load_lds(reinterpret_cast<const ATTNRES_GLOBAL uint32_t*>(reinterpret_cast<uintptr_t>(base + at)),
-                                     (ATTNRES_LDS uint32_t*)(reinterpret_cast<char*>(lds) + slot + j * 1024), 16, 0, 0);
+    if constexpr (!ROWS) at += static_cast<uint32_t>(min(row + j * 2, left)) * static_cast<uint32_t>(o.ld * 2);
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+                 :
+                 : "s"(lds + slot + j * 1024), "v"(at), "s"(base)
+                 : "m0");
   }
 };
+
+// The LDS byte of a pointer into LDS.
+__device__ __forceinline__ uint32_t lds_byte(const uint16_t* p) {
+  return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((const ATTNRES_LDS uint16_t*)p));
+}
 
 // Fragment r (32 entries) of the 16 k's at `step`: lane l holds entry l % 32, k = 8 (l / 32) + 0..7.
 template <bool ROWS>
 __device__ __forceinline__ s16x8 fragment(const uint16_t* lds, int entry, int step, int lane) {
   if constexpr (ROWS) {
     const int row = entry + lane % 32;
-    const int slot = (step * 2 + lane / 32) ^ (lane & 7);
+    const int slot = (step * 2 + lane / 32) ^ (lane / 2 % 4);
     return *reinterpret_cast<const s16x8*>(lds + row * kDepth + slot * 8);
   } else {
     // 16 lanes read 4 k's of 16 entries and get one entry's 4 k's each
@@ -162,6 +167,8 @@ __device__ __forceinline__ f32x16 mfma(s16x8 a, s16x8 b, f32x16 c) {
   }
 }
 
+__device__ __forceinline__ int wave_index() { return __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x / 64)); }
+
 struct TileAt {
   int a, b, split;
 };
@@ -183,65 +190,133 @@ __device__ __forceinline__ TileAt tile_at(const Product& p) {
   return {at / size, group * kGroup + at % size, split};
 }
 
-using Accumulators = f32x16[4][2];  // [32 entries of A][32 entries of B]; lane l, register i: entry
+using Accumulators = f32x16[4][4];  // [32 entries of A][32 entries of B]; lane l, register i: entry
                                     // 8 (i / 4) + 4 (l / 32) + i % 4 of A, l % 32 of B
 
-// The sum of a tile over its split's k's; SEGMENTS 3: hi hi + hi lo + lo hi.
+// A pointer that every lane holds, in scalar registers, and opaque from here on.
+__device__ __forceinline__ const char* scalar(const char* p) {
+  const uint64_t bits = reinterpret_cast<uint64_t>(p);
+  uint32_t lo = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(bits)));
+  uint32_t hi = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(bits >> 32)));
+  asm volatile("" : "+s"(lo), "+s"(hi));
+  return reinterpret_cast<const char*>(static_cast<uint64_t>(hi) << 32 | lo);
+}
+
+// This wavefront's reads from LDS are done and its loads of the next stage have landed, and so it is for every
+// wavefront (a barrier alone waits for neither).  Loads arrive in order: with `more`, those of
+// the two stages after the next one may still be on their way.
+__device__ __forceinline__ void landed(bool more) {
+  static_assert(kStages == 4 && kLoads == 4, "two stages of eight loads");
+  if (more) {
+    asm volatile("s_waitcnt vmcnt(16) lgkmcnt(0)" ::: "memory");
+  } else {
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+  }
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+// The stages of a tile's split; none where there are fewer stages than splits.
+struct Stages {
+  int first, count;
+};
+__device__ __forceinline__ Stages stages_of(const Product& p, int split) {
+  const int64_t depth = p.depth_is_count ? *p.count : p.depth;
+  const int64_t all = (depth + kDepth - 1) / kDepth;
+  const int first = static_cast<int>(all * split / p.splits);
+  return {__builtin_amdgcn_readfirstlane(first),
+          __builtin_amdgcn_readfirstlane(static_cast<int>(all * (split + 1) / p.splits) - first)};
+}
+
+// The sum of a tile over its split's k's (at least one stage); SEGMENTS 3: hi hi + hi lo + lo hi.
 template <class T, int SEGMENTS, bool A_ROWS, bool B_ROWS>
-__device__ __forceinline__ void multiply(const Product& p, const TileAt& tile, uint16_t* lds, Accumulators& acc) {
-  const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
+__device__ __forceinline__ void multiply(const Product& p, const TileAt& tile, const Stages& range, uint16_t* lds, Accumulators& acc) {
+  const int wave = wave_index(), lane = threadIdx.x % 64;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
 #pragma unroll
-    for (int j = 0; j < 2; ++j) acc[i][j] = f32x16{};
+    for (int j = 0; j < 4; ++j) acc[i][j] = f32x16{};
   }
-  const int64_t depth = p.depth_is_count ? (static_cast<int64_t>(*p.count) + kDepth - 1) / kDepth * kDepth : p.depth;
-  const int stages_all = static_cast<int>(depth / kDepth);
-  const int first = static_cast<int>(static_cast<int64_t>(stages_all) * tile.split / p.splits);
-  const int stages = static_cast<int>(static_cast<int64_t>(stages_all) * (tile.split + 1) / p.splits) - first;
-  if (stages == 0) return;
+  const int first = range.first, stages = range.count;
   const int64_t a0 = static_cast<int64_t>(tile.a) * kTile, b0 = static_cast<int64_t>(tile.b) * kTile;
   Loader<A_ROWS> load_a;
   Loader<B_ROWS> load_b;
   load_a.init(p.a, a0, wave, lane);
   load_b.init(p.b, b0, wave, lane);
-  const int64_t origin_a = A_ROWS ? a0 * p.a.ld : a0, origin_b = B_ROWS ? b0 * p.b.ld : b0;
+  // bytes from the operand's start to the tile, and from a stage to the next
+  const int64_t origin_a = (A_ROWS ? a0 * p.a.ld : a0) * 2, origin_b = (B_ROWS ? b0 * p.b.ld : b0) * 2;
+  const int64_t next_a = (A_ROWS ? 1 : p.a.ld) * kDepth * 2, next_b = (B_ROWS ? 1 : p.b.ld) * kDepth * 2;
   int segment = 0, stage = 0;  // of the next load
-  const auto load_stage = [&](int buffer) {
-    uint16_t* to = lds + buffer * 2 * kOperand;
-    const int64_t k0 = static_cast<int64_t>(first + stage) * kDepth;
-    const uint16_t* a = p.a.part[SEGMENTS == 3 && segment == 2] + origin_a;
-    const uint16_t* b = p.b.part[SEGMENTS == 3 && segment == 1] + origin_b;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      load_a.load(p.a, a, k0, to, j);
-      load_b.load(p.b, b, k0, to + kOperand, j);
-    }
+  // one scalar base per half stage and 32-bit offsets
+  const auto base_a = [&] {
+    return scalar(reinterpret_cast<const char*>(p.a.part[SEGMENTS == 3 && segment == 2]) + origin_a + (first + stage) * next_a);
+  };
+  const auto base_b = [&] {
+    return scalar(reinterpret_cast<const char*>(p.b.part[SEGMENTS == 3 && segment == 1]) + origin_b + (first + stage) * next_b);
+  };
+  // k's left in a column operand from this stage on, less one
+  const auto left = [&](const Operand& o) {
+    return __builtin_amdgcn_readfirstlane(static_cast<int>(o.depth - 1 - static_cast<int64_t>(first + stage) * kDepth));
+  };
+  const auto loaded = [&] {
     if (++stage == stages) stage = 0, ++segment;
   };
-  load_stage(0);
-  const int total = stages * SEGMENTS;
-  const int wa = (wave % 2) * 128, wb = (wave / 2) * 64;
-  for (int s = 0; s < total; ++s) {
-    // the stage has landed (a barrier alone does not wait for loads into LDS), and the other
-    // buffer is no longer read
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-    if (s + 1 < total) load_stage((s + 1) & 1);
-    const uint16_t* from = lds + (s & 1) * 2 * kOperand;
+  const auto buffer = [&](int s) { return lds + (s % kStages) * 2 * kOperand; };
+  const int wa = (wave % 2) * 128, wb = (wave / 2) * 128;
+  using Fragments = s16x8[4];
+  // One step: 16 matrix instructions on (a, b), between them the reads of the next step's
+  // fragments, in the order of their use, and up to four loads.  In order, because a wavefront
+  // issues in order: a burst of reads or loads would keep the matrix core waiting.
+  const auto step = [&](const Fragments& a, const Fragments& b, Fragments& na, Fragments& nb, const uint16_t* from, int next,
+                        auto load) {
 #pragma unroll
-    for (int step = 0; step < kDepth / 16; ++step) {
-      s16x8 a[4], b[2];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) a[i] = fragment<A_ROWS>(from, wa + i * 32, step, lane);
-#pragma unroll
-      for (int j = 0; j < 2; ++j) b[j] = fragment<B_ROWS>(from + kOperand, wb + j * 32, step, lane);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-#pragma unroll
-        for (int j = 0; j < 2; ++j) acc[i][j] = mfma<T>(a[i], b[j], acc[i][j]);
+    for (int m = 0; m < 16; ++m) {
+      acc[m / 4][m % 4] = mfma<T>(a[m / 4], b[m % 4], acc[m / 4][m % 4]);
+      if (m % 2 == 0) {
+        constexpr int kOrder[8] = {0, 4, 5, 6, 7, 1, 2, 3};  // a: 0..3, b: 4..7
+        const int f = kOrder[m / 2];
+        if (f < 4) na[f] = fragment<A_ROWS>(from, wa + f * 32, next, lane);
+        else nb[f - 4] = fragment<B_ROWS>(from + kOperand, wb + (f - 4) * 32, next, lane);
       }
+      if (m % 4 == 3) load(m / 4);
+      if (m % 2 == 1) __builtin_amdgcn_sched_barrier(0);
     }
+  };
+  const int total = stages * SEGMENTS;
+  for (int s = 0; s < kStages && s < total; ++s) {
+    const char *a = base_a(), *b = base_b();
+    const int left_a = left(p.a), left_b = left(p.b);
+    for (int j = 0; j < kLoads; ++j) load_a.load(p.a, a, left_a, lds_byte(buffer(s)), j);
+    for (int j = 0; j < kLoads; ++j) load_b.load(p.b, b, left_b, lds_byte(buffer(s) + kOperand), j);
+    loaded();
+  }
+  landed(total >= kStages);
+  Fragments a0f, b0f, a1f, b1f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    a0f[i] = fragment<A_ROWS>(lds, wa + i * 32, 0, lane);
+    b0f[i] = fragment<B_ROWS>(lds + kOperand, wb + i * 32, 0, lane);
+  }
+  for (int s = 0; s < total; ++s) {
+    // B's half of the stage three ahead, whose A's half was loaded in the last trip.  The branches hold the
+    // loads alone: no accumulator meets another path.
+    const bool late = s > 0 && s + kStages - 1 < total;
+    const char* b = base_b();
+    const int left_b = left(p.b);
+    const uint32_t to_b = lds_byte(buffer(s + kStages - 1) + kOperand);
+    step(a0f, b0f, a1f, b1f, buffer(s), 1, [&](int j) {
+      if (late) load_b.load(p.b, b, left_b, to_b, j);
+    });
+    if (late) loaded();
+    // both steps' fragments of this stage are in registers: its buffer is free; the next stage has landed
+    landed(s + kStages - 1 < total);
+    const bool early = s + kStages < total;
+    const char* a = base_a();
+    const int left_a = left(p.a);
+    const uint32_t to_a = lds_byte(buffer(s));
+    step(a1f, b1f, a0f, b0f, buffer(s + 1), 0, [&](int j) {
+      if (early) load_a.load(p.a, a, left_a, to_a, j);
+    });
   }
   __syncthreads();  // LDS is free for the epilogue
 }
@@ -290,48 +365,68 @@ struct LogitArgs {
 // Forward: (maximum, sum) of a tile's 256 logits per row, and the target's logit.
 template <class T, int SEGMENTS>
 __global__ void __launch_bounds__(kThreads) attnres_loss_logits_kernel(LogitArgs g) {
-  __shared__ __align__(16) uint16_t lds[4 * kOperand];
+  __shared__ __align__(16) uint16_t lds[kStages * 2 * kOperand];
   const TileAt tile = tile_at(g.product);
   const int count = *g.product.count;
   if (tile.b * kTile >= count) return;
   Accumulators acc;
-  multiply<T, SEGMENTS, true, true>(g.product, tile, lds, acc);
-  const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
+  multiply<T, SEGMENTS, true, true>(g.product, tile, stages_of(g.product, 0), lds, acc);
+  const int wave = wave_index(), lane = threadIdx.x % 64;
   const Unscale unscale(SEGMENTS == 3 ? g.header : nullptr);
   const int64_t v0 = static_cast<int64_t>(tile.a) * kTile + (wave % 2) * 128;
-  const int limit = static_cast<int>(g.vocab - v0 < 128 ? g.vocab - v0 : 128);
+  const int limit = __builtin_amdgcn_readfirstlane(static_cast<int>(g.vocab - v0 < 128 ? g.vocab - v0 : 128));
   f32x2* meet = reinterpret_cast<f32x2*>(lds);  // [2][256]
+  // ENDS: the vocabulary ends in this half of the tile
+  const auto reduce = [&](auto ends) {
+    constexpr bool ENDS = decltype(ends)::value;
+    const int last = limit - 4 * (lane / 32);  // entries below it count
 #pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    const int column = (wave / 2) * 64 + j * 32 + lane % 32;
-    const int row = tile.b * kTile + column;
-    const int64_t from_v0 = row < count ? g.target[row] - v0 : -1;
-    const int rel = from_v0 >= 0 && from_v0 < 128 ? static_cast<int>(from_v0) : -1;
-    float top = -__builtin_inff();
+    for (int j = 0; j < 4; ++j) {
+      const int column = (wave / 2) * 128 + j * 32 + lane % 32;
+      const int row = tile.b * kTile + column;
+      const int64_t from_v0 = g.target[min(row, count - 1)] - v0;
+      const int rel = row < count && from_v0 >= 0 && from_v0 < 128 ? static_cast<int>(from_v0) : -1;
+      float top = -__builtin_inff();
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+      for (int i = 0; i < 4; ++i) {
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const int v = i * 32 + 8 * (e / 4) + 4 * (lane / 32) + e % 4;
-        const float l = v < limit ? unscale(acc[i][j][e]) : -__builtin_inff();
-        acc[i][j][e] = l;
-        top = fmaxf(top, l);
-        if (v == rel) g.target_logit[row] = l;
+        for (int e = 0; e < 16; ++e) {
+          const float x = acc[i][j][e];
+          top = fmaxf(top, !ENDS || i * 32 + 8 * (e / 4) + e % 4 < last ? x : -__builtin_inff());
+        }
       }
-    }
-    top = fmaxf(top, __shfl_xor(top, 32, 64));
-    const float from = top == -__builtin_inff() ? 0.0f : top;  // nothing but NaN, or nothing at all
-    float sum = 0.0f;
+      top = unscale(fmaxf(top, __shfl_xor(top, 32, 64)));
+      if (__any(rel >= 0)) {
+        float own = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < 4; ++i) {
 #pragma unroll
-      for (int e = 0; e < 16; ++e) sum += __expf(acc[i][j][e] - from);
+          for (int e = 0; e < 16; ++e) own = i * 32 + 8 * (e / 4) + e % 4 == rel - 4 * (lane / 32) ? acc[i][j][e] : own;
+        }
+        if (rel >= 0 && (rel >> 2 & 1) == lane / 32) g.target_logit[row] = unscale(own);
+      }
+      const float from = top == -__builtin_inff() ? 0.0f : top;  // nothing but NaN, or nothing at all
+      float sum = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const float x = __expf(unscale(acc[i][j][e]) - from);
+          sum += !ENDS || i * 32 + 8 * (e / 4) + e % 4 < last ? x : 0.0f;
+        }
+      }
+      sum += __shfl_xor(sum, 32, 64);
+      if (lane < 32) meet[(wave % 2) * kTile + column] = f32x2{top, sum};
+      __builtin_amdgcn_sched_barrier(0);  // one column's outputs at a time: no registers to spill
     }
-    sum += __shfl_xor(sum, 32, 64);
-    if (lane < 32) meet[(wave % 2) * kTile + column] = f32x2{top, sum};
+  };
+  if (limit < 128) {
+    reduce(std::true_type{});
+  } else {
+    reduce(std::false_type{});
   }
   __syncthreads();
-  if (threadIdx.x < kTile) {
+  if (threadIdx.x < kTile) {  // every thread a row
     g.sums[static_cast<int64_t>(tile.a) * g.row_tiles + tile.b * kTile + threadIdx.x] =
         join(meet[threadIdx.x], meet[kTile + threadIdx.x]);
   }
@@ -344,63 +439,79 @@ __device__ __forceinline__ int staged(int row, int chunk) { return row * 32 + (c
 // Backward: P of a tile, rounded to the operands' type.
 template <class T, int SEGMENTS>
 __global__ void __launch_bounds__(kThreads) attnres_loss_probability_kernel(LogitArgs g) {
-  __shared__ __align__(16) uint16_t lds[4 * kOperand];
+  __shared__ __align__(16) uint16_t lds[kStages * 2 * kOperand];
   const TileAt tile = tile_at(g.product);
   const int count = *g.product.count;
   if (tile.b * kTile >= count) return;
   Accumulators acc;
-  multiply<T, SEGMENTS, true, true>(g.product, tile, lds, acc);
-  const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
+  multiply<T, SEGMENTS, true, true>(g.product, tile, stages_of(g.product, 0), lds, acc);
+  const int wave = wave_index(), lane = threadIdx.x % 64;
   const Unscale unscale(SEGMENTS == 3 ? g.header : nullptr);
   const int64_t v0 = g.first + static_cast<int64_t>(tile.a) * kTile + (wave % 2) * 128;
-  const int limit = static_cast<int>(g.vocab - v0 < 128 ? g.vocab - v0 : 128);
+  const int limit = __builtin_amdgcn_readfirstlane(static_cast<int>(g.vocab - v0 < 128 ? g.vocab - v0 : 128));
   constexpr int kParts = SEGMENTS == 3 ? 2 : 1;
+  // With two parts, the columns of two wavefronts at a time: hi and lo of 128 rows are staged together.
+  constexpr int kColumns = kTile / kParts;
+  const auto stage = [&](auto ends, int base) {
+    constexpr bool ENDS = decltype(ends)::value;
+    const int last = limit - 4 * (lane / 32);
 #pragma unroll
-  for (int part = 0; part < kParts; ++part) {
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const int column = (wave / 2) * 64 + j * 32 + lane % 32;
+    for (int j = 0; j < 4; ++j) {
+      const int column = (wave / 2) * 128 + j * 32 + lane % 32;
       const int row = tile.b * kTile + column;
-      const bool live = row < count;
-      const int64_t from_v0 = live ? g.target[row] - v0 : -1;
-      const int rel = from_v0 >= 0 && from_v0 < 128 ? static_cast<int>(from_v0) : -1;
-      const f32x2 stats = live ? g.stats[row] : f32x2{0.0f, 0.0f};
-      const float by = live ? g.row_scale[row] : 0.0f;
+      const int at = min(row, count - 1);
+      const int64_t from_v0 = g.target[at] - v0;
+      const int rel = from_v0 >= 0 && from_v0 < 128 ? static_cast<int>(from_v0) - 4 * (lane / 32) : -128;
+      // a row past the last one has zeros in H, so logits of 0, and a factor of 0
+      const f32x2 stats = {row < count ? g.stats[at].x : 0.0f, g.stats[at].y};
+      const float by = g.row_scale[row];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          uint32_t packed[2];
+          float x[4];
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const int v = i * 32 + 8 * q + 4 * (lane / 32) + e;
-            if (part == 0) {
-              float x = __expf(unscale(acc[i][j][4 * q + e]) - stats.x) * stats.y;
-              if (v == rel) x -= 1.0f;
-              acc[i][j][4 * q + e] = live && v < limit ? x * by : 0.0f;
-            }
-          }
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            packed[e] = pack2<T>(acc[i][j][4 * q + 2 * e], acc[i][j][4 * q + 2 * e + 1]);
-            if (kParts == 2 && part == 0) {  // what the first part leaves
-              acc[i][j][4 * q + 2 * e] -= to_f32(T{static_cast<uint16_t>(packed[e] & 0xffffu)});
-              acc[i][j][4 * q + 2 * e + 1] -= to_f32(T{static_cast<uint16_t>(packed[e] >> 16)});
-            }
+            x[e] = __expf(unscale(acc[i][j][4 * q + e]) - stats.x) * stats.y;
+            if (i * 32 + 8 * q + e == rel) x[e] -= 1.0f;
+            x[e] *= by;
+            if (ENDS && i * 32 + 8 * q + e >= last) x[e] = 0.0f;
+            // the FP32 value itself: hi has to be the same number where it is stored and where lo
+            // is what it leaves, and a product folded into one of the conversions rounds apart
+            if (kParts == 2) asm("" : "+v"(x[e]));
           }
           const int chunk = (wave % 2) * 16 + i * 4 + q;
-          *reinterpret_cast<uint64_t*>(lds + staged(column, chunk) * 8 + (lane / 32) * 4) =
-              static_cast<uint64_t>(packed[1]) << 32 | packed[0];
+          uint16_t* to = lds + staged(column - base, chunk) * 8 + (lane / 32) * 4;
+#pragma unroll
+          for (int part = 0; part < kParts; ++part) {
+            const uint32_t packed[2] = {pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3])};
+            *reinterpret_cast<uint64_t*>(to + part * kColumns * kTile) = static_cast<uint64_t>(packed[1]) << 32 | packed[0];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] -= to_f32(T{static_cast<uint16_t>(packed[e / 2] >> (16 * (e % 2)))});  // lo
+          }
         }
+        __builtin_amdgcn_sched_barrier(0);  // 16 outputs at a time: no registers to spill
+      }
+    }
+  };
+  for (int base = 0; base < kTile; base += kColumns) {
+    if (kParts == 1 || wave / 2 == base / kColumns) {
+      if (limit < 128) {
+        stage(std::true_type{}, base);
+      } else {
+        stage(std::false_type{}, base);
       }
     }
     __syncthreads();
-    for (int k = threadIdx.x; k < kTile * 32; k += kThreads) {
-      const int column = k / 32, chunk = k % 32;
-      *reinterpret_cast<u32x4*>(g.p[part] + (static_cast<int64_t>(tile.b) * kTile + column) * g.p_ld + tile.a * kTile + chunk * 8) =
-          *reinterpret_cast<const u32x4*>(lds + staged(column, chunk) * 8);
+#pragma unroll
+    for (int part = 0; part < kParts; ++part) {
+      for (int k = threadIdx.x; k < kColumns * 32; k += kThreads) {
+        const int column = k / 32, chunk = k % 32;
+        *reinterpret_cast<u32x4*>(g.p[part] + (static_cast<int64_t>(tile.b) * kTile + base + column) * g.p_ld + tile.a * kTile +
+                                  chunk * 8) = *reinterpret_cast<const u32x4*>(lds + part * kColumns * kTile + staged(column, chunk) * 8);
+      }
     }
-    if (part + 1 < kParts) __syncthreads();
+    if (base + kColumns < kTile) __syncthreads();
   }
 }
 
@@ -418,16 +529,28 @@ struct GradientArgs {
   int live_only;       // entries of B past the packed rows are not needed
 };
 
+// A tile's outputs where there is nothing to multiply.
+template <class OUT>
+__device__ __forceinline__ void zero_tile(const GradientArgs& g, const TileAt& tile, OUT* out) {
+  if (g.add) return;
+  out += tile.split * g.split_stride;
+  const int64_t a = static_cast<int64_t>(tile.a) * kTile + threadIdx.x, b0 = static_cast<int64_t>(tile.b) * kTile;
+  if (a >= g.entries_a) return;
+  for (int64_t b = b0; b < b0 + kTile && b < g.entries_b; ++b) out[b * g.ld + a] = from_f32<OUT>(0.0f);
+}
+
 // dH (A: W by columns, B: P by rows) and dW (A: H by columns, B: P by columns).  OUT float:
 // FP32 partial sums or an FP32 gradient; else the 16-bit gradient itself.
 template <class T, class OUT, int SEGMENTS, bool B_ROWS>
 __global__ void __launch_bounds__(kThreads) attnres_loss_gradient_kernel(GradientArgs g) {
-  __shared__ __align__(16) uint16_t lds[4 * kOperand];
+  __shared__ __align__(16) uint16_t lds[kStages * 2 * kOperand];
   const TileAt tile = tile_at(g.product);
   if (g.live_only && tile.b * kTile >= *g.product.count) return;
+  const Stages stages = stages_of(g.product, tile.split);
+  if (stages.count == 0) return zero_tile(g, tile, static_cast<OUT*>(g.out));
   Accumulators acc;
-  multiply<T, SEGMENTS, false, B_ROWS>(g.product, tile, lds, acc);
-  const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
+  multiply<T, SEGMENTS, false, B_ROWS>(g.product, tile, stages, lds, acc);
+  const int wave = wave_index(), lane = threadIdx.x % 64;
   const float by = g.alpha != nullptr ? g.alpha[0] : 1.0f, unscale = g.alpha != nullptr ? g.alpha[1] : 1.0f;
   OUT* out = static_cast<OUT*>(g.out) + tile.split * g.split_stride;
   const int64_t a0 = static_cast<int64_t>(tile.a) * kTile, b0 = static_cast<int64_t>(tile.b) * kTile;
@@ -438,8 +561,8 @@ __global__ void __launch_bounds__(kThreads) attnres_loss_gradient_kernel(Gradien
   for (int round = 0; round < kRounds; ++round) {
     if (!kWide || wave % 2 == round) {
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const int column = (wave / 2) * 64 + j * 32 + lane % 32;
+      for (int j = 0; j < 4; ++j) {
+        const int column = (wave / 2) * 128 + j * 32 + lane % 32;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
 #pragma unroll
@@ -456,6 +579,7 @@ __global__ void __launch_bounds__(kThreads) attnres_loss_gradient_kernel(Gradien
                   static_cast<uint64_t>(pack2<OUT>(x[2], x[3])) << 32 | pack2<OUT>(x[0], x[1]);
             }
           }
+          __builtin_amdgcn_sched_barrier(0);  // 16 outputs at a time: no registers to spill
         }
       }
     }
@@ -591,7 +715,8 @@ __global__ void __launch_bounds__(kBlock) attnres_loss_pack_kernel(const X* __re
       if constexpr (std::is_same_v<X, float>) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float a = v[2 * e] * scale, b = v[2 * e + 1] * scale;
+          float a = v[2 * e] * scale, b = v[2 * e + 1] * scale;
+          asm("" : "+v"(a), "+v"(b));  // one rounding to hi, as in the probabilities
           h[e] = pack2<F16>(a, b);
           l[e] = pack2<F16>(a - to_f32(F16{static_cast<uint16_t>(h[e] & 0xffffu)}),
                             b - to_f32(F16{static_cast<uint16_t>(h[e] >> 16)}));
@@ -724,12 +849,12 @@ constexpr int64_t kPieceBytes = int64_t{512} << 20;  // of P at a time
 constexpr int kUnits = 256;                          // compute units, one workgroup each
 
 // How many parts the depth is cut into so that the workgroups fill the chip: the number with the fullest last
-// round, the smaller at a tie; a part keeps at least 8 stages.
+// round, the smaller at a tie; a part keeps at least 16 stages.
 int choose_splits(int64_t tiles, int64_t depth) {
   int best = 1;
   double best_fill = 0.0;
   for (int s = 1; s <= 32; ++s) {
-    if (s > 1 && depth / kDepth / s < 8) break;
+    if (s > 1 && depth / kDepth / s < 16) break;
     const int64_t work = tiles * s, rounds = (work + kUnits - 1) / kUnits;
     const double fill = static_cast<double>(work) / static_cast<double>(rounds * kUnits) - 0.01 * s;
     if (fill > best_fill + 1e-9) best = s, best_fill = fill;
