@@ -32,8 +32,14 @@ namespace {
 constexpr int kTile = 256;     // rows and columns of a workgroup's tile
 constexpr int kDepth = 32;     // of a stage of a tile's operands in LDS
 constexpr int kStages = 4;     // in LDS: one that is multiplied, three on their way
-constexpr int kThreads = 256;  // 4 wavefronts of 128 x 128 outputs, one per SIMD
-constexpr int kLoads = 4;      // per wavefront, operand and stage: 1 KB each
+#ifndef WAVES
+#define WAVES 8
+#endif
+constexpr int kWaveCount = WAVES;            // wavefronts of 128 x kWaveCols outputs
+constexpr int kThreads = 64 * kWaveCount;
+constexpr int kWaveCols = 512 / kWaveCount;
+constexpr int kCols = kWaveCols / 32;        // 32 x 32 tiles of a wavefront across; 4 down
+constexpr int kLoads = 16 / kWaveCount;  // per wavefront, operand and stage: 1 KB each
 constexpr int kOperand = kTile * kDepth;  // elements of one operand's stage
 constexpr float kProbabilityScale = 16384.0f;
 
@@ -79,7 +85,7 @@ inline Saved saved_views(void* base, int64_t rows) {
 // columns (row k holds all of the operand's entries).  Both go to LDS as they lie, 16 bytes
 // per lane straight from memory; a column operand's fragments are transposed on the way
 // from LDS (ds_read_b64_tr_b16).  16-byte slots are permuted within an LDS row so that the lanes of
-// a fragment read meet every bank once: slot = chunk ^ (row / 2 % 4) for rows of k (64 bytes), chunk ^
+// a fragment read meet every bank once: slot = chunk ^ (row / 4 % 4) for rows of k (64 bytes), chunk ^
 // 4 (k % 4) for columns (512 bytes).
 
 struct Operand {
@@ -100,10 +106,8 @@ struct Product {
 template <bool ROWS>
 struct Loader {
   uint32_t offset[kLoads];  // bytes from the stage's origin; columns: of the chunk alone
-  uint32_t slot;            // LDS byte of this wavefront's first load
   int row;                  // columns: k of the first load
   __device__ __forceinline__ void init(const Operand& o, int64_t entry0, int wave, int lane) {
-    slot = static_cast<uint32_t>(wave) * (kLoads * 1024);
     row = wave * kLoads * 2 + lane / 32;
 #pragma unroll
     for (int j = 0; j < kLoads; ++j) {
@@ -111,7 +115,7 @@ struct Loader {
         const int r = (wave * kLoads + j) * 16 + lane / 4;
         const int64_t left = o.entries - 1 - entry0;
         const int64_t at = r < left ? r : left;
-        offset[j] = static_cast<uint32_t>((at * o.ld + ((lane % 4) ^ (lane / 8 % 4)) * 8) * 2);
+        offset[j] = static_cast<uint32_t>((at * o.ld + ((lane % 4) ^ (lane / 16)) * 8) * 2);
       } else {
         const int chunk = (lane % 32) ^ (((row + j * 2) & 3) << 2);
         const int64_t left = o.entries - 8 - entry0;
@@ -120,43 +124,62 @@ struct Loader {
       }
     }
   }
-  // The j-th 1-KB load of a stage into LDS byte `lds`; base: the stage's origin (scalar), left: k's
-  // of the stage that a column operand holds, less one.  Written out, since the compiler makes transposing LDS reads
-  // wait for every load into LDS that it knows of; what has to have landed is waited for in landed().
-  // The address registers are read when the load is issued, and nothing comes back in registers.
-  __device__ __forceinline__ void load(const Operand& o, const char* base, int left, uint32_t lds, int j) const {
-    uint32_t at = offset[j];
-    if constexpr (!ROWS) at += static_cast<uint32_t>(min(row + j * 2, left)) * static_cast<uint32_t>(o.ld * 2);
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
-                 :
-                 : "s"(lds + slot + j * 1024), "v"(at), "s"(base)
-                 : "m0");
+  // Offsets of a stage; left: k's of it that a column operand holds, less one.
+  __device__ __forceinline__ void offsets(const Operand& o, int left, uint32_t (&at)[kLoads]) const {
+#pragma unroll
+    for (int j = 0; j < kLoads; ++j) {
+      at[j] = offset[j];
+      if constexpr (!ROWS) at[j] += static_cast<uint32_t>(min(row + j * 2, left)) * static_cast<uint32_t>(o.ld * 2);
+    }
   }
 };
+
+// A 1-KB load into LDS byte `lds` from `base` (scalar) and `at` bytes on, 16 bytes per lane.  Written out,
+// since the compiler makes transposing LDS reads wait for every load into LDS that it knows of; what has to
+// have landed is waited for in landed().  The address registers are read when the load is issued, and
+// nothing comes back in registers.
+__device__ __forceinline__ void load_lds(const char* base, uint32_t at, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(lds), "v"(at), "s"(base));
+}
 
 // The LDS byte of a pointer into LDS.
 __device__ __forceinline__ uint32_t lds_byte(const uint16_t* p) {
   return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((const ATTNRES_LDS uint16_t*)p));
 }
 
-// Fragment r (32 entries) of the 16 k's at `step`: lane l holds entry l % 32, k = 8 (l / 32) + 0..7.
+// Fragments of 32 entries and 16 k's: lane l holds entry l % 32, k = 8 (l / 32) + 0..7.  The lane's
+// addresses of a stage are kept; the fragment's number and step are constants beside them.
 template <bool ROWS>
-__device__ __forceinline__ s16x8 fragment(const uint16_t* lds, int entry, int step, int lane) {
-  if constexpr (ROWS) {
-    const int row = entry + lane % 32;
-    const int slot = (step * 2 + lane / 32) ^ (lane / 2 % 4);
-    return *reinterpret_cast<const s16x8*>(lds + row * kDepth + slot * 8);
-  } else {
-    // 16 lanes read 4 k's of 16 entries and get one entry's 4 k's each
-    const int group = lane / 16, j = lane % 16;
-    const int column = entry + (group % 2) * 16 + (j % 4) * 4;
-    const int k = step * 16 + (group / 2) * 8 + j / 4;
-    const uint16_t* at = lds + k * kTile + ((column / 8) ^ ((j / 4) << 2)) * 8 + column % 8;
-    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((ATTNRES_LDS s16x4*)at);
-    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((ATTNRES_LDS s16x4*)(at + 4 * kTile));
-    return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+struct Reader {
+  uint32_t at[ROWS ? 2 : 4];
+  __device__ __forceinline__ void init(int entry, int lane) {
+    if constexpr (ROWS) {
+#pragma unroll
+      for (int step = 0; step < 2; ++step) {
+        at[step] = static_cast<uint32_t>((entry + lane % 32) * kDepth + ((step * 2 + lane / 32) ^ (lane / 4 % 4)) * 8) * 2;
+      }
+    } else {
+      // 16 lanes read 4 k's of 16 entries and get one entry's 4 k's each
+      const int group = lane / 16, j = lane % 16;
+      const int k = (group / 2) * 8 + j / 4;
+#pragma unroll
+      for (int f = 0; f < 4; ++f) {
+        const int column = entry + f * 32 + (group % 2) * 16 + (j % 4) * 4;
+        at[f] = static_cast<uint32_t>(k * kTile + ((column / 8) ^ ((j / 4) << 2)) * 8 + column % 8) * 2;
+      }
+    }
   }
-}
+  __device__ __forceinline__ s16x8 read(uint32_t stage, int f, int step) const {
+    if constexpr (ROWS) {
+      return *(ATTNRES_LDS const s16x8*)(stage + at[step] + f * 32 * kDepth * 2);
+    } else {
+      const uint32_t from = stage + at[f] + step * 16 * kTile * 2;
+      const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((ATTNRES_LDS s16x4*)(from));
+      const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((ATTNRES_LDS s16x4*)(from + 4 * kTile * 2));
+      return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+  }
+};
 
 template <class T>
 __device__ __forceinline__ f32x16 mfma(s16x8 a, s16x8 b, f32x16 c) {
@@ -190,7 +213,7 @@ __device__ __forceinline__ TileAt tile_at(const Product& p) {
   return {at / size, group * kGroup + at % size, split};
 }
 
-using Accumulators = f32x16[4][4];  // [32 entries of A][32 entries of B]; lane l, register i: entry
+using Accumulators = f32x16[4][kCols];  // [32 entries of A][32 entries of B]; lane l, register i: entry
                                     // 8 (i / 4) + 4 (l / 32) + i % 4 of A, l % 32 of B
 
 // A pointer that every lane holds, in scalar registers, and opaque from here on.
@@ -204,11 +227,10 @@ __device__ __forceinline__ const char* scalar(const char* p) {
 
 // This wavefront's reads from LDS are done and its loads of the next stage have landed, and so it is for every
 // wavefront (a barrier alone waits for neither).  Loads arrive in order: with `more`, those of
-// the two stages after the next one may still be on their way.
+// the stages after the next one may still be on their way.
 __device__ __forceinline__ void landed(bool more) {
-  static_assert(kStages == 4 && kLoads == 4, "two stages of eight loads");
   if (more) {
-    asm volatile("s_waitcnt vmcnt(16) lgkmcnt(0)" ::: "memory");
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"i"((kStages - 2) * 2 * kLoads) : "memory");
   } else {
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
   }
@@ -235,7 +257,7 @@ __device__ __forceinline__ void multiply(const Product& p, const TileAt& tile, c
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) acc[i][j] = f32x16{};
+    for (int j = 0; j < kCols; ++j) acc[i][j] = f32x16{};
   }
   const int first = range.first, stages = range.count;
   const int64_t a0 = static_cast<int64_t>(tile.a) * kTile, b0 = static_cast<int64_t>(tile.b) * kTile;
@@ -261,63 +283,80 @@ __device__ __forceinline__ void multiply(const Product& p, const TileAt& tile, c
   const auto loaded = [&] {
     if (++stage == stages) stage = 0, ++segment;
   };
-  const auto buffer = [&](int s) { return lds + (s % kStages) * 2 * kOperand; };
-  const int wa = (wave % 2) * 128, wb = (wave / 2) * 128;
-  using Fragments = s16x8[4];
-  // One step: 16 matrix instructions on (a, b), between them the reads of the next step's
-  // fragments, in the order of their use, and up to four loads.  In order, because a wavefront
-  // issues in order: a burst of reads or loads would keep the matrix core waiting.
-  const auto step = [&](const Fragments& a, const Fragments& b, Fragments& na, Fragments& nb, const uint16_t* from, int next,
+  const uint32_t lds0 = lds_byte(lds);
+  const auto buffer = [&](int s) { return lds0 + (s % kStages) * (2 * kOperand * 2); };
+  constexpr uint32_t kB = kOperand * 2;  // B's operand in a stage, bytes
+  const uint32_t slot = wave * (kLoads * 1024);
+  Reader<A_ROWS> read_a;
+  Reader<B_ROWS> read_b;
+  read_a.init((wave % 2) * 128, lane);
+  read_b.init((wave / 2) * kWaveCols, lane);
+  using FragmentsA = s16x8[4];
+  using FragmentsB = s16x8[kCols];
+  // One step: the matrix instructions on (a, b), between them the reads of the next step's fragments, in
+  // the order of their use, and the loads.  In order, because a wavefront issues in order, and with
+  // nothing else beside them: a matrix instruction takes 32 cycles, the time of some eight others.
+  const auto step = [&](const FragmentsA& a, const FragmentsB& b, FragmentsA& na, FragmentsB& nb, uint32_t from, auto next,
                         auto load) {
+    constexpr int kNext = decltype(next)::value;  // step of the reads; -1: none
+    constexpr int kMfma = 4 * kCols, kReads = 4 + kCols;
 #pragma unroll
-    for (int m = 0; m < 16; ++m) {
-      acc[m / 4][m % 4] = mfma<T>(a[m / 4], b[m % 4], acc[m / 4][m % 4]);
-      if (m % 2 == 0) {
-        constexpr int kOrder[8] = {0, 4, 5, 6, 7, 1, 2, 3};  // a: 0..3, b: 4..7
-        const int f = kOrder[m / 2];
-        if (f < 4) na[f] = fragment<A_ROWS>(from, wa + f * 32, next, lane);
-        else nb[f - 4] = fragment<B_ROWS>(from + kOperand, wb + (f - 4) * 32, next, lane);
+    for (int m = 0; m < kMfma; ++m) {
+      acc[m / kCols][m % kCols] = mfma<T>(a[m / kCols], b[m % kCols], acc[m / kCols][m % kCols]);
+      if constexpr (kNext >= 0) {
+#pragma unroll
+        for (int r = m * kReads / kMfma; r < (m + 1) * kReads / kMfma; ++r) {  // a0, all of b, the other a's
+          if (r == 0) na[0] = read_a.read(from, 0, kNext);
+          else if (r <= kCols) nb[r - 1] = read_b.read(from + kB, r - 1, kNext);
+          else na[r - kCols] = read_a.read(from, r - kCols, kNext);
+        }
       }
-      if (m % 4 == 3) load(m / 4);
-      if (m % 2 == 1) __builtin_amdgcn_sched_barrier(0);
+      if (m % 4 == 1) load(m / 4);
+      __builtin_amdgcn_sched_barrier(0);
     }
   };
+  using Step0 = std::integral_constant<int, 0>;
+  using Step1 = std::integral_constant<int, 1>;
+  const auto nothing = [](int) {};
   const int total = stages * SEGMENTS;
+  uint32_t at[kLoads];
   for (int s = 0; s < kStages && s < total; ++s) {
     const char *a = base_a(), *b = base_b();
-    const int left_a = left(p.a), left_b = left(p.b);
-    for (int j = 0; j < kLoads; ++j) load_a.load(p.a, a, left_a, lds_byte(buffer(s)), j);
-    for (int j = 0; j < kLoads; ++j) load_b.load(p.b, b, left_b, lds_byte(buffer(s) + kOperand), j);
+    load_a.offsets(p.a, left(p.a), at);
+    for (int j = 0; j < kLoads; ++j) load_lds(a, at[j], buffer(s) + slot + j * 1024);
+    load_b.offsets(p.b, left(p.b), at);
+    for (int j = 0; j < kLoads; ++j) load_lds(b, at[j], buffer(s) + kB + slot + j * 1024);
     loaded();
   }
   landed(total >= kStages);
-  Fragments a0f, b0f, a1f, b1f;
+  FragmentsA a0f, a1f;
+  FragmentsB b0f, b1f;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    a0f[i] = fragment<A_ROWS>(lds, wa + i * 32, 0, lane);
-    b0f[i] = fragment<B_ROWS>(lds + kOperand, wb + i * 32, 0, lane);
-  }
-  for (int s = 0; s < total; ++s) {
-    // B's half of the stage three ahead, whose A's half was loaded in the last trip.  The branches hold the
-    // loads alone: no accumulator meets another path.
-    const bool late = s > 0 && s + kStages - 1 < total;
-    const char* b = base_b();
-    const int left_b = left(p.b);
-    const uint32_t to_b = lds_byte(buffer(s + kStages - 1) + kOperand);
-    step(a0f, b0f, a1f, b1f, buffer(s), 1, [&](int j) {
-      if (late) load_b.load(p.b, b, left_b, to_b, j);
-    });
-    if (late) loaded();
-    // both steps' fragments of this stage are in registers: its buffer is free; the next stage has landed
-    landed(s + kStages - 1 < total);
-    const bool early = s + kStages < total;
+  for (int i = 0; i < 4; ++i) a0f[i] = read_a.read(lds0, i, 0);
+#pragma unroll
+  for (int j = 0; j < kCols; ++j) b0f[j] = read_b.read(lds0 + kB, j, 0);
+  // A stage's second step and the next one's first make a trip.  Loads go to the buffer whose stage is
+  // finished but for fragments in registers: every wavefront has passed landed() since it read them.
+  step(a0f, b0f, a1f, b1f, lds0, Step1{}, nothing);
+  landed(total >= kStages);
+  int s = 1;
+  for (; s + kStages - 1 < total; ++s) {
+    const uint32_t to = buffer(s + kStages - 1) + slot;
     const char* a = base_a();
-    const int left_a = left(p.a);
-    const uint32_t to_a = lds_byte(buffer(s));
-    step(a1f, b1f, a0f, b0f, buffer(s + 1), 0, [&](int j) {
-      if (early) load_a.load(p.a, a, left_a, to_a, j);
-    });
+    load_a.offsets(p.a, left(p.a), at);
+    step(a1f, b1f, a0f, b0f, buffer(s), Step0{}, [&](int j) { load_lds(a, at[j], to + j * 1024); });
+    const char* b = base_b();
+    load_b.offsets(p.b, left(p.b), at);
+    step(a0f, b0f, a1f, b1f, buffer(s), Step1{}, [&](int j) { load_lds(b, at[j], to + kB + j * 1024); });
+    loaded();
+    landed(true);
   }
+  for (; s < total; ++s) {  // the last stages: nothing more to load
+    step(a1f, b1f, a0f, b0f, buffer(s), Step0{}, nothing);
+    step(a0f, b0f, a1f, b1f, buffer(s), Step1{}, nothing);
+    landed(false);
+  }
+  step(a1f, b1f, a0f, b0f, lds0, std::integral_constant<int, -1>{}, nothing);
   __syncthreads();  // LDS is free for the epilogue
 }
 
@@ -381,8 +420,8 @@ __global__ void __launch_bounds__(kThreads) attnres_loss_logits_kernel(LogitArgs
     constexpr bool ENDS = decltype(ends)::value;
     const int last = limit - 4 * (lane / 32);  // entries below it count
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int column = (wave / 2) * 128 + j * 32 + lane % 32;
+    for (int j = 0; j < kCols; ++j) {
+      const int column = (wave / 2) * kWaveCols + j * 32 + lane % 32;
       const int row = tile.b * kTile + column;
       const int64_t from_v0 = g.target[min(row, count - 1)] - v0;
       const int rel = row < count && from_v0 >= 0 && from_v0 < 128 ? static_cast<int>(from_v0) : -1;
@@ -426,7 +465,7 @@ __global__ void __launch_bounds__(kThreads) attnres_loss_logits_kernel(LogitArgs
     reduce(std::false_type{});
   }
   __syncthreads();
-  if (threadIdx.x < kTile) {  // every thread a row
+  if (threadIdx.x < kTile) {
     g.sums[static_cast<int64_t>(tile.a) * g.row_tiles + tile.b * kTile + threadIdx.x] =
         join(meet[threadIdx.x], meet[kTile + threadIdx.x]);
   }
@@ -456,8 +495,8 @@ __global__ void __launch_bounds__(kThreads) attnres_loss_probability_kernel(Logi
     constexpr bool ENDS = decltype(ends)::value;
     const int last = limit - 4 * (lane / 32);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int column = (wave / 2) * 128 + j * 32 + lane % 32;
+    for (int j = 0; j < kCols; ++j) {
+      const int column = (wave / 2) * kWaveCols + j * 32 + lane % 32;
       const int row = tile.b * kTile + column;
       const int at = min(row, count - 1);
       const int64_t from_v0 = g.target[at] - v0;
@@ -495,7 +534,7 @@ __global__ void __launch_bounds__(kThreads) attnres_loss_probability_kernel(Logi
     }
   };
   for (int base = 0; base < kTile; base += kColumns) {
-    if (kParts == 1 || wave / 2 == base / kColumns) {
+    if (kParts == 1 || (wave / 2) * kWaveCols / kColumns == base / kColumns) {
       if (limit < 128) {
         stage(std::true_type{}, base);
       } else {
@@ -561,8 +600,8 @@ __global__ void __launch_bounds__(kThreads) attnres_loss_gradient_kernel(Gradien
   for (int round = 0; round < kRounds; ++round) {
     if (!kWide || wave % 2 == round) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int column = (wave / 2) * 128 + j * 32 + lane % 32;
+      for (int j = 0; j < kCols; ++j) {
+        const int column = (wave / 2) * kWaveCols + j * 32 + lane % 32;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
 #pragma unroll
