@@ -30,20 +30,16 @@ namespace layers {
 namespace {
 
 constexpr int kTile = 256;     // rows and columns of a workgroup's tile
+constexpr int kWaves = 8;      // of 128 x 64 outputs, two per SIMD
+constexpr int kThreads = 64 * kWaves;
+constexpr int kDown = 8;       // 16 x 16 tiles of a wavefront: down (A) and across (B)
+constexpr int kAcross = 4;
 constexpr int kDepth = 32;     // of a stage of a tile's operands in LDS
 constexpr int kStages = 4;     // in LDS: one that is multiplied, three on their way
-#ifndef WAVES
-#define WAVES 8
-#endif
-constexpr int kWaveCount = WAVES;            // wavefronts of 128 x kWaveCols outputs
-constexpr int kThreads = 64 * kWaveCount;
-constexpr int kWaveCols = 512 / kWaveCount;
-constexpr int kCols = kWaveCols / 32;        // 32 x 32 tiles of a wavefront across; 4 down
-constexpr int kLoads = 16 / kWaveCount;  // per wavefront, operand and stage: 1 KB each
+constexpr int kLoads = 2;      // per wavefront, operand and stage: 1 KB each
 constexpr int kOperand = kTile * kDepth;  // elements of one operand's stage
 constexpr float kProbabilityScale = 16384.0f;
 
-typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
@@ -84,9 +80,11 @@ inline Saved saved_views(void* base, int64_t rows) {
 // one of the output.  An operand lies either as rows of k (ROWS: the row is contiguous in k) or as
 // columns (row k holds all of the operand's entries).  Both go to LDS as they lie, 16 bytes
 // per lane straight from memory; a column operand's fragments are transposed on the way
-// from LDS (ds_read_b64_tr_b16).  16-byte slots are permuted within an LDS row so that the lanes of
-// a fragment read meet every bank once: slot = chunk ^ (row / 4 % 4) for rows of k (64 bytes), chunk ^
-// 4 (k % 4) for columns (512 bytes).
+// from LDS (ds_read_b64_tr_b16).  16-byte slots are permuted within an LDS row so that the lanes which
+// LDS serves together meet every bank once: slot = chunk ^ (-(row / 4) % 4) for rows of k (64 bytes; lanes 0-3,
+// 12-15, 20-23 and 24-27 go together), chunk ^ (4 (k % 4) + 2 (k / 8 % 2)) for columns (512 bytes).
+// 16 x 16 x 32 matrix instructions: the chip is limited by power here (1.7 of 2.4 GHz), and on registers alone
+// these reach 2.2 PFLOP/s, 32 x 32 x 16 ones 2.0.
 
 struct Operand {
   const uint16_t* part[2];  // hi, lo
@@ -103,6 +101,9 @@ struct Product {
   int tiles_a, tiles_b, splits;
 };
 
+__device__ __forceinline__ int row_swizzle(int row) { return -(row >> 2) & 3; }
+__device__ __forceinline__ int column_swizzle(int k) { return (k & 3) << 2 | (k >> 3 & 1) << 1; }
+
 template <bool ROWS>
 struct Loader {
   uint32_t offset[kLoads];  // bytes from the stage's origin; columns: of the chunk alone
@@ -115,9 +116,9 @@ struct Loader {
         const int r = (wave * kLoads + j) * 16 + lane / 4;
         const int64_t left = o.entries - 1 - entry0;
         const int64_t at = r < left ? r : left;
-        offset[j] = static_cast<uint32_t>((at * o.ld + ((lane % 4) ^ (lane / 16)) * 8) * 2);
+        offset[j] = static_cast<uint32_t>((at * o.ld + ((lane % 4) ^ row_swizzle(r)) * 8) * 2);
       } else {
-        const int chunk = (lane % 32) ^ (((row + j * 2) & 3) << 2);
+        const int chunk = (lane % 32) ^ column_swizzle(row + j * 2);
         const int64_t left = o.entries - 8 - entry0;
         const int64_t at = chunk * 8 < left ? chunk * 8 : left;
         offset[j] = static_cast<uint32_t>(at * 2);
@@ -147,33 +148,29 @@ __device__ __forceinline__ uint32_t lds_byte(const uint16_t* p) {
   return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((const ATTNRES_LDS uint16_t*)p));
 }
 
-// Fragments of 32 entries and 16 k's: lane l holds entry l % 32, k = 8 (l / 32) + 0..7.  The lane's
-// addresses of a stage are kept; the fragment's number and step are constants beside them.
+// Fragments of 16 entries and a stage's 32 k's: lane l holds entry l % 16, k = 8 (l / 16) + 0..7.
 template <bool ROWS>
 struct Reader {
-  uint32_t at[ROWS ? 2 : 4];
+  uint32_t at;      // the lane's byte of a stage; columns: of its row of k
+  uint32_t column;  // columns: the lane's byte in that row, before the fragment's number is permuted in
   __device__ __forceinline__ void init(int entry, int lane) {
+    const int group = lane / 16, j = lane % 16;
     if constexpr (ROWS) {
-#pragma unroll
-      for (int step = 0; step < 2; ++step) {
-        at[step] = static_cast<uint32_t>((entry + lane % 32) * kDepth + ((step * 2 + lane / 32) ^ (lane / 4 % 4)) * 8) * 2;
-      }
+      at = static_cast<uint32_t>((entry + j) * kDepth + (group ^ row_swizzle(j)) * 8) * 2;
+      column = 0;
     } else {
       // 16 lanes read 4 k's of 16 entries and get one entry's 4 k's each
-      const int group = lane / 16, j = lane % 16;
-      const int k = (group / 2) * 8 + j / 4;
-#pragma unroll
-      for (int f = 0; f < 4; ++f) {
-        const int column = entry + f * 32 + (group % 2) * 16 + (j % 4) * 4;
-        at[f] = static_cast<uint32_t>(k * kTile + ((column / 8) ^ ((j / 4) << 2)) * 8 + column % 8) * 2;
-      }
+      const int k = group * 8 + j / 4;
+      const int chunk = entry / 8 + j % 4 / 2;  // the fragment's number is a part of its low four bits
+      at = static_cast<uint32_t>(k * kTile + chunk / 16 * 128) * 2;
+      column = static_cast<uint32_t>((chunk % 16 ^ column_swizzle(k)) * 8 + j % 2 * 4) * 2;
     }
   }
-  __device__ __forceinline__ s16x8 read(uint32_t stage, int f, int step) const {
+  __device__ __forceinline__ s16x8 read(uint32_t stage, int f) const {
     if constexpr (ROWS) {
-      return *(ATTNRES_LDS const s16x8*)(stage + at[step] + f * 32 * kDepth * 2);
+      return *(ATTNRES_LDS const s16x8*)(stage + at + f * 16 * kDepth * 2);
     } else {
-      const uint32_t from = stage + at[f] + step * 16 * kTile * 2;
+      const uint32_t from = stage + at + (column ^ (f * 32u));
       const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((ATTNRES_LDS s16x4*)(from));
       const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((ATTNRES_LDS s16x4*)(from + 4 * kTile * 2));
       return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
@@ -182,11 +179,11 @@ struct Reader {
 };
 
 template <class T>
-__device__ __forceinline__ f32x16 mfma(s16x8 a, s16x8 b, f32x16 c) {
+__device__ __forceinline__ f32x4 mfma(s16x8 a, s16x8 b, f32x4 c) {
   if constexpr (std::is_same_v<T, Bf16>) {
-    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
   } else {
-    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
   }
 }
 
@@ -213,8 +210,8 @@ __device__ __forceinline__ TileAt tile_at(const Product& p) {
   return {at / size, group * kGroup + at % size, split};
 }
 
-using Accumulators = f32x16[4][kCols];  // [32 entries of A][32 entries of B]; lane l, register i: entry
-                                    // 8 (i / 4) + 4 (l / 32) + i % 4 of A, l % 32 of B
+// [16 entries of A][16 entries of B]; lane l, register e: entry 4 (l / 16) + e of A, l % 16 of B.
+using Accumulators = f32x4[kDown][kAcross];
 
 // A pointer that every lane holds, in scalar registers, and opaque from here on.
 __device__ __forceinline__ const char* scalar(const char* p) {
@@ -255,9 +252,9 @@ template <class T, int SEGMENTS, bool A_ROWS, bool B_ROWS>
 __device__ __forceinline__ void multiply(const Product& p, const TileAt& tile, const Stages& range, uint16_t* lds, Accumulators& acc) {
   const int wave = wave_index(), lane = threadIdx.x % 64;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < kDown; ++i) {
 #pragma unroll
-    for (int j = 0; j < kCols; ++j) acc[i][j] = f32x16{};
+    for (int j = 0; j < kAcross; ++j) acc[i][j] = f32x4{};
   }
   const int first = range.first, stages = range.count;
   const int64_t a0 = static_cast<int64_t>(tile.a) * kTile, b0 = static_cast<int64_t>(tile.b) * kTile;
@@ -290,33 +287,40 @@ __device__ __forceinline__ void multiply(const Product& p, const TileAt& tile, c
   Reader<A_ROWS> read_a;
   Reader<B_ROWS> read_b;
   read_a.init((wave % 2) * 128, lane);
-  read_b.init((wave / 2) * kWaveCols, lane);
-  using FragmentsA = s16x8[4];
-  using FragmentsB = s16x8[kCols];
-  // One step: the matrix instructions on (a, b), between them the reads of the next step's fragments, in
-  // the order of their use, and the loads.  In order, because a wavefront issues in order, and with
-  // nothing else beside them: a matrix instruction takes 32 cycles, the time of some eight others.
-  const auto step = [&](const FragmentsA& a, const FragmentsB& b, FragmentsA& na, FragmentsB& nb, uint32_t from, auto next,
-                        auto load) {
-    constexpr int kNext = decltype(next)::value;  // step of the reads; -1: none
-    constexpr int kMfma = 4 * kCols, kReads = 4 + kCols;
+  read_b.init((wave / 2) * (16 * kAcross), lane);
+  // A stage in two steps, the upper and the lower half of A's fragments, with all of B's.
+  constexpr int kHalf = kDown / 2;
+  using FragmentsA = s16x8[kHalf];
+  using FragmentsB = s16x8[kAcross];
+  // One step: the matrix instructions on (a, b), between them the reads of the next step's fragments, in the
+  // order of their use, and the loads.
+  const auto step = [&](auto lower, const FragmentsA& a, const FragmentsB& b, auto read, auto load) {
+    constexpr int kFirst = decltype(lower)::value ? kHalf : 0;
 #pragma unroll
-    for (int m = 0; m < kMfma; ++m) {
-      acc[m / kCols][m % kCols] = mfma<T>(a[m / kCols], b[m % kCols], acc[m / kCols][m % kCols]);
-      if constexpr (kNext >= 0) {
-#pragma unroll
-        for (int r = m * kReads / kMfma; r < (m + 1) * kReads / kMfma; ++r) {  // a0, all of b, the other a's
-          if (r == 0) na[0] = read_a.read(from, 0, kNext);
-          else if (r <= kCols) nb[r - 1] = read_b.read(from + kB, r - 1, kNext);
-          else na[r - kCols] = read_a.read(from, r - kCols, kNext);
-        }
-      }
-      if (m % 4 == 1) load(m / 4);
+    for (int m = 0; m < kHalf * kAcross; ++m) {
+      f32x4& c = acc[kFirst + m / kAcross][m % kAcross];
+      c = mfma<T>(a[m / kAcross], b[m % kAcross], c);
+      if (m % 2 == 0) read(m / 2);
+      if (m % 8 == 1) load(m / 8);
       __builtin_amdgcn_sched_barrier(0);
     }
   };
-  using Step0 = std::integral_constant<int, 0>;
-  using Step1 = std::integral_constant<int, 1>;
+  FragmentsA upper, lower;
+  FragmentsB b_even, b_odd;  // of even and odd stages
+  // Reads of a step, eight at most: the lower half of the stage, or the next stage's upper half and B.
+  const auto read_lower = [&](uint32_t from) {
+    return [&, from](int r) {
+      if (r < kHalf) lower[r] = read_a.read(from, kHalf + r);
+    };
+  };
+  const auto read_next = [&](uint32_t from, FragmentsB& b) {
+    return [&, from](int r) {
+      if (r == 0) upper[0] = read_a.read(from, 0);
+      else if (r <= kAcross) b[r - 1] = read_b.read(from + kB, r - 1);
+      else upper[r - kAcross] = read_a.read(from, r - kAcross);
+    };
+  };
+  static_assert(kHalf + kAcross == 8 && kHalf * kAcross == 16, "eight reads, one per two matrix instructions");
   const auto nothing = [](int) {};
   const int total = stages * SEGMENTS;
   uint32_t at[kLoads];
@@ -329,34 +333,51 @@ __device__ __forceinline__ void multiply(const Product& p, const TileAt& tile, c
     loaded();
   }
   landed(total >= kStages);
-  FragmentsA a0f, a1f;
-  FragmentsB b0f, b1f;
+  const auto read_first = read_next(lds0, b_even);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) a0f[i] = read_a.read(lds0, i, 0);
-#pragma unroll
-  for (int j = 0; j < kCols; ++j) b0f[j] = read_b.read(lds0 + kB, j, 0);
-  // A stage's second step and the next one's first make a trip.  Loads go to the buffer whose stage is
-  // finished but for fragments in registers: every wavefront has passed landed() since it read them.
-  step(a0f, b0f, a1f, b1f, lds0, Step1{}, nothing);
+  for (int r = 0; r < 8; ++r) read_first(r);
+  step(std::false_type{}, upper, b_even, read_lower(lds0), nothing);
   landed(total >= kStages);
+  // A stage's lower step and the next one's upper step make a trip.  Loads go to the buffer whose stage is
+  // finished but for fragments in registers: every wavefront has passed landed() since it read them.
   int s = 1;
-  for (; s + kStages - 1 < total; ++s) {
+  const auto trip = [&](FragmentsB& now, FragmentsB& next) {
     const uint32_t to = buffer(s + kStages - 1) + slot;
     const char* a = base_a();
     load_a.offsets(p.a, left(p.a), at);
-    step(a1f, b1f, a0f, b0f, buffer(s), Step0{}, [&](int j) { load_lds(a, at[j], to + j * 1024); });
+    step(std::true_type{}, lower, now, read_next(buffer(s), next), [&](int j) { load_lds(a, at[j], to + j * 1024); });
     const char* b = base_b();
     load_b.offsets(p.b, left(p.b), at);
-    step(a0f, b0f, a1f, b1f, buffer(s), Step1{}, [&](int j) { load_lds(b, at[j], to + kB + j * 1024); });
+    step(std::false_type{}, upper, next, read_lower(buffer(s)), [&](int j) { load_lds(b, at[j], to + kB + j * 1024); });
     loaded();
     landed(true);
-  }
-  for (; s < total; ++s) {  // the last stages: nothing more to load
-    step(a1f, b1f, a0f, b0f, buffer(s), Step0{}, nothing);
-    step(a0f, b0f, a1f, b1f, buffer(s), Step1{}, nothing);
+    ++s;
+  };
+  const auto last_trip = [&](FragmentsB& now, FragmentsB& next) {  // nothing more to load
+    step(std::true_type{}, lower, now, read_next(buffer(s), next), nothing);
+    step(std::false_type{}, upper, next, read_lower(buffer(s)), nothing);
     landed(false);
+    ++s;
+  };
+  while (s + kStages < total) {
+    trip(b_even, b_odd);
+    trip(b_odd, b_even);
   }
-  step(a1f, b1f, a0f, b0f, lds0, std::integral_constant<int, -1>{}, nothing);
+  // fewer than two trips with loads are left, then those without; after an odd number B's fragments change
+  // their registers
+  const auto swap = [&] {
+#pragma unroll
+    for (int j = 0; j < kAcross; ++j) b_even[j] = b_odd[j];
+  };
+  if (s + kStages - 1 < total) {
+    trip(b_even, b_odd);
+    swap();
+  }
+  while (s < total) {
+    last_trip(b_even, b_odd);
+    swap();
+  }
+  step(std::true_type{}, lower, b_even, nothing, nothing);
   __syncthreads();  // LDS is free for the epilogue
 }
 
@@ -418,44 +439,43 @@ __global__ void __launch_bounds__(kThreads) attnres_loss_logits_kernel(LogitArgs
   // ENDS: the vocabulary ends in this half of the tile
   const auto reduce = [&](auto ends) {
     constexpr bool ENDS = decltype(ends)::value;
-    const int last = limit - 4 * (lane / 32);  // entries below it count
+    const int last = limit - 4 * (lane / 16);  // entries below it count
 #pragma unroll
-    for (int j = 0; j < kCols; ++j) {
-      const int column = (wave / 2) * kWaveCols + j * 32 + lane % 32;
+    for (int j = 0; j < kAcross; ++j) {
+      const int column = (wave / 2) * (16 * kAcross) + j * 16 + lane % 16;
       const int row = tile.b * kTile + column;
       const int64_t from_v0 = g.target[min(row, count - 1)] - v0;
       const int rel = row < count && from_v0 >= 0 && from_v0 < 128 ? static_cast<int>(from_v0) : -1;
       float top = -__builtin_inff();
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
+      for (int i = 0; i < kDown; ++i) {
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const float x = acc[i][j][e];
-          top = fmaxf(top, !ENDS || i * 32 + 8 * (e / 4) + e % 4 < last ? x : -__builtin_inff());
-        }
+        for (int e = 0; e < 4; ++e) top = fmaxf(top, !ENDS || i * 16 + e < last ? acc[i][j][e] : -__builtin_inff());
       }
+      top = fmaxf(top, __shfl_xor(top, 16, 64));
       top = unscale(fmaxf(top, __shfl_xor(top, 32, 64)));
       if (__any(rel >= 0)) {
         float own = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < kDown; ++i) {
 #pragma unroll
-          for (int e = 0; e < 16; ++e) own = i * 32 + 8 * (e / 4) + e % 4 == rel - 4 * (lane / 32) ? acc[i][j][e] : own;
+          for (int e = 0; e < 4; ++e) own = i * 16 + e == rel - 4 * (lane / 16) ? acc[i][j][e] : own;
         }
-        if (rel >= 0 && (rel >> 2 & 1) == lane / 32) g.target_logit[row] = unscale(own);
+        if (rel >= 0 && (rel >> 2 & 3) == lane / 16) g.target_logit[row] = unscale(own);
       }
       const float from = top == -__builtin_inff() ? 0.0f : top;  // nothing but NaN, or nothing at all
       float sum = 0.0f;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
+      for (int i = 0; i < kDown; ++i) {
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
+        for (int e = 0; e < 4; ++e) {
           const float x = __expf(unscale(acc[i][j][e]) - from);
-          sum += !ENDS || i * 32 + 8 * (e / 4) + e % 4 < last ? x : 0.0f;
+          sum += !ENDS || i * 16 + e < last ? x : 0.0f;
         }
       }
+      sum += __shfl_xor(sum, 16, 64);
       sum += __shfl_xor(sum, 32, 64);
-      if (lane < 32) meet[(wave % 2) * kTile + column] = f32x2{top, sum};
+      if (lane < 16) meet[(wave % 2) * kTile + column] = f32x2{top, sum};
       __builtin_amdgcn_sched_barrier(0);  // one column's outputs at a time: no registers to spill
     }
   };
@@ -489,52 +509,49 @@ __global__ void __launch_bounds__(kThreads) attnres_loss_probability_kernel(Logi
   const int64_t v0 = g.first + static_cast<int64_t>(tile.a) * kTile + (wave % 2) * 128;
   const int limit = __builtin_amdgcn_readfirstlane(static_cast<int>(g.vocab - v0 < 128 ? g.vocab - v0 : 128));
   constexpr int kParts = SEGMENTS == 3 ? 2 : 1;
-  // With two parts, the columns of two wavefronts at a time: hi and lo of 128 rows are staged together.
+  // With two parts, the columns of four wavefronts at a time: hi and lo of 128 rows are staged together.
   constexpr int kColumns = kTile / kParts;
   const auto stage = [&](auto ends, int base) {
     constexpr bool ENDS = decltype(ends)::value;
-    const int last = limit - 4 * (lane / 32);
+    const int last = limit - 4 * (lane / 16);
 #pragma unroll
-    for (int j = 0; j < kCols; ++j) {
-      const int column = (wave / 2) * kWaveCols + j * 32 + lane % 32;
+    for (int j = 0; j < kAcross; ++j) {
+      const int column = (wave / 2) * (16 * kAcross) + j * 16 + lane % 16;
       const int row = tile.b * kTile + column;
       const int at = min(row, count - 1);
       const int64_t from_v0 = g.target[at] - v0;
-      const int rel = from_v0 >= 0 && from_v0 < 128 ? static_cast<int>(from_v0) - 4 * (lane / 32) : -128;
+      const int rel = from_v0 >= 0 && from_v0 < 128 ? static_cast<int>(from_v0) - 4 * (lane / 16) : -128;
       // a row past the last one has zeros in H, so logits of 0, and a factor of 0
       const f32x2 stats = {row < count ? g.stats[at].x : 0.0f, g.stats[at].y};
       const float by = g.row_scale[row];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
+      for (int i = 0; i < kDown; ++i) {
+        float x[4];
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          float x[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            x[e] = __expf(unscale(acc[i][j][4 * q + e]) - stats.x) * stats.y;
-            if (i * 32 + 8 * q + e == rel) x[e] -= 1.0f;
-            x[e] *= by;
-            if (ENDS && i * 32 + 8 * q + e >= last) x[e] = 0.0f;
-            // the FP32 value itself: hi has to be the same number where it is stored and where lo
-            // is what it leaves, and a product folded into one of the conversions rounds apart
-            if (kParts == 2) asm("" : "+v"(x[e]));
-          }
-          const int chunk = (wave % 2) * 16 + i * 4 + q;
-          uint16_t* to = lds + staged(column - base, chunk) * 8 + (lane / 32) * 4;
-#pragma unroll
-          for (int part = 0; part < kParts; ++part) {
-            const uint32_t packed[2] = {pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3])};
-            *reinterpret_cast<uint64_t*>(to + part * kColumns * kTile) = static_cast<uint64_t>(packed[1]) << 32 | packed[0];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) x[e] -= to_f32(T{static_cast<uint16_t>(packed[e / 2] >> (16 * (e % 2)))});  // lo
-          }
+        for (int e = 0; e < 4; ++e) {
+          x[e] = __expf(unscale(acc[i][j][e]) - stats.x) * stats.y;
+          if (i * 16 + e == rel) x[e] -= 1.0f;
+          x[e] *= by;
+          if (ENDS && i * 16 + e >= last) x[e] = 0.0f;
+          // the FP32 value itself: hi has to be the same number where it is stored and where lo
+          // is what it leaves, and a product folded into one of the conversions rounds apart
+          if (kParts == 2) asm("" : "+v"(x[e]));
         }
-        __builtin_amdgcn_sched_barrier(0);  // 16 outputs at a time: no registers to spill
+        const int chunk = (wave % 2) * 16 + i * 2 + lane / 32;
+        uint16_t* to = lds + staged(column - base, chunk) * 8 + (lane / 16 % 2) * 4;
+#pragma unroll
+        for (int part = 0; part < kParts; ++part) {
+          const uint32_t packed[2] = {pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3])};
+          *reinterpret_cast<uint64_t*>(to + part * kColumns * kTile) = static_cast<uint64_t>(packed[1]) << 32 | packed[0];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[e] -= to_f32(T{static_cast<uint16_t>(packed[e / 2] >> (16 * (e % 2)))});  // lo
+        }
+        if (i % 2 == 1) __builtin_amdgcn_sched_barrier(0);  // a few outputs at a time: no registers to spill
       }
     }
   };
   for (int base = 0; base < kTile; base += kColumns) {
-    if (kParts == 1 || (wave / 2) * kWaveCols / kColumns == base / kColumns) {
+    if (kParts == 1 || (wave / 2) * (16 * kAcross) / kColumns == base / kColumns) {
       if (limit < 128) {
         stage(std::true_type{}, base);
       } else {
@@ -600,25 +617,19 @@ __global__ void __launch_bounds__(kThreads) attnres_loss_gradient_kernel(Gradien
   for (int round = 0; round < kRounds; ++round) {
     if (!kWide || wave % 2 == round) {
 #pragma unroll
-      for (int j = 0; j < kCols; ++j) {
-        const int column = (wave / 2) * kWaveCols + j * 32 + lane % 32;
+      for (int j = 0; j < kAcross; ++j) {
+        const int column = (wave / 2) * (16 * kAcross) + j * 16 + lane % 16;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            float x[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) x[e] = acc[i][j][4 * q + e] * by * unscale;
-            if constexpr (kWide) {
-              const int chunk = i * 8 + q * 2 + lane / 32;
-              *reinterpret_cast<f32x4*>(lds + staged(column, chunk) * 8) = f32x4{x[0], x[1], x[2], x[3]};
-            } else {
-              const int chunk = (wave % 2) * 16 + i * 4 + q;
-              *reinterpret_cast<uint64_t*>(lds + staged(column, chunk) * 8 + (lane / 32) * 4) =
-                  static_cast<uint64_t>(pack2<OUT>(x[2], x[3])) << 32 | pack2<OUT>(x[0], x[1]);
-            }
+        for (int i = 0; i < kDown; ++i) {
+          const f32x4 x = acc[i][j] * by * unscale;
+          if constexpr (kWide) {
+            *reinterpret_cast<f32x4*>(lds + staged(column, i * 4 + lane / 16) * 8) = x;
+          } else {
+            const int chunk = (wave % 2) * 16 + i * 2 + lane / 32;
+            *reinterpret_cast<uint64_t*>(lds + staged(column, chunk) * 8 + (lane / 16 % 2) * 4) =
+                static_cast<uint64_t>(pack2<OUT>(x[2], x[3])) << 32 | pack2<OUT>(x[0], x[1]);
           }
-          __builtin_amdgcn_sched_barrier(0);  // 16 outputs at a time: no registers to spill
+          if (i % 2 == 1) __builtin_amdgcn_sched_barrier(0);  // a few outputs at a time: no registers to spill
         }
       }
     }
