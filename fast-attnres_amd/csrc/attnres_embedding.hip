@@ -85,27 +85,29 @@ __device__ __forceinline__ uint32_t sort_key(const SortPass& p, int64_t i) {
   return static_cast<uint32_t>(token >= 0 && token < p.vocab ? token : p.vocab);
 }
 
+// Elements first .. end-1 of the table's gradient, to clear.
 template <class W>
 struct ZeroFill {
   W* to;
-  int64_t elements;
+  int64_t first, end;
+  bool past;  // the caches
 };
 
 template <class W>
 __device__ __forceinline__ void zero_fill(const ZeroFill<W>& z, int64_t block, int64_t blocks) {
   float zero[kVec] = {};
-  const int64_t step = blocks * kBlock * kVec;
-  for (int64_t i = (block * kBlock + threadIdx.x) * kVec; i < z.elements; i += step) {
-    if (i + kVec <= z.elements) {
-      store8(z.to + i, zero);
+  const int64_t step = blocks * blockDim.x * kVec;
+  for (int64_t i = z.first + (block * blockDim.x + threadIdx.x) * kVec; i < z.end; i += step) {
+    if (i + kVec <= z.end) {
+      store8(z.to + i, zero, z.past);
     } else {
-      for (int64_t e = i; e < z.elements; ++e) z.to[e] = from_f32<W>(0.0f);
+      for (int64_t e = i; e < z.end; ++e) z.to[e] = from_f32<W>(0.0f);
     }
   }
 }
 
-// Blocks 0 .. tiles-1 count their tile's digits; in the first pass the others
-// clear the table's gradient meanwhile.
+// Blocks 0 .. tiles-1 count their tile's digits, or place its entries; the others clear a part of the
+// table's gradient meanwhile.
 template <class W>
 __global__ void __launch_bounds__(kBlock) attnres_sort_count_kernel(SortPass p, ZeroFill<W> zero) {
   const int tile = blockIdx.x;
@@ -122,7 +124,9 @@ __global__ void __launch_bounds__(kBlock) attnres_sort_count_kernel(SortPass p, 
   for (int d = threadIdx.x; d < digits; d += kBlock) p.counts[static_cast<int64_t>(tile) * digits + d] = count[d];
 }
 
-__global__ void __launch_bounds__(kBlock) attnres_sort_place_kernel(SortPass p) {
+template <class W>
+__global__ void __launch_bounds__(kBlock) attnres_sort_place_kernel(SortPass p, ZeroFill<W> zero) {
+  if (static_cast<int>(blockIdx.x) >= p.tiles) return zero_fill(zero, blockIdx.x - p.tiles, gridDim.x - p.tiles);
   __shared__ uint32_t place[kWaves][kMaxDigits];  // next place of the wavefront's entries of a digit
   __shared__ uint32_t block_sums[kWaves];
   const int tile = blockIdx.x, wave = threadIdx.x / 64, lane = threadIdx.x % 64;
@@ -212,6 +216,98 @@ __global__ void __launch_bounds__(kBlock) attnres_sort_place_kernel(SortPass p) 
   }
 }
 
+// Up to kSmall tokens: one workgroup sorts them, pass after pass, and the others clear the table's gradient
+// meanwhile: one launch for all of it (2048 tokens of a 32768 x 1024 FP32 table: 26 us, the time of its 134 MB; four
+// launches 46).  Its 16 wavefronts take a sixteenth of the list each; between the passes the list lies in
+// memory, which a barrier of the workgroup orders.  It sorts 1024 tokens in about 5.5 us.
+constexpr int kSmall = 4096;
+constexpr int kSmallBlock = 1024;
+constexpr int kSmallWaves = kSmallBlock / 64;
+
+__device__ __forceinline__ void sort_pass_small(const SortPass& p, uint32_t (*place)[kMaxDigits], uint32_t* block_sums) {
+  const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
+  const int digits = 1 << p.bits, mask = digits - 1;
+  for (int d = threadIdx.x; d < digits * kSmallWaves; d += kSmallBlock) place[d / digits][d % digits] = 0;
+  __syncthreads();
+  const int n = static_cast<int>(p.n);
+  const int share = (n + kSmallBlock - 1) / kSmallBlock * 64;
+  const int first = wave * share, end = min(first + share, n);
+#pragma unroll 4
+  for (int i = first + lane; i < end; i += 64) atomicAdd(&place[wave][sort_key(p, i) >> p.shift & mask], 1u);
+  __syncthreads();
+  const int d = threadIdx.x;  // at most as many digits as threads
+  uint32_t mine = 0;
+  if (d < digits) {
+    for (int w = 0; w < kSmallWaves; ++w) mine += place[w][d];
+  }
+  uint32_t scan = mine;
+#pragma unroll
+  for (int step = 1; step < 64; step <<= 1) {
+    const uint32_t other = __shfl_up(scan, step, 64);
+    scan += lane >= step ? other : 0;
+  }
+  if (lane == 63) block_sums[wave] = scan;
+  __syncthreads();
+  if (d < digits) {
+    uint32_t next = scan - mine;
+    for (int w = 0; w < wave; ++w) next += block_sums[w];
+    for (int w = 0; w < kSmallWaves; ++w) {
+      const uint32_t c = place[w][d];
+      place[w][d] = next;
+      next += c;
+    }
+  }
+  __syncthreads();
+  constexpr int kRounds = 4;  // whose loads are under way together
+  for (int i0 = first; i0 < end; i0 += 64 * kRounds) {
+    uint32_t keys[kRounds], values[kRounds];
+#pragma unroll
+    for (int k = 0; k < kRounds; ++k) {
+      const int i = min(i0 + k * 64 + lane, n - 1);
+      keys[k] = sort_key(p, i);
+      values[k] = p.tokens != nullptr ? static_cast<uint32_t>(i) : p.values_in[i];
+    }
+#pragma unroll
+    for (int k = 0; k < kRounds; ++k) {
+      const bool live = i0 + k * 64 + lane < end;
+      const int digit = keys[k] >> p.shift & mask;
+      uint64_t same = __ballot(live);
+      for (int b = 0; b < p.bits; ++b) {
+        const uint64_t set = __ballot(live && (digit >> b & 1));
+        same &= digit >> b & 1 ? set : ~set;
+      }
+      const uint64_t below = same & ((uint64_t{1} << lane) - 1);
+      uint32_t at = 0;
+      if (live) at = place[wave][digit] + __popcll(below);
+      __builtin_amdgcn_wave_barrier();  // every lane has read its place before one of them moves it
+      if (live && below == 0) place[wave][digit] += __popcll(same);
+      __builtin_amdgcn_wave_barrier();
+      if (live) {
+        p.keys_out[at] = keys[k];
+        p.values_out[at] = values[k];
+      }
+    }
+  }
+  __syncthreads();
+}
+
+template <class W>
+__global__ void __launch_bounds__(kSmallBlock) attnres_sort_small_kernel(SortPass p, int passes, uint32_t* keys0, uint32_t* values0,
+                                                                         uint32_t* keys1, uint32_t* values1, ZeroFill<W> zero) {
+  __shared__ uint32_t place[kSmallWaves][kMaxDigits];
+  __shared__ uint32_t block_sums[kSmallWaves];
+  if (blockIdx.x > 0) return zero_fill(zero, blockIdx.x - 1, gridDim.x - 1);
+  for (int pass = 0; pass < passes; ++pass) {
+    p.keys_out = pass % 2 ? keys1 : keys0;
+    p.values_out = pass % 2 ? values1 : values0;
+    sort_pass_small(p, place, block_sums);
+    p.tokens = nullptr;
+    p.keys_in = p.keys_out;
+    p.values_in = p.values_out;
+    p.shift += p.bits;
+  }
+}
+
 // --------------------------------------------------------------------- sums
 // The sorted list in pieces: a run of one token inside a piece is its table row's
 // gradient; what crosses a piece's border goes to the piece's partial rows
@@ -226,36 +322,46 @@ struct Runs {
   float* partial;  // [pieces][2][width]
 };
 
-constexpr int kAhead = 4;  // rows in flight per thread
+constexpr int kAhead = 8;       // rows in flight per thread
+constexpr int kMaxPiece = 64;
 
 template <class O, class W>
 __global__ void __launch_bounds__(kBlock) attnres_embedding_sum_kernel(Runs r, const O* __restrict__ grad_out, int width, float scale,
                                                                        W* __restrict__ grad_weight, int threads) {
-  const int per_block = kBlock / threads;
-  const int64_t piece = static_cast<int64_t>(blockIdx.x) * per_block + threadIdx.x / threads;
+  __shared__ uint32_t all_keys[kBlock / 8 * (kMaxPiece + 1)], all_values[kBlock / 8 * kMaxPiece];
+  const int per_block = kBlock / threads, group = threadIdx.x / threads, member = threadIdx.x % threads;
+  const int64_t piece = static_cast<int64_t>(blockIdx.x) * per_block + group;
   const int64_t first = piece * r.piece;
-  const int c = (static_cast<int>(blockIdx.y) * threads + threadIdx.x % threads) * kVec;
-  if (first >= r.n || c >= width) return;
-  const int count = static_cast<int>(r.n - first < r.piece ? r.n - first : r.piece);
-  bool from_left = first > 0 && r.keys[first - 1] == r.keys[first];
+  const int count = static_cast<int>(max(min(r.n - first, static_cast<int64_t>(r.piece)), int64_t{0}));
+  uint32_t* keys = all_keys + group * (r.piece + 1);
+  uint32_t* values = all_values + group * r.piece;
+  for (int i = member; i < count; i += threads) {
+    keys[i] = r.keys[first + i];
+    values[i] = r.values[first + i];
+  }
+  if (member == 0 && count > 0) keys[count] = first + count < r.n ? r.keys[first + count] : ~0u;
+  __syncthreads();
+  const int c = (static_cast<int>(blockIdx.y) * threads + member) * kVec;
+  if (count == 0 || c >= width) return;
+  uint32_t key = keys[0];
+  bool from_left = first > 0 && r.keys[first - 1] == key;
   float sum[kVec] = {};
-  uint32_t key = r.keys[first];
   for (int i0 = 0; i0 < count; i0 += kAhead) {
-    float x[kAhead][kVec];
-    uint32_t next[kAhead];
+    Chunk<O> rows[kAhead];
 #pragma unroll
     for (int j = 0; j < kAhead; ++j) {
-      const int64_t i = first + (i0 + j < count ? i0 + j : count - 1);
-      load_chunk(grad_out + static_cast<int64_t>(r.values[i]) * width, c, width, x[j]);
-      next[j] = i + 1 < r.n ? r.keys[i + 1] : ~0u;
+      rows[j].load(grad_out + static_cast<int64_t>(values[min(i0 + j, count - 1)]) * width, c, width);
     }
 #pragma unroll
     for (int j = 0; j < kAhead; ++j) {
       if (i0 + j >= count) break;
       if (key >= r.vocab) return;  // tokens outside the table: the rest of the list
+      float x[kVec];
+      rows[j].unpack(x);
 #pragma unroll
-      for (int e = 0; e < kVec; ++e) sum[e] += x[j][e];
-      const bool goes_on = next[j] == key;
+      for (int e = 0; e < kVec; ++e) sum[e] += x[e];
+      const uint32_t next = keys[i0 + j + 1];
+      const bool goes_on = next == key;
       if (goes_on && i0 + j + 1 < count) continue;
       if (from_left || goes_on) {
         store_chunk(r.partial + (piece * 2 + (from_left ? 0 : 1)) * width, c, width, sum);
@@ -268,30 +374,53 @@ __global__ void __launch_bounds__(kBlock) attnres_embedding_sum_kernel(Runs r, c
 #pragma unroll
       for (int e = 0; e < kVec; ++e) sum[e] = 0.0f;
       from_left = false;
-      key = next[j];
+      key = next;
     }
   }
 }
 
-// The runs that cross pieces: the piece where one begins adds up the others' partial rows.
+// The runs that cross pieces: for the piece where one begins, kJoinCols chunks of columns by kJoinGroups; a
+// group adds up every kJoinGroups-th partial row of the run, the groups' sums are added in order.
+constexpr int kJoinGroups = 8;
+constexpr int kJoinCols = kBlock / kJoinGroups;
+
 template <class W>
-__global__ void __launch_bounds__(kBlock) attnres_embedding_join_kernel(Runs r, int width, float scale, W* __restrict__ grad_weight,
-                                                                        int threads) {
-  const int per_block = kBlock / threads;
-  const int64_t piece = static_cast<int64_t>(blockIdx.x) * per_block + threadIdx.x / threads;
+__device__ __forceinline__ void join_runs(const Runs& r, int64_t piece, int width, float scale, W* grad_weight,
+                                          float (*sums)[kJoinCols * kVec]) {
   const int64_t first = piece * r.piece, end = first + r.piece;
-  const int c = (static_cast<int>(blockIdx.y) * threads + threadIdx.x % threads) * kVec;
-  if (end >= r.n || c >= width) return;
+  if (end >= r.n) return;
   const uint32_t key = r.keys[end - 1];
   if (key >= r.vocab || r.keys[end] != key) return;
   if (r.keys[first] == key && first > 0 && r.keys[first - 1] == key) return;  // began before this piece
-  float sum[kVec];
-  load_chunk(r.partial + (piece * 2 + 1) * width, c, width, sum);
-  for (int64_t p = piece + 1; p * r.piece < r.n && r.keys[p * r.piece] == key; ++p) {
-    float x[kVec];
-    load_chunk(r.partial + p * 2 * width, c, width, x);
+  const int group = threadIdx.x / kJoinCols, member = threadIdx.x % kJoinCols;
+  const int c = (static_cast<int>(blockIdx.y) * kJoinCols + member) * kVec;
+  const int64_t pieces = (r.n + r.piece - 1) / r.piece;
+  float sum[kVec] = {};
+  if (group == 0) load_chunk(r.partial + (piece * 2 + 1) * width, c, width, sum);
+  bool on = true;
+  for (int64_t p = piece + 1 + group; on; p += kJoinGroups * 4) {
+    float x[4][kVec];
+    bool same[4];
 #pragma unroll
-    for (int e = 0; e < kVec; ++e) sum[e] += x[e];
+    for (int j = 0; j < 4; ++j) {
+      const int64_t at = p + j * kJoinGroups < pieces ? p + j * kJoinGroups : pieces - 1;
+      same[j] = p + j * kJoinGroups < pieces && r.keys[at * r.piece] == key;
+      load_chunk(r.partial + at * 2 * width, c, width, x[j]);  // stale where the run has ended: not added
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      on = on && same[j];
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) sum[e] = on ? sum[e] + x[j][e] : sum[e];
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < kVec; ++e) sums[group][member * kVec + e] = sum[e];
+  __syncthreads();
+  if (group > 0 || c >= width) return;
+  for (int g = 1; g < kJoinGroups; ++g) {
+#pragma unroll
+    for (int e = 0; e < kVec; ++e) sum[e] += sums[g][member * kVec + e];
   }
 #pragma unroll
   for (int e = 0; e < kVec; ++e) sum[e] *= scale;
@@ -299,25 +428,33 @@ __global__ void __launch_bounds__(kBlock) attnres_embedding_join_kernel(Runs r, 
 }
 
 template <class O, class W>
-__global__ void __launch_bounds__(kBlock) attnres_positions_kernel(const O* __restrict__ grad_out, int64_t batch, int64_t length,
-                                                                   int width, W* __restrict__ grad_positions, int64_t position_rows,
-                                                                   int threads) {
-  const int per_block = kBlock / threads;
-  const int64_t t = static_cast<int64_t>(blockIdx.x) * per_block + threadIdx.x / threads;
-  if (t >= position_rows) return;
-  for (int c = (threadIdx.x % threads) * kVec; c < width; c += threads * kVec) {
-    float sum[kVec] = {};
-    if (t < length) {
+struct Places {
+  const O* grad_out;
+  int64_t batch, length;
+  W* grad_positions;
+  int64_t rows;
+};
+
+// Blocks 0 .. join-1 join a piece's run, the others sum the positions' gradient over the batch.
+template <class O, class W>
+__global__ void __launch_bounds__(kBlock) attnres_embedding_join_kernel(Runs r, int width, float scale, W* __restrict__ grad_weight,
+                                                                        int join, Places<O, W> place) {
+  __shared__ float sums[kJoinGroups][kJoinCols * kVec];
+  if (static_cast<int>(blockIdx.x) < join) return join_runs(r, blockIdx.x, width, scale, grad_weight, sums);
+  const int64_t t = static_cast<int64_t>(blockIdx.x - join) * kJoinGroups + threadIdx.x / kJoinCols;
+  const int c = (static_cast<int>(blockIdx.y) * kJoinCols + threadIdx.x % kJoinCols) * kVec;
+  if (t >= place.rows || c >= width) return;
+  float sum[kVec] = {};
+  if (t < place.length) {
 #pragma unroll 4
-      for (int64_t b = 0; b < batch; ++b) {
-        float x[kVec];
-        load_chunk(grad_out + (b * length + t) * width, c, width, x);
+    for (int64_t b = 0; b < place.batch; ++b) {
+      float x[kVec];
+      load_chunk(place.grad_out + (b * place.length + t) * width, c, width, x);
 #pragma unroll
-        for (int e = 0; e < kVec; ++e) sum[e] += x[e];
-      }
+      for (int e = 0; e < kVec; ++e) sum[e] += x[e];
     }
-    store_chunk(grad_positions + t * width, c, width, sum);
   }
+  store_chunk(place.grad_positions + t * width, c, width, sum);
 }
 
 // ---------------------------------------------------------------------- host
@@ -334,9 +471,9 @@ Plan plan(int64_t n, int64_t vocab, int64_t width) {
   p.passes = (bits + 9) / 10;           // digits of at most 10 bits
   p.bits = (bits + p.passes - 1) / p.passes;
   p.tiles = static_cast<int>((n + kTile - 1) / kTile);
-  // pieces of 4 to 64 entries, about a thousand of them
-  p.piece = 4;
-  while (p.piece < 64 && p.piece * 1024 < n) p.piece *= 2;
+  // pieces of 8 to 64 entries, about a thousand of them
+  p.piece = 8;
+  while (p.piece < kMaxPiece && p.piece * 1024 < n) p.piece *= 2;
   p.pieces = (n + p.piece - 1) / p.piece;
   int64_t at = 0;
   const auto take = [&](int64_t bytes) {
@@ -357,10 +494,13 @@ void embedding_backward(const void* grad_out, const void* tokens, int token_byte
                         char* workspace, hipStream_t stream) {
   const int64_t n = batch * length;
   const int threads = row_threads(width), per_block = kBlock / threads;
+  const unsigned slabs = static_cast<unsigned>((width + threads * kVec - 1) / (threads * kVec));
+  Runs runs{};
+  int join = 0;
   if (grad_weight != nullptr) {
     const Plan p = plan(n, vocab, width);
-    const ZeroFill<W> zero{static_cast<W*>(grad_weight), vocab * width};
-    const int64_t fill = std::min<int64_t>((zero.elements + kBlock * kVec - 1) / (kBlock * kVec), 2048);
+    const int64_t elements = vocab * width;
+    ZeroFill<W> zero{static_cast<W*>(grad_weight), 0, elements, elements * static_cast<int64_t>(sizeof(W)) >= kPastCaches};
     uint32_t* keys[2];
     uint32_t* values[2];
     for (int k = 0; k < 2; ++k) {
@@ -374,31 +514,47 @@ void embedding_backward(const void* grad_out, const void* tokens, int token_byte
     s.vocab = vocab;
     s.bits = p.bits;
     s.tiles = p.tiles;
-    for (int pass = 0; pass < p.passes; ++pass) {
-      s.tokens = pass == 0 ? tokens : nullptr;
-      s.keys_in = keys[(pass + 1) % 2];
-      s.values_in = values[(pass + 1) % 2];
-      s.keys_out = keys[pass % 2];
-      s.values_out = values[pass % 2];
-      s.shift = pass * p.bits;
-      const unsigned grid = static_cast<unsigned>(p.tiles + (pass == 0 ? fill : 0));
-      if (grid > 0) hipLaunchKernelGGL((attnres_sort_count_kernel<W>), dim3(grid), dim3(kBlock), 0, stream, s, zero);
-      if (n > 0) hipLaunchKernelGGL(attnres_sort_place_kernel, dim3(p.tiles), dim3(kBlock), 0, stream, s);
+    const int last = (p.passes - 1) % 2;
+    if (n <= kSmall) {
+      s.tokens = tokens;
+      const unsigned blocks = static_cast<unsigned>(std::min<int64_t>((elements + 8191) / 8192, 512));
+      hipLaunchKernelGGL((attnres_sort_small_kernel<W>), dim3(1 + blocks), dim3(kSmallBlock), 0, stream, s, n > 0 ? p.passes : 0,
+                         keys[0], values[0], keys[1], values[1], zero);
+    } else {
+      // every launch of the sort, which leaves most of the chip idle, clears its share of the table's gradient
+      const int64_t share = (elements / (2 * p.passes) + 255) / 256 * 256;
+      const unsigned fill = static_cast<unsigned>(std::min<int64_t>(share / (kBlock * kVec) + 1, 2048));
+      for (int pass = 0; pass < p.passes; ++pass) {
+        s.tokens = pass == 0 ? tokens : nullptr;
+        s.keys_in = keys[(pass + 1) % 2];
+        s.values_in = values[(pass + 1) % 2];
+        s.keys_out = keys[pass % 2];
+        s.values_out = values[pass % 2];
+        s.shift = pass * p.bits;
+        const auto next_share = [&](bool rest) {
+          zero.first = pass == 0 && !rest ? 0 : zero.end;
+          zero.end = rest && pass == p.passes - 1 ? elements : std::min(zero.first + share, elements);
+        };
+        next_share(false);
+        hipLaunchKernelGGL((attnres_sort_count_kernel<W>), dim3(p.tiles + fill), dim3(kBlock), 0, stream, s, zero);
+        next_share(true);
+        hipLaunchKernelGGL((attnres_sort_place_kernel<W>), dim3(p.tiles + fill), dim3(kBlock), 0, stream, s, zero);
+      }
     }
+    runs = Runs{keys[last], values[last], n, vocab, p.piece, reinterpret_cast<float*>(workspace + p.partial)};
     if (n > 0) {
-      const Runs r{s.keys_out, s.values_out, n, vocab, p.piece, reinterpret_cast<float*>(workspace + p.partial)};
-      const dim3 grid(static_cast<unsigned>((p.pieces + per_block - 1) / per_block),
-                      static_cast<unsigned>((width + threads * kVec - 1) / (threads * kVec)));
-      hipLaunchKernelGGL((attnres_embedding_sum_kernel<O, W>), grid, dim3(kBlock), 0, stream, r,
+      join = static_cast<int>(p.pieces);
+      hipLaunchKernelGGL((attnres_embedding_sum_kernel<O, W>), dim3((join + per_block - 1) / per_block, slabs), dim3(kBlock), 0, stream, runs,
                          static_cast<const O*>(grad_out), static_cast<int>(width), scale, static_cast<W*>(grad_weight), threads);
-      hipLaunchKernelGGL((attnres_embedding_join_kernel<W>), grid, dim3(kBlock), 0, stream, r, static_cast<int>(width), scale,
-                         static_cast<W*>(grad_weight), threads);
     }
   }
-  if (grad_positions != nullptr && position_rows > 0) {
-    hipLaunchKernelGGL((attnres_positions_kernel<O, W>), dim3(static_cast<unsigned>((position_rows + per_block - 1) / per_block)),
-                       dim3(kBlock), 0, stream, static_cast<const O*>(grad_out), batch, length, static_cast<int>(width),
-                       static_cast<W*>(grad_positions), position_rows, threads);
+  const Places<O, W> place{static_cast<const O*>(grad_out), batch, length, static_cast<W*>(grad_positions),
+                           grad_positions != nullptr ? position_rows : 0};
+  const int64_t blocks = join + (place.rows + kJoinGroups - 1) / kJoinGroups;
+  if (blocks > 0) {
+    const unsigned columns = static_cast<unsigned>((width + kJoinCols * kVec - 1) / (kJoinCols * kVec));
+    hipLaunchKernelGGL((attnres_embedding_join_kernel<O, W>), dim3(static_cast<unsigned>(blocks), columns), dim3(kBlock), 0, stream,
+                       runs, static_cast<int>(width), scale, static_cast<W*>(grad_weight), join, place);
   }
 }
 

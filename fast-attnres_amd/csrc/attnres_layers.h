@@ -21,6 +21,9 @@ namespace layers {
 
 constexpr int kBlock = 256;
 constexpr int kVec = 8;  // elements per chunk
+// Results from here on are stored past the caches: beside what they are made of they do not stay in the 256 MB of
+// the last one anyway.
+constexpr int64_t kPastCaches = int64_t{128} << 20;
 
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
@@ -88,16 +91,27 @@ __device__ __forceinline__ void load8(const T* p, float* x) {
   }
 }
 
+// `past`: past the caches, for results too large to stay in them.
 template <class T>
-__device__ __forceinline__ void store8(T* p, const float* x) {
+__device__ __forceinline__ void store8(T* p, const float* x, bool past = false) {
   if constexpr (std::is_same_v<T, float>) {
-    reinterpret_cast<Raw32*>(p)->v = f32x4{x[0], x[1], x[2], x[3]};
-    reinterpret_cast<Raw32*>(p + 4)->v = f32x4{x[4], x[5], x[6], x[7]};
+    const f32x4 a = {x[0], x[1], x[2], x[3]}, b = {x[4], x[5], x[6], x[7]};
+    if (past) {
+      __builtin_nontemporal_store(a, &reinterpret_cast<Raw32*>(p)->v);
+      __builtin_nontemporal_store(b, &reinterpret_cast<Raw32*>(p + 4)->v);
+    } else {
+      reinterpret_cast<Raw32*>(p)->v = a;
+      reinterpret_cast<Raw32*>(p + 4)->v = b;
+    }
   } else {
     u32x4 w;
 #pragma unroll
     for (int e = 0; e < 4; ++e) w[e] = pack2<T>(x[2 * e], x[2 * e + 1]);
-    reinterpret_cast<Raw16*>(p)->v = w;
+    if (past) {
+      __builtin_nontemporal_store(w, &reinterpret_cast<Raw16*>(p)->v);
+    } else {
+      reinterpret_cast<Raw16*>(p)->v = w;
+    }
   }
 }
 
@@ -114,9 +128,9 @@ __device__ __forceinline__ void load_chunk(const T* row, int c, int width, float
 }
 
 template <class T>
-__device__ __forceinline__ void store_chunk(T* row, int c, int width, const float* x) {
+__device__ __forceinline__ void store_chunk(T* row, int c, int width, const float* x, bool past = false) {
   if (c + kVec <= width) {
-    store8(row + c, x);
+    store8(row + c, x, past);
   } else {
 #pragma unroll
     for (int e = 0; e < kVec; ++e) {
@@ -125,13 +139,61 @@ __device__ __forceinline__ void store_chunk(T* row, int c, int width, const floa
   }
 }
 
-// Sum over groups of LANES lanes of a wavefront (LANES a power of two <= 64), in
-// every lane of the group; the tree's order is fixed.
+// The same eight elements as they lie, for loads that are under way while others are worked on.
+template <class T>
+struct Chunk {
+  u32x4 w[sizeof(T) / 2];
+  __device__ __forceinline__ void load(const T* row, int c, int width) {
+    if (c + kVec <= width) {
+#pragma unroll
+      for (size_t k = 0; k < sizeof(T) / 2; ++k) w[k] = reinterpret_cast<const Raw16*>(row + c)[k].v;
+    } else {
+      float x[kVec];
+      load_chunk(row, c, width, x);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if constexpr (std::is_same_v<T, float>) {
+          w[0][e] = __float_as_uint(x[e]);
+          w[1][e] = __float_as_uint(x[4 + e]);
+        } else {
+          w[0][e] = pack2<T>(x[2 * e], x[2 * e + 1]);
+        }
+      }
+    }
+  }
+  __device__ __forceinline__ void unpack(float* x) const {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if constexpr (std::is_same_v<T, float>) {
+        x[e] = __uint_as_float(w[0][e]);
+        x[4 + e] = __uint_as_float(w[1][e]);
+      } else {
+        x[2 * e] = to_f32(T{static_cast<uint16_t>(w[0][e] & 0xffffu)});
+        x[2 * e + 1] = to_f32(T{static_cast<uint16_t>(w[0][e] >> 16)});
+      }
+    }
+  }
+};
+
+template <int CTRL>
+__device__ __forceinline__ float dpp(float x) {
+  return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), CTRL, 0xf, 0xf, false));
+}
+__device__ __forceinline__ float lane_value(float x, int lane) {
+  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), lane));
+}
+
+// Sum over groups of 16 lanes or a whole wavefront, the same bits in every lane of the
+// group: quad permutations and row mirrors within 16 lanes, lane reads across them.
 template <int LANES>
 __device__ __forceinline__ float group_sum(float x) {
-#pragma unroll
-  for (int step = LANES / 2; step > 0; step >>= 1) x += __shfl_xor(x, step, 64);
-  return x;
+  static_assert(LANES == 16 || LANES == 64, "a DPP row or a wavefront");
+  x += dpp<0xb1>(x);   // quad_perm [1,0,3,2]
+  x += dpp<0x4e>(x);   // quad_perm [2,3,0,1]
+  x += dpp<0x141>(x);  // row_half_mirror
+  x += dpp<0x140>(x);  // row_mirror
+  if constexpr (LANES == 16) return x;
+  return (lane_value(x, 0) + lane_value(x, 16)) + (lane_value(x, 32) + lane_value(x, 48));
 }
 
 }  // namespace layers
