@@ -34,7 +34,8 @@ template <class W, class O>
 __global__ void __launch_bounds__(kBlock) attnres_embedding_fwd_kernel(const void* __restrict__ tokens, int token_bytes, int64_t rows,
                                                                        int64_t length, const W* __restrict__ weight, int64_t vocab,
                                                                        int width, const W* __restrict__ positions, float scale,
-                                                                       O* __restrict__ out, int threads) {
+                                                                       O* __restrict__ out, int threads,
+                                                                       bool past) {
   const int per_block = kBlock / threads;
   const int64_t row = static_cast<int64_t>(blockIdx.x) * per_block + threadIdx.x / threads;
   if (row >= rows) return;
@@ -52,7 +53,7 @@ __global__ void __launch_bounds__(kBlock) attnres_embedding_fwd_kernel(const voi
       if (place != nullptr) x[e] += p[e];
       if (!known) x[e] = __builtin_nanf("");
     }
-    store_chunk(out + row * width, c, width, x);
+    store_chunk(out + row * width, c, width, x, past);
   }
 }
 
@@ -62,7 +63,7 @@ __global__ void __launch_bounds__(kBlock) attnres_embedding_fwd_kernel(const voi
 // per digit, then a place for each entry -- the entries of smaller digits, of earlier tiles and
 // of earlier wavefronts, then the order within the wavefront (ballots of the digit's bits).
 
-constexpr int kTile = 2048;
+constexpr int kTile = 1024;
 constexpr int kWaves = kBlock / 64;
 constexpr int kMaxDigits = 1024;
 
@@ -611,7 +612,7 @@ int attnres_hip_embedding_forward(const void* tokens, int token_bytes, int64_t b
     hipLaunchKernelGGL((attnres_embedding_fwd_kernel<W, O>), dim3(static_cast<unsigned>((rows + per_block - 1) / per_block)),
                        dim3(kBlock), 0, static_cast<hipStream_t>(stream), tokens, token_bytes, rows, length,
                        static_cast<const W*>(weight), vocab, static_cast<int>(width), static_cast<const W*>(positions), scale,
-                       static_cast<O*>(out), threads);
+                       static_cast<O*>(out), threads, rows * width * static_cast<int64_t>(sizeof(O)) >= kPastCaches);
   });
   return layer_launch_status("embedding forward");
 }

@@ -195,19 +195,22 @@ struct TileAt {
 
 // Workgroup to tile: workgroups go round the 8 XCDs in turn, so each XCD takes one contiguous part of
 // the tiles' order, in which 8 tiles of B by all of A's follow each other: the 32 tiles that run on an
-// XCD at a time share 8 + 4 operand stripes in its L2.
-__device__ __forceinline__ TileAt tile_at(const Product& p) {
-  const int total = p.tiles_a * p.tiles_b * p.splits;
+// XCD at a time share 8 + 4 operand stripes in its L2.  tiles_b: those with rows that count, so that the XCDs
+// get equal shares of them; false for the workgroups past the last tile.
+__device__ __forceinline__ bool tile_at(const Product& p, int tiles_b, TileAt* tile) {
+  const int total = p.tiles_a * tiles_b * p.splits;
   const int id = blockIdx.x;
+  if (id >= total) return false;
   const int q = total / 8, r = total % 8, xcd = id % 8, i = id / 8;
   int at = xcd < r ? xcd * (q + 1) + i : r * (q + 1) + (xcd - r) * q + i;
-  const int split = at / (p.tiles_a * p.tiles_b);
-  at -= split * p.tiles_a * p.tiles_b;
+  const int split = at / (p.tiles_a * tiles_b);
+  at -= split * p.tiles_a * tiles_b;
   constexpr int kGroup = 8;
   const int group = at / (kGroup * p.tiles_a);
-  const int size = min(kGroup, p.tiles_b - group * kGroup);
+  const int size = min(kGroup, tiles_b - group * kGroup);
   at -= group * kGroup * p.tiles_a;
-  return {at / size, group * kGroup + at % size, split};
+  *tile = {at / size, group * kGroup + at % size, split};
+  return true;
 }
 
 // [16 entries of A][16 entries of B]; lane l, register e: entry 4 (l / 16) + e of A, l % 16 of B.
@@ -426,9 +429,9 @@ struct LogitArgs {
 template <class T, int SEGMENTS>
 __global__ void __launch_bounds__(kThreads) attnres_loss_logits_kernel(LogitArgs g) {
   __shared__ __align__(16) uint16_t lds[kStages * 2 * kOperand];
-  const TileAt tile = tile_at(g.product);
-  const int count = *g.product.count;
-  if (tile.b * kTile >= count) return;
+  const int count = __builtin_amdgcn_readfirstlane(*g.product.count);
+  TileAt tile;
+  if (!tile_at(g.product, (count + kTile - 1) / kTile, &tile)) return;
   Accumulators acc;
   multiply<T, SEGMENTS, true, true>(g.product, tile, stages_of(g.product, 0), lds, acc);
   const int wave = wave_index(), lane = threadIdx.x % 64;
@@ -499,9 +502,9 @@ __device__ __forceinline__ int staged(int row, int chunk) { return row * 32 + (c
 template <class T, int SEGMENTS>
 __global__ void __launch_bounds__(kThreads) attnres_loss_probability_kernel(LogitArgs g) {
   __shared__ __align__(16) uint16_t lds[kStages * 2 * kOperand];
-  const TileAt tile = tile_at(g.product);
-  const int count = *g.product.count;
-  if (tile.b * kTile >= count) return;
+  const int count = __builtin_amdgcn_readfirstlane(*g.product.count);
+  TileAt tile;
+  if (!tile_at(g.product, (count + kTile - 1) / kTile, &tile)) return;
   Accumulators acc;
   multiply<T, SEGMENTS, true, true>(g.product, tile, stages_of(g.product, 0), lds, acc);
   const int wave = wave_index(), lane = threadIdx.x % 64;
@@ -600,8 +603,9 @@ __device__ __forceinline__ void zero_tile(const GradientArgs& g, const TileAt& t
 template <class T, class OUT, int SEGMENTS, bool B_ROWS>
 __global__ void __launch_bounds__(kThreads) attnres_loss_gradient_kernel(GradientArgs g) {
   __shared__ __align__(16) uint16_t lds[kStages * 2 * kOperand];
-  const TileAt tile = tile_at(g.product);
-  if (g.live_only && tile.b * kTile >= *g.product.count) return;
+  const int live = (__builtin_amdgcn_readfirstlane(*g.product.count) + kTile - 1) / kTile;
+  TileAt tile;
+  if (!tile_at(g.product, g.live_only ? live : g.product.tiles_b, &tile)) return;
   const Stages stages = stages_of(g.product, tile.split);
   if (stages.count == 0) return zero_tile(g, tile, static_cast<OUT*>(g.out));
   Accumulators acc;
@@ -663,43 +667,189 @@ __global__ void __launch_bounds__(kThreads) attnres_loss_gradient_kernel(Gradien
 
 // ------------------------------------------------------------------ small passes
 
-// One workgroup: the rows whose target counts, in order.  A target outside the
-// vocabulary is marked -1 (the row's loss and gradients become NaN).
+// One workgroup: the rows whose target counts, in order, eight rounds of 1024 rows at a time.  A target outside
+// the vocabulary is marked -1 (the row's loss and gradients become NaN).
 constexpr int kScanThreads = 1024;
+constexpr int kScanRounds = 8;
+constexpr int kScanWaves = kScanThreads / 64;
 
 __global__ void __launch_bounds__(kScanThreads) attnres_loss_rows_kernel(const void* targets, int target_bytes, int64_t rows, int64_t vocab,
                                                                          int64_t ignore_index, Saved s) {
-  __shared__ int waves[kScanThreads / 64];
+  __shared__ int before[kScanRounds * kScanWaves + 1];  // rows that count before a round's wavefront
   const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
   int base = 0;
-  for (int64_t r0 = 0; r0 < rows; r0 += kScanThreads) {
-    const int64_t row = r0 + threadIdx.x;
-    int64_t target = ignore_index;
-    if (row < rows) {
-      target = target_bytes == 8 ? static_cast<const int64_t*>(targets)[row] : static_cast<const int32_t*>(targets)[row];
+  for (int64_t r0 = 0; r0 < rows; r0 += kScanThreads * kScanRounds) {
+    int64_t target[kScanRounds];
+#pragma unroll
+    for (int k = 0; k < kScanRounds; ++k) {
+      const int64_t row = min(r0 + k * kScanThreads + threadIdx.x, rows - 1);
+      target[k] = target_bytes == 8 ? static_cast<const int64_t*>(targets)[row] : static_cast<const int32_t*>(targets)[row];
     }
-    const bool counts = row < rows && target != ignore_index;
-    const uint64_t ballot = __ballot(counts);
-    if (lane == 0) waves[wave] = __popcll(ballot);
+    uint64_t counts[kScanRounds];
+#pragma unroll
+    for (int k = 0; k < kScanRounds; ++k) {
+      counts[k] = __ballot(r0 + k * kScanThreads + threadIdx.x < rows && target[k] != ignore_index);
+      if (lane == 0) before[k * kScanWaves + wave] = __popcll(counts[k]);
+    }
     __syncthreads();
-    int before = base, all = 0;
-    for (int w = 0; w < kScanThreads / 64; ++w) {
-      before += w < wave ? waves[w] : 0;
-      all += waves[w];
+    if (wave == 0) {  // two entries per lane
+      static_assert(kScanRounds * kScanWaves == 128, "two counts per lane");
+      const int x = before[2 * lane], y = before[2 * lane + 1];
+      int scan = x + y;
+#pragma unroll
+      for (int step = 1; step < 64; step <<= 1) {
+        const int other = __shfl_up(scan, step, 64);
+        scan += lane >= step ? other : 0;
+      }
+      before[2 * lane] = scan - x - y;
+      before[2 * lane + 1] = scan - y;
+      if (lane == 63) before[128] = scan;
     }
-    const int at = before + __popcll(ballot & ((uint64_t{1} << lane) - 1));
-    if (row < rows) s.packed[row] = counts ? at : -1;
-    if (counts) {
-      s.index[at] = static_cast<int32_t>(row);
-      s.target[at] = target >= 0 && target < vocab ? static_cast<int32_t>(target) : -1;
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < kScanRounds; ++k) {
+      const int64_t row = r0 + k * kScanThreads + threadIdx.x;
+      const bool live = counts[k] >> lane & 1;
+      const int at = base + before[k * kScanWaves + wave] + __popcll(counts[k] & ((uint64_t{1} << lane) - 1));
+      if (row < rows) s.packed[row] = live ? at : -1;
+      if (live) {
+        s.index[at] = static_cast<int32_t>(row);
+        s.target[at] = target[k] >= 0 && target[k] < vocab ? static_cast<int32_t>(target[k]) : -1;
+      }
     }
-    base += all;
+    base += before[128];
     __syncthreads();
   }
   if (threadIdx.x == 0) {
     s.header->count = base;
     s.header->scale[0] = s.header->scale[1] = 1.0f;
     s.header->amax[0] = s.header->amax[1] = 0;
+  }
+}
+
+// ------------------------------------------------------------------- few rows
+// The forward of up to kFewRows rows reads W once and is bound by that: 64 words per workgroup, 16
+// per wavefront, W and H straight to registers as they lie (any width and alignment; FP32 inputs
+// by FP32 matrix instructions, which the few rows have time for), no packing.  A lane holds 16 consecutive k's of its
+// word or row per 64; the order of the k's in a matrix instruction is of no account, as both operands share it.
+constexpr int kFewRows = 64;
+constexpr int kFewWords = 64;
+
+template <class X>
+struct FewChunk {  // 16 consecutive elements, as they lie
+  u32x4 w[sizeof(X)];
+  __device__ __forceinline__ void load(const X* row, int k, int width) {
+    Chunk<X> a, b;
+    a.load(row, k, width);
+    b.load(row, k + kVec, width);
+#pragma unroll
+    for (size_t i = 0; i < sizeof(X) / 2; ++i) w[i] = a.w[i], w[sizeof(X) / 2 + i] = b.w[i];
+  }
+};
+
+template <class X>
+__device__ __forceinline__ f32x4 few_mfma(const FewChunk<X>& a, const FewChunk<X>& b, f32x4 c) {
+  if constexpr (std::is_same_v<X, float>) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a.w[i][e]), __uint_as_float(b.w[i][e]), c, 0, 0, 0);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) c = mfma<X>(__builtin_bit_cast(s16x8, a.w[i]), __builtin_bit_cast(s16x8, b.w[i]), c);
+  }
+  return c;
+}
+
+template <class X>
+struct FewArgs {
+  const X* hidden;
+  const X* weight;
+  int64_t hidden_stride, weight_stride, vocab;
+  int width;
+  Saved saved;
+  f32x2* sums;          // [workgroups][kFewRows]
+  float* target_logit;  // [kFewRows]
+};
+
+template <class X, int TILES>  // of 16 rows
+__global__ void __launch_bounds__(kBlock) attnres_loss_few_kernel(FewArgs<X> g) {
+  __shared__ f32x2 meet[4][TILES * 16];
+  const int wave = wave_index(), lane = threadIdx.x % 64, group = lane / 16, entry = lane % 16;
+  const int64_t v0 = static_cast<int64_t>(blockIdx.x) * kFewWords + wave * 16;
+  const X* w = g.weight + min(v0 + entry, g.vocab - 1) * g.weight_stride;
+  constexpr int kSteps = sizeof(X) == 4 || TILES == 4 ? 2 : 4;  // of 64 k's under way together
+  constexpr int kSpan = kSteps * 64;
+  FewChunk<X> next[kSteps];
+  const auto fetch = [&](int k0) {
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) next[s].load(w, k0 + s * 64 + group * 16, g.width);
+  };
+  fetch(0);  // before what has to be known of the rows
+  const int count = g.saved.header->count;
+  if (count == 0) return;
+  const X* h[TILES];
+#pragma unroll
+  for (int t = 0; t < TILES; ++t) {
+    h[t] = g.hidden + g.saved.index[min(t * 16 + entry, count - 1)] * g.hidden_stride;
+  }
+  FewChunk<X> next_h[kSteps][TILES];
+  const auto fetch_h = [&](int k0) {
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+#pragma unroll
+      for (int t = 0; t < TILES; ++t) next_h[s][t].load(h[t], k0 + s * 64 + group * 16, g.width);
+    }
+  };
+  fetch_h(0);
+  f32x4 acc[TILES] = {};
+  for (int k0 = 0; k0 < g.width; k0 += kSpan) {
+    FewChunk<X> now[kSteps], now_h[kSteps][TILES];
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+      now[s] = next[s];
+#pragma unroll
+      for (int t = 0; t < TILES; ++t) now_h[s][t] = next_h[s][t];
+    }
+    if (k0 + kSpan < g.width) {
+      fetch(k0 + kSpan);
+      fetch_h(k0 + kSpan);
+    }
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+#pragma unroll
+      for (int t = 0; t < TILES; ++t) acc[t] = few_mfma<X>(now[s], now_h[s][t], acc[t]);
+    }
+  }
+  const int last = static_cast<int>(min(g.vocab - v0, int64_t{16})) - 4 * group;  // entries below it count
+#pragma unroll
+  for (int t = 0; t < TILES; ++t) {
+    const int row = t * 16 + entry;
+    const int64_t from_v0 = g.saved.target[min(row, count - 1)] - v0;
+    const int rel = row < count && from_v0 >= 4 * group && from_v0 < 4 * group + 4 ? static_cast<int>(from_v0) - 4 * group : -1;
+    float top = -__builtin_inff();
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      top = fmaxf(top, e < last ? acc[t][e] : -__builtin_inff());
+      if (e == rel) g.target_logit[row] = acc[t][e];
+    }
+    top = fmaxf(top, __shfl_xor(top, 16, 64));
+    top = fmaxf(top, __shfl_xor(top, 32, 64));
+    const float from = top == -__builtin_inff() ? 0.0f : top;
+    float sum = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) sum += e < last ? __expf(acc[t][e] - from) : 0.0f;
+    sum += __shfl_xor(sum, 16, 64);
+    sum += __shfl_xor(sum, 32, 64);
+    if (lane < 16) meet[wave][row] = f32x2{top, sum};
+  }
+  __syncthreads();
+  if (threadIdx.x < TILES * 16) {
+    g.sums[static_cast<int64_t>(blockIdx.x) * kFewRows + threadIdx.x] =
+        join(join(meet[0][threadIdx.x], meet[1][threadIdx.x]), join(meet[2][threadIdx.x], meet[3][threadIdx.x]));
   }
 }
 
@@ -781,28 +931,34 @@ __global__ void __launch_bounds__(kBlock) attnres_loss_pack_kernel(const X* __re
   }
 }
 
-// Per row of the input: its log-sum from the tiles' sums, and its loss.  64 rows by 4 parts
-// of the tiles per workgroup.
+// Per row of the input: its log-sum from the tiles' sums, and its loss.  4 rows by 64 parts
+// of the tiles per workgroup: with few rows the tiles' sums are long chains, and their latency is all there is.
+constexpr int kReduceRows = 4, kReduceParts = kBlock / kReduceRows;
+
 __global__ void __launch_bounds__(kBlock) attnres_loss_reduce_kernel(const f32x2* __restrict__ sums, int tiles, int64_t row_tiles,
                                                                      const float* __restrict__ target_logit, int64_t rows, Saved s,
                                                                      float* __restrict__ loss) {
-  __shared__ f32x2 part[4][64];
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * 64 + threadIdx.x % 64;
-  const int which = threadIdx.x / 64;
+  __shared__ f32x2 part[kBlock / 64][kReduceRows];
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * kReduceRows + threadIdx.x % kReduceRows;
+  const int which = threadIdx.x / kReduceRows;
   const int at = row < rows ? s.packed[row] : -1;
   f32x2 total = {-__builtin_inff(), 0.0f};
   if (at >= 0) {
 #pragma unroll 8
-    for (int t = which; t < tiles; t += 4) total = join(total, sums[static_cast<int64_t>(t) * row_tiles + at]);
+    for (int t = which; t < tiles; t += kReduceParts) total = join(total, sums[static_cast<int64_t>(t) * row_tiles + at]);
   }
-  part[which][threadIdx.x % 64] = total;
+#pragma unroll
+  for (int step = kReduceRows; step < 64; step <<= 1) {
+    total = join(total, f32x2{__shfl_xor(total.x, step, 64), __shfl_xor(total.y, step, 64)});
+  }
+  if (threadIdx.x % 64 < kReduceRows) part[threadIdx.x / 64][threadIdx.x % 64] = total;
   __syncthreads();
   if (which != 0 || row >= rows) return;
   if (at < 0) {
     loss[row] = 0.0f;
     return;
   }
-  for (int k = 1; k < 4; ++k) total = join(total, part[k][threadIdx.x]);
+  for (int k = 1; k < kBlock / 64; ++k) total = join(total, part[k][threadIdx.x]);
   const bool known = s.target[at] >= 0;
   s.stats[at] = f32x2{total.x, known ? 1.0f / total.y : __builtin_nanf("")};
   // the logarithm of the sum by itself: at a probability of one it is the whole loss
@@ -898,16 +1054,19 @@ constexpr int64_t kMaxStride = int64_t{1} << 22;  // of W multiplied in place: 2
 constexpr int64_t kPieceBytes = int64_t{512} << 20;  // of P at a time
 constexpr int kUnits = 256;                          // compute units, one workgroup each
 
-// How many parts the depth is cut into so that the workgroups fill the chip: the number with the fullest last
-// round, the smaller at a tie; a part keeps at least 16 stages.
-int choose_splits(int64_t tiles, int64_t depth) {
+// How many parts the depth of a gradient product is cut into, so that its workgroups fill the chip: what takes the
+// least time at 1.1 PFLOP/s for full rounds of workgroups and 4.5 TB/s for the FP32 partial sums that are
+// written and read again (both as measured).  `direct`: one part needs no partial sums.  A part keeps at least 8 stages.
+int choose_splits(int64_t tiles, int64_t depth, int segments, bool direct) {
   int best = 1;
-  double best_fill = 0.0;
+  double best_time = 0.0;
   for (int s = 1; s <= 32; ++s) {
-    if (s > 1 && depth / kDepth / s < 16) break;
-    const int64_t work = tiles * s, rounds = (work + kUnits - 1) / kUnits;
-    const double fill = static_cast<double>(work) / static_cast<double>(rounds * kUnits) - 0.01 * s;
-    if (fill > best_fill + 1e-9) best = s, best_fill = fill;
+    if (s > 1 && depth / kDepth / s < 8) break;
+    const int64_t rounds = (tiles * s + kUnits - 1) / kUnits;
+    const double tile = 2.0 * kTile * kTile * static_cast<double>(depth) * segments / s / (1.1e15 / kUnits);
+    const double partial = s == 1 && direct ? 0.0 : 8.0 * kTile * kTile * static_cast<double>(tiles) * s / 4.5e12;
+    const double time = static_cast<double>(rounds) * tile + partial;
+    if (s == 1 || time < best_time) best = s, best_time = time;
   }
   return best;
 }
@@ -935,12 +1094,13 @@ LossPlan loss_plan(int64_t rows, int64_t vocab, int64_t width, int dtype, bool b
     at += round_up(bytes, 256);
     return from;
   };
-  for (int k = 0; k < parts; ++k) p.hidden[k] = take(2 * p.rows_pad * p.width_pad);
-  if (p.pack_weight) {
-    for (int k = 0; k < parts; ++k) p.weight[k] = take(2 * vocab * p.width_pad);
+  const bool few = !backward && rows <= kFewRows;
+  if (!few) {
+    for (int k = 0; k < parts; ++k) p.hidden[k] = take(2 * p.rows_pad * p.width_pad);
+    for (int k = 0; p.pack_weight && k < parts; ++k) p.weight[k] = take(2 * vocab * p.width_pad);
   }
   if (!backward) {
-    p.sums = take(8 * (p.vocab_pad / kTile) * p.rows_pad);
+    p.sums = take(few ? 8 * ((vocab + kFewWords - 1) / kFewWords) * kFewRows : 8 * (p.vocab_pad / kTile) * p.rows_pad);
     p.target_logit = take(4 * p.rows_pad);
     p.losses = take(4 * rows);
   } else {
@@ -951,9 +1111,9 @@ LossPlan loss_plan(int64_t rows, int64_t vocab, int64_t width, int dtype, bool b
     p.piece = round_up((p.vocab_pad + pieces - 1) / pieces, kTile);
     for (int k = 0; k < parts; ++k) p.p[k] = take(2 * p.rows_pad * p.piece);
     const int64_t tiles_d = (width + kTile - 1) / kTile;
-    p.splits_h = choose_splits(tiles_d * (p.rows_pad / kTile), p.piece);
+    p.splits_h = choose_splits(tiles_d * (p.rows_pad / kTile), p.piece, p.split ? 3 : 1, false);
     p.dh = take(4 * p.splits_h * p.rows_pad * p.width_pad);
-    p.splits_w = choose_splits(tiles_d * (p.piece / kTile), p.rows_pad);
+    p.splits_w = choose_splits(tiles_d * (p.piece / kTile), p.rows_pad, p.split ? 3 : 1, true);
     if (p.splits_w > 1) p.dw = take(4 * p.splits_w * p.piece * p.width_pad);
   }
   p.bytes = at;
@@ -1018,24 +1178,39 @@ void loss_forward(const Call& c, const void* targets, int target_bytes, int64_t 
   hipLaunchKernelGGL(attnres_loss_rows_kernel, dim3(1), dim3(kScanThreads), 0, c.stream, targets, target_bytes, c.rows, c.vocab,
                      ignore_index, c.saved);
   if (c.rows > 0) {
-    LogitArgs g{};
-    prepare_operands<X>(c, true, &g.product.b, &g.product.a);
-    g.product.count = &c.saved.header->count;
-    g.product.depth = p.width_pad;
-    g.product.tiles_a = static_cast<int>(p.vocab_pad / kTile);
-    g.product.tiles_b = static_cast<int>(p.rows_pad / kTile);
-    g.product.splits = 1;
-    g.header = c.saved.header;
-    g.target = c.saved.target;
-    g.vocab = c.vocab;
-    g.row_tiles = p.rows_pad;
-    g.sums = c.at<f32x2>(p.sums);
-    g.target_logit = c.at<float>(p.target_logit);
-    hipLaunchKernelGGL((attnres_loss_logits_kernel<T, SEGMENTS>), dim3(g.product.tiles_a * g.product.tiles_b), dim3(kThreads), 0,
-                       c.stream, g);
+    f32x2* sums = c.at<f32x2>(p.sums);
+    float* target_logit = c.at<float>(p.target_logit);
+    int tiles;
+    int64_t row_tiles;
+    if (c.rows <= kFewRows) {
+      tiles = static_cast<int>((c.vocab + kFewWords - 1) / kFewWords);
+      row_tiles = kFewRows;
+      const FewArgs<X> g{static_cast<const X*>(c.hidden), static_cast<const X*>(c.weight), c.hidden_stride, c.weight_stride, c.vocab,
+                         static_cast<int>(c.width), c.saved, sums, target_logit};
+      const auto kernel = c.rows <= 16   ? attnres_loss_few_kernel<X, 1>
+                          : c.rows <= 32 ? attnres_loss_few_kernel<X, 2>
+                                         : attnres_loss_few_kernel<X, 4>;
+      hipLaunchKernelGGL(kernel, dim3(tiles), dim3(kBlock), 0, c.stream, g);
+    } else {
+      LogitArgs g{};
+      prepare_operands<X>(c, true, &g.product.b, &g.product.a);
+      g.product.count = &c.saved.header->count;
+      g.product.depth = p.width_pad;
+      g.product.tiles_a = tiles = static_cast<int>(p.vocab_pad / kTile);
+      g.product.tiles_b = static_cast<int>(p.rows_pad / kTile);
+      g.product.splits = 1;
+      g.header = c.saved.header;
+      g.target = c.saved.target;
+      g.vocab = c.vocab;
+      g.row_tiles = row_tiles = p.rows_pad;
+      g.sums = sums;
+      g.target_logit = target_logit;
+      hipLaunchKernelGGL((attnres_loss_logits_kernel<T, SEGMENTS>), dim3(g.product.tiles_a * g.product.tiles_b), dim3(kThreads), 0,
+                         c.stream, g);
+    }
     float* losses = reduction == ATTNRES_REDUCE_NONE ? loss : c.at<float>(p.losses);
-    hipLaunchKernelGGL(attnres_loss_reduce_kernel, dim3(static_cast<unsigned>((c.rows + 63) / 64)), dim3(kBlock), 0, c.stream, g.sums,
-                       g.product.tiles_a, p.rows_pad, g.target_logit, c.rows, c.saved, losses);
+    hipLaunchKernelGGL(attnres_loss_reduce_kernel, dim3(static_cast<unsigned>((c.rows + kReduceRows - 1) / kReduceRows)), dim3(kBlock), 0,
+                       c.stream, sums, tiles, row_tiles, target_logit, c.rows, c.saved, losses);
   }
   if (reduction != ATTNRES_REDUCE_NONE) {
     hipLaunchKernelGGL(attnres_loss_total_kernel, dim3(1), dim3(kScanThreads), 0, c.stream, c.at<const float>(p.losses), c.rows,
@@ -1048,7 +1223,7 @@ void loss_backward(const Call& c, int reduction, const float* grad_loss, void* g
   const LossPlan& p = c.plan;
   constexpr int kParts = SEGMENTS == 3 ? 2 : 1;
   Operand h{}, w{};
-  prepare_operands<X>(c, false, &h, &w);
+  prepare_operands<X>(c, c.rows <= kFewRows, &h, &w);  // whose forward needed no scales
   const float p_scale = std::is_same_v<T, Bf16> ? 1.0f : kProbabilityScale;
   float* alpha = c.at<float>(p.alpha);
   float* row_scale = c.at<float>(p.row_scale);
