@@ -911,9 +911,9 @@ def run_model(cfg: dict, steps: int, warmup: int, variant: str = "both", autocas
     """model / model_block / model_ref: training steps of the causal LM (benchmarks/model.py).
 
     ``variant`` "both" times the plain step (the line's value), then the
-    source-bank step with gathered gradients, with accumulated gradients and
-    with inductor-compiled sublayers; "plain", "bank", "bank_accumulate" or
-    "bank_compiled" times one of them alone (for traces), "compiled" the plain
+    source-bank step with gathered gradients, with accumulated gradients, with
+    inductor-compiled sublayers and with the layers of attnres.layers; "plain", "bank",
+    "bank_accumulate", "bank_compiled" or "bank_fused" times one of them alone (for traces), "compiled" the plain
     model under whole-model inductor compilation, "graph" the whole step
     (compiled model and loss under BF16 autocast, fused capturable AdamW)
     captured in one HIP graph and replayed (benchmarks/training_graph.py). A
@@ -933,10 +933,10 @@ def run_model(cfg: dict, steps: int, warmup: int, variant: str = "both", autocas
     tokens = torch.randint(config.vocab, (config.batch, config.sequence), device="cuda", generator=generator)
     targets = torch.roll(tokens, -1, dims=1)
 
-    def time_steps(source_bank, bank_gradients="gather", compiled=False, compile_layers=False):
+    def time_steps(source_bank, bank_gradients="gather", compiled=False, compile_layers=False, fused_layers=False):
         torch.manual_seed(0)
         model = make_model(config, backend="kernel", source_bank=source_bank, bank_gradients=bank_gradients,
-                           compile_layers=compile_layers).cuda()
+                           compile_layers=compile_layers, fused_layers=fused_layers).cuda()
         optimizer = torch.optim.AdamW(model.parameters(), lr=1e-4, fused=cfg.get("fused_adamw", False))
         if compiled:  # inductor around the model; the reads stay opaque custom ops
             torch._dynamo.reset()
@@ -1006,6 +1006,7 @@ def run_model(cfg: dict, steps: int, warmup: int, variant: str = "both", autocas
     comp_ms, comp_loss = time_steps(False, compiled=True) if variant == "compiled" else (None, None)
     bc_ms, bc_loss = (time_steps(True, compile_layers=True) if variant in ("both", "bank_compiled")
                       else (None, None))
+    bf_ms, bf_loss = (time_steps(True, fused_layers=True) if variant in ("both", "bank_fused") else (None, None))
     inference_ms = time_inference(False) if variant == "both" else None
     inference_bank_ms = time_inference(True) if variant == "both" else None
 
@@ -1017,7 +1018,7 @@ def run_model(cfg: dict, steps: int, warmup: int, variant: str = "both", autocas
 
     timed_name, timed_ms = next(((name, t) for name, t in (("plain", ms), ("graph", graph_ms), ("compiled", comp_ms),
                                                             ("bank", bank_ms), ("bank_accumulate", acc_ms),
-                                                            ("bank_compiled", bc_ms)) if t is not None), (None, None))
+                                                            ("bank_compiled", bc_ms), ("bank_fused", bf_ms)) if t is not None), (None, None))
     counts = read_sources_per_step(config)
     reads = len(counts)
     read_bytes_per_step = sum(sum(read_bytes(s, n_tokens, config.width)) for s in counts)
@@ -1048,6 +1049,9 @@ def run_model(cfg: dict, steps: int, warmup: int, variant: str = "both", autocas
         # the source-bank step with each sublayer compiled by inductor (regional compilation)
         "source_bank_compiled_layers": {"ms_per_step": rounded(bc_ms, 3), "tokens_per_s": rate(bc_ms),
                                         "loss": rounded(bc_loss, 4)},
+        # the source-bank step with embedding, layer norms and loss from attnres.layers
+        "source_bank_fused_layers": {"ms_per_step": rounded(bf_ms, 3), "tokens_per_s": rate(bf_ms),
+                                     "loss": rounded(bf_loss, 4)},
         # --model-variant compiled: the plain model under torch.compile(fullgraph=True) (inductor)
         "compiled": {"ms_per_step": rounded(comp_ms, 3), "tokens_per_s": rate(comp_ms), "loss": rounded(comp_loss, 4)},
         # --model-variant graph: the whole step captured in one HIP graph (BF16 autocast)
@@ -1074,10 +1078,12 @@ def main(argv=None) -> int:
                         help="--config model / model_block: run the steps under torch.autocast (BF16), as the "
                              "reference's 24-layer timings do")
     parser.add_argument("--model-variant",
-                        choices=("both", "plain", "bank", "bank_accumulate", "bank_compiled", "compiled", "graph"),
+                        choices=("both", "plain", "bank", "bank_accumulate", "bank_compiled", "bank_fused", "compiled",
+                                 "graph"),
                         default="both",
                         help="--config model / model_block: time the plain step, the source-bank step (gathered "
-                             "or accumulated gradients, or with compiled sublayers), all four (both), or the plain "
+                             "or accumulated gradients, or with compiled sublayers, or with the layers of "
+                             "attnres.layers), all five (both), or the plain "
                              "model under inductor")
     args = parser.parse_args(argv)
 

@@ -30,6 +30,12 @@ slot of its own; ``push_sum`` forms the partial and its BF16 copy in one
 kernel (the caller step of reference model.py:333 fused with the next read's
 cast), and the block's last partial is written straight into the next
 completed slot.
+
+``fused_layers=True`` (HIP backend; no reference counterpart) takes the layers
+around the reads from ``attnres.layers``: the token and position lookup in one
+kernel with its gradient by sorted tokens, the layer norms, and the LM head
+with the cross entropy (``CausalAttnResLM.loss``, which ``training_step``
+calls), which never stores the logits.  The weights are the same parameters.
 """
 
 from __future__ import annotations
@@ -101,10 +107,11 @@ def block_ends(events: int, blocks: int) -> tuple[int, ...]:
 class TransformerLayer(nn.Module):
     """Pre-norm causal self-attention and a SwiGLU MLP, as two sublayers."""
 
-    def __init__(self, config: TrainingConfig) -> None:
+    def __init__(self, config: TrainingConfig, fused_layers: bool = False) -> None:
         super().__init__()
         d = config.width
         self.heads = config.heads
+        self.fused_layers = fused_layers
         self.attn_norm = nn.LayerNorm(d)
         self.qkv = nn.Linear(d, 3 * d, bias=False)
         self.attn_out = nn.Linear(d, d, bias=False)
@@ -112,15 +119,22 @@ class TransformerLayer(nn.Module):
         self.gate_up = nn.Linear(d, 2 * config.ffn, bias=False)
         self.down = nn.Linear(config.ffn, d, bias=False)
 
+    def _norm(self, norm: nn.LayerNorm, x: Tensor) -> Tensor:
+        if not self.fused_layers:
+            return norm(x)
+        from attnres.layers import layer_norm
+
+        return layer_norm(x, norm.weight, norm.bias, eps=norm.eps)
+
     def attention(self, x: Tensor) -> Tensor:
         b, t, d = x.shape
-        q, k, v = self.qkv(self.attn_norm(x)).view(b, t, 3, self.heads, d // self.heads).unbind(2)
+        q, k, v = self.qkv(self._norm(self.attn_norm, x)).view(b, t, 3, self.heads, d // self.heads).unbind(2)
         y = F.scaled_dot_product_attention(q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2),
                                            is_causal=True)
         return self.attn_out(y.transpose(1, 2).reshape(b, t, d))
 
     def mlp(self, x: Tensor) -> Tensor:
-        gate, up = self.gate_up(self.mlp_norm(x)).chunk(2, dim=-1)
+        gate, up = self.gate_up(self._norm(self.mlp_norm, x)).chunk(2, dim=-1)
         return self.down(F.silu(gate) * up)
 
 
@@ -128,19 +142,22 @@ class CausalAttnResLM(nn.Module):
     """Small causal Transformer with Full or Block AttnRes residual reads."""
 
     def __init__(self, config: TrainingConfig, backend: Backend = "kernel", *, source_bank: bool = False,
-                 bank_gradients: str = "gather", compile_layers: bool = False) -> None:
+                 bank_gradients: str = "gather", compile_layers: bool = False, fused_layers: bool = False) -> None:
         super().__init__()
         if source_bank and backend != "kernel":
             raise ValueError("source_bank needs the HIP backend")
+        if fused_layers and backend != "kernel":
+            raise ValueError("fused_layers needs the HIP backend")
         if bank_gradients not in ("gather", "accumulate"):
             raise ValueError("bank_gradients must be 'gather' or 'accumulate'")
         self.config = config
         self.backend = backend
         self.source_bank = bool(source_bank)
         self.bank_gradients = bank_gradients
+        self.fused_layers = bool(fused_layers)
         self.token_embedding = nn.Embedding(config.vocab, config.width)
         self.position_embedding = nn.Parameter(torch.empty(config.sequence, config.width))
-        self.layers = nn.ModuleList(TransformerLayer(config) for _ in range(config.layers))
+        self.layers = nn.ModuleList(TransformerLayer(config, self.fused_layers) for _ in range(config.layers))
         self.lm_head = nn.Linear(config.width, config.vocab, bias=False)
         # one query per read: before sublayers 2 .. 2L and before the LM head
         self.queries = nn.ParameterList(nn.Parameter(torch.empty(config.rank)) for _ in range(2 * config.layers))
@@ -254,31 +271,56 @@ class CausalAttnResLM(nn.Module):
             partial = None
         return self.read(completed, self.queries[-1])
 
-    def forward(self, tokens: Tensor) -> Tensor:
+    def _embed(self, tokens: Tensor) -> Tensor:
+        # the stream in the autocast dtype (model.py:243-244)
+        autocast = torch.is_autocast_enabled(tokens.device.type)
+        dtype = torch.get_autocast_dtype(tokens.device.type) if autocast else None
+        if self.fused_layers:
+            from attnres.layers import embedding
+
+            return embedding(tokens, self.token_embedding.weight, self.position_embedding, dtype=dtype)
+        embedded = self.token_embedding(tokens) + self.position_embedding[: tokens.shape[1]]
+        return embedded if dtype is None else embedded.to(dtype)
+
+    def hidden(self, tokens: Tensor) -> Tensor:
+        """The last read of the residual stream, which the LM head projects."""
         if tokens.ndim != 2:
             raise ValueError("tokens must have shape [batch, sequence]")
         if tokens.dtype.is_floating_point or tokens.dtype == torch.bool:
             raise TypeError("tokens must contain integer token ids")
         if tokens.shape[1] > self.config.sequence:
             raise ValueError("token sequence exceeds configured sequence length")
-        embedded = self.token_embedding(tokens) + self.position_embedding[: tokens.shape[1]]
-        if torch.is_autocast_enabled(embedded.device.type):  # the stream in the autocast dtype (model.py:243-244)
-            embedded = embedded.to(torch.get_autocast_dtype(embedded.device.type))
-        hidden = self._forward_full(embedded) if self.config.mode == "full" else self._forward_block(embedded)
-        return self.lm_head(hidden)
+        embedded = self._embed(tokens)
+        return self._forward_full(embedded) if self.config.mode == "full" else self._forward_block(embedded)
+
+    def forward(self, tokens: Tensor) -> Tensor:
+        return self.lm_head(self.hidden(tokens))
+
+    def loss(self, tokens: Tensor, targets: Tensor) -> Tensor:
+        """Mean cross entropy of the targets (those equal to -100 left out); with ``fused_layers``
+        without storing the logits."""
+        if not self.fused_layers:
+            logits = self(tokens)
+            return F.cross_entropy(logits.reshape(-1, logits.shape[-1]).float(), targets.reshape(-1))
+        from attnres.layers import linear_cross_entropy
+
+        hidden = self.hidden(tokens)
+        return linear_cross_entropy(hidden, self.lm_head.weight.to(hidden.dtype), targets)
 
 
 def make_model(config: TrainingConfig, backend: Backend = "kernel", *, source_bank: bool = False,
-               bank_gradients: str = "gather", compile_layers: bool = False) -> CausalAttnResLM:
+               bank_gradients: str = "gather", compile_layers: bool = False,
+               fused_layers: bool = False) -> CausalAttnResLM:
     """Construct a model with the given residual-read backend (``bank_gradients``:
     the source bank's gradient path, see ``attnres.SourceBank``; ``compile_layers``:
-    each attention and MLP sublayer under ``torch.compile(fullgraph=True)``)."""
+    each attention and MLP sublayer under ``torch.compile(fullgraph=True)``;
+    ``fused_layers``: the layers around the reads from ``attnres.layers``)."""
     if not isinstance(config, TrainingConfig):
         raise TypeError("config must be a TrainingConfig")
     if not (backend == "kernel" or callable(backend)):
         raise ValueError("backend must be 'kernel' or a callable")
     return CausalAttnResLM(config, backend, source_bank=source_bank, bank_gradients=bank_gradients,
-                           compile_layers=compile_layers)
+                           compile_layers=compile_layers, fused_layers=fused_layers)
 
 
 def training_step(model: nn.Module, optimizer: torch.optim.Optimizer, tokens: Tensor, targets: Tensor,
@@ -303,8 +345,11 @@ def training_step(model: nn.Module, optimizer: torch.optim.Optimizer, tokens: Te
     optimizer.zero_grad(set_to_none=True)
     losses = []
     for micro_tokens, micro_targets in batches:
-        logits = model(micro_tokens)
-        loss = F.cross_entropy(logits.reshape(-1, logits.shape[-1]).float(), micro_targets.reshape(-1))
+        if getattr(model, "fused_layers", False):
+            loss = model.loss(micro_tokens, micro_targets)
+        else:
+            logits = model(micro_tokens)
+            loss = F.cross_entropy(logits.reshape(-1, logits.shape[-1]).float(), micro_targets.reshape(-1))
         losses.append(loss.detach())
         (loss / len(batches)).backward()
     optimizer.step()
