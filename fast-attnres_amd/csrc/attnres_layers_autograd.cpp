@@ -7,6 +7,8 @@
 
 #include <torch/extension.h>
 
+#include <torch/csrc/autograd/functions/basic_ops.h>
+
 #include "attnres_layers_hip.h"
 #include "attnres_nodes.h"
 
@@ -45,6 +47,23 @@ Rows rows_view(const Tensor& tensor) {
   if (const std::optional<int64_t> stride = row_stride(tensor)) return {tensor, *stride};
   Tensor copy = tensor.contiguous();
   return {copy, copy.size(-1)};
+}
+
+// First-order gradients: in a backward pass that is itself recorded (create_graph), differentiating the
+// gradients again raises instead of leaving these layers' terms out.
+variable_list once_differentiable(variable_list grads) {
+  if (!at::GradMode::is_enabled()) return grads;
+  variable_list defined;
+  for (const Tensor& grad : grads) {
+    if (grad.defined()) defined.push_back(grad.detach().requires_grad_(true));
+  }
+  torch::autograd::DelayedError error("attnres layers have first-order gradients only", static_cast<int64_t>(defined.size()));
+  const variable_list marked = error.apply(std::move(defined));
+  size_t next = 0;
+  for (Tensor& grad : grads) {
+    if (grad.defined()) grad = marked[next++];
+  }
+  return grads;
 }
 
 // -------------------------------------------------------------- layer norm
@@ -119,7 +138,7 @@ struct LayerNorm : public torch::autograd::Function<LayerNorm> {
     if (want_x) result[0] = grad_x;
     if (want_weight) result[1] = grad_weight;
     if (want_bias) result[2] = grad_bias;
-    return result;
+    return once_differentiable(std::move(result));
   }
 };
 
@@ -202,7 +221,7 @@ struct Embedding : public torch::autograd::Function<Embedding> {
         want_positions);
     if (want_weight) result[0] = grad_weight;
     if (want_positions) result[1] = grad_positions;
-    return result;
+    return once_differentiable(std::move(result));
   }
 };
 
@@ -303,7 +322,7 @@ struct LinearCrossEntropy : public torch::autograd::Function<LinearCrossEntropy>
                                                           ctx->saved_data["reduction"].toInt(), want_hidden, want_weight);
     if (want_hidden) result[0] = grad_hidden;
     if (want_weight) result[1] = grad_weight;
-    return result;
+    return once_differentiable(std::move(result));
   }
 };
 

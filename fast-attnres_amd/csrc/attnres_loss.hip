@@ -1371,12 +1371,12 @@ int attnres_hip_loss_forward(const void* hidden, int64_t hidden_stride, const vo
 }
 
 int attnres_hip_loss_backward(const void* hidden, int64_t hidden_stride, const void* weight, int64_t weight_stride, int64_t rows,
-                              int64_t vocab, int64_t width, int dtype, int reduction, const void* saved, const float* grad_loss,
+                              int64_t vocab, int64_t width, int dtype, int reduction, void* saved, const float* grad_loss,
                               void* grad_hidden, void* grad_weight, void* workspace, int64_t workspace_bytes, void* stream) {
   if (const int status = check_loss(hidden, hidden_stride, weight, weight_stride, rows, vocab, width, dtype, reduction)) return status;
   if (saved == nullptr || grad_loss == nullptr) return layer_error(ATTNRES_ERR_NULL_POINTER, "saved or grad_loss is NULL");
   const Call c{hidden, hidden_stride, weight, weight_stride, rows, vocab, width, loss_plan(rows, vocab, width, dtype, true),
-               saved_views(const_cast<void*>(saved), rows), static_cast<char*>(workspace), static_cast<hipStream_t>(stream)};
+               saved_views(saved, rows), static_cast<char*>(workspace), static_cast<hipStream_t>(stream)};
   if (workspace == nullptr || workspace_bytes < c.plan.bytes) {
     return layer_error(ATTNRES_ERR_WORKSPACE, "workspace of %lld bytes, %lld needed", (long long)workspace_bytes,
                        (long long)c.plan.bytes);

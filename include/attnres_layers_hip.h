@@ -82,7 +82,8 @@ int attnres_hip_embedding_backward(const void* grad_out, int out_dtype, const vo
  * when none does).  A target that is neither ignore_index nor in 0..vocab-1 makes
  * the loss and the gradients NaN.  The logits are never stored: FP32 sums of exponentials in
  * pieces of the vocabulary, formed again in the backward.
- * saved: attnres_hip_loss_saved_bytes(rows) bytes that the backward reads. */
+ * saved: attnres_hip_loss_saved_bytes(rows) bytes that the backward reads (and completes, with
+ * the same values every time, where a forward of few FP32 rows needed less). */
 int64_t attnres_hip_loss_saved_bytes(int64_t rows);
 int64_t attnres_hip_loss_workspace_bytes(int64_t rows, int64_t vocab, int64_t width, int dtype, int backward);
 
@@ -94,7 +95,7 @@ int attnres_hip_loss_forward(const void* hidden, int64_t hidden_stride, const vo
 /* grad_loss (FP32): one value, or [rows] for ATTNRES_REDUCE_NONE.  grad_hidden
  * [rows, width] and grad_weight [vocab, width] contiguous, of dtype; either may be NULL. */
 int attnres_hip_loss_backward(const void* hidden, int64_t hidden_stride, const void* weight, int64_t weight_stride,
-                              int64_t rows, int64_t vocab, int64_t width, int dtype, int reduction, const void* saved,
+                              int64_t rows, int64_t vocab, int64_t width, int dtype, int reduction, void* saved,
                               const float* grad_loss, void* grad_hidden, void* grad_weight, void* workspace,
                               int64_t workspace_bytes, void* stream);
 

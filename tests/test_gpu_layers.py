@@ -70,6 +70,14 @@ def test_layer_norm_many_rows():
         _check_norm(x, _randn(g, width), _randn(g, width), _randn(g, rows, width).to(BF16))
 
 
+@pytest.mark.parametrize("rows,width,dtype", [(20001, 3331, BF16), (9000, 4099, FP32)])
+def test_layer_norm_of_results_past_the_caches(rows, width, dtype):
+    """Results of more than 128 MiB, of rows that no store is aligned to."""
+    g = _generator(rows)
+    x = _randn(g, rows, width).to(dtype)
+    _check_norm(x, _randn(g, width), _randn(g, width), _randn(g, rows, width).to(dtype))
+
+
 @pytest.mark.parametrize("layout", ["slice", "offset", "transposed", "expanded", "vector", "steps"])
 @pytest.mark.parametrize("dtype", [BF16, FP32])
 def test_layer_norm_layouts(layout, dtype):
@@ -246,6 +254,24 @@ def test_loss_in_several_pieces_of_the_vocabulary():
     _check_loss(hidden, weight, targets, "mean", g)
 
 
+def test_loss_fp32_in_several_pieces_of_the_vocabulary():
+    g, hidden, weight, targets = _loss_inputs(39, 1900, 40, 70001, FP32, 0.1)
+    _check_loss(hidden, weight, targets, "none", g)
+
+
+@pytest.mark.parametrize("rows", [15, 16, 17, 32, 33, 63, 64, 65])
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+def test_loss_around_the_forward_of_few_rows(rows, dtype):
+    for width, vocab, ignored in ((72, 63, 0.0), (1000, 130, 0.5)):
+        g, hidden, weight, targets = _loss_inputs(rows + width, rows, width, vocab, dtype, ignored)
+        _check_loss(hidden, weight, targets, "none", g)
+
+
+def test_loss_of_one_token_without_axes():
+    g, hidden, weight, targets = _loss_inputs(40, 1, 64, 50, BF16)
+    _check_loss(hidden[0].detach(), weight, targets[0], "mean", g)
+
+
 def test_loss_of_no_targets():
     g, hidden, weight, targets = _loss_inputs(41, 300, 64, 500, BF16)
     targets.fill_(-100)
@@ -372,6 +398,49 @@ def test_loss_gradient_against_differences():
     # moved FP32 inputs are rounded: 2^-24 of |h| and |w| along the gradient, below 1e-6 in the loss
     difference = slope(lambda h, w: layers.linear_cross_entropy(h, w, targets), hidden.detach(), weight.detach())
     assert abs(difference - length) <= left_out + (1e-5 + 1e-6) / step
+
+
+# ------------------------------------------------------------ autograd's other ways
+
+def _each_layer(leaf):
+    """The three layers as functions of one leaf [4, 64]."""
+    tokens = torch.tensor([[0, 3, 1, 1]], device="cuda")
+    yield lambda: layers.layer_norm(leaf)
+    yield lambda: layers.embedding(tokens, leaf)
+    yield lambda: layers.linear_cross_entropy(leaf, leaf.detach().clone(), tokens[0])
+
+
+def test_differentiating_the_gradients_again_is_refused():
+    leaf = _randn(_generator(131), 4, 64).requires_grad_(True)
+    for call in _each_layer(leaf):
+        (grad,) = torch.autograd.grad(call().sum(), leaf, create_graph=True)
+        (plain,) = torch.autograd.grad(call().sum(), leaf)
+        assert torch.equal(grad.detach(), plain)
+        with pytest.raises(RuntimeError, match="first-order"):
+            grad.square().sum().backward()
+
+
+def test_inference_mode_and_recomputation():
+    from torch.utils.checkpoint import checkpoint
+
+    leaf = _randn(_generator(137), 4, 64).requires_grad_(True)
+    for call in _each_layer(leaf):
+        out = call()
+        with torch.inference_mode():
+            assert torch.equal(call(), out)
+        (expected,) = torch.autograd.grad(out.sum(), leaf, retain_graph=True)
+        (again,) = torch.autograd.grad(out.sum(), leaf)
+        (recomputed,) = torch.autograd.grad(checkpoint(call, use_reentrant=False).sum(), leaf)
+        assert torch.equal(again, expected) and torch.equal(recomputed, expected)
+
+
+def test_inputs_changed_before_the_backward_are_refused():
+    weight = _randn(_generator(139), 64).requires_grad_(True)
+    x = _randn(_generator(140), 4, 64)
+    out = layers.layer_norm(x, weight)
+    x.add_(1.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        out.sum().backward()
 
 
 # ----------------------------------------------------------- streams, capture
