@@ -730,22 +730,42 @@ __global__ void __launch_bounds__(kScanThreads) attnres_loss_rows_kernel(const v
 }
 
 // ------------------------------------------------------------------- few rows
-// The forward of up to kFewRows rows reads W once and is bound by that: 64 words per workgroup, 16
-// per wavefront, W and H straight to registers as they lie (any width and alignment; FP32 inputs
-// by FP32 matrix instructions, which the few rows have time for), no packing.  A lane holds 16 consecutive k's of its
-// word or row per 64; the order of the k's in a matrix instruction is of no account, as both operands share it.
+// The forward of few rows (few_rows()) reads W once and is bound by that.  A workgroup takes 128 words, 32 to four
+// wavefronts, which share the k's (so that all of W is asked for at once); W and H go straight to registers as
+// they lie (any width and alignment; FP32 inputs by FP32 matrix instructions, which the few rows have time for),
+// no packing: a row's logits are its own, so ignored rows are worked on and left out afterwards.  A
+// lane holds 16 bytes of every 64 of its word or row; the order of the k's in a matrix instruction is of no
+// account, as both operands share it.  16 rows of a 32768 x 1024 BF16 vocabulary (67 MB): 17.6 us, 3.8 TB/s (by 256 x
+// 256 tiles 27 us and 8 for packing).
 constexpr int kFewRows = 64;
-constexpr int kFewWords = 64;
+constexpr int kFewWords = 128;                        // of a workgroup; 32 to a wavefront
+constexpr int kFewParts = 4;                          // of the k's
+constexpr int kFewBlock = kFewWords / 32 * kFewParts * 64;
 
 template <class X>
-struct FewChunk {  // 16 consecutive elements, as they lie
-  u32x4 w[sizeof(X)];
-  __device__ __forceinline__ void load(const X* row, int k, int width) {
-    Chunk<X> a, b;
-    a.load(row, k, width);
-    b.load(row, k + kVec, width);
+struct FewChunk {  // a lane's 16 of 64 k's, as they lie: 16 bytes of every 64
+  static constexpr int kPieces = sizeof(X);
+  static constexpr int kPiece = 16 / sizeof(X);
+  u32x4 w[kPieces];
+  __device__ __forceinline__ void load(const X* row, int k0, int group, int width) {
 #pragma unroll
-    for (size_t i = 0; i < sizeof(X) / 2; ++i) w[i] = a.w[i], w[sizeof(X) / 2 + i] = b.w[i];
+    for (int i = 0; i < kPieces; ++i) {
+      const int k = k0 + (i * 4 + group) * kPiece;
+      if (k + kPiece <= width) {
+        w[i] = reinterpret_cast<const Raw16*>(row + k)->v;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if constexpr (std::is_same_v<X, float>) {
+            w[i][e] = k + e < width ? __float_as_uint(row[k + e]) : 0;
+          } else {
+            const uint32_t lo = k + 2 * e < width ? row[k + 2 * e].bits : 0;
+            const uint32_t hi = k + 2 * e + 1 < width ? row[k + 2 * e + 1].bits : 0;
+            w[i][e] = hi << 16 | lo;
+          }
+        }
+      }
+    }
   }
 };
 
@@ -771,87 +791,120 @@ struct FewArgs {
   const X* hidden;
   const X* weight;
   int64_t hidden_stride, weight_stride, vocab;
-  int width;
+  int width, rows;
+  const void* targets;
+  int target_bytes;
+  int64_t ignore_index;
   Saved saved;
   f32x2* sums;          // [workgroups][kFewRows]
   float* target_logit;  // [kFewRows]
 };
 
 template <class X, int TILES>  // of 16 rows
-__global__ void __launch_bounds__(kBlock) attnres_loss_few_kernel(FewArgs<X> g) {
-  __shared__ f32x2 meet[4][TILES * 16];
+__global__ void __launch_bounds__(kFewBlock) attnres_loss_few_kernel(FewArgs<X> g) {
+  __shared__ int target[kFewRows];  // -1: not known or ignored
+  __shared__ f32x4 parts[kFewBlock / 64][64];
+  __shared__ f32x2 meet[kFewWords / 32][TILES * 16];
   const int wave = wave_index(), lane = threadIdx.x % 64, group = lane / 16, entry = lane % 16;
-  const int64_t v0 = static_cast<int64_t>(blockIdx.x) * kFewWords + wave * 16;
-  const X* w = g.weight + min(v0 + entry, g.vocab - 1) * g.weight_stride;
-  constexpr int kSteps = sizeof(X) == 4 || TILES == 4 ? 2 : 4;  // of 64 k's under way together
+  const int part = wave % kFewParts, words = wave / kFewParts;
+  const int64_t v0 = static_cast<int64_t>(blockIdx.x) * kFewWords + words * 32;
+  const X* w[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) w[i] = g.weight + min(v0 + i * 16 + entry, g.vocab - 1) * g.weight_stride;
+  constexpr int kSteps = sizeof(X) == 4 || TILES == 4 ? 1 : 2;  // of 64 k's under way together
   constexpr int kSpan = kSteps * 64;
-  FewChunk<X> next[kSteps];
+  FewChunk<X> next[kSteps][2];
   const auto fetch = [&](int k0) {
 #pragma unroll
-    for (int s = 0; s < kSteps; ++s) next[s].load(w, k0 + s * 64 + group * 16, g.width);
+    for (int s = 0; s < kSteps; ++s) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) next[s][i].load(w[i], k0 + s * 64, group, g.width);
+    }
   };
-  fetch(0);  // before what has to be known of the rows
-  const int count = g.saved.header->count;
-  if (count == 0) return;
+  fetch(part * kSpan);
   const X* h[TILES];
 #pragma unroll
-  for (int t = 0; t < TILES; ++t) {
-    h[t] = g.hidden + g.saved.index[min(t * 16 + entry, count - 1)] * g.hidden_stride;
-  }
-  FewChunk<X> next_h[kSteps][TILES];
-  const auto fetch_h = [&](int k0) {
-#pragma unroll
-    for (int s = 0; s < kSteps; ++s) {
-#pragma unroll
-      for (int t = 0; t < TILES; ++t) next_h[s][t].load(h[t], k0 + s * 64 + group * 16, g.width);
-    }
-  };
-  fetch_h(0);
-  f32x4 acc[TILES] = {};
-  for (int k0 = 0; k0 < g.width; k0 += kSpan) {
-    FewChunk<X> now[kSteps], now_h[kSteps][TILES];
-#pragma unroll
-    for (int s = 0; s < kSteps; ++s) {
-      now[s] = next[s];
-#pragma unroll
-      for (int t = 0; t < TILES; ++t) now_h[s][t] = next_h[s][t];
-    }
-    if (k0 + kSpan < g.width) {
-      fetch(k0 + kSpan);
-      fetch_h(k0 + kSpan);
-    }
-#pragma unroll
-    for (int s = 0; s < kSteps; ++s) {
-#pragma unroll
-      for (int t = 0; t < TILES; ++t) acc[t] = few_mfma<X>(now[s], now_h[s][t], acc[t]);
+  for (int t = 0; t < TILES; ++t) h[t] = g.hidden + min(t * 16 + entry, g.rows - 1) * g.hidden_stride;
+  if (wave == 0) {
+    const int row = min(lane, g.rows - 1);
+    const int64_t t = g.target_bytes == 8 ? static_cast<const int64_t*>(g.targets)[row] : static_cast<const int32_t*>(g.targets)[row];
+    const bool counts = lane < g.rows && t != g.ignore_index;
+    const int known = counts && t >= 0 && t < g.vocab ? static_cast<int>(t) : -1;
+    target[lane] = known;
+    if (blockIdx.x == 0) {
+      const uint64_t all = __ballot(counts);
+      const int at = __popcll(all & ((uint64_t{1} << lane) - 1));
+      if (lane < g.rows) g.saved.packed[lane] = counts ? at : -1;
+      if (counts) g.saved.index[at] = lane, g.saved.target[at] = known;
+      if (lane == 0) *g.saved.header = Header{static_cast<int32_t>(__popcll(all)), {1.0f, 1.0f}, {0, 0}};
     }
   }
-  const int last = static_cast<int>(min(g.vocab - v0, int64_t{16})) - 4 * group;  // entries below it count
+  f32x4 acc[2][TILES] = {};
+  for (int k0 = part * kSpan; k0 < g.width; k0 += kFewParts * kSpan) {
+    FewChunk<X> now[kSteps][2];
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) now[s][i] = next[s][i];
+    }
+    if (k0 + kFewParts * kSpan < g.width) fetch(k0 + kFewParts * kSpan);
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+#pragma unroll
+      for (int t = 0; t < TILES; ++t) {
+        FewChunk<X> b;  // the few rows stay in the caches
+        b.load(h[t], k0 + s * 64, group, g.width);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) acc[i][t] = few_mfma<X>(now[s][i], b, acc[i][t]);
+      }
+    }
+  }
+  // the parts in order, then the words' (maximum, sum) per row
 #pragma unroll
   for (int t = 0; t < TILES; ++t) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      __syncthreads();
+      parts[wave][lane] = acc[i][t];
+      __syncthreads();
+      if (part == 0) {
+#pragma unroll
+        for (int p = 1; p < kFewParts; ++p) acc[i][t] += parts[wave + p][lane];
+      }
+    }
+    if (part != 0) continue;
     const int row = t * 16 + entry;
-    const int64_t from_v0 = g.saved.target[min(row, count - 1)] - v0;
-    const int rel = row < count && from_v0 >= 4 * group && from_v0 < 4 * group + 4 ? static_cast<int>(from_v0) - 4 * group : -1;
-    float top = -__builtin_inff();
+    const int64_t from_v0 = target[row] - v0;  // -1 is before every word
+    float top = -__builtin_inff(), sum = 0.0f;
+    bool counts[2][4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      top = fmaxf(top, e < last ? acc[t][e] : -__builtin_inff());
-      if (e == rel) g.target_logit[row] = acc[t][e];
+    for (int i = 0; i < 2; ++i) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int v = i * 16 + 4 * group + e;
+        counts[i][e] = v0 + v < g.vocab;
+        top = fmaxf(top, counts[i][e] ? acc[i][t][e] : -__builtin_inff());
+        if (from_v0 == v) g.target_logit[row] = acc[i][t][e];
+      }
     }
     top = fmaxf(top, __shfl_xor(top, 16, 64));
     top = fmaxf(top, __shfl_xor(top, 32, 64));
     const float from = top == -__builtin_inff() ? 0.0f : top;
-    float sum = 0.0f;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) sum += e < last ? __expf(acc[t][e] - from) : 0.0f;
+    for (int i = 0; i < 2; ++i) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sum += counts[i][e] ? __expf(acc[i][t][e] - from) : 0.0f;
+    }
     sum += __shfl_xor(sum, 16, 64);
     sum += __shfl_xor(sum, 32, 64);
-    if (lane < 16) meet[wave][row] = f32x2{top, sum};
+    if (lane < 16) meet[words][row] = f32x2{top, sum};
   }
   __syncthreads();
   if (threadIdx.x < TILES * 16) {
-    g.sums[static_cast<int64_t>(blockIdx.x) * kFewRows + threadIdx.x] =
-        join(join(meet[0][threadIdx.x], meet[1][threadIdx.x]), join(meet[2][threadIdx.x], meet[3][threadIdx.x]));
+    f32x2 sum = meet[0][threadIdx.x];
+#pragma unroll
+    for (int k = 1; k < kFewWords / 32; ++k) sum = join(sum, meet[k][threadIdx.x]);
+    g.sums[static_cast<int64_t>(blockIdx.x) * kFewRows + threadIdx.x] = sum;
   }
 }
 
@@ -933,21 +986,22 @@ __global__ void __launch_bounds__(kBlock) attnres_loss_pack_kernel(const X* __re
   }
 }
 
-// Per row of the input: its log-sum from the tiles' sums, and its loss.  4 rows by 64 parts
+// Per row of the input: its log-sum from the tiles' sums (by packed row, or by row), and its loss.  4 rows by 64 parts
 // of the tiles per workgroup: with few rows the tiles' sums are long chains, and their latency is all there is.
 constexpr int kReduceRows = 4, kReduceParts = kBlock / kReduceRows;
 
 __global__ void __launch_bounds__(kBlock) attnres_loss_reduce_kernel(const f32x2* __restrict__ sums, int tiles, int64_t row_tiles,
-                                                                     const float* __restrict__ target_logit, int64_t rows, Saved s,
-                                                                     float* __restrict__ loss) {
+                                                                     const float* __restrict__ target_logit, int64_t rows, bool packed,
+                                                                     Saved s, float* __restrict__ loss) {
   __shared__ f32x2 part[kBlock / 64][kReduceRows];
   const int64_t row = static_cast<int64_t>(blockIdx.x) * kReduceRows + threadIdx.x % kReduceRows;
   const int which = threadIdx.x / kReduceRows;
   const int at = row < rows ? s.packed[row] : -1;
+  const int64_t column = packed ? at : row;  // of the sums
   f32x2 total = {-__builtin_inff(), 0.0f};
   if (at >= 0) {
 #pragma unroll 8
-    for (int t = which; t < tiles; t += kReduceParts) total = join(total, sums[static_cast<int64_t>(t) * row_tiles + at]);
+    for (int t = which; t < tiles; t += kReduceParts) total = join(total, sums[static_cast<int64_t>(t) * row_tiles + column]);
   }
 #pragma unroll
   for (int step = kReduceRows; step < 64; step <<= 1) {
@@ -964,7 +1018,7 @@ __global__ void __launch_bounds__(kBlock) attnres_loss_reduce_kernel(const f32x2
   const bool known = s.target[at] >= 0;
   s.stats[at] = f32x2{total.x, known ? 1.0f / total.y : __builtin_nanf("")};
   // the logarithm of the sum by itself: at a probability of one it is the whole loss
-  loss[row] = known ? logf(total.y) + (total.x - target_logit[at]) : __builtin_nanf("");
+  loss[row] = known ? logf(total.y) + (total.x - target_logit[column]) : __builtin_nanf("");
 }
 
 __global__ void __launch_bounds__(kScanThreads) attnres_loss_total_kernel(const float* __restrict__ loss, int64_t rows, const Header* header,
@@ -1073,8 +1127,13 @@ int choose_splits(int64_t tiles, int64_t depth, int segments, bool direct) {
   return best;
 }
 
+// Rows that the forward of few rows takes.  Forward, us, its way -> by tiles, 16 / 32 / 64 rows: BF16, 32768 x 1024
+// 20.8 / 26.4 / 34.6 -> 37, 131072 x 2048 126 / 157 / 212 -> 156; where W has to be packed for the tiles, FP16, 50021 x 1000
+// 31 / 38 / 50 -> 71, FP32, 32768 x 1024 34 / 48 / 80 -> 166.
+int64_t few_rows(bool pack_weight) { return pack_weight ? kFewRows : kFewRows / 2; }
+
 struct LossPlan {
-  bool split, pack_weight;
+  bool split, pack_weight, few;
   int64_t rows_pad, width_pad, vocab_pad, piece;
   int64_t hidden[2], weight[2], sums, target_logit, losses;  // offsets
   int64_t row_scale, alpha, p[2], dh, dw;
@@ -1096,7 +1155,8 @@ LossPlan loss_plan(int64_t rows, int64_t vocab, int64_t width, int dtype, bool b
     at += round_up(bytes, 256);
     return from;
   };
-  const bool few = !backward && rows <= kFewRows;
+  p.few = rows <= few_rows(p.pack_weight);
+  const bool few = !backward && p.few;
   if (!few) {
     for (int k = 0; k < parts; ++k) p.hidden[k] = take(2 * p.rows_pad * p.width_pad);
     for (int k = 0; p.pack_weight && k < parts; ++k) p.weight[k] = take(2 * vocab * p.width_pad);
@@ -1177,22 +1237,25 @@ void prepare_operands(const Call& c, bool find_scales, Operand* h, Operand* w) {
 template <class X, class T, int SEGMENTS>
 void loss_forward(const Call& c, const void* targets, int target_bytes, int64_t ignore_index, int reduction, float* loss) {
   const LossPlan& p = c.plan;
-  hipLaunchKernelGGL(attnres_loss_rows_kernel, dim3(1), dim3(kScanThreads), 0, c.stream, targets, target_bytes, c.rows, c.vocab,
-                     ignore_index, c.saved);
+  if (c.rows == 0 || !p.few) {
+    hipLaunchKernelGGL(attnres_loss_rows_kernel, dim3(1), dim3(kScanThreads), 0, c.stream, targets, target_bytes, c.rows, c.vocab,
+                       ignore_index, c.saved);
+  }
   if (c.rows > 0) {
     f32x2* sums = c.at<f32x2>(p.sums);
     float* target_logit = c.at<float>(p.target_logit);
     int tiles;
     int64_t row_tiles;
-    if (c.rows <= kFewRows) {
+    if (p.few) {
       tiles = static_cast<int>((c.vocab + kFewWords - 1) / kFewWords);
       row_tiles = kFewRows;
       const FewArgs<X> g{static_cast<const X*>(c.hidden), static_cast<const X*>(c.weight), c.hidden_stride, c.weight_stride, c.vocab,
-                         static_cast<int>(c.width), c.saved, sums, target_logit};
+                         static_cast<int>(c.width), static_cast<int>(c.rows), targets, target_bytes, ignore_index, c.saved, sums,
+                         target_logit};
       const auto kernel = c.rows <= 16   ? attnres_loss_few_kernel<X, 1>
                           : c.rows <= 32 ? attnres_loss_few_kernel<X, 2>
                                          : attnres_loss_few_kernel<X, 4>;
-      hipLaunchKernelGGL(kernel, dim3(tiles), dim3(kBlock), 0, c.stream, g);
+      hipLaunchKernelGGL(kernel, dim3(tiles), dim3(kFewBlock), 0, c.stream, g);
     } else {
       LogitArgs g{};
       prepare_operands<X>(c, true, &g.product.b, &g.product.a);
@@ -1212,7 +1275,7 @@ void loss_forward(const Call& c, const void* targets, int target_bytes, int64_t 
     }
     float* losses = reduction == ATTNRES_REDUCE_NONE ? loss : c.at<float>(p.losses);
     hipLaunchKernelGGL(attnres_loss_reduce_kernel, dim3(static_cast<unsigned>((c.rows + kReduceRows - 1) / kReduceRows)), dim3(kBlock), 0,
-                       c.stream, sums, tiles, row_tiles, target_logit, c.rows, c.saved, losses);
+                       c.stream, sums, tiles, row_tiles, target_logit, c.rows, !p.few, c.saved, losses);
   }
   if (reduction != ATTNRES_REDUCE_NONE) {
     hipLaunchKernelGGL(attnres_loss_total_kernel, dim3(1), dim3(kScanThreads), 0, c.stream, c.at<const float>(p.losses), c.rows,
@@ -1225,7 +1288,7 @@ void loss_backward(const Call& c, int reduction, const float* grad_loss, void* g
   const LossPlan& p = c.plan;
   constexpr int kParts = SEGMENTS == 3 ? 2 : 1;
   Operand h{}, w{};
-  prepare_operands<X>(c, c.rows <= kFewRows, &h, &w);  // whose forward needed no scales
+  prepare_operands<X>(c, p.few, &h, &w);  // whose forward needed no scales
   const float p_scale = std::is_same_v<T, Bf16> ? 1.0f : kProbabilityScale;
   float* alpha = c.at<float>(p.alpha);
   float* row_scale = c.at<float>(p.row_scale);
