@@ -104,25 +104,31 @@ __global__ void __launch_bounds__(kBlock) attnres_norm_fwd_kernel(const X* __res
   __shared__ float scratch[2][kBlock / 64][2];
   const int lane = threadIdx.x % LANES, group = threadIdx.x / LANES;
   const int64_t step = static_cast<int64_t>(gridDim.x) * kGroups;
-  int64_t row = static_cast<int64_t>(blockIdx.x) * kGroups + group;
-  if (row >= rows) return;  // part of a workgroup only where its groups share no barrier
+  int64_t base = static_cast<int64_t>(blockIdx.x) * kGroups;
+  // groups of more than a wavefront share row_moments' barrier: as many trips for each, the last one idle for some
+  constexpr bool kShared = LANES > 64 && kGroups > 1;
+  const int64_t until = kShared ? rows : rows - group;
+  if (base >= until) return;
   Chunk<X> next[CH];
+  const auto fetch = [&](int64_t from) {
+    const int64_t at = !kShared || from + group < rows ? from + group : rows - 1;
 #pragma unroll
-  for (int k = 0; k < CH; ++k) next[k].load(x + row * x_stride, (k * LANES + lane) * kVec, width);
+    for (int k = 0; k < CH; ++k) next[k].load(x + at * x_stride, (k * LANES + lane) * kVec, width);
+  };
+  fetch(base);
   float w[CH][kVec], b[CH][kVec];
   load_row<LANES>(weight, lane, width, 1.0f, w);
   load_row<LANES>(bias, lane, width, 0.0f, b);
-  for (int parity = 0; row < rows; row += step, parity ^= 1) {
+  for (int parity = 0; base < until; base += step, parity ^= 1) {
+    const int64_t row = base + group;
     float v[CH][kVec];
 #pragma unroll
     for (int k = 0; k < CH; ++k) next[k].unpack(v[k]);
-    if (row + step < rows) {
-#pragma unroll
-      for (int k = 0; k < CH; ++k) next[k].load(x + (row + step) * x_stride, (k * LANES + lane) * kVec, width);
-    }
+    if (base + step < until) fetch(base + step);
     float mean, square;
     row_moments<LANES>(v, lane, width, scratch[parity], &mean, &square);
     const float rstd = 1.0f / sqrtf(square / static_cast<float>(width) + eps);
+    if (kShared && row >= rows) continue;
     if (stats != nullptr && lane == 0) {
       stats[row] = mean;
       stats[rows + row] = rstd;
@@ -287,8 +293,11 @@ bool past_caches(int64_t rows, int64_t width) {
   return rows * width * static_cast<int64_t>(sizeof(X)) >= kPastCaches;
 }
 
-// Rows of up to 128 elements take 16 lanes, up to 1024 a wavefront, wider ones 256 lanes, in the backward
-// 512 from 2049 elements on: it holds dw and db beside two rows.
+// Rows of up to 128 elements take 16 lanes, up to 1024 a wavefront, wider ones 256 lanes; in the backward 512
+// from 2049 elements on, as it holds dw and db beside two rows; in the forward of 16-bit rows a wavefront up to 2560 and
+// two up to 4096, so that fewer lanes idle past the row's end and fewer rows wait at barriers.  Forward, BF16,
+// 256 lanes -> as here, us: 32768 x 1536 42.4 -> 32.7, 65536 x 2048 111 -> 103, 32768 x 2560 85.2 -> 67.5, x
+// 4096 110 -> 102; FP32 rows of twice the registers: 8192 x 2048 21.8 -> 23.4, so they keep 256 lanes.
 template <int LANES, int CH, class X, class P>
 void launch_fwd(const X* x, int64_t x_stride, int64_t rows, int width, const P* weight, const P* bias, float eps, X* out,
                 float* stats, hipStream_t stream) {
@@ -309,6 +318,12 @@ void norm_forward(const void* x, int64_t x_stride, int64_t rows, int width, cons
   if (width <= 128) return call(launch_fwd<16, 1, X, P>);
   if (width <= 512) return call(launch_fwd<64, 1, X, P>);
   if (width <= 1024) return call(launch_fwd<64, 2, X, P>);
+  if constexpr (sizeof(X) == 2) {
+    if (width <= 1536) return call(launch_fwd<64, 3, X, P>);
+    if (width <= 2048) return call(launch_fwd<64, 4, X, P>);
+    if (width <= 2560) return call(launch_fwd<64, 5, X, P>);
+    if (width <= 4096) return call(launch_fwd<128, 4, X, P>);
+  }
   if (width <= 2048) return call(launch_fwd<256, 1, X, P>);
   if (width <= 4096) return call(launch_fwd<256, 2, X, P>);
   if (width <= 6144) return call(launch_fwd<256, 3, X, P>);
