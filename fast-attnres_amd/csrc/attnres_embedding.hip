@@ -16,8 +16,11 @@ namespace attnres_hip {
 namespace layers {
 namespace {
 
-constexpr int64_t kMaxTokens = int64_t{1} << 30;  // positions are sorted as 32-bit numbers
+// Launches take fewer than 2^32 threads: of 64 tokens per workgroup in the sums, of 8 rows of positions.
+constexpr int64_t kMaxTokens = int64_t{1} << 29;
+constexpr int64_t kMaxPlaces = int64_t{1} << 26;
 constexpr int64_t kMaxVocab = int64_t{1} << 30;
+constexpr int64_t kMaxFwdBlocks = int64_t{1} << 23;
 
 __device__ __forceinline__ int64_t token_at(const void* tokens, int bytes, int64_t i) {
   return bytes == 8 ? static_cast<const int64_t*>(tokens)[i] : static_cast<const int32_t*>(tokens)[i];
@@ -37,23 +40,24 @@ __global__ void __launch_bounds__(kBlock) attnres_embedding_fwd_kernel(const voi
                                                                        O* __restrict__ out, int threads,
                                                                        bool past) {
   const int per_block = kBlock / threads;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * per_block + threadIdx.x / threads;
-  if (row >= rows) return;
-  const int64_t token = token_at(tokens, token_bytes, row);
-  const bool known = token >= 0 && token < vocab;
-  const W* from = weight + (known ? token : 0) * width;
-  const W* place = positions != nullptr ? positions + row % length * width : nullptr;
-  for (int c = (threadIdx.x % threads) * kVec; c < width; c += threads * kVec) {
-    float x[kVec], p[kVec];
-    load_chunk(from, c, width, x);
-    if (place != nullptr) load_chunk(place, c, width, p);
+  for (int64_t row = static_cast<int64_t>(blockIdx.x) * per_block + threadIdx.x / threads; row < rows;
+       row += static_cast<int64_t>(gridDim.x) * per_block) {
+    const int64_t token = token_at(tokens, token_bytes, row);
+    const bool known = token >= 0 && token < vocab;
+    const W* from = weight + (known ? token : 0) * width;
+    const W* place = positions != nullptr ? positions + row % length * width : nullptr;
+    for (int c = (threadIdx.x % threads) * kVec; c < width; c += threads * kVec) {
+      float x[kVec], p[kVec];
+      load_chunk(from, c, width, x);
+      if (place != nullptr) load_chunk(place, c, width, p);
 #pragma unroll
-    for (int e = 0; e < kVec; ++e) {
-      x[e] *= scale;
-      if (place != nullptr) x[e] += p[e];
-      if (!known) x[e] = __builtin_nanf("");
+      for (int e = 0; e < kVec; ++e) {
+        x[e] *= scale;
+        if (place != nullptr) x[e] += p[e];
+        if (!known) x[e] = __builtin_nanf("");
+      }
+      store_chunk(out + row * width, c, width, x, past);
     }
-    store_chunk(out + row * width, c, width, x, past);
   }
 }
 
@@ -75,6 +79,7 @@ struct SortPass {
   uint32_t* keys_out;
   uint32_t* values_out;
   uint32_t* counts;  // [tiles][digits]
+  uint32_t* totals;  // [digits] where a launch of its own scans the counts, else nullptr
   int64_t n;
   int64_t vocab;
   int shift, bits, tiles;
@@ -125,6 +130,41 @@ __global__ void __launch_bounds__(kBlock) attnres_sort_count_kernel(SortPass p, 
   for (int d = threadIdx.x; d < digits; d += kBlock) p.counts[static_cast<int64_t>(tile) * digits + d] = count[d];
 }
 
+// Many tiles: counts to the sums of the tiles before, and all tiles' totals.  64 digits per workgroup, a
+// sixteenth of the tiles per wavefront.  Up to kDirectTiles every tile makes these sums for itself, which
+// saves the launches but grows with the square of the tiles.  Whole gradient of a 131072 x 1024 BF16 table, us,
+// direct / with this launch: 16384 tokens 81 / 87, 32768 98 / 100, 65536 128 / 125, 262144 312 / 288, 1048576 1221 / 816.
+constexpr int kScanBlock = 1024;
+constexpr int kDirectTiles = 48;
+
+__global__ void __launch_bounds__(kScanBlock) attnres_sort_scan_kernel(SortPass p) {
+  constexpr int kParts = kScanBlock / 64;
+  __shared__ uint32_t sums[kParts][64];
+  const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
+  const int digits = 1 << p.bits, d = blockIdx.x * 64 + lane;
+  const int share = (p.tiles + kParts - 1) / kParts;
+  const int first = min(wave * share, p.tiles), end = d < digits ? min(first + share, p.tiles) : first;
+  uint32_t* counts = p.counts + d;
+  uint32_t sum = 0;
+#pragma unroll 16
+  for (int t = first; t < end; ++t) sum += counts[static_cast<int64_t>(t) * digits];
+  sums[wave][lane] = sum;
+  __syncthreads();
+  uint32_t before = 0, total = 0;
+#pragma unroll
+  for (int w = 0; w < kParts; ++w) {
+    before += w < wave ? sums[w][lane] : 0;
+    total += sums[w][lane];
+  }
+#pragma unroll 16
+  for (int t = first; t < end; ++t) {
+    const uint32_t c = counts[static_cast<int64_t>(t) * digits];
+    counts[static_cast<int64_t>(t) * digits] = before;
+    before += c;
+  }
+  if (wave == 0 && d < digits) p.totals[d] = total;
+}
+
 template <class W>
 __global__ void __launch_bounds__(kBlock) attnres_sort_place_kernel(SortPass p, ZeroFill<W> zero) {
   if (static_cast<int>(blockIdx.x) >= p.tiles) return zero_fill(zero, blockIdx.x - p.tiles, gridDim.x - p.tiles);
@@ -160,11 +200,16 @@ __global__ void __launch_bounds__(kBlock) attnres_sort_place_kernel(SortPass p, 
     total[j] = before[j] = 0;
     const int d = threadIdx.x * per + j;
     if (j < per && d < digits) {
+      if (p.totals != nullptr) {
+        before[j] = p.counts[static_cast<int64_t>(tile) * digits + d];
+        total[j] = p.totals[d];
+      } else {
 #pragma unroll 8
-      for (int t = 0; t < p.tiles; ++t) {
-        const uint32_t c = p.counts[static_cast<int64_t>(t) * digits + d];
-        total[j] += c;
-        before[j] += t < tile ? c : 0;
+        for (int t = 0; t < p.tiles; ++t) {
+          const uint32_t c = p.counts[static_cast<int64_t>(t) * digits + d];
+          total[j] += c;
+          before[j] += t < tile ? c : 0;
+        }
       }
       mine += total[j];
     }
@@ -462,7 +507,7 @@ __global__ void __launch_bounds__(kBlock) attnres_embedding_join_kernel(Runs r, 
 
 struct Plan {
   int tiles, bits, passes, piece;
-  int64_t pieces, keys[2], values[2], counts, partial, bytes;
+  int64_t pieces, keys[2], values[2], counts, totals, partial, bytes;
 };
 
 Plan plan(int64_t n, int64_t vocab, int64_t width) {
@@ -484,6 +529,7 @@ Plan plan(int64_t n, int64_t vocab, int64_t width) {
   };
   for (int k = 0; k < 2; ++k) p.keys[k] = take(4 * n), p.values[k] = take(4 * n);
   p.counts = take(4 * (int64_t{1} << p.bits) * p.tiles);
+  p.totals = take(4 * (int64_t{1} << p.bits));
   p.partial = take(4 * p.pieces * 2 * width);
   p.bytes = at;
   return p;
@@ -511,6 +557,7 @@ void embedding_backward(const void* grad_out, const void* tokens, int token_byte
     SortPass s{};
     s.token_bytes = token_bytes;
     s.counts = reinterpret_cast<uint32_t*>(workspace + p.counts);
+    if (p.tiles > kDirectTiles) s.totals = reinterpret_cast<uint32_t*>(workspace + p.totals);
     s.n = n;
     s.vocab = vocab;
     s.bits = p.bits;
@@ -538,6 +585,9 @@ void embedding_backward(const void* grad_out, const void* tokens, int token_byte
         };
         next_share(false);
         hipLaunchKernelGGL((attnres_sort_count_kernel<W>), dim3(p.tiles + fill), dim3(kBlock), 0, stream, s, zero);
+        if (s.totals != nullptr) {
+          hipLaunchKernelGGL(attnres_sort_scan_kernel, dim3(((1 << s.bits) + 63) / 64), dim3(kScanBlock), 0, stream, s);
+        }
         next_share(true);
         hipLaunchKernelGGL((attnres_sort_place_kernel<W>), dim3(p.tiles + fill), dim3(kBlock), 0, stream, s, zero);
       }
@@ -562,7 +612,7 @@ void embedding_backward(const void* grad_out, const void* tokens, int token_byte
 int check_embedding(int64_t batch, int64_t length, int64_t vocab, int64_t width, int weight_dtype, int out_dtype,
                     int token_bytes) {
   if (batch < 0 || length < 0 || (length > 0 && batch > kMaxTokens / length)) {
-    return layer_error(ATTNRES_ERR_SHAPE, "batch=%lld x length=%lld outside 0..2^30 tokens", (long long)batch, (long long)length);
+    return layer_error(ATTNRES_ERR_SHAPE, "batch=%lld x length=%lld outside 0..2^29 tokens", (long long)batch, (long long)length);
   }
   if (vocab < 1 || vocab > kMaxVocab) return layer_error(ATTNRES_ERR_SHAPE, "vocab=%lld outside 1..2^30", (long long)vocab);
   if (width < 1 || width > ATTNRES_MAX_WIDTH) {
@@ -609,10 +659,11 @@ int attnres_hip_embedding_forward(const void* tokens, int token_bytes, int64_t b
   with_types(weight_dtype, out_dtype, [&](auto w, auto o) {
     using W = decltype(w);
     using O = decltype(o);
-    hipLaunchKernelGGL((attnres_embedding_fwd_kernel<W, O>), dim3(static_cast<unsigned>((rows + per_block - 1) / per_block)),
-                       dim3(kBlock), 0, static_cast<hipStream_t>(stream), tokens, token_bytes, rows, length,
-                       static_cast<const W*>(weight), vocab, static_cast<int>(width), static_cast<const W*>(positions), scale,
-                       static_cast<O*>(out), threads, rows * width * static_cast<int64_t>(sizeof(O)) >= kPastCaches);
+    const int64_t blocks = std::min((rows + per_block - 1) / per_block, kMaxFwdBlocks);
+    hipLaunchKernelGGL((attnres_embedding_fwd_kernel<W, O>), dim3(static_cast<unsigned>(blocks)), dim3(kBlock), 0,
+                       static_cast<hipStream_t>(stream), tokens, token_bytes, rows, length, static_cast<const W*>(weight), vocab,
+                       static_cast<int>(width), static_cast<const W*>(positions), scale, static_cast<O*>(out), threads,
+                       rows * width * static_cast<int64_t>(sizeof(O)) >= kPastCaches);
   });
   return layer_launch_status("embedding forward");
 }
@@ -633,8 +684,8 @@ int attnres_hip_embedding_backward(const void* grad_out, int out_dtype, const vo
   if (batch * length > 0 && (grad_out == nullptr || tokens == nullptr)) {
     return layer_error(ATTNRES_ERR_NULL_POINTER, "grad_out or tokens is NULL");
   }
-  if (grad_positions != nullptr && (position_rows < length || position_rows > kMaxTokens)) {
-    return layer_error(ATTNRES_ERR_SHAPE, "position_rows=%lld outside length=%lld..2^30", (long long)position_rows,
+  if (grad_positions != nullptr && (position_rows < length || position_rows > kMaxPlaces)) {
+    return layer_error(ATTNRES_ERR_SHAPE, "position_rows=%lld outside length=%lld..2^26", (long long)position_rows,
                        (long long)length);
   }
   const int64_t need = attnres_hip_embedding_workspace_bytes(batch, length, vocab, width);
