@@ -34,7 +34,9 @@ _REDUCTIONS = {"none": 0, "sum": 1, "mean": 2}
 _MAX_TABLE = 2**30   # rows of an embedding table
 _MAX_VOCAB = 2**24   # rows of a projection to a vocabulary
 _MAX_TOKENS = 2**24  # of one loss
-_MAX_LOOKUPS = 2**30
+_LOSS_TILE, _MAX_TILES = 256, 2**22  # of tokens by words
+_MAX_LOOKUPS = 2**29
+_MAX_PLACES = 2**26  # rows of positions
 
 
 # ------------------------------------------------------------------- checks
@@ -182,6 +184,8 @@ def embedding(tokens: Tensor, weight: Tensor, positions: Tensor | None = None, *
         _check_tensor(positions, "positions", _FLOATS)
         if positions.ndim != 2 or positions.shape[1] != weight.shape[1] or positions.shape[0] < tokens.shape[-1]:
             raise ValueError("positions must have shape [P,D] with P at least the tokens' last axis")
+        if positions.shape[0] > _MAX_PLACES:
+            raise ValueError(f"supported envelope is P<={_MAX_PLACES}")
         if positions.dtype != weight.dtype:
             raise TypeError("positions must have the dtype of weight")
         _check_place("positions", positions, "weight", weight)
@@ -272,6 +276,8 @@ def linear_cross_entropy(hidden: Tensor, weight: Tensor, targets: Tensor, *, ign
         raise ValueError("targets must have the shape of hidden without its last axis")
     if targets.numel() > _MAX_TOKENS:
         raise ValueError(f"supported envelope is at most {_MAX_TOKENS} targets")
+    if -(-targets.numel() // _LOSS_TILE) * -(-weight.shape[0] // _LOSS_TILE) > _MAX_TILES:
+        raise ValueError(f"supported envelope is at most {_MAX_TILES} tiles of {_LOSS_TILE} targets by {_LOSS_TILE} words")
     if weight.dtype != hidden.dtype:
         raise TypeError("weight must have the dtype of hidden")
     _check_place("weight", weight, "hidden", hidden)

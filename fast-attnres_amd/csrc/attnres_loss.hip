@@ -1208,7 +1208,7 @@ void prepare_operands(const Call& c, bool find_scales, Operand* h, Operand* w) {
   Header* header = c.saved.header;
   if constexpr (kSplit) {
     if (find_scales) {
-      const unsigned grid_h = static_cast<unsigned>(std::min<int64_t>(c.rows, 1024));
+      const unsigned grid_h = static_cast<unsigned>(std::clamp<int64_t>(c.rows, 1, 1024));
       hipLaunchKernelGGL(attnres_loss_amax_kernel, dim3(grid_h), dim3(kBlock), 0, c.stream, hidden, c.hidden_stride, c.rows,
                          static_cast<int>(c.width), c.saved.index, &header->count, &header->amax[0]);
       const unsigned grid_w = static_cast<unsigned>(std::min<int64_t>(c.vocab, 2048));
@@ -1367,9 +1367,21 @@ void loss_backward(const Call& c, int reduction, const float* grad_loss, void* g
   }
 }
 
-// Workgroups of the logits' launch.
+// A launch takes fewer than 2^32 threads: 2^23 workgroups of a tile each are too many.
+constexpr int64_t kMaxTiles = int64_t{1} << 22;
 bool fits_grid(int64_t rows, int64_t vocab) {
-  return (rows + kTile - 1) / kTile * ((vocab + kTile - 1) / kTile) <= int64_t{1} << 30;
+  return (rows + kTile - 1) / kTile * ((vocab + kTile - 1) / kTile) <= kMaxTiles;
+}
+
+// Offsets into both are multiples of 16 bytes, which the products' loads into LDS need.
+int check_places(const void* saved, const void* workspace, int64_t workspace_bytes, int64_t need) {
+  if (workspace == nullptr || workspace_bytes < need) {
+    return layer_error(ATTNRES_ERR_WORKSPACE, "workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)need);
+  }
+  if (((reinterpret_cast<uintptr_t>(saved) | reinterpret_cast<uintptr_t>(workspace)) & 15u) != 0) {
+    return layer_error(ATTNRES_ERR_WORKSPACE, "saved and workspace must start at multiples of 16 bytes");
+  }
+  return ATTNRES_OK;
 }
 
 int check_loss(const void* hidden, int64_t hidden_stride, const void* weight, int64_t weight_stride, int64_t rows, int64_t vocab,
@@ -1383,7 +1395,7 @@ int check_loss(const void* hidden, int64_t hidden_stride, const void* weight, in
   if (reduction < ATTNRES_REDUCE_NONE || reduction > ATTNRES_REDUCE_MEAN) {
     return layer_error(ATTNRES_ERR_SCALAR, "unknown reduction %d", reduction);
   }
-  if (!fits_grid(rows, vocab)) return layer_error(ATTNRES_ERR_SHAPE, "rows x vocab outside 2^46");
+  if (!fits_grid(rows, vocab)) return layer_error(ATTNRES_ERR_SHAPE, "rows x vocab outside 2^22 tiles of 256 x 256");
   if (hidden_stride < 0 || weight_stride < 0) return layer_error(ATTNRES_ERR_STRIDE, "negative row stride");
   if ((rows > 0 && hidden == nullptr) || weight == nullptr) return layer_error(ATTNRES_ERR_NULL_POINTER, "hidden or weight is NULL");
   if (dtype != ATTNRES_F32 && width % kDepth == 0 &&
@@ -1425,10 +1437,7 @@ int attnres_hip_loss_forward(const void* hidden, int64_t hidden_stride, const vo
   }
   const Call c{hidden, hidden_stride, weight, weight_stride, rows, vocab, width, loss_plan(rows, vocab, width, dtype, false),
                saved_views(saved, rows), static_cast<char*>(workspace), static_cast<hipStream_t>(stream)};
-  if (workspace == nullptr || workspace_bytes < c.plan.bytes) {
-    return layer_error(ATTNRES_ERR_WORKSPACE, "workspace of %lld bytes, %lld needed", (long long)workspace_bytes,
-                       (long long)c.plan.bytes);
-  }
+  if (const int status = check_places(saved, workspace, workspace_bytes, c.plan.bytes)) return status;
   if (dtype == ATTNRES_BF16) loss_forward<Bf16, Bf16, 1>(c, targets, target_bytes, ignore_index, reduction, loss);
   else if (dtype == ATTNRES_F16) loss_forward<F16, F16, 1>(c, targets, target_bytes, ignore_index, reduction, loss);
   else loss_forward<float, F16, 3>(c, targets, target_bytes, ignore_index, reduction, loss);
@@ -1442,10 +1451,7 @@ int attnres_hip_loss_backward(const void* hidden, int64_t hidden_stride, const v
   if (saved == nullptr || grad_loss == nullptr) return layer_error(ATTNRES_ERR_NULL_POINTER, "saved or grad_loss is NULL");
   const Call c{hidden, hidden_stride, weight, weight_stride, rows, vocab, width, loss_plan(rows, vocab, width, dtype, true),
                saved_views(saved, rows), static_cast<char*>(workspace), static_cast<hipStream_t>(stream)};
-  if (workspace == nullptr || workspace_bytes < c.plan.bytes) {
-    return layer_error(ATTNRES_ERR_WORKSPACE, "workspace of %lld bytes, %lld needed", (long long)workspace_bytes,
-                       (long long)c.plan.bytes);
-  }
+  if (const int status = check_places(saved, workspace, workspace_bytes, c.plan.bytes)) return status;
   if (grad_hidden == nullptr && grad_weight == nullptr) return ATTNRES_OK;
   if (dtype == ATTNRES_BF16) loss_backward<Bf16, Bf16, 1>(c, reduction, grad_loss, grad_hidden, grad_weight);
   else if (dtype == ATTNRES_F16) loss_backward<F16, F16, 1>(c, reduction, grad_loss, grad_hidden, grad_weight);

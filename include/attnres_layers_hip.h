@@ -57,7 +57,7 @@ int attnres_hip_layer_norm_backward(const void* grad_out, const void* x, int64_t
  * out_dtype.  tokens [batch, length] contiguous, int64 (token_bytes 8) or int32
  * (4); weight [vocab, width] and positions [>= length, width] contiguous, of
  * weight_dtype; positions may be NULL.  A token outside 0..vocab-1 gives a row
- * of NaN and takes part in no gradient. */
+ * of NaN and takes no part in the table's gradient. */
 int attnres_hip_embedding_forward(const void* tokens, int token_bytes, int64_t batch, int64_t length,
                                   const void* weight, int64_t vocab, int64_t width, int weight_dtype,
                                   const void* positions, float scale, void* out, int out_dtype, void* stream);
@@ -76,14 +76,18 @@ int attnres_hip_embedding_backward(const void* grad_out, int out_dtype, const vo
 
 /* ---- softmax cross entropy of logits = hidden weight^T ----
  * hidden [rows, width] (rows hidden_stride apart), weight [vocab, width] (rows
- * weight_stride apart) of one dtype; targets [rows] contiguous, int64 or int32
+ * weight_stride apart) of one dtype, 1 <= width <= ATTNRES_MAX_WIDTH, rows and vocab up
+ * to 2^24 each and to 2^22 tiles of 256 x 256 together.  Where weight is of 16 bits and width a multiple of
+ * 32, its rows start at multiples of 16 bytes, at most 2^22 elements apart (else ATTNRES_ERR_STRIDE): it is
+ * multiplied where it lies.  targets [rows] contiguous, int64 or int32
  * (target_bytes).  loss (FP32): [rows] for ATTNRES_REDUCE_NONE (0 where the target
  * is ignore_index), else one value; the mean is over the targets that count (NaN
  * when none does).  A target that is neither ignore_index nor in 0..vocab-1 makes
  * the loss and the gradients NaN.  The logits are never stored: FP32 sums of exponentials in
  * pieces of the vocabulary, formed again in the backward.
  * saved: attnres_hip_loss_saved_bytes(rows) bytes that the backward reads (and completes, with
- * the same values every time, where a forward of few FP32 rows needed less). */
+ * the same values every time, where a forward of few FP32 rows needed less).  saved and
+ * workspace start at multiples of 16 bytes (else ATTNRES_ERR_WORKSPACE). */
 int64_t attnres_hip_loss_saved_bytes(int64_t rows);
 int64_t attnres_hip_loss_workspace_bytes(int64_t rows, int64_t vocab, int64_t width, int dtype, int backward);
 

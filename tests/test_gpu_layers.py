@@ -9,7 +9,7 @@ import pytest
 import torch
 
 import layer_reference as reference
-from attnres import layers
+from attnres import _native, layers
 from layer_reference import assert_within
 
 pytestmark = pytest.mark.gpu
@@ -173,6 +173,25 @@ def test_embedding_runs_of_one_length(run):
     g = _generator(run)
     tokens = torch.arange(4096, device="cuda") // run
     _check_embedding(tokens[torch.randperm(4096, generator=g, device="cuda")], _randn(g, 4100, 24), None, 2.0, FP32)
+
+
+@pytest.mark.parametrize("length,vocab", [(48 * 1024, 500), (48 * 1024 + 1, 500), (70001, 3), (70001, 40000), (200000, 1500000)])
+def test_embedding_of_many_tokens(length, vocab):
+    """Around the number of tiles from which their counts are scanned by a launch of its own."""
+    g = _generator(length)
+    tokens = (torch.rand(length, generator=g, device="cuda")**2 * vocab).long().clamp_(0, vocab - 1)
+    tokens[5::1000] = vocab  # outside
+    _check_embedding(tokens, _randn(g, vocab, 16).to(BF16), None, 1.0, FP32)
+
+
+def test_embedding_of_more_rows_than_a_launch_has_groups():
+    """8 threads to a row: more than 2^32 of them."""
+    g = _generator(53)
+    weight = _randn(g, 1000, 1).to(BF16)
+    tokens = torch.randint(1000, (2**29,), generator=g, device="cuda", dtype=torch.int32)
+    out = layers.embedding(tokens, weight)
+    for part, ids in zip(out[:, 0].split(2**26), tokens.split(2**26)):
+        assert torch.equal(part, weight[:, 0].take(ids.long()))
 
 
 def test_embedding_integer_types_batches_and_layouts():
@@ -369,6 +388,29 @@ def test_loss_without_rows():
         grads = torch.autograd.grad(out, (hidden, weight), torch.ones_like(out))
         assert grads[0].shape == hidden.shape and not grads[1].any()
         assert out.numel() == 0 if reduction == "none" else bool(out.isnan() if reduction == "mean" else out == 0)
+
+
+@pytest.mark.parametrize("dtype", [0, 1, 2])
+def test_loss_without_rows_through_the_c_abi(dtype):
+    lib = _native.load()
+    vocab, width, mean = 300, 40, 2
+    weight = _randn(_generator(6), vocab, width).to((BF16, FP16, FP32)[dtype])
+    saved = torch.empty(lib.attnres_hip_loss_saved_bytes(0), dtype=torch.uint8, device="cuda")
+    loss, grad = torch.zeros((), device="cuda"), torch.ones((), device="cuda")
+    grad_weight = torch.full_like(weight, 7.0)
+    stream = torch.cuda.current_stream().cuda_stream
+    for backward in (0, 1):
+        size = lib.attnres_hip_loss_workspace_bytes(0, vocab, width, dtype, backward)
+        workspace = torch.empty(size, dtype=torch.uint8, device="cuda")
+        if backward:
+            status = lib.attnres_hip_loss_backward(None, width, weight.data_ptr(), width, 0, vocab, width, dtype, mean,
+                                                   saved.data_ptr(), grad.data_ptr(), None, grad_weight.data_ptr(),
+                                                   workspace.data_ptr(), size, stream)
+        else:
+            status = lib.attnres_hip_loss_forward(None, width, weight.data_ptr(), width, None, 8, 0, vocab, width, dtype, -100,
+                                                  mean, loss.data_ptr(), saved.data_ptr(), workspace.data_ptr(), size, stream)
+        assert status == 0, lib.attnres_hip_last_error().decode()
+    assert bool(loss.isnan()) and not grad_weight.any()
 
 
 def test_loss_gradient_against_differences():

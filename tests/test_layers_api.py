@@ -56,6 +56,8 @@ def test_cpu_tensors_are_refused_after_everything_else(call):
     (lambda: _embed(weight=torch.zeros(0, 8)), ValueError, "envelope"),
     (lambda: _embed(positions=torch.zeros(2, 8)), ValueError, "positions"),
     (lambda: _embed(positions=torch.zeros(4, 7)), ValueError, "positions"),
+    (lambda: _embed(positions=torch.zeros(1, 8).expand(2**26 + 1, 8)), ValueError, "envelope"),
+    (lambda: _embed(torch.zeros(1, dtype=torch.int64).expand(2**29 + 1), positions=None), ValueError, "tokens"),
     (lambda: _embed(positions=torch.zeros(4, 8, dtype=BF16)), TypeError, "dtype of weight"),
     (lambda: _embed(dtype=torch.float64), TypeError, "dtype"),
     (lambda: _embed(scale=float("inf")), ValueError, "finite"),
@@ -67,6 +69,8 @@ def test_cpu_tensors_are_refused_after_everything_else(call):
     (lambda: _loss(targets=torch.zeros(2, 3)), TypeError, "targets"),
     (lambda: _loss(targets=torch.zeros(6, dtype=torch.int64)), ValueError, "targets"),
     (lambda: _loss(targets=torch.zeros(2, 3, dtype=torch.int64, device="meta")), TypeError, "device"),
+    (lambda: _loss(torch.zeros(2**22, 1, device="meta"), torch.zeros(2**16 + 1, 1, device="meta"),
+                   torch.zeros(2**22, dtype=torch.int64, device="meta")), ValueError, "tiles"),
     (lambda: _loss(ignore_index=1.0), TypeError, "ignore_index"),
     (lambda: _loss(ignore_index=True), TypeError, "ignore_index"),
     (lambda: _loss(reduction="max"), ValueError, "reduction"),
@@ -167,6 +171,8 @@ def _status(name, **overrides):
     ("embedding_forward", {"token_bytes": 2}, _native.ERR_SHAPE),
     ("embedding_forward", {"vocab": 0}, _native.ERR_SHAPE),
     ("embedding_forward", {"batch": 2**20, "length": 2**20}, _native.ERR_SHAPE),
+    ("embedding_forward", {"batch": 2**15 + 1, "length": 2**14}, _native.ERR_SHAPE),
+    ("embedding_backward", {"grad_positions": _FAKE, "position_rows": 2**26 + 1}, _native.ERR_SHAPE),
     ("embedding_forward", {"out_dtype": 7}, _native.ERR_SHAPE),
     ("embedding_backward", {"grad_out": None}, _native.ERR_NULL_POINTER),
     ("embedding_backward", {"bytes": 100}, _native.ERR_WORKSPACE),
@@ -176,6 +182,10 @@ def _status(name, **overrides):
     ("loss_forward", {"saved": None}, _native.ERR_NULL_POINTER),
     ("loss_forward", {"rows": 2**24 + 1}, _native.ERR_SHAPE),
     ("loss_forward", {"rows": 2**24, "vocab": 2**24}, _native.ERR_SHAPE),
+    ("loss_forward", {"rows": 2**22, "vocab": 2**16 + 1}, _native.ERR_SHAPE),
+    ("loss_forward", {"workspace": _FAKE + 8}, _native.ERR_WORKSPACE),
+    ("loss_forward", {"saved": _FAKE + 4}, _native.ERR_WORKSPACE),
+    ("loss_backward", {"workspace": _FAKE + 8}, _native.ERR_WORKSPACE),
     ("loss_forward", {"width": 8193}, _native.ERR_SHAPE),
     ("loss_forward", {"target_bytes": 1}, _native.ERR_SHAPE),
     ("loss_forward", {"reduction": 3}, _native.ERR_SCALAR),
