@@ -50,8 +50,8 @@ typedef short s16x8 __attribute__((ext_vector_type(8)));
 
 inline int64_t round_up(int64_t x, int64_t to) { return (x + to - 1) / to * to; }
 
-// What the forward leaves for the backward: a header, then per packed row the (maximum,
-// 1 / sum of exponentials above it) of its logits, its source row and its target, and per
+// What the forward leaves for the backward: a header, then per packed row the (reference,
+// 1 / sum of powers above it) of its logits, its source row and its target, and per
 // source row its packed one (or -1).
 struct Header {
   int32_t count;      // packed rows
@@ -386,27 +386,41 @@ __device__ __forceinline__ void multiply(const Product& p, const TileAt& tile, c
 
 // -------------------------------------------------------------------- logits
 
-// Joins two (maximum, sum of exponentials above it).  A side without entries is (-inf, 0);
+// Exponentials are powers of two above a reference c, an integer near the largest logit over ln 2: one fused
+// multiply-add and one power per logit, the product with 1 / ln 2 exact in the sum with c, and powers of c's that
+// differ are exact.  (1 / ln 2 itself is off by 2^-26, as if every logit were: less than their rounding.)
+constexpr float kLog2e = 1.44269504f;
+constexpr float kLn2 = 0.693147181f;
+
+__device__ __forceinline__ float power(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// Joins two (reference, sum of powers above it).  A side without entries is (-inf, 0);
 // a NaN sum stays NaN.
 __device__ __forceinline__ f32x2 join(f32x2 x, f32x2 y) {
   const float top = fmaxf(x.x, y.x);
   if (top == -__builtin_inff()) return f32x2{top, x.y + y.y};
-  return f32x2{top, x.y * __expf(x.x - top) + y.y * __expf(y.x - top)};
+  return f32x2{top, x.y * power(x.x - top) + y.y * power(y.x - top)};
 }
 
-// A logit from the product of scaled operands: by the two powers of two in turn, the smaller
+// Logits from the product of scaled operands: by the two powers of two in turn, the smaller
 // first, so that neither step leaves FP32 where the logit itself does not.
-struct Unscale {
+struct Logit {
   float first = 1.0f, second = 1.0f;
   bool any;
-  __device__ __forceinline__ explicit Unscale(const Header* header) : any(header != nullptr) {
+  __device__ __forceinline__ explicit Logit(const Header* header) : any(header != nullptr) {
     if (!any) return;
     const float h = 1.0f / header->scale[0], w = 1.0f / header->scale[1];
     first = fminf(h, w);
     second = fmaxf(h, w);
   }
   __device__ __forceinline__ float operator()(float x) const { return any ? x * first * second : x; }
+  __device__ __forceinline__ float above(float x, float c) const {  // log2 of the power
+    return __builtin_fmaf(any ? x * first : x, second * kLog2e, -c);
+  }
 };
+
+// The reference for logits of at most `top`.
+__device__ __forceinline__ float reference(float top) { return rintf(top * kLog2e); }
 
 struct LogitArgs {
   Product product;  // A: W (vocabulary), B: H (packed rows)
@@ -416,7 +430,7 @@ struct LogitArgs {
   int64_t first;      // of the piece's columns
   int64_t row_tiles;  // packed rows, padded
   // forward
-  f32x2* sums;          // [tiles][row_tiles] (maximum, sum of exponentials above it)
+  f32x2* sums;          // [tiles][row_tiles] (reference, sum of powers above it)
   float* target_logit;  // [row_tiles]
   // backward
   const f32x2* stats;
@@ -435,7 +449,7 @@ __global__ void __launch_bounds__(kThreads) attnres_loss_logits_kernel(LogitArgs
   Accumulators acc;
   multiply<T, SEGMENTS, true, true>(g.product, tile, stages_of(g.product, 0), lds, acc);
   const int wave = wave_index(), lane = threadIdx.x % 64;
-  const Unscale unscale(SEGMENTS == 3 ? g.header : nullptr);
+  const Logit logit(SEGMENTS == 3 ? g.header : nullptr);
   const int64_t v0 = static_cast<int64_t>(tile.a) * kTile + (wave % 2) * 128;
   const int limit = __builtin_amdgcn_readfirstlane(static_cast<int>(g.vocab - v0 < 128 ? g.vocab - v0 : 128));
   f32x2* meet = reinterpret_cast<f32x2*>(lds);  // [2][256]
@@ -456,7 +470,7 @@ __global__ void __launch_bounds__(kThreads) attnres_loss_logits_kernel(LogitArgs
         for (int e = 0; e < 4; ++e) top = fmaxf(top, !ENDS || i * 16 + e < last ? acc[i][j][e] : -__builtin_inff());
       }
       top = fmaxf(top, __shfl_xor(top, 16, 64));
-      top = unscale(fmaxf(top, __shfl_xor(top, 32, 64)));
+      top = reference(logit(fmaxf(top, __shfl_xor(top, 32, 64))));
       if (__any(rel >= 0)) {
         float own = 0.0f;
 #pragma unroll
@@ -464,7 +478,7 @@ __global__ void __launch_bounds__(kThreads) attnres_loss_logits_kernel(LogitArgs
 #pragma unroll
           for (int e = 0; e < 4; ++e) own = i * 16 + e == rel - 4 * (lane / 16) ? acc[i][j][e] : own;
         }
-        if (rel >= 0 && (rel >> 2 & 3) == lane / 16) g.target_logit[row] = unscale(own);
+        if (rel >= 0 && (rel >> 2 & 3) == lane / 16) g.target_logit[row] = logit(own);
       }
       const float from = top == -__builtin_inff() ? 0.0f : top;  // nothing but NaN, or nothing at all
       float sum = 0.0f;
@@ -472,7 +486,7 @@ __global__ void __launch_bounds__(kThreads) attnres_loss_logits_kernel(LogitArgs
       for (int i = 0; i < kDown; ++i) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float x = __expf(unscale(acc[i][j][e]) - from);
+          const float x = power(logit.above(acc[i][j][e], from));
           sum += !ENDS || i * 16 + e < last ? x : 0.0f;
         }
       }
@@ -508,57 +522,60 @@ __global__ void __launch_bounds__(kThreads) attnres_loss_probability_kernel(Logi
   Accumulators acc;
   multiply<T, SEGMENTS, true, true>(g.product, tile, stages_of(g.product, 0), lds, acc);
   const int wave = wave_index(), lane = threadIdx.x % 64;
-  const Unscale unscale(SEGMENTS == 3 ? g.header : nullptr);
+  const Logit logit(SEGMENTS == 3 ? g.header : nullptr);
   const int64_t v0 = g.first + static_cast<int64_t>(tile.a) * kTile + (wave % 2) * 128;
   const int limit = __builtin_amdgcn_readfirstlane(static_cast<int>(g.vocab - v0 < 128 ? g.vocab - v0 : 128));
   constexpr int kParts = SEGMENTS == 3 ? 2 : 1;
   // With two parts, the columns of four wavefronts at a time: hi and lo of 128 rows are staged together.
   constexpr int kColumns = kTile / kParts;
-  const auto stage = [&](auto ends, int base) {
-    constexpr bool ENDS = decltype(ends)::value;
+  // SPECIAL: the vocabulary ends in these columns, or the target of one of the 16 rows is among them
+  const auto stage = [&](auto special, int j, int base) {
+    constexpr bool SPECIAL = decltype(special)::value;
     const int last = limit - 4 * (lane / 16);
+    const int column = (wave / 2) * (16 * kAcross) + j * 16 + lane % 16;
+    const int row = tile.b * kTile + column;
+    const int at = min(row, count - 1);
+    const int64_t from_v0 = g.target[at] - v0;
+    const int rel = from_v0 >= 0 && from_v0 < 128 ? static_cast<int>(from_v0) - 4 * (lane / 16) : -128;
+    // a row past the last one has zeros in H, so logits of 0, and a factor of 0
+    const float c = row < count ? g.stats[at].x : 0.0f;
+    const float by = g.row_scale[row], factor = row < count ? g.stats[at].y * by : 0.0f;
 #pragma unroll
-    for (int j = 0; j < kAcross; ++j) {
-      const int column = (wave / 2) * (16 * kAcross) + j * 16 + lane % 16;
-      const int row = tile.b * kTile + column;
-      const int at = min(row, count - 1);
-      const int64_t from_v0 = g.target[at] - v0;
-      const int rel = from_v0 >= 0 && from_v0 < 128 ? static_cast<int>(from_v0) - 4 * (lane / 16) : -128;
-      // a row past the last one has zeros in H, so logits of 0, and a factor of 0
-      const f32x2 stats = {row < count ? g.stats[at].x : 0.0f, g.stats[at].y};
-      const float by = g.row_scale[row];
+    for (int i = 0; i < kDown; ++i) {
+      float x[4];
 #pragma unroll
-      for (int i = 0; i < kDown; ++i) {
-        float x[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          x[e] = __expf(unscale(acc[i][j][e]) - stats.x) * stats.y;
-          if (i * 16 + e == rel) x[e] -= 1.0f;
-          x[e] *= by;
-          if (ENDS && i * 16 + e >= last) x[e] = 0.0f;
-          // the FP32 value itself: hi has to be the same number where it is stored and where lo
-          // is what it leaves, and a product folded into one of the conversions rounds apart
-          if (kParts == 2) asm("" : "+v"(x[e]));
+      for (int e = 0; e < 4; ++e) {
+        x[e] = power(logit.above(acc[i][j][e], c)) * factor;
+        if (SPECIAL) {
+          if (i * 16 + e == rel) x[e] -= by;
+          if (i * 16 + e >= last) x[e] = 0.0f;
         }
-        const int chunk = (wave % 2) * 16 + i * 2 + lane / 32;
-        uint16_t* to = lds + staged(column - base, chunk) * 8 + (lane / 16 % 2) * 4;
-#pragma unroll
-        for (int part = 0; part < kParts; ++part) {
-          const uint32_t packed[2] = {pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3])};
-          *reinterpret_cast<uint64_t*>(to + part * kColumns * kTile) = static_cast<uint64_t>(packed[1]) << 32 | packed[0];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) x[e] -= to_f32(T{static_cast<uint16_t>(packed[e / 2] >> (16 * (e % 2)))});  // lo
-        }
-        if (i % 2 == 1) __builtin_amdgcn_sched_barrier(0);  // a few outputs at a time: no registers to spill
+        // the FP32 value itself: hi has to be the same number where it is stored and where lo
+        // is what it leaves, and a product folded into one of the conversions rounds apart
+        if (kParts == 2) asm("" : "+v"(x[e]));
       }
+      const int chunk = (wave % 2) * 16 + i * 2 + lane / 32;
+      uint16_t* to = lds + staged(column - base, chunk) * 8 + (lane / 16 % 2) * 4;
+#pragma unroll
+      for (int part = 0; part < kParts; ++part) {
+        const uint32_t packed[2] = {pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3])};
+        *reinterpret_cast<uint64_t*>(to + part * kColumns * kTile) = static_cast<uint64_t>(packed[1]) << 32 | packed[0];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] -= to_f32(T{static_cast<uint16_t>(packed[e / 2] >> (16 * (e % 2)))});  // lo
+      }
+      if (i % 2 == 1) __builtin_amdgcn_sched_barrier(0);  // a few outputs at a time: no registers to spill
     }
   };
   for (int base = 0; base < kTile; base += kColumns) {
     if (kParts == 1 || (wave / 2) * (16 * kAcross) / kColumns == base / kColumns) {
-      if (limit < 128) {
-        stage(std::true_type{}, base);
-      } else {
-        stage(std::false_type{}, base);
+#pragma unroll
+      for (int j = 0; j < kAcross; ++j) {
+        const int64_t from_v0 = g.target[min(tile.b * kTile + (wave / 2) * (16 * kAcross) + j * 16 + lane % 16, count - 1)] - v0;
+        if (limit < 128 || __any(from_v0 >= 0 && from_v0 < 128)) {
+          stage(std::true_type{}, j, base);
+        } else {
+          stage(std::false_type{}, j, base);
+        }
       }
     }
     __syncthreads();
@@ -889,11 +906,12 @@ __global__ void __launch_bounds__(kFewBlock) attnres_loss_few_kernel(FewArgs<X> 
     }
     top = fmaxf(top, __shfl_xor(top, 16, 64));
     top = fmaxf(top, __shfl_xor(top, 32, 64));
+    top = reference(top);
     const float from = top == -__builtin_inff() ? 0.0f : top;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) sum += counts[i][e] ? __expf(acc[i][t][e] - from) : 0.0f;
+      for (int e = 0; e < 4; ++e) sum += counts[i][e] ? power(__builtin_fmaf(acc[i][t][e], kLog2e, -from)) : 0.0f;
     }
     sum += __shfl_xor(sum, 16, 64);
     sum += __shfl_xor(sum, 32, 64);
@@ -1017,8 +1035,9 @@ __global__ void __launch_bounds__(kBlock) attnres_loss_reduce_kernel(const f32x2
   for (int k = 1; k < kBlock / 64; ++k) total = join(total, part[k][threadIdx.x]);
   const bool known = s.target[at] >= 0;
   s.stats[at] = f32x2{total.x, known ? 1.0f / total.y : __builtin_nanf("")};
-  // the logarithm of the sum by itself: at a probability of one it is the whole loss
-  loss[row] = known ? logf(total.y) + (total.x - target_logit[column]) : __builtin_nanf("");
+  // both terms are small where the target's probability is near one, and the loss is not below zero
+  const float value = kLn2 * (log2f(total.y) - __builtin_fmaf(target_logit[column], kLog2e, -total.x));
+  loss[row] = !known ? __builtin_nanf("") : value < 0.0f ? 0.0f : value;
 }
 
 __global__ void __launch_bounds__(kScanThreads) attnres_loss_total_kernel(const float* __restrict__ loss, int64_t rows, const Header* header,
