@@ -107,13 +107,13 @@ LAYER_SIGNATURES = {
     "attnres_hip_embedding_backward": (ctypes.c_int, [
         _c_void_p, ctypes.c_int, _c_void_p, ctypes.c_int, _i64, _i64, _i64, _i64, ctypes.c_int, _f32, _c_void_p,
         _c_void_p, _i64, _c_void_p, _i64, _c_void_p]),
-    "attnres_hip_loss_saved_bytes": (_i64, [_i64]),
-    "attnres_hip_loss_workspace_bytes": (_i64, [_i64, _i64, _i64, ctypes.c_int, ctypes.c_int]),
+    "attnres_hip_loss_saved_bytes": (_i64, [_i64, _i64, _i64, ctypes.c_int, ctypes.c_int]),
+    "attnres_hip_loss_workspace_bytes": (_i64, [_i64, _i64, _i64, ctypes.c_int, ctypes.c_int, ctypes.c_int]),
     "attnres_hip_loss_forward": (ctypes.c_int, [
         _c_void_p, _i64, _c_void_p, _i64, _c_void_p, ctypes.c_int, _i64, _i64, _i64, ctypes.c_int, _i64, ctypes.c_int,
-        _c_void_p, _c_void_p, _c_void_p, _i64, _c_void_p]),
+        ctypes.c_int, _c_void_p, _c_void_p, _c_void_p, _i64, _c_void_p]),
     "attnres_hip_loss_backward": (ctypes.c_int, [
-        _c_void_p, _i64, _c_void_p, _i64, _i64, _i64, _i64, ctypes.c_int, ctypes.c_int, _c_void_p, _c_void_p,
+        _c_void_p, _i64, _c_void_p, _i64, _i64, _i64, _i64, ctypes.c_int, ctypes.c_int, ctypes.c_int, _c_void_p, _c_void_p,
         _c_void_p, _c_void_p, _c_void_p, _i64, _c_void_p]),
 }
 

@@ -35,6 +35,7 @@ _MAX_TABLE = 2**30   # rows of an embedding table
 _MAX_VOCAB = 2**24   # rows of a projection to a vocabulary
 _MAX_TOKENS = 2**24  # of one loss
 _LOSS_TILE, _MAX_TILES = 256, 2**22  # of tokens by words
+_MAX_KEPT = 2**33  # bytes of exponentials
 _MAX_LOOKUPS = 2**29
 _MAX_PLACES = 2**26  # rows of positions
 
@@ -247,8 +248,8 @@ _embedding.register_autograd(_embedding_autograd, setup_context=_embedding_conte
 # --------------------------------------------------------------------- loss
 
 def linear_cross_entropy(hidden: Tensor, weight: Tensor, targets: Tensor, *, ignore_index: int = -100,
-                         reduction: str = "mean") -> Tensor:
-    """Softmax cross entropy of the logits ``hidden @ weight.T``, which are never stored.
+                         reduction: str = "mean", recompute: bool = False) -> Tensor:
+    """Softmax cross entropy of the logits ``hidden @ weight.T``, which are never stored in full precision.
 
     ``hidden`` is ``[..., D]``, ``weight`` ``[V, D]``, both BF16, FP16 or FP32, one
     dtype, ``1 <= D <= 8192``; ``targets`` ``[...]`` int64 or int32.  The loss is
@@ -260,9 +261,11 @@ def linear_cross_entropy(hidden: Tensor, weight: Tensor, targets: Tensor, *, ign
 
     16-bit inputs are multiplied on the matrix cores as they are, FP32 ones to FP32's
     accuracy as pairs of FP16 numbers (relative to the largest magnitude of the tensor, so a tensor
-    whose values span more than 2^25 loses the smallest).  The backward forms the
-    probabilities again, for one piece of the vocabulary at a time.  Gradients
-    flow to ``hidden`` and ``weight``.
+    whose values span more than 2^25 loses the smallest, and infinities count as NaN).  Gradients
+    flow to ``hidden`` and ``weight``.  For them the forward keeps the logits' exponentials, FP16 relative to
+    the largest of 128 for BF16 inputs (2 bytes per target and word), else FP32 (4), where that is at most 8 GiB; beyond
+    that, or with ``recompute=True``, it keeps 20 bytes per target and the backward forms them again, for one piece of
+    the vocabulary at a time, which adds a third to its products.
     """
     _check_tensor(hidden, "hidden", _FLOATS)
     _check_tensor(weight, "weight", _FLOATS)
@@ -286,55 +289,66 @@ def linear_cross_entropy(hidden: Tensor, weight: Tensor, targets: Tensor, *, ign
         raise TypeError("ignore_index must be an integer")
     if reduction not in _REDUCTIONS:
         raise ValueError("reduction must be 'none', 'sum' or 'mean'")
+    if not isinstance(recompute, bool):
+        raise TypeError("recompute must be a bool")
     _check_gpu("linear_cross_entropy", hidden)
     code = _REDUCTIONS[reduction]
     if _eager(hidden, weight, targets):
-        return _native.load_autograd().linear_cross_entropy(hidden, weight, targets, ignore_index, code)
-    return _linear_cross_entropy(hidden, weight, targets, ignore_index, code)[0]
+        return _native.load_autograd().linear_cross_entropy(hidden, weight, targets, ignore_index, code, not recompute)
+    keep = not recompute and _needs_grad(hidden, weight)
+    return _linear_cross_entropy(hidden, weight, targets, ignore_index, code, keep)[0]
 
 
-_SAVED_HEADER, _SAVED_ROW = 256, 20  # bytes of attnres_hip_loss_saved_bytes
+def _loss_saved_bytes(rows: int, vocab: int, width: int, dtype: torch.dtype, keep: bool) -> int:
+    """attnres_hip_loss_saved_bytes, for sizes that may be symbols."""
+    size = 256 + 20 * rows
+    if not keep or rows <= (64 if dtype == torch.float32 or width % 32 else 32):
+        return size
+    rows, vocab = (-(-n // _LOSS_TILE) * _LOSS_TILE for n in (rows, vocab))
+    powers = (2 if dtype == torch.bfloat16 else 4) * rows * vocab
+    return size if powers > _MAX_KEPT else -(-size // 256) * 256 + 8 * (vocab // 128) * rows + powers
 
 
 @torch.library.custom_op("attnres_hip::linear_cross_entropy", mutates_args=(), device_types="cuda", tags=_OP_TAGS)
-def _linear_cross_entropy(hidden: Tensor, weight: Tensor, targets: Tensor, ignore_index: int,
-                          reduction: int) -> tuple[Tensor, Tensor]:
-    return _native.load_autograd().loss_forward(hidden, weight, targets, ignore_index, reduction)
+def _linear_cross_entropy(hidden: Tensor, weight: Tensor, targets: Tensor, ignore_index: int, reduction: int,
+                          keep: bool) -> tuple[Tensor, Tensor]:
+    return _native.load_autograd().loss_forward(hidden, weight, targets, ignore_index, reduction, keep)
 
 
 @_linear_cross_entropy.register_fake
-def _(hidden, weight, targets, ignore_index, reduction):
+def _(hidden, weight, targets, ignore_index, reduction, keep):
+    saved = _loss_saved_bytes(targets.numel(), weight.shape[0], weight.shape[1], weight.dtype, keep)
     return (hidden.new_empty(targets.shape if reduction == 0 else (), dtype=torch.float32),
-            hidden.new_empty((_SAVED_HEADER + _SAVED_ROW * targets.numel(),), dtype=torch.uint8))
+            hidden.new_empty((saved,), dtype=torch.uint8))
 
 
 @torch.library.custom_op("attnres_hip::linear_cross_entropy_backward", mutates_args=(), device_types="cuda", tags=_OP_TAGS)
-def _linear_cross_entropy_backward(grad: Tensor, hidden: Tensor, weight: Tensor, saved: Tensor, reduction: int,
+def _linear_cross_entropy_backward(grad: Tensor, hidden: Tensor, weight: Tensor, saved: Tensor, reduction: int, keep: bool,
                                    want_hidden: bool, want_weight: bool) -> tuple[Tensor, Tensor]:
-    return _native.load_autograd().loss_backward(grad, hidden, weight, saved, reduction, want_hidden, want_weight)
+    return _native.load_autograd().loss_backward(grad, hidden, weight, saved, reduction, keep, want_hidden, want_weight)
 
 
 @_linear_cross_entropy_backward.register_fake
-def _(grad, hidden, weight, saved, reduction, want_hidden, want_weight):
+def _(grad, hidden, weight, saved, reduction, keep, want_hidden, want_weight):
     return (hidden.new_empty(hidden.shape if want_hidden else (0,)), weight.new_empty(weight.shape if want_weight else (0,)))
 
 
 def _loss_context(ctx: Any, inputs: tuple, output: tuple) -> None:
-    hidden, weight, _targets, _ignore_index, reduction = inputs
+    hidden, weight, _targets, _ignore_index, reduction, keep = inputs
     saved = output[1]
     ctx.mark_non_differentiable(saved)
     ctx.set_materialize_grads(False)
     ctx.save_for_backward(hidden, weight, saved)
-    ctx.reduction = reduction
+    ctx.reduction, ctx.keep = reduction, keep
 
 
 def _loss_autograd(ctx: Any, grad, _saved):
     if grad is None:
-        return None, None, None, None, None
+        return None, None, None, None, None, None
     hidden, weight, saved = ctx.saved_tensors
     wanted = ctx.needs_input_grad[:2]
-    grads = _linear_cross_entropy_backward(grad, hidden, weight, saved, ctx.reduction, *wanted)
-    return (*(g if want else None for g, want in zip(grads, wanted)), None, None, None)
+    grads = _linear_cross_entropy_backward(grad, hidden, weight, saved, ctx.reduction, ctx.keep, *wanted)
+    return (*(g if want else None for g, want in zip(grads, wanted)), None, None, None, None)
 
 
 _linear_cross_entropy.register_autograd(_loss_autograd, setup_context=_loss_context)

@@ -161,6 +161,11 @@ struct Chunk {
       }
     }
   }
+  // Eight elements that are read once, and not from the caches.
+  __device__ __forceinline__ void load_past(const T* from) {
+#pragma unroll
+    for (size_t k = 0; k < sizeof(T) / 2; ++k) w[k] = __builtin_nontemporal_load(&reinterpret_cast<const Raw16*>(from)[k].v);
+  }
   __device__ __forceinline__ void unpack(float* x) const {
 #pragma unroll
     for (int e = 0; e < 4; ++e) {

@@ -248,16 +248,16 @@ Rows weight_rows(const Tensor& weight) {
   return rows;
 }
 
-Tensor loss_workspace(const Tensor& hidden, const Tensor& weight, int64_t rows, bool backward) {
+Tensor loss_workspace(const Tensor& hidden, const Tensor& weight, int64_t rows, bool keep, bool backward) {
   const int64_t bytes =
-      attnres_hip_loss_workspace_bytes(rows, weight.size(0), weight.size(1), dtype_of(weight.scalar_type()), backward);
+      attnres_hip_loss_workspace_bytes(rows, weight.size(0), weight.size(1), dtype_of(weight.scalar_type()), keep, backward);
   TORCH_CHECK_VALUE(bytes >= 0, "linear cross entropy: shape outside the supported envelope");
   return torch::empty({bytes}, hidden.options().dtype(torch::kUInt8));
 }
 
 // (loss, saved): the loss has the targets' shape for ATTNRES_REDUCE_NONE, else none.
 std::tuple<Tensor, Tensor> loss_forward(const Tensor& hidden, const Tensor& weight, const Tensor& targets, int64_t ignore_index,
-                                        int64_t reduction) {
+                                        int64_t reduction, bool keep) {
   const c10::DeviceGuard guard(hidden.device());
   const at::NoGradGuard no_grad;
   const Rows h = rows_view(hidden), w = weight_rows(weight);
@@ -265,12 +265,14 @@ std::tuple<Tensor, Tensor> loss_forward(const Tensor& hidden, const Tensor& weig
   const int64_t rows = ids.numel();
   const auto floats = hidden.options().dtype(torch::kFloat32);
   Tensor loss = reduction == ATTNRES_REDUCE_NONE ? torch::empty(targets.sizes(), floats) : torch::empty({}, floats);
-  Tensor saved = torch::empty({attnres_hip_loss_saved_bytes(rows)}, hidden.options().dtype(torch::kUInt8));
-  Tensor workspace = loss_workspace(hidden, weight, rows, false);
+  Tensor workspace = loss_workspace(hidden, weight, rows, keep, false);
+  Tensor saved = torch::empty(
+      {attnres_hip_loss_saved_bytes(rows, weight.size(0), weight.size(1), dtype_of(weight.scalar_type()), keep)},
+      hidden.options().dtype(torch::kUInt8));
   if (rows == 0 && reduction == ATTNRES_REDUCE_NONE) return {loss, saved};
   check(attnres_hip_loss_forward(h.tensor.data_ptr(), h.stride, w.tensor.data_ptr(), w.stride, data_of(ids),
                                  static_cast<int>(ids.element_size()), rows, weight.size(0), weight.size(1),
-                                 dtype_of(hidden.scalar_type()), ignore_index, static_cast<int>(reduction),
+                                 dtype_of(hidden.scalar_type()), ignore_index, static_cast<int>(reduction), keep,
                                  loss.data_ptr<float>(), saved.data_ptr(), workspace.data_ptr(), workspace.numel(),
                                  current_stream(hidden)),
         "linear cross entropy forward");
@@ -278,7 +280,7 @@ std::tuple<Tensor, Tensor> loss_forward(const Tensor& hidden, const Tensor& weig
 }
 
 std::tuple<Tensor, Tensor> loss_backward(const Tensor& grad_loss, const Tensor& hidden, const Tensor& weight, const Tensor& saved,
-                                         int64_t reduction, bool want_hidden, bool want_weight) {
+                                         int64_t reduction, bool keep, bool want_hidden, bool want_weight) {
   const c10::DeviceGuard guard(hidden.device());
   const at::NoGradGuard no_grad;
   const Rows h = rows_view(hidden), w = weight_rows(weight);
@@ -293,9 +295,9 @@ std::tuple<Tensor, Tensor> loss_backward(const Tensor& grad_loss, const Tensor& 
   }
   Tensor grad_weight = want_weight ? torch::empty(weight.sizes(), weight.options().memory_format(contiguous))
                                    : torch::empty({0}, weight.options());
-  Tensor workspace = loss_workspace(hidden, weight, rows, true);
+  Tensor workspace = loss_workspace(hidden, weight, rows, keep, true);
   check(attnres_hip_loss_backward(h.tensor.data_ptr(), h.stride, w.tensor.data_ptr(), w.stride, rows, weight.size(0),
-                                  weight.size(1), dtype_of(hidden.scalar_type()), static_cast<int>(reduction), saved.data_ptr(),
+                                  weight.size(1), dtype_of(hidden.scalar_type()), static_cast<int>(reduction), keep, saved.data_ptr(),
                                   grad.data_ptr<float>(), want_hidden ? grad_hidden.data_ptr() : nullptr,
                                   want_weight ? grad_weight.data_ptr() : nullptr, workspace.data_ptr(), workspace.numel(),
                                   current_stream(hidden)),
@@ -305,21 +307,23 @@ std::tuple<Tensor, Tensor> loss_backward(const Tensor& grad_loss, const Tensor& 
 
 struct LinearCrossEntropy : public torch::autograd::Function<LinearCrossEntropy> {
   static Tensor forward(AutogradContext* ctx, const Tensor& hidden, const Tensor& weight, const Tensor& targets,
-                        int64_t ignore_index, int64_t reduction) {
-    auto [loss, saved] = loss_forward(hidden, weight, targets, ignore_index, reduction);
+                        int64_t ignore_index, int64_t reduction, bool keep) {
+    auto [loss, saved] = loss_forward(hidden, weight, targets, ignore_index, reduction, keep);
     ctx->set_materialize_grads(false);
     ctx->save_for_backward({hidden, weight, saved});
     ctx->saved_data["reduction"] = reduction;
+    ctx->saved_data["keep"] = keep;
     return loss;
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
-    variable_list result(5);
+    variable_list result(6);
     if (!grads[0].defined()) return result;
     const variable_list saved = ctx->get_saved_variables();
     const bool want_hidden = ctx->needs_input_grad(0), want_weight = ctx->needs_input_grad(1);
     const auto [grad_hidden, grad_weight] = loss_backward(grads[0], saved[0], saved[1], saved[2],
-                                                          ctx->saved_data["reduction"].toInt(), want_hidden, want_weight);
+                                                          ctx->saved_data["reduction"].toInt(), ctx->saved_data["keep"].toBool(),
+                                                          want_hidden, want_weight);
     if (want_hidden) result[0] = grad_hidden;
     if (want_weight) result[1] = grad_weight;
     return once_differentiable(std::move(result));
@@ -327,9 +331,9 @@ struct LinearCrossEntropy : public torch::autograd::Function<LinearCrossEntropy>
 };
 
 Tensor linear_cross_entropy(const Tensor& hidden, const Tensor& weight, const Tensor& targets, int64_t ignore_index,
-                            int64_t reduction) {
-  if (!wants_grad({hidden, weight})) return std::get<0>(loss_forward(hidden, weight, targets, ignore_index, reduction));
-  return LinearCrossEntropy::apply(hidden, weight, targets, ignore_index, reduction);
+                            int64_t reduction, bool keep) {
+  if (!wants_grad({hidden, weight})) return std::get<0>(loss_forward(hidden, weight, targets, ignore_index, reduction, false));
+  return LinearCrossEntropy::apply(hidden, weight, targets, ignore_index, reduction, keep);
 }
 
 }  // namespace

@@ -48,7 +48,7 @@ typedef short s16x8 __attribute__((ext_vector_type(8)));
 #define ATTNRES_LDS __attribute__((address_space(3)))
 #define ATTNRES_GLOBAL __attribute__((address_space(1)))
 
-inline int64_t round_up(int64_t x, int64_t to) { return (x + to - 1) / to * to; }
+__host__ __device__ inline int64_t round_up(int64_t x, int64_t to) { return (x + to - 1) / to * to; }
 
 // What the forward leaves for the backward: a header, then per packed row the (reference,
 // 1 / sum of powers above it) of its logits, its source row and its target, and per
@@ -59,21 +59,18 @@ struct Header {
   uint32_t amax[2];   // their largest finite magnitudes, as bits
 };
 
+// With `keep` also the (reference, sum) of every row and 128 columns and the powers themselves.
 struct Saved {
   Header* header;
   f32x2* stats;
   int32_t* index;
   int32_t* packed;
   int32_t* target;
+  f32x2* sums;  // [columns / 128][row_tiles]
+  void* powers; // [row_tiles][vocabulary, padded]
 };
 
 constexpr int64_t kHeaderBytes = 256;
-inline int64_t saved_bytes(int64_t rows) { return kHeaderBytes + 20 * rows; }
-inline Saved saved_views(void* base, int64_t rows) {
-  char* at = static_cast<char*>(base) + kHeaderBytes;
-  return {static_cast<Header*>(base), reinterpret_cast<f32x2*>(at), reinterpret_cast<int32_t*>(at + 8 * rows),
-          reinterpret_cast<int32_t*>(at + 12 * rows), reinterpret_cast<int32_t*>(at + 16 * rows)};
-}
 
 // ------------------------------------------------------------- matrix product
 // out[b][a] = sum_k A[a][k] B[b][k] over a tile of 256 x 256: A's index is the contiguous
@@ -386,13 +383,19 @@ __device__ __forceinline__ void multiply(const Product& p, const TileAt& tile, c
 
 // -------------------------------------------------------------------- logits
 
-// Exponentials are powers of two above a reference c, an integer near the largest logit over ln 2: one fused
-// multiply-add and one power per logit, the product with 1 / ln 2 exact in the sum with c, and powers of c's that
-// differ are exact.  (1 / ln 2 itself is off by 2^-26, as if every logit were: less than their rounding.)
+// Exponentials are powers of two above a reference c, an integer near the largest logit over ln 2, so that joining sums
+// of different c's rounds nothing.  A logit over ln 2 is rounded before c is taken from it, the same wherever it is
+// formed: of logits so large that c's neighbours are far apart, the largest is still c itself.
 constexpr float kLog2e = 1.44269504f;
 constexpr float kLn2 = 0.693147181f;
 
 __device__ __forceinline__ float power(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// A product that is rounded, not fused with what follows.
+__device__ __forceinline__ float over_ln2(float x, float by = kLog2e) {
+#pragma clang fp contract(off)
+  return x * by;
+}
 
 // Joins two (reference, sum of powers above it).  A side without entries is (-inf, 0);
 // a NaN sum stays NaN.
@@ -415,12 +418,23 @@ struct Logit {
   }
   __device__ __forceinline__ float operator()(float x) const { return any ? x * first * second : x; }
   __device__ __forceinline__ float above(float x, float c) const {  // log2 of the power
-    return __builtin_fmaf(any ? x * first : x, second * kLog2e, -c);
+    return over_ln2(any ? x * first : x, second * kLog2e) - c;
   }
 };
 
-// The reference for logits of at most `top`.
-__device__ __forceinline__ float reference(float top) { return rintf(top * kLog2e); }
+// What powers are kept in for the backward.  BF16 operands: FP16, whose rounding of 2^-11 adds an eighth to
+// that of the probabilities to BF16.  Others: FP32, as FP16 would double the rounding of the probabilities to FP16.
+template <class T>
+using Power = std::conditional_t<std::is_same_v<T, Bf16>, F16, float>;
+
+// The reference for logits of at most `top`.  Powers that are kept in FP16 are shifted up by 15, so that those down
+// to 2^-29 of the largest are normal numbers; not where the reference is no exact integer any more.
+constexpr float kShift = 15.0f;
+template <class T>
+__device__ __forceinline__ float reference(float top) {
+  const float c = rintf(over_ln2(top));
+  return std::is_same_v<Power<T>, F16> && fabsf(c) < 8388608.0f ? c - kShift : c;
+}
 
 struct LogitArgs {
   Product product;  // A: W (vocabulary), B: H (packed rows)
@@ -430,8 +444,10 @@ struct LogitArgs {
   int64_t first;      // of the piece's columns
   int64_t row_tiles;  // packed rows, padded
   // forward
-  f32x2* sums;          // [tiles][row_tiles] (reference, sum of powers above it)
+  f32x2* sums;          // [columns / 128][row_tiles] (reference, sum of powers above it)
   float* target_logit;  // [row_tiles]
+  void* powers;         // [row_tiles][powers_ld], or nullptr: not kept
+  int64_t powers_ld;
   // backward
   const f32x2* stats;
   const float* row_scale;  // [row_tiles] upstream gradient per packed row, scaled; 0 past the last
@@ -439,8 +455,12 @@ struct LogitArgs {
   int64_t p_ld;
 };
 
-// Forward: (maximum, sum) of a tile's 256 logits per row, and the target's logit.
-template <class T, int SEGMENTS>
+// 16-byte slot of a staged output row of 512 bytes: a permutation per row, so that 32 lanes
+// writing one chunk of 32 rows meet 32 different slots.
+__device__ __forceinline__ int staged(int row, int chunk) { return row * 32 + (chunk ^ (row & 31)); }
+
+// Forward: (reference, sum) of a tile's two times 128 logits per row, and the target's logit.  KEEP: the powers too.
+template <class T, int SEGMENTS, bool KEEP>
 __global__ void __launch_bounds__(kThreads) attnres_loss_logits_kernel(LogitArgs g) {
   __shared__ __align__(16) uint16_t lds[kStages * 2 * kOperand];
   const int count = __builtin_amdgcn_readfirstlane(*g.product.count);
@@ -452,65 +472,154 @@ __global__ void __launch_bounds__(kThreads) attnres_loss_logits_kernel(LogitArgs
   const Logit logit(SEGMENTS == 3 ? g.header : nullptr);
   const int64_t v0 = static_cast<int64_t>(tile.a) * kTile + (wave % 2) * 128;
   const int limit = __builtin_amdgcn_readfirstlane(static_cast<int>(g.vocab - v0 < 128 ? g.vocab - v0 : 128));
-  f32x2* meet = reinterpret_cast<f32x2*>(lds);  // [2][256]
+  float tops[kAcross], sums[kAcross];  // from a round to the next
+  // The powers of 16 kDown / kRounds entries at a time, as many as LDS holds.
+  using E = Power<T>;
+  constexpr int kRounds = KEEP ? sizeof(E) / 2 : 1;
+  constexpr int kPart = kDown / kRounds;
   // ENDS: the vocabulary ends in this half of the tile
-  const auto reduce = [&](auto ends) {
+  const auto reduce = [&](auto ends, auto at) {
     constexpr bool ENDS = decltype(ends)::value;
+    constexpr int round = decltype(at)::value;
     const int last = limit - 4 * (lane / 16);  // entries below it count
 #pragma unroll
     for (int j = 0; j < kAcross; ++j) {
       const int column = (wave / 2) * (16 * kAcross) + j * 16 + lane % 16;
-      const int row = tile.b * kTile + column;
-      const int64_t from_v0 = g.target[min(row, count - 1)] - v0;
-      const int rel = row < count && from_v0 >= 0 && from_v0 < 128 ? static_cast<int>(from_v0) : -1;
-      float top = -__builtin_inff();
-#pragma unroll
-      for (int i = 0; i < kDown; ++i) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) top = fmaxf(top, !ENDS || i * 16 + e < last ? acc[i][j][e] : -__builtin_inff());
-      }
-      top = fmaxf(top, __shfl_xor(top, 16, 64));
-      top = reference(logit(fmaxf(top, __shfl_xor(top, 32, 64))));
-      if (__any(rel >= 0)) {
-        float own = 0.0f;
+      float top, sum = 0.0f;
+      if constexpr (round == 0) {
+        const int row = tile.b * kTile + column;
+        const int64_t from_v0 = g.target[min(row, count - 1)] - v0;
+        const int rel = row < count && from_v0 >= 0 && from_v0 < 128 ? static_cast<int>(from_v0) : -1;
+        float x = -__builtin_inff();
 #pragma unroll
         for (int i = 0; i < kDown; ++i) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) own = i * 16 + e == rel - 4 * (lane / 16) ? acc[i][j][e] : own;
+          for (int e = 0; e < 4; ++e) x = fmaxf(x, !ENDS || i * 16 + e < last ? acc[i][j][e] : -__builtin_inff());
         }
-        if (rel >= 0 && (rel >> 2 & 3) == lane / 16) g.target_logit[row] = logit(own);
+        x = fmaxf(x, __shfl_xor(x, 16, 64));
+        top = reference<T>(logit(fmaxf(x, __shfl_xor(x, 32, 64))));
+        if (__any(rel >= 0)) {
+          float own = 0.0f;
+#pragma unroll
+          for (int i = 0; i < kDown; ++i) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) own = i * 16 + e == rel - 4 * (lane / 16) ? acc[i][j][e] : own;
+          }
+          if (rel >= 0 && (rel >> 2 & 3) == lane / 16) g.target_logit[row] = logit(own);
+        }
+      } else {
+        top = tops[j];
+        sum = sums[j];
       }
       const float from = top == -__builtin_inff() ? 0.0f : top;  // nothing but NaN, or nothing at all
-      float sum = 0.0f;
 #pragma unroll
-      for (int i = 0; i < kDown; ++i) {
+      for (int i = 0; i < kPart; ++i) {
+        float x[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float x = power(logit.above(acc[i][j][e], from));
-          sum += !ENDS || i * 16 + e < last ? x : 0.0f;
+          x[e] = power(logit.above(acc[round * kPart + i][j][e], from));
+          if (ENDS) x[e] = (round * kPart + i) * 16 + e < last ? x[e] : 0.0f;
+          sum += x[e];
+        }
+        if constexpr (KEEP && std::is_same_v<E, F16>) {
+          const int chunk = (wave % 2) * 16 + i * 2 + lane / 32;
+          *reinterpret_cast<uint64_t*>(lds + staged(column, chunk) * 8 + (lane / 16 % 2) * 4) =
+              static_cast<uint64_t>(pack2<F16>(x[2], x[3])) << 32 | pack2<F16>(x[0], x[1]);
+        } else if constexpr (KEEP) {
+          *reinterpret_cast<f32x4*>(lds + staged(column, (wave % 2) * 16 + i * 4 + lane / 16) * 8) = f32x4{x[0], x[1], x[2], x[3]};
+        }
+        if (KEEP && i % 2 == 1) __builtin_amdgcn_sched_barrier(0);  // a few outputs at a time: no registers to spill
+      }
+      if constexpr (round < kRounds - 1) {
+        tops[j] = top;
+        sums[j] = sum;
+      } else {
+        sum += __shfl_xor(sum, 16, 64);
+        sum += __shfl_xor(sum, 32, 64);
+        if (lane < 16) {
+          g.sums[(static_cast<int64_t>(tile.a) * 2 + wave % 2) * g.row_tiles + tile.b * kTile + column] = f32x2{top, sum};
         }
       }
-      sum += __shfl_xor(sum, 16, 64);
-      sum += __shfl_xor(sum, 32, 64);
-      if (lane < 16) meet[(wave % 2) * kTile + column] = f32x2{top, sum};
-      __builtin_amdgcn_sched_barrier(0);  // one column's outputs at a time: no registers to spill
+      __builtin_amdgcn_sched_barrier(0);
     }
   };
-  if (limit < 128) {
-    reduce(std::true_type{});
-  } else {
-    reduce(std::false_type{});
-  }
-  __syncthreads();
-  if (threadIdx.x < kTile) {
-    g.sums[static_cast<int64_t>(tile.a) * g.row_tiles + tile.b * kTile + threadIdx.x] =
-        join(meet[threadIdx.x], meet[kTile + threadIdx.x]);
+  const auto pass = [&](auto at) {
+    constexpr int round = decltype(at)::value;
+    if (limit < 128) {
+      reduce(std::true_type{}, at);
+    } else {
+      reduce(std::false_type{}, at);
+    }
+    if constexpr (KEEP) {
+      __syncthreads();
+      constexpr int kChunk = 16 / sizeof(E);
+      for (int k = threadIdx.x; k < kTile * 32; k += kThreads) {
+        const int column = k / 32, chunk = k % 32;
+        const u32x4 x = *reinterpret_cast<const u32x4*>(lds + staged(column, chunk) * 8);
+        const int entry = chunk / 16 * 128 + round * 16 * kPart + chunk % 16 * kChunk;
+        E* to = static_cast<E*>(g.powers) + (static_cast<int64_t>(tile.b) * kTile + column) * g.powers_ld +
+                static_cast<int64_t>(tile.a) * kTile + entry;
+        __builtin_nontemporal_store(x, reinterpret_cast<u32x4*>(to));
+      }
+    }
+  };
+  pass(std::integral_constant<int, 0>{});
+  if constexpr (kRounds == 2) {
+    __syncthreads();
+    pass(std::integral_constant<int, 1>{});
   }
 }
 
-// 16-byte slot of a staged output row of 512 bytes: a permutation per row, so that 32 lanes
-// writing one chunk of 32 rows meet 32 different slots.
-__device__ __forceinline__ int staged(int row, int chunk) { return row * 32 + (chunk ^ (row & 31)); }
+// Backward of kept powers: P of a piece's columns, read from the powers and written as operands.  16 rows of 512
+// columns per workgroup, 8 columns per thread and row.
+constexpr int kScaleRows = 16, kScaleColumns = 64 * kVec;
+
+template <class E, class T, int PARTS>
+__global__ void __launch_bounds__(kBlock) attnres_loss_rescale_kernel(LogitArgs g, int64_t columns, int column_blocks) {
+  const int count = *g.product.count;
+  const int64_t row0 = static_cast<int64_t>(blockIdx.x / column_blocks) * kScaleRows + threadIdx.x / 64;
+  const int64_t column = static_cast<int64_t>(blockIdx.x % column_blocks) * kScaleColumns + threadIdx.x % 64 * kVec;
+  if (row0 >= round_up(count, kTile) || column >= columns) return;
+  constexpr int kRounds = kScaleRows / (kBlock / 64);
+  const int64_t v = g.first + column;
+  const E* powers = static_cast<const E*>(g.powers);
+  Chunk<E> chunk[kRounds];
+  float factor[kRounds], by[kRounds];
+  int64_t rel[kRounds];
+#pragma unroll
+  for (int k = 0; k < kRounds; ++k) {
+    const int64_t row = row0 + k * (kBlock / 64);
+    chunk[k].load_past(powers + row * g.powers_ld + v);
+    const int64_t at = row < count ? row : count - 1;
+    const f32x2 sum = g.sums[v / 128 * g.row_tiles + row], stats = g.stats[at];
+    by[k] = g.row_scale[row];
+    factor[k] = row < count ? power(sum.x - stats.x) * stats.y * by[k] : 0.0f;
+    rel[k] = g.target[at] - v;
+  }
+#pragma unroll
+  for (int k = 0; k < kRounds; ++k) {
+    const int64_t row = row0 + k * (kBlock / 64);
+    float x[kVec];
+    chunk[k].unpack(x);
+#pragma unroll
+    for (int e = 0; e < kVec; ++e) {
+      x[e] = row < count ? x[e] * factor[k] : 0.0f;
+      if (rel[k] == e) x[e] -= by[k];  // 0 past the last row
+      if (PARTS == 2) asm("" : "+v"(x[e]));  // one rounding to hi, as in the recomputed probabilities
+    }
+#pragma unroll
+    for (int part = 0; part < PARTS; ++part) {
+      u32x4 packed;
+#pragma unroll
+      for (int e = 0; e < kVec / 2; ++e) {
+        packed[e] = pack2<T>(x[2 * e], x[2 * e + 1]);
+        x[2 * e] -= to_f32(T{static_cast<uint16_t>(packed[e] & 0xffffu)});  // lo
+        x[2 * e + 1] -= to_f32(T{static_cast<uint16_t>(packed[e] >> 16)});
+      }
+      __builtin_nontemporal_store(packed, reinterpret_cast<u32x4*>(g.p[part] + row * g.p_ld + column));
+    }
+  }
+}
 
 // Backward: P of a tile, rounded to the operands' type.
 template <class T, int SEGMENTS>
@@ -906,12 +1015,12 @@ __global__ void __launch_bounds__(kFewBlock) attnres_loss_few_kernel(FewArgs<X> 
     }
     top = fmaxf(top, __shfl_xor(top, 16, 64));
     top = fmaxf(top, __shfl_xor(top, 32, 64));
-    top = reference(top);
+    top = reference<float>(top);
     const float from = top == -__builtin_inff() ? 0.0f : top;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) sum += counts[i][e] ? power(__builtin_fmaf(acc[i][t][e], kLog2e, -from)) : 0.0f;
+      for (int e = 0; e < 4; ++e) sum += counts[i][e] ? power(over_ln2(acc[i][t][e]) - from) : 0.0f;
     }
     sum += __shfl_xor(sum, 16, 64);
     sum += __shfl_xor(sum, 32, 64);
@@ -1036,7 +1145,9 @@ __global__ void __launch_bounds__(kBlock) attnres_loss_reduce_kernel(const f32x2
   const bool known = s.target[at] >= 0;
   s.stats[at] = f32x2{total.x, known ? 1.0f / total.y : __builtin_nanf("")};
   // both terms are small where the target's probability is near one, and the loss is not below zero
-  const float value = kLn2 * (log2f(total.y) - __builtin_fmaf(target_logit[column], kLog2e, -total.x));
+  const int up = fabsf(total.x) < 4194304.0f ? __builtin_amdgcn_frexp_expf(total.y) : 0;  // total.x + up: exact
+  const float rest = over_ln2(target_logit[column]) - (total.x + static_cast<float>(up));
+  const float value = kLn2 * (log2f(ldexpf(total.y, -up)) - rest);
   loss[row] = !known ? __builtin_nanf("") : value < 0.0f ? 0.0f : value;
 }
 
@@ -1127,6 +1238,7 @@ constexpr int64_t kMaxRows = int64_t{1} << 24;
 constexpr int64_t kMaxVocab = int64_t{1} << 24;
 constexpr int64_t kMaxStride = int64_t{1} << 22;  // of W multiplied in place: 256 rows stay within 32-bit offsets
 constexpr int64_t kPieceBytes = int64_t{512} << 20;  // of P at a time
+constexpr int64_t kKeepBytes = int64_t{8} << 30;     // of powers kept for the backward
 constexpr int kUnits = 256;                          // compute units, one workgroup each
 
 // How many parts the depth of a gradient product is cut into, so that its workgroups fill the chip: what takes the
@@ -1152,15 +1264,16 @@ int choose_splits(int64_t tiles, int64_t depth, int segments, bool direct) {
 int64_t few_rows(bool pack_weight) { return pack_weight ? kFewRows : kFewRows / 2; }
 
 struct LossPlan {
-  bool split, pack_weight, few;
+  bool split, pack_weight, few, keep;
   int64_t rows_pad, width_pad, vocab_pad, piece;
   int64_t hidden[2], weight[2], sums, target_logit, losses;  // offsets
   int64_t row_scale, alpha, p[2], dh, dw;
   int splits_h, splits_w;
   int64_t bytes;
+  int64_t saved_sums, saved_powers, saved_bytes;
 };
 
-LossPlan loss_plan(int64_t rows, int64_t vocab, int64_t width, int dtype, bool backward) {
+LossPlan loss_plan(int64_t rows, int64_t vocab, int64_t width, int dtype, bool keep, bool backward) {
   LossPlan p{};
   p.split = dtype == ATTNRES_F32;
   p.pack_weight = p.split || width % kDepth != 0;
@@ -1175,13 +1288,22 @@ LossPlan loss_plan(int64_t rows, int64_t vocab, int64_t width, int dtype, bool b
     return from;
   };
   p.few = rows <= few_rows(p.pack_weight);
+  const int64_t powers = (dtype == ATTNRES_BF16 ? 2 : 4) * p.rows_pad * p.vocab_pad;
+  p.keep = keep && !p.few && powers <= kKeepBytes;
+  p.saved_bytes = kHeaderBytes + 20 * rows;
+  if (p.keep) {
+    p.saved_sums = round_up(p.saved_bytes, 256);
+    p.saved_powers = p.saved_sums + 8 * (p.vocab_pad / 128) * p.rows_pad;
+    p.saved_bytes = p.saved_powers + powers;
+  }
   const bool few = !backward && p.few;
   if (!few) {
     for (int k = 0; k < parts; ++k) p.hidden[k] = take(2 * p.rows_pad * p.width_pad);
     for (int k = 0; p.pack_weight && k < parts; ++k) p.weight[k] = take(2 * vocab * p.width_pad);
   }
   if (!backward) {
-    p.sums = take(few ? 8 * ((vocab + kFewWords - 1) / kFewWords) * kFewRows : 8 * (p.vocab_pad / kTile) * p.rows_pad);
+    if (few) p.sums = take(8 * ((vocab + kFewWords - 1) / kFewWords) * kFewRows);
+    else if (!p.keep) p.sums = take(8 * (p.vocab_pad / 128) * p.rows_pad);
     p.target_logit = take(4 * p.rows_pad);
     p.losses = take(4 * rows);
   } else {
@@ -1199,6 +1321,14 @@ LossPlan loss_plan(int64_t rows, int64_t vocab, int64_t width, int dtype, bool b
   }
   p.bytes = at;
   return p;
+}
+
+Saved saved_views(void* base, int64_t rows, const LossPlan& p) {
+  char* from = static_cast<char*>(base);
+  char* at = from + kHeaderBytes;
+  return {reinterpret_cast<Header*>(from), reinterpret_cast<f32x2*>(at), reinterpret_cast<int32_t*>(at + 8 * rows),
+          reinterpret_cast<int32_t*>(at + 12 * rows), reinterpret_cast<int32_t*>(at + 16 * rows),
+          p.keep ? reinterpret_cast<f32x2*>(from + p.saved_sums) : nullptr, p.keep ? from + p.saved_powers : nullptr};
 }
 
 unsigned stride_grid(int64_t items) { return static_cast<unsigned>(std::min<int64_t>((items + kBlock - 1) / kBlock, 8192)); }
@@ -1261,7 +1391,7 @@ void loss_forward(const Call& c, const void* targets, int target_bytes, int64_t 
                        ignore_index, c.saved);
   }
   if (c.rows > 0) {
-    f32x2* sums = c.at<f32x2>(p.sums);
+    f32x2* sums = p.keep ? c.saved.sums : c.at<f32x2>(p.sums);
     float* target_logit = c.at<float>(p.target_logit);
     int tiles;
     int64_t row_tiles;
@@ -1280,7 +1410,8 @@ void loss_forward(const Call& c, const void* targets, int target_bytes, int64_t 
       prepare_operands<X>(c, true, &g.product.b, &g.product.a);
       g.product.count = &c.saved.header->count;
       g.product.depth = p.width_pad;
-      g.product.tiles_a = tiles = static_cast<int>(p.vocab_pad / kTile);
+      g.product.tiles_a = static_cast<int>(p.vocab_pad / kTile);
+      tiles = 2 * g.product.tiles_a;
       g.product.tiles_b = static_cast<int>(p.rows_pad / kTile);
       g.product.splits = 1;
       g.header = c.saved.header;
@@ -1289,7 +1420,10 @@ void loss_forward(const Call& c, const void* targets, int target_bytes, int64_t 
       g.row_tiles = row_tiles = p.rows_pad;
       g.sums = sums;
       g.target_logit = target_logit;
-      hipLaunchKernelGGL((attnres_loss_logits_kernel<T, SEGMENTS>), dim3(g.product.tiles_a * g.product.tiles_b), dim3(kThreads), 0,
+      g.powers = c.saved.powers;
+      g.powers_ld = p.vocab_pad;
+      const auto kernel = p.keep ? attnres_loss_logits_kernel<T, SEGMENTS, true> : attnres_loss_logits_kernel<T, SEGMENTS, false>;
+      hipLaunchKernelGGL(kernel, dim3(g.product.tiles_a * g.product.tiles_b), dim3(kThreads), 0,
                          c.stream, g);
     }
     float* losses = reduction == ATTNRES_REDUCE_NONE ? loss : c.at<float>(p.losses);
@@ -1333,7 +1467,18 @@ void loss_backward(const Call& c, int reduction, const float* grad_loss, void* g
     g.row_scale = row_scale;
     for (int k = 0; k < kParts; ++k) g.p[k] = c.at<uint16_t>(p.p[k]);
     g.p_ld = p.piece;
-    hipLaunchKernelGGL((attnres_loss_probability_kernel<T, SEGMENTS>), dim3(tiles_v * tiles_n), dim3(kThreads), 0, c.stream, g);
+    if (p.keep) {
+      using E = Power<T>;
+      g.sums = c.saved.sums;
+      g.powers = c.saved.powers;
+      g.powers_ld = p.vocab_pad;
+      const int64_t wide = static_cast<int64_t>(tiles_v) * kTile;
+      const int blocks = static_cast<int>((wide + kScaleColumns - 1) / kScaleColumns);
+      hipLaunchKernelGGL((attnres_loss_rescale_kernel<E, T, kParts>), dim3(static_cast<unsigned>(p.rows_pad / kScaleRows * blocks)),
+                         dim3(kBlock), 0, c.stream, g, wide, blocks);
+    } else {
+      hipLaunchKernelGGL((attnres_loss_probability_kernel<T, SEGMENTS>), dim3(tiles_v * tiles_n), dim3(kThreads), 0, c.stream, g);
+    }
     if (grad_weight != nullptr) {
       Operand a = h, b = probability;
       a.entries = p.width_pad;
@@ -1392,6 +1537,11 @@ bool fits_grid(int64_t rows, int64_t vocab) {
   return (rows + kTile - 1) / kTile * ((vocab + kTile - 1) / kTile) <= kMaxTiles;
 }
 
+bool known_shape(int64_t rows, int64_t vocab, int64_t width, int dtype) {
+  return rows >= 0 && rows <= kMaxRows && vocab >= 1 && vocab <= kMaxVocab && width >= 1 && width <= ATTNRES_MAX_WIDTH &&
+         dtype_known(dtype) && fits_grid(rows, vocab);
+}
+
 // Offsets into both are multiples of 16 bytes, which the products' loads into LDS need.
 int check_places(const void* saved, const void* workspace, int64_t workspace_bytes, int64_t need) {
   if (workspace == nullptr || workspace_bytes < need) {
@@ -1435,27 +1585,26 @@ using namespace attnres_hip::layers;
 
 extern "C" {
 
-int64_t attnres_hip_loss_saved_bytes(int64_t rows) { return rows < 0 || rows > kMaxRows ? -1 : saved_bytes(rows); }
+int64_t attnres_hip_loss_saved_bytes(int64_t rows, int64_t vocab, int64_t width, int dtype, int keep) {
+  return known_shape(rows, vocab, width, dtype) ? loss_plan(rows, vocab, width, dtype, keep != 0, false).saved_bytes : -1;
+}
 
-int64_t attnres_hip_loss_workspace_bytes(int64_t rows, int64_t vocab, int64_t width, int dtype, int backward) {
-  if (rows < 0 || rows > kMaxRows || vocab < 1 || vocab > kMaxVocab || width < 1 || width > ATTNRES_MAX_WIDTH || !dtype_known(dtype) ||
-      !fits_grid(rows, vocab)) {
-    return -1;
-  }
-  return loss_plan(rows, vocab, width, dtype, backward != 0).bytes;
+int64_t attnres_hip_loss_workspace_bytes(int64_t rows, int64_t vocab, int64_t width, int dtype, int keep, int backward) {
+  return known_shape(rows, vocab, width, dtype) ? loss_plan(rows, vocab, width, dtype, keep != 0, backward != 0).bytes : -1;
 }
 
 int attnres_hip_loss_forward(const void* hidden, int64_t hidden_stride, const void* weight, int64_t weight_stride,
                              const void* targets, int target_bytes, int64_t rows, int64_t vocab, int64_t width, int dtype,
-                             int64_t ignore_index, int reduction, float* loss, void* saved, void* workspace,
+                             int64_t ignore_index, int reduction, int keep, float* loss, void* saved, void* workspace,
                              int64_t workspace_bytes, void* stream) {
   if (const int status = check_loss(hidden, hidden_stride, weight, weight_stride, rows, vocab, width, dtype, reduction)) return status;
   if (target_bytes != 4 && target_bytes != 8) return layer_error(ATTNRES_ERR_SHAPE, "targets must be int32 or int64");
   if (loss == nullptr || saved == nullptr || (rows > 0 && targets == nullptr)) {
     return layer_error(ATTNRES_ERR_NULL_POINTER, "targets, loss or saved is NULL");
   }
-  const Call c{hidden, hidden_stride, weight, weight_stride, rows, vocab, width, loss_plan(rows, vocab, width, dtype, false),
-               saved_views(saved, rows), static_cast<char*>(workspace), static_cast<hipStream_t>(stream)};
+  const LossPlan plan = loss_plan(rows, vocab, width, dtype, keep != 0, false);
+  const Call c{hidden, hidden_stride, weight, weight_stride, rows, vocab, width, plan, saved_views(saved, rows, plan),
+               static_cast<char*>(workspace), static_cast<hipStream_t>(stream)};
   if (const int status = check_places(saved, workspace, workspace_bytes, c.plan.bytes)) return status;
   if (dtype == ATTNRES_BF16) loss_forward<Bf16, Bf16, 1>(c, targets, target_bytes, ignore_index, reduction, loss);
   else if (dtype == ATTNRES_F16) loss_forward<F16, F16, 1>(c, targets, target_bytes, ignore_index, reduction, loss);
@@ -1464,12 +1613,14 @@ int attnres_hip_loss_forward(const void* hidden, int64_t hidden_stride, const vo
 }
 
 int attnres_hip_loss_backward(const void* hidden, int64_t hidden_stride, const void* weight, int64_t weight_stride, int64_t rows,
-                              int64_t vocab, int64_t width, int dtype, int reduction, void* saved, const float* grad_loss,
-                              void* grad_hidden, void* grad_weight, void* workspace, int64_t workspace_bytes, void* stream) {
+                              int64_t vocab, int64_t width, int dtype, int reduction, int keep, void* saved,
+                              const float* grad_loss, void* grad_hidden, void* grad_weight, void* workspace,
+                              int64_t workspace_bytes, void* stream) {
   if (const int status = check_loss(hidden, hidden_stride, weight, weight_stride, rows, vocab, width, dtype, reduction)) return status;
   if (saved == nullptr || grad_loss == nullptr) return layer_error(ATTNRES_ERR_NULL_POINTER, "saved or grad_loss is NULL");
-  const Call c{hidden, hidden_stride, weight, weight_stride, rows, vocab, width, loss_plan(rows, vocab, width, dtype, true),
-               saved_views(saved, rows), static_cast<char*>(workspace), static_cast<hipStream_t>(stream)};
+  const LossPlan plan = loss_plan(rows, vocab, width, dtype, keep != 0, true);
+  const Call c{hidden, hidden_stride, weight, weight_stride, rows, vocab, width, plan, saved_views(saved, rows, plan),
+               static_cast<char*>(workspace), static_cast<hipStream_t>(stream)};
   if (const int status = check_places(saved, workspace, workspace_bytes, c.plan.bytes)) return status;
   if (grad_hidden == nullptr && grad_weight == nullptr) return ATTNRES_OK;
   if (dtype == ATTNRES_BF16) loss_backward<Bf16, Bf16, 1>(c, reduction, grad_loss, grad_hidden, grad_weight);

@@ -97,7 +97,7 @@ def embedding(tokens, weight, positions, scale, grad):
     return outs, bounds
 
 
-def loss(hidden, weight, targets, ignore_index, reduction, grad):
+def loss(hidden, weight, targets, ignore_index, reduction, grad, recompute=False):
     """(loss, dH, dW) and bounds.
 
     A logit adds D products, exact in FP32 for 16-bit inputs: off by at most D roundings of
@@ -106,6 +106,11 @@ def loss(hidden, weight, targets, ignore_index, reduction, grad):
     error (its own and the sum's), 16 roundings of the exponential, the reciprocal and the factors,
     and its storage: half a step of the operands' type (FP32: of 24 bits), or 2^-39 of
     the largest upstream gradient where FP16 runs out of exponents.
+
+    Without `recompute` the exponentials of BF16 inputs have been rounded to FP16 before: relative to the largest of
+    128, which is at most 2^15.5 then, off by 2^-11 of their own or, below the normal numbers, by 2^-25; so a
+    probability is off by 2^-11 of its own or by 2^-25 / 2^15 times at most 2^1.5 (the references are off by half a power of two
+    from either's largest).
     """
     dtype = hidden.dtype
     width, vocab = weight.shape[1], weight.shape[0]
@@ -141,7 +146,9 @@ def loss(hidden, weight, targets, ignore_index, reduction, grad):
     # row's factor times a probability below it (over a power of two of at most twice the largest
     # upstream gradient); three such losses stay below 2^-124 of that gradient
     off_p = off_p + 2.0**-124 * upstream.abs().amax() * kept[:, None]
-    if dtype != torch.bfloat16:
+    if dtype == torch.bfloat16 and not recompute:
+        off_p = off_p + (1 + HALF_STEP[dtype]) * 2.0**-11 * soft
+    if dtype != torch.bfloat16 or not recompute:
         off_p = off_p + 2.0**-38 * upstream.abs().amax() * kept[:, None]
     k = 16 * U32  # factors of the outputs, splits and pieces
     grad_hidden, grad_weight = p @ w, p.T @ h

@@ -236,14 +236,14 @@ def _loss_inputs(seed, rows, width, vocab, dtype, ignored=0.0):
     return g, hidden, weight, targets
 
 
-def _check_loss(hidden, weight, targets, reduction, g, ignore_index=-100):
+def _check_loss(hidden, weight, targets, reduction, g, ignore_index=-100, recompute=False):
     leaves = (hidden.requires_grad_(True), weight.requires_grad_(True))
-    out = layers.linear_cross_entropy(*leaves, targets, ignore_index=ignore_index, reduction=reduction)
+    out = layers.linear_cross_entropy(*leaves, targets, ignore_index=ignore_index, reduction=reduction, recompute=recompute)
     assert out.dtype == FP32 and out.shape == (targets.shape if reduction == "none" else ())
     grad = _randn(g, *out.shape) if out.dim() else _randn(g, 1)[0]
     grads = torch.autograd.grad(out, leaves, grad)
     with torch.no_grad():
-        values, bounds = reference.loss(hidden, weight, targets, ignore_index, reduction, grad)
+        values, bounds = reference.loss(hidden, weight, targets, ignore_index, reduction, grad, recompute)
         scored = layers.linear_cross_entropy(*leaves, targets, ignore_index=ignore_index, reduction=reduction)
     assert torch.equal(scored, out.detach()) or bool(out.isnan().any())
     for name, actual, value, bound in zip(("loss", "dH", "dW"), (out.detach(), *grads), values, bounds):
@@ -254,23 +254,26 @@ def _check_loss(hidden, weight, targets, reduction, g, ignore_index=-100):
                                               (257, 100, 1000), (300, 1000, 513), (16, 1024, 5001), (600, 320, 2049),
                                               (70, 4096, 300), (33, 8192, 129), (1500, 24, 96)])
 @pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
-def test_loss(rows, width, vocab, dtype):
+@pytest.mark.parametrize("recompute", [False, True])
+def test_loss(rows, width, vocab, dtype, recompute):
     g, hidden, weight, targets = _loss_inputs(rows + width + vocab, rows, width, vocab, dtype)
-    _check_loss(hidden, weight, targets, "mean", g)
+    _check_loss(hidden, weight, targets, "mean", g, recompute=recompute)
 
 
 @pytest.mark.parametrize("reduction", ["none", "sum", "mean"])
 @pytest.mark.parametrize("ignored", [0.3, 0.95])
 @pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
-def test_loss_with_ignored_targets(reduction, ignored, dtype):
+@pytest.mark.parametrize("recompute", [False, True])
+def test_loss_with_ignored_targets(reduction, ignored, dtype, recompute):
     g, hidden, weight, targets = _loss_inputs(31, 700, 200, 900, dtype, ignored)
-    _check_loss(hidden, weight, targets, reduction, g)
+    _check_loss(hidden, weight, targets, reduction, g, recompute=recompute)
 
 
-def test_loss_in_several_pieces_of_the_vocabulary():
+@pytest.mark.parametrize("recompute", [False, True])
+def test_loss_in_several_pieces_of_the_vocabulary(recompute):
     """More probabilities than are formed at once."""
     g, hidden, weight, targets = _loss_inputs(37, 4096, 64, 70001, BF16, 0.1)
-    _check_loss(hidden, weight, targets, "mean", g)
+    _check_loss(hidden, weight, targets, "mean", g, recompute=recompute)
 
 
 def test_loss_fp32_in_several_pieces_of_the_vocabulary():
@@ -308,7 +311,8 @@ def test_loss_does_not_look_at_ignored_rows(dtype):
     masked = targets == -100
     hidden[masked] = torch.where(torch.rand(int(masked.sum()), 128, generator=g, device="cuda") < 0.5, NAN, float("inf")).to(dtype)
     hidden[masked.nonzero()[0]] = torch.finfo(dtype).max
-    _check_loss(hidden, weight, targets, "none", g)
+    for recompute in (False, True):
+        _check_loss(hidden.detach(), weight.detach(), targets, "none", g, recompute=recompute)
 
 
 def test_loss_of_a_nonfinite_row_stays_in_its_own():
@@ -320,12 +324,13 @@ def test_loss_of_a_nonfinite_row_stays_in_its_own():
     assert torch.equal(out[keep], clean[keep]) and bool(out[7].isnan())
 
 
-def test_loss_marks_a_target_outside_the_vocabulary():
+@pytest.mark.parametrize("recompute", [False, True])
+def test_loss_marks_a_target_outside_the_vocabulary(recompute):
     g, hidden, weight, targets = _loss_inputs(53, 300, 128, 600, BF16)
     clean = layers.linear_cross_entropy(hidden, weight, targets, reduction="none")
     targets[4], targets[9], targets[200] = 600, -1, 2**33
     hidden.requires_grad_(True), weight.requires_grad_(True)
-    out = layers.linear_cross_entropy(hidden, weight, targets, reduction="none")
+    out = layers.linear_cross_entropy(hidden, weight, targets, reduction="none", recompute=recompute)
     bad = torch.zeros(300, device="cuda", dtype=torch.bool)
     bad[[4, 9, 200]] = True
     assert torch.equal(out.isnan(), bad) and torch.equal(out[~bad], clean[~bad])
@@ -341,13 +346,32 @@ def test_loss_of_large_logits(dtype):
     with torch.no_grad():
         hidden.mul_(300.0)
         targets[:100] = (hidden[:100].float() @ weight.float().T).argmax(-1)
-    _check_loss(hidden, weight, targets, "none", g)
+    for recompute in (False, True):
+        _check_loss(hidden.detach(), weight.detach(), targets, "none", g, recompute=recompute)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+def test_loss_of_huge_logits(dtype):
+    """Logits beyond 2^24, whose neighbours are more than 1 apart: rows of equal logits, whose losses are log V, and rows whose
+    target's logit is the largest, whose losses are 0.  Bounds: a few roundings of numbers up to 16."""
+    hidden = torch.tensor([[0.0, 2.0**26], [2.0**26, 0.0]], device="cuda").to(dtype).repeat(40, 1)
+    weight = torch.stack((torch.linspace(-8, 8, 300, device="cuda").to(dtype), torch.ones(300, device="cuda", dtype=dtype)), 1)
+    targets = torch.full((80,), 299, device="cuda")
+    for recompute in (False, True):
+        h, w = hidden.clone().requires_grad_(True), weight.clone().requires_grad_(True)
+        out = layers.linear_cross_entropy(h, w, targets, reduction="none", recompute=recompute)
+        (grad,) = torch.autograd.grad(out, h, torch.ones_like(out))
+        assert bool((out[0::2] - torch.tensor(300.0).log().cuda()).abs().max() <= 2.0**-18)
+        assert bool((out[1::2] >= 0).all()) and bool(out[1::2].max() <= 2.0**-18)
+        # P of the second kind of rows is 0 but for roundings of its one entry, 1 - 1: 2^-8 of weights up to 8
+        assert bool(grad[1::2].abs().max() <= 8 * (2.0**-8 if dtype == BF16 else 2.0**-20))
 
 
 @pytest.mark.parametrize("scale_h,scale_w", [(1e-6, 1.0), (1e-20, 1e18), (1e12, 1e-13), (0.0, 1.0), (1.0, 0.0)])
 def test_loss_fp32_over_the_exponents(scale_h, scale_w):
     g, hidden, weight, targets = _loss_inputs(61, 130, 96, 400, FP32)
-    _check_loss(hidden * scale_h, weight * scale_w, targets, "sum", g)
+    for recompute in (False, True):
+        _check_loss(hidden * scale_h, weight * scale_w, targets, "sum", g, recompute=recompute)
 
 
 @pytest.mark.parametrize("layout", ["slices", "misaligned", "transposed", "batched", "columns"])
@@ -395,20 +419,20 @@ def test_loss_without_rows_through_the_c_abi(dtype):
     lib = _native.load()
     vocab, width, mean = 300, 40, 2
     weight = _randn(_generator(6), vocab, width).to((BF16, FP16, FP32)[dtype])
-    saved = torch.empty(lib.attnres_hip_loss_saved_bytes(0), dtype=torch.uint8, device="cuda")
+    saved = torch.empty(lib.attnres_hip_loss_saved_bytes(0, vocab, width, dtype, 1), dtype=torch.uint8, device="cuda")
     loss, grad = torch.zeros((), device="cuda"), torch.ones((), device="cuda")
     grad_weight = torch.full_like(weight, 7.0)
     stream = torch.cuda.current_stream().cuda_stream
     for backward in (0, 1):
-        size = lib.attnres_hip_loss_workspace_bytes(0, vocab, width, dtype, backward)
+        size = lib.attnres_hip_loss_workspace_bytes(0, vocab, width, dtype, 1, backward)
         workspace = torch.empty(size, dtype=torch.uint8, device="cuda")
         if backward:
-            status = lib.attnres_hip_loss_backward(None, width, weight.data_ptr(), width, 0, vocab, width, dtype, mean,
+            status = lib.attnres_hip_loss_backward(None, width, weight.data_ptr(), width, 0, vocab, width, dtype, mean, 1,
                                                    saved.data_ptr(), grad.data_ptr(), None, grad_weight.data_ptr(),
                                                    workspace.data_ptr(), size, stream)
         else:
             status = lib.attnres_hip_loss_forward(None, width, weight.data_ptr(), width, None, 8, 0, vocab, width, dtype, -100,
-                                                  mean, loss.data_ptr(), saved.data_ptr(), workspace.data_ptr(), size, stream)
+                                                  mean, 1, loss.data_ptr(), saved.data_ptr(), workspace.data_ptr(), size, stream)
         assert status == 0, lib.attnres_hip_last_error().decode()
     assert bool(loss.isnan()) and not grad_weight.any()
 

@@ -74,6 +74,7 @@ def test_cpu_tensors_are_refused_after_everything_else(call):
     (lambda: _loss(ignore_index=1.0), TypeError, "ignore_index"),
     (lambda: _loss(ignore_index=True), TypeError, "ignore_index"),
     (lambda: _loss(reduction="max"), ValueError, "reduction"),
+    (lambda: _loss(recompute=1), TypeError, "recompute"),
 ])
 def test_refusals(call, error, match):
     with pytest.raises(error, match=match):
@@ -99,11 +100,20 @@ def test_fake_kernels():
         assert grads[0].shape == (10, 64) and grads[0].dtype == FP32
         head = torch.empty(10, 64, device="cuda", dtype=BF16)
         for code, shape in ((0, (2, 3)), (1, ()), (2, ())):
-            loss, saved = torch.ops.attnres_hip.linear_cross_entropy(x, head, tokens, -100, code)
+            loss, saved = torch.ops.attnres_hip.linear_cross_entropy(x, head, tokens, -100, code, True)
             assert loss.shape == shape and loss.dtype == FP32
-            assert saved.numel() == _native.load().attnres_hip_loss_saved_bytes(6)
-        grads = torch.ops.attnres_hip.linear_cross_entropy_backward(loss, x, head, saved, 2, True, False)
+        grads = torch.ops.attnres_hip.linear_cross_entropy_backward(loss, x, head, saved, 2, True, True, False)
         assert grads[0].shape == x.shape and grads[1].shape == (0,)
+
+
+@pytest.mark.parametrize("rows", [0, 1, 32, 33, 64, 65, 256, 257, 32768])
+@pytest.mark.parametrize("vocab,width", [(1, 64), (257, 33), (131072, 2048), (131073, 64)])
+@pytest.mark.parametrize("dtype", [BF16, torch.float16, FP32])
+@pytest.mark.parametrize("keep", [False, True])
+def test_saved_bytes_of_the_fake_kernel(rows, vocab, width, dtype, keep):
+    code = (BF16, torch.float16, FP32).index(dtype)
+    expected = _native.load().attnres_hip_loss_saved_bytes(rows, vocab, width, code, keep)
+    assert layers._loss_saved_bytes(rows, vocab, width, dtype, keep) == expected
 
 
 # ---------------------------------------------------------------------- C ABI
@@ -143,10 +153,10 @@ def _status(name, **overrides):
                                    weight_dtype=0, scale=1.0, grad_weight=_FAKE, grad_positions=None, position_rows=0,
                                    workspace=_FAKE, bytes=1 << 30, stream=None),
         "loss_forward": dict(hidden=_FAKE, hidden_stride=64, weight=_FAKE, weight_stride=64, targets=_FAKE, target_bytes=8, rows=3,
-                             vocab=10, width=64, dtype=0, ignore_index=-100, reduction=2, loss=_FAKE, saved=_FAKE, workspace=_FAKE,
-                             bytes=1 << 40, stream=None),
+                             vocab=10, width=64, dtype=0, ignore_index=-100, reduction=2, keep=0, loss=_FAKE, saved=_FAKE,
+                             workspace=_FAKE, bytes=1 << 40, stream=None),
         "loss_backward": dict(hidden=_FAKE, hidden_stride=64, weight=_FAKE, weight_stride=64, rows=3, vocab=10, width=64, dtype=0,
-                              reduction=2, saved=_FAKE, grad_loss=_FAKE, grad_hidden=_FAKE, grad_weight=_FAKE, workspace=_FAKE,
+                              reduction=2, keep=0, saved=_FAKE, grad_loss=_FAKE, grad_hidden=_FAKE, grad_weight=_FAKE, workspace=_FAKE,
                               bytes=1 << 40, stream=None),
     }[name]
     assert set(overrides) <= set(defaults)
@@ -208,8 +218,14 @@ def test_workspaces_are_of_the_shape_alone():
     assert lib.attnres_hip_layer_norm_workspace_elems(0, 64) == 0
     assert lib.attnres_hip_layer_norm_workspace_elems(4, 8193) == -1
     assert lib.attnres_hip_embedding_workspace_bytes(2, 3, 0, 64) == -1
-    assert lib.attnres_hip_loss_workspace_bytes(3, 10, 64, 9, 0) == -1
-    assert lib.attnres_hip_loss_saved_bytes(-1) == -1
+    assert lib.attnres_hip_loss_workspace_bytes(3, 10, 64, 9, 0, 0) == -1
+    assert lib.attnres_hip_loss_saved_bytes(-1, 10, 64, 0, 0) == -1
     # the probabilities of a large vocabulary are formed in pieces: the backward of 16384 tokens and
     # 131072 words needs far less than the 4 GiB of BF16 probabilities
-    assert lib.attnres_hip_loss_workspace_bytes(16384, 131072, 2048, 0, 1) < 1 << 30
+    for keep in (0, 1):
+        assert lib.attnres_hip_loss_workspace_bytes(16384, 131072, 2048, 0, keep, 1) < 1 << 30
+    # kept exponentials: 2 bytes each and 1 / 32 of that, up to 8 GiB
+    assert lib.attnres_hip_loss_saved_bytes(16384, 131072, 2048, 0, 0) == 256 + 20 * 16384
+    assert 1 << 32 < lib.attnres_hip_loss_saved_bytes(16384, 131072, 2048, 0, 1) < 1.04 * 2**32
+    assert 1 << 33 < lib.attnres_hip_loss_saved_bytes(32768, 131072, 2048, 0, 1) < 1.04 * 2**33
+    assert lib.attnres_hip_loss_saved_bytes(32769, 131072, 2048, 0, 1) == 256 + 20 * 32769
