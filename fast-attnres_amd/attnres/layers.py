@@ -302,11 +302,14 @@ def linear_cross_entropy(hidden: Tensor, weight: Tensor, targets: Tensor, *, ign
 def _loss_saved_bytes(rows: int, vocab: int, width: int, dtype: torch.dtype, keep: bool) -> int:
     """attnres_hip_loss_saved_bytes, for sizes that may be symbols."""
     size = 256 + 20 * rows
-    if not keep or rows <= (64 if dtype == torch.float32 or width % 32 else 32):
+    if not keep or rows == 0:
         return size
-    rows, vocab = (-(-n // _LOSS_TILE) * _LOSS_TILE for n in (rows, vocab))
-    powers = (2 if dtype == torch.bfloat16 else 4) * rows * vocab
-    return size if powers > _MAX_KEPT else -(-size // 256) * 256 + 8 * (vocab // 128) * rows + powers
+    if rows <= (64 if dtype == torch.float32 or width % 32 else 32):
+        sums, powers = 0, 4 * (16 if rows <= 16 else 32 if rows <= 32 else 64) * (-(-vocab // 128) * 128)
+    else:
+        rows, vocab = (-(-n // _LOSS_TILE) * _LOSS_TILE for n in (rows, vocab))
+        sums, powers = 8 * (vocab // 128) * rows, (2 if dtype == torch.bfloat16 else 4) * rows * vocab
+    return size if powers > _MAX_KEPT else -(-size // 256) * 256 + sums + powers
 
 
 @torch.library.custom_op("attnres_hip::linear_cross_entropy", mutates_args=(), device_types="cuda", tags=_OP_TAGS)

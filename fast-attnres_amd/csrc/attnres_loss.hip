@@ -924,6 +924,8 @@ struct FewArgs {
   Saved saved;
   f32x2* sums;          // [workgroups][kFewRows]
   float* target_logit;  // [kFewRows]
+  float* logits;        // [16 TILES][logits_ld], or nullptr: not kept
+  int64_t logits_ld;
 };
 
 template <class X, int TILES>  // of 16 rows
@@ -951,7 +953,9 @@ __global__ void __launch_bounds__(kFewBlock) attnres_loss_few_kernel(FewArgs<X> 
   const X* h[TILES];
 #pragma unroll
   for (int t = 0; t < TILES; ++t) h[t] = g.hidden + min(t * 16 + entry, g.rows - 1) * g.hidden_stride;
-  if (wave == 0) {
+  if (g.targets == nullptr) {
+    if (wave == 0) target[lane] = -1;
+  } else if (wave == 0) {
     const int row = min(lane, g.rows - 1);
     const int64_t t = g.target_bytes == 8 ? static_cast<const int64_t*>(g.targets)[row] : static_cast<const int32_t*>(g.targets)[row];
     const bool counts = lane < g.rows && t != g.ignore_index;
@@ -1000,6 +1004,12 @@ __global__ void __launch_bounds__(kFewBlock) attnres_loss_few_kernel(FewArgs<X> 
     }
     if (part != 0) continue;
     const int row = t * 16 + entry;
+    if (g.logits != nullptr) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        *reinterpret_cast<f32x4*>(g.logits + row * g.logits_ld + v0 + i * 16 + 4 * group) = acc[i][t];
+      }
+    }
     const int64_t from_v0 = target[row] - v0;  // -1 is before every word
     float top = -__builtin_inff(), sum = 0.0f;
     bool counts[2][4];
@@ -1032,6 +1042,204 @@ __global__ void __launch_bounds__(kFewBlock) attnres_loss_few_kernel(FewArgs<X> 
 #pragma unroll
     for (int k = 1; k < kFewWords / 32; ++k) sum = join(sum, meet[k][threadIdx.x]);
     g.sums[static_cast<int64_t>(blockIdx.x) * kFewRows + threadIdx.x] = sum;
+  }
+}
+
+// The backward of few rows reads W and writes dW once.  A workgroup takes 256 columns, 64 to a wavefront, and every
+// parts'th block of 32 words: it forms the block's P (FP32, from the kept logits) in LDS, adds P W to its sums of dH and
+// writes P^T H.  FP32 matrix instructions for all types: P is not rounded, and with so few rows they have the time.
+// Column n of an instruction stands for columns 4 n .. 4 n + 3 of four of them, so a lane loads and stores 4 columns
+// together.  The parts' sums of dH are added up in order after.  With the sums, 16 rows: 32768 x 1024 BF16 (134 MB of W and dW)
+// 46 us, FP32 60; more workgroups (768 to 2048) change that by less than their partial sums cost.
+constexpr int kBackWords = 32;
+constexpr int kBackColumns = 256;
+constexpr int kBackSteps = kBackWords / 4;
+constexpr int kBackStride = kBackWords + 4;  // of P's rows in LDS: 16 rows by 4 words meet 64 banks
+constexpr int kBackGroups = 512;             // workgroups
+
+template <class X>
+struct Quad {  // four columns as they lie
+  uint32_t w[sizeof(X)];
+  __device__ __forceinline__ void load(const X* row, int c, int width) {
+    if (c + 4 <= width) {
+      __builtin_memcpy(w, row + c, sizeof(w));
+    } else {
+      X x[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] = c + e < width ? row[c + e] : from_f32<X>(0.0f);
+      __builtin_memcpy(w, x, sizeof(w));
+    }
+  }
+  __device__ __forceinline__ float at(int e) const {
+    if constexpr (std::is_same_v<X, float>) {
+      return __uint_as_float(w[e]);
+    } else {
+      return to_f32(X{static_cast<uint16_t>(w[e / 2] >> (16 * (e % 2)))});
+    }
+  }
+};
+
+template <class X>
+struct FewBackArgs {
+  const X* hidden;
+  const X* weight;
+  int64_t hidden_stride, weight_stride, vocab;
+  int width, rows;
+  Saved saved;
+  const float* logits;
+  int64_t logits_ld;
+  const float* grad_loss;
+  int reduction;
+  X* grad_weight;  // or nullptr
+  float* partial;  // [parts][16 TILES][ld], or nullptr: dH is not wanted
+  int64_t ld;
+  int parts;
+};
+
+template <class X, int TILES>
+__global__ void __launch_bounds__(kBlock) attnres_loss_few_backward_kernel(FewBackArgs<X> g) {
+  constexpr int kRows = TILES * 16;
+  struct Row {
+    float c, factor, by;
+    int target;  // -2: ignored, or no row at all
+  };
+  __shared__ Row info[kRows];
+  __shared__ float lds[2][kRows][kBackStride];
+  const int lane = threadIdx.x % 64, group = lane / 16, entry = lane % 16;
+  const int column = static_cast<int>(blockIdx.y) * kBackColumns + wave_index() * 64 + entry * 4;
+  if (threadIdx.x < kRows) {
+    const int row = threadIdx.x;
+    Row r{0.0f, 0.0f, 0.0f, -2};
+    const int at = row < g.rows ? g.saved.packed[row] : -1;
+    if (at >= 0) {
+      r.by = g.reduction == ATTNRES_REDUCE_NONE ? g.grad_loss[row] : g.grad_loss[0];
+      if (g.reduction == ATTNRES_REDUCE_MEAN) r.by /= static_cast<float>(g.saved.header->count);
+      r.c = g.saved.stats[at].x;
+      r.factor = g.saved.stats[at].y * r.by;
+      r.target = g.saved.target[at];
+    }
+    info[row] = r;
+  }
+  __syncthreads();
+  // H: row 4 k + group; what an ignored row holds is not looked at
+  float h[kRows / 4][4];
+#pragma unroll
+  for (int k = 0; k < kRows / 4; ++k) {
+    const int row = k * 4 + group;
+    Quad<X> x;
+    x.load(g.hidden + min(row, g.rows - 1) * g.hidden_stride, column, g.width);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) h[k][e] = info[row].target == -2 ? 0.0f : x.at(e);
+  }
+  const int64_t blocks = (g.vocab + kBackWords - 1) / kBackWords;
+  Quad<X> next_w[kBackSteps];
+  float next_logit[TILES * 2];
+  const auto fetch = [&](int64_t block) {
+    const int64_t v0 = block * kBackWords;
+#pragma unroll
+    for (int s = 0; s < kBackSteps; ++s) {
+      next_w[s].load(g.weight + min(v0 + s * 4 + group, g.vocab - 1) * g.weight_stride, column, g.width);
+    }
+#pragma unroll
+    for (int i = 0; i < TILES * 2; ++i) {
+      next_logit[i] = g.logits[(threadIdx.x / kBackWords + i * 8) * g.logits_ld + v0 + threadIdx.x % kBackWords];
+    }
+  };
+  f32x4 dh[TILES][4] = {};
+  fetch(blockIdx.x);
+  int buffer = 0;
+  for (int64_t block = blockIdx.x; block < blocks; block += g.parts, buffer ^= 1) {
+    const int64_t v0 = block * kBackWords;
+#pragma unroll
+    for (int i = 0; i < TILES * 2; ++i) {
+      const int row = threadIdx.x / kBackWords + i * 8, word = threadIdx.x % kBackWords;
+      const Row r = info[row];
+      float x = power(over_ln2(next_logit[i]) - r.c) * r.factor;
+      if (r.target == v0 + word) x -= r.by;
+      lds[buffer][row][word] = r.target == -2 || v0 + word >= g.vocab ? 0.0f : x;
+    }
+    Quad<X> w[kBackSteps];
+#pragma unroll
+    for (int s = 0; s < kBackSteps; ++s) w[s] = next_w[s];
+    if (block + g.parts < blocks) fetch(block + g.parts);
+    __syncthreads();
+    if (g.partial != nullptr) {
+#pragma unroll
+      for (int s = 0; s < kBackSteps; ++s) {
+#pragma unroll
+        for (int t = 0; t < TILES; ++t) {
+          const float a = lds[buffer][t * 16 + entry][s * 4 + group];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) dh[t][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(a, w[s].at(e), dh[t][e], 0, 0, 0);
+        }
+      }
+    }
+    if (g.grad_weight != nullptr) {
+#pragma unroll
+      for (int m = 0; m < kBackWords / 16; ++m) {
+        f32x4 dw[4] = {};
+#pragma unroll
+        for (int k = 0; k < kRows / 4; ++k) {
+          const float a = lds[buffer][k * 4 + group][m * 16 + entry];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) dw[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(a, h[k][e], dw[e], 0, 0, 0);
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int64_t v = v0 + m * 16 + group * 4 + r;
+          if (v >= g.vocab) continue;
+          X x[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[e] = from_f32<X>(dw[e][r]);
+          X* to = g.grad_weight + v * g.width + column;
+          if (column + 4 <= g.width) {
+            __builtin_memcpy(to, x, sizeof(x));
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              if (column + e < g.width) to[e] = x[e];
+            }
+          }
+        }
+      }
+    }
+  }
+  if (g.partial == nullptr) return;
+#pragma unroll
+  for (int t = 0; t < TILES; ++t) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      if (column >= g.ld) continue;
+      float* to = g.partial + (static_cast<int64_t>(blockIdx.x) * kRows + t * 16 + group * 4 + r) * g.ld + column;
+      *reinterpret_cast<f32x4*>(to) = f32x4{dh[t][0][r], dh[t][1][r], dh[t][2][r], dh[t][3][r]};
+    }
+  }
+}
+
+// dH from the parts' sums: a row and 64 columns per workgroup, 16 groups that add up every 16th part each.
+constexpr int kFewJoinColumns = 64, kFewJoinGroups = kBlock / (kFewJoinColumns / 4);
+
+template <class X>
+__global__ void __launch_bounds__(kBlock) attnres_loss_few_join_kernel(const float* __restrict__ partial, int parts, int padded, int64_t ld,
+                                                                       const int32_t* packed, int width, X* __restrict__ out) {
+  __shared__ f32x4 sums[kFewJoinGroups][kFewJoinColumns / 4];
+  const int group = threadIdx.x / (kFewJoinColumns / 4), member = threadIdx.x % (kFewJoinColumns / 4);
+  const int64_t row = blockIdx.y;
+  const int column = static_cast<int>(blockIdx.x) * kFewJoinColumns + member * 4;
+  const int64_t from = min(static_cast<int64_t>(column), ld - 4);
+  f32x4 sum = {};
+#pragma unroll 8
+  for (int k = group; k < parts; k += kFewJoinGroups) {
+    sum += *reinterpret_cast<const f32x4*>(partial + (static_cast<int64_t>(k) * padded + row) * ld + from);
+  }
+  sums[group][member] = sum;
+  __syncthreads();
+  if (group != 0) return;
+  for (int k = 1; k < kFewJoinGroups; ++k) sum += sums[k][member];
+  const bool counts = packed[row] >= 0;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    if (column + e < width) out[row * width + column + e] = from_f32<X>(counts ? sum[e] : 0.0f);
   }
 }
 
@@ -1258,16 +1466,18 @@ int choose_splits(int64_t tiles, int64_t depth, int segments, bool direct) {
   return best;
 }
 
-// Rows that the forward of few rows takes.  Forward, us, its way -> by tiles, 16 / 32 / 64 rows: BF16, 32768 x 1024
+// Rows that go the way of few rows.  Forward, us, its way -> by tiles, 16 / 32 / 64 rows: BF16, 32768 x 1024
 // 20.8 / 26.4 / 34.6 -> 37, 131072 x 2048 126 / 157 / 212 -> 156; where W has to be packed for the tiles, FP16, 50021 x 1000
-// 31 / 38 / 50 -> 71, FP32, 32768 x 1024 34 / 48 / 80 -> 166.
+// 31 / 38 / 50 -> 71, FP32, 32768 x 1024 34 / 48 / 80 -> 166.  Backward: BF16, 32768 x 1024 46 / 63 / - -> 74, 131072 x 2048
+// 308 / 413 / - -> 338; FP16, 50021 x 1000 93 / - / 205 -> 154; FP32, 32768 x 1024 60 / 71 / 121 -> 216.
 int64_t few_rows(bool pack_weight) { return pack_weight ? kFewRows : kFewRows / 2; }
 
 struct LossPlan {
   bool split, pack_weight, few, keep;
   int64_t rows_pad, width_pad, vocab_pad, piece;
   int64_t hidden[2], weight[2], sums, target_logit, losses;  // offsets
-  int64_t row_scale, alpha, p[2], dh, dw;
+  int64_t row_scale, alpha, p[2], dh, dw, logits, logits_ld;
+  int few_tiles, parts;
   int splits_h, splits_w;
   int64_t bytes;
   int64_t saved_sums, saved_powers, saved_bytes;
@@ -1287,25 +1497,35 @@ LossPlan loss_plan(int64_t rows, int64_t vocab, int64_t width, int dtype, bool k
     at += round_up(bytes, 256);
     return from;
   };
-  p.few = rows <= few_rows(p.pack_weight);
-  const int64_t powers = (dtype == ATTNRES_BF16 ? 2 : 4) * p.rows_pad * p.vocab_pad;
-  p.keep = keep && !p.few && powers <= kKeepBytes;
+  p.few = rows > 0 && rows <= few_rows(p.pack_weight);
+  p.few_tiles = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
+  p.logits_ld = round_up(vocab, kFewWords);
+  const int64_t logits = 4 * 16 * p.few_tiles * p.logits_ld;
+  const int64_t powers = p.few ? logits : (dtype == ATTNRES_BF16 ? 2 : 4) * p.rows_pad * p.vocab_pad;
+  p.keep = keep && rows > 0 && powers <= kKeepBytes;
   p.saved_bytes = kHeaderBytes + 20 * rows;
   if (p.keep) {
     p.saved_sums = round_up(p.saved_bytes, 256);
-    p.saved_powers = p.saved_sums + 8 * (p.vocab_pad / 128) * p.rows_pad;
+    p.saved_powers = p.saved_sums + (p.few ? 0 : 8 * (p.vocab_pad / 128) * p.rows_pad);
     p.saved_bytes = p.saved_powers + powers;
   }
-  const bool few = !backward && p.few;
-  if (!few) {
+  const bool scores = !backward || (p.few && !p.keep);  // the forward's kernels run
+  if (!p.few) {
     for (int k = 0; k < parts; ++k) p.hidden[k] = take(2 * p.rows_pad * p.width_pad);
     for (int k = 0; p.pack_weight && k < parts; ++k) p.weight[k] = take(2 * vocab * p.width_pad);
   }
-  if (!backward) {
-    if (few) p.sums = take(8 * ((vocab + kFewWords - 1) / kFewWords) * kFewRows);
+  if (scores) {
+    if (p.few) p.sums = take(8 * (p.logits_ld / kFewWords) * kFewRows);
     else if (!p.keep) p.sums = take(8 * (p.vocab_pad / 128) * p.rows_pad);
     p.target_logit = take(4 * p.rows_pad);
+  }
+  if (!backward) {
     p.losses = take(4 * rows);
+  } else if (p.few) {
+    if (!p.keep) p.logits = take(logits);
+    const int64_t slabs = (width + kBackColumns - 1) / kBackColumns;
+    p.parts = static_cast<int>(std::min<int64_t>((vocab + kBackWords - 1) / kBackWords, std::max<int64_t>(kBackGroups / slabs, 1)));
+    p.dh = take(4 * p.parts * 16 * p.few_tiles * p.width_pad);
   } else {
     p.row_scale = take(4 * p.rows_pad);
     p.alpha = take(16);
@@ -1357,7 +1577,7 @@ void prepare_operands(const Call& c, bool find_scales, Operand* h, Operand* w) {
   Header* header = c.saved.header;
   if constexpr (kSplit) {
     if (find_scales) {
-      const unsigned grid_h = static_cast<unsigned>(std::clamp<int64_t>(c.rows, 1, 1024));
+      const unsigned grid_h = static_cast<unsigned>(std::min<int64_t>(c.rows, 1024));
       hipLaunchKernelGGL(attnres_loss_amax_kernel, dim3(grid_h), dim3(kBlock), 0, c.stream, hidden, c.hidden_stride, c.rows,
                          static_cast<int>(c.width), c.saved.index, &header->count, &header->amax[0]);
       const unsigned grid_w = static_cast<unsigned>(std::min<int64_t>(c.vocab, 2048));
@@ -1382,29 +1602,61 @@ void prepare_operands(const Call& c, bool find_scales, Operand* h, Operand* w) {
   }
 }
 
+// The logits of few rows; logits: where they are kept, or nullptr.  targets: nullptr in the backward, where
+// saved and ignored rows are known.
+template <class X>
+void launch_few(const Call& c, const void* targets, int target_bytes, int64_t ignore_index, float* logits) {
+  const LossPlan& p = c.plan;
+  const FewArgs<X> g{static_cast<const X*>(c.hidden), static_cast<const X*>(c.weight), c.hidden_stride, c.weight_stride, c.vocab,
+                     static_cast<int>(c.width), static_cast<int>(c.rows), targets, target_bytes, ignore_index, c.saved,
+                     c.at<f32x2>(p.sums), c.at<float>(p.target_logit), logits, p.logits_ld};
+  const auto kernel = p.few_tiles == 1   ? attnres_loss_few_kernel<X, 1>
+                      : p.few_tiles == 2 ? attnres_loss_few_kernel<X, 2>
+                                         : attnres_loss_few_kernel<X, 4>;
+  hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(p.logits_ld / kFewWords)), dim3(kFewBlock), 0, c.stream, g);
+}
+
+template <class X>
+void few_backward(const Call& c, int reduction, const float* grad_loss, void* grad_hidden, void* grad_weight) {
+  const LossPlan& p = c.plan;
+  const float* logits = static_cast<const float*>(c.saved.powers);
+  if (!p.keep) {
+    float* again = c.at<float>(p.logits);
+    launch_few<X>(c, nullptr, 8, 0, again);
+    logits = again;
+  }
+  const FewBackArgs<X> g{static_cast<const X*>(c.hidden), static_cast<const X*>(c.weight), c.hidden_stride, c.weight_stride, c.vocab,
+                         static_cast<int>(c.width), static_cast<int>(c.rows), c.saved, logits, p.logits_ld, grad_loss, reduction,
+                         static_cast<X*>(grad_weight), grad_hidden != nullptr ? c.at<float>(p.dh) : nullptr, p.width_pad, p.parts};
+  const auto kernel = p.few_tiles == 1   ? attnres_loss_few_backward_kernel<X, 1>
+                      : p.few_tiles == 2 ? attnres_loss_few_backward_kernel<X, 2>
+                                         : attnres_loss_few_backward_kernel<X, 4>;
+  const unsigned slabs = static_cast<unsigned>((c.width + kBackColumns - 1) / kBackColumns);
+  hipLaunchKernelGGL(kernel, dim3(p.parts, slabs), dim3(kBlock), 0, c.stream, g);
+  if (grad_hidden != nullptr) {
+    const dim3 grid(static_cast<unsigned>((c.width + kFewJoinColumns - 1) / kFewJoinColumns), static_cast<unsigned>(c.rows));
+    hipLaunchKernelGGL((attnres_loss_few_join_kernel<X>), grid, dim3(kBlock), 0, c.stream, c.at<const float>(p.dh), p.parts,
+                       16 * p.few_tiles, p.width_pad, c.saved.packed, static_cast<int>(c.width), static_cast<X*>(grad_hidden));
+  }
+}
+
 // X: the inputs' type; T: the operands'.
 template <class X, class T, int SEGMENTS>
 void loss_forward(const Call& c, const void* targets, int target_bytes, int64_t ignore_index, int reduction, float* loss) {
   const LossPlan& p = c.plan;
-  if (c.rows == 0 || !p.few) {
+  if (!p.few) {
     hipLaunchKernelGGL(attnres_loss_rows_kernel, dim3(1), dim3(kScanThreads), 0, c.stream, targets, target_bytes, c.rows, c.vocab,
                        ignore_index, c.saved);
   }
   if (c.rows > 0) {
-    f32x2* sums = p.keep ? c.saved.sums : c.at<f32x2>(p.sums);
+    f32x2* sums = p.keep && !p.few ? c.saved.sums : c.at<f32x2>(p.sums);
     float* target_logit = c.at<float>(p.target_logit);
     int tiles;
     int64_t row_tiles;
     if (p.few) {
-      tiles = static_cast<int>((c.vocab + kFewWords - 1) / kFewWords);
+      tiles = static_cast<int>(p.logits_ld / kFewWords);
       row_tiles = kFewRows;
-      const FewArgs<X> g{static_cast<const X*>(c.hidden), static_cast<const X*>(c.weight), c.hidden_stride, c.weight_stride, c.vocab,
-                         static_cast<int>(c.width), static_cast<int>(c.rows), targets, target_bytes, ignore_index, c.saved, sums,
-                         target_logit};
-      const auto kernel = c.rows <= 16   ? attnres_loss_few_kernel<X, 1>
-                          : c.rows <= 32 ? attnres_loss_few_kernel<X, 2>
-                                         : attnres_loss_few_kernel<X, 4>;
-      hipLaunchKernelGGL(kernel, dim3(tiles), dim3(kFewBlock), 0, c.stream, g);
+      launch_few<X>(c, targets, target_bytes, ignore_index, static_cast<float*>(c.saved.powers));
     } else {
       LogitArgs g{};
       prepare_operands<X>(c, true, &g.product.b, &g.product.a);
@@ -1440,8 +1692,9 @@ template <class X, class T, int SEGMENTS>
 void loss_backward(const Call& c, int reduction, const float* grad_loss, void* grad_hidden, void* grad_weight) {
   const LossPlan& p = c.plan;
   constexpr int kParts = SEGMENTS == 3 ? 2 : 1;
+  if (p.few) return few_backward<X>(c, reduction, grad_loss, grad_hidden, grad_weight);
   Operand h{}, w{};
-  prepare_operands<X>(c, p.few, &h, &w);  // whose forward needed no scales
+  prepare_operands<X>(c, false, &h, &w);
   const float p_scale = std::is_same_v<T, Bf16> ? 1.0f : kProbabilityScale;
   float* alpha = c.at<float>(p.alpha);
   float* row_scale = c.at<float>(p.row_scale);
@@ -1613,13 +1866,14 @@ int attnres_hip_loss_forward(const void* hidden, int64_t hidden_stride, const vo
 }
 
 int attnres_hip_loss_backward(const void* hidden, int64_t hidden_stride, const void* weight, int64_t weight_stride, int64_t rows,
-                              int64_t vocab, int64_t width, int dtype, int reduction, int keep, void* saved,
+                              int64_t vocab, int64_t width, int dtype, int reduction, int keep, const void* saved,
                               const float* grad_loss, void* grad_hidden, void* grad_weight, void* workspace,
                               int64_t workspace_bytes, void* stream) {
   if (const int status = check_loss(hidden, hidden_stride, weight, weight_stride, rows, vocab, width, dtype, reduction)) return status;
   if (saved == nullptr || grad_loss == nullptr) return layer_error(ATTNRES_ERR_NULL_POINTER, "saved or grad_loss is NULL");
   const LossPlan plan = loss_plan(rows, vocab, width, dtype, keep != 0, true);
-  const Call c{hidden, hidden_stride, weight, weight_stride, rows, vocab, width, plan, saved_views(saved, rows, plan),
+  const Call c{hidden, hidden_stride, weight, weight_stride, rows, vocab, width, plan,
+               saved_views(const_cast<void*>(saved), rows, plan),  // read only
                static_cast<char*>(workspace), static_cast<hipStream_t>(stream)};
   if (const int status = check_places(saved, workspace, workspace_bytes, c.plan.bytes)) return status;
   if (grad_hidden == nullptr && grad_weight == nullptr) return ATTNRES_OK;

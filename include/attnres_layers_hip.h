@@ -84,10 +84,9 @@ int attnres_hip_embedding_backward(const void* grad_out, int out_dtype, const vo
  * is ignore_index), else one value; the mean is over the targets that count (NaN
  * when none does).  A target that is neither ignore_index nor in 0..vocab-1 makes
  * the loss and the gradients NaN.
- * saved: what the backward reads (and completes, with the same values every time, where a forward of
- * few FP32 rows needed less).  keep, the same in all calls: nonzero lets the forward keep the exponentials of the
+ * saved: what the backward reads.  keep, the same in all calls: nonzero lets the forward keep the exponentials of the
  * logits there for the backward, 2 bytes each for BF16, else 4, rows and vocab padded
- * to 256, where that takes at most 8 GiB; otherwise, and with 0, saved is 256 + 20 * rows bytes and the backward
+ * to 256, where that takes at most 8 GiB (of few rows, up to 64, the FP32 logits); otherwise, and with 0, saved is 256 + 20 * rows bytes and the backward
  * forms them again, for one piece of the vocabulary at a time.  saved and
  * workspace start at multiples of 16 bytes (else ATTNRES_ERR_WORKSPACE). */
 int64_t attnres_hip_loss_saved_bytes(int64_t rows, int64_t vocab, int64_t width, int dtype, int keep);
@@ -101,7 +100,7 @@ int attnres_hip_loss_forward(const void* hidden, int64_t hidden_stride, const vo
 /* grad_loss (FP32): one value, or [rows] for ATTNRES_REDUCE_NONE.  grad_hidden
  * [rows, width] and grad_weight [vocab, width] contiguous, of dtype; either may be NULL. */
 int attnres_hip_loss_backward(const void* hidden, int64_t hidden_stride, const void* weight, int64_t weight_stride,
-                              int64_t rows, int64_t vocab, int64_t width, int dtype, int reduction, int keep, void* saved,
+                              int64_t rows, int64_t vocab, int64_t width, int dtype, int reduction, int keep, const void* saved,
                               const float* grad_loss, void* grad_hidden, void* grad_weight, void* workspace,
                               int64_t workspace_bytes, void* stream);
 
