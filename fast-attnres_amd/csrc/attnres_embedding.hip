@@ -3,8 +3,9 @@
 //   out[b, t] = scale W[tok[b, t]] + pos[t]
 //   dW[v] = scale sum_{i: tok_i = v} dO_i,   dpos[t] = sum_b dO[b, t]
 //
-// Memory bound: the lookup reads one table row and writes one output row per token; the
-// gradient reads dO once and writes the whole table.  The tokens are sorted (stable, least
+// Memory bound: the lookup reads one table row and writes one output row per token (32768 x 2048 BF16 of 131072 rows: 51
+// us); the gradient reads dO once and writes the whole table (there 537 MB: 210 us, half of it the sort's four launches,
+// which clear the table meanwhile at 5.1 TB/s).  The tokens are sorted (stable, least
 // significant digit first), so every table row's sum is a run of the sorted list, added up in
 // FP32 in the order of the tokens: no atomics on values, the same bits every time.
 
@@ -357,7 +358,8 @@ __global__ void __launch_bounds__(kSmallBlock) attnres_sort_small_kernel(SortPas
 // --------------------------------------------------------------------- sums
 // The sorted list in pieces: a run of one token inside a piece is its table row's
 // gradient; what crosses a piece's border goes to the piece's partial rows
-// (0: began before the piece, 1: began in it and goes on) and is joined after.
+// (0: began before the piece, 1: began in it and goes on) and is joined after.  About a thousand pieces: with twice as
+// many the partial rows cost more than the shorter walks gain.  32768 x 2048 BF16 65 us, joined in 16.
 
 struct Runs {
   const uint32_t* keys;

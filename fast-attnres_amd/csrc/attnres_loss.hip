@@ -3,21 +3,23 @@
 //   l[n, v] = <H_n, W_v>,  lse_n = log sum_v exp(l[n, v]),  loss_n = lse_n - l[n, t_n]
 //   P[n, v] = g_n (exp(l[n, v] - lse_n) - [v = t_n]),  dH = P W,  dW = P^T H
 //
-// Bound by the matrix cores: four products of 2 N V D operations (the logits in
-// the forward, again in the backward, and two gradient products), 8 N V D in all, against
-// O(V D + N D) bytes.  The logits are never stored: the forward keeps a running (maximum, sum of
-// exponentials) per row and tile of 256 columns, the backward forms P for one piece of the
-// vocabulary at a time.
+// Bound by the matrix cores: three products of 2 N V D operations (the logits and two gradient products) against
+// O(V D + N D) bytes.  The logits are never stored as they are.  The forward reduces them, per row and 128 columns, to a
+// reference and a sum of powers above it, and keeps the powers for the backward (2 or 4 bytes each, up to
+// kKeepBytes), which makes P of them in one pass, for one piece of the vocabulary at a time.  Without kept
+// powers the backward multiplies again, four products in all.  Forward and backward, kept / again: 16384 x 131072 x 2048 BF16
+// 22.5 / 27.9 ms, 2048 x 32768 x 1024 BF16 0.45 / 0.54, 4096 x 32768 x 1024 FP32 2.45 / 3.04.
 //
 // Rows whose target is ignored are left out before anything is multiplied: the rows that count are
-// packed together (in order, the row length padded with zeros to whole tiles), so ignored
+// packed together (in order, the row length padded with zeros to whole stages), so ignored
 // rows cost nothing and what they hold (NaN, infinities) reaches nothing.
 //
 // Operands are 16 bits wide.  BF16 and FP16 inputs are multiplied as they are.  FP32
 // inputs are scaled by a power of two to just under 2^15 and written as the sum of two FP16 numbers, hi +
 // lo (24 bits together for all within 2^-14 of the largest), and a product is
 // hi hi + hi lo + lo hi: what is left out, lo lo, is below 2^-24 of the product, like FP32's own
-// rounding.  Three FP16 products run at 16 / 3 times the rate of FP32 matrix instructions.
+// rounding.  Three FP16 products take 0.78 ms (16384 x 8192 x 1024, logits) where FP32 matrix instructions, at a
+// sixteenth of the FP16 rate, take 1.8 at the rate of a large library product.
 // P is rounded to the operands' type (BF16), or, for FP16 and FP32 inputs, scaled by
 // 2^14 and written as one or two FP16 numbers, so that probabilities down to 2^-28 are normal numbers.
 
@@ -81,7 +83,9 @@ constexpr int64_t kHeaderBytes = 256;
 // LDS serves together meet every bank once: slot = chunk ^ (-(row / 4) % 4) for rows of k (64 bytes; lanes 0-3,
 // 12-15, 20-23 and 24-27 go together), chunk ^ (4 (k % 4) + 2 (k / 8 % 2)) for columns (512 bytes).
 // 16 x 16 x 32 matrix instructions: the chip is limited by power here (1.7 of 2.4 GHz), and on registers alone
-// these reach 2.2 PFLOP/s, 32 x 32 x 16 ones 2.0.
+// these reach 2.2 PFLOP/s, 32 x 32 x 16 ones 2.0.  Measured, 16384 x 16384 x 2048: dH 785-836 us (1.36 PFLOP/s), dW 852-907 (both
+// operands transposed; 1.25), logits 1.13-1.25 with their reduction.  Five LDS stages, other depths and orders of loads, and
+// wave priorities were no faster.
 
 struct Operand {
   const uint16_t* part[2];  // hi, lo
@@ -93,7 +97,7 @@ struct Operand {
 struct Product {
   Operand a, b;
   const int32_t* count;  // live packed rows
-  int64_t depth;         // k of the whole product (a multiple of 64), of all splits
+  int64_t depth;         // k of the whole product, of all splits; operands hold zeros up to a whole stage
   int depth_is_count;    // depth: the packed rows
   int tiles_a, tiles_b, splits;
 };
@@ -459,7 +463,9 @@ struct LogitArgs {
 // writing one chunk of 32 rows meet 32 different slots.
 __device__ __forceinline__ int staged(int row, int chunk) { return row * 32 + (chunk ^ (row & 31)); }
 
-// Forward: (reference, sum) of a tile's two times 128 logits per row, and the target's logit.  KEEP: the powers too.
+// Forward: (reference, sum) of a tile's two times 128 logits per row, and the target's logit.  KEEP: the powers too, staged
+// in LDS and stored 512 bytes of a row at a time (256 where they are FP32, in two rounds).  The reduction is vector
+// work that the next tile's products do not cover: 16384 x 131072 x 2048 BF16 6.9 ms, with kept powers 7.8.
 template <class T, int SEGMENTS, bool KEEP>
 __global__ void __launch_bounds__(kThreads) attnres_loss_logits_kernel(LogitArgs g) {
   __shared__ __align__(16) uint16_t lds[kStages * 2 * kOperand];
@@ -570,8 +576,9 @@ __global__ void __launch_bounds__(kThreads) attnres_loss_logits_kernel(LogitArgs
   }
 }
 
-// Backward of kept powers: P of a piece's columns, read from the powers and written as operands.  16 rows of 512
-// columns per workgroup, 8 columns per thread and row.
+// Backward of kept powers: P of a piece's columns, read from the powers and written as operands, both past the caches.
+// 16 rows of 512 columns per workgroup, 8 columns per thread and row.  Memory bound: 16384 x 16384 of FP16 to BF16 (1.07
+// GB) 156 us, 6.9 TB/s.
 constexpr int kScaleRows = 16, kScaleColumns = 64 * kVec;
 
 template <class E, class T, int PARTS>
@@ -621,7 +628,7 @@ __global__ void __launch_bounds__(kBlock) attnres_loss_rescale_kernel(LogitArgs 
   }
 }
 
-// Backward: P of a tile, rounded to the operands' type.
+// Backward without kept powers: P of a tile, rounded to the operands' type; 893 us for 16384 x 16384 x 2048 BF16.
 template <class T, int SEGMENTS>
 __global__ void __launch_bounds__(kThreads) attnres_loss_probability_kernel(LogitArgs g) {
   __shared__ __align__(16) uint16_t lds[kStages * 2 * kOperand];
@@ -727,7 +734,7 @@ __device__ __forceinline__ void zero_tile(const GradientArgs& g, const TileAt& t
 }
 
 // dH (A: W by columns, B: P by rows) and dW (A: H by columns, B: P by columns).  OUT float:
-// FP32 partial sums or an FP32 gradient; else the 16-bit gradient itself.
+// FP32 partial sums or an FP32 gradient; else the 16-bit gradient itself.  dH is summed over the pieces in FP32, in order.
 template <class T, class OUT, int SEGMENTS, bool B_ROWS>
 __global__ void __launch_bounds__(kThreads) attnres_loss_gradient_kernel(GradientArgs g) {
   __shared__ __align__(16) uint16_t lds[kStages * 2 * kOperand];
@@ -1321,28 +1328,28 @@ __global__ void __launch_bounds__(kBlock) attnres_loss_pack_kernel(const X* __re
   }
 }
 
-// Per row of the input: its log-sum from the tiles' sums (by packed row, or by row), and its loss.  4 rows by 64 parts
-// of the tiles per workgroup: with few rows the tiles' sums are long chains, and their latency is all there is.
-constexpr int kReduceRows = 4, kReduceParts = kBlock / kReduceRows;
-
+// Per row of the input: its log-sum from the tiles' sums (by packed row, or by row), and its loss.  ROWS rows
+// by kBlock / ROWS parts of the tiles per workgroup: 16, which read whole lines, or 4 where that would leave units without work:
+// with few rows the tiles' sums are long chains, and their latency is all there is.
+template <int ROWS>
 __global__ void __launch_bounds__(kBlock) attnres_loss_reduce_kernel(const f32x2* __restrict__ sums, int tiles, int64_t row_tiles,
                                                                      const float* __restrict__ target_logit, int64_t rows, bool packed,
                                                                      Saved s, float* __restrict__ loss) {
-  __shared__ f32x2 part[kBlock / 64][kReduceRows];
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * kReduceRows + threadIdx.x % kReduceRows;
-  const int which = threadIdx.x / kReduceRows;
+  __shared__ f32x2 part[kBlock / 64][ROWS];
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * ROWS + threadIdx.x % ROWS;
+  const int which = threadIdx.x / ROWS;
   const int at = row < rows ? s.packed[row] : -1;
   const int64_t column = packed ? at : row;  // of the sums
   f32x2 total = {-__builtin_inff(), 0.0f};
   if (at >= 0) {
 #pragma unroll 8
-    for (int t = which; t < tiles; t += kReduceParts) total = join(total, sums[static_cast<int64_t>(t) * row_tiles + column]);
+    for (int t = which; t < tiles; t += (kBlock / ROWS)) total = join(total, sums[static_cast<int64_t>(t) * row_tiles + column]);
   }
 #pragma unroll
-  for (int step = kReduceRows; step < 64; step <<= 1) {
+  for (int step = ROWS; step < 64; step <<= 1) {
     total = join(total, f32x2{__shfl_xor(total.x, step, 64), __shfl_xor(total.y, step, 64)});
   }
-  if (threadIdx.x % 64 < kReduceRows) part[threadIdx.x / 64][threadIdx.x % 64] = total;
+  if (threadIdx.x % 64 < ROWS) part[threadIdx.x / 64][threadIdx.x % 64] = total;
   __syncthreads();
   if (which != 0 || row >= rows) return;
   if (at < 0) {
@@ -1679,8 +1686,10 @@ void loss_forward(const Call& c, const void* targets, int target_bytes, int64_t 
                          c.stream, g);
     }
     float* losses = reduction == ATTNRES_REDUCE_NONE ? loss : c.at<float>(p.losses);
-    hipLaunchKernelGGL(attnres_loss_reduce_kernel, dim3(static_cast<unsigned>((c.rows + kReduceRows - 1) / kReduceRows)), dim3(kBlock), 0,
-                       c.stream, sums, tiles, row_tiles, target_logit, c.rows, !p.few, c.saved, losses);
+    const bool many = c.rows >= 16 * kUnits;
+    const auto reduce = many ? attnres_loss_reduce_kernel<16> : attnres_loss_reduce_kernel<4>;
+    hipLaunchKernelGGL(reduce, dim3(static_cast<unsigned>((c.rows + (many ? 15 : 3)) / (many ? 16 : 4))), dim3(kBlock), 0, c.stream,
+                       sums, tiles, row_tiles, target_logit, c.rows, !p.few, c.saved, losses);
   }
   if (reduction != ATTNRES_REDUCE_NONE) {
     hipLaunchKernelGGL(attnres_loss_total_kernel, dim3(1), dim3(kScanThreads), 0, c.stream, c.at<const float>(p.losses), c.rows,

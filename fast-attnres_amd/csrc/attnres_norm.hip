@@ -6,7 +6,8 @@
 //
 // Memory bound: the forward reads x and writes out, the backward reads x and dO
 // and writes dx, with about one FP32 operation per byte.  A row stays in the
-// registers of its lanes between its sums and its output, so each is read once.
+// registers of its lanes between its sums and its output, so each is read once.  32768 x 4096 BF16: forward
+// 98 us (5.5 TB/s), backward 154 us (5.2), its column sums 5.
 // Statistics are FP32, the variance a second sum over the centred row in
 // registers (no difference of squares).
 
@@ -168,7 +169,8 @@ __device__ __forceinline__ void row_sums(float& x, float& y, float (*scratch)[2]
 
 // The backward: each group of lanes walks over rows, adding up dw and db of its
 // own columns in registers; the groups of a workgroup meet in LDS once, at the end,
-// and the workgroup writes one partial row of each.
+// and the workgroup writes one partial row of each.  512 workgroups of 512 threads: with 768 or 1024 of them the partial
+// rows cost more than the walk gains.
 constexpr int kBwdBlock = 512;
 
 template <int LANES, int CH, class X, class P, bool PARAMS, bool PAST>

@@ -289,6 +289,51 @@ def test_loss_around_the_forward_of_few_rows(rows, dtype):
         _check_loss(hidden, weight, targets, "none", g)
 
 
+@pytest.mark.parametrize("reduction", ["none", "sum", "mean"])
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
+@pytest.mark.parametrize("recompute", [False, True])
+def test_loss_of_few_rows(reduction, dtype, recompute):
+    """Rows that lie apart, ignored ones that hold NaN, one gradient at a time, the same graph twice."""
+    for rows, width, vocab in ((3, 1000, 257), (20, 333, 2049), (32, 256, 31), (50, 77, 700)):
+        g, hidden, weight, targets = _loss_inputs(67 + rows, rows, width, vocab, dtype, 0.4)
+        wide = torch.full((rows, width + 5), NAN, device="cuda", dtype=dtype)
+        wide[:, 2:width + 2] = torch.where((targets == -100)[:, None], torch.full_like(hidden, NAN), hidden)
+        hidden = wide[:, 2:width + 2]
+        _check_loss(hidden, weight, targets, reduction, g, recompute=recompute)
+        h, w = hidden.detach().requires_grad_(True), weight.detach().requires_grad_(True)
+        out = layers.linear_cross_entropy(h, w, targets, reduction=reduction, recompute=recompute)
+        both = torch.autograd.grad(out, (h, w), torch.ones_like(out), retain_graph=True)
+        again = torch.autograd.grad(out, (h, w), torch.ones_like(out))
+        assert all(torch.equal(a, b) for a, b in zip(both, again))
+        for k, leaf in enumerate((h, w)):
+            alone = (h if k == 0 else h.detach(), w if k == 1 else w.detach())
+            out = layers.linear_cross_entropy(*alone, targets, reduction=reduction, recompute=recompute)
+            (one,) = torch.autograd.grad(out, leaf, torch.ones_like(out))
+            assert torch.equal(one, both[k])
+
+
+def test_loss_of_few_rows_marks_a_target_outside_the_vocabulary():
+    for recompute in (False, True):
+        g, hidden, weight, targets = _loss_inputs(71, 12, 96, 200, BF16)
+        targets[5] = 200
+        hidden.requires_grad_(True), weight.requires_grad_(True)
+        out = layers.linear_cross_entropy(hidden, weight, targets, reduction="none", recompute=recompute)
+        grad_hidden, grad_weight = torch.autograd.grad(out, (hidden, weight), torch.ones_like(out))
+        bad = torch.arange(12, device="cuda") == 5
+        assert torch.equal(out.isnan(), bad) and torch.equal(grad_hidden.isnan().all(-1), bad)
+        assert bool(grad_hidden[~bad].isfinite().all()) and bool(grad_weight.isnan().all())
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
+def test_loss_graph_kept_for_a_second_backward(dtype):
+    g, hidden, weight, targets = _loss_inputs(73, 400, 128, 1000, dtype, 0.2)
+    hidden.requires_grad_(True), weight.requires_grad_(True)
+    out = layers.linear_cross_entropy(hidden, weight, targets)
+    first = torch.autograd.grad(out, (hidden, weight), retain_graph=True)
+    second = torch.autograd.grad(out, (hidden, weight))
+    assert all(torch.equal(a, b) for a, b in zip(first, second))
+
+
 def test_loss_of_one_token_without_axes():
     g, hidden, weight, targets = _loss_inputs(40, 1, 64, 50, BF16)
     _check_loss(hidden[0].detach(), weight, targets[0], "mean", g)
