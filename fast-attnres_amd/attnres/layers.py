@@ -263,8 +263,8 @@ def linear_cross_entropy(hidden: Tensor, weight: Tensor, targets: Tensor, *, ign
     accuracy as pairs of FP16 numbers (relative to the largest magnitude of the tensor, so a tensor
     whose values span more than 2^25 loses the smallest, and infinities count as NaN).  Gradients
     flow to ``hidden`` and ``weight``.  For them the forward keeps the logits' exponentials, FP16 relative to
-    the largest of 128 for BF16 inputs (2 bytes per target and word), else FP32 (4), where that is at most 8 GiB; beyond
-    that, or with ``recompute=True``, it keeps 20 bytes per target and the backward forms them again, for one piece of
+    the largest of 128 for BF16 inputs (2 bytes per target and word), else FP32 (4), where that is at most 8 GiB, and
+    the operands it has packed; beyond that, or with ``recompute=True``, it keeps 20 bytes per target and the backward forms them again, for one piece of
     the vocabulary at a time, which adds a third to its products.
     """
     _check_tensor(hidden, "hidden", _FLOATS)
@@ -304,12 +304,16 @@ def _loss_saved_bytes(rows: int, vocab: int, width: int, dtype: torch.dtype, kee
     size = 256 + 20 * rows
     if not keep or rows == 0:
         return size
-    if rows <= (64 if dtype == torch.float32 or width % 32 else 32):
-        sums, powers = 0, 4 * (16 if rows <= 16 else 32 if rows <= 32 else 64) * (-(-vocab // 128) * 128)
+    pack = dtype == torch.float32 or width % 32 != 0
+    if rows <= (64 if pack else 32):
+        other, powers = 0, 4 * (16 if rows <= 16 else 32 if rows <= 32 else 64) * (-(-vocab // 128) * 128)
     else:
-        rows, vocab = (-(-n // _LOSS_TILE) * _LOSS_TILE for n in (rows, vocab))
-        sums, powers = 8 * (vocab // 128) * rows, (2 if dtype == torch.bfloat16 else 4) * rows * vocab
-    return size if powers > _MAX_KEPT else -(-size // 256) * 256 + sums + powers
+        width = -(-width // 32) * 32
+        rows, padded = (-(-n // _LOSS_TILE) * _LOSS_TILE for n in (rows, vocab))
+        powers = (2 if dtype == torch.bfloat16 else 4) * rows * padded
+        operands = 2 * rows * width + (-(-2 * vocab * width // 256) * 256 if pack else 0)
+        other = 8 * (padded // 128) * rows + (2 if dtype == torch.float32 else 1) * operands
+    return size if powers > _MAX_KEPT else -(-size // 256) * 256 + other + powers
 
 
 @torch.library.custom_op("attnres_hip::linear_cross_entropy", mutates_args=(), device_types="cuda", tags=_OP_TAGS)

@@ -1517,9 +1517,15 @@ LossPlan loss_plan(int64_t rows, int64_t vocab, int64_t width, int dtype, bool k
     p.saved_bytes = p.saved_powers + powers;
   }
   const bool scores = !backward || (p.few && !p.keep);  // the forward's kernels run
-  if (!p.few) {
-    for (int k = 0; k < parts; ++k) p.hidden[k] = take(2 * p.rows_pad * p.width_pad);
-    for (int k = 0; p.pack_weight && k < parts; ++k) p.weight[k] = take(2 * vocab * p.width_pad);
+  if (!p.few) {  // packed operands: kept beside the powers
+    const auto place = [&](int64_t bytes) {
+      if (!p.keep) return take(bytes);
+      const int64_t from = p.saved_bytes;
+      p.saved_bytes += round_up(bytes, 256);
+      return from;
+    };
+    for (int k = 0; k < parts; ++k) p.hidden[k] = place(2 * p.rows_pad * p.width_pad);
+    for (int k = 0; p.pack_weight && k < parts; ++k) p.weight[k] = place(2 * vocab * p.width_pad);
   }
   if (scores) {
     if (p.few) p.sums = take(8 * (p.logits_ld / kFewWords) * kFewRows);
@@ -1572,18 +1578,22 @@ struct Call {
   hipStream_t stream;
   template <class X>
   X* at(int64_t offset) const { return reinterpret_cast<X*>(workspace + offset); }
+  uint16_t* operand(int64_t offset) const {
+    return reinterpret_cast<uint16_t*>((plan.keep ? reinterpret_cast<char*>(saved.header) : workspace) + offset);
+  }
 };
 
-// The operands of both directions: H's rows that count, packed, and W as it is or packed.
+// The operands of both directions: H's rows that count, packed, and W as it is or packed.  The backward finds
+// them packed where powers are kept.
 template <class X>
-void prepare_operands(const Call& c, bool find_scales, Operand* h, Operand* w) {
+void prepare_operands(const Call& c, bool forward, Operand* h, Operand* w) {
   const LossPlan& p = c.plan;
   constexpr bool kSplit = std::is_same_v<X, float>;
   const X* hidden = static_cast<const X*>(c.hidden);
   const X* weight = static_cast<const X*>(c.weight);
   Header* header = c.saved.header;
   if constexpr (kSplit) {
-    if (find_scales) {
+    if (forward) {
       const unsigned grid_h = static_cast<unsigned>(std::min<int64_t>(c.rows, 1024));
       hipLaunchKernelGGL(attnres_loss_amax_kernel, dim3(grid_h), dim3(kBlock), 0, c.stream, hidden, c.hidden_stride, c.rows,
                          static_cast<int>(c.width), c.saved.index, &header->count, &header->amax[0]);
@@ -1593,16 +1603,21 @@ void prepare_operands(const Call& c, bool find_scales, Operand* h, Operand* w) {
                          &header->amax[1]);
     }
   }
-  uint16_t* packed[2] = {c.at<uint16_t>(p.hidden[0]), kSplit ? c.at<uint16_t>(p.hidden[1]) : nullptr};
-  hipLaunchKernelGGL((attnres_loss_pack_kernel<X>), dim3(stride_grid(p.rows_pad * p.width_pad / kVec)), dim3(kBlock), 0, c.stream,
-                     hidden, c.hidden_stride, c.rows, static_cast<int>(c.width), c.saved.index, &header->count, p.rows_pad,
-                     static_cast<int>(p.width_pad), header, 0, find_scales, packed[0], packed[1]);
+  const bool pack = forward || !p.keep;
+  uint16_t* packed[2] = {c.operand(p.hidden[0]), kSplit ? c.operand(p.hidden[1]) : nullptr};
+  if (pack) {
+    hipLaunchKernelGGL((attnres_loss_pack_kernel<X>), dim3(stride_grid(p.rows_pad * p.width_pad / kVec)), dim3(kBlock), 0, c.stream,
+                       hidden, c.hidden_stride, c.rows, static_cast<int>(c.width), c.saved.index, &header->count, p.rows_pad,
+                       static_cast<int>(p.width_pad), header, 0, forward, packed[0], packed[1]);
+  }
   *h = {{packed[0], packed[1]}, p.width_pad, p.rows_pad, 0};
   if (p.pack_weight) {
-    uint16_t* to[2] = {c.at<uint16_t>(p.weight[0]), kSplit ? c.at<uint16_t>(p.weight[1]) : nullptr};
-    hipLaunchKernelGGL((attnres_loss_pack_kernel<X>), dim3(stride_grid(c.vocab * p.width_pad / kVec)), dim3(kBlock), 0, c.stream,
-                       weight, c.weight_stride, c.vocab, static_cast<int>(c.width), static_cast<const int32_t*>(nullptr),
-                       static_cast<const int32_t*>(nullptr), c.vocab, static_cast<int>(p.width_pad), header, 1, find_scales, to[0], to[1]);
+    uint16_t* to[2] = {c.operand(p.weight[0]), kSplit ? c.operand(p.weight[1]) : nullptr};
+    if (pack) {
+      hipLaunchKernelGGL((attnres_loss_pack_kernel<X>), dim3(stride_grid(c.vocab * p.width_pad / kVec)), dim3(kBlock), 0, c.stream,
+                         weight, c.weight_stride, c.vocab, static_cast<int>(c.width), static_cast<const int32_t*>(nullptr),
+                         static_cast<const int32_t*>(nullptr), c.vocab, static_cast<int>(p.width_pad), header, 1, forward, to[0], to[1]);
+    }
     *w = {{to[0], to[1]}, p.width_pad, c.vocab, 0};
   } else {
     *w = {{reinterpret_cast<const uint16_t*>(weight), nullptr}, c.weight_stride, c.vocab, 0};

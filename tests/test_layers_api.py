@@ -224,8 +224,8 @@ def test_workspaces_are_of_the_shape_alone():
     # 131072 words needs far less than the 4 GiB of BF16 probabilities
     for keep in (0, 1):
         assert lib.attnres_hip_loss_workspace_bytes(16384, 131072, 2048, 0, keep, 1) < 1 << 30
-    # kept exponentials: 2 bytes each and 1 / 32 of that, up to 8 GiB
+    # kept exponentials: 2 bytes each and 1 / 32 of that, up to 8 GiB, and the rows that count
     assert lib.attnres_hip_loss_saved_bytes(16384, 131072, 2048, 0, 0) == 256 + 20 * 16384
-    assert 1 << 32 < lib.attnres_hip_loss_saved_bytes(16384, 131072, 2048, 0, 1) < 1.04 * 2**32
-    assert 1 << 33 < lib.attnres_hip_loss_saved_bytes(32768, 131072, 2048, 0, 1) < 1.04 * 2**33
+    assert 1 << 32 < lib.attnres_hip_loss_saved_bytes(16384, 131072, 2048, 0, 1) < 1.04 * 2**32 + 2**26
+    assert 1 << 33 < lib.attnres_hip_loss_saved_bytes(32768, 131072, 2048, 0, 1) < 1.04 * 2**33 + 2**27
     assert lib.attnres_hip_loss_saved_bytes(32769, 131072, 2048, 0, 1) == 256 + 20 * 32769
