@@ -864,16 +864,17 @@ __global__ void __launch_bounds__(kScanThreads) attnres_loss_rows_kernel(const v
 
 // ------------------------------------------------------------------- few rows
 // The forward of few rows (few_rows()) reads W once and is bound by that.  A workgroup takes 128 words, 32 to four
-// wavefronts, which share the k's (so that all of W is asked for at once); W and H go straight to registers as
+// wavefronts, which share the k's (so that all of W is asked for at once); where that would leave half of the units
+// without work, 32 words to sixteen (3 rows of 3840 x 3510 FP16 32 -> 14 us; of 32767 x 1024 BF16 23 -> 32, as H is read
+// oftener); W and H go straight to registers as
 // they lie (any width and alignment; FP32 inputs by FP32 matrix instructions, which the few rows have time for),
 // no packing: a row's logits are its own, so ignored rows are worked on and left out afterwards.  A
 // lane holds 16 bytes of every 64 of its word or row; the order of the k's in a matrix instruction is of no
 // account, as both operands share it.  16 rows of a 32768 x 1024 BF16 vocabulary (67 MB): 17.6 us, 3.8 TB/s (by 256 x
 // 256 tiles 27 us and 8 for packing).
 constexpr int kFewRows = 64;
-constexpr int kFewWords = 128;                        // of a workgroup; 32 to a wavefront
-constexpr int kFewParts = 4;                          // of the k's
-constexpr int kFewBlock = kFewWords / 32 * kFewParts * 64;
+constexpr int kFewBlock = 1024;
+constexpr int kFewWords = 128;  // of a workgroup, at most
 
 template <class X>
 struct FewChunk {  // a lane's 16 of 64 k's, as they lie: 16 bytes of every 64
@@ -935,18 +936,19 @@ struct FewArgs {
   int64_t logits_ld;
 };
 
-template <class X, int TILES>  // of 16 rows
+template <class X, int TILES, int WORDS>  // TILES of 16 rows
 __global__ void __launch_bounds__(kFewBlock) attnres_loss_few_kernel(FewArgs<X> g) {
+  constexpr int kGroups = WORDS / 32, kFewParts = kFewBlock / 64 / kGroups;
   __shared__ int target[kFewRows];  // -1: not known or ignored
   __shared__ f32x4 parts[kFewBlock / 64][64];
-  __shared__ f32x2 meet[kFewWords / 32][TILES * 16];
+  __shared__ f32x2 meet[kGroups][TILES * 16];
   const int wave = wave_index(), lane = threadIdx.x % 64, group = lane / 16, entry = lane % 16;
   const int part = wave % kFewParts, words = wave / kFewParts;
-  const int64_t v0 = static_cast<int64_t>(blockIdx.x) * kFewWords + words * 32;
+  const int64_t v0 = static_cast<int64_t>(blockIdx.x) * WORDS + words * 32;
   const X* w[2];
 #pragma unroll
   for (int i = 0; i < 2; ++i) w[i] = g.weight + min(v0 + i * 16 + entry, g.vocab - 1) * g.weight_stride;
-  constexpr int kSteps = sizeof(X) == 4 || TILES == 4 ? 1 : 2;  // of 64 k's under way together
+  constexpr int kSteps = sizeof(X) == 4 || TILES == 4 || WORDS == 32 ? 1 : 2;  // of 64 k's under way together
   constexpr int kSpan = kSteps * 64;
   FewChunk<X> next[kSteps][2];
   const auto fetch = [&](int k0) {
@@ -1047,7 +1049,7 @@ __global__ void __launch_bounds__(kFewBlock) attnres_loss_few_kernel(FewArgs<X> 
   if (threadIdx.x < TILES * 16) {
     f32x2 sum = meet[0][threadIdx.x];
 #pragma unroll
-    for (int k = 1; k < kFewWords / 32; ++k) sum = join(sum, meet[k][threadIdx.x]);
+    for (int k = 1; k < kGroups; ++k) sum = join(sum, meet[k][threadIdx.x]);
     g.sums[static_cast<int64_t>(blockIdx.x) * kFewRows + threadIdx.x] = sum;
   }
 }
@@ -1484,7 +1486,7 @@ struct LossPlan {
   int64_t rows_pad, width_pad, vocab_pad, piece;
   int64_t hidden[2], weight[2], sums, target_logit, losses;  // offsets
   int64_t row_scale, alpha, p[2], dh, dw, logits, logits_ld;
-  int few_tiles, parts;
+  int few_tiles, few_words, parts;
   int splits_h, splits_w;
   int64_t bytes;
   int64_t saved_sums, saved_powers, saved_bytes;
@@ -1506,6 +1508,7 @@ LossPlan loss_plan(int64_t rows, int64_t vocab, int64_t width, int dtype, bool k
   };
   p.few = rows > 0 && rows <= few_rows(p.pack_weight);
   p.few_tiles = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
+  p.few_words = vocab > kFewWords / 2 * kUnits ? kFewWords : 32;
   p.logits_ld = round_up(vocab, kFewWords);
   const int64_t logits = 4 * 16 * p.few_tiles * p.logits_ld;
   const int64_t powers = p.few ? logits : (dtype == ATTNRES_BF16 ? 2 : 4) * p.rows_pad * p.vocab_pad;
@@ -1528,7 +1531,7 @@ LossPlan loss_plan(int64_t rows, int64_t vocab, int64_t width, int dtype, bool k
     for (int k = 0; p.pack_weight && k < parts; ++k) p.weight[k] = place(2 * vocab * p.width_pad);
   }
   if (scores) {
-    if (p.few) p.sums = take(8 * (p.logits_ld / kFewWords) * kFewRows);
+    if (p.few) p.sums = take(8 * (p.logits_ld / p.few_words) * kFewRows);
     else if (!p.keep) p.sums = take(8 * (p.vocab_pad / 128) * p.rows_pad);
     p.target_logit = take(4 * p.rows_pad);
   }
@@ -1632,10 +1635,18 @@ void launch_few(const Call& c, const void* targets, int target_bytes, int64_t ig
   const FewArgs<X> g{static_cast<const X*>(c.hidden), static_cast<const X*>(c.weight), c.hidden_stride, c.weight_stride, c.vocab,
                      static_cast<int>(c.width), static_cast<int>(c.rows), targets, target_bytes, ignore_index, c.saved,
                      c.at<f32x2>(p.sums), c.at<float>(p.target_logit), logits, p.logits_ld};
-  const auto kernel = p.few_tiles == 1   ? attnres_loss_few_kernel<X, 1>
-                      : p.few_tiles == 2 ? attnres_loss_few_kernel<X, 2>
-                                         : attnres_loss_few_kernel<X, 4>;
-  hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(p.logits_ld / kFewWords)), dim3(kFewBlock), 0, c.stream, g);
+  const auto launch = [&](auto words) {
+    constexpr int WORDS = decltype(words)::value;
+    const auto kernel = p.few_tiles == 1   ? attnres_loss_few_kernel<X, 1, WORDS>
+                        : p.few_tiles == 2 ? attnres_loss_few_kernel<X, 2, WORDS>
+                                           : attnres_loss_few_kernel<X, 4, WORDS>;
+    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(p.logits_ld / WORDS)), dim3(kFewBlock), 0, c.stream, g);
+  };
+  if (p.few_words == 32) {
+    launch(std::integral_constant<int, 32>{});
+  } else {
+    launch(std::integral_constant<int, kFewWords>{});
+  }
 }
 
 template <class X>
@@ -1676,7 +1687,7 @@ void loss_forward(const Call& c, const void* targets, int target_bytes, int64_t 
     int tiles;
     int64_t row_tiles;
     if (p.few) {
-      tiles = static_cast<int>(p.logits_ld / kFewWords);
+      tiles = static_cast<int>(p.logits_ld / p.few_words);
       row_tiles = kFewRows;
       launch_few<X>(c, targets, target_bytes, ignore_index, static_cast<float*>(c.saved.powers));
     } else {

@@ -294,7 +294,7 @@ def test_loss_around_the_forward_of_few_rows(rows, dtype):
 @pytest.mark.parametrize("recompute", [False, True])
 def test_loss_of_few_rows(reduction, dtype, recompute):
     """Rows that lie apart, ignored ones that hold NaN, one gradient at a time, the same graph twice."""
-    for rows, width, vocab in ((3, 1000, 257), (20, 333, 2049), (32, 256, 31), (50, 77, 700)):
+    for rows, width, vocab in ((3, 1000, 257), (20, 333, 2049), (32, 256, 31), (50, 77, 700), (17, 72, 16500)):
         g, hidden, weight, targets = _loss_inputs(67 + rows, rows, width, vocab, dtype, 0.4)
         wide = torch.full((rows, width + 5), NAN, device="cuda", dtype=dtype)
         wide[:, 2:width + 2] = torch.where((targets == -100)[:, None], torch.full_like(hidden, NAN), hidden)
