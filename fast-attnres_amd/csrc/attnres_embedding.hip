@@ -4,8 +4,8 @@
 //   dW[v] = scale sum_{i: tok_i = v} dO_i,   dpos[t] = sum_b dO[b, t]
 //
 // Memory bound: the lookup reads one table row and writes one output row per token (32768 x 2048 BF16 of 131072 rows: 51
-// us); the gradient reads dO once and writes the whole table (there 537 MB: 210 us, half of it the sort's four launches,
-// which clear the table meanwhile at 5.1 TB/s).  The tokens are sorted (stable, least
+// us); the gradient reads dO once and writes the whole table (there 537 MB: 175 us, half of it the sort's four launches,
+// which clear the table meanwhile at 5.7 TB/s).  The tokens are sorted (stable, least
 // significant digit first), so every table row's sum is a run of the sorted list, added up in
 // FP32 in the order of the tokens: no atomics on values, the same bits every time.
 
@@ -103,12 +103,16 @@ struct ZeroFill {
 template <class W>
 __device__ __forceinline__ void zero_fill(const ZeroFill<W>& z, int64_t block, int64_t blocks) {
   float zero[kVec] = {};
-  const int64_t step = blocks * blockDim.x * kVec;
-  for (int64_t i = z.first + (block * blockDim.x + threadIdx.x) * kVec; i < z.end; i += step) {
-    if (i + kVec <= z.end) {
+  // each block a contiguous part: the gradient of 32768 tokens, 131072 x 2048 BF16, 181 -> 175 us against parts that lie
+  // a grid apart, of 8192 tokens, 262144 x 2048, 270 -> 229
+  const int64_t chunk = static_cast<int64_t>(blockDim.x) * kVec;
+  const int64_t part = ((z.end - z.first + chunk - 1) / chunk + blocks - 1) / blocks * chunk;
+  const int64_t from = z.first + block * part, end = min(from + part, z.end);
+  for (int64_t i = from + threadIdx.x * kVec; i < end; i += chunk) {
+    if (i + kVec <= end) {
       store8(z.to + i, zero, z.past);
     } else {
-      for (int64_t e = i; e < z.end; ++e) z.to[e] = from_f32<W>(0.0f);
+      for (int64_t e = i; e < end; ++e) z.to[e] = from_f32<W>(0.0f);
     }
   }
 }
