@@ -249,7 +249,7 @@ _embedding.register_autograd(_embedding_autograd, setup_context=_embedding_conte
 
 def linear_cross_entropy(hidden: Tensor, weight: Tensor, targets: Tensor, *, ignore_index: int = -100,
                          reduction: str = "mean", recompute: bool = False) -> Tensor:
-    """Softmax cross entropy of the logits ``hidden @ weight.T``, which are never stored in full precision.
+    """Softmax cross entropy of the logits ``hidden @ weight.T``, reduced where they are formed.
 
     ``hidden`` is ``[..., D]``, ``weight`` ``[V, D]``, both BF16, FP16 or FP32, one
     dtype, ``1 <= D <= 8192``; ``targets`` ``[...]`` int64 or int32.  The loss is
@@ -260,12 +260,14 @@ def linear_cross_entropy(hidden: Tensor, weight: Tensor, targets: Tensor, *, ign
     ``ignore_index`` nor in ``0..V-1`` makes the loss and the gradients NaN.
 
     16-bit inputs are multiplied on the matrix cores as they are, FP32 ones to FP32's
-    accuracy as pairs of FP16 numbers (relative to the largest magnitude of the tensor, so a tensor
-    whose values span more than 2^25 loses the smallest, and infinities count as NaN).  Gradients
-    flow to ``hidden`` and ``weight``.  For them the forward keeps the logits' exponentials, FP16 relative to
-    the largest of 128 for BF16 inputs (2 bytes per target and word), else FP32 (4), where that is at most 8 GiB, and
-    the operands it has packed; beyond that, or with ``recompute=True``, it keeps 20 bytes per target and the backward forms them again, for one piece of
-    the vocabulary at a time, which adds a third to its products.
+    accuracy as pairs of FP16 numbers (relative to the largest magnitude of the tensor,
+    so a tensor whose values span more than 2^25 loses the smallest, and infinities
+    count as NaN).  Gradients flow to ``hidden`` and ``weight``.  For them the forward
+    keeps the logits' exponentials (BF16 inputs: FP16 relative to the largest of 128, 2
+    bytes per target and word; else FP32, 4 bytes), where that is at most 8 GiB, and the
+    operands it has packed; beyond that, or with ``recompute=True``, it keeps 20 bytes
+    per target, and the backward forms them again, for one piece of the vocabulary at a
+    time, which adds a third to its products.
     """
     _check_tensor(hidden, "hidden", _FLOATS)
     _check_tensor(weight, "weight", _FLOATS)
