@@ -608,6 +608,50 @@ def test_layers_captured_and_replayed():
         torch.cuda.synchronize()
 
 
+def test_layers_on_two_streams_at_once():
+    """Calls that overlap share nothing: several passes on each of two streams, none waiting for the other."""
+    each = [_pass_inputs(seed) for seed in (151, 157)]
+    expected = [[t.detach().clone() for t in _training_pass(*inputs)] for inputs in each]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    leaves = []
+    for stream, inputs in zip(streams, each):
+        with torch.cuda.stream(stream):
+            leaves.append([t.detach().clone().requires_grad_(t.requires_grad) for t in inputs])
+    got = [[], []]
+    for _ in range(4):
+        for k, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                got[k].append([t.detach() for t in _training_pass(*leaves[k])])
+    torch.cuda.synchronize()
+    for results, wanted in zip(got, expected):
+        for result in results:
+            assert all(torch.equal(a, b) for a, b in zip(result, wanted))
+
+
+def test_two_graphs_replayed_at_once():
+    streams, graphs, outputs, expected = [], [], [], []
+    for seed in (163, 167):
+        stream = torch.cuda.Stream()
+        stream.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(stream):
+            static = _pass_inputs(seed)
+            for _ in range(2):
+                first = [t.detach().clone() for t in _training_pass(*static)]
+        stream.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            outputs.append(_training_pass(*static))
+        streams.append(stream), graphs.append((graph, static)), expected.append(first)
+    for _ in range(3):
+        for stream, (graph, _static) in zip(streams, graphs):
+            with torch.cuda.stream(stream):
+                graph.replay()
+        torch.cuda.synchronize()
+        for got, wanted in zip(outputs, expected):
+            assert all(torch.equal(a.detach(), b) for a, b in zip(got, wanted))
+
+
 def test_layers_compiled_match_eager():
     inputs = _pass_inputs(109)
     expected = [t.detach() for t in _training_pass(*inputs)]
