@@ -21,7 +21,9 @@
 // rounding.  Three FP16 products take 0.78 ms (16384 x 8192 x 1024, logits) where FP32 matrix instructions, at a
 // sixteenth of the FP16 rate, take 1.8 at the rate of a large library product.
 // P is rounded to the operands' type (BF16), or, for FP16 and FP32 inputs, scaled by
-// 2^14 and written as one or two FP16 numbers, so that probabilities down to 2^-28 are normal numbers.
+// 2^14 and written as one or two FP16 numbers, so that probabilities down to 2^-28 are normal numbers.  For BF16
+// inputs this is the gradients' largest error beside their own rounding: 0.0019 to 0.0026 relative, root mean square, for both
+// together, 0.0017 for the outputs' rounding alone.  P in FP16 would need W in FP16 as well, another copy of it.
 
 #include "attnres_layers.h"
 
