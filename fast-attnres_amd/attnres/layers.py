@@ -264,7 +264,7 @@ def linear_cross_entropy(hidden: Tensor, weight: Tensor, targets: Tensor, *, ign
     so a tensor whose values span more than 2^25 loses the smallest, and infinities
     count as NaN).  Gradients flow to ``hidden`` and ``weight``.  For them the forward
     keeps the logits' exponentials (BF16 inputs: FP16 relative to the largest of 128, 2
-    bytes per target and word; else FP32, 4 bytes), where that is at most 8 GiB, and the
+    bytes per target and word, the target's own unrounded; else FP32, 4 bytes), where that is at most 8 GiB, and the
     operands it has packed; beyond that, or with ``recompute=True``, it keeps 20 bytes
     per target, and the backward forms them again, for one piece of the vocabulary at a
     time, which adds a third to its products.
@@ -315,6 +315,8 @@ def _loss_saved_bytes(rows: int, vocab: int, width: int, dtype: torch.dtype, kee
         powers = (2 if dtype == torch.bfloat16 else 4) * rows * padded
         operands = 2 * rows * width + (-(-2 * vocab * width // 256) * 256 if pack else 0)
         other = 8 * (padded // 128) * rows + (2 if dtype == torch.float32 else 1) * operands
+        if dtype == torch.bfloat16:
+            other = other + 4 * rows  # the targets' logits
     return size if powers > _MAX_KEPT else -(-size // 256) * 256 + other + powers
 
 

@@ -63,7 +63,8 @@ struct Header {
   uint32_t amax[2];   // their largest finite magnitudes, as bits
 };
 
-// With `keep` also the (reference, sum) of every row and 128 columns and the powers themselves.
+// With `keep` also the (reference, sum) of every row and 128 columns, the powers themselves and, where those are rounded to
+// FP16, the target's logit of every packed row.
 struct Saved {
   Header* header;
   f32x2* stats;
@@ -71,6 +72,7 @@ struct Saved {
   int32_t* packed;
   int32_t* target;
   f32x2* sums;  // [columns / 128][row_tiles]
+  float* target_logit;  // [row_tiles]
   void* powers; // [row_tiles][vocabulary, padded]
 };
 
@@ -429,7 +431,9 @@ struct Logit {
 };
 
 // What powers are kept in for the backward.  BF16 operands: FP16, whose rounding of 2^-11 adds an eighth to
-// that of the probabilities to BF16.  Others: FP32, as FP16 would double the rounding of the probabilities to FP16.
+// that of the probabilities to BF16.  At the target that would be 2^-11 of p where P is p - 1, far more than P itself for a
+// token that is all but certain, so there the backward takes the power from the target's own logit, kept in FP32.
+// Others: FP32, as FP16 would double the rounding of the probabilities to FP16.
 template <class T>
 using Power = std::conditional_t<std::is_same_v<T, Bf16>, F16, float>;
 
@@ -451,7 +455,7 @@ struct LogitArgs {
   int64_t row_tiles;  // packed rows, padded
   // forward
   f32x2* sums;          // [columns / 128][row_tiles] (reference, sum of powers above it)
-  float* target_logit;  // [row_tiles]
+  float* target_logit;  // [row_tiles]; in the backward where the powers are FP16
   void* powers;         // [row_tiles][powers_ld], or nullptr: not kept
   int64_t powers_ld;
   // backward
@@ -593,7 +597,7 @@ __global__ void __launch_bounds__(kBlock) attnres_loss_rescale_kernel(LogitArgs 
   const int64_t v = g.first + column;
   const E* powers = static_cast<const E*>(g.powers);
   Chunk<E> chunk[kRounds];
-  float factor[kRounds], by[kRounds];
+  float factor[kRounds], by[kRounds], own[kRounds];
   int64_t rel[kRounds];
 #pragma unroll
   for (int k = 0; k < kRounds; ++k) {
@@ -604,6 +608,11 @@ __global__ void __launch_bounds__(kBlock) attnres_loss_rescale_kernel(LogitArgs 
     by[k] = g.row_scale[row];
     factor[k] = row < count ? power(sum.x - stats.x) * stats.y * by[k] : 0.0f;
     rel[k] = g.target[at] - v;
+    // the target's entry of FP16 powers, from its logit as in the recomputed probabilities; 0 past the last row
+    own[k] = 0.0f;
+    if (std::is_same_v<E, F16> && row < count && rel[k] >= 0 && rel[k] < kVec) {
+      own[k] = power(over_ln2(g.target_logit[row]) - stats.x) * (stats.y * by[k]);
+    }
   }
 #pragma unroll
   for (int k = 0; k < kRounds; ++k) {
@@ -613,7 +622,7 @@ __global__ void __launch_bounds__(kBlock) attnres_loss_rescale_kernel(LogitArgs 
 #pragma unroll
     for (int e = 0; e < kVec; ++e) {
       x[e] = row < count ? x[e] * factor[k] : 0.0f;
-      if (rel[k] == e) x[e] -= by[k];  // 0 past the last row
+      if (rel[k] == e) x[e] = (std::is_same_v<E, F16> ? own[k] : x[e]) - by[k];  // by: 0 past the last row
       if (PARTS == 2) asm("" : "+v"(x[e]));  // one rounding to hi, as in the recomputed probabilities
     }
 #pragma unroll
@@ -1491,7 +1500,7 @@ struct LossPlan {
   int few_tiles, few_words, parts;
   int splits_h, splits_w;
   int64_t bytes;
-  int64_t saved_sums, saved_powers, saved_bytes;
+  int64_t saved_sums, saved_target, saved_powers, saved_bytes;
 };
 
 LossPlan loss_plan(int64_t rows, int64_t vocab, int64_t width, int dtype, bool keep, bool backward) {
@@ -1518,7 +1527,8 @@ LossPlan loss_plan(int64_t rows, int64_t vocab, int64_t width, int dtype, bool k
   p.saved_bytes = kHeaderBytes + 20 * rows;
   if (p.keep) {
     p.saved_sums = round_up(p.saved_bytes, 256);
-    p.saved_powers = p.saved_sums + (p.few ? 0 : 8 * (p.vocab_pad / 128) * p.rows_pad);
+    p.saved_target = p.saved_sums + (p.few ? 0 : 8 * (p.vocab_pad / 128) * p.rows_pad);
+    p.saved_powers = p.saved_target + (!p.few && dtype == ATTNRES_BF16 ? 4 * p.rows_pad : 0);
     p.saved_bytes = p.saved_powers + powers;
   }
   const bool scores = !backward || (p.few && !p.keep);  // the forward's kernels run
@@ -1566,7 +1576,9 @@ Saved saved_views(void* base, int64_t rows, const LossPlan& p) {
   char* at = from + kHeaderBytes;
   return {reinterpret_cast<Header*>(from), reinterpret_cast<f32x2*>(at), reinterpret_cast<int32_t*>(at + 8 * rows),
           reinterpret_cast<int32_t*>(at + 12 * rows), reinterpret_cast<int32_t*>(at + 16 * rows),
-          p.keep ? reinterpret_cast<f32x2*>(from + p.saved_sums) : nullptr, p.keep ? from + p.saved_powers : nullptr};
+          p.keep ? reinterpret_cast<f32x2*>(from + p.saved_sums) : nullptr,
+          p.saved_powers > p.saved_target ? reinterpret_cast<float*>(from + p.saved_target) : nullptr,
+          p.keep ? from + p.saved_powers : nullptr};
 }
 
 unsigned stride_grid(int64_t items) { return static_cast<unsigned>(std::min<int64_t>((items + kBlock - 1) / kBlock, 8192)); }
@@ -1685,7 +1697,7 @@ void loss_forward(const Call& c, const void* targets, int target_bytes, int64_t 
   }
   if (c.rows > 0) {
     f32x2* sums = p.keep && !p.few ? c.saved.sums : c.at<f32x2>(p.sums);
-    float* target_logit = c.at<float>(p.target_logit);
+    float* target_logit = c.saved.target_logit != nullptr ? c.saved.target_logit : c.at<float>(p.target_logit);
     int tiles;
     int64_t row_tiles;
     if (p.few) {
@@ -1760,6 +1772,7 @@ void loss_backward(const Call& c, int reduction, const float* grad_loss, void* g
     if (p.keep) {
       using E = Power<T>;
       g.sums = c.saved.sums;
+      g.target_logit = c.saved.target_logit;
       g.powers = c.saved.powers;
       g.powers_ld = p.vocab_pad;
       const int64_t wide = static_cast<int64_t>(tiles_v) * kTile;

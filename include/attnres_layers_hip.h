@@ -85,7 +85,7 @@ int attnres_hip_embedding_backward(const void* grad_out, int out_dtype, const vo
  * when none does).  A target that is neither ignore_index nor in 0..vocab-1 makes
  * the loss and the gradients NaN.
  * saved: what the backward reads.  keep, the same in all calls: nonzero lets the forward keep the exponentials of the
- * logits there for the backward, 2 bytes each for BF16, else 4, rows and vocab padded
+ * logits there for the backward, 2 bytes each for BF16 (and 4 per row, the target's logit), else 4, rows and vocab padded
  * to 256, where that takes at most 8 GiB, and its packed operands (of few rows, up to 64, the FP32 logits); otherwise, and with 0, saved is 256 + 20 * rows bytes and the backward
  * forms them again, for one piece of the vocabulary at a time.  saved and
  * workspace start at multiples of 16 bytes (else ATTNRES_ERR_WORKSPACE). */
