@@ -262,7 +262,9 @@ def linear_cross_entropy(hidden: Tensor, weight: Tensor, targets: Tensor, *, ign
     16-bit inputs are multiplied on the matrix cores as they are, FP32 ones to FP32's
     accuracy as pairs of FP16 numbers (relative to the largest magnitude of the tensor,
     so a tensor whose values span more than 2^25 loses the smallest, and infinities
-    count as NaN).  Gradients flow to ``hidden`` and ``weight``.  For them the forward
+    count as NaN).  Upstream gradients of ``reduction="none"`` may differ by any factor: a row
+    of ``hidden``'s gradient is as accurate as if it were alone; what it adds to that of ``weight`` is
+    held, for FP16 and FP32, to 2^-39 of the largest row of ``hidden`` times its upstream gradient.  Gradients flow to ``hidden`` and ``weight``.  For them the forward
     keeps the logits' exponentials (BF16 inputs: FP16 relative to the largest of 128, 2
     bytes per target and word, the target's own unrounded; else FP32, 4 bytes), where that is at most 8 GiB, and the
     operands it has packed; beyond that, or with ``recompute=True``, it keeps 20 bytes

@@ -248,7 +248,8 @@ Rows weight_rows(const Tensor& weight) {
   return rows;
 }
 
-Tensor loss_workspace(const Tensor& hidden, const Tensor& weight, int64_t rows, bool keep, bool backward) {
+// backward: as attnres_hip_loss_workspace_bytes takes it.
+Tensor loss_workspace(const Tensor& hidden, const Tensor& weight, int64_t rows, bool keep, int backward) {
   const int64_t bytes =
       attnres_hip_loss_workspace_bytes(rows, weight.size(0), weight.size(1), dtype_of(weight.scalar_type()), keep, backward);
   TORCH_CHECK_VALUE(bytes >= 0, "linear cross entropy: shape outside the supported envelope");
@@ -265,7 +266,7 @@ std::tuple<Tensor, Tensor> loss_forward(const Tensor& hidden, const Tensor& weig
   const int64_t rows = ids.numel();
   const auto floats = hidden.options().dtype(torch::kFloat32);
   Tensor loss = reduction == ATTNRES_REDUCE_NONE ? torch::empty(targets.sizes(), floats) : torch::empty({}, floats);
-  Tensor workspace = loss_workspace(hidden, weight, rows, keep, false);
+  Tensor workspace = loss_workspace(hidden, weight, rows, keep, 0);
   Tensor saved = torch::empty(
       {attnres_hip_loss_saved_bytes(rows, weight.size(0), weight.size(1), dtype_of(weight.scalar_type()), keep)},
       hidden.options().dtype(torch::kUInt8));
@@ -295,7 +296,7 @@ std::tuple<Tensor, Tensor> loss_backward(const Tensor& grad_loss, const Tensor& 
   }
   Tensor grad_weight = want_weight ? torch::empty(weight.sizes(), weight.options().memory_format(contiguous))
                                    : torch::empty({0}, weight.options());
-  Tensor workspace = loss_workspace(hidden, weight, rows, keep, true);
+  Tensor workspace = loss_workspace(hidden, weight, rows, keep, reduction == ATTNRES_REDUCE_NONE ? 1 : 2);
   check(attnres_hip_loss_backward(h.tensor.data_ptr(), h.stride, w.tensor.data_ptr(), w.stride, rows, weight.size(0),
                                   weight.size(1), dtype_of(hidden.scalar_type()), static_cast<int>(reduction), keep, saved.data_ptr(),
                                   grad.data_ptr<float>(), want_hidden ? grad_hidden.data_ptr() : nullptr,

@@ -1263,20 +1263,33 @@ __global__ void __launch_bounds__(kBlock) attnres_loss_few_join_kernel(const flo
   }
 }
 
+// Upstream gradients of rows that differ (no reduction), for operands of FP16, which has no exponents for them: P is of a
+// gradient in [1/2, 1), and the rest, a power of two per row, multiplies the row of dH after its product and the row of H before
+// that of dW, in a copy of H of its own (P with the largest row's power would hold a row of weight w of it to 2^-39 / w).  What a row
+// adds to dW is held to 2^-39 of the largest product of H and its row's power.
+struct RowPowers {
+  const float* power;  // per packed row; nullptr: none
+  float* alpha;        // dW's two factors, the largest magnitude of H times its row's power over the largest power (as bits), that power
+  __device__ __forceinline__ float of(int64_t row) const { return power[row] / alpha[3]; }
+};
+
 // Largest finite magnitude of the rows (an integer maximum of the bits: the same in any order).
-__global__ void __launch_bounds__(kBlock) attnres_loss_amax_kernel(const float* __restrict__ x, int64_t stride, int64_t rows, int width,
-                                                                   const int32_t* index, const int32_t* count, uint32_t* amax) {
+template <class X>
+__global__ void __launch_bounds__(kBlock) attnres_loss_amax_kernel(const X* __restrict__ x, int64_t stride, int64_t rows, int width,
+                                                                   const int32_t* index, const int32_t* count, RowPowers powers,
+                                                                   uint32_t* amax) {
   __shared__ uint32_t waves[kBlock / 64];
   const int64_t live = count != nullptr ? *count : rows;
   uint32_t top = 0;
   for (int64_t r = blockIdx.x; r < live; r += gridDim.x) {
-    const float* row = x + (index != nullptr ? index[r] : r) * stride;
+    const X* row = x + (index != nullptr ? index[r] : r) * stride;
+    const float by = powers.power != nullptr ? powers.of(r) : 1.0f;
     for (int c = threadIdx.x * kVec; c < width; c += kBlock * kVec) {
       float v[kVec];
       load_chunk(row, c, width, v);
 #pragma unroll
       for (int e = 0; e < kVec; ++e) {
-        const uint32_t bits = __float_as_uint(v[e]) & 0x7fffffffu;
+        const uint32_t bits = __float_as_uint(v[e] * by) & 0x7fffffffu;
         if (bits < 0x7f800000u && bits > top) top = bits;
       }
     }
@@ -1291,6 +1304,9 @@ __global__ void __launch_bounds__(kBlock) attnres_loss_amax_kernel(const float* 
   }
 }
 
+// Of a power of two that is a normal number.
+__device__ __forceinline__ int exponent_of(float x) { return static_cast<int>(__float_as_uint(x) >> 23) - 127; }
+
 // The power of two that takes the largest magnitude into [2^14, 2^15), within 2^-110..2^110.
 __device__ __forceinline__ float split_scale(uint32_t amax) {
   if (amax == 0) return 1.0f;
@@ -1300,15 +1316,25 @@ __device__ __forceinline__ float split_scale(uint32_t amax) {
 }
 
 // Rows to operands: [rows_out][width_out] zero-padded, as they are (X 16 bits) or as hi and
-// lo (X float).  index/count: the rows that count.
-template <class X>
+// lo (X float).  index/count: the rows that count.  WEIGHED: times their rows' powers, scaled as FP32 rows are.
+template <class X, bool WEIGHED>
 __global__ void __launch_bounds__(kBlock) attnres_loss_pack_kernel(const X* __restrict__ x, int64_t stride, int64_t rows, int width,
                                                                    const int32_t* index, const int32_t* count, int64_t rows_out,
                                                                    int width_out, Header* header, int which, bool keep_scale,
-                                                                   uint16_t* __restrict__ hi, uint16_t* __restrict__ lo) {
+                                                                   RowPowers powers, uint16_t* __restrict__ hi,
+                                                                   uint16_t* __restrict__ lo) {
   const int64_t live = count != nullptr ? *count : rows;
   float scale = 1.0f;
-  if constexpr (std::is_same_v<X, float>) {
+  if constexpr (WEIGHED) {
+    scale = split_scale(__float_as_uint(powers.alpha[2]));
+    if (blockIdx.x == 0 && threadIdx.x == 0) {
+      // of dW: the largest power over the scales of P and of this copy, in two factors where one does not hold it
+      const int exponent = exponent_of(powers.alpha[3]) - exponent_of(kProbabilityScale) - exponent_of(scale);
+      const int first = min(127, max(-126, exponent));
+      powers.alpha[0] = ldexpf(1.0f, first);
+      powers.alpha[1] = ldexpf(1.0f, exponent - first);
+    }
+  } else if constexpr (std::is_same_v<X, float>) {
     scale = split_scale(header->amax[which]);
     if (keep_scale && blockIdx.x == 0 && threadIdx.x == 0) header->scale[which] = scale;
   }
@@ -1322,10 +1348,11 @@ __global__ void __launch_bounds__(kBlock) attnres_loss_pack_kernel(const X* __re
       const X* row = x + (index != nullptr ? index[r] : r) * stride;
       float v[kVec];
       load_chunk(row, c, width, v);
+      const float by = WEIGHED ? powers.of(r) * scale : scale;
       if constexpr (std::is_same_v<X, float>) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          float a = v[2 * e] * scale, b = v[2 * e + 1] * scale;
+          float a = v[2 * e] * by, b = v[2 * e + 1] * by;
           asm("" : "+v"(a), "+v"(b));  // one rounding to hi, as in the probabilities
           h[e] = pack2<F16>(a, b);
           l[e] = pack2<F16>(a - to_f32(F16{static_cast<uint16_t>(h[e] & 0xffffu)}),
@@ -1333,7 +1360,7 @@ __global__ void __launch_bounds__(kBlock) attnres_loss_pack_kernel(const X* __re
         }
       } else {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) h[e] = pack2<X>(v[2 * e], v[2 * e + 1]);
+        for (int e = 0; e < 4; ++e) h[e] = WEIGHED ? pack2<X>(v[2 * e] * by, v[2 * e + 1] * by) : pack2<X>(v[2 * e], v[2 * e + 1]);
       }
     }
     *reinterpret_cast<u32x4*>(hi + i * kVec) = h;
@@ -1394,14 +1421,18 @@ __global__ void __launch_bounds__(kScanThreads) attnres_loss_total_kernel(const 
   out[0] = mean ? sum / static_cast<float>(header->count) : sum;
 }
 
-// Factors of the backward: per packed row its upstream gradient over the largest one's power of two (one
-// row's factor is at most 1), times the scale of P; and what the outputs are multiplied by.
+// Factors of the backward: per packed row its upstream gradient over a power of two, its own (row_power) or the
+// largest one's (one row's factor is at most 1), times the scale of P; and what the outputs are multiplied by.
 __global__ void __launch_bounds__(kScanThreads) attnres_loss_factors_kernel(const float* __restrict__ grad_loss, int reduction, Saved s,
                                                                             int64_t row_tiles, float p_scale, float* row_scale,
-                                                                            float* alpha) {
+                                                                            float* row_power, float* alpha) {
   __shared__ uint32_t waves[kScanThreads / 64];
   const int count = s.header->count;
-  float outer = count > 0 ? 1.0f : 0.0f;  // nothing counts: zero gradients
+  float outer = count > 0 || row_power != nullptr ? 1.0f : 0.0f;  // nothing counts: zero gradients
+  // the power of two above a magnitude, from 2^(least - 127) to 2^(most - 127)
+  const auto above = [](uint32_t bits, int least, int most) {
+    return __uint_as_float(static_cast<uint32_t>(min(most, max(least, static_cast<int>(bits >> 23) + 1))) << 23);
+  };
   if (count > 0 && reduction == ATTNRES_REDUCE_NONE) {
     uint32_t top = 0;
     for (int r = threadIdx.x; r < count; r += kScanThreads) {
@@ -1414,29 +1445,44 @@ __global__ void __launch_bounds__(kScanThreads) attnres_loss_factors_kernel(cons
     __syncthreads();
     top = 0;
     for (int w = 0; w < kScanThreads / 64; ++w) top = max(top, waves[w]);
-    if (top != 0) outer = __uint_as_float(static_cast<uint32_t>(min(227, max(27, static_cast<int>(top >> 23) + 1))) << 23);
+    if (top != 0) outer = row_power != nullptr ? above(top, 1, 254) : above(top, 27, 227);
   } else if (count > 0) {
     outer = reduction == ATTNRES_REDUCE_MEAN ? grad_loss[0] / static_cast<float>(count) : grad_loss[0];
   }
   for (int64_t r = threadIdx.x; r < row_tiles; r += kScanThreads) {
     float by = 0.0f;
-    if (r < count) by = reduction == ATTNRES_REDUCE_NONE ? grad_loss[s.index[r]] / outer * p_scale : p_scale;
+    if (r < count && reduction == ATTNRES_REDUCE_NONE) {
+      const float grad = grad_loss[s.index[r]];
+      float over = outer;
+      if (row_power != nullptr) {
+        const uint32_t bits = __float_as_uint(grad) & 0x7fffffffu;
+        if (bits < 0x7f800000u) over = above(bits, 1, 254);
+        row_power[r] = over;
+      }
+      by = grad / over * p_scale;
+    } else if (r < count) {
+      by = p_scale;
+    }
     row_scale[r] = by;
   }
   if (threadIdx.x == 0) {
     // of dH = P W and dW = P^T H; two factors each, as their product may leave FP32 where the gradient does not
-    alpha[0] = alpha[2] = outer / p_scale;
+    alpha[0] = (row_power != nullptr ? 1.0f : outer) / p_scale;
     alpha[1] = 1.0f / s.header->scale[1];
+    alpha[2] = outer / p_scale;
     alpha[3] = 1.0f / s.header->scale[0];
+    alpha[4] = 0.0f;  // the rest for row_power
+    alpha[5] = outer;
   }
 }
 
-// out[r] = both alpha's times the sum of the splits' partial rows; packed: of the row's packed one, zeros
-// where it has none.
+// out[r] = both alpha's (and the row's power) times the sum of the splits' partial rows; packed: of the row's packed one,
+// zeros where it has none.
 template <class OUT>
 __global__ void __launch_bounds__(kBlock) attnres_loss_join_kernel(const float* __restrict__ partial, int splits, int64_t split_stride,
                                                                    int64_t ld, const int32_t* packed, int64_t rows, int width,
-                                                                   const float* __restrict__ alpha, OUT* __restrict__ out) {
+                                                                   const float* __restrict__ alpha, const float* __restrict__ row_power,
+                                                                   OUT* __restrict__ out) {
   const float by = alpha[0], unscale = alpha[1];
   const int chunks = (width + kVec - 1) / kVec;
   const int64_t all = rows * chunks;
@@ -1454,7 +1500,11 @@ __global__ void __launch_bounds__(kBlock) attnres_loss_join_kernel(const float* 
         for (int e = 0; e < kVec; ++e) sum[e] += x[e];
       }
 #pragma unroll
-      for (int e = 0; e < kVec; ++e) sum[e] = sum[e] * by * unscale;
+      for (int e = 0; e < kVec; ++e) {
+        // powers of two all three: their exponents' sum leaves FP32 only where the gradient does
+        sum[e] = row_power != nullptr ? ldexpf(sum[e], exponent_of(by) + exponent_of(unscale) + exponent_of(row_power[at]))
+                                      : sum[e] * by * unscale;
+      }
     }
     store_chunk(out + r * width, c, width, sum);
   }
@@ -1496,14 +1546,17 @@ struct LossPlan {
   bool split, pack_weight, few, keep;
   int64_t rows_pad, width_pad, vocab_pad, piece;
   int64_t hidden[2], weight[2], sums, target_logit, losses;  // offsets
-  int64_t row_scale, alpha, p[2], dh, dw, logits, logits_ld;
+  int64_t row_scale, row_power, alpha, weighed[2], p[2], dh, dw, logits, logits_ld;
   int few_tiles, few_words, parts;
   int splits_h, splits_w;
   int64_t bytes;
   int64_t saved_sums, saved_target, saved_powers, saved_bytes;
 };
 
-LossPlan loss_plan(int64_t rows, int64_t vocab, int64_t width, int dtype, bool keep, bool backward) {
+enum Pass { kForward = 0, kBackward = 1, kBackwardOfTotal = 2 };  // the last: of a sum or mean, which has one upstream gradient
+
+LossPlan loss_plan(int64_t rows, int64_t vocab, int64_t width, int dtype, bool keep, int pass) {
+  const bool backward = pass != kForward;
   LossPlan p{};
   p.split = dtype == ATTNRES_F32;
   p.pack_weight = p.split || width % kDepth != 0;
@@ -1556,7 +1609,11 @@ LossPlan loss_plan(int64_t rows, int64_t vocab, int64_t width, int dtype, bool k
     p.dh = take(4 * p.parts * 16 * p.few_tiles * p.width_pad);
   } else {
     p.row_scale = take(4 * p.rows_pad);
-    p.alpha = take(16);
+    p.alpha = take(32);
+    if (pass != kBackwardOfTotal && dtype != ATTNRES_BF16) {
+      p.row_power = take(4 * p.rows_pad);
+      for (int k = 0; k < parts; ++k) p.weighed[k] = take(2 * p.rows_pad * p.width_pad);
+    }
     p.piece = std::min(p.vocab_pad, std::max<int64_t>(kPieceBytes / (2 * parts * p.rows_pad) / kTile, 1) * kTile);
     const int64_t pieces = (p.vocab_pad + p.piece - 1) / p.piece;
     p.piece = round_up((p.vocab_pad + pieces - 1) / pieces, kTile);
@@ -1612,33 +1669,50 @@ void prepare_operands(const Call& c, bool forward, Operand* h, Operand* w) {
   if constexpr (kSplit) {
     if (forward) {
       const unsigned grid_h = static_cast<unsigned>(std::min<int64_t>(c.rows, 1024));
-      hipLaunchKernelGGL(attnres_loss_amax_kernel, dim3(grid_h), dim3(kBlock), 0, c.stream, hidden, c.hidden_stride, c.rows,
-                         static_cast<int>(c.width), c.saved.index, &header->count, &header->amax[0]);
+      hipLaunchKernelGGL(attnres_loss_amax_kernel<float>, dim3(grid_h), dim3(kBlock), 0, c.stream, hidden, c.hidden_stride, c.rows,
+                         static_cast<int>(c.width), c.saved.index, &header->count, RowPowers{}, &header->amax[0]);
       const unsigned grid_w = static_cast<unsigned>(std::min<int64_t>(c.vocab, 2048));
-      hipLaunchKernelGGL(attnres_loss_amax_kernel, dim3(grid_w), dim3(kBlock), 0, c.stream, weight, c.weight_stride, c.vocab,
+      hipLaunchKernelGGL(attnres_loss_amax_kernel<float>, dim3(grid_w), dim3(kBlock), 0, c.stream, weight, c.weight_stride, c.vocab,
                          static_cast<int>(c.width), static_cast<const int32_t*>(nullptr), static_cast<const int32_t*>(nullptr),
-                         &header->amax[1]);
+                         RowPowers{}, &header->amax[1]);
     }
   }
   const bool pack = forward || !p.keep;
   uint16_t* packed[2] = {c.operand(p.hidden[0]), kSplit ? c.operand(p.hidden[1]) : nullptr};
   if (pack) {
-    hipLaunchKernelGGL((attnres_loss_pack_kernel<X>), dim3(stride_grid(p.rows_pad * p.width_pad / kVec)), dim3(kBlock), 0, c.stream,
+    hipLaunchKernelGGL((attnres_loss_pack_kernel<X, false>), dim3(stride_grid(p.rows_pad * p.width_pad / kVec)), dim3(kBlock), 0, c.stream,
                        hidden, c.hidden_stride, c.rows, static_cast<int>(c.width), c.saved.index, &header->count, p.rows_pad,
-                       static_cast<int>(p.width_pad), header, 0, forward, packed[0], packed[1]);
+                       static_cast<int>(p.width_pad), header, 0, forward, RowPowers{}, packed[0], packed[1]);
   }
   *h = {{packed[0], packed[1]}, p.width_pad, p.rows_pad, 0};
   if (p.pack_weight) {
     uint16_t* to[2] = {c.operand(p.weight[0]), kSplit ? c.operand(p.weight[1]) : nullptr};
     if (pack) {
-      hipLaunchKernelGGL((attnres_loss_pack_kernel<X>), dim3(stride_grid(c.vocab * p.width_pad / kVec)), dim3(kBlock), 0, c.stream,
+      hipLaunchKernelGGL((attnres_loss_pack_kernel<X, false>), dim3(stride_grid(c.vocab * p.width_pad / kVec)), dim3(kBlock), 0, c.stream,
                          weight, c.weight_stride, c.vocab, static_cast<int>(c.width), static_cast<const int32_t*>(nullptr),
-                         static_cast<const int32_t*>(nullptr), c.vocab, static_cast<int>(p.width_pad), header, 1, forward, to[0], to[1]);
+                         static_cast<const int32_t*>(nullptr), c.vocab, static_cast<int>(p.width_pad), header, 1, forward, RowPowers{}, to[0],
+                         to[1]);
     }
     *w = {{to[0], to[1]}, p.width_pad, c.vocab, 0};
   } else {
     *w = {{reinterpret_cast<const uint16_t*>(weight), nullptr}, c.weight_stride, c.vocab, 0};
   }
+}
+
+// H times its rows' powers, for dW.
+template <class X>
+Operand weigh_rows(const Call& c, const RowPowers& powers) {
+  const LossPlan& p = c.plan;
+  const X* hidden = static_cast<const X*>(c.hidden);
+  Header* header = c.saved.header;
+  hipLaunchKernelGGL((attnres_loss_amax_kernel<X>), dim3(static_cast<unsigned>(std::min<int64_t>(c.rows, 1024))), dim3(kBlock), 0,
+                     c.stream, hidden, c.hidden_stride, c.rows, static_cast<int>(c.width), c.saved.index, &header->count, powers,
+                     reinterpret_cast<uint32_t*>(powers.alpha + 2));
+  uint16_t* to[2] = {c.at<uint16_t>(p.weighed[0]), std::is_same_v<X, float> ? c.at<uint16_t>(p.weighed[1]) : nullptr};
+  hipLaunchKernelGGL((attnres_loss_pack_kernel<X, true>), dim3(stride_grid(p.rows_pad * p.width_pad / kVec)), dim3(kBlock), 0, c.stream,
+                     hidden, c.hidden_stride, c.rows, static_cast<int>(c.width), c.saved.index, &header->count, p.rows_pad,
+                     static_cast<int>(p.width_pad), header, 0, false, powers, to[0], to[1]);
+  return {{to[0], to[1]}, p.width_pad, p.rows_pad, 0};
 }
 
 // The logits of few rows; logits: where they are kept, or nullptr.  targets: nullptr in the backward, where
@@ -1747,8 +1821,16 @@ void loss_backward(const Call& c, int reduction, const float* grad_loss, void* g
   const float p_scale = std::is_same_v<T, Bf16> ? 1.0f : kProbabilityScale;
   float* alpha = c.at<float>(p.alpha);
   float* row_scale = c.at<float>(p.row_scale);
+  float* row_power = !std::is_same_v<T, Bf16> && reduction == ATTNRES_REDUCE_NONE ? c.at<float>(p.row_power) : nullptr;
   hipLaunchKernelGGL(attnres_loss_factors_kernel, dim3(1), dim3(kScanThreads), 0, c.stream, grad_loss, reduction, c.saved,
-                     p.rows_pad, p_scale, row_scale, alpha);
+                     p.rows_pad, p_scale, row_scale, row_power, alpha);
+  Operand rows = h;  // of dW
+  if constexpr (!std::is_same_v<T, Bf16>) {
+    if (row_power != nullptr && grad_weight != nullptr && c.rows > 0) {
+      // from alpha + 2 on: the factors that go with these rows, and what they are made from
+      rows = weigh_rows<X>(c, RowPowers{row_power, alpha + 2});
+    }
+  }
   const int32_t* count = &c.saved.header->count;
   const int tiles_d = static_cast<int>((c.width + kTile - 1) / kTile), tiles_n = static_cast<int>(p.rows_pad / kTile);
   Operand probability{{c.at<const uint16_t>(p.p[0]), kParts == 2 ? c.at<const uint16_t>(p.p[1]) : nullptr}, p.piece, 0, 0};
@@ -1783,7 +1865,7 @@ void loss_backward(const Call& c, int reduction, const float* grad_loss, void* g
       hipLaunchKernelGGL((attnres_loss_probability_kernel<T, SEGMENTS>), dim3(tiles_v * tiles_n), dim3(kThreads), 0, c.stream, g);
     }
     if (grad_weight != nullptr) {
-      Operand a = h, b = probability;
+      Operand a = rows, b = probability;
       a.entries = p.width_pad;
       a.depth = b.depth = p.rows_pad;
       b.entries = p.piece;
@@ -1806,7 +1888,8 @@ void loss_backward(const Call& c, int reduction, const float* grad_loss, void* g
         hipLaunchKernelGGL((attnres_loss_gradient_kernel<T, float, SEGMENTS, false>), grid, dim3(kThreads), 0, c.stream, e);
         hipLaunchKernelGGL((attnres_loss_join_kernel<X>), dim3(stride_grid(columns * ((c.width + kVec - 1) / kVec))), dim3(kBlock), 0,
                            c.stream, c.at<const float>(p.dw), p.splits_w, e.split_stride, p.width_pad,
-                           static_cast<const int32_t*>(nullptr), columns, static_cast<int>(c.width), alpha + 2, out);
+                           static_cast<const int32_t*>(nullptr), columns, static_cast<int>(c.width), alpha + 2,
+                           static_cast<const float*>(nullptr), out);
       }
     }
     if (grad_hidden != nullptr) {
@@ -1830,7 +1913,7 @@ void loss_backward(const Call& c, int reduction, const float* grad_loss, void* g
   if (grad_hidden != nullptr && c.rows > 0) {
     hipLaunchKernelGGL((attnres_loss_join_kernel<X>), dim3(stride_grid(c.rows * ((c.width + kVec - 1) / kVec))), dim3(kBlock), 0,
                        c.stream, c.at<const float>(p.dh), p.splits_h, p.rows_pad * p.width_pad, p.width_pad, c.saved.packed, c.rows,
-                       static_cast<int>(c.width), alpha, static_cast<X*>(grad_hidden));
+                       static_cast<int>(c.width), alpha, row_power, static_cast<X*>(grad_hidden));
   }
 }
 
@@ -1889,11 +1972,11 @@ using namespace attnres_hip::layers;
 extern "C" {
 
 int64_t attnres_hip_loss_saved_bytes(int64_t rows, int64_t vocab, int64_t width, int dtype, int keep) {
-  return known_shape(rows, vocab, width, dtype) ? loss_plan(rows, vocab, width, dtype, keep != 0, false).saved_bytes : -1;
+  return known_shape(rows, vocab, width, dtype) ? loss_plan(rows, vocab, width, dtype, keep != 0, kForward).saved_bytes : -1;
 }
 
 int64_t attnres_hip_loss_workspace_bytes(int64_t rows, int64_t vocab, int64_t width, int dtype, int keep, int backward) {
-  return known_shape(rows, vocab, width, dtype) ? loss_plan(rows, vocab, width, dtype, keep != 0, backward != 0).bytes : -1;
+  return known_shape(rows, vocab, width, dtype) ? loss_plan(rows, vocab, width, dtype, keep != 0, backward).bytes : -1;
 }
 
 int attnres_hip_loss_forward(const void* hidden, int64_t hidden_stride, const void* weight, int64_t weight_stride,
@@ -1905,7 +1988,7 @@ int attnres_hip_loss_forward(const void* hidden, int64_t hidden_stride, const vo
   if (loss == nullptr || saved == nullptr || (rows > 0 && targets == nullptr)) {
     return layer_error(ATTNRES_ERR_NULL_POINTER, "targets, loss or saved is NULL");
   }
-  const LossPlan plan = loss_plan(rows, vocab, width, dtype, keep != 0, false);
+  const LossPlan plan = loss_plan(rows, vocab, width, dtype, keep != 0, kForward);
   const Call c{hidden, hidden_stride, weight, weight_stride, rows, vocab, width, plan, saved_views(saved, rows, plan),
                static_cast<char*>(workspace), static_cast<hipStream_t>(stream)};
   if (const int status = check_places(saved, workspace, workspace_bytes, c.plan.bytes)) return status;
@@ -1921,7 +2004,8 @@ int attnres_hip_loss_backward(const void* hidden, int64_t hidden_stride, const v
                               int64_t workspace_bytes, void* stream) {
   if (const int status = check_loss(hidden, hidden_stride, weight, weight_stride, rows, vocab, width, dtype, reduction)) return status;
   if (saved == nullptr || grad_loss == nullptr) return layer_error(ATTNRES_ERR_NULL_POINTER, "saved or grad_loss is NULL");
-  const LossPlan plan = loss_plan(rows, vocab, width, dtype, keep != 0, true);
+  const LossPlan plan = loss_plan(rows, vocab, width, dtype, keep != 0,
+                                  reduction == ATTNRES_REDUCE_NONE ? kBackward : kBackwardOfTotal);
   const Call c{hidden, hidden_stride, weight, weight_stride, rows, vocab, width, plan,
                saved_views(const_cast<void*>(saved), rows, plan),  // read only
                static_cast<char*>(workspace), static_cast<hipStream_t>(stream)};

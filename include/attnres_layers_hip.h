@@ -87,8 +87,9 @@ int attnres_hip_embedding_backward(const void* grad_out, int out_dtype, const vo
  * saved: what the backward reads.  keep, the same in all calls: nonzero lets the forward keep the exponentials of the
  * logits there for the backward, 2 bytes each for BF16 (and 4 per row, the target's logit), else 4, rows and vocab padded
  * to 256, where that takes at most 8 GiB, and its packed operands (of few rows, up to 64, the FP32 logits); otherwise, and with 0, saved is 256 + 20 * rows bytes and the backward
- * forms them again, for one piece of the vocabulary at a time.  saved and
- * workspace start at multiples of 16 bytes (else ATTNRES_ERR_WORKSPACE). */
+ * forms them again, for one piece of the vocabulary at a time.
+ * workspace: backward 0 for the forward's, 1 for the backward's, 2 for that of a sum or a mean alone, which is smaller for F16 and
+ * F32.  saved and workspace start at multiples of 16 bytes (else ATTNRES_ERR_WORKSPACE). */
 int64_t attnres_hip_loss_saved_bytes(int64_t rows, int64_t vocab, int64_t width, int dtype, int keep);
 int64_t attnres_hip_loss_workspace_bytes(int64_t rows, int64_t vocab, int64_t width, int dtype, int keep, int backward);
 
