@@ -9,7 +9,8 @@ the last read into a loss.  No counterpart in the reference, whose model takes
 them from PyTorch (`benchmarks/model.py:180-355`).
 
 Sums, statistics and norms are FP32; results are rounded once.  First-order
-gradients; every result and gradient is the same bits from call to call (no
+reverse-mode gradients (differentiating them again raises, and so do inputs with a
+forward-mode tangent); every result and gradient is the same bits from call to call (no
 floating-point atomics).  In eager mode the calls go through C++ autograd nodes
 (`csrc/attnres_layers_autograd.cpp`), under ``torch.compile`` through the
 ``attnres_hip::`` ops below, which launch the same kernels.  Nothing

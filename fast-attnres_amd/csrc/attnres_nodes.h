@@ -6,6 +6,7 @@
 
 #include <torch/extension.h>
 
+#include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 
@@ -53,6 +54,18 @@ inline std::optional<int64_t> row_stride(const Tensor& tensor) {
     rows *= tensor.size(d);
   }
   return stride.value_or(0);
+}
+
+// Nothing here carries a forward-mode derivative: a launch refuses inputs that have a tangent instead of returning outputs
+// without one (a node's forward, within which forward mode is off, is refused by the node itself).  Where forward mode
+// is off (inference mode) tangents are dropped, as everywhere.
+inline void refuse_tangents(at::TensorList tensors, const char* what) {
+  for (const Tensor& tensor : tensors) {
+    if (tensor.defined() && tensor._fw_grad(/*level=*/0).defined() &&
+        c10::AutogradState::get_tls_state().get_fw_grad_mode()) {
+      TORCH_CHECK_NOT_IMPLEMENTED(false, what, " has no forward-mode derivative");
+    }
+  }
 }
 
 inline int64_t rows_of(const Tensor& tensor) { return tensor.dim() > 1 ? tensor.numel() / tensor.size(-1) : 1; }
