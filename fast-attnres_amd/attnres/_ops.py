@@ -59,6 +59,7 @@ from typing import Any
 
 import torch
 from torch import Tensor
+from torch.autograd import forward_ad
 
 from . import _native
 
@@ -172,6 +173,13 @@ def _stream(device: torch.device) -> int:
 _NO_SWITCH = contextlib.nullcontext()
 
 
+def _refuse_tangents(*tensors: Tensor) -> None:
+    """Raises for inputs with a forward-mode tangent, which a launch would drop
+    (as the C++ nodes' ``refuse_tangents``)."""
+    if torch._C._is_fwd_grad_enabled() and any(forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError("attnres has no forward-mode derivative")
+
+
 def _on_device(device: torch.device):
     """``torch.cuda.device(device)``, or nothing when it is the current device."""
     return _NO_SWITCH if device.index == torch.cuda.current_device() else torch.cuda.device(device)
@@ -245,6 +253,7 @@ def packed_forward_impl(values: Tensor, query: Tensor, eps: float, scale: float,
     """The packed forward launch; ``save`` chooses whether the refinement is
     stored (``out_refine`` ``[N, D]``) or not (``[0, D]``); ``pooled`` as for
     ``_saved_state``."""
+    _refuse_tangents(values, query)
     values = _unit_feature_stride(values)
     query = _contiguous(query)
     sources, tokens, width = (int(size) for size in values.shape)
@@ -318,6 +327,7 @@ def packed_backward_impl(values: Tensor, query: Tensor, out: Tensor, out_refine:
                          scale: float) -> tuple[Tensor, Tensor]:
     """The packed backward launch (dv rows and dq); an empty ``out_refine``
     means nothing was saved (delta from the value rows)."""
+    _refuse_tangents(grad_out)
     return _packed_backward_launch(values, query, out, grad_out,
                                    _state_addresses(out_refine, logit, inv_rms, stats), scale)
 
@@ -425,6 +435,7 @@ def sources_forward_impl(sources: list[Tensor], query: Tensor, eps: float, scale
                          save: bool, pooled: bool = False) -> tuple[Tensor, Tensor, Tensor, Tensor, Tensor]:
     """The source-list forward launch; ``save`` and ``pooled`` as for
     ``packed_forward_impl``."""
+    _refuse_tangents(query, *sources)
     first = sources[0]
     query = _contiguous(query)
     count, tokens, width = len(sources), _rows_of(first.shape), int(first.shape[-1])
@@ -499,6 +510,7 @@ def sources_backward_impl(sources: list[Tensor], query: Tensor, out: Tensor, out
                           grad_out: Tensor, logit: Tensor, inv_rms: Tensor, stats: Tensor,
                           scale: float) -> list[Tensor]:
     """The source-list backward launch: one dv buffer per list position, then dq."""
+    _refuse_tangents(grad_out)
     return _sources_backward_launch(sources, query, out, grad_out,
                                     _state_addresses(out_refine, logit, inv_rms, stats), scale)
 

@@ -46,7 +46,8 @@ import torch
 from torch import Tensor
 
 from . import _native
-from ._ops import _contiguous, _dq_workspace, _on_device, _source_table, _stream, sources_forward_impl
+from ._ops import (_contiguous, _dq_workspace, _on_device, _refuse_tangents, _source_table, _stream,
+                   sources_forward_impl)
 from ._sources import _EPS, _MAX_SOURCES, _MAX_WIDTH, check_query, check_sources
 
 _MAX_GATHER_READS = 48  # attnres_hip.h ATTNRES_MAX_GATHER_READS
@@ -88,6 +89,7 @@ class _SharedState:
                   logit: Tensor, inv_rms: Tensor, stats: Tensor, scale: float) -> Tensor:
         """One read's backward: dv into the shared buffers (written by the
         first read of this pass, accumulated by the others); returns dq."""
+        _refuse_tangents(grad_out)
         lib = _native.load()
         first = self.sources[0]
         count, width = len(self.sources), int(first.shape[-1])

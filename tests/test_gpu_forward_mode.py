@@ -6,9 +6,11 @@ import pytest
 import torch
 from torch.autograd import forward_ad
 
-from attnres import layers
+from attnres import SharedSources, SourceBank, attnres, layers
 
 pytestmark = pytest.mark.gpu
+
+BF16 = torch.bfloat16
 
 
 def _randn(*shape, dtype=torch.float32):
@@ -24,6 +26,21 @@ def _layer_calls():
         ("embedding", lambda t: layers.embedding(tokens, t["w"], t["p"]), {"w": _randn(5, 64), "p": _randn(4, 64)}),
         ("linear_cross_entropy", lambda t: layers.linear_cross_entropy(t["h"], t["w"], tokens[0]),
          {"h": _randn(4, 64), "w": _randn(5, 64)}),
+    ]
+
+
+def _read_calls():
+    def bank(tensors):
+        b = SourceBank(2)
+        b.push(tensors["s"]), b.push(tensors["s"] * 2)
+        return b.read(tensors["q"])
+
+    rows = {"s": _randn(3, 64, dtype=BF16), "q": _randn(64, dtype=BF16)}
+    return [
+        ("packed", lambda t: attnres(torch.stack((t["s"], t["s"])), t["q"]), rows),
+        ("list", lambda t: attnres([t["s"], t["s"]], t["q"]), rows),
+        ("shared", lambda t: SharedSources([t["s"], t["s"]]).read(t["q"]), rows),
+        ("bank", bank, rows),
     ]
 
 
@@ -58,9 +75,7 @@ def test_layers_refuse_tangents(index):
     _check(call, tensors)
 
 
-@pytest.mark.parametrize("index", range(3), ids=["layer_norm", "embedding", "linear_cross_entropy"])
-def test_compiled_layers_refuse_tangents(index):
-    _name, call, tensors = _layer_calls()[index]
+def _check_compiled(call, tensors):
     compiled = torch.compile(call, fullgraph=True, backend="aot_eager")
     expected = call(tensors)
     for name in tensors:
@@ -69,3 +84,19 @@ def test_compiled_layers_refuse_tangents(index):
             with pytest.raises(RuntimeError, match="forward|jvp"):
                 compiled(leaves)
     assert torch.equal(compiled(tensors), expected)
+
+
+@pytest.mark.parametrize("index", range(3), ids=["layer_norm", "embedding", "linear_cross_entropy"])
+def test_compiled_layers_refuse_tangents(index):
+    _check_compiled(*_layer_calls()[index][1:])
+
+
+@pytest.mark.parametrize("index", range(4), ids=["packed", "list", "shared", "bank"])
+def test_reads_refuse_tangents(index):
+    _name, call, tensors = _read_calls()[index]
+    _check(call, tensors)
+
+
+@pytest.mark.parametrize("index", range(2), ids=["packed", "list"])
+def test_compiled_reads_refuse_tangents(index):
+    _check_compiled(*_read_calls()[index][1:])
