@@ -17,11 +17,13 @@ namespace attnres_hip {
 namespace layers {
 namespace {
 
-// Launches take fewer than 2^32 threads: of 64 tokens per workgroup in the sums, of 8 rows of positions.
+// Launches take fewer than 2^32 threads, 2^24 workgroups: one for 64 tokens in the sums and in the joins, which share their
+// launch with the positions' workgroups.
 constexpr int64_t kMaxTokens = int64_t{1} << 29;
 constexpr int64_t kMaxPlaces = int64_t{1} << 26;
 constexpr int64_t kMaxVocab = int64_t{1} << 30;
 constexpr int64_t kMaxFwdBlocks = int64_t{1} << 23;
+constexpr int64_t kMaxPlaceBlocks = int64_t{1} << 22;
 
 __device__ __forceinline__ int64_t token_at(const void* tokens, int bytes, int64_t i) {
   return bytes == 8 ? static_cast<const int64_t*>(tokens)[i] : static_cast<const int32_t*>(tokens)[i];
@@ -493,20 +495,22 @@ __global__ void __launch_bounds__(kBlock) attnres_embedding_join_kernel(Runs r, 
                                                                         int join, Places<O, W> place) {
   __shared__ float sums[kJoinGroups][kJoinCols * kVec];
   if (static_cast<int>(blockIdx.x) < join) return join_runs(r, blockIdx.x, width, scale, grad_weight, sums);
-  const int64_t t = static_cast<int64_t>(blockIdx.x - join) * kJoinGroups + threadIdx.x / kJoinCols;
   const int c = (static_cast<int>(blockIdx.y) * kJoinCols + threadIdx.x % kJoinCols) * kVec;
-  if (t >= place.rows || c >= width) return;
-  float sum[kVec] = {};
-  if (t < place.length) {
+  if (c >= width) return;
+  const int64_t step = static_cast<int64_t>(gridDim.x - join) * kJoinGroups;
+  for (int64_t t = static_cast<int64_t>(blockIdx.x - join) * kJoinGroups + threadIdx.x / kJoinCols; t < place.rows; t += step) {
+    float sum[kVec] = {};
+    if (t < place.length) {
 #pragma unroll 4
-    for (int64_t b = 0; b < place.batch; ++b) {
-      float x[kVec];
-      load_chunk(place.grad_out + (b * place.length + t) * width, c, width, x);
+      for (int64_t b = 0; b < place.batch; ++b) {
+        float x[kVec];
+        load_chunk(place.grad_out + (b * place.length + t) * width, c, width, x);
 #pragma unroll
-      for (int e = 0; e < kVec; ++e) sum[e] += x[e];
+        for (int e = 0; e < kVec; ++e) sum[e] += x[e];
+      }
     }
+    store_chunk(place.grad_positions + t * width, c, width, sum);
   }
-  store_chunk(place.grad_positions + t * width, c, width, sum);
 }
 
 // ---------------------------------------------------------------------- host
@@ -607,7 +611,7 @@ void embedding_backward(const void* grad_out, const void* tokens, int token_byte
   }
   const Places<O, W> place{static_cast<const O*>(grad_out), batch, length, static_cast<W*>(grad_positions),
                            grad_positions != nullptr ? position_rows : 0};
-  const int64_t blocks = join + (place.rows + kJoinGroups - 1) / kJoinGroups;
+  const int64_t blocks = join + std::min((place.rows + kJoinGroups - 1) / kJoinGroups, kMaxPlaceBlocks);
   if (blocks > 0) {
     const unsigned columns = static_cast<unsigned>((width + kJoinCols * kVec - 1) / (kJoinCols * kVec));
     hipLaunchKernelGGL((attnres_embedding_join_kernel<O, W>), dim3(static_cast<unsigned>(blocks), columns), dim3(kBlock), 0, stream,
