@@ -104,6 +104,7 @@ LAYER_SIGNATURES = {
         _c_void_p, ctypes.c_int, _i64, _i64, _c_void_p, _i64, _i64, ctypes.c_int, _c_void_p, _f32, _c_void_p,
         ctypes.c_int, _c_void_p]),
     "attnres_hip_embedding_workspace_bytes": (_i64, [_i64, _i64, _i64, _i64]),
+    "attnres_hip_embedding_positions_workspace_bytes": (_i64, [_i64, _i64, _i64]),
     "attnres_hip_embedding_backward": (ctypes.c_int, [
         _c_void_p, ctypes.c_int, _c_void_p, ctypes.c_int, _i64, _i64, _i64, _i64, ctypes.c_int, _f32, _c_void_p,
         _c_void_p, _i64, _c_void_p, _i64, _c_void_p]),

@@ -481,13 +481,46 @@ __device__ __forceinline__ void join_runs(const Runs& r, int64_t piece, int widt
   store_chunk(grad_weight + static_cast<int64_t>(key) * width, c, width, sum);
 }
 
+// The positions' gradient, a sum over the batch for each of `length` rows.  A lane adds up 64 sequences and then these sums, as one
+// FP32 sum of a large batch loses what it counts (a million equal values: 1e-2 relative; ones end at 2^24).  Where the rows are too few for
+// the chip the batch goes in parts, whose sums (FP32) a second launch adds up in order: BF16, us, one part / parts, 512 sequences
+// of 128 at 1024 columns 166 / 31, 4096 of 16 at 256 1227 / 26, 65536 of 1 at 64 18600 / 68.
+struct PlacePlan {
+  int64_t share;  // sequences of a part
+  int parts;
+  int64_t bytes;
+};
+constexpr int64_t kInner = 64;
+constexpr int64_t kPlaceRows = 4096;  // of 256 columns, eight to a workgroup: two workgroups per CU
+
 template <class O, class W>
 struct Places {
   const O* grad_out;
   int64_t batch, length;
   W* grad_positions;
   int64_t rows;
+  PlacePlan plan;
+  float* partial;  // [parts][length][width]
 };
+
+// Sum of a row of the sequences first .. end-1.
+template <class O, class W>
+__device__ __forceinline__ void place_sum(const Places<O, W>& place, int64_t t, int64_t first, int64_t end, int c, int width,
+                                          float (&sum)[kVec]) {
+  for (int64_t b0 = first; b0 < end; b0 += kInner) {
+    float inner[kVec] = {};
+    const int64_t b1 = min(b0 + kInner, end);
+#pragma unroll 4
+    for (int64_t b = b0; b < b1; ++b) {
+      float x[kVec];
+      load_chunk(place.grad_out + (b * place.length + t) * width, c, width, x);
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) inner[e] += x[e];
+    }
+#pragma unroll
+    for (int e = 0; e < kVec; ++e) sum[e] += inner[e];
+  }
+}
 
 // Blocks 0 .. join-1 join a piece's run, the others sum the positions' gradient over the batch.
 template <class O, class W>
@@ -498,29 +531,73 @@ __global__ void __launch_bounds__(kBlock) attnres_embedding_join_kernel(Runs r, 
   const int c = (static_cast<int>(blockIdx.y) * kJoinCols + threadIdx.x % kJoinCols) * kVec;
   if (c >= width) return;
   const int64_t step = static_cast<int64_t>(gridDim.x - join) * kJoinGroups;
-  for (int64_t t = static_cast<int64_t>(blockIdx.x - join) * kJoinGroups + threadIdx.x / kJoinCols; t < place.rows; t += step) {
+  // parts times length rows of sums, then the rows past length
+  const int64_t sums_end = place.plan.parts * place.length, all = sums_end + place.rows - place.length;
+  for (int64_t r = static_cast<int64_t>(blockIdx.x - join) * kJoinGroups + threadIdx.x / kJoinCols; r < all; r += step) {
     float sum[kVec] = {};
-    if (t < place.length) {
-#pragma unroll 4
-      for (int64_t b = 0; b < place.batch; ++b) {
-        float x[kVec];
-        load_chunk(place.grad_out + (b * place.length + t) * width, c, width, x);
-#pragma unroll
-        for (int e = 0; e < kVec; ++e) sum[e] += x[e];
-      }
+    if (r >= sums_end) {
+      store_chunk(place.grad_positions + (place.length + r - sums_end) * width, c, width, sum);
+      continue;
     }
-    store_chunk(place.grad_positions + t * width, c, width, sum);
+    const int64_t part = r / place.length, t = r - part * place.length;
+    const int64_t first = part * place.plan.share;
+    place_sum(place, t, first, min(first + place.plan.share, place.batch), c, width, sum);
+    if (place.plan.parts == 1) {
+      store_chunk(place.grad_positions + t * width, c, width, sum);
+    } else {
+      store_chunk(place.partial + r * width, c, width, sum);
+    }
   }
 }
 
+// The parts' sums of one row: kJoinGroups groups that add up every kJoinGroups-th part, then the groups in order.
+template <class W>
+__global__ void __launch_bounds__(kBlock) attnres_embedding_places_kernel(const float* __restrict__ partial, int parts, int64_t length,
+                                                                          int width, W* __restrict__ grad_positions) {
+  __shared__ float sums[kJoinGroups][kJoinCols * kVec];
+  const int group = threadIdx.x / kJoinCols, member = threadIdx.x % kJoinCols;
+  const int64_t t = blockIdx.x;
+  const int c = (static_cast<int>(blockIdx.y) * kJoinCols + member) * kVec;
+  float sum[kVec] = {};
+#pragma unroll 4
+  for (int p = group; p < parts; p += kJoinGroups) {
+    float x[kVec];
+    load_chunk(partial + (p * length + t) * width, c, width, x);
+#pragma unroll
+    for (int e = 0; e < kVec; ++e) sum[e] += x[e];
+  }
+#pragma unroll
+  for (int e = 0; e < kVec; ++e) sums[group][member * kVec + e] = sum[e];
+  __syncthreads();
+  if (group > 0 || c >= width) return;
+  for (int g = 1; g < kJoinGroups; ++g) {
+#pragma unroll
+    for (int e = 0; e < kVec; ++e) sum[e] += sums[g][member * kVec + e];
+  }
+  store_chunk(grad_positions + t * width, c, width, sum);
+}
+
 // ---------------------------------------------------------------------- host
+
+PlacePlan place_plan(int64_t batch, int64_t length, int64_t width) {
+  const int64_t rows = length * ((width + kJoinCols * kVec - 1) / (kJoinCols * kVec));
+  const int64_t most = (batch + kInner - 1) / kInner;  // whole inner sums
+  const int64_t parts = rows > 0 ? std::max<int64_t>(std::min(kPlaceRows / rows, most), 1) : 1;
+  PlacePlan p{};
+  p.share = (batch + parts - 1) / parts;
+  p.parts = static_cast<int>(p.share > 0 ? (batch + p.share - 1) / p.share : 1);
+  p.bytes = p.parts > 1 ? (4 * p.parts * length * width + 255) / 256 * 256 : 0;
+  return p;
+}
 
 struct Plan {
   int tiles, bits, passes, piece;
   int64_t pieces, keys[2], values[2], counts, totals, partial, bytes;
 };
 
-Plan plan(int64_t n, int64_t vocab, int64_t width) {
+// The workspace: the positions' sums, then the table's part.
+Plan plan(int64_t batch, int64_t length, int64_t vocab, int64_t width) {
+  const int64_t n = batch * length;
   Plan p{};
   int bits = 1;
   while ((vocab >> bits) != 0) ++bits;  // keys 0 .. vocab
@@ -531,7 +608,7 @@ Plan plan(int64_t n, int64_t vocab, int64_t width) {
   p.piece = 8;
   while (p.piece < kMaxPiece && p.piece * 1024 < n) p.piece *= 2;
   p.pieces = (n + p.piece - 1) / p.piece;
-  int64_t at = 0;
+  int64_t at = place_plan(batch, length, width).bytes;
   const auto take = [&](int64_t bytes) {
     const int64_t from = at;
     at += (bytes + 255) / 256 * 256;
@@ -555,7 +632,7 @@ void embedding_backward(const void* grad_out, const void* tokens, int token_byte
   Runs runs{};
   int join = 0;
   if (grad_weight != nullptr) {
-    const Plan p = plan(n, vocab, width);
+    const Plan p = plan(batch, length, vocab, width);
     const int64_t elements = vocab * width;
     ZeroFill<W> zero{static_cast<W*>(grad_weight), 0, elements, elements * static_cast<int64_t>(sizeof(W)) >= kPastCaches};
     uint32_t* keys[2];
@@ -609,13 +686,23 @@ void embedding_backward(const void* grad_out, const void* tokens, int token_byte
                          static_cast<const O*>(grad_out), static_cast<int>(width), scale, static_cast<W*>(grad_weight), threads);
     }
   }
-  const Places<O, W> place{static_cast<const O*>(grad_out), batch, length, static_cast<W*>(grad_positions),
-                           grad_positions != nullptr ? position_rows : 0};
-  const int64_t blocks = join + std::min((place.rows + kJoinGroups - 1) / kJoinGroups, kMaxPlaceBlocks);
+  Places<O, W> place{static_cast<const O*>(grad_out), batch, length, static_cast<W*>(grad_positions), 0, {batch, 1, 0},
+                     reinterpret_cast<float*>(workspace)};
+  int64_t place_rows = 0;
+  if (grad_positions != nullptr) {
+    if (workspace != nullptr) place.plan = place_plan(batch, length, width);
+    place.rows = position_rows;
+    place_rows = place.plan.parts * length + position_rows - length;
+  }
+  const int64_t blocks = join + std::min((place_rows + kJoinGroups - 1) / kJoinGroups, kMaxPlaceBlocks);
   if (blocks > 0) {
     const unsigned columns = static_cast<unsigned>((width + kJoinCols * kVec - 1) / (kJoinCols * kVec));
     hipLaunchKernelGGL((attnres_embedding_join_kernel<O, W>), dim3(static_cast<unsigned>(blocks), columns), dim3(kBlock), 0, stream,
                        runs, static_cast<int>(width), scale, static_cast<W*>(grad_weight), join, place);
+    if (grad_positions != nullptr && place.plan.parts > 1) {
+      hipLaunchKernelGGL((attnres_embedding_places_kernel<W>), dim3(static_cast<unsigned>(length), columns), dim3(kBlock), 0, stream,
+                         place.partial, place.plan.parts, length, static_cast<int>(width), static_cast<W*>(grad_positions));
+    }
   }
 }
 
@@ -683,7 +770,12 @@ int64_t attnres_hip_embedding_workspace_bytes(int64_t batch, int64_t length, int
       width > ATTNRES_MAX_WIDTH) {
     return -1;
   }
-  return plan(batch * length, vocab, width).bytes;
+  return plan(batch, length, vocab, width).bytes;
+}
+
+int64_t attnres_hip_embedding_positions_workspace_bytes(int64_t batch, int64_t length, int64_t width) {
+  if (batch < 0 || length < 0 || (length > 0 && batch > kMaxTokens / length) || width < 1 || width > ATTNRES_MAX_WIDTH) return -1;
+  return place_plan(batch, length, width).bytes;
 }
 
 int attnres_hip_embedding_backward(const void* grad_out, int out_dtype, const void* tokens, int token_bytes, int64_t batch,
@@ -702,6 +794,10 @@ int attnres_hip_embedding_backward(const void* grad_out, int out_dtype, const vo
   if (grad_weight != nullptr && need > 0 && (workspace == nullptr || workspace_bytes < need)) {
     return layer_error(ATTNRES_ERR_WORKSPACE, "workspace of %lld bytes, %lld needed", (long long)workspace_bytes,
                        (long long)need);
+  }
+  if (grad_weight == nullptr && workspace != nullptr &&
+      workspace_bytes < attnres_hip_embedding_positions_workspace_bytes(batch, length, width)) {
+    workspace = nullptr;  // as without one
   }
   with_types(weight_dtype, out_dtype, [&](auto w, auto o) {
     embedding_backward<decltype(o), decltype(w)>(grad_out, tokens, token_bytes, batch, length, vocab, width, scale,

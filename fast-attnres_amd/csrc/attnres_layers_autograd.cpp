@@ -186,8 +186,9 @@ std::tuple<Tensor, Tensor> embedding_backward(const Tensor& grad_out, const Tens
   Tensor grad_weight = torch::empty({want_weight ? vocab : 0, width}, options);
   Tensor grad_positions = torch::empty({want_positions ? position_rows : 0, width}, options);
   Tensor workspace;
-  if (want_weight) {
-    const int64_t bytes = attnres_hip_embedding_workspace_bytes(batch, length, vocab, width);
+  if (want_weight || want_positions) {
+    const int64_t bytes = want_weight ? attnres_hip_embedding_workspace_bytes(batch, length, vocab, width)
+                                      : attnres_hip_embedding_positions_workspace_bytes(batch, length, width);
     TORCH_CHECK_VALUE(bytes >= 0, "embedding backward: shape outside the supported envelope");
     workspace = torch::empty({bytes}, grad.options().dtype(torch::kUInt8));
   }

@@ -62,13 +62,15 @@ int attnres_hip_embedding_forward(const void* tokens, int token_bytes, int64_t b
                                   const void* weight, int64_t vocab, int64_t width, int weight_dtype,
                                   const void* positions, float scale, void* out, int out_dtype, void* stream);
 
-/* Bytes of the backward's workspace (-1: outside the envelope). */
+/* Bytes of the backward's workspace (-1: outside the envelope), and of grad_positions alone (0: none needed). */
 int64_t attnres_hip_embedding_workspace_bytes(int64_t batch, int64_t length, int64_t vocab, int64_t width);
+int64_t attnres_hip_embedding_positions_workspace_bytes(int64_t batch, int64_t length, int64_t width);
 
 /* Gradients: grad_weight [vocab, width] (every row written: zeros where no token
  * points) and grad_positions [position_rows, width] (zeros past length), of
  * weight_dtype; either may be NULL.  grad_out [batch, length, width] contiguous, of
- * out_dtype.  Rows are summed in FP32 in the order of the tokens. */
+ * out_dtype.  Rows are summed in FP32 in the order of the tokens.  Without grad_weight a workspace that is NULL or too small
+ * is not used, and the sums over a large batch of few positions are not shared out (slower, other roundings). */
 int attnres_hip_embedding_backward(const void* grad_out, int out_dtype, const void* tokens, int token_bytes,
                                    int64_t batch, int64_t length, int64_t vocab, int64_t width, int weight_dtype,
                                    float scale, void* grad_weight, void* grad_positions, int64_t position_rows,
