@@ -145,7 +145,7 @@ struct Loader {
 // have landed is waited for in landed().  The address registers are read when the load is issued, and
 // nothing comes back in registers.
 __device__ __forceinline__ void load_lds(const char* base, uint32_t at, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(lds), "v"(at), "s"(base));
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(lds), "v"(at), "s"(base) : "m0");
 }
 
 // The LDS byte of a pointer into LDS.
