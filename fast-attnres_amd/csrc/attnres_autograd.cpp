@@ -151,7 +151,7 @@ struct PackedRead : public torch::autograd::Function<PackedRead> {
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     if (!grads[0].defined()) return {Tensor(), Tensor(), Tensor(), Tensor()};
-    refuse_tangents({grads[0]}, "attnres's backward");
+    refuse_tangents("attnres's backward", grads[0]);
     const variable_list saved = ctx->get_saved_variables();
     const Tensor& rows = saved[0];  // [S, N, D]
     const Tensor& query = saved[1];
@@ -213,7 +213,7 @@ struct SourcesRead : public torch::autograd::Function<SourcesRead> {
     const int64_t S = ctx->saved_data["count"].toInt();
     variable_list result(3 + S);  // query, eps, scale, then one per source
     if (!grads[0].defined()) return result;
-    refuse_tangents({grads[0]}, "attnres's backward");
+    refuse_tangents("attnres's backward", grads[0]);
     const variable_list saved = ctx->get_saved_variables();
     const std::vector<Tensor> sources(saved.begin(), saved.begin() + S);
     const Tensor& query = saved[S];
@@ -303,14 +303,13 @@ Tensor sources_forward_only(const Tensor& query, double eps, double scale, at::T
 }
 
 Tensor packed_read(const Tensor& values, const Tensor& query, double eps, double scale) {
-  refuse_tangents({values, query}, "attnres");
+  refuse_tangents("attnres", values, query);
   if (!needs_grad(query, values)) return packed_forward_only(values, query, eps, scale);
   return PackedRead::apply(values, query, eps, scale);
 }
 
 Tensor sources_read(const Tensor& query, double eps, double scale, const std::vector<Tensor>& sources) {
-  refuse_tangents(sources, "attnres");
-  refuse_tangents({query}, "attnres");
+  refuse_tangents("attnres", query, sources);
   if (!needs_grad(query, sources)) return sources_forward_only(query, eps, scale, sources);
   return SourcesRead::apply(query, eps, scale, at::TensorList(sources));
 }
@@ -616,7 +615,7 @@ struct BankPushSum : public torch::autograd::Function<BankPushSum> {
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
-    refuse_tangents({grads[0]}, "SourceBank.push_sum's backward");
+    refuse_tangents("SourceBank.push_sum's backward", grads[0]);
     const auto bank = bank_of(ctx);
     const auto dtype = static_cast<at::ScalarType>(ctx->saved_data["dtype"].toInt());
     Tensor grad = bank->take(ctx->saved_data["slot"].toInt(), dtype);
@@ -657,7 +656,7 @@ struct BankRead : public torch::autograd::Function<BankRead> {
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     variable_list result(7);  // bank, count, tail, query, eps, scale, token
-    refuse_tangents({grads[0]}, "SourceBank.read's backward");
+    refuse_tangents("SourceBank.read's backward", grads[0]);
     const auto bank = bank_of(ctx);
     const Slots slots{ctx->saved_data["count"].toInt(), ctx->saved_data["tail"].toInt()};
     const float scale = static_cast<float>(ctx->saved_data["scale"].toDouble());
@@ -758,7 +757,7 @@ std::tuple<Tensor, Tensor> bank_push_sum(const c10::intrusive_ptr<BankState>& ba
 // through the token -- require one): the forward alone, nothing saved.
 Tensor bank_read(const c10::intrusive_ptr<BankState>& bank, int64_t count, int64_t tail, const Tensor& query,
                  double eps, double scale, const Tensor& token) {
-  refuse_tangents({query}, "SourceBank.read");
+  refuse_tangents("SourceBank.read", query);
   if (at::GradMode::is_enabled() && (query.requires_grad() || token.requires_grad())) {
     return BankRead::apply(bank, count, tail, query, eps, scale, token);
   }

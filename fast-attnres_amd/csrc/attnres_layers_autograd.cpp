@@ -70,7 +70,7 @@ variable_list once_differentiable(variable_list grads) {
 
 std::tuple<Tensor, Tensor> layer_norm_forward(const Tensor& x, const OptionalTensor& weight, const OptionalTensor& bias,
                                               double eps, bool save) {
-  refuse_tangents({x, value_of(weight), value_of(bias)}, "layer_norm");
+  refuse_tangents("layer_norm", x, weight, bias);
   const c10::DeviceGuard guard(x.device());
   const Rows rows = rows_view(x);
   const int64_t width = x.size(-1), count = x.numel() / width;
@@ -89,7 +89,7 @@ std::tuple<Tensor, Tensor> layer_norm_forward(const Tensor& x, const OptionalTen
 std::tuple<Tensor, Tensor, Tensor> layer_norm_backward(const Tensor& grad_out, const Tensor& x, const OptionalTensor& weight,
                                                        at::ScalarType param, const Tensor& stats, bool want_x, bool want_weight,
                                                        bool want_bias) {
-  refuse_tangents({grad_out, x, value_of(weight)}, "layer_norm's backward");
+  refuse_tangents("layer_norm's backward", grad_out, x, weight);
   const c10::DeviceGuard guard(x.device());
   const Rows rows = rows_view(x);
   const int64_t width = x.size(-1), count = x.numel() / width;
@@ -160,7 +160,7 @@ int64_t batch_of(const Tensor& tokens) {
 
 Tensor embedding_forward(const Tensor& tokens, const Tensor& weight, const OptionalTensor& positions, double scale,
                          at::ScalarType dtype) {
-  refuse_tangents({weight, value_of(positions)}, "embedding");
+  refuse_tangents("embedding", weight, positions);
   const c10::DeviceGuard guard(weight.device());
   const Tensor ids = tokens.contiguous(), table = weight.contiguous();
   const Tensor places = positions ? positions->contiguous() : Tensor();
@@ -178,7 +178,7 @@ Tensor embedding_forward(const Tensor& tokens, const Tensor& weight, const Optio
 // position_rows: of the positions' gradient; gradients that are not wanted come back empty.
 std::tuple<Tensor, Tensor> embedding_backward(const Tensor& grad_out, const Tensor& tokens, int64_t vocab, int64_t position_rows,
                                               at::ScalarType table, double scale, bool want_weight, bool want_positions) {
-  refuse_tangents({grad_out}, "embedding's backward");
+  refuse_tangents("embedding's backward", grad_out);
   const c10::DeviceGuard guard(grad_out.device());
   const Tensor grad = grad_out.contiguous(), ids = tokens.contiguous();
   const int64_t width = grad.size(-1), batch = batch_of(ids), length = length_of(ids);
@@ -264,7 +264,7 @@ Tensor loss_workspace(const Tensor& hidden, const Tensor& weight, int64_t rows, 
 // (loss, saved): the loss has the targets' shape for ATTNRES_REDUCE_NONE, else none.
 std::tuple<Tensor, Tensor> loss_forward(const Tensor& hidden, const Tensor& weight, const Tensor& targets, int64_t ignore_index,
                                         int64_t reduction, bool keep) {
-  refuse_tangents({hidden, weight}, "linear_cross_entropy");
+  refuse_tangents("linear_cross_entropy", hidden, weight);
   const c10::DeviceGuard guard(hidden.device());
   const at::NoGradGuard no_grad;
   const Rows h = rows_view(hidden), w = weight_rows(weight);
@@ -288,7 +288,7 @@ std::tuple<Tensor, Tensor> loss_forward(const Tensor& hidden, const Tensor& weig
 
 std::tuple<Tensor, Tensor> loss_backward(const Tensor& grad_loss, const Tensor& hidden, const Tensor& weight, const Tensor& saved,
                                          int64_t reduction, bool keep, bool want_hidden, bool want_weight) {
-  refuse_tangents({grad_loss, hidden, weight}, "linear_cross_entropy's backward");
+  refuse_tangents("linear_cross_entropy's backward", grad_loss, hidden, weight);
   const c10::DeviceGuard guard(hidden.device());
   const at::NoGradGuard no_grad;
   const Rows h = rows_view(hidden), w = weight_rows(weight);

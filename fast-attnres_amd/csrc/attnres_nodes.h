@@ -11,6 +11,7 @@
 #include <c10/hip/HIPStream.h>
 
 #include <optional>
+#include <vector>
 
 #include "attnres_hip.h"
 
@@ -59,13 +60,18 @@ inline std::optional<int64_t> row_stride(const Tensor& tensor) {
 // Nothing here carries a forward-mode derivative: a launch refuses inputs that have a tangent instead of returning outputs
 // without one (a node's forward, within which forward mode is off, is refused by the node itself).  Where forward mode
 // is off (inference mode) tangents are dropped, as everywhere.
-inline void refuse_tangents(at::TensorList tensors, const char* what) {
+inline bool has_tangent(const Tensor& tensor) { return tensor.defined() && tensor._fw_grad(/*level=*/0).defined(); }
+inline bool has_tangent(const std::optional<Tensor>& tensor) { return tensor && has_tangent(*tensor); }
+inline bool has_tangent(const std::vector<Tensor>& tensors) {
   for (const Tensor& tensor : tensors) {
-    if (tensor.defined() && tensor._fw_grad(/*level=*/0).defined() &&
-        c10::AutogradState::get_tls_state().get_fw_grad_mode()) {
-      TORCH_CHECK_NOT_IMPLEMENTED(false, what, " has no forward-mode derivative");
-    }
+    if (has_tangent(tensor)) return true;
   }
+  return false;
+}
+template <class... T>
+void refuse_tangents(const char* what, const T&... tensors) {
+  if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
+  TORCH_CHECK_NOT_IMPLEMENTED(!(has_tangent(tensors) || ...), what, " has no forward-mode derivative");
 }
 
 inline int64_t rows_of(const Tensor& tensor) { return tensor.dim() > 1 ? tensor.numel() / tensor.size(-1) : 1; }
