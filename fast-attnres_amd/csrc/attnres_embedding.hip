@@ -481,17 +481,8 @@ __device__ __forceinline__ void join_runs(const Runs& r, int64_t piece, int widt
   store_chunk(grad_weight + static_cast<int64_t>(key) * width, c, width, sum);
 }
 
-// The positions' gradient, a sum over the batch for each of `length` rows.  A lane adds up 64 sequences and then these sums, as one
-// FP32 sum of a large batch loses what it counts (a million equal values: 1e-2 relative; ones end at 2^24).  Where the rows are too few for
-// the chip the batch goes in parts, whose sums (FP32) a second launch adds up in order: BF16, us, one part / parts, 512 sequences
-// of 128 at 1024 columns 166 / 31, 4096 of 16 at 256 1227 / 26, 65536 of 1 at 64 18600 / 68.
-struct PlacePlan {
-  int64_t share;  // sequences of a part
-  int parts;
-  int64_t bytes;
-};
+// The positions' gradient is a sum over the batch for each of `length` rows: up to kInner sequences, beside the joins.
 constexpr int64_t kInner = 64;
-constexpr int64_t kPlaceRows = 4096;  // of 256 columns, eight to a workgroup: two workgroups per CU
 
 template <class O, class W>
 struct Places {
@@ -499,28 +490,7 @@ struct Places {
   int64_t batch, length;
   W* grad_positions;
   int64_t rows;
-  PlacePlan plan;
-  float* partial;  // [parts][length][width]
 };
-
-// Sum of a row of the sequences first .. end-1.
-template <class O, class W>
-__device__ __forceinline__ void place_sum(const Places<O, W>& place, int64_t t, int64_t first, int64_t end, int c, int width,
-                                          float (&sum)[kVec]) {
-  for (int64_t b0 = first; b0 < end; b0 += kInner) {
-    float inner[kVec] = {};
-    const int64_t b1 = min(b0 + kInner, end);
-#pragma unroll 4
-    for (int64_t b = b0; b < b1; ++b) {
-      float x[kVec];
-      load_chunk(place.grad_out + (b * place.length + t) * width, c, width, x);
-#pragma unroll
-      for (int e = 0; e < kVec; ++e) inner[e] += x[e];
-    }
-#pragma unroll
-    for (int e = 0; e < kVec; ++e) sum[e] += inner[e];
-  }
-}
 
 // Blocks 0 .. join-1 join a piece's run, the others sum the positions' gradient over the batch.
 template <class O, class W>
@@ -531,21 +501,65 @@ __global__ void __launch_bounds__(kBlock) attnres_embedding_join_kernel(Runs r, 
   const int c = (static_cast<int>(blockIdx.y) * kJoinCols + threadIdx.x % kJoinCols) * kVec;
   if (c >= width) return;
   const int64_t step = static_cast<int64_t>(gridDim.x - join) * kJoinGroups;
+  for (int64_t t = static_cast<int64_t>(blockIdx.x - join) * kJoinGroups + threadIdx.x / kJoinCols; t < place.rows; t += step) {
+    float sum[kVec] = {};
+    if (t < place.length) {
+#pragma unroll 4
+      for (int64_t b = 0; b < place.batch; ++b) {
+        float x[kVec];
+        load_chunk(place.grad_out + (b * place.length + t) * width, c, width, x);
+#pragma unroll
+        for (int e = 0; e < kVec; ++e) sum[e] += x[e];
+      }
+    }
+    store_chunk(place.grad_positions + t * width, c, width, sum);
+  }
+}
+
+// Larger batches: a lane adds up kInner sequences and then these sums, as one FP32 sum of a large batch loses what it counts (a
+// million equal values: 1e-2 relative; ones end at 2^24).  Where the rows are too few for the chip the batch goes in parts, whose sums
+// (FP32) a second launch adds up in order: BF16, us, one sum / parts, 512 sequences of 128 at 1024 columns 166 / 31, 4096 of
+// 16 at 256 1227 / 26, 65536 of 1 at 64 18600 / 68.  A launch of its own, for the registers of the joins.
+struct PlacePlan {
+  int64_t share;  // sequences of a part
+  int parts;
+  int64_t bytes;
+};
+constexpr int64_t kPlaceRows = 4096;  // of 256 columns, eight to a workgroup: two workgroups per CU
+
+template <class O, class W>
+__global__ void __launch_bounds__(kBlock) attnres_embedding_batch_kernel(Places<O, W> place, PlacePlan plan, int width,
+                                                                         float* __restrict__ partial) {
+  const int c = (static_cast<int>(blockIdx.y) * kJoinCols + threadIdx.x % kJoinCols) * kVec;
+  if (c >= width) return;
   // parts times length rows of sums, then the rows past length
-  const int64_t sums_end = place.plan.parts * place.length, all = sums_end + place.rows - place.length;
-  for (int64_t r = static_cast<int64_t>(blockIdx.x - join) * kJoinGroups + threadIdx.x / kJoinCols; r < all; r += step) {
+  const int64_t sums_end = plan.parts * place.length, all = sums_end + place.rows - place.length;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * kJoinGroups;
+  for (int64_t r = static_cast<int64_t>(blockIdx.x) * kJoinGroups + threadIdx.x / kJoinCols; r < all; r += step) {
     float sum[kVec] = {};
     if (r >= sums_end) {
       store_chunk(place.grad_positions + (place.length + r - sums_end) * width, c, width, sum);
       continue;
     }
-    const int64_t part = r / place.length, t = r - part * place.length;
-    const int64_t first = part * place.plan.share;
-    place_sum(place, t, first, min(first + place.plan.share, place.batch), c, width, sum);
-    if (place.plan.parts == 1) {
+    const int64_t part = plan.parts == 1 ? 0 : r / place.length, t = r - part * place.length;
+    const int64_t first = part * plan.share, end = min(first + plan.share, place.batch);
+    for (int64_t b0 = first; b0 < end; b0 += kInner) {
+      float inner[kVec] = {};
+      const int64_t b1 = min(b0 + kInner, end);
+#pragma unroll 4
+      for (int64_t b = b0; b < b1; ++b) {
+        float x[kVec];
+        load_chunk(place.grad_out + (b * place.length + t) * width, c, width, x);
+#pragma unroll
+        for (int e = 0; e < kVec; ++e) inner[e] += x[e];
+      }
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) sum[e] += inner[e];
+    }
+    if (plan.parts == 1) {
       store_chunk(place.grad_positions + t * width, c, width, sum);
     } else {
-      store_chunk(place.partial + r * width, c, width, sum);
+      store_chunk(partial + r * width, c, width, sum);
     }
   }
 }
@@ -686,22 +700,25 @@ void embedding_backward(const void* grad_out, const void* tokens, int token_byte
                          static_cast<const O*>(grad_out), static_cast<int>(width), scale, static_cast<W*>(grad_weight), threads);
     }
   }
-  Places<O, W> place{static_cast<const O*>(grad_out), batch, length, static_cast<W*>(grad_positions), 0, {batch, 1, 0},
-                     reinterpret_cast<float*>(workspace)};
-  int64_t place_rows = 0;
-  if (grad_positions != nullptr) {
-    if (workspace != nullptr) place.plan = place_plan(batch, length, width);
-    place.rows = position_rows;
-    place_rows = place.plan.parts * length + position_rows - length;
-  }
-  const int64_t blocks = join + std::min((place_rows + kJoinGroups - 1) / kJoinGroups, kMaxPlaceBlocks);
+  const Places<O, W> place{static_cast<const O*>(grad_out), batch, length, static_cast<W*>(grad_positions),
+                           grad_positions != nullptr ? position_rows : 0};
+  const bool large = place.rows > 0 && batch > kInner;
+  const unsigned columns = static_cast<unsigned>((width + kJoinCols * kVec - 1) / (kJoinCols * kVec));
+  const auto blocks_of = [](int64_t rows) { return std::min((rows + kJoinGroups - 1) / kJoinGroups, kMaxPlaceBlocks); };
+  const int64_t blocks = join + (large ? 0 : blocks_of(place.rows));
   if (blocks > 0) {
-    const unsigned columns = static_cast<unsigned>((width + kJoinCols * kVec - 1) / (kJoinCols * kVec));
     hipLaunchKernelGGL((attnres_embedding_join_kernel<O, W>), dim3(static_cast<unsigned>(blocks), columns), dim3(kBlock), 0, stream,
                        runs, static_cast<int>(width), scale, static_cast<W*>(grad_weight), join, place);
-    if (grad_positions != nullptr && place.plan.parts > 1) {
+  }
+  if (large) {
+    const PlacePlan p = workspace != nullptr ? place_plan(batch, length, width) : PlacePlan{batch, 1, 0};
+    float* partial = reinterpret_cast<float*>(workspace);
+    hipLaunchKernelGGL((attnres_embedding_batch_kernel<O, W>),
+                       dim3(static_cast<unsigned>(blocks_of(p.parts * length + position_rows - length)), columns), dim3(kBlock), 0, stream,
+                       place, p, static_cast<int>(width), partial);
+    if (p.parts > 1) {
       hipLaunchKernelGGL((attnres_embedding_places_kernel<W>), dim3(static_cast<unsigned>(length), columns), dim3(kBlock), 0, stream,
-                         place.partial, place.plan.parts, length, static_cast<int>(width), static_cast<W*>(grad_positions));
+                         partial, p.parts, length, static_cast<int>(width), static_cast<W*>(grad_positions));
     }
   }
 }
