@@ -5,7 +5,7 @@ from __future__ import annotations
 import pytest
 import torch
 
-from attnres import layers
+from attnres import _native, layers
 from layer_reference import U32, assert_within
 
 pytestmark = pytest.mark.gpu
@@ -38,6 +38,25 @@ def test_sums_over_large_batches(batch, length, width, want_table):
     assert_within("dpos", got[0], expected, 512 * U32 * size)
     again = _positions_gradient(tokens, length + 3, width, grad, FP32, want_table=want_table)
     assert all(torch.equal(a, b) for a, b in zip(got, again))
+
+
+@pytest.mark.parametrize("batch,length,width", [(65536, 1, 64), (3000, 6, 300), (65, 5, 24)])
+def test_sums_through_the_c_abi_with_and_without_a_workspace(batch, length, width):
+    """Without one the blocks of 64 are added up in one sum: batch / 64 + 64 roundings in a row."""
+    lib = _native.load()
+    g = torch.Generator(device="cuda").manual_seed(batch)
+    grad = torch.rand(batch, length, width, generator=g, device="cuda")
+    tokens = torch.zeros(batch, length, device="cuda", dtype=torch.int64)
+    size = lib.attnres_hip_embedding_positions_workspace_bytes(batch, length, width)
+    workspace = torch.empty(size, device="cuda", dtype=torch.uint8)
+    expected = torch.zeros(length + 2, width, device="cuda", dtype=torch.float64)
+    expected[:length] = grad.double().sum(0)
+    for pointer, bytes in ((None, 0), (workspace.data_ptr(), size), (workspace.data_ptr(), max(size - 1, 0))):
+        out = torch.full((length + 2, width), 7.0, device="cuda")
+        status = lib.attnres_hip_embedding_backward(grad.data_ptr(), 2, tokens.data_ptr(), 8, batch, length, 10, width, 2, 1.0, None,
+                                                    out.data_ptr(), length + 2, pointer, bytes, torch.cuda.current_stream().cuda_stream)
+        assert status == 0, lib.attnres_hip_last_error().decode()
+        assert_within("dpos", out, expected, (batch / 64 + 64) * U32 * expected)
 
 
 def test_a_batch_beyond_what_an_accumulator_counts():

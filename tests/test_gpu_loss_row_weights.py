@@ -69,6 +69,29 @@ def test_a_row_is_the_same_beside_a_large_weight(dtype):
         assert torch.equal(beside[17], alone[17] * 2.0**40) and torch.equal(beside[90], alone[90] * 2.0**-30)
 
 
+@pytest.mark.parametrize("dtype", [FP16, FP32])
+def test_weighted_rows_captured_and_replayed(dtype):
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        _, hidden, weight, targets = _inputs(9, 150, 64, 300, dtype)
+        upstream = torch.ones(150, device="cuda")
+        for _ in range(2):
+            _weighted(hidden, weight, targets, upstream, False)
+    stream.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        outputs = _weighted(hidden, weight, targets, upstream, False)
+    for seed in range(3):
+        g = torch.Generator(device="cuda").manual_seed(seed)
+        upstream.copy_(10.0**(-6 * torch.rand(150, generator=g, device="cuda")))
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in outputs]
+        assert all(torch.equal(a, b) for a, b in zip(got, _weighted(hidden, weight, targets, upstream, False)))
+        torch.cuda.synchronize()
+
+
 @pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
 @pytest.mark.parametrize("recompute", [False, True])
 def test_rows_of_no_weight_and_of_a_nonfinite_one(dtype, recompute):
