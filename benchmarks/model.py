@@ -35,7 +35,8 @@ completed slot.
 around the reads from ``attnres.layers``: the token and position lookup in one
 kernel with its gradient by sorted tokens, the layer norms, and the LM head
 with the cross entropy (``CausalAttnResLM.loss``, which ``training_step``
-calls), which never stores the logits.  The weights are the same parameters.
+calls), which forms the logits tile by tile and keeps their exponentials for
+the backward, 2 or 4 bytes each.  The weights are the same parameters.
 """
 
 from __future__ import annotations
@@ -298,7 +299,7 @@ class CausalAttnResLM(nn.Module):
 
     def loss(self, tokens: Tensor, targets: Tensor) -> Tensor:
         """Mean cross entropy of the targets (those equal to -100 left out); with ``fused_layers``
-        without storing the logits."""
+        without a tensor of the logits in FP32 (see ``linear_cross_entropy`` for what it keeps)."""
         if not self.fused_layers:
             logits = self(tokens)
             return F.cross_entropy(logits.reshape(-1, logits.shape[-1]).float(), targets.reshape(-1))

@@ -260,15 +260,22 @@ def linear_cross_entropy(hidden: Tensor, weight: Tensor, targets: Tensor, *, ign
     their hidden states are not looked at.  A target that is neither
     ``ignore_index`` nor in ``0..V-1`` makes the loss and the gradients NaN.
 
-    16-bit inputs are multiplied on the matrix cores as they are, FP32 ones to FP32's
-    accuracy as pairs of FP16 numbers (relative to the largest magnitude of the tensor,
-    so a tensor whose values span more than 2^25 loses the smallest, and infinities
-    count as NaN).  Upstream gradients of ``reduction="none"`` may differ by any factor: a row
-    of ``hidden``'s gradient is as accurate as if it were alone; what it adds to that of ``weight`` is
-    held, for FP16 and FP32, to 2^-39 of the largest row of ``hidden`` times its upstream gradient.  Gradients flow to ``hidden`` and ``weight``.  For them the forward
-    keeps the logits' exponentials (BF16 inputs: FP16 relative to the largest of 128, 2
-    bytes per target and word, the target's own unrounded; else FP32, 4 bytes), where that is at most 8 GiB, and the
-    operands it has packed; beyond that, or with ``recompute=True``, it keeps 20 bytes
+    16-bit inputs are multiplied on the matrix cores as they are, FP32 ones as pairs of
+    FP16 numbers relative to the largest magnitude of the tensor: with FP32's 24 bits for values
+    down to 2^-16 of it and, as the pairs end at 2^-40, a bit less for every further
+    power of two (15 bits at 2^-25); infinities count as NaN.  (Up to 64 targets FP32 inputs
+    are multiplied as they are.)
+
+    Gradients flow to ``hidden`` and ``weight``.  Upstream gradients of
+    ``reduction="none"`` may differ by any factor: a row of ``hidden``'s gradient is as accurate
+    as if it were alone; what it adds to ``weight``'s is held, for FP16 and FP32, to 2^-39 of the
+    largest row of ``hidden`` times its upstream gradient.  The probabilities are rounded to the type of
+    16-bit inputs for the gradients' products.
+
+    For the gradients the forward keeps the logits' exponentials (BF16 inputs: FP16
+    relative to the largest of 128, 2 bytes per target and word, the target's own unrounded;
+    else FP32, 4 bytes), where that is at most 8 GiB, and the operands it has packed, in every
+    live graph; beyond that, or with ``recompute=True``, it keeps 20 bytes
     per target, and the backward forms them again, for one piece of the vocabulary at a
     time, which adds a third to its products.
     """

@@ -4,10 +4,10 @@
 //   P[n, v] = g_n (exp(l[n, v] - lse_n) - [v = t_n]),  dH = P W,  dW = P^T H
 //
 // Bound by the matrix cores: three products of 2 N V D operations (the logits and two gradient products) against
-// O(V D + N D) bytes.  The logits are never stored as they are.  The forward reduces them, per row and 128 columns, to a
+// O(V D + N D) bytes.  The forward reduces the logits, per row and 128 columns, to a
 // reference and a sum of powers above it, and keeps the powers for the backward (2 or 4 bytes each, up to
-// kKeepBytes), which makes P of them in one pass, for one piece of the vocabulary at a time.  Without kept
-// powers the backward multiplies again, four products in all.  Forward and backward, kept / again: 16384 x 131072 x 2048 BF16
+// kKeepBytes; of few rows the FP32 logits themselves), which makes P of them in one pass, for one piece of the vocabulary at a time.
+// Without kept powers the backward multiplies again, four products in all.  Forward and backward, kept / again: 16384 x 131072 x 2048 BF16
 // 22.5 / 27.9 ms, 2048 x 32768 x 1024 BF16 0.45 / 0.54, 4096 x 32768 x 1024 FP32 2.45 / 3.04.
 //
 // Rows whose target is ignored are left out before anything is multiplied: the rows that count are
@@ -16,11 +16,11 @@
 //
 // Operands are 16 bits wide.  BF16 and FP16 inputs are multiplied as they are.  FP32
 // inputs are scaled by a power of two to just under 2^15 and written as the sum of two FP16 numbers, hi +
-// lo (24 bits together for all within 2^-14 of the largest), and a product is
-// hi hi + hi lo + lo hi: what is left out, lo lo, is below 2^-24 of the product, like FP32's own
+// lo, and a product is hi hi + hi lo + lo hi.  The pair has 24 bits for all within 2^-16 of the largest; it ends at 2^-40 of
+// that, so smaller numbers have a bit less for every further power of two (15 at 2^-25).  What is left out, lo lo, is below 2^-24 of the product, like FP32's own
 // rounding.  Three FP16 products take 0.78 ms (16384 x 8192 x 1024, logits) where FP32 matrix instructions, at a
 // sixteenth of the FP16 rate, take 1.8 at the rate of a large library product.
-// P is rounded to the operands' type (BF16), or, for FP16 and FP32 inputs, scaled by
+// P is rounded to the operands' type (BF16), or, for FP16 and FP32 inputs, without its row's power of two (RowPowers) scaled by
 // 2^14 and written as one or two FP16 numbers, so that probabilities down to 2^-28 are normal numbers.  For BF16
 // inputs this is the gradients' largest error beside their own rounding: 0.0019 to 0.0026 relative, root mean square, for both
 // together, 0.0017 for the outputs' rounding alone.  P in FP16 would need W in FP16 as well, another copy of it.
@@ -87,8 +87,8 @@ constexpr int64_t kHeaderBytes = 256;
 // LDS serves together meet every bank once: slot = chunk ^ (-(row / 4) % 4) for rows of k (64 bytes; lanes 0-3,
 // 12-15, 20-23 and 24-27 go together), chunk ^ (4 (k % 4) + 2 (k / 8 % 2)) for columns (512 bytes).
 // 16 x 16 x 32 matrix instructions: the chip is limited by power here (1.7 of 2.4 GHz), and on registers alone
-// these reach 2.2 PFLOP/s, 32 x 32 x 16 ones 2.0.  Measured, 16384 x 16384 x 2048: dH 785-836 us (1.36 PFLOP/s), dW 852-907 (both
-// operands transposed; 1.25), logits 1.13-1.25 with their reduction.  Five LDS stages, other depths and orders of loads, and
+// these reach 2.2 PFLOP/s, 32 x 32 x 16 ones 2.0.  Measured, 16384 x 16384 x 2048: dW (both operands transposed) 785-836 us (1.36
+// PFLOP/s), dH with its FP32 sums over the pieces 830-907 (1.25), logits 1.13-1.25 with their reduction.  Five LDS stages, other depths and orders of loads, and
 // wave priorities were no faster.
 
 struct Operand {
@@ -584,7 +584,7 @@ __global__ void __launch_bounds__(kThreads) attnres_loss_logits_kernel(LogitArgs
 
 // Backward of kept powers: P of a piece's columns, read from the powers and written as operands, both past the caches.
 // 16 rows of 512 columns per workgroup, 8 columns per thread and row.  Memory bound: 16384 x 16384 of FP16 to BF16 (1.07
-// GB) 156 us, 6.9 TB/s.
+// GB) 160 us, 6.7 TB/s.
 constexpr int kScaleRows = 16, kScaleColumns = 64 * kVec;
 
 template <class E, class T, int PARTS>
