@@ -267,8 +267,8 @@ def linear_cross_entropy(hidden: Tensor, weight: Tensor, targets: Tensor, *, ign
     are multiplied as they are.)
 
     Gradients flow to ``hidden`` and ``weight``.  Upstream gradients of
-    ``reduction="none"`` may differ by any factor: a row of ``hidden``'s gradient is as accurate
-    as if it were alone; what it adds to ``weight``'s is held, for FP16 and FP32, to 2^-39 of the
+    ``reduction="none"`` may lie far apart (BF16: by 2^90): a row of ``hidden``'s gradient is as
+    accurate as if it were alone; what it adds to ``weight``'s is held, for FP16 and FP32, to 2^-39 of the
     largest row of ``hidden`` times its upstream gradient.  The probabilities are rounded to the type of
     16-bit inputs for the gradients' products.
 

@@ -108,3 +108,13 @@ def test_rows_of_no_weight_and_of_a_nonfinite_one(dtype, recompute):
         assert torch.equal(grads[0][rows], clean[rows])
         assert not bool(grads[0][40].isfinite().any()) and not bool(grads[1].isfinite().any())
     assert not _weighted(hidden, weight, targets, torch.zeros(150, device="cuda"), recompute)[1].any()
+
+
+@pytest.mark.parametrize("dtype", [FP16, FP32])
+def test_weights_of_rows_that_are_all_ignored(dtype):
+    g, hidden, weight, targets = _inputs(11, 150, 64, 300, dtype)
+    hidden[5] = float("nan")
+    targets.fill_(-100)
+    for recompute in (False, True):
+        grads = _weighted(hidden, weight, targets, torch.full((150,), 1e6, device="cuda"), recompute)
+        assert not grads[0].any() and not grads[1].any()
