@@ -116,6 +116,14 @@ LAYER_SIGNATURES = {
     "attnres_hip_loss_backward": (ctypes.c_int, [
         _c_void_p, _i64, _c_void_p, _i64, _i64, _i64, _i64, ctypes.c_int, ctypes.c_int, ctypes.c_int, _c_void_p, _c_void_p,
         _c_void_p, _c_void_p, _c_void_p, _i64, _c_void_p]),
+    "attnres_hip_gated_ffn_saved_bytes": (_i64, [_i64, _i64, _i64, _i64, ctypes.c_int]),
+    "attnres_hip_gated_ffn_workspace_bytes": (_i64, [_i64, _i64, _i64, _i64, ctypes.c_int, ctypes.c_int]),
+    "attnres_hip_gated_ffn_forward": (ctypes.c_int, [
+        _c_void_p, _i64, _c_void_p, _i64, _c_void_p, _i64, _i64, _i64, _i64, _i64, ctypes.c_int, ctypes.c_int, _c_void_p,
+        _c_void_p, _c_void_p, _i64, _c_void_p]),
+    "attnres_hip_gated_ffn_backward": (ctypes.c_int, [
+        _c_void_p, _c_void_p, _i64, _c_void_p, _i64, _c_void_p, _i64, _i64, _i64, _i64, _i64, ctypes.c_int, ctypes.c_int,
+        _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _i64, _c_void_p]),
 }
 
 _lock = threading.Lock()

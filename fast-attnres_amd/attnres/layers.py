@@ -39,6 +39,8 @@ _LOSS_TILE, _MAX_TILES = 256, 2**22  # of tokens by words
 _MAX_KEPT = 2**33  # bytes of exponentials
 _MAX_LOOKUPS = 2**29
 _MAX_PLACES = 2**26  # rows of positions
+_MAX_HIDDEN = 2**16  # of a feed-forward block
+_ACTIVATIONS = {"silu": 0, "gelu": 1}
 
 
 # ------------------------------------------------------------------- checks
@@ -375,4 +377,104 @@ def _loss_autograd(ctx: Any, grad, _saved):
 _linear_cross_entropy.register_autograd(_loss_autograd, setup_context=_loss_context)
 
 
-__all__ = ["embedding", "layer_norm", "linear_cross_entropy"]
+# ------------------------------------------------------- gated feed-forward
+
+def gated_feed_forward(x: Tensor, gate_up: Tensor, down: Tensor, *, activation: str = "silu",
+                       recompute: bool = False) -> Tensor:
+    """``(act(x @ gate.T) * (x @ up.T)) @ down.T``: a model's gated feed-forward block.
+
+    ``x`` is ``[..., D]``, ``gate_up`` ``[2F, D]`` (the gate's rows, then the up
+    projection's), ``down`` ``[E, F]``, all BF16, FP16 or FP32, one dtype, ``1 <= D, E
+    <= 8192``, ``1 <= F <= 65536``; ``activation`` is ``"silu"`` or ``"gelu"`` (by the error
+    function).  The result is ``[..., E]``, contiguous, in ``x``'s dtype.
+
+    Sums are FP32, and so are the projections that the activation is formed from.  What the
+    second product multiplies, and in the backward the gradients of both projections, is
+    rounded to 16-bit inputs' type.  FP32 inputs are multiplied as sums of three BF16 numbers, with FP32's 24
+    bits; infinities count as NaN.
+
+    Gradients flow to all three.  For them the forward keeps both projections, 6 bytes per
+    row and hidden entry each pair (FP32: 8), in every live graph; with ``recompute=True``
+    nothing, and the backward forms them again, which adds two ninths to its products.
+    """
+    for name, value in (("x", x), ("gate_up", gate_up), ("down", down)):
+        _check_tensor(value, name, _FLOATS)
+    if x.ndim < 1 or gate_up.ndim != 2 or x.shape[-1] != gate_up.shape[1]:
+        raise ValueError("expected x [...,D] and gate_up [2F,D]")
+    if down.ndim != 2 or gate_up.shape[0] != 2 * down.shape[1]:
+        raise ValueError("expected gate_up [2F,D] and down [E,F]")
+    _check_width(x.shape[-1])
+    if not 1 <= down.shape[0] <= _MAX_WIDTH:
+        raise ValueError(f"supported envelope is 1<=E<={_MAX_WIDTH}")
+    if not 1 <= down.shape[1] <= _MAX_HIDDEN:
+        raise ValueError(f"supported envelope is 1<=F<={_MAX_HIDDEN}")
+    rows = x.numel() // x.shape[-1]
+    if rows > _MAX_TOKENS or -(-rows // 256) * -(-down.shape[1] // 128) > _MAX_TILES:
+        raise ValueError(f"supported envelope is at most {_MAX_TOKENS} rows and {_MAX_TILES} tiles of 256 rows by 128 hidden entries")
+    for name, value in (("gate_up", gate_up), ("down", down)):
+        if value.dtype != x.dtype:
+            raise TypeError(f"{name} must have the dtype of x")
+        _check_place(name, value, "x", x)
+    if activation not in _ACTIVATIONS:
+        raise ValueError("activation must be 'silu' or 'gelu'")
+    if not isinstance(recompute, bool):
+        raise TypeError("recompute must be a bool")
+    _check_gpu("gated_feed_forward", x)
+    code = _ACTIVATIONS[activation]
+    if _eager(x, gate_up, down):
+        return _native.load_autograd().gated_feed_forward(x, gate_up, down, code, not recompute)
+    keep = not recompute and _needs_grad(x, gate_up, down)
+    return _gated_feed_forward(x, gate_up, down, code, keep)[0]
+
+
+def _feed_forward_saved_bytes(rows: int, hidden: int, dtype: torch.dtype) -> int:
+    """attnres_hip_gated_ffn_saved_bytes, for sizes that may be symbols."""
+    return -(-rows // 16) * (-(-hidden // 32) * 2) * (2048 if dtype == torch.float32 else 1536)
+
+
+@torch.library.custom_op("attnres_hip::gated_feed_forward", mutates_args=(), device_types="cuda", tags=_OP_TAGS)
+def _gated_feed_forward(x: Tensor, gate_up: Tensor, down: Tensor, activation: int, keep: bool) -> tuple[Tensor, Tensor]:
+    return _native.load_autograd().feed_forward_forward(x, gate_up, down, activation, keep)
+
+
+@_gated_feed_forward.register_fake
+def _(x, gate_up, down, activation, keep):
+    rows = x.numel() // x.shape[-1]
+    saved = _feed_forward_saved_bytes(rows, down.shape[1], x.dtype) if keep else 0
+    return x.new_empty((*x.shape[:-1], down.shape[0])), x.new_empty((saved,), dtype=torch.uint8)
+
+
+@torch.library.custom_op("attnres_hip::gated_feed_forward_backward", mutates_args=(), device_types="cuda", tags=_OP_TAGS)
+def _gated_feed_forward_backward(grad: Tensor, x: Tensor, gate_up: Tensor, down: Tensor, saved: Tensor, activation: int, want_x: bool,
+                                 want_gate_up: bool, want_down: bool) -> tuple[Tensor, Tensor, Tensor]:
+    return _native.load_autograd().feed_forward_backward(grad, x, gate_up, down, saved, activation, want_x, want_gate_up, want_down)
+
+
+@_gated_feed_forward_backward.register_fake
+def _(grad, x, gate_up, down, saved, activation, want_x, want_gate_up, want_down):
+    return (x.new_empty(x.shape if want_x else (0,)), gate_up.new_empty(gate_up.shape if want_gate_up else (0,)),
+            down.new_empty(down.shape if want_down else (0,)))
+
+
+def _gated_feed_forward_context(ctx: Any, inputs: tuple, output: tuple) -> None:
+    x, gate_up, down, activation, _keep = inputs
+    saved = output[1]
+    ctx.mark_non_differentiable(saved)
+    ctx.set_materialize_grads(False)
+    ctx.save_for_backward(x, gate_up, down, saved)
+    ctx.activation = activation
+
+
+def _gated_feed_forward_autograd(ctx: Any, grad, _saved):
+    if grad is None:
+        return None, None, None, None, None
+    x, gate_up, down, saved = ctx.saved_tensors
+    wanted = ctx.needs_input_grad[:3]
+    grads = _gated_feed_forward_backward(grad, x, gate_up, down, saved, ctx.activation, *wanted)
+    return (*(g if want else None for g, want in zip(grads, wanted)), None, None)
+
+
+_gated_feed_forward.register_autograd(_gated_feed_forward_autograd, setup_context=_gated_feed_forward_context)
+
+
+__all__ = ["embedding", "gated_feed_forward", "layer_norm", "linear_cross_entropy"]

@@ -13,8 +13,9 @@ library:
   whose part 2 is scheduled with LLVM's iterative-minreg strategy, and once
   more for the (64, 4) token-block and whole-row key-resident backwards,
   scheduled with the max-ilp strategy;
-* `csrc/attnres_norm.hip`, `attnres_embedding.hip`, `attnres_loss.hip`: the
-  layers around the reads (`include/attnres_layers_hip.h`);
+* `csrc/attnres_norm.hip`, `attnres_embedding.hip`, `attnres_loss.hip`,
+  `attnres_ffn.hip`: the layers around the reads
+  (`include/attnres_layers_hip.h`);
 
 and, against PyTorch's headers and libraries, the eager autograd nodes
 `csrc/attnres_autograd.cpp` and `csrc/attnres_layers_autograd.cpp` ->
@@ -58,7 +59,7 @@ FLAGS = ["-O3", "-std=c++17", "-fPIC", "-Xclang", "-target-feature", "-Xclang", 
 AUTOGRAD_SOURCES = (CSRC / "attnres_autograd.cpp", CSRC / "attnres_layers_autograd.cpp")
 AUTOGRAD_OBJECTS = tuple(BUILD_DIR / f"{source.stem}.o" for source in AUTOGRAD_SOURCES)
 # the layers around the reads, one unit each
-LAYER_UNITS = ("attnres_norm", "attnres_embedding", "attnres_loss")
+LAYER_UNITS = ("attnres_norm", "attnres_embedding", "attnres_loss", "attnres_ffn")
 AUTOGRAD_OUTPUT = HERE / "attnres" / "_lib" / "_autograd.so"
 ROCM_INCLUDE = Path(os.environ.get("ROCM_PATH", "/opt/rocm")) / "include"
 

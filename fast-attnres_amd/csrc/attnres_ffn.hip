@@ -1,0 +1,764 @@
+// attnres_ffn.hip - the gated feed-forward block, forward and backward, for gfx950.
+//
+//   g = X Wg^T,  u = X Wu^T,  a = act(g) u,  Y = a Wd^T            (act: silu or gelu)
+//   da = dY Wd,  du = da act(g),  dg = da u act'(g)
+//   dWd = dY^T a,  dX = [dg du] W,  dW = [dg du]^T X,              W = [Wg; Wu]
+//
+// Bound by the matrix cores: 6 N D F operations forward (N rows, D wide, F hidden), 12 backward, against O(N F + D F)
+// bytes.  Five launches of tiles of 256 x 256 (attnres_product.h): g and u in one, a gate's and an up's entry in the same
+// lane, so that a is formed from the FP32 sums; Y; da, from which dg, du and a again are formed; dWd; dX; dW.
+// Products whose tiles do not fill the chip are cut along their depth, and the parts' FP32 sums added up in order.
+//
+// What goes from the forward to the backward is g and u, in the order in which a lane holds them, so both sides
+// move them 16 bytes per lane with no detour over LDS: FP32 for FP32 inputs, else FP32 cut to 24 bits (2^-17).  Rounded to
+// 16 bits they would be the gradients' largest error: BF16, root mean square, 0.0032 of dX and dW, 0.0024 as it is.
+// With `saved` NULL the backward forms them again, which adds a third to its products.
+//
+// 16-bit operands are multiplied as they are; a, dg and du are rounded to their type.  FP32 values are written as the
+// sum of three BF16 numbers, 24 bits over FP32's whole range, and a product is the six products of parts that are
+// not below 2^-26 of it: FP32 matrix instructions run at a sixteenth of the BF16 rate.
+
+#include "attnres_product.h"
+
+#include <algorithm>
+
+namespace attnres_hip {
+namespace layers {
+namespace {
+
+constexpr int kPairTile = kTile / 2;  // hidden entries of a tile of g and u
+constexpr int kSub = 16;              // rows and columns of a subtile of saved g and u
+
+template <class X>
+constexpr int kParts = std::is_same_v<X, float> ? 3 : 1;
+template <class X>
+constexpr int kSegments = std::is_same_v<X, float> ? 6 : 1;
+template <class X>
+using Part = std::conditional_t<std::is_same_v<X, float>, Bf16, X>;
+
+// ---------------------------------------------------------------- activation
+
+// FP32 inputs: the library's exponential.  16-bit ones: the instruction's, whose argument's rounding is 2^-24 |x| relative.
+template <class X>
+__device__ __forceinline__ float exponential(float x) {
+  if constexpr (std::is_same_v<X, float>) return expf(x);
+  return __builtin_amdgcn_exp2f(x * 1.44269504f);
+}
+template <class X>
+__device__ __forceinline__ float reciprocal(float x) {
+  if constexpr (std::is_same_v<X, float>) return 1.0f / x;
+  return __builtin_amdgcn_rcpf(x);
+}
+
+struct Activated {
+  float value, slope;
+};
+
+template <class X, bool SLOPE>
+__device__ __forceinline__ Activated activate(float g, int activation) {
+  if (activation == ATTNRES_SILU) {
+    const float s = reciprocal<X>(1.0f + exponential<X>(-g));
+    return {g * s, SLOPE ? s * (1.0f + g * (1.0f - s)) : 0.0f};
+  }
+  const float phi = 0.5f * (1.0f + erff(g * 0.707106781f));
+  return {g * phi, SLOPE ? phi + g * 0.398942280f * exponential<X>(-0.5f * g * g) : 0.0f};
+}
+
+// --------------------------------------------------------------- saved g and u
+
+// A subtile of 16 rows by 16 hidden entries: lane l holds row l % 16 and entries 4 (l / 16) + 0..3.
+template <class X>
+constexpr int kSubBytes = std::is_same_v<X, float> ? 2048 : 1536;
+
+template <class X>
+__device__ __forceinline__ void save_pair(char* to, int lane, f32x4 g, f32x4 u) {
+  if constexpr (std::is_same_v<X, float>) {
+    *reinterpret_cast<f32x4*>(to + lane * 16) = g;
+    *reinterpret_cast<f32x4*>(to + 1024 + lane * 16) = u;
+  } else {
+    // to nearest 24 bits, ties away from zero; infinities and NaN as they are
+    uint32_t w[8];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      w[e] = __float_as_uint(g[e]);
+      w[4 + e] = __float_as_uint(u[e]);
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) w[e] = (w[e] & 0x7f800000u) == 0x7f800000u ? w[e] : w[e] + 0x80u;
+    u32x4 high;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) high[e] = __builtin_amdgcn_perm(w[2 * e + 1], w[2 * e], 0x07060302u);
+    uint32_t low[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const uint32_t x = __builtin_amdgcn_perm(w[4 * e + 1], w[4 * e], 0x0c0c0501u);
+      const uint32_t y = __builtin_amdgcn_perm(w[4 * e + 3], w[4 * e + 2], 0x0c0c0501u);
+      low[e] = y << 16 | x;
+    }
+    *reinterpret_cast<u32x4*>(to + lane * 16) = high;
+    *reinterpret_cast<uint64_t*>(to + 1024 + lane * 8) = static_cast<uint64_t>(low[1]) << 32 | low[0];
+  }
+}
+
+template <class X>
+struct Pair {
+  u32x4 high;
+  u32x4 rest;  // 16-bit inputs: two words
+  __device__ __forceinline__ void load(const char* from, int lane) {
+    high = *reinterpret_cast<const u32x4*>(from + lane * 16);
+    if constexpr (std::is_same_v<X, float>) {
+      rest = *reinterpret_cast<const u32x4*>(from + 1024 + lane * 16);
+    } else {
+      const uint64_t low = *reinterpret_cast<const uint64_t*>(from + 1024 + lane * 8);
+      rest = u32x4{static_cast<uint32_t>(low), static_cast<uint32_t>(low >> 32), 0, 0};
+    }
+  }
+  __device__ __forceinline__ float word(int e) const {  // g: 0..3, u: 4..7
+    const uint32_t top = e % 2 == 0 ? high[e / 2] << 16 : high[e / 2] & 0xffff0000u;
+    return __uint_as_float(top | (rest[e / 4] >> (8 * (e % 4)) & 0xffu) << 8);
+  }
+  __device__ __forceinline__ float gate(int e) const {
+    if constexpr (std::is_same_v<X, float>) return __uint_as_float(high[e]);
+    return word(e);
+  }
+  __device__ __forceinline__ float up(int e) const {
+    if constexpr (std::is_same_v<X, float>) return __uint_as_float(rest[e]);
+    return word(4 + e);
+  }
+};
+
+// What is left of x's for the next part, once `packed` has their leading one.
+template <class T>
+__device__ __forceinline__ void take_part(float* x, const uint32_t* packed, int count) {
+#pragma unroll
+  for (int e = 0; e < count; ++e) x[e] -= to_f32(T{static_cast<uint16_t>(packed[e / 2] >> (16 * (e % 2)))});
+}
+
+// ------------------------------------------------------------------ g, u and a
+
+struct GateArgs {
+  Product product;  // A: gate's and up's rows, paired; B: X
+  int64_t rows, hidden, hidden_pad;
+  int activation;
+  char* saved;      // or nullptr
+  uint16_t* out[3]; // a [rows][hidden_pad], zeros past hidden; or nullptr
+};
+
+template <class X>
+__global__ void __launch_bounds__(kThreads) attnres_ffn_gate_kernel(GateArgs g) {
+  using T = Part<X>;
+  __shared__ __align__(16) uint16_t lds[kStages * 2 * kOperand];
+  TileAt tile;
+  if (!tile_at(g.product, g.product.tiles_b, &tile)) return;
+  Accumulators acc;
+  multiply<T, kSegments<X>, true, true, true>(g.product, tile, stages_of(g.product, 0), lds, acc);
+  const int wave = wave_index(), lane = threadIdx.x % 64;
+  const int64_t f0 = static_cast<int64_t>(tile.a) * kPairTile, n0 = static_cast<int64_t>(tile.b) * kTile;
+  const int64_t sub_f = g.hidden_pad / kSub, sub_n = (g.rows + kSub - 1) / kSub;
+#pragma unroll
+  for (int j = 0; j < kAcross; ++j) {
+    const int64_t at_n = n0 / kSub + (wave / 2) * kAcross + j;
+#pragma unroll
+    for (int i = 0; i < kDown / 2; ++i) {
+      const int64_t at_f = f0 / kSub + (wave % 2) * (kDown / 2) + i;
+      const f32x4 gate = acc[i][j], up = acc[i + kDown / 2][j];
+      if (g.saved != nullptr && at_n < sub_n && at_f < sub_f) {
+        save_pair<X>(g.saved + (at_n * sub_f + at_f) * kSubBytes<X>, lane, gate, up);
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float x = activate<X, false>(gate[e], g.activation).value * up[e];
+        acc[i][j][e] = at_f * kSub + 4 * (lane / 16) + e < g.hidden ? x : 0.0f;
+      }
+      __builtin_amdgcn_sched_barrier(0);  // a few outputs at a time: no registers to spill
+    }
+  }
+  if (g.out[0] == nullptr) return;
+  // rows of 256 bytes in LDS, their 16-byte slots permuted as in staged()
+  const auto slot = [](int row, int chunk) { return row * 16 + (chunk ^ (row & 15)); };
+#pragma unroll
+  for (int part = 0; part < kParts<X>; ++part) {
+#pragma unroll
+    for (int j = 0; j < kAcross; ++j) {
+      const int row = (wave / 2) * (16 * kAcross) + j * 16 + lane % 16;
+#pragma unroll
+      for (int i = 0; i < kDown / 2; ++i) {
+        float x[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = acc[i][j][e];
+        const uint32_t packed[2] = {pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3])};
+        if (part + 1 < kParts<X>) {
+          take_part<T>(x, packed, 4);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[i][j][e] = x[e];
+        }
+        const int chunk = (wave % 2) * 8 + i * 2 + lane / 32;
+        *reinterpret_cast<uint64_t*>(lds + slot(row, chunk) * 8 + (lane / 16 % 2) * 4) =
+            static_cast<uint64_t>(packed[1]) << 32 | packed[0];
+      }
+    }
+    __syncthreads();
+    for (int k = threadIdx.x; k < kTile * 16; k += kThreads) {
+      const int row = k / 16, chunk = k % 16;
+      const int64_t f = f0 + chunk * 8;
+      if (n0 + row < g.rows && f < g.hidden_pad) {
+        *reinterpret_cast<u32x4*>(g.out[part] + (n0 + row) * g.hidden_pad + f) = *reinterpret_cast<const u32x4*>(lds + slot(row, chunk) * 8);
+      }
+    }
+    if (part + 1 < kParts<X>) __syncthreads();
+  }
+}
+
+// ------------------------------------------------------------- da, dg, du and a
+
+struct SlopeArgs {
+  Product product;  // A: Wd by columns, B: dY by rows
+  int64_t rows, rows_pad, hidden, hidden_pad;
+  int activation;
+  const char* saved;
+  uint16_t* both[3];  // [rows_pad][2 hidden_pad]: dg, du; zeros past rows and hidden
+  uint16_t* out[3];   // a [rows_pad][hidden_pad], likewise
+};
+
+template <class X>
+__global__ void __launch_bounds__(kThreads) attnres_ffn_slope_kernel(SlopeArgs g) {
+  using T = Part<X>;
+  __shared__ __align__(16) uint16_t lds[kStages * 2 * kOperand];
+  TileAt tile;
+  if (!tile_at(g.product, g.product.tiles_b, &tile)) return;
+  Accumulators acc;
+  multiply<T, kSegments<X>, false, true>(g.product, tile, stages_of(g.product, 0), lds, acc);
+  const int wave = wave_index(), lane = threadIdx.x % 64;
+  const int64_t f0 = static_cast<int64_t>(tile.a) * kTile, n0 = static_cast<int64_t>(tile.b) * kTile;
+  const int64_t sub_f = g.hidden_pad / kSub, sub_n = (g.rows + kSub - 1) / kSub;
+  // A round: 64 rows, 16 of every wavefront, of three planes in LDS: dg, du and a; of FP32 one of them in its three parts.
+  constexpr int kRows = 16 * (kWaves / 2);
+  constexpr int kPlane = kRows * kTile;
+  constexpr int kTurns = kParts<X>;
+#pragma unroll
+  for (int j = 0; j < kAcross; ++j) {
+    const int64_t at_n = n0 / kSub + (wave / 2) * kAcross + j;
+    const bool counts = at_n * kSub + lane % 16 < g.rows;
+    const int row = (wave / 2) * 16 + lane % 16;
+#pragma unroll
+    for (int turn = 0; turn < kTurns; ++turn) {
+      if (j + turn > 0) __syncthreads();
+#pragma unroll
+      for (int i = 0; i < kDown; ++i) {
+        const int64_t at_f = f0 / kSub + (wave % 2) * kDown + i;
+        Pair<X> pair{};
+        if (at_n < sub_n && at_f < sub_f) pair.load(g.saved + (at_n * sub_f + at_f) * kSubBytes<X>, lane);
+        float x[3][4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const bool inside = counts && at_f * kSub + 4 * (lane / 16) + e < g.hidden;
+          const Activated act = activate<X, true>(pair.gate(e), g.activation);
+          const float da = acc[i][j][e], up = pair.up(e);
+          x[0][e] = inside ? da * up * act.slope : 0.0f;
+          x[1][e] = inside ? da * act.value : 0.0f;
+          x[2][e] = inside ? act.value * up : 0.0f;
+        }
+        const int chunk = (wave % 2) * 16 + i * 2 + lane / 32;
+        uint16_t* to = lds + staged(row, chunk) * 8 + (lane / 16 % 2) * 4;
+#pragma unroll
+        for (int plane = 0; plane < 3; ++plane) {
+          float* value = x[kTurns == 1 ? plane : turn];
+          const uint32_t packed[2] = {pack2<T>(value[0], value[1]), pack2<T>(value[2], value[3])};
+          *reinterpret_cast<uint64_t*>(to + plane * kPlane) = static_cast<uint64_t>(packed[1]) << 32 | packed[0];
+          if constexpr (kTurns > 1) take_part<T>(value, packed, 4);
+        }
+        if (i % 2 == 1) __builtin_amdgcn_sched_barrier(0);
+      }
+      __syncthreads();
+#pragma unroll
+      for (int plane = 0; plane < 3; ++plane) {
+        const int what = kTurns == 1 ? plane : turn, part = kTurns == 1 ? 0 : plane;
+        uint16_t* out = what == 2 ? g.out[part] : g.both[part];
+        if (out == nullptr) continue;
+        const int64_t ld = what == 2 ? g.hidden_pad : 2 * g.hidden_pad;
+        const int64_t first = what == 1 ? g.hidden_pad : 0;
+        for (int k = threadIdx.x; k < kRows * 32; k += kThreads) {
+          const int r = k / 32, chunk = k % 32;
+          const int64_t n = n0 + r / 16 * (16 * kAcross) + j * 16 + r % 16, f = f0 + chunk * 8;
+          if (n < g.rows_pad && f < g.hidden_pad) {
+            *reinterpret_cast<u32x4*>(out + n * ld + first + f) = *reinterpret_cast<const u32x4*>(lds + plane * kPlane + staged(r, chunk) * 8);
+          }
+        }
+      }
+    }
+  }
+}
+
+// --------------------------------------------------------------- Y and gradients
+
+struct OutArgs {
+  Product product;
+  void* out;            // [splits][rows of B][ld]
+  int64_t ld, split_stride;
+  int64_t entries_a;    // valid contiguous entries
+  int64_t half, half_pad;  // entries of B: halves of `half` that count of `half_pad`, in the output one after the other
+  int64_t entries_b;
+};
+
+template <class X, class OUT, bool A_ROWS, bool B_ROWS>
+__global__ void __launch_bounds__(kThreads) attnres_ffn_out_kernel(OutArgs g) {
+  __shared__ __align__(16) uint16_t lds[kStages * 2 * kOperand];
+  TileAt tile;
+  if (!tile_at(g.product, g.product.tiles_b, &tile)) return;
+  Accumulators acc;
+  multiply<Part<X>, kSegments<X>, A_ROWS, B_ROWS>(g.product, tile, stages_of(g.product, tile.split), lds, acc);
+  const int wave = wave_index(), lane = threadIdx.x % 64;
+  OUT* out = static_cast<OUT*>(g.out) + tile.split * g.split_stride;
+  const int64_t a0 = static_cast<int64_t>(tile.a) * kTile, b0 = static_cast<int64_t>(tile.b) * kTile;
+  constexpr bool kWide = std::is_same_v<OUT, float>;
+  constexpr int kRounds = kWide ? 2 : 1;  // 512-byte rows: 128 FP32 or 256 16-bit outputs
+  constexpr int kChunk = kWide ? 4 : 8;   // outputs per 16 bytes
+#pragma unroll
+  for (int round = 0; round < kRounds; ++round) {
+    if (!kWide || wave % 2 == round) {
+#pragma unroll
+      for (int j = 0; j < kAcross; ++j) {
+        const int column = (wave / 2) * (16 * kAcross) + j * 16 + lane % 16;
+#pragma unroll
+        for (int i = 0; i < kDown; ++i) {
+          const f32x4 x = acc[i][j];
+          if constexpr (kWide) {
+            *reinterpret_cast<f32x4*>(lds + staged(column, i * 4 + lane / 16) * 8) = x;
+          } else {
+            const int chunk = (wave % 2) * 16 + i * 2 + lane / 32;
+            *reinterpret_cast<uint64_t*>(lds + staged(column, chunk) * 8 + (lane / 16 % 2) * 4) =
+                static_cast<uint64_t>(pack2<OUT>(x[2], x[3])) << 32 | pack2<OUT>(x[0], x[1]);
+          }
+          if (i % 2 == 1) __builtin_amdgcn_sched_barrier(0);  // a few outputs at a time: no registers to spill
+        }
+      }
+    }
+    __syncthreads();
+    for (int k = threadIdx.x; k < kTile * 32; k += kThreads) {
+      const int column = k / 32, chunk = k % 32;
+      const int64_t a = a0 + round * 128 + chunk * kChunk, b = b0 + column;
+      const int64_t second = b >= g.half_pad ? 1 : 0, within = b - second * g.half_pad;
+      if (b >= g.entries_b || within >= g.half || a >= g.entries_a) continue;
+      OUT* to = out + (second * g.half + within) * g.ld + a;
+      const uint16_t* from = lds + staged(column, chunk) * 8;
+      if constexpr (kWide) {
+        const f32x4 x = *reinterpret_cast<const f32x4*>(from);
+        if (a + kChunk <= g.entries_a) {
+          reinterpret_cast<Raw32*>(to)->v = x;
+        } else {
+          for (int e = 0; a + e < g.entries_a; ++e) to[e] = x[e];
+        }
+      } else {
+        const u32x4 x = *reinterpret_cast<const u32x4*>(from);
+        if (a + kChunk <= g.entries_a) {
+          reinterpret_cast<Raw16*>(to)->v = x;
+        } else {
+          for (int e = 0; a + e < g.entries_a; ++e) to[e].bits = from[e];
+        }
+      }
+    }
+    if (round + 1 < kRounds) __syncthreads();
+  }
+}
+
+// out[r] = the sum of the parts' rows, in order.
+template <class X>
+__global__ void __launch_bounds__(kBlock) attnres_ffn_join_kernel(const float* __restrict__ partial, int splits, int64_t split_stride,
+                                                                  int64_t ld, int64_t rows, int width, X* __restrict__ out) {
+  const int chunks = (width + kVec - 1) / kVec;
+  const int64_t all = rows * chunks;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * kBlock + threadIdx.x; i < all; i += static_cast<int64_t>(gridDim.x) * kBlock) {
+    const int64_t r = i / chunks;
+    const int c = static_cast<int>(i - r * chunks) * kVec;
+    float sum[kVec] = {};
+#pragma unroll 4
+    for (int k = 0; k < splits; ++k) {
+      float x[kVec];
+      load8(partial + k * split_stride + r * ld + c, x);  // rows are padded to whole chunks
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) sum[e] += x[e];
+    }
+    store_chunk(out + r * width, c, width, sum);
+  }
+}
+
+// Rows to operands: [2 or 1 halves of half_pad][width_pad], zero-padded, of rows in halves of `half`.
+template <class X>
+struct PackArgs {
+  const X* x;
+  int64_t stride, half, half_pad, rows_out;
+  int width, width_pad;
+  uint16_t* to[3];
+};
+
+template <class X>
+__global__ void __launch_bounds__(kBlock) attnres_ffn_pack_kernel(PackArgs<X> g) {
+  using T = Part<X>;
+  const int chunks = g.width_pad / kVec;
+  const int64_t all = g.rows_out * chunks;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * kBlock + threadIdx.x; i < all; i += static_cast<int64_t>(gridDim.x) * kBlock) {
+    const int64_t r = i / chunks;
+    const int c = static_cast<int>(i - r * chunks) * kVec;
+    const int64_t second = r >= g.half_pad ? 1 : 0, within = r - second * g.half_pad;
+    float v[kVec] = {};
+    if (within < g.half && c < g.width) load_chunk(g.x + (second * g.half + within) * g.stride, c, g.width, v);
+#pragma unroll
+    for (int part = 0; part < kParts<X>; ++part) {
+      uint32_t packed[kVec / 2];
+#pragma unroll
+      for (int e = 0; e < kVec / 2; ++e) packed[e] = pack2<T>(v[2 * e], v[2 * e + 1]);
+      *reinterpret_cast<u32x4*>(g.to[part] + i * kVec) = u32x4{packed[0], packed[1], packed[2], packed[3]};
+      if (part + 1 < kParts<X>) take_part<T>(v, packed, kVec);
+    }
+  }
+}
+
+// ---------------------------------------------------------------------- host
+
+constexpr int64_t kMaxRows = int64_t{1} << 24;
+constexpr int64_t kMaxHidden = int64_t{1} << 16;
+constexpr int64_t kMaxStride = int64_t{1} << 22;  // of operands multiplied in place: 256 rows stay within 32-bit offsets
+constexpr int64_t kMaxSecond = int64_t{1} << 30;  // from the gate's rows to the up's
+constexpr int64_t kMaxTiles = int64_t{1} << 22;   // a launch takes fewer than 2^32 threads
+
+enum Pass { kForward = 0, kBackward = 1, kBackwardAgain = 2 };  // the last: without saved g and u
+
+struct Sizes {
+  int64_t rows, width, hidden, out_width;
+  int dtype;
+};
+
+struct FfnPlan {
+  int parts, segments;
+  int64_t rows_pad, width_pad, hidden_pad, out_pad;
+  bool pack_x, pack_gate_up, pack_down, pack_grad;
+  int64_t x[3], gate_up[3], down[3], grad[3], a[3], both[3];  // offsets
+  int64_t saved, partial;
+  int splits_out, splits_x, splits_gate_up, splits_down;
+  int64_t bytes, saved_bytes;
+};
+
+int64_t tiles_of(int64_t n, int64_t tile) { return (n + tile - 1) / tile; }
+
+FfnPlan ffn_plan(const Sizes& s, int pass) {
+  FfnPlan p{};
+  const bool split = s.dtype == ATTNRES_F32, backward = pass != kForward;
+  p.parts = split ? 3 : 1;
+  p.segments = split ? 6 : 1;
+  p.rows_pad = round_up(s.rows, kDepth);
+  p.width_pad = round_up(s.width, kDepth);
+  p.hidden_pad = round_up(s.hidden, kDepth);
+  p.out_pad = round_up(s.out_width, kDepth);
+  // the depth of a product is a whole number of stages, the rest of the last one zeros
+  p.pack_x = split || s.width != p.width_pad || (backward && s.rows != p.rows_pad);
+  p.pack_gate_up = split || s.width != p.width_pad || s.hidden != p.hidden_pad;
+  p.pack_down = split || s.hidden != p.hidden_pad || (backward && s.out_width != p.out_pad);
+  p.pack_grad = backward && (split || s.out_width != p.out_pad || s.rows != p.rows_pad);
+  p.saved_bytes = tiles_of(s.rows, kSub) * (p.hidden_pad / kSub) * (split ? kSubBytes<float> : kSubBytes<Bf16>);
+  int64_t at = 0;
+  const auto take = [&](int64_t bytes) {
+    const int64_t from = at;
+    at += round_up(bytes, 256);
+    return from;
+  };
+  for (int k = 0; k < p.parts; ++k) {
+    if (p.pack_x) p.x[k] = take(2 * p.rows_pad * p.width_pad);
+    if (p.pack_gate_up) p.gate_up[k] = take(4 * p.hidden_pad * p.width_pad);
+    if (p.pack_down) p.down[k] = take(2 * p.out_pad * p.hidden_pad);
+    if (p.pack_grad) p.grad[k] = take(2 * p.rows_pad * p.out_pad);
+    p.a[k] = take(2 * p.rows_pad * p.hidden_pad);
+    if (backward) p.both[k] = take(4 * p.rows_pad * p.hidden_pad);
+  }
+  if (pass == kBackwardAgain) p.saved = take(p.saved_bytes);
+  int64_t partial = 0;
+  const auto splits = [&](int64_t entries_a, int64_t entries_b, int64_t depth) {
+    const int64_t tiles = tiles_of(entries_a, kTile) * tiles_of(entries_b, kTile);
+    const int n = choose_splits(tiles, depth, p.segments, true);
+    if (n > 1) partial = std::max(partial, 4 * n * entries_b * round_up(entries_a, kVec));
+    return n;
+  };
+  if (!backward) {
+    p.splits_out = splits(s.out_width, s.rows, p.hidden_pad);
+  } else {
+    p.splits_x = splits(s.width, s.rows, 2 * p.hidden_pad);
+    p.splits_gate_up = splits(s.width, 2 * p.hidden_pad, p.rows_pad);
+    p.splits_down = splits(s.hidden, s.out_width, p.rows_pad);
+  }
+  p.partial = take(partial);
+  p.bytes = at;
+  return p;
+}
+
+unsigned stride_grid(int64_t items) { return static_cast<unsigned>(std::min<int64_t>((items + kBlock - 1) / kBlock, 8192)); }
+
+struct Call {
+  Sizes s;
+  const void* x;
+  int64_t x_stride;
+  const void* gate_up;
+  int64_t gate_up_stride;
+  const void* down;
+  int64_t down_stride;
+  int activation;
+  FfnPlan plan;
+  char* workspace;
+  hipStream_t stream;
+  uint16_t* operand(int64_t offset) const { return reinterpret_cast<uint16_t*>(workspace + offset); }
+};
+
+// An operand where it lies, or packed into the workspace; `half`, `half_pad`: see PackArgs.
+template <class X>
+Operand place_operand(const Call& c, bool pack, const int64_t* offsets, const void* x, int64_t stride, int64_t half, int64_t half_pad,
+                      int64_t rows_out, int64_t width, int64_t width_pad) {
+  if (!pack) return {{static_cast<const uint16_t*>(x), nullptr, nullptr}, stride, 0, 0, 0};
+  PackArgs<X> g{static_cast<const X*>(x), stride, half, half_pad, rows_out, static_cast<int>(width), static_cast<int>(width_pad), {}};
+  Operand o{{nullptr, nullptr, nullptr}, width_pad, 0, 0, 0};
+  for (int k = 0; k < kParts<X>; ++k) o.part[k] = g.to[k] = c.operand(offsets[k]);
+  hipLaunchKernelGGL((attnres_ffn_pack_kernel<X>), dim3(stride_grid(rows_out * width_pad / kVec)), dim3(kBlock), 0, c.stream, g);
+  return o;
+}
+
+template <class X>
+Operand place_x(const Call& c) {
+  const FfnPlan& p = c.plan;
+  return place_operand<X>(c, p.pack_x, p.x, c.x, c.x_stride, c.s.rows, p.rows_pad, p.rows_pad, c.s.width, p.width_pad);
+}
+template <class X>
+Operand place_gate_up(const Call& c) {
+  const FfnPlan& p = c.plan;
+  return place_operand<X>(c, p.pack_gate_up, p.gate_up, c.gate_up, c.gate_up_stride, c.s.hidden, p.hidden_pad, 2 * p.hidden_pad,
+                          c.s.width, p.width_pad);
+}
+template <class X>
+Operand place_down(const Call& c) {
+  const FfnPlan& p = c.plan;
+  return place_operand<X>(c, p.pack_down, p.down, c.down, c.down_stride, c.s.out_width, p.out_pad, p.out_pad, c.s.hidden,
+                          p.hidden_pad);
+}
+
+// g and u, and a from them.
+template <class X>
+void launch_gate(const Call& c, const Operand& x, const Operand& gate_up, char* saved, const int64_t* a) {
+  const FfnPlan& p = c.plan;
+  GateArgs g{};
+  Operand w = gate_up, rows = x;
+  w.entries = p.pack_gate_up ? p.hidden_pad : c.s.hidden;
+  w.second = w.entries * w.ld;
+  rows.entries = c.s.rows;
+  g.product = {w, rows, nullptr, p.width_pad, 0, static_cast<int>(tiles_of(p.hidden_pad, kPairTile)),
+               static_cast<int>(tiles_of(c.s.rows, kTile)), 1};
+  g.rows = c.s.rows;
+  g.hidden = c.s.hidden;
+  g.hidden_pad = p.hidden_pad;
+  g.activation = c.activation;
+  g.saved = saved;
+  for (int k = 0; a != nullptr && k < kParts<X>; ++k) g.out[k] = c.operand(a[k]);
+  hipLaunchKernelGGL((attnres_ffn_gate_kernel<X>), dim3(g.product.tiles_a * g.product.tiles_b), dim3(kThreads), 0, c.stream, g);
+}
+
+// out[b][a], by halves of B's entries; joined where the depth is cut.
+template <class X, bool A_ROWS, bool B_ROWS>
+void launch_out(const Call& c, const Operand& a, const Operand& b, int64_t depth, int64_t entries_a, int64_t half, int64_t half_pad,
+                int64_t entries_b, int splits, void* out) {
+  OutArgs g{};
+  g.product = {a, b, nullptr, depth, 0, static_cast<int>(tiles_of(entries_a, kTile)), static_cast<int>(tiles_of(entries_b, kTile)),
+               splits};
+  g.entries_a = entries_a;
+  g.half = half;
+  g.half_pad = half_pad;
+  g.entries_b = entries_b;
+  g.out = out;
+  g.ld = entries_a;
+  const dim3 grid(static_cast<unsigned>(g.product.tiles_a) * g.product.tiles_b * splits);
+  if (splits == 1) {
+    hipLaunchKernelGGL((attnres_ffn_out_kernel<X, X, A_ROWS, B_ROWS>), grid, dim3(kThreads), 0, c.stream, g);
+    return;
+  }
+  const int64_t rows = entries_b / half_pad * half;
+  float* partial = reinterpret_cast<float*>(c.workspace + c.plan.partial);
+  g.out = partial;
+  g.ld = round_up(entries_a, kVec);
+  g.split_stride = rows * g.ld;
+  hipLaunchKernelGGL((attnres_ffn_out_kernel<X, float, A_ROWS, B_ROWS>), grid, dim3(kThreads), 0, c.stream, g);
+  hipLaunchKernelGGL((attnres_ffn_join_kernel<X>), dim3(stride_grid(rows * (g.ld / kVec))), dim3(kBlock), 0, c.stream, partial, splits,
+                     g.split_stride, g.ld, rows, static_cast<int>(entries_a), static_cast<X*>(out));
+}
+
+template <class X>
+void ffn_forward(const Call& c, void* out, char* saved) {
+  const FfnPlan& p = c.plan;
+  launch_gate<X>(c, place_x<X>(c), place_gate_up<X>(c), saved, p.a);
+  Operand down = place_down<X>(c), a{};
+  down.entries = c.s.out_width;
+  for (int k = 0; k < kParts<X>; ++k) a.part[k] = c.operand(p.a[k]);
+  a.ld = p.hidden_pad;
+  a.entries = c.s.rows;
+  launch_out<X, true, true>(c, down, a, p.hidden_pad, c.s.out_width, c.s.rows, c.s.rows, c.s.rows, p.splits_out, out);
+}
+
+template <class X>
+void ffn_backward(const Call& c, const void* grad_out, const char* saved, void* grad_x, void* grad_gate_up, void* grad_down) {
+  const FfnPlan& p = c.plan;
+  Operand x{}, gate_up{};
+  if (saved == nullptr || grad_gate_up != nullptr) x = place_x<X>(c);
+  if (saved == nullptr || grad_x != nullptr) gate_up = place_gate_up<X>(c);
+  if (saved == nullptr) {
+    char* again = c.workspace + p.saved;
+    launch_gate<X>(c, x, gate_up, again, nullptr);
+    saved = again;
+  }
+  const Operand grad = place_operand<X>(c, p.pack_grad, p.grad, grad_out, c.s.out_width, c.s.rows, p.rows_pad, p.rows_pad,
+                                        c.s.out_width, p.out_pad);
+  {
+    SlopeArgs g{};
+    Operand down = place_down<X>(c), rows = grad;
+    down.entries = p.hidden_pad;
+    down.depth = p.out_pad;
+    rows.entries = c.s.rows;
+    g.product = {down, rows, nullptr, p.out_pad, 0, static_cast<int>(tiles_of(p.hidden_pad, kTile)),
+                 static_cast<int>(tiles_of(p.rows_pad, kTile)), 1};
+    g.rows = c.s.rows;
+    g.rows_pad = p.rows_pad;
+    g.hidden = c.s.hidden;
+    g.hidden_pad = p.hidden_pad;
+    g.activation = c.activation;
+    g.saved = saved;
+    for (int k = 0; k < kParts<X>; ++k) {
+      if (grad_x != nullptr || grad_gate_up != nullptr) g.both[k] = c.operand(p.both[k]);
+      if (grad_down != nullptr) g.out[k] = c.operand(p.a[k]);
+    }
+    hipLaunchKernelGGL((attnres_ffn_slope_kernel<X>), dim3(g.product.tiles_a * g.product.tiles_b), dim3(kThreads), 0, c.stream, g);
+  }
+  Operand both{}, a{};
+  for (int k = 0; k < kParts<X>; ++k) {
+    both.part[k] = c.operand(p.both[k]);
+    a.part[k] = c.operand(p.a[k]);
+  }
+  both.ld = 2 * p.hidden_pad;
+  a.ld = p.hidden_pad;
+  both.depth = a.depth = p.rows_pad;
+  if (grad_down != nullptr) {
+    Operand rows = grad;
+    rows.entries = p.pack_grad ? p.out_pad : c.s.out_width;
+    rows.depth = p.rows_pad;
+    a.entries = p.hidden_pad;
+    launch_out<X, false, false>(c, a, rows, p.rows_pad, c.s.hidden, c.s.out_width, c.s.out_width, c.s.out_width, p.splits_down, grad_down);
+  }
+  if (grad_gate_up != nullptr) {
+    x.entries = p.pack_x ? p.width_pad : c.s.width;
+    x.depth = p.rows_pad;
+    both.entries = 2 * p.hidden_pad;
+    launch_out<X, false, false>(c, x, both, p.rows_pad, c.s.width, c.s.hidden, p.hidden_pad, 2 * p.hidden_pad, p.splits_gate_up,
+                                grad_gate_up);
+  }
+  if (grad_x != nullptr) {
+    gate_up.entries = p.pack_gate_up ? p.width_pad : c.s.width;
+    gate_up.depth = 2 * p.hidden_pad;
+    both.entries = c.s.rows;
+    launch_out<X, false, true>(c, gate_up, both, 2 * p.hidden_pad, c.s.width, c.s.rows, c.s.rows, c.s.rows, p.splits_x, grad_x);
+  }
+}
+
+bool known_sizes(const Sizes& s) {
+  return s.rows >= 0 && s.rows <= kMaxRows && s.width >= 1 && s.width <= ATTNRES_MAX_WIDTH && s.hidden >= 1 && s.hidden <= kMaxHidden &&
+         s.out_width >= 1 && s.out_width <= ATTNRES_MAX_WIDTH && dtype_known(s.dtype) &&
+         tiles_of(s.rows, kTile) * tiles_of(s.hidden, kPairTile) <= kMaxTiles;
+}
+
+int check_sizes(const Sizes& s, int activation) {
+  if (s.rows < 0 || s.rows > kMaxRows) return layer_error(ATTNRES_ERR_SHAPE, "rows=%lld outside 0..2^24", (long long)s.rows);
+  if (s.width < 1 || s.width > ATTNRES_MAX_WIDTH || s.out_width < 1 || s.out_width > ATTNRES_MAX_WIDTH) {
+    return layer_error(ATTNRES_ERR_SHAPE, "width=%lld or out_width=%lld outside 1..%d", (long long)s.width, (long long)s.out_width,
+                       ATTNRES_MAX_WIDTH);
+  }
+  if (s.hidden < 1 || s.hidden > kMaxHidden) return layer_error(ATTNRES_ERR_SHAPE, "hidden=%lld outside 1..2^16", (long long)s.hidden);
+  if (!dtype_known(s.dtype)) return layer_error(ATTNRES_ERR_SHAPE, "unknown dtype %d", s.dtype);
+  if (!known_sizes(s)) return layer_error(ATTNRES_ERR_SHAPE, "rows x hidden outside 2^22 tiles of 256 x 128");
+  if (activation != ATTNRES_SILU && activation != ATTNRES_GELU) return layer_error(ATTNRES_ERR_SCALAR, "unknown activation %d", activation);
+  return ATTNRES_OK;
+}
+
+// Operands that are multiplied where they lie: whole 16-byte loads, 32-bit offsets.
+int check_rows(const char* name, const void* x, int64_t stride, bool in_place, int64_t least, int64_t most) {
+  if (x == nullptr) return layer_error(ATTNRES_ERR_NULL_POINTER, "%s is NULL", name);
+  if (stride < 0) return layer_error(ATTNRES_ERR_STRIDE, "negative row stride of %s", name);
+  if (in_place && ((reinterpret_cast<uintptr_t>(x) & 15u) != 0 || stride % 8 != 0 || stride < least || stride > most)) {
+    return layer_error(ATTNRES_ERR_STRIDE, "rows of %s must start at multiples of 16 bytes, at most %lld elements apart", name,
+                       (long long)most);
+  }
+  return ATTNRES_OK;
+}
+
+int check_call(const Call& c, const void* saved, int64_t workspace_bytes) {
+  const FfnPlan& p = c.plan;
+  if (const int status = check_rows("x", c.x, c.x_stride, !p.pack_x, 0, kMaxStride)) return status;
+  if (const int status = check_rows("gate_up", c.gate_up, c.gate_up_stride, !p.pack_gate_up, c.s.width,
+                                    std::min(kMaxStride, kMaxSecond / c.s.hidden))) {
+    return status;
+  }
+  if (const int status = check_rows("down", c.down, c.down_stride, !p.pack_down, c.s.hidden, kMaxStride)) return status;
+  if (c.workspace == nullptr || workspace_bytes < p.bytes) {
+    return layer_error(ATTNRES_ERR_WORKSPACE, "workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)p.bytes);
+  }
+  if (((reinterpret_cast<uintptr_t>(saved) | reinterpret_cast<uintptr_t>(c.workspace)) & 15u) != 0) {
+    return layer_error(ATTNRES_ERR_WORKSPACE, "saved and workspace must start at multiples of 16 bytes");
+  }
+  return ATTNRES_OK;
+}
+
+}  // namespace
+}  // namespace layers
+}  // namespace attnres_hip
+
+using namespace attnres_hip;
+using namespace attnres_hip::layers;
+
+extern "C" {
+
+int64_t attnres_hip_gated_ffn_saved_bytes(int64_t rows, int64_t width, int64_t hidden, int64_t out_width, int dtype) {
+  const Sizes s{rows, width, hidden, out_width, dtype};
+  return known_sizes(s) ? ffn_plan(s, kForward).saved_bytes : -1;
+}
+
+int64_t attnres_hip_gated_ffn_workspace_bytes(int64_t rows, int64_t width, int64_t hidden, int64_t out_width, int dtype, int backward) {
+  const Sizes s{rows, width, hidden, out_width, dtype};
+  return known_sizes(s) && backward >= kForward && backward <= kBackwardAgain ? ffn_plan(s, backward).bytes : -1;
+}
+
+int attnres_hip_gated_ffn_forward(const void* x, int64_t x_stride, const void* gate_up, int64_t gate_up_stride, const void* down,
+                                  int64_t down_stride, int64_t rows, int64_t width, int64_t hidden, int64_t out_width, int dtype,
+                                  int activation, void* out, void* saved, void* workspace, int64_t workspace_bytes, void* stream) {
+  const Sizes s{rows, width, hidden, out_width, dtype};
+  if (const int status = check_sizes(s, activation)) return status;
+  if (rows == 0) return ATTNRES_OK;
+  const Call c{s, x, x_stride, gate_up, gate_up_stride, down, down_stride, activation, ffn_plan(s, kForward),
+               static_cast<char*>(workspace), static_cast<hipStream_t>(stream)};
+  if (const int status = check_call(c, saved, workspace_bytes)) return status;
+  if (out == nullptr) return layer_error(ATTNRES_ERR_NULL_POINTER, "out is NULL");
+  if (dtype == ATTNRES_BF16) ffn_forward<Bf16>(c, out, static_cast<char*>(saved));
+  else if (dtype == ATTNRES_F16) ffn_forward<F16>(c, out, static_cast<char*>(saved));
+  else ffn_forward<float>(c, out, static_cast<char*>(saved));
+  return layer_launch_status("gated feed-forward forward");
+}
+
+int attnres_hip_gated_ffn_backward(const void* grad_out, const void* x, int64_t x_stride, const void* gate_up, int64_t gate_up_stride,
+                                   const void* down, int64_t down_stride, int64_t rows, int64_t width, int64_t hidden,
+                                   int64_t out_width, int dtype, int activation, const void* saved, void* grad_x, void* grad_gate_up,
+                                   void* grad_down, void* workspace, int64_t workspace_bytes, void* stream) {
+  const Sizes s{rows, width, hidden, out_width, dtype};
+  if (const int status = check_sizes(s, activation)) return status;
+  if (rows == 0) return layer_error(ATTNRES_ERR_SHAPE, "no rows: the weights' gradients are zeros, which the caller writes");
+  const Call c{s, x, x_stride, gate_up, gate_up_stride, down, down_stride, activation,
+               ffn_plan(s, saved != nullptr ? kBackward : kBackwardAgain), static_cast<char*>(workspace),
+               static_cast<hipStream_t>(stream)};
+  if (const int status = check_call(c, saved, workspace_bytes)) return status;
+  if (const int status = check_rows("grad_out", grad_out, out_width, !c.plan.pack_grad, 0, kMaxStride)) return status;
+  if (grad_x == nullptr && grad_gate_up == nullptr && grad_down == nullptr) return ATTNRES_OK;
+  const char* kept = static_cast<const char*>(saved);
+  if (dtype == ATTNRES_BF16) ffn_backward<Bf16>(c, grad_out, kept, grad_x, grad_gate_up, grad_down);
+  else if (dtype == ATTNRES_F16) ffn_backward<F16>(c, grad_out, kept, grad_x, grad_gate_up, grad_down);
+  else ffn_backward<float>(c, grad_out, kept, grad_x, grad_gate_up, grad_down);
+  return layer_launch_status("gated feed-forward backward");
+}
+
+}  // extern "C"

@@ -1,5 +1,5 @@
 // The eager autograd nodes of the layers (attnres.layers), in C++ over the C ABI
-// (attnres_layers_hip.h): layer norm, embedding and the loss over a vocabulary.
+// (attnres_layers_hip.h): layer norm, embedding, the loss over a vocabulary and the gated feed-forward block.
 //
 // Each layer has a forward and a backward function that allocate and launch; the nodes
 // call them without Python, and so do the torch.library ops that stand for the nodes
@@ -8,6 +8,8 @@
 #include <torch/extension.h>
 
 #include <torch/csrc/autograd/functions/basic_ops.h>
+
+#include <algorithm>
 
 #include "attnres_layers_hip.h"
 #include "attnres_nodes.h"
@@ -344,6 +346,123 @@ Tensor linear_cross_entropy(const Tensor& hidden, const Tensor& weight, const Te
   return LinearCrossEntropy::apply(hidden, weight, targets, ignore_index, reduction, keep);
 }
 
+// ----------------------------------------------------- gated feed-forward
+
+// Rows as the products take them: 16-bit rows of whole 32-element steps are multiplied where they lie and have to
+// start at multiples of 16 bytes, `least` to `most` elements apart; a copy does.
+Rows product_rows(const Tensor& tensor, bool in_place, int64_t least, int64_t most) {
+  Rows rows = rows_view(tensor);
+  if (rows_of(tensor) == 1 && rows.stride < least) rows.stride = least;
+  if (in_place && (reinterpret_cast<uintptr_t>(rows.tensor.data_ptr()) % 16 != 0 || rows.stride % 8 != 0 ||
+                   rows.stride < least || rows.stride > most)) {
+    Tensor copy = torch::empty(tensor.sizes(), tensor.options().memory_format(at::MemoryFormat::Contiguous));
+    copy.copy_(tensor);
+    rows = {copy, copy.size(-1)};
+  }
+  return rows;
+}
+
+struct FeedForward {
+  Rows x, gate_up, down;
+  int64_t rows, width, hidden, out_width;
+  int dtype;
+  FeedForward(const Tensor& input, const Tensor& weights, const Tensor& last)
+      : rows(input.numel() / input.size(-1)), width(weights.size(1)), hidden(last.size(1)), out_width(last.size(0)),
+        dtype(dtype_of(input.scalar_type())) {
+    const bool half = dtype != ATTNRES_F32, even = hidden % 32 == 0;
+    constexpr int64_t kMost = int64_t{1} << 22;
+    x = product_rows(input, half && width % 32 == 0, 0, kMost);
+    gate_up = product_rows(weights, half && width % 32 == 0 && even, width, std::min(kMost, (int64_t{1} << 30) / hidden));
+    down = product_rows(last, half && even, hidden, kMost);
+  }
+  Tensor workspace(const Tensor& like, int backward) const {
+    const int64_t bytes = attnres_hip_gated_ffn_workspace_bytes(rows, width, hidden, out_width, dtype, backward);
+    TORCH_CHECK_VALUE(bytes >= 0, "gated feed-forward: shape outside the supported envelope");
+    return torch::empty({bytes}, like.options().dtype(torch::kUInt8));
+  }
+};
+
+// (out, saved): saved is empty where it is not kept.
+std::tuple<Tensor, Tensor> feed_forward_forward(const Tensor& x, const Tensor& gate_up, const Tensor& down, int64_t activation,
+                                                bool keep) {
+  refuse_tangents("gated_feed_forward", x, gate_up, down);
+  const c10::DeviceGuard guard(x.device());
+  const at::NoGradGuard no_grad;
+  const FeedForward f(x, gate_up, down);
+  std::vector<int64_t> shape = x.sizes().vec();
+  shape.back() = f.out_width;
+  Tensor out = torch::empty(shape, x.options().memory_format(at::MemoryFormat::Contiguous));
+  const auto bytes = x.options().dtype(torch::kUInt8);
+  if (f.rows == 0) return {out, torch::empty({0}, bytes)};
+  const Tensor workspace = f.workspace(x, 0);
+  Tensor saved = torch::empty({keep ? attnres_hip_gated_ffn_saved_bytes(f.rows, f.width, f.hidden, f.out_width, f.dtype) : 0}, bytes);
+  check(attnres_hip_gated_ffn_forward(f.x.tensor.data_ptr(), f.x.stride, f.gate_up.tensor.data_ptr(), f.gate_up.stride,
+                                      f.down.tensor.data_ptr(), f.down.stride, f.rows, f.width, f.hidden, f.out_width, f.dtype,
+                                      static_cast<int>(activation), out.data_ptr(), keep ? saved.data_ptr() : nullptr,
+                                      workspace.data_ptr(), workspace.numel(), current_stream(x)),
+        "gated feed-forward forward");
+  return {out, saved};
+}
+
+// saved: empty where the backward forms it again; gradients that are not wanted come back empty.
+std::tuple<Tensor, Tensor, Tensor> feed_forward_backward(const Tensor& grad_out, const Tensor& x, const Tensor& gate_up,
+                                                         const Tensor& down, const Tensor& saved, int64_t activation, bool want_x,
+                                                         bool want_gate_up, bool want_down) {
+  refuse_tangents("gated_feed_forward's backward", grad_out, x, gate_up, down);
+  const c10::DeviceGuard guard(x.device());
+  const at::NoGradGuard no_grad;
+  const FeedForward f(x, gate_up, down);
+  const auto result = [&](const Tensor& like, bool wanted) {
+    if (!wanted) return torch::empty({0}, like.options());
+    const auto options = like.options().memory_format(at::MemoryFormat::Contiguous);
+    return f.rows == 0 ? torch::zeros(like.sizes(), options) : torch::empty(like.sizes(), options);
+  };
+  Tensor grad_x = result(x, want_x), grad_gate_up = result(gate_up, want_gate_up), grad_down = result(down, want_down);
+  if (f.rows == 0) return {grad_x, grad_gate_up, grad_down};
+  Tensor grad = grad_out.to(x.scalar_type()).contiguous();
+  if (reinterpret_cast<uintptr_t>(grad.data_ptr()) % 16 != 0) grad = grad.clone();
+  const Tensor workspace = f.workspace(x, saved.numel() > 0 ? 1 : 2);
+  check(attnres_hip_gated_ffn_backward(grad.data_ptr(), f.x.tensor.data_ptr(), f.x.stride, f.gate_up.tensor.data_ptr(),
+                                       f.gate_up.stride, f.down.tensor.data_ptr(), f.down.stride, f.rows, f.width, f.hidden,
+                                       f.out_width, f.dtype, static_cast<int>(activation),
+                                       saved.numel() > 0 ? saved.data_ptr() : nullptr, want_x ? grad_x.data_ptr() : nullptr,
+                                       want_gate_up ? grad_gate_up.data_ptr() : nullptr,
+                                       want_down ? grad_down.data_ptr() : nullptr, workspace.data_ptr(), workspace.numel(),
+                                       current_stream(x)),
+        "gated feed-forward backward");
+  return {grad_x, grad_gate_up, grad_down};
+}
+
+struct GatedFeedForward : public torch::autograd::Function<GatedFeedForward> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& gate_up, const Tensor& down, int64_t activation,
+                        bool keep) {
+    auto [out, saved] = feed_forward_forward(x, gate_up, down, activation, keep);
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({x, gate_up, down, saved});
+    ctx->saved_data["activation"] = activation;
+    return out;
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    variable_list result(5);
+    if (!grads[0].defined()) return result;
+    const variable_list saved = ctx->get_saved_variables();
+    const bool want[3] = {ctx->needs_input_grad(0), ctx->needs_input_grad(1), ctx->needs_input_grad(2)};
+    const auto [grad_x, grad_gate_up, grad_down] =
+        feed_forward_backward(grads[0], saved[0], saved[1], saved[2], saved[3], ctx->saved_data["activation"].toInt(), want[0],
+                              want[1], want[2]);
+    if (want[0]) result[0] = grad_x;
+    if (want[1]) result[1] = grad_gate_up;
+    if (want[2]) result[2] = grad_down;
+    return once_differentiable(std::move(result));
+  }
+};
+
+Tensor gated_feed_forward(const Tensor& x, const Tensor& gate_up, const Tensor& down, int64_t activation, bool keep) {
+  if (!wants_grad({x, gate_up, down})) return std::get<0>(feed_forward_forward(x, gate_up, down, activation, false));
+  return GatedFeedForward::apply(x, gate_up, down, activation, keep);
+}
+
 }  // namespace
 
 void bind_layers(pybind11::module_& m) {
@@ -356,6 +475,9 @@ void bind_layers(pybind11::module_& m) {
   m.def("linear_cross_entropy", &linear_cross_entropy, "loss over a vocabulary (eager autograd node)");
   m.def("loss_forward", &loss_forward, "(loss, saved)");
   m.def("loss_backward", &loss_backward, "(grad_hidden, grad_weight)");
+  m.def("gated_feed_forward", &gated_feed_forward, "gated feed-forward block (eager autograd node)");
+  m.def("feed_forward_forward", &feed_forward_forward, "(out, saved)");
+  m.def("feed_forward_backward", &feed_forward_backward, "(grad_x, grad_gate_up, grad_down)");
 }
 
 }  // namespace attnres_nodes

@@ -1,0 +1,389 @@
+// attnres_product.h - the matrix product of the layers: tiles of 256 x 256 outputs of 16-bit operands on the matrix
+// cores, summed in FP32 (attnres_loss.hip, attnres_ffn.hip).
+#ifndef ATTNRES_PRODUCT_H
+#define ATTNRES_PRODUCT_H
+
+#include "attnres_layers.h"
+
+namespace attnres_hip {
+namespace layers {
+
+constexpr int kTile = 256;     // rows and columns of a workgroup's tile
+constexpr int kWaves = 8;      // of 128 x 64 outputs, two per SIMD
+constexpr int kThreads = 64 * kWaves;
+constexpr int kDown = 8;       // 16 x 16 tiles of a wavefront: down (A) and across (B)
+constexpr int kAcross = 4;
+constexpr int kDepth = 32;     // of a stage of a tile's operands in LDS
+constexpr int kStages = 4;     // in LDS: one that is multiplied, three on their way
+constexpr int kLoads = 2;      // per wavefront, operand and stage: 1 KB each
+constexpr int kOperand = kTile * kDepth;  // elements of one operand's stage
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+
+#define ATTNRES_LDS __attribute__((address_space(3)))
+#define ATTNRES_GLOBAL __attribute__((address_space(1)))
+
+__host__ __device__ inline int64_t round_up(int64_t x, int64_t to) { return (x + to - 1) / to * to; }
+
+// out[b][a] = sum_k A[a][k] B[b][k] over a tile of 256 x 256: A's index is the contiguous
+// one of the output.  An operand lies either as rows of k (ROWS: the row is contiguous in k) or as
+// columns (row k holds all of the operand's entries).  Both go to LDS as they lie, 16 bytes
+// per lane straight from memory; a column operand's fragments are transposed on the way
+// from LDS (ds_read_b64_tr_b16).  16-byte slots are permuted within an LDS row so that the lanes which
+// LDS serves together meet every bank once: slot = chunk ^ (-(row / 4) % 4) for rows of k (64 bytes; lanes 0-3,
+// 12-15, 20-23 and 24-27 go together), chunk ^ (4 (k % 4) + 2 (k / 8 % 2)) for columns (512 bytes).
+// 16 x 16 x 32 matrix instructions: the chip is limited by power here (1.7 of 2.4 GHz), and on registers alone
+// these reach 2.2 PFLOP/s, 32 x 32 x 16 ones 2.0.  Measured, 16384 x 16384 x 2048: dW (both operands transposed) 785-836 us (1.36
+// PFLOP/s), dH with its FP32 sums over the pieces 830-907 (1.25), logits 1.13-1.25 with their reduction.  Five LDS stages, other depths and orders of loads, and
+// wave priorities were no faster.
+
+struct Operand {
+  const uint16_t* part[3];  // hi, lo; or the three parts of FP32 values
+  int64_t ld;
+  int64_t entries;          // readable entries (rows: clamped row; columns: multiple of 8)
+  int64_t depth;            // readable k of a column operand
+  int64_t second;           // PAIRED rows: elements from the first half's start to the second's
+};
+
+struct Product {
+  Operand a, b;
+  const int32_t* count;  // live packed rows
+  int64_t depth;         // k of the whole product, of all splits; operands hold zeros up to a whole stage
+  int depth_is_count;    // depth: the packed rows
+  int tiles_a, tiles_b, splits;
+};
+
+__device__ __forceinline__ int row_swizzle(int row) { return -(row >> 2) & 3; }
+__device__ __forceinline__ int column_swizzle(int k) { return (k & 3) << 2 | (k >> 3 & 1) << 1; }
+
+// PAIRED rows: a tile holds 128 entries of each of two operands of one shape, so that a wavefront's accumulators
+// i and i + kDown / 2 are entry e of the one and of the other: 64 of the first, 64 of the second, in turn.
+constexpr int kPaired = 64;
+
+template <bool ROWS, bool PAIRED = false>
+struct Loader {
+  uint32_t offset[kLoads];  // bytes from the stage's origin; columns: of the chunk alone
+  int row;                  // columns: k of the first load
+  __device__ __forceinline__ void init(const Operand& o, int64_t entry0, int wave, int lane) {
+    row = wave * kLoads * 2 + lane / 32;
+#pragma unroll
+    for (int j = 0; j < kLoads; ++j) {
+      if constexpr (ROWS) {
+        const int r = (wave * kLoads + j) * 16 + lane / 4;
+        const int entry = PAIRED ? r / (2 * kPaired) * kPaired + r % kPaired : r;
+        const int64_t left = o.entries - 1 - entry0;
+        const int64_t at = entry < left ? entry : left;
+        const int64_t from = at * o.ld + (PAIRED && r / kPaired % 2 == 1 ? o.second : 0);
+        offset[j] = static_cast<uint32_t>((from + ((lane % 4) ^ row_swizzle(r)) * 8) * 2);
+      } else {
+        const int chunk = (lane % 32) ^ column_swizzle(row + j * 2);
+        const int64_t left = o.entries - 8 - entry0;
+        const int64_t at = chunk * 8 < left ? chunk * 8 : left;
+        offset[j] = static_cast<uint32_t>(at * 2);
+      }
+    }
+  }
+  // Offsets of a stage; left: k's of it that a column operand holds, less one.
+  __device__ __forceinline__ void offsets(const Operand& o, int left, uint32_t (&at)[kLoads]) const {
+#pragma unroll
+    for (int j = 0; j < kLoads; ++j) {
+      at[j] = offset[j];
+      if constexpr (!ROWS) at[j] += static_cast<uint32_t>(min(row + j * 2, left)) * static_cast<uint32_t>(o.ld * 2);
+    }
+  }
+};
+
+// A 1-KB load into LDS byte `lds` from `base` (scalar) and `at` bytes on, 16 bytes per lane.  Written out,
+// since the compiler makes transposing LDS reads wait for every load into LDS that it knows of; what has to
+// have landed is waited for in landed().  The address registers are read when the load is issued, and
+// nothing comes back in registers.
+__device__ __forceinline__ void load_lds(const char* base, uint32_t at, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(lds), "v"(at), "s"(base) : "m0");
+}
+
+// The LDS byte of a pointer into LDS.
+__device__ __forceinline__ uint32_t lds_byte(const uint16_t* p) {
+  return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((const ATTNRES_LDS uint16_t*)p));
+}
+
+// Fragments of 16 entries and a stage's 32 k's: lane l holds entry l % 16, k = 8 (l / 16) + 0..7.
+template <bool ROWS>
+struct Reader {
+  uint32_t at;      // the lane's byte of a stage; columns: of its row of k
+  uint32_t column;  // columns: the lane's byte in that row, before the fragment's number is permuted in
+  __device__ __forceinline__ void init(int entry, int lane) {
+    const int group = lane / 16, j = lane % 16;
+    if constexpr (ROWS) {
+      at = static_cast<uint32_t>((entry + j) * kDepth + (group ^ row_swizzle(j)) * 8) * 2;
+      column = 0;
+    } else {
+      // 16 lanes read 4 k's of 16 entries and get one entry's 4 k's each
+      const int k = group * 8 + j / 4;
+      const int chunk = entry / 8 + j % 4 / 2;  // the fragment's number is a part of its low four bits
+      at = static_cast<uint32_t>(k * kTile + chunk / 16 * 128) * 2;
+      column = static_cast<uint32_t>((chunk % 16 ^ column_swizzle(k)) * 8 + j % 2 * 4) * 2;
+    }
+  }
+  __device__ __forceinline__ s16x8 read(uint32_t stage, int f) const {
+    if constexpr (ROWS) {
+      return *(ATTNRES_LDS const s16x8*)(stage + at + f * 16 * kDepth * 2);
+    } else {
+      const uint32_t from = stage + at + (column ^ (f * 32u));
+      const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((ATTNRES_LDS s16x4*)(from));
+      const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((ATTNRES_LDS s16x4*)(from + 4 * kTile * 2));
+      return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+  }
+};
+
+template <class T>
+__device__ __forceinline__ f32x4 mfma(s16x8 a, s16x8 b, f32x4 c) {
+  if constexpr (std::is_same_v<T, Bf16>) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  } else {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  }
+}
+
+__device__ __forceinline__ int wave_index() { return __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x / 64)); }
+
+struct TileAt {
+  int a, b, split;
+};
+
+// Workgroup to tile: workgroups go round the 8 XCDs in turn, so each XCD takes one contiguous part of
+// the tiles' order, in which 4 tiles of B by all of A's follow each other: the 32 tiles that run on an
+// XCD at a time share 4 + 8 operand stripes in its L2.  tiles_b: those with rows that count, so that the XCDs
+// get equal shares of them; false for the workgroups past the last tile.
+__device__ __forceinline__ bool tile_at(const Product& p, int tiles_b, TileAt* tile) {
+  const int total = p.tiles_a * tiles_b * p.splits;
+  const int id = blockIdx.x;
+  if (id >= total) return false;
+  const int q = total / 8, r = total % 8, xcd = id % 8, i = id / 8;
+  int at = xcd < r ? xcd * (q + 1) + i : r * (q + 1) + (xcd - r) * q + i;
+  const int split = at / (p.tiles_a * tiles_b);
+  at -= split * p.tiles_a * tiles_b;
+  constexpr int kGroup = 4;
+  const int group = at / (kGroup * p.tiles_a);
+  const int size = min(kGroup, tiles_b - group * kGroup);
+  at -= group * kGroup * p.tiles_a;
+  *tile = {at / size, group * kGroup + at % size, split};
+  return true;
+}
+
+// [16 entries of A][16 entries of B]; lane l, register e: entry 4 (l / 16) + e of A, l % 16 of B.
+using Accumulators = f32x4[kDown][kAcross];
+
+// A pointer that every lane holds, in scalar registers, and opaque from here on.
+__device__ __forceinline__ const char* scalar(const char* p) {
+  const uint64_t bits = reinterpret_cast<uint64_t>(p);
+  uint32_t lo = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(bits)));
+  uint32_t hi = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(bits >> 32)));
+  asm volatile("" : "+s"(lo), "+s"(hi));
+  return reinterpret_cast<const char*>(static_cast<uint64_t>(hi) << 32 | lo);
+}
+
+// This wavefront's reads from LDS are done and its loads of the next stage have landed, and so it is for every
+// wavefront (a barrier alone waits for neither).  Loads arrive in order: with `more`, those of
+// the stages after the next one may still be on their way.
+__device__ __forceinline__ void landed(bool more) {
+  if (more) {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"i"((kStages - 2) * 2 * kLoads) : "memory");
+  } else {
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+  }
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+// The stages of a tile's split; none where there are fewer stages than splits.
+struct Stages {
+  int first, count;
+};
+__device__ __forceinline__ Stages stages_of(const Product& p, int split) {
+  const int64_t depth = p.depth_is_count ? *p.count : p.depth;
+  const int64_t all = (depth + kDepth - 1) / kDepth;
+  const int first = static_cast<int>(all * split / p.splits);
+  return {__builtin_amdgcn_readfirstlane(first),
+          __builtin_amdgcn_readfirstlane(static_cast<int>(all * (split + 1) / p.splits) - first)};
+}
+
+// The parts that a segment multiplies.  3: hi hi + hi lo + lo hi; 6: of three parts each those products that are not
+// below 2^-26 of the whole.
+template <int SEGMENTS>
+__device__ __forceinline__ int part_of_a(int segment) {
+  if constexpr (SEGMENTS == 3) return segment == 2;
+  if constexpr (SEGMENTS == 6) return segment == 5 ? 2 : segment / 2 % 2;  // 0 0 1 1 0 2
+  return 0;
+}
+template <int SEGMENTS>
+__device__ __forceinline__ int part_of_b(int segment) {
+  if constexpr (SEGMENTS == 3) return segment == 1;
+  if constexpr (SEGMENTS == 6) return segment == 4 ? 2 : segment == 5 ? 0 : segment % 2;  // 0 1 0 1 2 0
+  return 0;
+}
+
+// The sum of a tile over its split's k's (at least one stage).  PAIRED: tile.a counts tiles of 128 entries.
+template <class T, int SEGMENTS, bool A_ROWS, bool B_ROWS, bool PAIRED = false>
+__device__ __forceinline__ void multiply(const Product& p, const TileAt& tile, const Stages& range, uint16_t* lds, Accumulators& acc) {
+  const int wave = wave_index(), lane = threadIdx.x % 64;
+#pragma unroll
+  for (int i = 0; i < kDown; ++i) {
+#pragma unroll
+    for (int j = 0; j < kAcross; ++j) acc[i][j] = f32x4{};
+  }
+  const int first = range.first, stages = range.count;
+  const int64_t a0 = static_cast<int64_t>(tile.a) * (PAIRED ? kTile / 2 : kTile), b0 = static_cast<int64_t>(tile.b) * kTile;
+  Loader<A_ROWS, PAIRED> load_a;
+  Loader<B_ROWS> load_b;
+  load_a.init(p.a, a0, wave, lane);
+  load_b.init(p.b, b0, wave, lane);
+  // bytes from the operand's start to the tile, and from a stage to the next
+  const int64_t origin_a = (A_ROWS ? a0 * p.a.ld : a0) * 2, origin_b = (B_ROWS ? b0 * p.b.ld : b0) * 2;
+  const int64_t next_a = (A_ROWS ? 1 : p.a.ld) * kDepth * 2, next_b = (B_ROWS ? 1 : p.b.ld) * kDepth * 2;
+  int segment = 0, stage = 0;  // of the next load
+  // one scalar base per half stage and 32-bit offsets
+  const auto base_a = [&] {
+    return scalar(reinterpret_cast<const char*>(p.a.part[part_of_a<SEGMENTS>(segment)]) + origin_a + (first + stage) * next_a);
+  };
+  const auto base_b = [&] {
+    return scalar(reinterpret_cast<const char*>(p.b.part[part_of_b<SEGMENTS>(segment)]) + origin_b + (first + stage) * next_b);
+  };
+  // k's left in a column operand from this stage on, less one
+  const auto left = [&](const Operand& o) {
+    return __builtin_amdgcn_readfirstlane(static_cast<int>(o.depth - 1 - static_cast<int64_t>(first + stage) * kDepth));
+  };
+  const auto loaded = [&] {
+    if (++stage == stages) stage = 0, ++segment;
+  };
+  const uint32_t lds0 = lds_byte(lds);
+  const auto buffer = [&](int s) { return lds0 + (s % kStages) * (2 * kOperand * 2); };
+  constexpr uint32_t kB = kOperand * 2;  // B's operand in a stage, bytes
+  const uint32_t slot = wave * (kLoads * 1024);
+  Reader<A_ROWS> read_a;
+  Reader<B_ROWS> read_b;
+  read_a.init((wave % 2) * 128, lane);
+  read_b.init((wave / 2) * (16 * kAcross), lane);
+  // A stage in two steps, the upper and the lower half of A's fragments, with all of B's.
+  constexpr int kHalf = kDown / 2;
+  using FragmentsA = s16x8[kHalf];
+  using FragmentsB = s16x8[kAcross];
+  // One step: the matrix instructions on (a, b), between them the reads of the next step's fragments, in the
+  // order of their use, and the loads.
+  const auto step = [&](auto lower, const FragmentsA& a, const FragmentsB& b, auto read, auto load) {
+    constexpr int kFirst = decltype(lower)::value ? kHalf : 0;
+#pragma unroll
+    for (int m = 0; m < kHalf * kAcross; ++m) {
+      f32x4& c = acc[kFirst + m / kAcross][m % kAcross];
+      c = mfma<T>(a[m / kAcross], b[m % kAcross], c);
+      if (m % 2 == 0) read(m / 2);
+      if (m % 8 == 1) load(m / 8);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  FragmentsA upper, lower;
+  FragmentsB b_even, b_odd;  // of even and odd stages
+  // Reads of a step, eight at most: the lower half of the stage, or the next stage's upper half and B.
+  const auto read_lower = [&](uint32_t from) {
+    return [&, from](int r) {
+      if (r < kHalf) lower[r] = read_a.read(from, kHalf + r);
+    };
+  };
+  const auto read_next = [&](uint32_t from, FragmentsB& b) {
+    return [&, from](int r) {
+      if (r == 0) upper[0] = read_a.read(from, 0);
+      else if (r <= kAcross) b[r - 1] = read_b.read(from + kB, r - 1);
+      else upper[r - kAcross] = read_a.read(from, r - kAcross);
+    };
+  };
+  static_assert(kHalf + kAcross == 8 && kHalf * kAcross == 16, "eight reads, one per two matrix instructions");
+  const auto nothing = [](int) {};
+  const int total = stages * SEGMENTS;
+  uint32_t at[kLoads];
+  for (int s = 0; s < kStages && s < total; ++s) {
+    const char *a = base_a(), *b = base_b();
+    load_a.offsets(p.a, left(p.a), at);
+    for (int j = 0; j < kLoads; ++j) load_lds(a, at[j], buffer(s) + slot + j * 1024);
+    load_b.offsets(p.b, left(p.b), at);
+    for (int j = 0; j < kLoads; ++j) load_lds(b, at[j], buffer(s) + kB + slot + j * 1024);
+    loaded();
+  }
+  landed(total >= kStages);
+  const auto read_first = read_next(lds0, b_even);
+#pragma unroll
+  for (int r = 0; r < 8; ++r) read_first(r);
+  step(std::false_type{}, upper, b_even, read_lower(lds0), nothing);
+  landed(total >= kStages);
+  // A stage's lower step and the next one's upper step make a trip.  Loads go to the buffer whose stage is
+  // finished but for fragments in registers: every wavefront has passed landed() since it read them.
+  int s = 1;
+  const auto trip = [&](FragmentsB& now, FragmentsB& next) {
+    const uint32_t to = buffer(s + kStages - 1) + slot;
+    const char* a = base_a();
+    load_a.offsets(p.a, left(p.a), at);
+    step(std::true_type{}, lower, now, read_next(buffer(s), next), [&](int j) { load_lds(a, at[j], to + j * 1024); });
+    const char* b = base_b();
+    load_b.offsets(p.b, left(p.b), at);
+    step(std::false_type{}, upper, next, read_lower(buffer(s)), [&](int j) { load_lds(b, at[j], to + kB + j * 1024); });
+    loaded();
+    landed(true);
+    ++s;
+  };
+  const auto last_trip = [&](FragmentsB& now, FragmentsB& next) {  // nothing more to load
+    step(std::true_type{}, lower, now, read_next(buffer(s), next), nothing);
+    step(std::false_type{}, upper, next, read_lower(buffer(s)), nothing);
+    landed(false);
+    ++s;
+  };
+  while (s + kStages < total) {
+    trip(b_even, b_odd);
+    trip(b_odd, b_even);
+  }
+  // fewer than two trips with loads are left, then those without; after an odd number B's fragments change
+  // their registers
+  const auto swap = [&] {
+#pragma unroll
+    for (int j = 0; j < kAcross; ++j) b_even[j] = b_odd[j];
+  };
+  if (s + kStages - 1 < total) {
+    trip(b_even, b_odd);
+    swap();
+  }
+  while (s < total) {
+    last_trip(b_even, b_odd);
+    swap();
+  }
+  step(std::true_type{}, lower, b_even, nothing, nothing);
+  __syncthreads();  // LDS is free for the epilogue
+}
+
+// 16-byte slot of a staged output row of 512 bytes: a permutation per row, so that 32 lanes
+// writing one chunk of 32 rows meet 32 different slots.
+__device__ __forceinline__ int staged(int row, int chunk) { return row * 32 + (chunk ^ (row & 31)); }
+
+constexpr int kUnits = 256;  // compute units, one workgroup each
+
+// How many parts the depth of a gradient product is cut into, so that its workgroups fill the chip: what takes the
+// least time at 1.1 PFLOP/s for full rounds of workgroups and 4.5 TB/s for the FP32 partial sums that are
+// written and read again (both as measured).  `direct`: one part needs no partial sums.  A part keeps at least 8 stages.
+inline int choose_splits(int64_t tiles, int64_t depth, int segments, bool direct) {
+  int best = 1;
+  double best_time = 0.0;
+  for (int s = 1; s <= 32; ++s) {
+    if (s > 1 && depth / kDepth / s < 8) break;
+    const int64_t rounds = (tiles * s + kUnits - 1) / kUnits;
+    const double tile = 2.0 * kTile * kTile * static_cast<double>(depth) * segments / s / (1.1e15 / kUnits);
+    const double partial = s == 1 && direct ? 0.0 : 8.0 * kTile * kTile * static_cast<double>(tiles) * s / 4.5e12;
+    const double time = static_cast<double>(rounds) * tile + partial;
+    if (s == 1 || time < best_time) best = s, best_time = time;
+  }
+  return best;
+}
+
+}  // namespace layers
+}  // namespace attnres_hip
+
+#endif  // ATTNRES_PRODUCT_H

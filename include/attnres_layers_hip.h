@@ -1,6 +1,6 @@
 /* attnres_layers_hip.h - C ABI of the layers around the residual reads:
- * layer norm, embedding and the softmax cross entropy over a vocabulary, each
- * forward and backward, as gfx950 HIP kernels.  Part of libattnres_hip.so.
+ * layer norm, embedding, the softmax cross entropy over a vocabulary and the gated
+ * feed-forward block, each forward and backward, as gfx950 HIP kernels.  Part of libattnres_hip.so.
  *
  * Contract, as in attnres_hip.h: device pointers; sizes and strides in
  * elements; the stream is passed explicitly (NULL: the legacy stream); the
@@ -106,6 +106,35 @@ int attnres_hip_loss_backward(const void* hidden, int64_t hidden_stride, const v
                               int64_t rows, int64_t vocab, int64_t width, int dtype, int reduction, int keep, const void* saved,
                               const float* grad_loss, void* grad_hidden, void* grad_weight, void* workspace,
                               int64_t workspace_bytes, void* stream);
+
+/* ---- gated feed-forward block ----
+ * out = (act(x Wg^T) * (x Wu^T)) Wd^T.  x [rows, width] (rows x_stride apart), gate_up [2 hidden, width]: Wg's
+ * rows, then Wu's (gate_up_stride apart), down [out_width, hidden] (down_stride apart), out [rows, out_width]
+ * contiguous, all of one dtype; 1 <= width, out_width <= ATTNRES_MAX_WIDTH, 1 <= hidden <= 2^16, rows up to 2^24 and
+ * rows and hidden up to 2^22 tiles of 256 x 128 together.  Operands of 16 bits whose widths are multiples of 32 are
+ * multiplied where they lie: their rows start at multiples of 16 bytes, at most 2^22 elements apart, and hidden *
+ * gate_up_stride is at most 2^30 (else ATTNRES_ERR_STRIDE).
+ * saved: NULL, or what the backward reads (g = x Wg^T and u = x Wu^T in FP32, of 16-bit inputs cut to 24 bits).
+ * workspace: backward 0 for the forward's, 1 for the backward's, 2 for that of a backward without saved, which forms
+ * g and u again.  saved and workspace start at multiples of 16 bytes (else ATTNRES_ERR_WORKSPACE). */
+enum attnres_activation { ATTNRES_SILU = 0, ATTNRES_GELU = 1 };
+
+int64_t attnres_hip_gated_ffn_saved_bytes(int64_t rows, int64_t width, int64_t hidden, int64_t out_width, int dtype);
+int64_t attnres_hip_gated_ffn_workspace_bytes(int64_t rows, int64_t width, int64_t hidden, int64_t out_width, int dtype,
+                                              int backward);
+
+int attnres_hip_gated_ffn_forward(const void* x, int64_t x_stride, const void* gate_up, int64_t gate_up_stride,
+                                  const void* down, int64_t down_stride, int64_t rows, int64_t width, int64_t hidden,
+                                  int64_t out_width, int dtype, int activation, void* out, void* saved, void* workspace,
+                                  int64_t workspace_bytes, void* stream);
+
+/* grad_out [rows, out_width] contiguous; grad_x [rows, width], grad_gate_up [2 hidden, width] and grad_down
+ * [out_width, hidden] contiguous, of dtype; each may be NULL when it is not wanted.  rows >= 1. */
+int attnres_hip_gated_ffn_backward(const void* grad_out, const void* x, int64_t x_stride, const void* gate_up,
+                                   int64_t gate_up_stride, const void* down, int64_t down_stride, int64_t rows,
+                                   int64_t width, int64_t hidden, int64_t out_width, int dtype, int activation,
+                                   const void* saved, void* grad_x, void* grad_gate_up, void* grad_down, void* workspace,
+                                   int64_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }
