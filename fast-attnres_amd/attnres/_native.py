@@ -1,5 +1,6 @@
-"""ctypes binding of the C ABI in `include/attnres_hip.h` and
-`include/attnres_layers_hip.h`, and the loader of the eager autograd nodes.
+"""ctypes binding of the C ABI in `include/attnres_hip.h`,
+`include/attnres_layers_hip.h` and `include/attnres_optim_hip.h`, and the loader of
+the eager autograd nodes.
 
 The shared library `_lib/libattnres_hip.so` is built in-tree from
 `csrc/attnres_hip.hip` by `build_native.py` (hipcc, gfx950), and so is
@@ -33,6 +34,7 @@ ERR_LAUNCH = 6
 _c_void_p = ctypes.c_void_p
 _i64 = ctypes.c_int64
 _f32 = ctypes.c_float
+_f64 = ctypes.c_double
 
 # name -> (restype, argtypes); one entry per declaration in attnres_hip.h.
 SIGNATURES = {
@@ -126,6 +128,21 @@ LAYER_SIGNATURES = {
         _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _i64, _c_void_p]),
 }
 
+# The optimizer step's (attnres_optim_hip.h), likewise.
+OPTIM_SIGNATURES = {
+    "attnres_hip_adamw": (ctypes.c_int, [
+        _c_void_p, _i64, ctypes.c_int, ctypes.c_int, ctypes.c_int, _f64, _c_void_p, _f64, _f64, _f64, _f64, _i64, _c_void_p,
+        _c_void_p, _c_void_p]),
+}
+
+
+class AdamwTensor(ctypes.Structure):
+    """`struct attnres_adamw_tensor`."""
+
+    _fields_ = [(name, _c_void_p) for name in ("param", "grad", "exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale",
+                                               "master")] + [("elements", _i64)]
+
+
 _lock = threading.Lock()
 _library: ctypes.CDLL | None = None
 
@@ -146,7 +163,7 @@ def load() -> ctypes.CDLL:
                 library = ctypes.CDLL(str(path))
             except OSError as error:
                 raise RuntimeError(f"attnres HIP extension failed to load: {error}") from error
-            for name, (restype, argtypes) in (*SIGNATURES.items(), *LAYER_SIGNATURES.items()):
+            for name, (restype, argtypes) in (*SIGNATURES.items(), *LAYER_SIGNATURES.items(), *OPTIM_SIGNATURES.items()):
                 function = getattr(library, name)
                 function.restype = restype
                 function.argtypes = argtypes
@@ -193,4 +210,5 @@ def check(status: int, what: str) -> None:
     raise RuntimeError(f"{what}: {message} (status {status})")
 
 
-__all__ = ["AUTOGRAD_PATH", "LAYER_SIGNATURES", "LIBRARY_PATH", "SIGNATURES", "check", "load", "load_autograd"]
+__all__ = ["AUTOGRAD_PATH", "AdamwTensor", "LAYER_SIGNATURES", "LIBRARY_PATH", "OPTIM_SIGNATURES", "SIGNATURES", "check", "load",
+           "load_autograd"]

@@ -16,10 +16,12 @@ library:
 * `csrc/attnres_norm.hip`, `attnres_embedding.hip`, `attnres_loss.hip`,
   `attnres_ffn.hip`: the layers around the reads
   (`include/attnres_layers_hip.h`);
+* `csrc/attnres_adamw.hip`: the optimizer step
+  (`include/attnres_optim_hip.h`);
 
 and, against PyTorch's headers and libraries, the eager autograd nodes
-`csrc/attnres_autograd.cpp` and `csrc/attnres_layers_autograd.cpp` ->
-`attnres/_lib/_autograd.so` (host C++, no device code; linked to the library
+`csrc/attnres_autograd.cpp` and `csrc/attnres_layers_autograd.cpp` and the
+optimizer's host side `csrc/attnres_optim.cpp` -> `attnres/_lib/_autograd.so` (host C++, no device code; linked to the library
 above with an `$ORIGIN` run path).
 
 Packed-FP32 VALU ops are disabled (``-target-feature -packed-fp32-ops``); the
@@ -56,10 +58,10 @@ GEOMETRIES = ((16, 1), (32, 1), (32, 2), (32, 3), (32, 4), (64, 3), (64, 4), (64
 # launch_fwd)
 SPLIT_GEOMETRIES = {(64, 8): ["-mllvm", "-amdgpu-sched-strategy=iterative-minreg"]}
 FLAGS = ["-O3", "-std=c++17", "-fPIC", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
-AUTOGRAD_SOURCES = (CSRC / "attnres_autograd.cpp", CSRC / "attnres_layers_autograd.cpp")
+AUTOGRAD_SOURCES = (CSRC / "attnres_autograd.cpp", CSRC / "attnres_layers_autograd.cpp", CSRC / "attnres_optim.cpp")
 AUTOGRAD_OBJECTS = tuple(BUILD_DIR / f"{source.stem}.o" for source in AUTOGRAD_SOURCES)
-# the layers around the reads, one unit each
-LAYER_UNITS = ("attnres_norm", "attnres_embedding", "attnres_loss", "attnres_ffn")
+# the layers around the reads and the optimizer step, one unit each
+LAYER_UNITS = ("attnres_norm", "attnres_embedding", "attnres_loss", "attnres_ffn", "attnres_adamw")
 AUTOGRAD_OUTPUT = HERE / "attnres" / "_lib" / "_autograd.so"
 ROCM_INCLUDE = Path(os.environ.get("ROCM_PATH", "/opt/rocm")) / "include"
 

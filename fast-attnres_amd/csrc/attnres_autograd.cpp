@@ -789,4 +789,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("bank_read", &bank_read, "read of leading slots and a tail slot (-1: none)");
   m.def("pool_layout", &layout_of, "(head, block, size) of the pooled saved state");
   bind_layers(m);
+  bind_optim(m);
 }

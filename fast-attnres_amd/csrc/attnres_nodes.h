@@ -1,6 +1,7 @@
 // attnres_nodes.h - what the eager autograd nodes share: errors, streams and row
 // layouts (attnres_autograd.cpp: the reads and the source bank;
-// attnres_layers_autograd.cpp: the layers around them).
+// attnres_layers_autograd.cpp: the layers around them; attnres_optim.cpp: the optimizer
+// step).
 #ifndef ATTNRES_NODES_H
 #define ATTNRES_NODES_H
 
@@ -78,6 +79,9 @@ inline int64_t rows_of(const Tensor& tensor) { return tensor.dim() > 1 ? tensor.
 
 // Registers the layers' functions in the extension module.
 void bind_layers(pybind11::module_& m);
+
+// And the optimizer step.
+void bind_optim(pybind11::module_& m);
 
 }  // namespace attnres_nodes
 
