@@ -413,6 +413,152 @@ __global__ void __launch_bounds__(kBlock) attnres_ffn_pack_kernel(PackArgs<X> g)
   }
 }
 
+// ------------------------------------------------------------------- few rows
+// The forward of up to kFewRows rows reads the weights once and is bound by that: wavefronts share the depth of 16
+// entries of A (of a gate's 8 and the up projection's 8 that belong to them), so that all of a workgroup's weights are asked
+// for at once, and no operand is packed.  FP32 inputs by FP32 matrix instructions, which so few rows have time for.
+constexpr int64_t kFewRows = 64;
+
+// The wavefronts' sums over their shares of the depth, in LDS; ROWS of a's tiles by TILES of the rows'.
+template <class X, int WAVES, int ATILES, int TILES>
+__device__ __forceinline__ void few_product(const X* const (&a)[ATILES], const X* const (&b)[TILES], int depth,
+                                            f32x4 (*parts)[ATILES][TILES][64]) {
+  const int wave = wave_index(), lane = threadIdx.x % 64, group = lane / 16;
+  constexpr int kSteps = sizeof(X) == 4 || ATILES * TILES > 2 ? 1 : 2;  // of 64 k's under way together
+  constexpr int kSpan = kSteps * 64;
+  FewChunk<X> next[kSteps][ATILES];
+  const auto fetch = [&](int k0) {
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+#pragma unroll
+      for (int i = 0; i < ATILES; ++i) next[s][i].load(a[i], k0 + s * 64, group, depth);
+    }
+  };
+  f32x4 acc[ATILES][TILES] = {};
+  if (wave * kSpan < depth) fetch(wave * kSpan);
+  for (int k0 = wave * kSpan; k0 < depth; k0 += WAVES * kSpan) {
+    FewChunk<X> now[kSteps][ATILES];
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+#pragma unroll
+      for (int i = 0; i < ATILES; ++i) now[s][i] = next[s][i];
+    }
+    if (k0 + WAVES * kSpan < depth) fetch(k0 + WAVES * kSpan);
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+#pragma unroll
+      for (int t = 0; t < TILES; ++t) {
+        FewChunk<X> x;  // the few rows stay in the caches
+        x.load(b[t], k0 + s * 64, group, depth);
+#pragma unroll
+        for (int i = 0; i < ATILES; ++i) acc[i][t] = few_mfma<X>(now[s][i], x, acc[i][t]);
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < ATILES; ++i) {
+#pragma unroll
+    for (int t = 0; t < TILES; ++t) parts[wave][i][t][lane] = acc[i][t];
+  }
+  __syncthreads();
+}
+
+template <class X, int WAVES, int ATILES, int TILES>
+__device__ __forceinline__ f32x4 few_sum(const f32x4 (*parts)[ATILES][TILES][64], int i, int t, int lane) {
+  f32x4 sum = parts[0][i][t][lane];
+#pragma unroll
+  for (int w = 1; w < WAVES; ++w) sum += parts[w][i][t][lane];
+  return sum;
+}
+
+template <class X>
+struct FewGateArgs {
+  const X* x;
+  const X* gate_up;
+  int64_t x_stride, gate_up_stride;
+  int rows, width, hidden, hidden_pad, activation;
+  char* saved;  // or nullptr
+  X* out;       // a [rows][hidden_pad], or nullptr
+};
+
+template <class T>
+__device__ __forceinline__ void store_quad(T* to, int left, const float* x) {
+  T v[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) v[e] = from_f32<T>(x[e]);
+  if (left >= 4) {
+    __builtin_memcpy(to, v, sizeof(v));
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if (e < left) to[e] = v[e];
+    }
+  }
+}
+
+template <class X, int WAVES, int ATILES, int TILES>
+__global__ void __launch_bounds__(64 * WAVES) attnres_ffn_few_gate_kernel(FewGateArgs<X> g) {
+  __shared__ f32x4 parts[WAVES][ATILES][TILES][64];
+  const int entry = threadIdx.x % 16;
+  const int f0 = static_cast<int>(blockIdx.x) * (8 * ATILES);
+  const X* a[ATILES];
+  const X* b[TILES];
+#pragma unroll
+  for (int i = 0; i < ATILES; ++i) {
+    const int64_t f = min(f0 + i * 8 + entry % 8, g.hidden - 1);
+    a[i] = g.gate_up + (f + (entry < 8 ? 0 : g.hidden)) * g.gate_up_stride;
+  }
+#pragma unroll
+  for (int t = 0; t < TILES; ++t) b[t] = g.x + min(t * 16 + entry, g.rows - 1) * g.x_stride;
+  few_product<X, WAVES, ATILES, TILES>(a, b, g.width, parts);
+  // a thread per row and four hidden entries: lanes 0..31 hold a tile's gates, 32..63 what belongs to them
+  for (int k = threadIdx.x; k < ATILES * TILES * 32; k += 64 * WAVES) {
+    const int i = k / (TILES * 32), t = k / 32 % TILES, lane = k % 32;
+    const int row = t * 16 + lane % 16, f = f0 + i * 8 + lane / 16 * 4;
+    if (row >= g.rows || f >= g.hidden) continue;
+    const f32x4 gate = few_sum<X, WAVES, ATILES, TILES>(parts, i, t, lane), up = few_sum<X, WAVES, ATILES, TILES>(parts, i, t, lane + 32);
+    if (g.saved != nullptr) {
+      const int64_t sub = static_cast<int64_t>(row / kSub) * (g.hidden_pad / kSub) + f / kSub;
+      save_pair<X>(g.saved + sub * kSubBytes<X>, f % kSub / 4 * 16 + row % kSub, gate, up);
+    }
+    if (g.out != nullptr) {
+      float x[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] = activate<X, false>(gate[e], g.activation).value * up[e];
+      store_quad(g.out + static_cast<int64_t>(row) * g.hidden_pad + f, g.hidden - f, x);
+    }
+  }
+}
+
+template <class X>
+struct FewOutArgs {
+  const X* a;
+  const X* down;
+  int64_t a_stride, down_stride;
+  int rows, hidden, out_width;
+  X* out;
+};
+
+template <class X, int WAVES, int TILES>
+__global__ void __launch_bounds__(64 * WAVES) attnres_ffn_few_out_kernel(FewOutArgs<X> g) {
+  __shared__ f32x4 parts[WAVES][1][TILES][64];
+  const int entry = threadIdx.x % 16;
+  const int e0 = static_cast<int>(blockIdx.x) * 16;
+  const X* const a[1] = {g.down + min(e0 + entry, g.out_width - 1) * g.down_stride};
+  const X* b[TILES];
+#pragma unroll
+  for (int t = 0; t < TILES; ++t) b[t] = g.a + min(t * 16 + entry, g.rows - 1) * g.a_stride;
+  few_product<X, WAVES, 1, TILES>(a, b, g.hidden, parts);
+  for (int k = threadIdx.x; k < TILES * 64; k += 64 * WAVES) {
+    const int t = k / 64, lane = k % 64;
+    const int row = t * 16 + lane % 16, e = e0 + lane / 16 * 4;
+    if (row >= g.rows || e >= g.out_width) continue;
+    const f32x4 sum = few_sum<X, WAVES, 1, TILES>(parts, 0, t, lane);
+    const float x[4] = {sum[0], sum[1], sum[2], sum[3]};
+    store_quad(g.out + static_cast<int64_t>(row) * g.out_width + e, g.out_width - e, x);
+  }
+}
+
 // ---------------------------------------------------------------------- host
 
 constexpr int64_t kMaxRows = int64_t{1} << 24;
@@ -430,6 +576,7 @@ struct Sizes {
 
 struct FfnPlan {
   int parts, segments;
+  bool few;
   int64_t rows_pad, width_pad, hidden_pad, out_pad;
   bool pack_x, pack_gate_up, pack_down, pack_grad;
   int64_t x[3], gate_up[3], down[3], grad[3], a[3], both[3];  // offsets
@@ -450,9 +597,11 @@ FfnPlan ffn_plan(const Sizes& s, int pass) {
   p.hidden_pad = round_up(s.hidden, kDepth);
   p.out_pad = round_up(s.out_width, kDepth);
   // the depth of a product is a whole number of stages, the rest of the last one zeros
-  p.pack_x = split || s.width != p.width_pad || (backward && s.rows != p.rows_pad);
-  p.pack_gate_up = split || s.width != p.width_pad || s.hidden != p.hidden_pad;
-  p.pack_down = split || s.hidden != p.hidden_pad || (backward && s.out_width != p.out_pad);
+  p.few = s.rows <= kFewRows;
+  const bool tiles = backward || !p.few;
+  p.pack_x = tiles && (split || s.width != p.width_pad || (backward && s.rows != p.rows_pad));
+  p.pack_gate_up = tiles && (split || s.width != p.width_pad || s.hidden != p.hidden_pad);
+  p.pack_down = tiles && (split || s.hidden != p.hidden_pad || (backward && s.out_width != p.out_pad));
   p.pack_grad = backward && (split || s.out_width != p.out_pad || s.rows != p.rows_pad);
   p.saved_bytes = tiles_of(s.rows, kSub) * (p.hidden_pad / kSub) * (split ? kSubBytes<float> : kSubBytes<Bf16>);
   int64_t at = 0;
@@ -466,9 +615,10 @@ FfnPlan ffn_plan(const Sizes& s, int pass) {
     if (p.pack_gate_up) p.gate_up[k] = take(4 * p.hidden_pad * p.width_pad);
     if (p.pack_down) p.down[k] = take(2 * p.out_pad * p.hidden_pad);
     if (p.pack_grad) p.grad[k] = take(2 * p.rows_pad * p.out_pad);
-    p.a[k] = take(2 * p.rows_pad * p.hidden_pad);
+    if (tiles) p.a[k] = take(2 * p.rows_pad * p.hidden_pad);
     if (backward) p.both[k] = take(4 * p.rows_pad * p.hidden_pad);
   }
+  if (!tiles) p.a[0] = take(s.rows * p.hidden_pad * dtype_size(s.dtype));
   if (pass == kBackwardAgain) p.saved = take(p.saved_bytes);
   int64_t partial = 0;
   const auto splits = [&](int64_t entries_a, int64_t entries_b, int64_t depth) {
@@ -477,7 +627,8 @@ FfnPlan ffn_plan(const Sizes& s, int pass) {
     if (n > 1) partial = std::max(partial, 4 * n * entries_b * round_up(entries_a, kVec));
     return n;
   };
-  if (!backward) {
+  if (!tiles) {
+  } else if (!backward) {
     p.splits_out = splits(s.out_width, s.rows, p.hidden_pad);
   } else {
     p.splits_x = splits(s.width, s.rows, 2 * p.hidden_pad);
@@ -556,6 +707,32 @@ void launch_gate(const Call& c, const Operand& x, const Operand& gate_up, char* 
   hipLaunchKernelGGL((attnres_ffn_gate_kernel<X>), dim3(g.product.tiles_a * g.product.tiles_b), dim3(kThreads), 0, c.stream, g);
 }
 
+// Of few rows: g and u, and a from them.
+template <class X>
+void launch_few_gate(const Call& c, char* saved, X* a) {
+  const FewGateArgs<X> g{static_cast<const X*>(c.x), static_cast<const X*>(c.gate_up), c.x_stride, c.gate_up_stride,
+                         static_cast<int>(c.s.rows), static_cast<int>(c.s.width), static_cast<int>(c.s.hidden),
+                         static_cast<int>(c.plan.hidden_pad), c.activation, saved, a};
+  const auto launch = [&](auto kernel, int waves, int tiles) {
+    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(tiles_of(c.s.hidden, 8 * tiles))), dim3(64 * waves), 0, c.stream, g);
+  };
+  if (c.s.rows <= 16) launch(attnres_ffn_few_gate_kernel<X, 8, 1, 1>, 8, 1);
+  else if (c.s.rows <= 32) launch(attnres_ffn_few_gate_kernel<X, 8, 2, 2>, 8, 2);
+  else launch(attnres_ffn_few_gate_kernel<X, 8, 2, 4>, 8, 2);
+}
+
+template <class X>
+void few_forward(const Call& c, void* out, char* saved) {
+  X* a = reinterpret_cast<X*>(c.workspace + c.plan.a[0]);
+  launch_few_gate<X>(c, saved, a);
+  const FewOutArgs<X> g{a, static_cast<const X*>(c.down), c.plan.hidden_pad, c.down_stride, static_cast<int>(c.s.rows),
+                        static_cast<int>(c.s.hidden), static_cast<int>(c.s.out_width), static_cast<X*>(out)};
+  const auto kernel = c.s.rows <= 16   ? attnres_ffn_few_out_kernel<X, 16, 1>
+                      : c.s.rows <= 32 ? attnres_ffn_few_out_kernel<X, 16, 2>
+                                       : attnres_ffn_few_out_kernel<X, 16, 4>;
+  hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(tiles_of(c.s.out_width, 16))), dim3(1024), 0, c.stream, g);
+}
+
 // out[b][a], by halves of B's entries; joined where the depth is cut.
 template <class X, bool A_ROWS, bool B_ROWS>
 void launch_out(const Call& c, const Operand& a, const Operand& b, int64_t depth, int64_t entries_a, int64_t half, int64_t half_pad,
@@ -587,6 +764,7 @@ void launch_out(const Call& c, const Operand& a, const Operand& b, int64_t depth
 template <class X>
 void ffn_forward(const Call& c, void* out, char* saved) {
   const FfnPlan& p = c.plan;
+  if (p.few) return few_forward<X>(c, out, saved);
   launch_gate<X>(c, place_x<X>(c), place_gate_up<X>(c), saved, p.a);
   Operand down = place_down<X>(c), a{};
   down.entries = c.s.out_width;
@@ -600,12 +778,14 @@ template <class X>
 void ffn_backward(const Call& c, const void* grad_out, const char* saved, void* grad_x, void* grad_gate_up, void* grad_down) {
   const FfnPlan& p = c.plan;
   Operand x{}, gate_up{};
-  if (saved == nullptr || grad_gate_up != nullptr) x = place_x<X>(c);
-  if (saved == nullptr || grad_x != nullptr) gate_up = place_gate_up<X>(c);
+  const bool again = saved == nullptr && !p.few;
+  if (again || grad_gate_up != nullptr) x = place_x<X>(c);
+  if (again || grad_x != nullptr) gate_up = place_gate_up<X>(c);
   if (saved == nullptr) {
-    char* again = c.workspace + p.saved;
-    launch_gate<X>(c, x, gate_up, again, nullptr);
-    saved = again;
+    char* formed = c.workspace + p.saved;
+    if (p.few) launch_few_gate<X>(c, formed, nullptr);
+    else launch_gate<X>(c, x, gate_up, formed, nullptr);
+    saved = formed;
   }
   const Operand grad = place_operand<X>(c, p.pack_grad, p.grad, grad_out, c.s.out_width, c.s.rows, p.rows_pad, p.rows_pad,
                                         c.s.out_width, p.out_pad);
@@ -691,12 +871,14 @@ int check_rows(const char* name, const void* x, int64_t stride, bool in_place, i
 
 int check_call(const Call& c, const void* saved, int64_t workspace_bytes) {
   const FfnPlan& p = c.plan;
-  if (const int status = check_rows("x", c.x, c.x_stride, !p.pack_x, 0, kMaxStride)) return status;
-  if (const int status = check_rows("gate_up", c.gate_up, c.gate_up_stride, !p.pack_gate_up, c.s.width,
+  const bool half = c.s.dtype != ATTNRES_F32, even = c.s.hidden == p.hidden_pad;
+  const bool wide = half && c.s.width == p.width_pad;
+  if (const int status = check_rows("x", c.x, c.x_stride, wide, 0, kMaxStride)) return status;
+  if (const int status = check_rows("gate_up", c.gate_up, c.gate_up_stride, wide && even, c.s.width,
                                     std::min(kMaxStride, kMaxSecond / c.s.hidden))) {
     return status;
   }
-  if (const int status = check_rows("down", c.down, c.down_stride, !p.pack_down, c.s.hidden, kMaxStride)) return status;
+  if (const int status = check_rows("down", c.down, c.down_stride, half && even, c.s.hidden, kMaxStride)) return status;
   if (c.workspace == nullptr || workspace_bytes < p.bytes) {
     return layer_error(ATTNRES_ERR_WORKSPACE, "workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)p.bytes);
   }

@@ -360,6 +360,54 @@ __device__ __forceinline__ void multiply(const Product& p, const TileAt& tile, c
   __syncthreads();  // LDS is free for the epilogue
 }
 
+// ------------------------------------------------------------- few rows
+// Operands that go straight to registers as they lie (any width and alignment): a lane holds 16 bytes of every 64 of its
+// row; the order of the k's in a matrix instruction is of no account, as both operands share it.
+
+template <class X>
+struct FewChunk {  // a lane's 16 of 64 k's, as they lie: 16 bytes of every 64
+  static constexpr int kPieces = sizeof(X);
+  static constexpr int kPiece = 16 / sizeof(X);
+  u32x4 w[kPieces];
+  __device__ __forceinline__ void load(const X* row, int k0, int group, int width) {
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) {
+      const int k = k0 + (i * 4 + group) * kPiece;
+      if (k + kPiece <= width) {
+        w[i] = reinterpret_cast<const Raw16*>(row + k)->v;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if constexpr (std::is_same_v<X, float>) {
+            w[i][e] = k + e < width ? __float_as_uint(row[k + e]) : 0;
+          } else {
+            const uint32_t lo = k + 2 * e < width ? row[k + 2 * e].bits : 0;
+            const uint32_t hi = k + 2 * e + 1 < width ? row[k + 2 * e + 1].bits : 0;
+            w[i][e] = hi << 16 | lo;
+          }
+        }
+      }
+    }
+  }
+};
+
+template <class X>
+__device__ __forceinline__ f32x4 few_mfma(const FewChunk<X>& a, const FewChunk<X>& b, f32x4 c) {
+  if constexpr (std::is_same_v<X, float>) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a.w[i][e]), __uint_as_float(b.w[i][e]), c, 0, 0, 0);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) c = mfma<X>(__builtin_bit_cast(s16x8, a.w[i]), __builtin_bit_cast(s16x8, b.w[i]), c);
+  }
+  return c;
+}
+
 // 16-byte slot of a staged output row of 512 bytes: a permutation per row, so that 32 lanes
 // writing one chunk of 32 rows meet 32 different slots.
 __device__ __forceinline__ int staged(int row, int chunk) { return row * 32 + (chunk ^ (row & 31)); }
