@@ -26,7 +26,6 @@ namespace attnres_hip {
 namespace layers {
 namespace {
 
-constexpr int kPairTile = kTile / 2;  // hidden entries of a tile of g and u
 constexpr int kSub = 16;              // rows and columns of a subtile of saved g and u
 
 template <class X>
@@ -144,16 +143,18 @@ struct GateArgs {
   uint16_t* out[3]; // a [rows][hidden_pad], zeros past hidden; or nullptr
 };
 
-template <class X>
-__global__ void __launch_bounds__(kThreads) attnres_ffn_gate_kernel(GateArgs g) {
+template <class X, int TILE>
+__global__ void __launch_bounds__(Shape<TILE>::kThreadsOf, Shape<TILE>::kGroupsOf) attnres_ffn_gate_kernel(GateArgs g) {
   using T = Part<X>;
-  __shared__ __align__(16) uint16_t lds[kStages * 2 * kOperand];
+  using S = Shape<TILE>;
+  constexpr int kDown = S::kDownOf, kAcross = S::kAcrossOf;
+  __shared__ __align__(16) uint16_t lds[S::kLds];
   TileAt tile;
   if (!tile_at(g.product, g.product.tiles_b, &tile)) return;
-  Accumulators acc;
-  multiply<T, kSegments<X>, true, true, true>(g.product, tile, stages_of(g.product, 0), lds, acc);
+  typename S::Sums acc;
+  multiply_tile<TILE, T, kSegments<X>, true, true, true>(g.product, tile, stages_of(g.product, 0), lds, acc);
   const int wave = wave_index(), lane = threadIdx.x % 64;
-  const int64_t f0 = static_cast<int64_t>(tile.a) * kPairTile, n0 = static_cast<int64_t>(tile.b) * kTile;
+  const int64_t f0 = static_cast<int64_t>(tile.a) * (TILE / 2), n0 = static_cast<int64_t>(tile.b) * TILE;
   const int64_t sub_f = g.hidden_pad / kSub, sub_n = (g.rows + kSub - 1) / kSub;
 #pragma unroll
   for (int j = 0; j < kAcross; ++j) {
@@ -174,8 +175,7 @@ __global__ void __launch_bounds__(kThreads) attnres_ffn_gate_kernel(GateArgs g) 
     }
   }
   if (g.out[0] == nullptr) return;
-  // rows of 256 bytes in LDS, their 16-byte slots permuted as in staged()
-  const auto slot = [](int row, int chunk) { return row * 16 + (chunk ^ (row & 15)); };
+  constexpr int kChunks = TILE / 16;  // of a row in LDS
 #pragma unroll
   for (int part = 0; part < kParts<X>; ++part) {
 #pragma unroll
@@ -192,17 +192,18 @@ __global__ void __launch_bounds__(kThreads) attnres_ffn_gate_kernel(GateArgs g) 
 #pragma unroll
           for (int e = 0; e < 4; ++e) acc[i][j][e] = x[e];
         }
-        const int chunk = (wave % 2) * 8 + i * 2 + lane / 32;
-        *reinterpret_cast<uint64_t*>(lds + slot(row, chunk) * 8 + (lane / 16 % 2) * 4) =
+        const int chunk = (wave % 2) * kDown + i * 2 + lane / 32;
+        *reinterpret_cast<uint64_t*>(lds + staged<kChunks>(row, chunk) * 8 + (lane / 16 % 2) * 4) =
             static_cast<uint64_t>(packed[1]) << 32 | packed[0];
       }
     }
     __syncthreads();
-    for (int k = threadIdx.x; k < kTile * 16; k += kThreads) {
-      const int row = k / 16, chunk = k % 16;
+    for (int k = threadIdx.x; k < TILE * kChunks; k += S::kThreadsOf) {
+      const int row = k / kChunks, chunk = k % kChunks;
       const int64_t f = f0 + chunk * 8;
       if (n0 + row < g.rows && f < g.hidden_pad) {
-        *reinterpret_cast<u32x4*>(g.out[part] + (n0 + row) * g.hidden_pad + f) = *reinterpret_cast<const u32x4*>(lds + slot(row, chunk) * 8);
+        *reinterpret_cast<u32x4*>(g.out[part] + (n0 + row) * g.hidden_pad + f) =
+            *reinterpret_cast<const u32x4*>(lds + staged<kChunks>(row, chunk) * 8);
       }
     }
     if (part + 1 < kParts<X>) __syncthreads();
@@ -220,72 +221,93 @@ struct SlopeArgs {
   uint16_t* out[3];   // a [rows_pad][hidden_pad], likewise
 };
 
-template <class X>
-__global__ void __launch_bounds__(kThreads) attnres_ffn_slope_kernel(SlopeArgs g) {
+template <class X, int TILE>
+__global__ void __launch_bounds__(Shape<TILE>::kThreadsOf, Shape<TILE>::kGroupsOf) attnres_ffn_slope_kernel(SlopeArgs g) {
   using T = Part<X>;
-  __shared__ __align__(16) uint16_t lds[kStages * 2 * kOperand];
+  using S = Shape<TILE>;
+  constexpr int kDown = S::kDownOf, kAcross = S::kAcrossOf;
+  __shared__ __align__(16) uint16_t lds[S::kLds];
   TileAt tile;
   if (!tile_at(g.product, g.product.tiles_b, &tile)) return;
-  Accumulators acc;
-  multiply<T, kSegments<X>, false, true>(g.product, tile, stages_of(g.product, 0), lds, acc);
+  typename S::Sums acc;
+  multiply_tile<TILE, T, kSegments<X>, false, true>(g.product, tile, stages_of(g.product, 0), lds, acc);
   const int wave = wave_index(), lane = threadIdx.x % 64;
-  const int64_t f0 = static_cast<int64_t>(tile.a) * kTile, n0 = static_cast<int64_t>(tile.b) * kTile;
+  const int64_t f0 = static_cast<int64_t>(tile.a) * TILE, n0 = static_cast<int64_t>(tile.b) * TILE;
   const int64_t sub_f = g.hidden_pad / kSub, sub_n = (g.rows + kSub - 1) / kSub;
-  // A round: 64 rows, 16 of every wavefront, of three planes in LDS: dg, du and a; of FP32 one of them in its three parts.
-  constexpr int kRows = 16 * (kWaves / 2);
-  constexpr int kPlane = kRows * kTile;
+  const int64_t at_f = f0 / kSub + (wave % 2) * kDown, at_n = n0 / kSub + (wave / 2) * kAcross;
+  // The saved pairs of a round; the next one's are loaded while a round is stored.
+  Pair<X> pairs[kDown];
+  const auto load_pairs = [&](int j) {
+    const int64_t n = min(at_n + j, sub_n - 1);  // past the last subtile: the last one's, which are left out
+#pragma unroll
+    for (int i = 0; i < kDown; ++i) pairs[i].load(g.saved + (n * sub_f + min(at_f + i, sub_f - 1)) * kSubBytes<X>, lane);
+  };
+  load_pairs(0);
+  // A round: 16 rows of every wavefront, of three planes in LDS: dg, du and a; of FP32 one of them in its three parts.
+  constexpr int kRows = 16 * (S::kWavesOf / 2), kChunks = TILE / 8;
+  constexpr int kPlane = kRows * TILE;
+  static_assert(3 * kPlane <= S::kLds, "three planes");
   constexpr int kTurns = kParts<X>;
-#pragma unroll
-  for (int j = 0; j < kAcross; ++j) {
-    const int64_t at_n = n0 / kSub + (wave / 2) * kAcross + j;
-    const bool counts = at_n * kSub + lane % 16 < g.rows;
+  const auto round = [&](auto number, auto turn_number) {
+    constexpr int j = decltype(number)::value, turn = decltype(turn_number)::value;
+    const bool counts = (at_n + j) * kSub + lane % 16 < g.rows;
     const int row = (wave / 2) * 16 + lane % 16;
+    if (j + turn > 0) __syncthreads();
 #pragma unroll
-    for (int turn = 0; turn < kTurns; ++turn) {
-      if (j + turn > 0) __syncthreads();
+    for (int i = 0; i < kDown; ++i) {
+      const Pair<X>& pair = pairs[i];
+      float x[3][4];
 #pragma unroll
-      for (int i = 0; i < kDown; ++i) {
-        const int64_t at_f = f0 / kSub + (wave % 2) * kDown + i;
-        Pair<X> pair{};
-        if (at_n < sub_n && at_f < sub_f) pair.load(g.saved + (at_n * sub_f + at_f) * kSubBytes<X>, lane);
-        float x[3][4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const bool inside = counts && at_f * kSub + 4 * (lane / 16) + e < g.hidden;
-          const Activated act = activate<X, true>(pair.gate(e), g.activation);
-          const float da = acc[i][j][e], up = pair.up(e);
-          x[0][e] = inside ? da * up * act.slope : 0.0f;
-          x[1][e] = inside ? da * act.value : 0.0f;
-          x[2][e] = inside ? act.value * up : 0.0f;
-        }
-        const int chunk = (wave % 2) * 16 + i * 2 + lane / 32;
-        uint16_t* to = lds + staged(row, chunk) * 8 + (lane / 16 % 2) * 4;
-#pragma unroll
-        for (int plane = 0; plane < 3; ++plane) {
-          float* value = x[kTurns == 1 ? plane : turn];
-          const uint32_t packed[2] = {pack2<T>(value[0], value[1]), pack2<T>(value[2], value[3])};
-          *reinterpret_cast<uint64_t*>(to + plane * kPlane) = static_cast<uint64_t>(packed[1]) << 32 | packed[0];
-          if constexpr (kTurns > 1) take_part<T>(value, packed, 4);
-        }
-        if (i % 2 == 1) __builtin_amdgcn_sched_barrier(0);
+      for (int e = 0; e < 4; ++e) {
+        const bool inside = counts && (at_f + i) * kSub + 4 * (lane / 16) + e < g.hidden;
+        const Activated act = activate<X, true>(pair.gate(e), g.activation);
+        const float da = acc[i][j][e], up = pair.up(e);
+        x[0][e] = inside ? da * up * act.slope : 0.0f;
+        x[1][e] = inside ? da * act.value : 0.0f;
+        x[2][e] = inside ? act.value * up : 0.0f;
       }
-      __syncthreads();
+      const int chunk = (wave % 2) * (2 * kDown) + i * 2 + lane / 32;
+      uint16_t* to = lds + staged<kChunks>(row, chunk) * 8 + (lane / 16 % 2) * 4;
 #pragma unroll
       for (int plane = 0; plane < 3; ++plane) {
-        const int what = kTurns == 1 ? plane : turn, part = kTurns == 1 ? 0 : plane;
-        uint16_t* out = what == 2 ? g.out[part] : g.both[part];
-        if (out == nullptr) continue;
-        const int64_t ld = what == 2 ? g.hidden_pad : 2 * g.hidden_pad;
-        const int64_t first = what == 1 ? g.hidden_pad : 0;
-        for (int k = threadIdx.x; k < kRows * 32; k += kThreads) {
-          const int r = k / 32, chunk = k % 32;
-          const int64_t n = n0 + r / 16 * (16 * kAcross) + j * 16 + r % 16, f = f0 + chunk * 8;
-          if (n < g.rows_pad && f < g.hidden_pad) {
-            *reinterpret_cast<u32x4*>(out + n * ld + first + f) = *reinterpret_cast<const u32x4*>(lds + plane * kPlane + staged(r, chunk) * 8);
-          }
+        float* value = x[kTurns == 1 ? plane : turn];
+        const uint32_t packed[2] = {pack2<T>(value[0], value[1]), pack2<T>(value[2], value[3])};
+        *reinterpret_cast<uint64_t*>(to + plane * kPlane) = static_cast<uint64_t>(packed[1]) << 32 | packed[0];
+        if constexpr (kTurns > 1) take_part<T>(value, packed, 4);
+      }
+      if (i % 2 == 1) __builtin_amdgcn_sched_barrier(0);
+    }
+    if constexpr (turn + 1 == kTurns && j + 1 < kAcross) load_pairs(j + 1);
+    __syncthreads();
+#pragma unroll
+    for (int plane = 0; plane < 3; ++plane) {
+      const int what = kTurns == 1 ? plane : turn, part = kTurns == 1 ? 0 : plane;
+      uint16_t* out = what == 2 ? g.out[part] : g.both[part];
+      if (out == nullptr) continue;
+      const int64_t ld = what == 2 ? g.hidden_pad : 2 * g.hidden_pad;
+      const int64_t first = what == 1 ? g.hidden_pad : 0;
+      for (int k = threadIdx.x; k < kRows * kChunks; k += S::kThreadsOf) {
+        const int r = k / kChunks, chunk = k % kChunks;
+        const int64_t n = n0 + r / 16 * (16 * kAcross) + j * 16 + r % 16, f = f0 + chunk * 8;
+        if (n < g.rows_pad && f < g.hidden_pad) {
+          *reinterpret_cast<u32x4*>(out + n * ld + first + f) =
+              *reinterpret_cast<const u32x4*>(lds + plane * kPlane + staged<kChunks>(r, chunk) * 8);
         }
       }
     }
+  };
+  const auto turns = [&](auto number) {
+    round(number, std::integral_constant<int, 0>{});
+    if constexpr (kTurns == 3) {
+      round(number, std::integral_constant<int, 1>{});
+      round(number, std::integral_constant<int, 2>{});
+    }
+  };
+  turns(std::integral_constant<int, 0>{});
+  turns(std::integral_constant<int, 1>{});
+  if constexpr (kAcross == 4) {
+    turns(std::integral_constant<int, 2>{});
+    turns(std::integral_constant<int, 3>{});
   }
 }
 
@@ -300,33 +322,31 @@ struct OutArgs {
   int64_t entries_b;
 };
 
-template <class X, class OUT, bool A_ROWS, bool B_ROWS>
-__global__ void __launch_bounds__(kThreads) attnres_ffn_out_kernel(OutArgs g) {
-  __shared__ __align__(16) uint16_t lds[kStages * 2 * kOperand];
-  TileAt tile;
-  if (!tile_at(g.product, g.product.tiles_b, &tile)) return;
-  Accumulators acc;
-  multiply<Part<X>, kSegments<X>, A_ROWS, B_ROWS>(g.product, tile, stages_of(g.product, tile.split), lds, acc);
+// A tile's sums, rounded once or as a part's FP32 sums.
+template <class OUT, int TILE>
+__device__ __forceinline__ void store_tile(const OutArgs& g, const TileAt& tile, const typename Shape<TILE>::Sums& acc, uint16_t* lds) {
+  using S = Shape<TILE>;
   const int wave = wave_index(), lane = threadIdx.x % 64;
   OUT* out = static_cast<OUT*>(g.out) + tile.split * g.split_stride;
-  const int64_t a0 = static_cast<int64_t>(tile.a) * kTile, b0 = static_cast<int64_t>(tile.b) * kTile;
+  const int64_t a0 = static_cast<int64_t>(tile.a) * TILE, b0 = static_cast<int64_t>(tile.b) * TILE;
   constexpr bool kWide = std::is_same_v<OUT, float>;
-  constexpr int kRounds = kWide ? 2 : 1;  // 512-byte rows: 128 FP32 or 256 16-bit outputs
+  constexpr int kRounds = kWide ? 2 : 1;  // rows of 2 TILE bytes in LDS: half of the FP32 outputs, or all 16-bit ones
+  constexpr int kChunks = TILE / 8;
   constexpr int kChunk = kWide ? 4 : 8;   // outputs per 16 bytes
 #pragma unroll
   for (int round = 0; round < kRounds; ++round) {
     if (!kWide || wave % 2 == round) {
 #pragma unroll
-      for (int j = 0; j < kAcross; ++j) {
-        const int column = (wave / 2) * (16 * kAcross) + j * 16 + lane % 16;
+      for (int j = 0; j < S::kAcrossOf; ++j) {
+        const int column = (wave / 2) * (16 * S::kAcrossOf) + j * 16 + lane % 16;
 #pragma unroll
-        for (int i = 0; i < kDown; ++i) {
+        for (int i = 0; i < S::kDownOf; ++i) {
           const f32x4 x = acc[i][j];
           if constexpr (kWide) {
-            *reinterpret_cast<f32x4*>(lds + staged(column, i * 4 + lane / 16) * 8) = x;
+            *reinterpret_cast<f32x4*>(lds + staged<kChunks>(column, i * 4 + lane / 16) * 8) = x;
           } else {
-            const int chunk = (wave % 2) * 16 + i * 2 + lane / 32;
-            *reinterpret_cast<uint64_t*>(lds + staged(column, chunk) * 8 + (lane / 16 % 2) * 4) =
+            const int chunk = (wave % 2) * (2 * S::kDownOf) + i * 2 + lane / 32;
+            *reinterpret_cast<uint64_t*>(lds + staged<kChunks>(column, chunk) * 8 + (lane / 16 % 2) * 4) =
                 static_cast<uint64_t>(pack2<OUT>(x[2], x[3])) << 32 | pack2<OUT>(x[0], x[1]);
           }
           if (i % 2 == 1) __builtin_amdgcn_sched_barrier(0);  // a few outputs at a time: no registers to spill
@@ -334,13 +354,13 @@ __global__ void __launch_bounds__(kThreads) attnres_ffn_out_kernel(OutArgs g) {
       }
     }
     __syncthreads();
-    for (int k = threadIdx.x; k < kTile * 32; k += kThreads) {
-      const int column = k / 32, chunk = k % 32;
-      const int64_t a = a0 + round * 128 + chunk * kChunk, b = b0 + column;
+    for (int k = threadIdx.x; k < TILE * kChunks; k += S::kThreadsOf) {
+      const int column = k / kChunks, chunk = k % kChunks;
+      const int64_t a = a0 + round * (TILE / 2) + chunk * kChunk, b = b0 + column;
       const int64_t second = b >= g.half_pad ? 1 : 0, within = b - second * g.half_pad;
       if (b >= g.entries_b || within >= g.half || a >= g.entries_a) continue;
       OUT* to = out + (second * g.half + within) * g.ld + a;
-      const uint16_t* from = lds + staged(column, chunk) * 8;
+      const uint16_t* from = lds + staged<kChunks>(column, chunk) * 8;
       if constexpr (kWide) {
         const f32x4 x = *reinterpret_cast<const f32x4*>(from);
         if (a + kChunk <= g.entries_a) {
@@ -359,6 +379,45 @@ __global__ void __launch_bounds__(kThreads) attnres_ffn_out_kernel(OutArgs g) {
     }
     if (round + 1 < kRounds) __syncthreads();
   }
+}
+
+// Y (A: Wd by rows, B: a by rows).
+template <class X, class OUT, int TILE>
+__global__ void __launch_bounds__(Shape<TILE>::kThreadsOf, Shape<TILE>::kGroupsOf) attnres_ffn_out_kernel(OutArgs g) {
+  using S = Shape<TILE>;
+  __shared__ __align__(16) uint16_t lds[S::kLds];
+  TileAt tile;
+  if (!tile_at(g.product, g.product.tiles_b, &tile)) return;
+  typename S::Sums acc;
+  multiply_tile<TILE, Part<X>, kSegments<X>, true, true>(g.product, tile, stages_of(g.product, tile.split), lds, acc);
+  store_tile<OUT, TILE>(g, tile, acc, lds);
+}
+
+// dX (A: W by columns, B: [dg du] by rows), dW (A: X, B: [dg du], both by columns) and dWd (A: a, B: dY, both by columns) in one
+// launch, the tiles that take longest first, so that the three fill the chip together.
+struct GradientsArgs {
+  OutArgs of[3];
+  uint32_t first[3];  // workgroup of each; past the last: none
+  int b_rows[3], wide[3];
+};
+
+template <class X, int TILE>
+__global__ void __launch_bounds__(Shape<TILE>::kThreadsOf, Shape<TILE>::kGroupsOf) attnres_ffn_gradients_kernel(GradientsArgs args) {
+  using S = Shape<TILE>;
+  __shared__ __align__(16) uint16_t lds[S::kLds];
+  const int which = (blockIdx.x >= args.first[1] ? 1 : 0) + (blockIdx.x >= args.first[2] ? 1 : 0);
+  const OutArgs& g = args.of[which];
+  TileAt tile;
+  if (!tile_at(g.product, g.product.tiles_b, static_cast<int>(blockIdx.x - args.first[which]), &tile)) return;
+  const Stages stages = stages_of(g.product, tile.split);
+  typename S::Sums acc;
+  if (args.b_rows[which]) {
+    multiply_tile<TILE, Part<X>, kSegments<X>, false, true>(g.product, tile, stages, lds, acc);
+  } else {
+    multiply_tile<TILE, Part<X>, kSegments<X>, false, false>(g.product, tile, stages, lds, acc);
+  }
+  if (std::is_same_v<X, float> || args.wide[which]) store_tile<float, TILE>(g, tile, acc, lds);
+  else store_tile<X, TILE>(g, tile, acc, lds);
 }
 
 // out[r] = the sum of the parts' rows, in order.
@@ -574,6 +633,14 @@ struct Sizes {
   int dtype;
 };
 
+// How products are shared out: the tiles' size, and the parts that the depth of each is cut into.
+struct Cut {
+  int tile, splits[3];
+};
+struct Outputs {
+  int64_t a, b, depth;  // entries; 0: not asked for
+};
+
 struct FfnPlan {
   int parts, segments;
   bool few;
@@ -581,11 +648,90 @@ struct FfnPlan {
   bool pack_x, pack_gate_up, pack_down, pack_grad;
   int64_t x[3], gate_up[3], down[3], grad[3], a[3], both[3];  // offsets
   int64_t saved, partial;
-  int splits_out, splits_x, splits_gate_up, splits_down;
+  Cut gate, slope, out, gradients;
+  int64_t partials[3];
   int64_t bytes, saved_bytes;
 };
 
 int64_t tiles_of(int64_t n, int64_t tile) { return (n + tile - 1) / tile; }
+
+// When the last unit is done, if each takes the next tile as soon as it is free: `count` tiles that take `each`, longest first.
+class Schedule {
+ public:
+  void add(int64_t count, double each) {
+    const int64_t whole = std::max<int64_t>(count / kUnits - 1, 0);  // rounds of all units
+    for (int i = 0; i < size_; ++i) level_[i].time += static_cast<double>(whole) * each;
+    for (count -= whole * kUnits; count > 0;) {
+      int first = 0;
+      for (int i = 1; i < size_; ++i) {
+        if (level_[i].time < level_[first].time) first = i;
+      }
+      Level& level = level_[first];
+      if (count >= level.units || size_ == kLevels) {
+        level.time += each;
+        count -= level.units;
+      } else {
+        level_[size_++] = {level.time + each, static_cast<int>(count)};
+        level.units -= static_cast<int>(count);
+        count = 0;
+      }
+    }
+  }
+  double end() const {
+    double last = 0.0;
+    for (int i = 0; i < size_; ++i) last = std::max(last, level_[i].time);
+    return last;
+  }
+
+ private:
+  static constexpr int kLevels = 8;  // one more per product at most
+  struct Level {
+    double time;
+    int units;
+  };
+  Level level_[kLevels] = {{0.0, kUnits}};
+  int size_ = 1;
+};
+
+// The cut that takes the least time: the schedule of all tiles at a unit's rate for them, and the partial sums' way to memory and
+// back.  Rates as measured on a full chip.
+Cut choose_cut(const Outputs* outputs, int count, int segments, bool whole) {
+  Cut best{256, {1, 1, 1}};
+  double least = 0.0;
+  for (const int tile : {256, 128, 64}) {
+    // a workgroup alone on a unit that has room for more reaches two thirds of its rate
+    const double alone = tile == 256 ? 1.0 : 1.5;
+    const double rate = (tile == 256 ? 1.2e15 : tile == 128 ? 0.9e15 : 0.6e15) / kUnits;
+    int64_t tiles[3] = {};
+    bool fits = true;
+    for (int i = 0; i < count; ++i) {
+      tiles[i] = tiles_of(outputs[i].a, tile) * tiles_of(outputs[i].b, tile);
+      fits = fits && (tile == 256 || tiles[i] <= kMaxTiles);
+    }
+    if (!fits) continue;
+    Cut cut{tile, {1, 1, 1}};
+    for (;;) {
+      double each[3], partial = 0.0;
+      int order[3] = {0, 1, 2};
+      for (int i = 0; i < count; ++i) {
+        each[i] = 2.0 * tile * tile * static_cast<double>(outputs[i].depth) * segments / cut.splits[i] / rate;
+        if (cut.splits[i] > 1) partial += 4e-6 + 8.0 * static_cast<double>(outputs[i].a * outputs[i].b) * cut.splits[i] / 4.5e12;
+      }
+      std::sort(order, order + count, [&](int i, int j) { return each[i] > each[j]; });
+      Schedule schedule;
+      for (int i = 0; i < count; ++i) schedule.add(tiles[order[i]] * cut.splits[order[i]], each[order[i]]);
+      const int longest = order[0];
+      const double time = std::max(schedule.end(), alone * each[longest]) + partial;
+      if (least == 0.0 || time < least) {
+        least = time;
+        best = cut;
+      }
+      if (whole || cut.splits[longest] >= 32 || outputs[longest].depth / kDepth / (cut.splits[longest] + 1) < 4) break;
+      ++cut.splits[longest];
+    }
+  }
+  return best;
+}
 
 FfnPlan ffn_plan(const Sizes& s, int pass) {
   FfnPlan p{};
@@ -621,19 +767,24 @@ FfnPlan ffn_plan(const Sizes& s, int pass) {
   if (!tiles) p.a[0] = take(s.rows * p.hidden_pad * dtype_size(s.dtype));
   if (pass == kBackwardAgain) p.saved = take(p.saved_bytes);
   int64_t partial = 0;
-  const auto splits = [&](int64_t entries_a, int64_t entries_b, int64_t depth) {
-    const int64_t tiles = tiles_of(entries_a, kTile) * tiles_of(entries_b, kTile);
-    const int n = choose_splits(tiles, depth, p.segments, true);
-    if (n > 1) partial = std::max(partial, 4 * n * entries_b * round_up(entries_a, kVec));
-    return n;
+  // what the sums of g, u and da go into needs them whole
+  const auto one = [&](int64_t a, int64_t b, int64_t depth, bool whole) {
+    const Outputs o{a, b, depth};
+    return choose_cut(&o, 1, p.segments, whole);
   };
-  if (!tiles) {
-  } else if (!backward) {
-    p.splits_out = splits(s.out_width, s.rows, p.hidden_pad);
-  } else {
-    p.splits_x = splits(s.width, s.rows, 2 * p.hidden_pad);
-    p.splits_gate_up = splits(s.width, 2 * p.hidden_pad, p.rows_pad);
-    p.splits_down = splits(s.hidden, s.out_width, p.rows_pad);
+  if (tiles) p.gate = one(2 * p.hidden_pad, s.rows, p.width_pad, true);
+  if (!backward && tiles) {
+    p.out = one(s.out_width, s.rows, p.hidden_pad, false);
+    if (p.out.splits[0] > 1) partial = 4 * p.out.splits[0] * s.rows * round_up(s.out_width, kVec);
+  }
+  if (backward) {
+    p.slope = one(p.hidden_pad, p.rows_pad, p.out_pad, true);
+    const Outputs o[3] = {{s.width, s.rows, 2 * p.hidden_pad}, {s.width, 2 * p.hidden_pad, p.rows_pad}, {s.hidden, s.out_width, p.rows_pad}};
+    p.gradients = choose_cut(o, 3, p.segments, false);
+    for (int i = 0; i < 3; ++i) {
+      p.partials[i] = partial;
+      if (p.gradients.splits[i] > 1) partial += round_up(4 * p.gradients.splits[i] * o[i].b * round_up(o[i].a, kVec), 256);
+    }
   }
   p.partial = take(partial);
   p.bytes = at;
@@ -656,6 +807,13 @@ struct Call {
   hipStream_t stream;
   uint16_t* operand(int64_t offset) const { return reinterpret_cast<uint16_t*>(workspace + offset); }
 };
+
+template <class F>
+void with_tile(int tile, F f) {
+  if (tile == 256) f(std::integral_constant<int, 256>{});
+  else if (tile == 128) f(std::integral_constant<int, 128>{});
+  else f(std::integral_constant<int, 64>{});
+}
 
 // An operand where it lies, or packed into the workspace; `half`, `half_pad`: see PackArgs.
 template <class X>
@@ -696,15 +854,20 @@ void launch_gate(const Call& c, const Operand& x, const Operand& gate_up, char* 
   w.entries = p.pack_gate_up ? p.hidden_pad : c.s.hidden;
   w.second = w.entries * w.ld;
   rows.entries = c.s.rows;
-  g.product = {w, rows, nullptr, p.width_pad, 0, static_cast<int>(tiles_of(p.hidden_pad, kPairTile)),
-               static_cast<int>(tiles_of(c.s.rows, kTile)), 1};
+  const int tile = p.gate.tile;
+  g.product = {w, rows, nullptr, p.width_pad, 0, static_cast<int>(tiles_of(p.hidden_pad, tile / 2)),
+               static_cast<int>(tiles_of(c.s.rows, tile)), 1};
   g.rows = c.s.rows;
   g.hidden = c.s.hidden;
   g.hidden_pad = p.hidden_pad;
   g.activation = c.activation;
   g.saved = saved;
   for (int k = 0; a != nullptr && k < kParts<X>; ++k) g.out[k] = c.operand(a[k]);
-  hipLaunchKernelGGL((attnres_ffn_gate_kernel<X>), dim3(g.product.tiles_a * g.product.tiles_b), dim3(kThreads), 0, c.stream, g);
+  with_tile(tile, [&](auto size) {
+    constexpr int TILE = decltype(size)::value;
+    hipLaunchKernelGGL((attnres_ffn_gate_kernel<X, TILE>), dim3(g.product.tiles_a * g.product.tiles_b), dim3(Shape<TILE>::kThreadsOf), 0,
+                       c.stream, g);
+  });
 }
 
 // Of few rows: g and u, and a from them.
@@ -733,32 +896,33 @@ void few_forward(const Call& c, void* out, char* saved) {
   hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(tiles_of(c.s.out_width, 16))), dim3(1024), 0, c.stream, g);
 }
 
-// out[b][a], by halves of B's entries; joined where the depth is cut.
-template <class X, bool A_ROWS, bool B_ROWS>
-void launch_out(const Call& c, const Operand& a, const Operand& b, int64_t depth, int64_t entries_a, int64_t half, int64_t half_pad,
-                int64_t entries_b, int splits, void* out) {
+// A product into out[b][a], by halves of B's entries, or its parts into the workspace.
+OutArgs out_args(const Call& c, const Operand& a, const Operand& b, int64_t depth, int64_t entries_a, int64_t half, int64_t half_pad,
+                 int64_t entries_b, int tile, int splits, int64_t partial, void* out) {
   OutArgs g{};
-  g.product = {a, b, nullptr, depth, 0, static_cast<int>(tiles_of(entries_a, kTile)), static_cast<int>(tiles_of(entries_b, kTile)),
-               splits};
+  g.product = {a, b, nullptr, depth, 0, static_cast<int>(tiles_of(entries_a, tile)), static_cast<int>(tiles_of(entries_b, tile)), splits};
   g.entries_a = entries_a;
   g.half = half;
   g.half_pad = half_pad;
   g.entries_b = entries_b;
   g.out = out;
   g.ld = entries_a;
-  const dim3 grid(static_cast<unsigned>(g.product.tiles_a) * g.product.tiles_b * splits);
-  if (splits == 1) {
-    hipLaunchKernelGGL((attnres_ffn_out_kernel<X, X, A_ROWS, B_ROWS>), grid, dim3(kThreads), 0, c.stream, g);
-    return;
+  if (splits > 1) {
+    g.out = c.workspace + c.plan.partial + partial;
+    g.ld = round_up(entries_a, kVec);
+    g.split_stride = entries_b / half_pad * half * g.ld;
   }
-  const int64_t rows = entries_b / half_pad * half;
-  float* partial = reinterpret_cast<float*>(c.workspace + c.plan.partial);
-  g.out = partial;
-  g.ld = round_up(entries_a, kVec);
-  g.split_stride = rows * g.ld;
-  hipLaunchKernelGGL((attnres_ffn_out_kernel<X, float, A_ROWS, B_ROWS>), grid, dim3(kThreads), 0, c.stream, g);
-  hipLaunchKernelGGL((attnres_ffn_join_kernel<X>), dim3(stride_grid(rows * (g.ld / kVec))), dim3(kBlock), 0, c.stream, partial, splits,
-                     g.split_stride, g.ld, rows, static_cast<int>(entries_a), static_cast<X*>(out));
+  return g;
+}
+
+unsigned workgroups(const OutArgs& g) { return static_cast<unsigned>(g.product.tiles_a) * g.product.tiles_b * g.product.splits; }
+
+template <class X>
+void join_parts(const Call& c, const OutArgs& g, void* out) {
+  const int64_t rows = g.split_stride / g.ld;
+  hipLaunchKernelGGL((attnres_ffn_join_kernel<X>), dim3(stride_grid(rows * (g.ld / kVec))), dim3(kBlock), 0, c.stream,
+                     static_cast<const float*>(g.out), g.product.splits, g.split_stride, g.ld, rows, static_cast<int>(g.entries_a),
+                     static_cast<X*>(out));
 }
 
 template <class X>
@@ -771,7 +935,14 @@ void ffn_forward(const Call& c, void* out, char* saved) {
   for (int k = 0; k < kParts<X>; ++k) a.part[k] = c.operand(p.a[k]);
   a.ld = p.hidden_pad;
   a.entries = c.s.rows;
-  launch_out<X, true, true>(c, down, a, p.hidden_pad, c.s.out_width, c.s.rows, c.s.rows, c.s.rows, p.splits_out, out);
+  const int splits = p.out.splits[0];
+  const OutArgs g = out_args(c, down, a, p.hidden_pad, c.s.out_width, c.s.rows, c.s.rows, c.s.rows, p.out.tile, splits, 0, out);
+  with_tile(p.out.tile, [&](auto size) {
+    constexpr int TILE = decltype(size)::value;
+    const auto kernel = splits > 1 ? attnres_ffn_out_kernel<X, float, TILE> : attnres_ffn_out_kernel<X, X, TILE>;
+    hipLaunchKernelGGL(kernel, dim3(workgroups(g)), dim3(Shape<TILE>::kThreadsOf), 0, c.stream, g);
+  });
+  if (splits > 1) join_parts<X>(c, g, out);
 }
 
 template <class X>
@@ -795,8 +966,9 @@ void ffn_backward(const Call& c, const void* grad_out, const char* saved, void* 
     down.entries = p.hidden_pad;
     down.depth = p.out_pad;
     rows.entries = c.s.rows;
-    g.product = {down, rows, nullptr, p.out_pad, 0, static_cast<int>(tiles_of(p.hidden_pad, kTile)),
-                 static_cast<int>(tiles_of(p.rows_pad, kTile)), 1};
+    const int tile = p.slope.tile;
+    g.product = {down, rows, nullptr, p.out_pad, 0, static_cast<int>(tiles_of(p.hidden_pad, tile)),
+                 static_cast<int>(tiles_of(p.rows_pad, tile)), 1};
     g.rows = c.s.rows;
     g.rows_pad = p.rows_pad;
     g.hidden = c.s.hidden;
@@ -807,7 +979,11 @@ void ffn_backward(const Call& c, const void* grad_out, const char* saved, void* 
       if (grad_x != nullptr || grad_gate_up != nullptr) g.both[k] = c.operand(p.both[k]);
       if (grad_down != nullptr) g.out[k] = c.operand(p.a[k]);
     }
-    hipLaunchKernelGGL((attnres_ffn_slope_kernel<X>), dim3(g.product.tiles_a * g.product.tiles_b), dim3(kThreads), 0, c.stream, g);
+    with_tile(tile, [&](auto size) {
+      constexpr int TILE = decltype(size)::value;
+      hipLaunchKernelGGL((attnres_ffn_slope_kernel<X, TILE>), dim3(g.product.tiles_a * g.product.tiles_b), dim3(Shape<TILE>::kThreadsOf), 0,
+                         c.stream, g);
+    });
   }
   Operand both{}, a{};
   for (int k = 0; k < kParts<X>; ++k) {
@@ -817,32 +993,58 @@ void ffn_backward(const Call& c, const void* grad_out, const char* saved, void* 
   both.ld = 2 * p.hidden_pad;
   a.ld = p.hidden_pad;
   both.depth = a.depth = p.rows_pad;
-  if (grad_down != nullptr) {
-    Operand rows = grad;
-    rows.entries = p.pack_grad ? p.out_pad : c.s.out_width;
-    rows.depth = p.rows_pad;
-    a.entries = p.hidden_pad;
-    launch_out<X, false, false>(c, a, rows, p.rows_pad, c.s.hidden, c.s.out_width, c.s.out_width, c.s.out_width, p.splits_down, grad_down);
+  // in the order of the plan's cut
+  OutArgs of[3] = {};
+  const int tile = p.gradients.tile;
+  const int* splits = p.gradients.splits;
+  void* const results[3] = {grad_x, grad_gate_up, grad_down};
+  if (grad_x != nullptr) {
+    gate_up.entries = p.pack_gate_up ? p.width_pad : c.s.width;
+    gate_up.depth = 2 * p.hidden_pad;
+    both.entries = c.s.rows;
+    of[0] = out_args(c, gate_up, both, 2 * p.hidden_pad, c.s.width, c.s.rows, c.s.rows, c.s.rows, tile, splits[0], p.partials[0], grad_x);
   }
   if (grad_gate_up != nullptr) {
     x.entries = p.pack_x ? p.width_pad : c.s.width;
     x.depth = p.rows_pad;
     both.entries = 2 * p.hidden_pad;
-    launch_out<X, false, false>(c, x, both, p.rows_pad, c.s.width, c.s.hidden, p.hidden_pad, 2 * p.hidden_pad, p.splits_gate_up,
-                                grad_gate_up);
+    of[1] = out_args(c, x, both, p.rows_pad, c.s.width, c.s.hidden, p.hidden_pad, 2 * p.hidden_pad, tile, splits[1], p.partials[1],
+                     grad_gate_up);
   }
-  if (grad_x != nullptr) {
-    gate_up.entries = p.pack_gate_up ? p.width_pad : c.s.width;
-    gate_up.depth = 2 * p.hidden_pad;
-    both.entries = c.s.rows;
-    launch_out<X, false, true>(c, gate_up, both, 2 * p.hidden_pad, c.s.width, c.s.rows, c.s.rows, c.s.rows, p.splits_x, grad_x);
+  if (grad_down != nullptr) {
+    Operand rows = grad;
+    rows.entries = p.pack_grad ? p.out_pad : c.s.out_width;
+    rows.depth = p.rows_pad;
+    a.entries = p.hidden_pad;
+    of[2] = out_args(c, a, rows, p.rows_pad, c.s.hidden, c.s.out_width, c.s.out_width, c.s.out_width, tile, splits[2], p.partials[2],
+                     grad_down);
+  }
+  GradientsArgs g{};
+  int order[3] = {0, 1, 2}, count = 0;
+  std::sort(order, order + 3, [&](int i, int j) { return of[i].product.depth * splits[j] > of[j].product.depth * splits[i]; });
+  uint32_t grid = 0;
+  for (const int i : order) {
+    if (results[i] == nullptr) continue;
+    g.of[count] = of[i];
+    g.b_rows[count] = i == 0;
+    g.wide[count] = splits[i] > 1;
+    g.first[count++] = grid;
+    grid += static_cast<uint32_t>(round_up(workgroups(of[i]), 8));  // whole rounds of the XCDs
+  }
+  for (int k = count; k < 3; ++k) g.first[k] = UINT32_MAX;
+  with_tile(tile, [&](auto size) {
+    constexpr int TILE = decltype(size)::value;
+    hipLaunchKernelGGL((attnres_ffn_gradients_kernel<X, TILE>), dim3(grid), dim3(Shape<TILE>::kThreadsOf), 0, c.stream, g);
+  });
+  for (int i = 0; i < 3; ++i) {
+    if (results[i] != nullptr && splits[i] > 1) join_parts<X>(c, of[i], results[i]);
   }
 }
 
 bool known_sizes(const Sizes& s) {
   return s.rows >= 0 && s.rows <= kMaxRows && s.width >= 1 && s.width <= ATTNRES_MAX_WIDTH && s.hidden >= 1 && s.hidden <= kMaxHidden &&
          s.out_width >= 1 && s.out_width <= ATTNRES_MAX_WIDTH && dtype_known(s.dtype) &&
-         tiles_of(s.rows, kTile) * tiles_of(s.hidden, kPairTile) <= kMaxTiles;
+         tiles_of(s.rows, kTile) * tiles_of(s.hidden, kTile / 2) <= kMaxTiles;
 }
 
 int check_sizes(const Sizes& s, int activation) {

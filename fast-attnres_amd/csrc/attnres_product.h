@@ -158,9 +158,8 @@ struct TileAt {
 // the tiles' order, in which 4 tiles of B by all of A's follow each other: the 32 tiles that run on an
 // XCD at a time share 4 + 8 operand stripes in its L2.  tiles_b: those with rows that count, so that the XCDs
 // get equal shares of them; false for the workgroups past the last tile.
-__device__ __forceinline__ bool tile_at(const Product& p, int tiles_b, TileAt* tile) {
+__device__ __forceinline__ bool tile_at(const Product& p, int tiles_b, int id, TileAt* tile) {
   const int total = p.tiles_a * tiles_b * p.splits;
-  const int id = blockIdx.x;
   if (id >= total) return false;
   const int q = total / 8, r = total % 8, xcd = id % 8, i = id / 8;
   int at = xcd < r ? xcd * (q + 1) + i : r * (q + 1) + (xcd - r) * q + i;
@@ -172,6 +171,9 @@ __device__ __forceinline__ bool tile_at(const Product& p, int tiles_b, TileAt* t
   at -= group * kGroup * p.tiles_a;
   *tile = {at / size, group * kGroup + at % size, split};
   return true;
+}
+__device__ __forceinline__ bool tile_at(const Product& p, int tiles_b, TileAt* tile) {
+  return tile_at(p, tiles_b, static_cast<int>(blockIdx.x), tile);
 }
 
 // [16 entries of A][16 entries of B]; lane l, register e: entry 4 (l / 16) + e of A, l % 16 of B.
@@ -360,6 +362,230 @@ __device__ __forceinline__ void multiply(const Product& p, const TileAt& tile, c
   __syncthreads();  // LDS is free for the epilogue
 }
 
+// -------------------------------------------------------------- smaller tiles
+// The same product in tiles of 128 x 128 or 64 x 64, four wavefronts each, two by two, and two or four workgroups on a
+// unit: for outputs that tiles of 256 do not share out evenly.  Where an operand lies as rows of k a stage is 64 k's, so that
+// they are read by whole lines of 128 bytes (4096 x 16384 x 4096, both as rows, tiles of 128: 710 -> 614 us), else 32, twice as many stages ahead
+// (both as columns: 610 -> 592; tiles of 64 are faster with 64, 55 -> 47 us for 1024 x 5632 x 2048).  A step is 32 k's, and the next
+// one's fragments are read meanwhile.
+template <int TILE>
+struct Shape {
+  static constexpr int kTileOf = TILE;
+  static constexpr int kWavesOf = TILE == 256 ? kWaves : 4;  // two along A, the others along B
+  static constexpr int kThreadsOf = 64 * kWavesOf;
+  static constexpr int kGroupsOf = TILE == 64 ? 4 : 2;  // wavefronts per SIMD, and workgroups per unit of the smaller tiles
+  static constexpr int kDownOf = TILE / 32;
+  static constexpr int kAcrossOf = TILE == 256 ? kAcross : TILE / 32;
+  static constexpr int kPairedOf = kDownOf * 8;  // PAIRED rows: entries of a wavefront's half
+  static constexpr int kLds = kStages * 2 * TILE * kDepth;  // 16-bit elements: 4 stages of 32 k's, or 2 of 64
+  using Sums = f32x4[kDownOf][kAcrossOf];
+};
+static_assert(Shape<256>::kDownOf == kDown && Shape<256>::kPairedOf == kPaired, "one shape");
+
+// 16-byte slots within an LDS row.  Rows of k (128 bytes) and columns of 64 alternate between the banks' halves by themselves.
+__device__ __forceinline__ int small_row_swizzle(int row) { return row >> 1 & 7; }
+template <int TILE>
+__device__ __forceinline__ int small_column_swizzle(int k) {
+  return TILE == 64 ? (k >> 1 & 1) << 1 | (k >> 3 & 1) << 2 : column_swizzle(k);
+}
+
+template <int TILE, int DEPTH, bool ROWS, bool PAIRED>
+struct SmallLoader {
+  using S = Shape<TILE>;
+  static constexpr int kLoadsOf = TILE * DEPTH / 512 / S::kWavesOf;  // of 1 KB per wavefront and stage
+  static constexpr int kRowsOfLoad = ROWS ? 8 : 512 / TILE, kLanesOfRow = 64 / kRowsOfLoad;
+  uint32_t offset[kLoadsOf];  // bytes from the stage's origin; columns: of the chunk alone
+  int row;                    // of the first load
+  __device__ __forceinline__ void init(const Operand& o, int64_t entry0, int wave, int lane) {
+    row = wave * kLoadsOf * kRowsOfLoad + lane / kLanesOfRow;
+#pragma unroll
+    for (int j = 0; j < kLoadsOf; ++j) {
+      const int r = row + j * kRowsOfLoad;
+      if constexpr (ROWS) {
+        const int entry = PAIRED ? r / (2 * S::kPairedOf) * S::kPairedOf + r % S::kPairedOf : r;
+        const int64_t left = o.entries - 1 - entry0;
+        const int64_t at = entry < left ? entry : left;
+        const int64_t from = at * o.ld + (PAIRED && r / S::kPairedOf % 2 == 1 ? o.second : 0);
+        offset[j] = static_cast<uint32_t>((from + ((lane % 8) ^ small_row_swizzle(r)) * 8) * 2);
+      } else {
+        const int chunk = (lane % kLanesOfRow) ^ small_column_swizzle<TILE>(r);
+        const int64_t left = o.entries - 8 - entry0;
+        const int64_t at = chunk * 8 < left ? chunk * 8 : left;
+        offset[j] = static_cast<uint32_t>(at * 2);
+      }
+    }
+  }
+  // Of load j of a stage; left: k's of it that the operand holds, less one.  Of a stage of 32 k's rows load them twice.
+  __device__ __forceinline__ uint32_t at(const Operand& o, int left, bool half, int lane, int j) const {
+    if constexpr (ROWS) {
+      const bool upper = (((lane % 8) ^ small_row_swizzle(row + j * kRowsOfLoad)) & 4) != 0;
+      return half && upper ? offset[j] - 64 : offset[j];
+    } else {
+      return offset[j] + static_cast<uint32_t>(min(row + j * kRowsOfLoad, left)) * static_cast<uint32_t>(o.ld * 2);
+    }
+  }
+};
+
+// Fragments of 16 entries and a step's 32 k's, as Reader's.
+template <int TILE, bool ROWS>
+struct SmallReader {
+  uint32_t at, column;
+  __device__ __forceinline__ void init(int entry, int lane) {
+    const int group = lane / 16, j = lane % 16;
+    if constexpr (ROWS) {
+      at = static_cast<uint32_t>((entry + j) * 128);
+      column = static_cast<uint32_t>((group ^ small_row_swizzle(j)) * 16);
+    } else {
+      const int k = group * 8 + j / 4;
+      at = static_cast<uint32_t>(k * TILE) * 2;
+      column = static_cast<uint32_t>(((entry / 8 + j % 4 / 2) ^ small_column_swizzle<TILE>(k)) * 8 + j % 2 * 4) * 2;
+    }
+  }
+  __device__ __forceinline__ s16x8 read(uint32_t stage, int step, int f) const {
+    if constexpr (ROWS) {
+      return *(ATTNRES_LDS const s16x8*)(stage + at + (column ^ (step * 64u)) + f * 16 * 128);
+    } else {
+      const uint32_t from = stage + step * 32 * TILE * 2 + at + (column ^ (f * 32u));
+      const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((ATTNRES_LDS s16x4*)(from));
+      const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((ATTNRES_LDS s16x4*)(from + 4 * TILE * 2));
+      return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+  }
+};
+
+// As multiply(): the sum of a tile over its split's k's (at least one stage of 32).
+template <int TILE, class T, int SEGMENTS, bool A_ROWS, bool B_ROWS, bool PAIRED>
+__device__ __forceinline__ void small_multiply(const Product& p, const TileAt& tile, const Stages& range, uint16_t* lds,
+                                               typename Shape<TILE>::Sums& acc) {
+  using S = Shape<TILE>;
+  constexpr int kDownOf = S::kDownOf, kAcrossOf = S::kAcrossOf;
+  constexpr int kSteps = A_ROWS || B_ROWS || TILE == 64 ? 2 : 1, kDepthOf = kSteps * kDepth, kStagesOf = kStages / kSteps;
+  const int wave = wave_index(), lane = threadIdx.x % 64;
+#pragma unroll
+  for (int i = 0; i < kDownOf; ++i) {
+#pragma unroll
+    for (int j = 0; j < kAcrossOf; ++j) acc[i][j] = f32x4{};
+  }
+  const int first = range.first, stages = (range.count + kSteps - 1) / kSteps, total = stages * SEGMENTS;
+  const bool odd = range.count % kSteps != 0;  // the last stage is one step
+  const int64_t a0 = static_cast<int64_t>(tile.a) * (PAIRED ? TILE / 2 : TILE), b0 = static_cast<int64_t>(tile.b) * TILE;
+  SmallLoader<TILE, kDepthOf, A_ROWS, PAIRED> load_a;
+  SmallLoader<TILE, kDepthOf, B_ROWS, false> load_b;
+  constexpr int kLoadsOf = decltype(load_a)::kLoadsOf;
+  load_a.init(p.a, a0, wave, lane);
+  load_b.init(p.b, b0, wave, lane);
+  const int64_t origin_a = (A_ROWS ? a0 * p.a.ld : a0) * 2, origin_b = (B_ROWS ? b0 * p.b.ld : b0) * 2;
+  const int64_t next_a = (A_ROWS ? 1 : p.a.ld) * kDepthOf * 2, next_b = (B_ROWS ? 1 : p.b.ld) * kDepthOf * 2;
+  const int64_t from_a = origin_a + first * (next_a / kSteps), from_b = origin_b + first * (next_b / kSteps);
+  const uint32_t lds0 = lds_byte(lds);
+  constexpr uint32_t kB = TILE * kDepthOf * 2, kStageBytes = 2 * kB;
+  const uint32_t slot = wave * (kLoadsOf * 1024);
+  int segment = 0, stage = 0;  // of the next load
+  const auto load = [&](uint32_t buffer) {
+    const char* a = scalar(reinterpret_cast<const char*>(p.a.part[part_of_a<SEGMENTS>(segment)]) + from_a + stage * next_a);
+    const char* b = scalar(reinterpret_cast<const char*>(p.b.part[part_of_b<SEGMENTS>(segment)]) + from_b + stage * next_b);
+    const int64_t k = (first + static_cast<int64_t>(stage) * kSteps) * kDepth;
+    const int left_a = __builtin_amdgcn_readfirstlane(static_cast<int>(p.a.depth - 1 - k));
+    const int left_b = __builtin_amdgcn_readfirstlane(static_cast<int>(p.b.depth - 1 - k));
+    const bool half = odd && stage + 1 == stages;
+#pragma unroll
+    for (int j = 0; j < kLoadsOf; ++j) load_lds(a, load_a.at(p.a, left_a, half, lane, j), buffer + slot + j * 1024);
+#pragma unroll
+    for (int j = 0; j < kLoadsOf; ++j) load_lds(b, load_b.at(p.b, left_b, half, lane, j), buffer + kB + slot + j * 1024);
+    if (++stage == stages) stage = 0, ++segment;
+  };
+  SmallReader<TILE, A_ROWS> read_a;
+  SmallReader<TILE, B_ROWS> read_b;
+  read_a.init((wave % 2) * (16 * kDownOf), lane);
+  read_b.init((wave / 2) * (16 * kAcrossOf), lane);
+  struct Fragments {
+    s16x8 a[kDownOf], b[kAcrossOf];
+  };
+  constexpr int kReads = kDownOf + kAcrossOf, kProducts = kDownOf * kAcrossOf;
+  static_assert(kReads <= kProducts, "a read between two products at most");
+  const auto read = [&](uint32_t buffer, int step, Fragments& f, int r) {
+    if (r < kAcrossOf) f.b[r] = read_b.read(buffer + kB, step, r);
+    else f.a[r - kAcrossOf] = read_a.read(buffer, step, r - kAcrossOf);
+  };
+  const auto read_all = [&](uint32_t buffer, Fragments& f) {
+#pragma unroll
+    for (int r = 0; r < kReads; ++r) read(buffer, 0, f, r);
+  };
+  // Every wavefront's reads from LDS are done and its loads have landed but for those of `ahead` stages.
+  const auto arrived = [&](auto ahead) {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"i"(decltype(ahead)::value * 2 * kLoadsOf) : "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+  };
+  const auto next = [&](int& at) {  // a stage's buffer
+    const uint32_t buffer = lds0 + at;
+    at = at + kStageBytes == kStagesOf * kStageBytes ? 0 : at + kStageBytes;
+    return buffer;
+  };
+  const auto products = [&](Fragments& now, auto meanwhile) {
+#pragma unroll
+    for (int m = 0; m < kProducts; ++m) {
+      f32x4& c = acc[m / kAcrossOf][m % kAcrossOf];
+      c = mfma<T>(now.a[m / kAcrossOf], now.b[m % kAcrossOf], c);
+      if (m * kReads / kProducts != (m + 1) * kReads / kProducts) meanwhile(m * kReads / kProducts);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  const auto nothing = [](int) {};
+  int loading = 0, reading = 0;  // LDS bytes of the next buffer
+  for (int s = 0; s < kStagesOf && s < total; ++s) load(next(loading));
+  if (total >= kStagesOf) arrived(std::integral_constant<int, kStagesOf - 1>{});
+  else arrived(std::integral_constant<int, 0>{});
+  Fragments lower, upper;
+  uint32_t buffer = next(reading);
+  read_all(buffer, lower);
+  // From stage s to the next one, all of s in registers: its buffer gets the loads of a stage to come.
+  const auto cross = [&](int s) {
+    if (s + kStagesOf - 1 < total) arrived(std::integral_constant<int, kStagesOf - 2>{});
+    else arrived(std::integral_constant<int, 0>{});
+    if (s + kStagesOf < total) load(next(loading));
+    buffer = next(reading);
+  };
+  if constexpr (kSteps == 2) {
+    int within = 0;  // the stage's number in its segment
+    for (int s = 0; s < total; ++s) {
+      products(lower, [&](int r) { read(buffer, 1, upper, r); });
+      const bool half = odd && within + 1 == stages;
+      within = within + 1 == stages ? 0 : within + 1;
+      if (s + 1 == total) {
+        if (!half) products(upper, nothing);
+        break;
+      }
+      cross(s);
+      if (half) read_all(buffer, lower);
+      else products(upper, [&](int r) { read(buffer, 0, lower, r); });
+    }
+  } else {
+    int s = 0;
+    for (; s + 2 < total; s += 2) {
+      cross(s);
+      products(lower, [&](int r) { read(buffer, 0, upper, r); });
+      cross(s + 1);
+      products(upper, [&](int r) { read(buffer, 0, lower, r); });
+    }
+    if (s + 1 < total) {
+      cross(s);
+      products(lower, [&](int r) { read(buffer, 0, upper, r); });
+      products(upper, nothing);
+    } else {
+      products(lower, nothing);
+    }
+  }
+  __syncthreads();  // LDS is free for the epilogue
+}
+
+template <int TILE, class T, int SEGMENTS, bool A_ROWS, bool B_ROWS, bool PAIRED = false>
+__device__ __forceinline__ void multiply_tile(const Product& p, const TileAt& tile, const Stages& range, uint16_t* lds,
+                                              typename Shape<TILE>::Sums& acc) {
+  if constexpr (TILE == 256) multiply<T, SEGMENTS, A_ROWS, B_ROWS, PAIRED>(p, tile, range, lds, acc);
+  else small_multiply<TILE, T, SEGMENTS, A_ROWS, B_ROWS, PAIRED>(p, tile, range, lds, acc);
+}
+
 // ------------------------------------------------------------- few rows
 // Operands that go straight to registers as they lie (any width and alignment): a lane holds 16 bytes of every 64 of its
 // row; the order of the k's in a matrix instruction is of no account, as both operands share it.
@@ -408,9 +634,10 @@ __device__ __forceinline__ f32x4 few_mfma(const FewChunk<X>& a, const FewChunk<X
   return c;
 }
 
-// 16-byte slot of a staged output row of 512 bytes: a permutation per row, so that 32 lanes
+// 16-byte slot of a staged output row of 512 bytes (CHUNKS of 16): a permutation per row, so that 32 lanes
 // writing one chunk of 32 rows meet 32 different slots.
-__device__ __forceinline__ int staged(int row, int chunk) { return row * 32 + (chunk ^ (row & 31)); }
+template <int CHUNKS = 32>
+__device__ __forceinline__ int staged(int row, int chunk) { return row * CHUNKS + (chunk ^ (row & (CHUNKS - 1))); }
 
 constexpr int kUnits = 256;  // compute units, one workgroup each
 
