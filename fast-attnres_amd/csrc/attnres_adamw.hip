@@ -165,7 +165,7 @@ __device__ __forceinline__ float largest_magnitude(f32x4 x) {
 // Values to E4M3 numbers and their scale.
 template <bool ROOT, bool PAST>
 __device__ __forceinline__ float to_numbers(f32x4 x, Four<E4m3, PAST>* numbers) {
-  float scale = largest_magnitude(x) / kLargest;
+  float scale = largest_magnitude(x) * (1.0f / kLargest);
   if (scale < kLeastScale) scale = 0.0f;
   if (!(scale < __builtin_inff())) scale = __builtin_nanf("");  // the whole block
   const float by = scale > 0.0f ? 1.0f / scale : 0.0f;
@@ -178,6 +178,17 @@ __device__ __forceinline__ float to_numbers(f32x4 x, Four<E4m3, PAST>* numbers) 
   }
   numbers->set(number);
   return scale;
+}
+
+struct Moments {
+  float m, v;
+};
+
+// Every operation rounded by itself: the numbers that a state is rounded to then do not depend on how a compiler joins operations,
+// and any FP32 arithmetic in this order finds the same ones.
+__device__ __forceinline__ Moments next_moments(float m, float v, float d, float keep1, float add1, float keep2, float add2) {
+#pragma clang fp contract(off)
+  return {keep1 * m + add1 * d, keep2 * v + add2 * d * d};
 }
 
 // PAST: past the caches.
@@ -233,8 +244,9 @@ __global__ void __launch_bounds__(kBlock) attnres_adamw_kernel(StepArgs g) {
     f32x4 root;
 #pragma unroll
     for (int e = 0; e < kLane; ++e) {
-      m[e] = g.keep1 * m[e] + g.add1 * d[e];
-      v[e] = g.keep2 * v[e] + g.add2 * d[e] * d[e];
+      const Moments next = next_moments(m[e], v[e], d[e], g.keep1, g.add1, g.keep2, g.add2);
+      m[e] = next.m;
+      v[e] = next.v;
       root[e] = sqrtf(v[e]);
       w[e] = f.decay * w[e] - f.rate * (m[e] / (root[e] * f.unbias + g.eps));
     }

@@ -75,7 +75,7 @@ __device__ __forceinline__ void save_pair(char* to, int lane, f32x4 g, f32x4 u) 
     *reinterpret_cast<f32x4*>(to + lane * 16) = g;
     *reinterpret_cast<f32x4*>(to + 1024 + lane * 16) = u;
   } else {
-    // to nearest 24 bits, ties away from zero; infinities and NaN as they are
+    // to nearest 24 bits, ties away from zero; NaN of products of 16-bit numbers has zeros there, so it stays NaN
     uint32_t w[8];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
@@ -83,7 +83,7 @@ __device__ __forceinline__ void save_pair(char* to, int lane, f32x4 g, f32x4 u) 
       w[4 + e] = __float_as_uint(u[e]);
     }
 #pragma unroll
-    for (int e = 0; e < 8; ++e) w[e] = (w[e] & 0x7f800000u) == 0x7f800000u ? w[e] : w[e] + 0x80u;
+    for (int e = 0; e < 8; ++e) w[e] += 0x80u;
     u32x4 high;
 #pragma unroll
     for (int e = 0; e < 4; ++e) high[e] = __builtin_amdgcn_perm(w[2 * e + 1], w[2 * e], 0x07060302u);
@@ -113,8 +113,9 @@ struct Pair {
     }
   }
   __device__ __forceinline__ float word(int e) const {  // g: 0..3, u: 4..7
-    const uint32_t top = e % 2 == 0 ? high[e / 2] << 16 : high[e / 2] & 0xffff0000u;
-    return __uint_as_float(top | (rest[e / 4] >> (8 * (e % 4)) & 0xffu) << 8);
+    // bytes: 0, the low one, the two high ones
+    const uint32_t select = (e % 2 == 0 ? 0x0504000cu : 0x0706000cu) | static_cast<uint32_t>(e % 4) << 8;
+    return __uint_as_float(__builtin_amdgcn_perm(high[e / 2], rest[e / 4], select));
   }
   __device__ __forceinline__ float gate(int e) const {
     if constexpr (std::is_same_v<X, float>) return __uint_as_float(high[e]);
@@ -143,33 +144,35 @@ struct GateArgs {
   uint16_t* out[3]; // a [rows][hidden_pad], zeros past hidden; or nullptr
 };
 
-template <class X, int TILE>
-__global__ void __launch_bounds__(Shape<TILE>::kThreadsOf, Shape<TILE>::kGroupsOf) attnres_ffn_gate_kernel(GateArgs g) {
+template <class X, int SHAPE>
+__global__ void __launch_bounds__(Shape<SHAPE>::kAllThreads, Shape<SHAPE>::kGroupsOf) attnres_ffn_gate_kernel(GateArgs g) {
   using T = Part<X>;
-  using S = Shape<TILE>;
-  constexpr int kDown = S::kDownOf, kAcross = S::kAcrossOf;
+  using S = Shape<SHAPE>;
+  constexpr int TILE = S::kTileOf, kDown = S::kDownOf, kAcross = S::kAcrossOf;
   __shared__ __align__(16) uint16_t lds[S::kLds];
   TileAt tile;
   if (!tile_at(g.product, g.product.tiles_b, &tile)) return;
   typename S::Sums acc;
-  multiply_tile<TILE, T, kSegments<X>, true, true, true>(g.product, tile, stages_of(g.product, 0), lds, acc);
+  if (!multiply_tile<SHAPE, T, kSegments<X>, true, true, true>(g.product, tile, stages_of(g.product, 0), lds, acc)) return;
   const int wave = wave_index(), lane = threadIdx.x % 64;
-  const int64_t f0 = static_cast<int64_t>(tile.a) * (TILE / 2), n0 = static_cast<int64_t>(tile.b) * TILE;
-  const int64_t sub_f = g.hidden_pad / kSub, sub_n = (g.rows + kSub - 1) / kSub;
+  const int f0 = tile.a * (TILE / 2);
+  const int64_t n0 = static_cast<int64_t>(tile.b) * TILE;
+  const int sub_f = static_cast<int>(g.hidden_pad) / kSub, sub_n = static_cast<int>((g.rows + kSub - 1) / kSub);
+  const int at_f = f0 / kSub + (wave % 2) * (kDown / 2), at_n = static_cast<int>(n0) / kSub + (wave / 2) * kAcross;
+  const int inside = static_cast<int>(g.hidden) - at_f * kSub - 4 * (lane / 16);  // this lane's entries that count, 16 to a subtile
+  char* const saved = g.saved + (static_cast<int64_t>(at_n) * sub_f + at_f) * kSubBytes<X>;
 #pragma unroll
   for (int j = 0; j < kAcross; ++j) {
-    const int64_t at_n = n0 / kSub + (wave / 2) * kAcross + j;
 #pragma unroll
     for (int i = 0; i < kDown / 2; ++i) {
-      const int64_t at_f = f0 / kSub + (wave % 2) * (kDown / 2) + i;
       const f32x4 gate = acc[i][j], up = acc[i + kDown / 2][j];
-      if (g.saved != nullptr && at_n < sub_n && at_f < sub_f) {
-        save_pair<X>(g.saved + (at_n * sub_f + at_f) * kSubBytes<X>, lane, gate, up);
+      if (g.saved != nullptr && at_n + j < sub_n && at_f + i < sub_f) {
+        save_pair<X>(saved + (static_cast<int64_t>(j) * sub_f + i) * kSubBytes<X>, lane, gate, up);
       }
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const float x = activate<X, false>(gate[e], g.activation).value * up[e];
-        acc[i][j][e] = at_f * kSub + 4 * (lane / 16) + e < g.hidden ? x : 0.0f;
+        acc[i][j][e] = i * kSub + e < inside ? x : 0.0f;
       }
       __builtin_amdgcn_sched_barrier(0);  // a few outputs at a time: no registers to spill
     }
@@ -200,7 +203,7 @@ __global__ void __launch_bounds__(Shape<TILE>::kThreadsOf, Shape<TILE>::kGroupsO
     __syncthreads();
     for (int k = threadIdx.x; k < TILE * kChunks; k += S::kThreadsOf) {
       const int row = k / kChunks, chunk = k % kChunks;
-      const int64_t f = f0 + chunk * 8;
+      const int f = f0 + chunk * 8;
       if (n0 + row < g.rows && f < g.hidden_pad) {
         *reinterpret_cast<u32x4*>(g.out[part] + (n0 + row) * g.hidden_pad + f) =
             *reinterpret_cast<const u32x4*>(lds + staged<kChunks>(row, chunk) * 8);
@@ -221,26 +224,31 @@ struct SlopeArgs {
   uint16_t* out[3];   // a [rows_pad][hidden_pad], likewise
 };
 
-template <class X, int TILE>
-__global__ void __launch_bounds__(Shape<TILE>::kThreadsOf, Shape<TILE>::kGroupsOf) attnres_ffn_slope_kernel(SlopeArgs g) {
+template <class X, int SHAPE>
+__global__ void __launch_bounds__(Shape<SHAPE>::kAllThreads, Shape<SHAPE>::kGroupsOf) attnres_ffn_slope_kernel(SlopeArgs g) {
   using T = Part<X>;
-  using S = Shape<TILE>;
-  constexpr int kDown = S::kDownOf, kAcross = S::kAcrossOf;
+  using S = Shape<SHAPE>;
+  constexpr int TILE = S::kTileOf, kDown = S::kDownOf, kAcross = S::kAcrossOf;
   __shared__ __align__(16) uint16_t lds[S::kLds];
   TileAt tile;
   if (!tile_at(g.product, g.product.tiles_b, &tile)) return;
   typename S::Sums acc;
-  multiply_tile<TILE, T, kSegments<X>, false, true>(g.product, tile, stages_of(g.product, 0), lds, acc);
+  if (!multiply_tile<SHAPE, T, kSegments<X>, false, true>(g.product, tile, stages_of(g.product, 0), lds, acc)) return;
   const int wave = wave_index(), lane = threadIdx.x % 64;
-  const int64_t f0 = static_cast<int64_t>(tile.a) * TILE, n0 = static_cast<int64_t>(tile.b) * TILE;
-  const int64_t sub_f = g.hidden_pad / kSub, sub_n = (g.rows + kSub - 1) / kSub;
-  const int64_t at_f = f0 / kSub + (wave % 2) * kDown, at_n = n0 / kSub + (wave / 2) * kAcross;
+  const int f0 = tile.a * TILE;
+  const int64_t n0 = static_cast<int64_t>(tile.b) * TILE;
+  const int sub_f = static_cast<int>(g.hidden_pad) / kSub, sub_n = static_cast<int>((g.rows + kSub - 1) / kSub);
+  const int at_f = f0 / kSub + (wave % 2) * kDown, at_n = static_cast<int>(n0) / kSub + (wave / 2) * kAcross;
+  const int inside_f = static_cast<int>(g.hidden) - at_f * kSub - 4 * (lane / 16);  // this lane's entries that count, 16 to a subtile
+  const int inside_n = static_cast<int>(g.rows) - at_n * kSub - lane % 16;
+  const bool whole = f0 + TILE <= g.hidden && n0 + TILE <= g.rows;
   // The saved pairs of a round; the next one's are loaded while a round is stored.
   Pair<X> pairs[kDown];
   const auto load_pairs = [&](int j) {
-    const int64_t n = min(at_n + j, sub_n - 1);  // past the last subtile: the last one's, which are left out
+    // past the last subtile: the last one's, which are left out
+    const char* from = g.saved + static_cast<int64_t>(min(at_n + j, sub_n - 1)) * sub_f * kSubBytes<X>;
 #pragma unroll
-    for (int i = 0; i < kDown; ++i) pairs[i].load(g.saved + (n * sub_f + min(at_f + i, sub_f - 1)) * kSubBytes<X>, lane);
+    for (int i = 0; i < kDown; ++i) pairs[i].load(from + static_cast<int64_t>(min(at_f + i, sub_f - 1)) * kSubBytes<X>, lane);
   };
   load_pairs(0);
   // A round: 16 rows of every wavefront, of three planes in LDS: dg, du and a; of FP32 one of them in its three parts.
@@ -250,33 +258,40 @@ __global__ void __launch_bounds__(Shape<TILE>::kThreadsOf, Shape<TILE>::kGroupsO
   constexpr int kTurns = kParts<X>;
   const auto round = [&](auto number, auto turn_number) {
     constexpr int j = decltype(number)::value, turn = decltype(turn_number)::value;
-    const bool counts = (at_n + j) * kSub + lane % 16 < g.rows;
     const int row = (wave / 2) * 16 + lane % 16;
     if (j + turn > 0) __syncthreads();
+    const auto form = [&](auto all) {  // all: every entry counts
 #pragma unroll
-    for (int i = 0; i < kDown; ++i) {
-      const Pair<X>& pair = pairs[i];
-      float x[3][4];
+      for (int i = 0; i < kDown; ++i) {
+        const Pair<X>& pair = pairs[i];
+        float x[3][4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const bool inside = counts && (at_f + i) * kSub + 4 * (lane / 16) + e < g.hidden;
-        const Activated act = activate<X, true>(pair.gate(e), g.activation);
-        const float da = acc[i][j][e], up = pair.up(e);
-        x[0][e] = inside ? da * up * act.slope : 0.0f;
-        x[1][e] = inside ? da * act.value : 0.0f;
-        x[2][e] = inside ? act.value * up : 0.0f;
+        for (int e = 0; e < 4; ++e) {
+          const Activated act = activate<X, true>(pair.gate(e), g.activation);
+          const float da = acc[i][j][e], up = pair.up(e);
+          x[0][e] = da * up * act.slope;
+          x[1][e] = da * act.value;
+          x[2][e] = act.value * up;
+          if constexpr (!decltype(all)::value) {
+            const bool inside = j * kSub < inside_n && i * kSub + e < inside_f;
+#pragma unroll
+            for (int plane = 0; plane < 3; ++plane) x[plane][e] = inside ? x[plane][e] : 0.0f;
+          }
+        }
+        const int chunk = (wave % 2) * (2 * kDown) + i * 2 + lane / 32;
+        uint16_t* to = lds + staged<kChunks>(row, chunk) * 8 + (lane / 16 % 2) * 4;
+#pragma unroll
+        for (int plane = 0; plane < 3; ++plane) {
+          float* value = x[kTurns == 1 ? plane : turn];
+          const uint32_t packed[2] = {pack2<T>(value[0], value[1]), pack2<T>(value[2], value[3])};
+          *reinterpret_cast<uint64_t*>(to + plane * kPlane) = static_cast<uint64_t>(packed[1]) << 32 | packed[0];
+          if constexpr (kTurns > 1) take_part<T>(value, packed, 4);
+        }
+        if (i % 2 == 1) __builtin_amdgcn_sched_barrier(0);
       }
-      const int chunk = (wave % 2) * (2 * kDown) + i * 2 + lane / 32;
-      uint16_t* to = lds + staged<kChunks>(row, chunk) * 8 + (lane / 16 % 2) * 4;
-#pragma unroll
-      for (int plane = 0; plane < 3; ++plane) {
-        float* value = x[kTurns == 1 ? plane : turn];
-        const uint32_t packed[2] = {pack2<T>(value[0], value[1]), pack2<T>(value[2], value[3])};
-        *reinterpret_cast<uint64_t*>(to + plane * kPlane) = static_cast<uint64_t>(packed[1]) << 32 | packed[0];
-        if constexpr (kTurns > 1) take_part<T>(value, packed, 4);
-      }
-      if (i % 2 == 1) __builtin_amdgcn_sched_barrier(0);
-    }
+    };
+    if (whole) form(std::true_type{});
+    else form(std::false_type{});
     if constexpr (turn + 1 == kTurns && j + 1 < kAcross) load_pairs(j + 1);
     __syncthreads();
 #pragma unroll
@@ -288,7 +303,8 @@ __global__ void __launch_bounds__(Shape<TILE>::kThreadsOf, Shape<TILE>::kGroupsO
       const int64_t first = what == 1 ? g.hidden_pad : 0;
       for (int k = threadIdx.x; k < kRows * kChunks; k += S::kThreadsOf) {
         const int r = k / kChunks, chunk = k % kChunks;
-        const int64_t n = n0 + r / 16 * (16 * kAcross) + j * 16 + r % 16, f = f0 + chunk * 8;
+        const int64_t n = n0 + r / 16 * (16 * kAcross) + j * 16 + r % 16;
+        const int f = f0 + chunk * 8;
         if (n < g.rows_pad && f < g.hidden_pad) {
           *reinterpret_cast<u32x4*>(out + n * ld + first + f) =
               *reinterpret_cast<const u32x4*>(lds + plane * kPlane + staged<kChunks>(r, chunk) * 8);
@@ -323,9 +339,10 @@ struct OutArgs {
 };
 
 // A tile's sums, rounded once or as a part's FP32 sums.
-template <class OUT, int TILE>
-__device__ __forceinline__ void store_tile(const OutArgs& g, const TileAt& tile, const typename Shape<TILE>::Sums& acc, uint16_t* lds) {
-  using S = Shape<TILE>;
+template <class OUT, int SHAPE>
+__device__ __forceinline__ void store_tile(const OutArgs& g, const TileAt& tile, const typename Shape<SHAPE>::Sums& acc, uint16_t* lds) {
+  using S = Shape<SHAPE>;
+  constexpr int TILE = S::kTileOf;
   const int wave = wave_index(), lane = threadIdx.x % 64;
   OUT* out = static_cast<OUT*>(g.out) + tile.split * g.split_stride;
   const int64_t a0 = static_cast<int64_t>(tile.a) * TILE, b0 = static_cast<int64_t>(tile.b) * TILE;
@@ -382,15 +399,15 @@ __device__ __forceinline__ void store_tile(const OutArgs& g, const TileAt& tile,
 }
 
 // Y (A: Wd by rows, B: a by rows).
-template <class X, class OUT, int TILE>
-__global__ void __launch_bounds__(Shape<TILE>::kThreadsOf, Shape<TILE>::kGroupsOf) attnres_ffn_out_kernel(OutArgs g) {
-  using S = Shape<TILE>;
+template <class X, class OUT, int SHAPE>
+__global__ void __launch_bounds__(Shape<SHAPE>::kAllThreads, Shape<SHAPE>::kGroupsOf) attnres_ffn_out_kernel(OutArgs g) {
+  using S = Shape<SHAPE>;
   __shared__ __align__(16) uint16_t lds[S::kLds];
   TileAt tile;
   if (!tile_at(g.product, g.product.tiles_b, &tile)) return;
   typename S::Sums acc;
-  multiply_tile<TILE, Part<X>, kSegments<X>, true, true>(g.product, tile, stages_of(g.product, tile.split), lds, acc);
-  store_tile<OUT, TILE>(g, tile, acc, lds);
+  if (!multiply_tile<SHAPE, Part<X>, kSegments<X>, true, true>(g.product, tile, stages_of(g.product, tile.split), lds, acc)) return;
+  store_tile<OUT, SHAPE>(g, tile, acc, lds);
 }
 
 // dX (A: W by columns, B: [dg du] by rows), dW (A: X, B: [dg du], both by columns) and dWd (A: a, B: dY, both by columns) in one
@@ -401,9 +418,9 @@ struct GradientsArgs {
   int b_rows[3], wide[3];
 };
 
-template <class X, int TILE>
-__global__ void __launch_bounds__(Shape<TILE>::kThreadsOf, Shape<TILE>::kGroupsOf) attnres_ffn_gradients_kernel(GradientsArgs args) {
-  using S = Shape<TILE>;
+template <class X, int SHAPE>
+__global__ void __launch_bounds__(Shape<SHAPE>::kAllThreads, Shape<SHAPE>::kGroupsOf) attnres_ffn_gradients_kernel(GradientsArgs args) {
+  using S = Shape<SHAPE>;
   __shared__ __align__(16) uint16_t lds[S::kLds];
   const int which = (blockIdx.x >= args.first[1] ? 1 : 0) + (blockIdx.x >= args.first[2] ? 1 : 0);
   const OutArgs& g = args.of[which];
@@ -412,12 +429,12 @@ __global__ void __launch_bounds__(Shape<TILE>::kThreadsOf, Shape<TILE>::kGroupsO
   const Stages stages = stages_of(g.product, tile.split);
   typename S::Sums acc;
   if (args.b_rows[which]) {
-    multiply_tile<TILE, Part<X>, kSegments<X>, false, true>(g.product, tile, stages, lds, acc);
+    if (!multiply_tile<SHAPE, Part<X>, kSegments<X>, false, true>(g.product, tile, stages, lds, acc)) return;
   } else {
-    multiply_tile<TILE, Part<X>, kSegments<X>, false, false>(g.product, tile, stages, lds, acc);
+    if (!multiply_tile<SHAPE, Part<X>, kSegments<X>, false, false>(g.product, tile, stages, lds, acc)) return;
   }
-  if (std::is_same_v<X, float> || args.wide[which]) store_tile<float, TILE>(g, tile, acc, lds);
-  else store_tile<X, TILE>(g, tile, acc, lds);
+  if (std::is_same_v<X, float> || args.wide[which]) store_tile<float, SHAPE>(g, tile, acc, lds);
+  else store_tile<X, SHAPE>(g, tile, acc, lds);
 }
 
 // out[r] = the sum of the parts' rows, in order.
@@ -473,9 +490,11 @@ __global__ void __launch_bounds__(kBlock) attnres_ffn_pack_kernel(PackArgs<X> g)
 }
 
 // ------------------------------------------------------------------- few rows
-// The forward of up to kFewRows rows reads the weights once and is bound by that: wavefronts share the depth of 16
-// entries of A (of a gate's 8 and the up projection's 8 that belong to them), so that all of a workgroup's weights are asked
-// for at once, and no operand is packed.  FP32 inputs by FP32 matrix instructions, which so few rows have time for.
+// The forward of up to 16 rows, or of kFewRows where tiles need packed weights, reads the weights once and is bound by that: wavefronts
+// share the depth of 16 entries of A (of a gate's 8 and the up projection's 8 that belong to them), so that all of a workgroup's weights
+// are asked for at once, and nothing is packed.  FP32 inputs by FP32 matrix instructions, which so few rows have time for.
+// A lane's 16 bytes are of a row of its own, which the caches serve slowly: BF16, 2048 x 5632, by tiles in brackets, 1 row 19.2 (31) us, 16
+// 26.2 (25.8), 48 46.6 (26.8); 1024 x 2816, 1 row 10.7 (20), 32 15.9 (18.4).
 constexpr int64_t kFewRows = 64;
 
 // The wavefronts' sums over their shares of the depth, in LDS; ROWS of a's tiles by TILES of the rows'.
@@ -636,6 +655,8 @@ struct Sizes {
 // How products are shared out: the tiles' size, and the parts that the depth of each is cut into.
 struct Cut {
   int tile, splits[3];
+  bool shared;  // the depth of tiles of 64, by more wavefronts: a unit has one workgroup at most
+  int shape() const { return tile + (shared ? 1 : 0); }
 };
 struct Outputs {
   int64_t a, b, depth;  // entries; 0: not asked for
@@ -696,7 +717,7 @@ class Schedule {
 // The cut that takes the least time: the schedule of all tiles at a unit's rate for them, and the partial sums' way to memory and
 // back.  Rates as measured on a full chip.
 Cut choose_cut(const Outputs* outputs, int count, int segments, bool whole) {
-  Cut best{256, {1, 1, 1}};
+  Cut best{256, {1, 1, 1}, false};
   double least = 0.0;
   for (const int tile : {256, 128, 64}) {
     // a workgroup alone on a unit that has room for more reaches two thirds of its rate
@@ -709,11 +730,14 @@ Cut choose_cut(const Outputs* outputs, int count, int segments, bool whole) {
       fits = fits && (tile == 256 || tiles[i] <= kMaxTiles);
     }
     if (!fits) continue;
-    Cut cut{tile, {1, 1, 1}};
+    Cut cut{tile, {1, 1, 1}, false};
     for (;;) {
       double each[3], partial = 0.0;
       int order[3] = {0, 1, 2};
+      int64_t workgroups = 0, least_depth = int64_t{1} << 40;
       for (int i = 0; i < count; ++i) {
+        workgroups += tiles[i] * cut.splits[i];
+        if (tiles[i] > 0) least_depth = std::min(least_depth, outputs[i].depth / cut.splits[i]);
         each[i] = 2.0 * tile * tile * static_cast<double>(outputs[i].depth) * segments / cut.splits[i] / rate;
         if (cut.splits[i] > 1) partial += 4e-6 + 8.0 * static_cast<double>(outputs[i].a * outputs[i].b) * cut.splits[i] / 4.5e12;
       }
@@ -725,6 +749,7 @@ Cut choose_cut(const Outputs* outputs, int count, int segments, bool whole) {
       if (least == 0.0 || time < least) {
         least = time;
         best = cut;
+        best.shared = tile == 64 && workgroups <= kUnits && least_depth / kDepth >= 16;
       }
       if (whole || cut.splits[longest] >= 32 || outputs[longest].depth / kDepth / (cut.splits[longest] + 1) < 4) break;
       ++cut.splits[longest];
@@ -743,7 +768,7 @@ FfnPlan ffn_plan(const Sizes& s, int pass) {
   p.hidden_pad = round_up(s.hidden, kDepth);
   p.out_pad = round_up(s.out_width, kDepth);
   // the depth of a product is a whole number of stages, the rest of the last one zeros
-  p.few = s.rows <= kFewRows;
+  p.few = s.rows <= (split || s.width != p.width_pad || s.hidden != p.hidden_pad ? kFewRows : kFewRows / 4);
   const bool tiles = backward || !p.few;
   p.pack_x = tiles && (split || s.width != p.width_pad || (backward && s.rows != p.rows_pad));
   p.pack_gate_up = tiles && (split || s.width != p.width_pad || s.hidden != p.hidden_pad);
@@ -809,10 +834,13 @@ struct Call {
 };
 
 template <class F>
-void with_tile(int tile, F f) {
-  if (tile == 256) f(std::integral_constant<int, 256>{});
-  else if (tile == 128) f(std::integral_constant<int, 128>{});
-  else f(std::integral_constant<int, 64>{});
+void with_shape(const Cut& cut, F f) {
+  switch (cut.shape()) {
+    case 256: return f(std::integral_constant<int, 256>{});
+    case 128: return f(std::integral_constant<int, 128>{});
+    case 65: return f(std::integral_constant<int, 65>{});
+    default: return f(std::integral_constant<int, 64>{});
+  }
 }
 
 // An operand where it lies, or packed into the workspace; `half`, `half_pad`: see PackArgs.
@@ -863,9 +891,9 @@ void launch_gate(const Call& c, const Operand& x, const Operand& gate_up, char* 
   g.activation = c.activation;
   g.saved = saved;
   for (int k = 0; a != nullptr && k < kParts<X>; ++k) g.out[k] = c.operand(a[k]);
-  with_tile(tile, [&](auto size) {
-    constexpr int TILE = decltype(size)::value;
-    hipLaunchKernelGGL((attnres_ffn_gate_kernel<X, TILE>), dim3(g.product.tiles_a * g.product.tiles_b), dim3(Shape<TILE>::kThreadsOf), 0,
+  with_shape(p.gate, [&](auto size) {
+    constexpr int SHAPE = decltype(size)::value;
+    hipLaunchKernelGGL((attnres_ffn_gate_kernel<X, SHAPE>), dim3(g.product.tiles_a * g.product.tiles_b), dim3(Shape<SHAPE>::kAllThreads), 0,
                        c.stream, g);
   });
 }
@@ -937,10 +965,10 @@ void ffn_forward(const Call& c, void* out, char* saved) {
   a.entries = c.s.rows;
   const int splits = p.out.splits[0];
   const OutArgs g = out_args(c, down, a, p.hidden_pad, c.s.out_width, c.s.rows, c.s.rows, c.s.rows, p.out.tile, splits, 0, out);
-  with_tile(p.out.tile, [&](auto size) {
-    constexpr int TILE = decltype(size)::value;
-    const auto kernel = splits > 1 ? attnres_ffn_out_kernel<X, float, TILE> : attnres_ffn_out_kernel<X, X, TILE>;
-    hipLaunchKernelGGL(kernel, dim3(workgroups(g)), dim3(Shape<TILE>::kThreadsOf), 0, c.stream, g);
+  with_shape(p.out, [&](auto size) {
+    constexpr int SHAPE = decltype(size)::value;
+    const auto kernel = splits > 1 ? attnres_ffn_out_kernel<X, float, SHAPE> : attnres_ffn_out_kernel<X, X, SHAPE>;
+    hipLaunchKernelGGL(kernel, dim3(workgroups(g)), dim3(Shape<SHAPE>::kAllThreads), 0, c.stream, g);
   });
   if (splits > 1) join_parts<X>(c, g, out);
 }
@@ -979,9 +1007,9 @@ void ffn_backward(const Call& c, const void* grad_out, const char* saved, void* 
       if (grad_x != nullptr || grad_gate_up != nullptr) g.both[k] = c.operand(p.both[k]);
       if (grad_down != nullptr) g.out[k] = c.operand(p.a[k]);
     }
-    with_tile(tile, [&](auto size) {
-      constexpr int TILE = decltype(size)::value;
-      hipLaunchKernelGGL((attnres_ffn_slope_kernel<X, TILE>), dim3(g.product.tiles_a * g.product.tiles_b), dim3(Shape<TILE>::kThreadsOf), 0,
+    with_shape(p.slope, [&](auto size) {
+      constexpr int SHAPE = decltype(size)::value;
+      hipLaunchKernelGGL((attnres_ffn_slope_kernel<X, SHAPE>), dim3(g.product.tiles_a * g.product.tiles_b), dim3(Shape<SHAPE>::kAllThreads), 0,
                          c.stream, g);
     });
   }
@@ -1032,9 +1060,9 @@ void ffn_backward(const Call& c, const void* grad_out, const char* saved, void* 
     grid += static_cast<uint32_t>(round_up(workgroups(of[i]), 8));  // whole rounds of the XCDs
   }
   for (int k = count; k < 3; ++k) g.first[k] = UINT32_MAX;
-  with_tile(tile, [&](auto size) {
-    constexpr int TILE = decltype(size)::value;
-    hipLaunchKernelGGL((attnres_ffn_gradients_kernel<X, TILE>), dim3(grid), dim3(Shape<TILE>::kThreadsOf), 0, c.stream, g);
+  with_shape(p.gradients, [&](auto size) {
+    constexpr int SHAPE = decltype(size)::value;
+    hipLaunchKernelGGL((attnres_ffn_gradients_kernel<X, SHAPE>), dim3(grid), dim3(Shape<SHAPE>::kAllThreads), 0, c.stream, g);
   });
   for (int i = 0; i < 3; ++i) {
     if (results[i] != nullptr && splits[i] > 1) join_parts<X>(c, of[i], results[i]);

@@ -368,16 +368,23 @@ __device__ __forceinline__ void multiply(const Product& p, const TileAt& tile, c
 // they are read by whole lines of 128 bytes (4096 x 16384 x 4096, both as rows, tiles of 128: 710 -> 614 us), else 32, twice as many stages ahead
 // (both as columns: 610 -> 592; tiles of 64 are faster with 64, 55 -> 47 us for 1024 x 5632 x 2048).  A step is 32 k's, and the next
 // one's fragments are read meanwhile.
-template <int TILE>
+// SHAPE: the tile's size, or 65: tiles of 64 by four times as many wavefronts, which share the depth and have a ring of stages each.  For launches of
+// one workgroup to a unit, which has nothing else to do while a step's reads and the barrier are waited for (64 x 11264 x 2048 19.6 -> 13.0 us,
+// 1024 x 1024 x 2816 24.6 -> 16.4; more stages ahead change nothing).
+template <int SHAPE>
 struct Shape {
-  static constexpr int kTileOf = TILE;
-  static constexpr int kWavesOf = TILE == 256 ? kWaves : 4;  // two along A, the others along B
-  static constexpr int kThreadsOf = 64 * kWavesOf;
-  static constexpr int kGroupsOf = TILE == 64 ? 4 : 2;  // wavefronts per SIMD, and workgroups per unit of the smaller tiles
+  static constexpr bool kShared = SHAPE == 65;
+  static constexpr int kTileOf = SHAPE - (kShared ? 1 : 0), TILE = kTileOf;
+  static constexpr int kWavesOf = TILE == 256 ? kWaves : 4;  // of a sharer: two along A, the others along B
+  static constexpr int kSharers = kShared ? 4 : 1;
+  static constexpr int kThreadsOf = 64 * kWavesOf;           // of the epilogue
+  static constexpr int kAllThreads = kThreadsOf * kSharers;
+  static constexpr int kGroupsOf = TILE == 64 ? 4 : 2;       // wavefronts per SIMD
   static constexpr int kDownOf = TILE / 32;
   static constexpr int kAcrossOf = TILE == 256 ? kAcross : TILE / 32;
   static constexpr int kPairedOf = kDownOf * 8;  // PAIRED rows: entries of a wavefront's half
-  static constexpr int kLds = kStages * 2 * TILE * kDepth;  // 16-bit elements: 4 stages of 32 k's, or 2 of 64
+  static constexpr int kRing = kStages * 2 * TILE * kDepth;  // 16-bit elements: 4 stages of 32 k's, or 2 of 64
+  static constexpr int kLds = kRing * kSharers;
   using Sums = f32x4[kDownOf][kAcrossOf];
 };
 static_assert(Shape<256>::kDownOf == kDown && Shape<256>::kPairedOf == kPaired, "one shape");
@@ -391,7 +398,7 @@ __device__ __forceinline__ int small_column_swizzle(int k) {
 
 template <int TILE, int DEPTH, bool ROWS, bool PAIRED>
 struct SmallLoader {
-  using S = Shape<TILE>;
+  using S = Shape<TILE>;  // its tile and wavefronts are all that is used
   static constexpr int kLoadsOf = TILE * DEPTH / 512 / S::kWavesOf;  // of 1 KB per wavefront and stage
   static constexpr int kRowsOfLoad = ROWS ? 8 : 512 / TILE, kLanesOfRow = 64 / kRowsOfLoad;
   uint32_t offset[kLoadsOf];  // bytes from the stage's origin; columns: of the chunk alone
@@ -453,14 +460,21 @@ struct SmallReader {
   }
 };
 
-// As multiply(): the sum of a tile over its split's k's (at least one stage of 32).
-template <int TILE, class T, int SEGMENTS, bool A_ROWS, bool B_ROWS, bool PAIRED>
-__device__ __forceinline__ void small_multiply(const Product& p, const TileAt& tile, const Stages& range, uint16_t* lds,
-                                               typename Shape<TILE>::Sums& acc) {
-  using S = Shape<TILE>;
-  constexpr int kDownOf = S::kDownOf, kAcrossOf = S::kAcrossOf;
+// As multiply(): the sum of a tile over its split's k's (at least one stage of 32 for each sharer).  False for the wavefronts that
+// have no part in the epilogue: they end, and barriers are then met by the others alone.
+template <int SHAPE, class T, int SEGMENTS, bool A_ROWS, bool B_ROWS, bool PAIRED>
+__device__ __forceinline__ bool small_multiply(const Product& p, const TileAt& tile, const Stages& whole, uint16_t* lds,
+                                               typename Shape<SHAPE>::Sums& acc) {
+  using S = Shape<SHAPE>;
+  constexpr int TILE = S::kTileOf, kDownOf = S::kDownOf, kAcrossOf = S::kAcrossOf, kSharers = S::kSharers;
   constexpr int kSteps = A_ROWS || B_ROWS || TILE == 64 ? 2 : 1, kDepthOf = kSteps * kDepth, kStagesOf = kStages / kSteps;
-  const int wave = wave_index(), lane = threadIdx.x % 64;
+  const int wave = wave_index() % S::kWavesOf, sharer = wave_index() / S::kWavesOf, lane = threadIdx.x % 64;
+  // a sharer's stages, at least one; by pairs of 32 k's, so that lines stay whole
+  const auto share = [&](int which) {
+    const int pairs = (whole.count + 1) / 2, from = pairs * which / kSharers, to = pairs * (which + 1) / kSharers;
+    return Stages{whole.first + 2 * from, min(2 * (to - from), whole.count - 2 * from)};
+  };
+  const Stages range = kSharers == 1 ? whole : share(sharer);
 #pragma unroll
   for (int i = 0; i < kDownOf; ++i) {
 #pragma unroll
@@ -477,7 +491,7 @@ __device__ __forceinline__ void small_multiply(const Product& p, const TileAt& t
   const int64_t origin_a = (A_ROWS ? a0 * p.a.ld : a0) * 2, origin_b = (B_ROWS ? b0 * p.b.ld : b0) * 2;
   const int64_t next_a = (A_ROWS ? 1 : p.a.ld) * kDepthOf * 2, next_b = (B_ROWS ? 1 : p.b.ld) * kDepthOf * 2;
   const int64_t from_a = origin_a + first * (next_a / kSteps), from_b = origin_b + first * (next_b / kSteps);
-  const uint32_t lds0 = lds_byte(lds);
+  const uint32_t lds0 = lds_byte(lds + sharer * S::kRing);
   constexpr uint32_t kB = TILE * kDepthOf * 2, kStageBytes = 2 * kB;
   const uint32_t slot = wave * (kLoadsOf * 1024);
   int segment = 0, stage = 0;  // of the next load
@@ -512,6 +526,7 @@ __device__ __forceinline__ void small_multiply(const Product& p, const TileAt& t
     for (int r = 0; r < kReads; ++r) read(buffer, 0, f, r);
   };
   // Every wavefront's reads from LDS are done and its loads have landed but for those of `ahead` stages.
+  static_assert((kStagesOf - 1) * 2 * kLoadsOf < 64, "the counter has six bits");
   const auto arrived = [&](auto ahead) {
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"i"(decltype(ahead)::value * 2 * kLoadsOf) : "memory");
     __builtin_amdgcn_s_barrier();
@@ -576,14 +591,40 @@ __device__ __forceinline__ void small_multiply(const Product& p, const TileAt& t
       products(lower, nothing);
     }
   }
+  if constexpr (kSharers > 1) {
+    // as many barriers as the sharer with the most stages has met
+    int most = 0;
+    for (int which = 0; which < kSharers; ++which) most = max(most, (share(which).count + kSteps - 1) / kSteps * SEGMENTS);
+    for (int extra = total; extra < most; ++extra) __builtin_amdgcn_s_barrier();
+    __syncthreads();
+    // the first sharer adds up the sums, in order; the others are done
+    f32x4* sums = reinterpret_cast<f32x4*>(lds);
+    const auto place = [&](int which, int m) { return (((which - 1) * S::kWavesOf + wave) * kProducts + m) * 64 + lane; };
+    if (sharer > 0) {
+#pragma unroll
+      for (int m = 0; m < kProducts; ++m) sums[place(sharer, m)] = acc[m / kAcrossOf][m % kAcrossOf];
+    }
+    __syncthreads();
+    if (sharer > 0) return false;
+#pragma unroll
+    for (int which = 1; which < kSharers; ++which) {
+#pragma unroll
+      for (int m = 0; m < kProducts; ++m) acc[m / kAcrossOf][m % kAcrossOf] += sums[place(which, m)];
+    }
+  }
   __syncthreads();  // LDS is free for the epilogue
+  return true;
 }
 
-template <int TILE, class T, int SEGMENTS, bool A_ROWS, bool B_ROWS, bool PAIRED = false>
-__device__ __forceinline__ void multiply_tile(const Product& p, const TileAt& tile, const Stages& range, uint16_t* lds,
-                                              typename Shape<TILE>::Sums& acc) {
-  if constexpr (TILE == 256) multiply<T, SEGMENTS, A_ROWS, B_ROWS, PAIRED>(p, tile, range, lds, acc);
-  else small_multiply<TILE, T, SEGMENTS, A_ROWS, B_ROWS, PAIRED>(p, tile, range, lds, acc);
+template <int SHAPE, class T, int SEGMENTS, bool A_ROWS, bool B_ROWS, bool PAIRED = false>
+__device__ __forceinline__ bool multiply_tile(const Product& p, const TileAt& tile, const Stages& range, uint16_t* lds,
+                                              typename Shape<SHAPE>::Sums& acc) {
+  if constexpr (SHAPE == 256) {
+    multiply<T, SEGMENTS, A_ROWS, B_ROWS, PAIRED>(p, tile, range, lds, acc);
+    return true;
+  } else {
+    return small_multiply<SHAPE, T, SEGMENTS, A_ROWS, B_ROWS, PAIRED>(p, tile, range, lds, acc);
+  }
 }
 
 // ------------------------------------------------------------- few rows
