@@ -437,56 +437,95 @@ __global__ void __launch_bounds__(Shape<SHAPE>::kAllThreads, Shape<SHAPE>::kGrou
   else store_tile<X, SHAPE>(g, tile, acc, lds);
 }
 
+// Passes over rows of chunks of kVec, several tensors in one launch: a workgroup takes whole rows, kChunksOfGroup chunks or one row.
+constexpr int kChunksOfGroup = 4 * kBlock;
+
+struct Rows {
+  int64_t rows;
+  int chunks;      // of a row
+  uint32_t first;  // workgroup; UINT32_MAX: not there
+  __host__ __device__ int of_group() const { return chunks >= kChunksOfGroup ? 1 : kChunksOfGroup / chunks; }
+  uint32_t groups() const { return static_cast<uint32_t>((rows + of_group() - 1) / of_group()); }
+};
+
+// f(row, chunk) for the workgroup's rows.
+template <class F>
+__device__ __forceinline__ void for_chunks(const Rows& r, F f) {
+  const int of_group = r.of_group();
+  const int64_t row0 = static_cast<int64_t>(blockIdx.x - r.first) * of_group;
+  const int here = static_cast<int>(min(static_cast<int64_t>(of_group), r.rows - row0)) * r.chunks;
+  for (int i = threadIdx.x; i < here; i += kBlock) f(row0 + i / r.chunks, i % r.chunks);
+}
+
 // out[r] = the sum of the parts' rows, in order.
 template <class X>
-__global__ void __launch_bounds__(kBlock) attnres_ffn_join_kernel(const float* __restrict__ partial, int splits, int64_t split_stride,
-                                                                  int64_t ld, int64_t rows, int width, X* __restrict__ out) {
-  const int chunks = (width + kVec - 1) / kVec;
-  const int64_t all = rows * chunks;
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * kBlock + threadIdx.x; i < all; i += static_cast<int64_t>(gridDim.x) * kBlock) {
-    const int64_t r = i / chunks;
-    const int c = static_cast<int>(i - r * chunks) * kVec;
+struct JoinArgs {
+  Rows rows[3];
+  const float* partial[3];
+  int splits[3], width[3];
+  int64_t split_stride[3];
+  X* out[3];
+};
+
+template <class X>
+__global__ void __launch_bounds__(kBlock) attnres_ffn_join_kernel(JoinArgs<X> g) {
+  const int which = (blockIdx.x >= g.rows[1].first ? 1 : 0) + (blockIdx.x >= g.rows[2].first ? 1 : 0);
+  const int splits = g.splits[which], width = g.width[which];
+  const int64_t stride = g.split_stride[which];
+  const float* partial = g.partial[which];
+  X* out = g.out[which];
+  const int64_t ld = static_cast<int64_t>(g.rows[which].chunks) * kVec;  // rows are padded to whole chunks
+  for_chunks(g.rows[which], [&](int64_t r, int chunk) {
+    const float* from = partial + r * ld + chunk * kVec;
     float sum[kVec] = {};
 #pragma unroll 4
     for (int k = 0; k < splits; ++k) {
       float x[kVec];
-      load8(partial + k * split_stride + r * ld + c, x);  // rows are padded to whole chunks
+      load8(from + k * stride, x);
 #pragma unroll
       for (int e = 0; e < kVec; ++e) sum[e] += x[e];
     }
-    store_chunk(out + r * width, c, width, sum);
-  }
+    store_chunk(out + r * width, chunk * kVec, width, sum);
+  });
 }
 
 // Rows to operands: [2 or 1 halves of half_pad][width_pad], zero-padded, of rows in halves of `half`.
 template <class X>
 struct PackArgs {
+  Rows rows;  // of the operand
   const X* x;
-  int64_t stride, half, half_pad, rows_out;
-  int width, width_pad;
+  int64_t stride, half, half_pad;
+  int width;
   uint16_t* to[3];
 };
 
 template <class X>
-__global__ void __launch_bounds__(kBlock) attnres_ffn_pack_kernel(PackArgs<X> g) {
+struct PacksArgs {
+  PackArgs<X> of[4];
+};
+
+template <class X>
+__global__ void __launch_bounds__(kBlock) attnres_ffn_pack_kernel(PacksArgs<X> args) {
   using T = Part<X>;
-  const int chunks = g.width_pad / kVec;
-  const int64_t all = g.rows_out * chunks;
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * kBlock + threadIdx.x; i < all; i += static_cast<int64_t>(gridDim.x) * kBlock) {
-    const int64_t r = i / chunks;
-    const int c = static_cast<int>(i - r * chunks) * kVec;
+  int which = 0;
+#pragma unroll
+  for (int k = 1; k < 4; ++k) which += blockIdx.x >= args.of[k].rows.first ? 1 : 0;
+  const PackArgs<X>& g = args.of[which];
+  for_chunks(g.rows, [&](int64_t r, int chunk) {
+    const int c = chunk * kVec;
     const int64_t second = r >= g.half_pad ? 1 : 0, within = r - second * g.half_pad;
     float v[kVec] = {};
     if (within < g.half && c < g.width) load_chunk(g.x + (second * g.half + within) * g.stride, c, g.width, v);
+    const int64_t at = (r * g.rows.chunks + chunk) * kVec;
 #pragma unroll
     for (int part = 0; part < kParts<X>; ++part) {
       uint32_t packed[kVec / 2];
 #pragma unroll
       for (int e = 0; e < kVec / 2; ++e) packed[e] = pack2<T>(v[2 * e], v[2 * e + 1]);
-      *reinterpret_cast<u32x4*>(g.to[part] + i * kVec) = u32x4{packed[0], packed[1], packed[2], packed[3]};
+      *reinterpret_cast<u32x4*>(g.to[part] + at) = u32x4{packed[0], packed[1], packed[2], packed[3]};
       if (part + 1 < kParts<X>) take_part<T>(v, packed, kVec);
     }
-  }
+  });
 }
 
 // ------------------------------------------------------------------- few rows
@@ -731,6 +770,8 @@ Cut choose_cut(const Outputs* outputs, int count, int segments, bool whole) {
     }
     if (!fits) continue;
     Cut cut{tile, {1, 1, 1}, false};
+    int worse = 0;  // cuts since the best one of this size
+    double nearest = 1e9;
     for (;;) {
       double each[3], partial = 0.0;
       int order[3] = {0, 1, 2};
@@ -746,19 +787,25 @@ Cut choose_cut(const Outputs* outputs, int count, int segments, bool whole) {
       for (int i = 0; i < count; ++i) schedule.add(tiles[order[i]] * cut.splits[order[i]], each[order[i]]);
       const int longest = order[0];
       const double time = std::max(schedule.end(), alone * each[longest]) + partial;
+      worse = time < nearest ? 0 : worse + 1;
+      nearest = std::min(nearest, time);
       if (least == 0.0 || time < least) {
         least = time;
         best = cut;
         best.shared = tile == 64 && workgroups <= kUnits && least_depth / kDepth >= 16;
       }
-      if (whole || cut.splits[longest] >= 32 || outputs[longest].depth / kDepth / (cut.splits[longest] + 1) < 4) break;
+      if (whole || worse == 4 || cut.splits[longest] >= 32 || outputs[longest].depth / kDepth / (cut.splits[longest] + 1) < 4) break;
       ++cut.splits[longest];
     }
   }
   return best;
 }
 
-FfnPlan ffn_plan(const Sizes& s, int pass) {
+int64_t saved_bytes(const Sizes& s) {
+  return tiles_of(s.rows, kSub) * (round_up(s.hidden, kDepth) / kSub) * (s.dtype == ATTNRES_F32 ? kSubBytes<float> : kSubBytes<Bf16>);
+}
+
+FfnPlan make_plan(const Sizes& s, int pass) {
   FfnPlan p{};
   const bool split = s.dtype == ATTNRES_F32, backward = pass != kForward;
   p.parts = split ? 3 : 1;
@@ -774,7 +821,7 @@ FfnPlan ffn_plan(const Sizes& s, int pass) {
   p.pack_gate_up = tiles && (split || s.width != p.width_pad || s.hidden != p.hidden_pad);
   p.pack_down = tiles && (split || s.hidden != p.hidden_pad || (backward && s.out_width != p.out_pad));
   p.pack_grad = backward && (split || s.out_width != p.out_pad || s.rows != p.rows_pad);
-  p.saved_bytes = tiles_of(s.rows, kSub) * (p.hidden_pad / kSub) * (split ? kSubBytes<float> : kSubBytes<Bf16>);
+  p.saved_bytes = saved_bytes(s);
   int64_t at = 0;
   const auto take = [&](int64_t bytes) {
     const int64_t from = at;
@@ -816,7 +863,26 @@ FfnPlan ffn_plan(const Sizes& s, int pass) {
   return p;
 }
 
-unsigned stride_grid(int64_t items) { return static_cast<unsigned>(std::min<int64_t>((items + kBlock - 1) / kBlock, 8192)); }
+// The plan of these sizes; a call asks for it up to three times, and a program for the same few.
+const FfnPlan& ffn_plan(const Sizes& s, int pass) {
+  struct Known {
+    Sizes s{-1, 0, 0, 0, 0};
+    int pass = 0;
+    FfnPlan plan{};
+  };
+  thread_local Known known[8];
+  thread_local int oldest = 0;
+  for (const Known& k : known) {
+    if (k.pass == pass && k.s.rows == s.rows && k.s.width == s.width && k.s.hidden == s.hidden && k.s.out_width == s.out_width &&
+        k.s.dtype == s.dtype) {
+      return k.plan;
+    }
+  }
+  Known& k = known[oldest];
+  oldest = (oldest + 1) % 8;
+  k = {s, pass, make_plan(s, pass)};
+  return k.plan;
+}
 
 struct Call {
   Sizes s;
@@ -843,35 +909,46 @@ void with_shape(const Cut& cut, F f) {
   }
 }
 
-// An operand where it lies, or packed into the workspace; `half`, `half_pad`: see PackArgs.
+// Operands where they lie, or packed into the workspace, all by one launch.
 template <class X>
-Operand place_operand(const Call& c, bool pack, const int64_t* offsets, const void* x, int64_t stride, int64_t half, int64_t half_pad,
-                      int64_t rows_out, int64_t width, int64_t width_pad) {
-  if (!pack) return {{static_cast<const uint16_t*>(x), nullptr, nullptr}, stride, 0, 0, 0};
-  PackArgs<X> g{static_cast<const X*>(x), stride, half, half_pad, rows_out, static_cast<int>(width), static_cast<int>(width_pad), {}};
-  Operand o{{nullptr, nullptr, nullptr}, width_pad, 0, 0, 0};
-  for (int k = 0; k < kParts<X>; ++k) o.part[k] = g.to[k] = c.operand(offsets[k]);
-  hipLaunchKernelGGL((attnres_ffn_pack_kernel<X>), dim3(stride_grid(rows_out * width_pad / kVec)), dim3(kBlock), 0, c.stream, g);
-  return o;
-}
+class Operands {
+ public:
+  explicit Operands(const Call& c) : c_(c) {
+    for (auto& p : args_.of) p.rows.first = UINT32_MAX;
+  }
+  Operand x() { return place(c_.plan.pack_x, c_.plan.x, c_.x, c_.x_stride, c_.s.rows, c_.plan.rows_pad, 1, c_.s.width, c_.plan.width_pad); }
+  Operand gate_up() {
+    return place(c_.plan.pack_gate_up, c_.plan.gate_up, c_.gate_up, c_.gate_up_stride, c_.s.hidden, c_.plan.hidden_pad, 2, c_.s.width,
+                 c_.plan.width_pad);
+  }
+  Operand down() {
+    return place(c_.plan.pack_down, c_.plan.down, c_.down, c_.down_stride, c_.s.out_width, c_.plan.out_pad, 1, c_.s.hidden,
+                 c_.plan.hidden_pad);
+  }
+  Operand grad(const void* grad) {
+    return place(c_.plan.pack_grad, c_.plan.grad, grad, c_.s.out_width, c_.s.rows, c_.plan.rows_pad, 1, c_.s.out_width, c_.plan.out_pad);
+  }
+  void pack() {
+    if (count_ > 0) hipLaunchKernelGGL((attnres_ffn_pack_kernel<X>), dim3(groups_), dim3(kBlock), 0, c_.stream, args_);
+  }
 
-template <class X>
-Operand place_x(const Call& c) {
-  const FfnPlan& p = c.plan;
-  return place_operand<X>(c, p.pack_x, p.x, c.x, c.x_stride, c.s.rows, p.rows_pad, p.rows_pad, c.s.width, p.width_pad);
-}
-template <class X>
-Operand place_gate_up(const Call& c) {
-  const FfnPlan& p = c.plan;
-  return place_operand<X>(c, p.pack_gate_up, p.gate_up, c.gate_up, c.gate_up_stride, c.s.hidden, p.hidden_pad, 2 * p.hidden_pad,
-                          c.s.width, p.width_pad);
-}
-template <class X>
-Operand place_down(const Call& c) {
-  const FfnPlan& p = c.plan;
-  return place_operand<X>(c, p.pack_down, p.down, c.down, c.down_stride, c.s.out_width, p.out_pad, p.out_pad, c.s.hidden,
-                          p.hidden_pad);
-}
+ private:
+  Operand place(bool pack, const int64_t* offsets, const void* x, int64_t stride, int64_t half, int64_t half_pad, int halves, int64_t width,
+                int64_t width_pad) {
+    if (!pack) return {{static_cast<const uint16_t*>(x), nullptr, nullptr}, stride, 0, 0, 0};
+    PackArgs<X>& g = args_.of[count_++];
+    g = {{halves * half_pad, static_cast<int>(width_pad / kVec), groups_}, static_cast<const X*>(x), stride, half, half_pad,
+         static_cast<int>(width), {}};
+    groups_ += g.rows.groups();
+    Operand o{{nullptr, nullptr, nullptr}, width_pad, 0, 0, 0};
+    for (int k = 0; k < kParts<X>; ++k) o.part[k] = g.to[k] = c_.operand(offsets[k]);
+    return o;
+  }
+  const Call& c_;
+  PacksArgs<X> args_{};
+  int count_ = 0;
+  uint32_t groups_ = 0;
+};
 
 // g and u, and a from them.
 template <class X>
@@ -945,20 +1022,35 @@ OutArgs out_args(const Call& c, const Operand& a, const Operand& b, int64_t dept
 
 unsigned workgroups(const OutArgs& g) { return static_cast<unsigned>(g.product.tiles_a) * g.product.tiles_b * g.product.splits; }
 
+// The sums of the parts of those of three products that are cut.
 template <class X>
-void join_parts(const Call& c, const OutArgs& g, void* out) {
-  const int64_t rows = g.split_stride / g.ld;
-  hipLaunchKernelGGL((attnres_ffn_join_kernel<X>), dim3(stride_grid(rows * (g.ld / kVec))), dim3(kBlock), 0, c.stream,
-                     static_cast<const float*>(g.out), g.product.splits, g.split_stride, g.ld, rows, static_cast<int>(g.entries_a),
-                     static_cast<X*>(out));
+void join_parts(const Call& c, const OutArgs (&of)[3], void* const (&results)[3]) {
+  JoinArgs<X> g{};
+  int count = 0;
+  uint32_t groups = 0;
+  for (int i = 0; i < 3; ++i) {
+    if (results[i] == nullptr || of[i].product.splits == 1) continue;
+    g.rows[count] = {of[i].split_stride / of[i].ld, static_cast<int>(of[i].ld / kVec), groups};
+    g.partial[count] = static_cast<const float*>(of[i].out);
+    g.splits[count] = of[i].product.splits;
+    g.width[count] = static_cast<int>(of[i].entries_a);
+    g.split_stride[count] = of[i].split_stride;
+    g.out[count] = static_cast<X*>(results[i]);
+    groups += g.rows[count++].groups();
+  }
+  for (int k = count; k < 3; ++k) g.rows[k].first = UINT32_MAX;
+  if (count > 0) hipLaunchKernelGGL((attnres_ffn_join_kernel<X>), dim3(groups), dim3(kBlock), 0, c.stream, g);
 }
 
 template <class X>
 void ffn_forward(const Call& c, void* out, char* saved) {
   const FfnPlan& p = c.plan;
   if (p.few) return few_forward<X>(c, out, saved);
-  launch_gate<X>(c, place_x<X>(c), place_gate_up<X>(c), saved, p.a);
-  Operand down = place_down<X>(c), a{};
+  Operands<X> operands(c);
+  const Operand x = operands.x(), gate_up = operands.gate_up();
+  Operand down = operands.down(), a{};
+  operands.pack();
+  launch_gate<X>(c, x, gate_up, saved, p.a);
   down.entries = c.s.out_width;
   for (int k = 0; k < kParts<X>; ++k) a.part[k] = c.operand(p.a[k]);
   a.ld = p.hidden_pad;
@@ -970,27 +1062,29 @@ void ffn_forward(const Call& c, void* out, char* saved) {
     const auto kernel = splits > 1 ? attnres_ffn_out_kernel<X, float, SHAPE> : attnres_ffn_out_kernel<X, X, SHAPE>;
     hipLaunchKernelGGL(kernel, dim3(workgroups(g)), dim3(Shape<SHAPE>::kAllThreads), 0, c.stream, g);
   });
-  if (splits > 1) join_parts<X>(c, g, out);
+  join_parts<X>(c, {g, OutArgs{}, OutArgs{}}, {out, nullptr, nullptr});
 }
 
 template <class X>
 void ffn_backward(const Call& c, const void* grad_out, const char* saved, void* grad_x, void* grad_gate_up, void* grad_down) {
   const FfnPlan& p = c.plan;
+  Operands<X> operands(c);
   Operand x{}, gate_up{};
   const bool again = saved == nullptr && !p.few;
-  if (again || grad_gate_up != nullptr) x = place_x<X>(c);
-  if (again || grad_x != nullptr) gate_up = place_gate_up<X>(c);
+  if (again || grad_gate_up != nullptr) x = operands.x();
+  if (again || grad_x != nullptr) gate_up = operands.gate_up();
+  Operand down = operands.down();
+  const Operand grad = operands.grad(grad_out);
+  operands.pack();
   if (saved == nullptr) {
     char* formed = c.workspace + p.saved;
     if (p.few) launch_few_gate<X>(c, formed, nullptr);
     else launch_gate<X>(c, x, gate_up, formed, nullptr);
     saved = formed;
   }
-  const Operand grad = place_operand<X>(c, p.pack_grad, p.grad, grad_out, c.s.out_width, c.s.rows, p.rows_pad, p.rows_pad,
-                                        c.s.out_width, p.out_pad);
   {
     SlopeArgs g{};
-    Operand down = place_down<X>(c), rows = grad;
+    Operand rows = grad;
     down.entries = p.hidden_pad;
     down.depth = p.out_pad;
     rows.entries = c.s.rows;
@@ -1064,9 +1158,7 @@ void ffn_backward(const Call& c, const void* grad_out, const char* saved, void* 
     constexpr int SHAPE = decltype(size)::value;
     hipLaunchKernelGGL((attnres_ffn_gradients_kernel<X, SHAPE>), dim3(grid), dim3(Shape<SHAPE>::kAllThreads), 0, c.stream, g);
   });
-  for (int i = 0; i < 3; ++i) {
-    if (results[i] != nullptr && splits[i] > 1) join_parts<X>(c, of[i], results[i]);
-  }
+  join_parts<X>(c, of, results);
 }
 
 bool known_sizes(const Sizes& s) {
@@ -1129,7 +1221,7 @@ extern "C" {
 
 int64_t attnres_hip_gated_ffn_saved_bytes(int64_t rows, int64_t width, int64_t hidden, int64_t out_width, int dtype) {
   const Sizes s{rows, width, hidden, out_width, dtype};
-  return known_sizes(s) ? ffn_plan(s, kForward).saved_bytes : -1;
+  return known_sizes(s) ? saved_bytes(s) : -1;
 }
 
 int64_t attnres_hip_gated_ffn_workspace_bytes(int64_t rows, int64_t width, int64_t hidden, int64_t out_width, int dtype, int backward) {
