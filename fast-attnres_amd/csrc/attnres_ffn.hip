@@ -263,20 +263,29 @@ __global__ void __launch_bounds__(Shape<SHAPE>::kAllThreads, Shape<SHAPE>::kGrou
     const auto form = [&](auto all) {  // all: every entry counts
 #pragma unroll
       for (int i = 0; i < kDown; ++i) {
-        const Pair<X>& pair = pairs[i];
+        Pair<X>& pair = pairs[i];
         float x[3][4];
+        if constexpr (turn == 0) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const Activated act = activate<X, true>(pair.gate(e), g.activation);
-          const float da = acc[i][j][e], up = pair.up(e);
-          x[0][e] = da * up * act.slope;
-          x[1][e] = da * act.value;
-          x[2][e] = act.value * up;
-          if constexpr (!decltype(all)::value) {
-            const bool inside = j * kSub < inside_n && i * kSub + e < inside_f;
+          for (int e = 0; e < 4; ++e) {
+            const Activated act = activate<X, true>(pair.gate(e), g.activation);
+            const float da = acc[i][j][e], up = pair.up(e);
+            x[0][e] = da * up * act.slope;
+            x[1][e] = da * act.value;
+            x[2][e] = act.value * up;
+            if constexpr (!decltype(all)::value) {
+              const bool inside = j * kSub < inside_n && i * kSub + e < inside_f;
 #pragma unroll
-            for (int plane = 0; plane < 3; ++plane) x[plane][e] = inside ? x[plane][e] : 0.0f;
+              for (int plane = 0; plane < 3; ++plane) x[plane][e] = inside ? x[plane][e] : 0.0f;
+            }
+            if constexpr (kTurns == 3) {  // the two other turns' values in place of g and u
+              pair.high[e] = __float_as_uint(x[1][e]);
+              pair.rest[e] = __float_as_uint(x[2][e]);
+            }
           }
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[turn][e] = __uint_as_float(turn == 1 ? pair.high[e] : pair.rest[e]);
         }
         const int chunk = (wave % 2) * (2 * kDown) + i * 2 + lane / 32;
         uint16_t* to = lds + staged<kChunks>(row, chunk) * 8 + (lane / 16 % 2) * 4;
@@ -438,7 +447,7 @@ __global__ void __launch_bounds__(Shape<SHAPE>::kAllThreads, Shape<SHAPE>::kGrou
 }
 
 // Passes over rows of chunks of kVec, several tensors in one launch: a workgroup takes whole rows, kChunksOfGroup chunks or one row.
-constexpr int kChunksOfGroup = 4 * kBlock;
+constexpr int kChunksOfGroup = kBlock;
 
 struct Rows {
   int64_t rows;
@@ -761,7 +770,8 @@ Cut choose_cut(const Outputs* outputs, int count, int segments, bool whole) {
   for (const int tile : {256, 128, 64}) {
     // a workgroup alone on a unit that has room for more reaches two thirds of its rate
     const double alone = tile == 256 ? 1.0 : 1.5;
-    const double rate = (tile == 256 ? 1.2e15 : tile == 128 ? 0.9e15 : 0.6e15) / kUnits;
+    const double rate = (tile == 256 ? 1.25e15 : tile == 128 ? 0.87e15 : 0.6e15) / kUnits;
+    const double ends = tile == 256 ? 5e-6 : tile == 128 ? 2e-6 : 1e-6;  // of a tile: its first loads and its epilogue
     int64_t tiles[3] = {};
     bool fits = true;
     for (int i = 0; i < count; ++i) {
@@ -779,7 +789,7 @@ Cut choose_cut(const Outputs* outputs, int count, int segments, bool whole) {
       for (int i = 0; i < count; ++i) {
         workgroups += tiles[i] * cut.splits[i];
         if (tiles[i] > 0) least_depth = std::min(least_depth, outputs[i].depth / cut.splits[i]);
-        each[i] = 2.0 * tile * tile * static_cast<double>(outputs[i].depth) * segments / cut.splits[i] / rate;
+        each[i] = 2.0 * tile * tile * static_cast<double>(outputs[i].depth) * segments / cut.splits[i] / rate + ends;
         if (cut.splits[i] > 1) partial += 4e-6 + 8.0 * static_cast<double>(outputs[i].a * outputs[i].b) * cut.splits[i] / 4.5e12;
       }
       std::sort(order, order + count, [&](int i, int j) { return each[i] > each[j]; });
