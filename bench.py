@@ -912,8 +912,9 @@ def run_model(cfg: dict, steps: int, warmup: int, variant: str = "both", autocas
 
     ``variant`` "both" times the plain step (the line's value), then the
     source-bank step with gathered gradients, with accumulated gradients, with
-    inductor-compiled sublayers and with the layers of attnres.layers; "plain", "bank",
-    "bank_accumulate", "bank_compiled" or "bank_fused" times one of them alone (for traces), "compiled" the plain
+    inductor-compiled sublayers, with the layers of attnres.layers and with those, the feed-forward blocks and
+    the optimizer step of attnres; "plain", "bank", "bank_accumulate", "bank_compiled", "bank_fused" or
+    "bank_fused_step" times one of them alone (for traces), "compiled" the plain
     model under whole-model inductor compilation, "graph" the whole step
     (compiled model and loss under BF16 autocast, fused capturable AdamW)
     captured in one HIP graph and replayed (benchmarks/training_graph.py). A
@@ -933,11 +934,17 @@ def run_model(cfg: dict, steps: int, warmup: int, variant: str = "both", autocas
     tokens = torch.randint(config.vocab, (config.batch, config.sequence), device="cuda", generator=generator)
     targets = torch.roll(tokens, -1, dims=1)
 
-    def time_steps(source_bank, bank_gradients="gather", compiled=False, compile_layers=False, fused_layers=False):
+    def time_steps(source_bank, bank_gradients="gather", compiled=False, compile_layers=False, fused_layers=False,
+                   fused_step=False):
         torch.manual_seed(0)
         model = make_model(config, backend="kernel", source_bank=source_bank, bank_gradients=bank_gradients,
-                           compile_layers=compile_layers, fused_layers=fused_layers).cuda()
-        optimizer = torch.optim.AdamW(model.parameters(), lr=1e-4, fused=cfg.get("fused_adamw", False))
+                           compile_layers=compile_layers, fused_layers=fused_layers, fused_feed_forward=fused_step).cuda()
+        if fused_step:
+            from attnres.optim import AdamW
+
+            optimizer = AdamW(model.parameters(), lr=1e-4)
+        else:
+            optimizer = torch.optim.AdamW(model.parameters(), lr=1e-4, fused=cfg.get("fused_adamw", False))
         if compiled:  # inductor around the model; the reads stay opaque custom ops
             torch._dynamo.reset()
             model = torch.compile(model, fullgraph=True)
@@ -1007,6 +1014,8 @@ def run_model(cfg: dict, steps: int, warmup: int, variant: str = "both", autocas
     bc_ms, bc_loss = (time_steps(True, compile_layers=True) if variant in ("both", "bank_compiled")
                       else (None, None))
     bf_ms, bf_loss = (time_steps(True, fused_layers=True) if variant in ("both", "bank_fused") else (None, None))
+    fs_ms, fs_loss = (time_steps(True, fused_layers=True, fused_step=True) if variant in ("both", "bank_fused_step")
+                      else (None, None))
     inference_ms = time_inference(False) if variant == "both" else None
     inference_bank_ms = time_inference(True) if variant == "both" else None
 
@@ -1018,7 +1027,8 @@ def run_model(cfg: dict, steps: int, warmup: int, variant: str = "both", autocas
 
     timed_name, timed_ms = next(((name, t) for name, t in (("plain", ms), ("graph", graph_ms), ("compiled", comp_ms),
                                                             ("bank", bank_ms), ("bank_accumulate", acc_ms),
-                                                            ("bank_compiled", bc_ms), ("bank_fused", bf_ms)) if t is not None), (None, None))
+                                                            ("bank_compiled", bc_ms), ("bank_fused", bf_ms),
+                                                            ("bank_fused_step", fs_ms)) if t is not None), (None, None))
     counts = read_sources_per_step(config)
     reads = len(counts)
     read_bytes_per_step = sum(sum(read_bytes(s, n_tokens, config.width)) for s in counts)
@@ -1052,6 +1062,8 @@ def run_model(cfg: dict, steps: int, warmup: int, variant: str = "both", autocas
         # the source-bank step with embedding, layer norms and loss from attnres.layers
         "source_bank_fused_layers": {"ms_per_step": rounded(bf_ms, 3), "tokens_per_s": rate(bf_ms),
                                      "loss": rounded(bf_loss, 4)},
+        # the same with the feed-forward blocks of attnres.layers and the optimizer step of attnres.optim
+        "source_bank_fused_step": {"ms_per_step": rounded(fs_ms, 3), "tokens_per_s": rate(fs_ms), "loss": rounded(fs_loss, 4)},
         # --model-variant compiled: the plain model under torch.compile(fullgraph=True) (inductor)
         "compiled": {"ms_per_step": rounded(comp_ms, 3), "tokens_per_s": rate(comp_ms), "loss": rounded(comp_loss, 4)},
         # --model-variant graph: the whole step captured in one HIP graph (BF16 autocast)
@@ -1078,12 +1090,13 @@ def main(argv=None) -> int:
                         help="--config model / model_block: run the steps under torch.autocast (BF16), as the "
                              "reference's 24-layer timings do")
     parser.add_argument("--model-variant",
-                        choices=("both", "plain", "bank", "bank_accumulate", "bank_compiled", "bank_fused", "compiled",
-                                 "graph"),
+                        choices=("both", "plain", "bank", "bank_accumulate", "bank_compiled", "bank_fused", "bank_fused_step",
+                                 "compiled", "graph"),
                         default="both",
                         help="--config model / model_block: time the plain step, the source-bank step (gathered "
-                             "or accumulated gradients, or with compiled sublayers, or with the layers of "
-                             "attnres.layers), all five (both), or the plain "
+                             "or accumulated gradients, or with compiled sublayers, with the layers of "
+                             "attnres.layers, or with its feed-forward blocks and optimizer step too), all six "
+                             "(both), or the plain "
                              "model under inductor")
     args = parser.parse_args(argv)
 

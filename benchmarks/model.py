@@ -37,6 +37,10 @@ kernel with its gradient by sorted tokens, the layer norms, and the LM head
 with the cross entropy (``CausalAttnResLM.loss``, which ``training_step``
 calls), which forms the logits tile by tile and keeps their exponentials for
 the backward, 2 or 4 bytes each.  The weights are the same parameters.
+
+``fused_feed_forward=True`` (HIP backend; no reference counterpart) runs every MLP sublayer's
+projections as ``attnres.layers.gated_feed_forward``, with the weights in the autocast dtype
+under autocast.  ``training_step`` takes any optimizer, ``attnres.optim.AdamW`` among them.
 """
 
 from __future__ import annotations
@@ -108,11 +112,12 @@ def block_ends(events: int, blocks: int) -> tuple[int, ...]:
 class TransformerLayer(nn.Module):
     """Pre-norm causal self-attention and a SwiGLU MLP, as two sublayers."""
 
-    def __init__(self, config: TrainingConfig, fused_layers: bool = False) -> None:
+    def __init__(self, config: TrainingConfig, fused_layers: bool = False, fused_feed_forward: bool = False) -> None:
         super().__init__()
         d = config.width
         self.heads = config.heads
         self.fused_layers = fused_layers
+        self.fused_feed_forward = fused_feed_forward
         self.attn_norm = nn.LayerNorm(d)
         self.qkv = nn.Linear(d, 3 * d, bias=False)
         self.attn_out = nn.Linear(d, d, bias=False)
@@ -135,6 +140,12 @@ class TransformerLayer(nn.Module):
         return self.attn_out(y.transpose(1, 2).reshape(b, t, d))
 
     def mlp(self, x: Tensor) -> Tensor:
+        if self.fused_feed_forward:
+            from attnres.layers import gated_feed_forward
+
+            x = self._norm(self.mlp_norm, x)
+            dtype = torch.get_autocast_dtype(x.device.type) if torch.is_autocast_enabled(x.device.type) else x.dtype
+            return gated_feed_forward(x.to(dtype), self.gate_up.weight.to(dtype), self.down.weight.to(dtype))
         gate, up = self.gate_up(self._norm(self.mlp_norm, x)).chunk(2, dim=-1)
         return self.down(F.silu(gate) * up)
 
@@ -143,12 +154,15 @@ class CausalAttnResLM(nn.Module):
     """Small causal Transformer with Full or Block AttnRes residual reads."""
 
     def __init__(self, config: TrainingConfig, backend: Backend = "kernel", *, source_bank: bool = False,
-                 bank_gradients: str = "gather", compile_layers: bool = False, fused_layers: bool = False) -> None:
+                 bank_gradients: str = "gather", compile_layers: bool = False, fused_layers: bool = False,
+                 fused_feed_forward: bool = False) -> None:
         super().__init__()
         if source_bank and backend != "kernel":
             raise ValueError("source_bank needs the HIP backend")
         if fused_layers and backend != "kernel":
             raise ValueError("fused_layers needs the HIP backend")
+        if fused_feed_forward and backend != "kernel":
+            raise ValueError("fused_feed_forward needs the HIP backend")
         if bank_gradients not in ("gather", "accumulate"):
             raise ValueError("bank_gradients must be 'gather' or 'accumulate'")
         self.config = config
@@ -158,7 +172,8 @@ class CausalAttnResLM(nn.Module):
         self.fused_layers = bool(fused_layers)
         self.token_embedding = nn.Embedding(config.vocab, config.width)
         self.position_embedding = nn.Parameter(torch.empty(config.sequence, config.width))
-        self.layers = nn.ModuleList(TransformerLayer(config, self.fused_layers) for _ in range(config.layers))
+        self.fused_feed_forward = bool(fused_feed_forward)
+        self.layers = nn.ModuleList(TransformerLayer(config, self.fused_layers, self.fused_feed_forward) for _ in range(config.layers))
         self.lm_head = nn.Linear(config.width, config.vocab, bias=False)
         # one query per read: before sublayers 2 .. 2L and before the LM head
         self.queries = nn.ParameterList(nn.Parameter(torch.empty(config.rank)) for _ in range(2 * config.layers))
@@ -311,17 +326,18 @@ class CausalAttnResLM(nn.Module):
 
 def make_model(config: TrainingConfig, backend: Backend = "kernel", *, source_bank: bool = False,
                bank_gradients: str = "gather", compile_layers: bool = False,
-               fused_layers: bool = False) -> CausalAttnResLM:
+               fused_layers: bool = False, fused_feed_forward: bool = False) -> CausalAttnResLM:
     """Construct a model with the given residual-read backend (``bank_gradients``:
     the source bank's gradient path, see ``attnres.SourceBank``; ``compile_layers``:
     each attention and MLP sublayer under ``torch.compile(fullgraph=True)``;
-    ``fused_layers``: the layers around the reads from ``attnres.layers``)."""
+    ``fused_layers``: the layers around the reads from ``attnres.layers``;
+    ``fused_feed_forward``: the MLP sublayers' projections from there too)."""
     if not isinstance(config, TrainingConfig):
         raise TypeError("config must be a TrainingConfig")
     if not (backend == "kernel" or callable(backend)):
         raise ValueError("backend must be 'kernel' or a callable")
     return CausalAttnResLM(config, backend, source_bank=source_bank, bank_gradients=bank_gradients,
-                           compile_layers=compile_layers, fused_layers=fused_layers)
+                           compile_layers=compile_layers, fused_layers=fused_layers, fused_feed_forward=fused_feed_forward)
 
 
 def training_step(model: nn.Module, optimizer: torch.optim.Optimizer, tokens: Tensor, targets: Tensor,

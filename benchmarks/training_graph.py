@@ -44,7 +44,8 @@ def _step(model, loss_fn, optimizer: torch.optim.Optimizer, tokens: Tensor, targ
 class _StateSnapshot:
     """Model parameters/buffers and optimizer state, restored in place (the
     graph keeps the tensors' addresses).  Optimizer state that did not exist
-    when the snapshot was taken is reset to AdamW's initial values."""
+    when the snapshot was taken is reset to AdamW's initial values: zeros, and
+    FP32 masters to their parameters."""
 
     def __init__(self, model: torch.nn.Module, optimizer: torch.optim.Optimizer) -> None:
         self.model = {name: t.detach().clone() for name, t in model.state_dict().items()}
@@ -60,7 +61,12 @@ class _StateSnapshot:
             saved = self.optimizer.get(id(p), {})
             for key, value in state.items():
                 if torch.is_tensor(value):
-                    value.copy_(saved[key]) if key in saved else value.zero_()
+                    if key in saved:
+                        value.copy_(saved[key])
+                    elif key == "master":
+                        value.copy_(p)
+                    else:
+                        value.zero_()
 
 
 class CapturedTrainingStep:
@@ -119,7 +125,7 @@ def capture_training_step(model: torch.nn.Module, optimizer: torch.optim.Optimiz
                           targets: Tensor, *, accumulation: int = 1) -> CapturedTrainingStep:
     """Compile and capture one complete training step for a fixed batch shape.
     The optimizer must be AdamW (or another optimizer) with ``fused=True`` and
-    ``capturable=True``; two warm-up steps initialise the compiler and the
+    ``capturable=True`` (``attnres.optim.AdamW`` is fused by itself); two warm-up steps initialise the compiler and the
     optimizer state and are undone."""
     return CapturedTrainingStep(model, optimizer, tokens, targets, accumulation)
 
