@@ -106,17 +106,28 @@ class AdamW(torch.optim.Optimizer):
 
     def __init__(self, params: Iterable, lr: float | Tensor = 1e-3, betas: tuple[float, float] = (0.9, 0.999), eps: float = 1e-8,
                  weight_decay: float = 1e-2, *, state_bits: int = 32, masters: bool = False, capturable: bool = False) -> None:
-        if not isinstance(lr, Tensor):
-            _check_factor(lr, "lr")
-        betas = _check_betas(betas)
-        eps, weight_decay = _check_factor(eps, "eps"), _check_factor(weight_decay, "weight_decay")
-        if state_bits not in (8, 32):
+        defaults = dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits, masters=masters,
+                        capturable=capturable, fused=True)
+        self._check_options(defaults)
+        super().__init__(params, defaults)
+
+    @staticmethod
+    def _check_options(options: dict) -> None:
+        if not isinstance(options["lr"], Tensor):
+            _check_factor(options["lr"], "lr")
+        _check_betas(options["betas"])
+        for name in ("eps", "weight_decay"):
+            _check_factor(options[name], name)
+        if options["state_bits"] not in (8, 32):
             raise ValueError("state_bits must be 8 or 32")
-        for name, value in (("masters", masters), ("capturable", capturable)):
-            if not isinstance(value, bool):
+        for name in ("masters", "capturable"):
+            if not isinstance(options[name], bool):
                 raise TypeError(f"{name} must be a bool")
-        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits, masters=masters,
-                                      capturable=capturable, fused=True))
+
+    def add_param_group(self, param_group: dict) -> None:
+        """As in ``torch.optim.Optimizer``, with the group's options checked."""
+        self._check_options({**self.defaults, **param_group})
+        super().add_param_group(param_group)
 
     def _own_state(self, p: Tensor, group: dict, shared: dict) -> dict:
         """The parameter's state, made at its first step; `shared`: device step counts made in this call."""
@@ -202,6 +213,7 @@ class AdamW(torch.optim.Optimizer):
         for group in self.param_groups:
             for name in self.defaults:
                 group.setdefault(name, self.defaults[name])
+            group["fused"] = True
         saved_ids = [i for group in state_dict["param_groups"] for i in group["params"]]
         params = [(p, group) for group in self.param_groups for p in group["params"]]
         shared: dict[tuple, Tensor] = {}

@@ -290,6 +290,49 @@ def test_compiled_matches_eager():
         assert torch.equal(compiled(x, gate_up, down), results[0][0])
 
 
+def test_compiled_for_any_number_of_rows():
+    _x, gate_up, down, _grad = _inputs(27, 1, 96, 160, 64, BF16)
+    gate_up.requires_grad_(True), down.requires_grad_(True)
+    compiled = torch.compile(lambda x: layers.gated_feed_forward(x, gate_up, down), fullgraph=True, backend="aot_eager", dynamic=True)
+    for rows in (3, 40, 200):
+        x, _gate_up, _down, grad = _inputs(28, rows, 96, 160, 64, BF16)
+        results = []
+        for call in (compiled, lambda x: layers.gated_feed_forward(x, gate_up, down)):
+            leaf = x.detach().requires_grad_(True)
+            out = call(leaf)
+            results.append((out.detach(), *torch.autograd.grad(out, (leaf, gate_up, down), grad)))
+        assert all(torch.equal(a, b) for a, b in zip(*results))
+
+
+def test_checkpointed():
+    """The forward again in the backward gives the bits of the first one, few rows or many."""
+    from torch.utils.checkpoint import checkpoint
+
+    for rows in (5, 60, 300):
+        x, gate_up, down, grad = _inputs(29, rows, 96, 160, 64, BF16)
+        results = []
+        for call in (lambda *t: checkpoint(layers.gated_feed_forward, *t, use_reentrant=False), layers.gated_feed_forward):
+            leaves = [t.detach().requires_grad_(True) for t in (x, gate_up, down)]
+            out = call(*leaves)
+            results.append((out.detach(), *torch.autograd.grad(out, leaves, grad)))
+        assert all(torch.equal(a, b) for a, b in zip(*results))
+
+
+def test_on_two_streams_at_once():
+    inputs = [_inputs(30 + k, 700, 256, 512, 256, BF16) for k in range(2)]
+    expected = [_run(*i) for i in inputs]
+    torch.cuda.synchronize()
+    streams, results = [torch.cuda.Stream() for _ in inputs], [[], []]
+    for _ in range(3):
+        for k, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                results[k].append(_run(*inputs[k]))
+    torch.cuda.synchronize()
+    for k in range(2):
+        for result in results[k]:
+            assert all(torch.equal(a, b) for a, b in zip(result, expected[k]))
+
+
 def test_differentiating_the_gradients_again_is_refused():
     x, gate_up, down, _grad = _inputs(22, 8, 32, 32, 32, BF16)
     x.requires_grad_(True)

@@ -108,6 +108,17 @@ def test_optimizer_refusals(kw, error):
         optim.AdamW([torch.nn.Parameter(torch.zeros(3))], **kw)
 
 
+def test_options_of_a_group_are_checked():
+    first, second = (torch.nn.Parameter(torch.zeros(3)) for _ in range(2))
+    with pytest.raises(ValueError, match="state_bits"):
+        optim.AdamW([{"params": [first], "state_bits": 4}])
+    optimizer = optim.AdamW([first])
+    with pytest.raises(ValueError, match="betas"):
+        optimizer.add_param_group({"params": [second], "betas": (0.9, 1.5)})
+    optimizer.add_param_group({"params": [second], "lr": 0.5, "masters": True})
+    assert optimizer.param_groups[1]["lr"] == 0.5 and optimizer.param_groups[1]["fused"]
+
+
 def test_optimizer_needs_gpu_parameters_and_dense_gradients():
     p = torch.nn.Parameter(torch.zeros(3, 4))
     optimizer = optim.AdamW([p])
