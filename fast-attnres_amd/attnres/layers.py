@@ -1,11 +1,12 @@
-"""The layers around the residual reads, as gfx950 kernels: layer norm, embedding
-and the softmax cross entropy of a projection to a vocabulary.
+"""The layers around the residual reads, as gfx950 kernels: layer norm, embedding,
+the gated feed-forward block and the softmax cross entropy of a projection to a
+vocabulary.
 
-    from attnres.layers import embedding, layer_norm, linear_cross_entropy
+    from attnres.layers import embedding, gated_feed_forward, layer_norm, linear_cross_entropy
 
-They are the rest of a model's path from tokens to its loss: every sublayer
-normalises the output of a read, the bottom looks tokens up, and the top turns
-the last read into a loss.  No counterpart in the reference, whose model takes
+They are the rest of a model's path from tokens to its loss but for its attention:
+every sublayer normalises the output of a read, every other one is a feed-forward
+block, the bottom looks tokens up, and the top turns the last read into a loss.  No counterpart in the reference, whose model takes
 them from PyTorch (`benchmarks/model.py:180-355`).
 
 Sums, statistics and norms are FP32; results are rounded once.  First-order
@@ -395,7 +396,7 @@ def gated_feed_forward(x: Tensor, gate_up: Tensor, down: Tensor, *, activation: 
 
     Gradients flow to all three.  For them the forward keeps both projections, 6 bytes per
     row and hidden entry each pair (FP32: 8), in every live graph; with ``recompute=True``
-    nothing, and the backward forms them again, which adds two ninths to its products.
+    nothing, and the backward forms them again, which adds a third to its products.
     """
     for name, value in (("x", x), ("gate_up", gate_up), ("down", down)):
         _check_tensor(value, name, _FLOATS)

@@ -12,8 +12,8 @@
 // masters 1.77 ms (6.4 TB/s; 1.96).  torch's copy of 4 GiB reaches 4.8 TB/s on this card.
 //
 // 8-bit states: the 256 elements of a wavefront's turn are a block with a scale of its own, so a block's largest magnitude
-// is a maximum over the wavefront's registers.  Numbers are E4M3 relative to it: 3 bits of mantissa, and 2^17 from
-// the largest to the least normal number's half.  v is held by its root, which has half the exponents to span, and a root above
+// is a maximum over the wavefront's registers.  Numbers are E4M3 relative to it: 3 bits of mantissa down to
+// 2^-15 of it, and the least at 2^-18.  v is held by its root, which has half the exponents to span, and a root above
 // zero is never rounded to zero, since the update divides by it.
 
 #include "attnres_layers.h"

@@ -5,14 +5,17 @@
 //   dWd = dY^T a,  dX = [dg du] W,  dW = [dg du]^T X,              W = [Wg; Wu]
 //
 // Bound by the matrix cores: 6 N D F operations forward (N rows, D wide, F hidden), 12 backward, against O(N F + D F)
-// bytes.  Five launches of tiles of 256 x 256 (attnres_product.h): g and u in one, a gate's and an up's entry in the same
-// lane, so that a is formed from the FP32 sums; Y; da, from which dg, du and a again are formed; dWd; dX; dW.
-// Products whose tiles do not fill the chip are cut along their depth, and the parts' FP32 sums added up in order.
+// bytes.  Launches of tiles (attnres_product.h): g and u in one, a gate's and an up's entry in the same lane, so that a is
+// formed from the FP32 sums; Y; da, from which dg, du and a again are formed; and dX, dW and dWd in one, or where they are large
+// in one each (kTogether).  Tiles are of 256, 128 or 64 by a model of when the chip's last unit is done (choose_cut); products whose
+// tiles do not fill the chip are cut along their depth, and the parts' FP32 sums added up in order.
+// 16384 x 4096 x 11264, BF16: forward 3.8 ms (1.19 PFLOP/s), backward 8.0 (1.13); power sets the clock there, and the library's
+// products of these sizes reach 1.40.  2048 x 1024 x 2816 in 167 us of kernels, 0.64.
 //
 // What goes from the forward to the backward is g and u, in the order in which a lane holds them, so both sides
 // move them 16 bytes per lane with no detour over LDS: FP32 for FP32 inputs, else FP32 cut to 24 bits (2^-17).  Rounded to
-// 16 bits they would be the gradients' largest error: BF16, root mean square, 0.0032 of dX and dW, 0.0024 as it is.
-// With `saved` NULL the backward forms them again, which adds a third to its products.
+// BF16, g and u would each bring an error of the size of the gradients' own rounding (0.0017, root mean square); as it is the gradients
+// are off by 0.0024.  With `saved` NULL the backward forms them again, which adds a third to its products.
 //
 // 16-bit operands are multiplied as they are; a, dg and du are rounded to their type.  FP32 values are written as the
 // sum of three BF16 numbers, 24 bits over FP32's whole range, and a product is the six products of parts that are
@@ -135,6 +138,8 @@ __device__ __forceinline__ void take_part(float* x, const uint32_t* packed, int 
 }
 
 // ------------------------------------------------------------------ g, u and a
+// 16384 x 4096 x 11264, BF16, 2.45-2.54 ms with g and u saved (1.19-1.24 PFLOP/s); 4096 x 2048 x 8192, FP16, 0.27-0.31 without, of
+// which about 9 us for each of a unit's four tiles go to filling the ring and to the epilogue; 48 x 2048 x 5632 14 us, reading W at 3.3 TB/s.
 
 struct GateArgs {
   Product product;  // A: gate's and up's rows, paired; B: X
@@ -214,6 +219,8 @@ __global__ void __launch_bounds__(Shape<SHAPE>::kAllThreads, Shape<SHAPE>::kGrou
 }
 
 // ------------------------------------------------------------- da, dg, du and a
+// The product, and in its epilogue 12 bytes per entry and row, 6 read and 6 written (FP32: 8 and 18): 16384 x 4096 x 11264, BF16, 1.64 ms
+// (0.92 PFLOP/s), 2048 x 1024 x 2816 on tiles of 128 35 us (0.34); FP32, 16384 x 1024 x 2816, 0.80 ms.
 
 struct SlopeArgs {
   Product product;  // A: Wd by columns, B: dY by rows
@@ -407,7 +414,8 @@ __device__ __forceinline__ void store_tile(const OutArgs& g, const TileAt& tile,
   }
 }
 
-// Y (A: Wd by rows, B: a by rows).
+// Y (A: Wd by rows, B: a by rows).  16384 x 4096 x 11264, BF16, 1.25-1.33 ms (1.1-1.2 PFLOP/s); 48 x 2048 x 5632 in 8 parts 9.4 us, reading
+// Wd at 2.5 TB/s.
 template <class X, class OUT, int SHAPE>
 __global__ void __launch_bounds__(Shape<SHAPE>::kAllThreads, Shape<SHAPE>::kGroupsOf) attnres_ffn_out_kernel(OutArgs g) {
   using S = Shape<SHAPE>;
@@ -420,7 +428,8 @@ __global__ void __launch_bounds__(Shape<SHAPE>::kAllThreads, Shape<SHAPE>::kGrou
 }
 
 // dX (A: W by columns, B: [dg du] by rows), dW (A: X, B: [dg du], both by columns) and dWd (A: a, B: dY, both by columns) in one
-// launch, the tiles that take longest first, so that the three fill the chip together.
+// launch, the tiles that take longest first, so that the three fill the chip together: 2048 x 1024 x 2816, BF16, 63 us (0.94 PFLOP/s);
+// 16384 x 4096 x 11264 in three launches 6.2-6.5 ms (1.17-1.23 PFLOP/s).
 struct GradientsArgs {
   OutArgs of[3];
   uint32_t first[3];  // workgroup of each; past the last: none
@@ -466,7 +475,7 @@ __device__ __forceinline__ void for_chunks(const Rows& r, F f) {
   for (int i = threadIdx.x; i < here; i += kBlock) f(row0 + i / r.chunks, i % r.chunks);
 }
 
-// out[r] = the sum of the parts' rows, in order.
+// out[r] = the sum of the parts' rows, in order.  Bound by memory: 4096 x 2048 of two parts 13.7 us (6.1 TB/s).
 template <class X>
 struct JoinArgs {
   Rows rows[3];
@@ -498,7 +507,8 @@ __global__ void __launch_bounds__(kBlock) attnres_ffn_join_kernel(JoinArgs<X> g)
   });
 }
 
-// Rows to operands: [2 or 1 halves of half_pad][width_pad], zero-padded, of rows in halves of `half`.
+// Rows to operands: [2 or 1 halves of half_pad][width_pad], zero-padded, of rows in halves of `half`.  Bound by memory: x, W and Wd of
+// 16384 x 1024 x 2816, FP32, 40 us (6.4 TB/s), of 4095 x 1537 x 2051, FP16, 15 (4.2).
 template <class X>
 struct PackArgs {
   Rows rows;  // of the operand

@@ -1,5 +1,5 @@
 // attnres_layers.h - element types, loads and sums shared by the kernels of the
-// layers (attnres_norm.hip, attnres_embedding.hip, attnres_loss.hip).
+// layers and of the optimizer (attnres_{norm,embedding,loss,ffn,adamw}.hip).
 #ifndef ATTNRES_LAYERS_H
 #define ATTNRES_LAYERS_H
 

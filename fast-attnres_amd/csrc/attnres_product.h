@@ -1,5 +1,5 @@
-// attnres_product.h - the matrix product of the layers: tiles of 256 x 256 outputs of 16-bit operands on the matrix
-// cores, summed in FP32 (attnres_loss.hip, attnres_ffn.hip).
+// attnres_product.h - the matrix product of the layers: tiles of 256 x 256, 128 x 128 or 64 x 64 outputs of 16-bit
+// operands on the matrix cores, summed in FP32 (attnres_loss.hip, attnres_ffn.hip).
 #ifndef ATTNRES_PRODUCT_H
 #define ATTNRES_PRODUCT_H
 
