@@ -9,8 +9,8 @@
 // formed from the FP32 sums; Y; da, from which dg, du and a again are formed; and dX, dW and dWd in one, or where they are large
 // in one each (kTogether).  Tiles are of 256, 128 or 64 by a model of when the chip's last unit is done (choose_cut); products whose
 // tiles do not fill the chip are cut along their depth, and the parts' FP32 sums added up in order.
-// 16384 x 4096 x 11264, BF16: forward 3.8 ms (1.19 PFLOP/s), backward 8.0 (1.13); power sets the clock there, and the library's
-// products of these sizes reach 1.40.  2048 x 1024 x 2816 in 167 us of kernels, 0.64.
+// 16384 x 4096 x 11264, BF16: forward 3.7 ms (1.22 PFLOP/s), backward 7.9 (1.15); power sets the clock there, and the library's
+// products of these sizes reach 1.40.  2048 x 1024 x 2816 in 162 us of kernels, 0.65.
 //
 // What goes from the forward to the backward is g and u, in the order in which a lane holds them, so both sides
 // move them 16 bytes per lane with no detour over LDS: FP32 for FP32 inputs, else FP32 cut to 24 bits (2^-17).  Rounded to
@@ -56,14 +56,36 @@ struct Activated {
   float value, slope;
 };
 
-template <class X, bool SLOPE>
-__device__ __forceinline__ Activated activate(float g, int activation) {
-  if (activation == ATTNRES_SILU) {
+// gelu of 16-bit inputs: Abramowitz and Stegun's 7.1.26, the error function's complement as a polynomial of 1 / (1 + p x) times
+// e^(-x^2), which the slope needs too.  Phi is within 3e-7, g Phi within 5e-7 (by the library's function, which takes two
+// branches, too), and the tail keeps relative bits that 1 + erf loses: 2^-9 of Phi(-5) instead of 2^-4.  16384 x 4096 x 11264, by the
+// library's function in brackets: g and u 2.42 (2.54) ms, da 1.54 (1.66).
+
+template <class X, int ACTIVATION, bool SLOPE>
+__device__ __forceinline__ Activated activate(float g) {
+  if constexpr (ACTIVATION == ATTNRES_SILU) {
     const float s = reciprocal<X>(1.0f + exponential<X>(-g));
     return {g * s, SLOPE ? s * (1.0f + g * (1.0f - s)) : 0.0f};
   }
-  const float phi = 0.5f * (1.0f + erff(g * 0.707106781f));
-  return {g * phi, SLOPE ? phi + g * 0.398942280f * exponential<X>(-0.5f * g * g) : 0.0f};
+  float phi, bell = 0.0f;  // the normal distribution's integral, and e^(-g^2 / 2)
+  if constexpr (std::is_same_v<X, float>) {
+    phi = 0.5f * (1.0f + erff(g * 0.707106781f));
+    if (SLOPE) bell = expf(-0.5f * g * g);
+  } else {
+    bell = __builtin_amdgcn_exp2f(g * g * -0.721347520f);
+    const float t = __builtin_amdgcn_rcpf(1.0f + 0.231641888f * fabsf(g));
+    const float tail = t * (0.127414796f + t * (-0.142248368f + t * (0.710706871f + t * (-0.726576014f + t * 0.530702714f)))) * bell;
+    phi = g < 0.0f ? tail : 1.0f - tail;
+  }
+  return {g * phi, SLOPE ? phi + g * 0.398942280f * bell : 0.0f};
+}
+
+// f with the activation as a constant: a branch around a few entries, so that theirs are formed side by side: da of
+// 2048 x 1024 x 2816 32 us, 34 with a branch around each.
+template <class F>
+__device__ __forceinline__ void with_activation(int activation, F f) {
+  if (activation == ATTNRES_SILU) f(std::integral_constant<int, ATTNRES_SILU>{});
+  else f(std::integral_constant<int, ATTNRES_GELU>{});
 }
 
 // --------------------------------------------------------------- saved g and u
@@ -138,7 +160,7 @@ __device__ __forceinline__ void take_part(float* x, const uint32_t* packed, int 
 }
 
 // ------------------------------------------------------------------ g, u and a
-// 16384 x 4096 x 11264, BF16, 2.45-2.54 ms with g and u saved (1.19-1.24 PFLOP/s); 4096 x 2048 x 8192, FP16, 0.27-0.31 without, of
+// 16384 x 4096 x 11264, BF16, 2.40-2.43 ms with g and u saved (1.25 PFLOP/s); 4096 x 2048 x 8192, FP16, 0.26-0.29 without, of
 // which about 9 us for each of a unit's four tiles go to filling the ring and to the epilogue; 48 x 2048 x 5632 14 us, reading W at 3.3 TB/s.
 
 struct GateArgs {
@@ -174,11 +196,13 @@ __global__ void __launch_bounds__(Shape<SHAPE>::kAllThreads, Shape<SHAPE>::kGrou
       if (g.saved != nullptr && at_n + j < sub_n && at_f + i < sub_f) {
         save_pair<X>(saved + (static_cast<int64_t>(j) * sub_f + i) * kSubBytes<X>, lane, gate, up);
       }
+      with_activation(g.activation, [&](auto activation) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float x = activate<X, false>(gate[e], g.activation).value * up[e];
-        acc[i][j][e] = i * kSub + e < inside ? x : 0.0f;
-      }
+        for (int e = 0; e < 4; ++e) {
+          const float x = activate<X, decltype(activation)::value, false>(gate[e]).value * up[e];
+          acc[i][j][e] = i * kSub + e < inside ? x : 0.0f;
+        }
+      });
       __builtin_amdgcn_sched_barrier(0);  // a few outputs at a time: no registers to spill
     }
   }
@@ -219,8 +243,8 @@ __global__ void __launch_bounds__(Shape<SHAPE>::kAllThreads, Shape<SHAPE>::kGrou
 }
 
 // ------------------------------------------------------------- da, dg, du and a
-// The product, and in its epilogue 12 bytes per entry and row, 6 read and 6 written (FP32: 8 and 18): 16384 x 4096 x 11264, BF16, 1.64 ms
-// (0.92 PFLOP/s), 2048 x 1024 x 2816 on tiles of 128 35 us (0.34); FP32, 16384 x 1024 x 2816, 0.80 ms.
+// The product, and in its epilogue 12 bytes per entry and row, 6 read and 6 written (FP32: 8 and 18): 16384 x 4096 x 11264, BF16, 1.52 ms
+// (0.99 PFLOP/s), 2048 x 1024 x 2816 on tiles of 128 32 us (0.37); FP32, 16384 x 1024 x 2816, 0.76 ms.
 
 struct SlopeArgs {
   Product product;  // A: Wd by columns, B: dY by rows
@@ -273,9 +297,14 @@ __global__ void __launch_bounds__(Shape<SHAPE>::kAllThreads, Shape<SHAPE>::kGrou
         Pair<X>& pair = pairs[i];
         float x[3][4];
         if constexpr (turn == 0) {
+          Activated formed[4];
+          with_activation(g.activation, [&](auto activation) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) formed[e] = activate<X, decltype(activation)::value, true>(pair.gate(e));
+          });
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const Activated act = activate<X, true>(pair.gate(e), g.activation);
+            const Activated act = formed[e];
             const float da = acc[i][j][e], up = pair.up(e);
             x[0][e] = da * up * act.slope;
             x[1][e] = da * act.value;
@@ -659,8 +688,10 @@ __global__ void __launch_bounds__(64 * WAVES) attnres_ffn_few_gate_kernel(FewGat
     }
     if (g.out != nullptr) {
       float x[4];
+      with_activation(g.activation, [&](auto activation) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) x[e] = activate<X, false>(gate[e], g.activation).value * up[e];
+        for (int e = 0; e < 4; ++e) x[e] = activate<X, decltype(activation)::value, false>(gate[e]).value * up[e];
+      });
       store_quad(g.out + static_cast<int64_t>(row) * g.hidden_pad + f, g.hidden - f, x);
     }
   }
