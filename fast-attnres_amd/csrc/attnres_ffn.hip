@@ -749,8 +749,8 @@ struct Sizes {
 // How products are shared out: the tiles' size, and the parts that the depth of each is cut into.
 struct Cut {
   int tile, splits[3];
-  bool shared;  // the depth of tiles of 64, by more wavefronts: a unit has one workgroup at most
-  int shape() const { return tile + (shared ? 1 : 0); }
+  int shared;  // the depth of tiles of 64, by two (1) or four (2) times as many wavefronts
+  int shape() const { return tile + shared; }
 };
 struct Outputs {
   int64_t a, b, depth;  // entries; 0: not asked for
@@ -811,7 +811,7 @@ class Schedule {
 // The cut that takes the least time: the schedule of all tiles at a unit's rate for them, and the partial sums' way to memory and
 // back.  Rates as measured on a full chip.
 Cut choose_cut(const Outputs* outputs, int count, int segments, bool whole) {
-  Cut best{256, {1, 1, 1}, false};
+  Cut best{256, {1, 1, 1}, 0};
   double least = 0.0;
   for (const int tile : {256, 128, 64}) {
     // a workgroup alone on a unit that has room for more reaches two thirds of its rate
@@ -848,7 +848,7 @@ Cut choose_cut(const Outputs* outputs, int count, int segments, bool whole) {
       if (least == 0.0 || time < least) {
         least = time;
         best = cut;
-        best.shared = tile == 64 && workgroups <= kUnits && least_depth / kDepth >= 16;
+        best.shared = tile != 64 || least_depth / kDepth < 16 ? 0 : workgroups <= kUnits ? 2 : workgroups <= 2 * kUnits && least_depth / kDepth >= 32 ? 1 : 0;
       }
       if (whole || worse == 4 || cut.splits[longest] >= 32 || outputs[longest].depth / kDepth / (cut.splits[longest] + 1) < 4) break;
       ++cut.splits[longest];
@@ -961,6 +961,7 @@ void with_shape(const Cut& cut, F f) {
     case 256: return f(std::integral_constant<int, 256>{});
     case 128: return f(std::integral_constant<int, 128>{});
     case 65: return f(std::integral_constant<int, 65>{});
+    case 66: return f(std::integral_constant<int, 66>{});
     default: return f(std::integral_constant<int, 64>{});
   }
 }
