@@ -35,20 +35,28 @@ template <class X>
 constexpr int kParts = std::is_same_v<X, float> ? 3 : 1;
 template <class X>
 constexpr int kSegments = std::is_same_v<X, float> ? 6 : 1;
+// FP32 inputs of fewer rows, as they are, by FP32 matrix instructions.
+struct Single {};
 template <class X>
-using Part = std::conditional_t<std::is_same_v<X, float>, Bf16, X>;
+using Value = std::conditional_t<std::is_same_v<X, Single>, float, X>;  // of the tensors
+template <class X>
+constexpr bool kFp32 = std::is_same_v<Value<X>, float>;
+template <class X>
+using Part = std::conditional_t<std::is_same_v<X, float>, Bf16, Value<X>>;  // of the products
+template <class X>
+constexpr int kHalves = sizeof(Part<X>) / 2;
 
 // ---------------------------------------------------------------- activation
 
 // FP32 inputs: the library's exponential.  16-bit ones: the instruction's, whose argument's rounding is 2^-24 |x| relative.
 template <class X>
 __device__ __forceinline__ float exponential(float x) {
-  if constexpr (std::is_same_v<X, float>) return expf(x);
+  if constexpr (kFp32<X>) return expf(x);
   return __builtin_amdgcn_exp2f(x * 1.44269504f);
 }
 template <class X>
 __device__ __forceinline__ float reciprocal(float x) {
-  if constexpr (std::is_same_v<X, float>) return 1.0f / x;
+  if constexpr (kFp32<X>) return 1.0f / x;
   return __builtin_amdgcn_rcpf(x);
 }
 
@@ -68,7 +76,7 @@ __device__ __forceinline__ Activated activate(float g) {
     return {g * s, SLOPE ? s * (1.0f + g * (1.0f - s)) : 0.0f};
   }
   float phi, bell = 0.0f;  // the normal distribution's integral, and e^(-g^2 / 2)
-  if constexpr (std::is_same_v<X, float>) {
+  if constexpr (kFp32<X>) {
     phi = 0.5f * (1.0f + erff(g * 0.707106781f));
     if (SLOPE) bell = expf(-0.5f * g * g);
   } else {
@@ -92,11 +100,11 @@ __device__ __forceinline__ void with_activation(int activation, F f) {
 
 // A subtile of 16 rows by 16 hidden entries: lane l holds row l % 16 and entries 4 (l / 16) + 0..3.
 template <class X>
-constexpr int kSubBytes = std::is_same_v<X, float> ? 2048 : 1536;
+constexpr int kSubBytes = kFp32<X> ? 2048 : 1536;
 
 template <class X>
 __device__ __forceinline__ void save_pair(char* to, int lane, f32x4 g, f32x4 u) {
-  if constexpr (std::is_same_v<X, float>) {
+  if constexpr (kFp32<X>) {
     *reinterpret_cast<f32x4*>(to + lane * 16) = g;
     *reinterpret_cast<f32x4*>(to + 1024 + lane * 16) = u;
   } else {
@@ -130,7 +138,7 @@ struct Pair {
   u32x4 rest;  // 16-bit inputs: two words
   __device__ __forceinline__ void load(const char* from, int lane) {
     high = *reinterpret_cast<const u32x4*>(from + lane * 16);
-    if constexpr (std::is_same_v<X, float>) {
+    if constexpr (kFp32<X>) {
       rest = *reinterpret_cast<const u32x4*>(from + 1024 + lane * 16);
     } else {
       const uint64_t low = *reinterpret_cast<const uint64_t*>(from + 1024 + lane * 8);
@@ -143,11 +151,11 @@ struct Pair {
     return __uint_as_float(__builtin_amdgcn_perm(high[e / 2], rest[e / 4], select));
   }
   __device__ __forceinline__ float gate(int e) const {
-    if constexpr (std::is_same_v<X, float>) return __uint_as_float(high[e]);
+    if constexpr (kFp32<X>) return __uint_as_float(high[e]);
     return word(e);
   }
   __device__ __forceinline__ float up(int e) const {
-    if constexpr (std::is_same_v<X, float>) return __uint_as_float(rest[e]);
+    if constexpr (kFp32<X>) return __uint_as_float(rest[e]);
     return word(4 + e);
   }
 };
@@ -155,8 +163,10 @@ struct Pair {
 // What is left of x's for the next part, once `packed` has their leading one.
 template <class T>
 __device__ __forceinline__ void take_part(float* x, const uint32_t* packed, int count) {
+  if constexpr (!std::is_same_v<T, float>) {
 #pragma unroll
-  for (int e = 0; e < count; ++e) x[e] -= to_f32(T{static_cast<uint16_t>(packed[e / 2] >> (16 * (e % 2)))});
+    for (int e = 0; e < count; ++e) x[e] -= to_f32(T{static_cast<uint16_t>(packed[e / 2] >> (16 * (e % 2)))});
+  }
 }
 
 // ------------------------------------------------------------------ g, u and a
@@ -207,7 +217,7 @@ __global__ void __launch_bounds__(Shape<SHAPE>::kAllThreads, Shape<SHAPE>::kGrou
     }
   }
   if (g.out[0] == nullptr) return;
-  constexpr int kChunks = TILE / 16;  // of a row in LDS
+  constexpr int kChunks = TILE / 16 * kHalves<X>;  // of 16 bytes, of a row in LDS
 #pragma unroll
   for (int part = 0; part < kParts<X>; ++part) {
 #pragma unroll
@@ -215,6 +225,11 @@ __global__ void __launch_bounds__(Shape<SHAPE>::kAllThreads, Shape<SHAPE>::kGrou
       const int row = (wave / 2) * (16 * kAcross) + j * 16 + lane % 16;
 #pragma unroll
       for (int i = 0; i < kDown / 2; ++i) {
+        if constexpr (kHalves<X> == 2) {
+          const int chunk = (wave % 2) * (2 * kDown) + i * 4 + lane / 16;
+          *reinterpret_cast<f32x4*>(lds + staged<kChunks>(row, chunk) * 8) = acc[i][j];
+          continue;
+        }
         float x[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) x[e] = acc[i][j][e];
@@ -232,9 +247,9 @@ __global__ void __launch_bounds__(Shape<SHAPE>::kAllThreads, Shape<SHAPE>::kGrou
     __syncthreads();
     for (int k = threadIdx.x; k < TILE * kChunks; k += S::kThreadsOf) {
       const int row = k / kChunks, chunk = k % kChunks;
-      const int f = f0 + chunk * 8;
+      const int f = f0 + chunk * (8 / kHalves<X>);
       if (n0 + row < g.rows && f < g.hidden_pad) {
-        *reinterpret_cast<u32x4*>(g.out[part] + (n0 + row) * g.hidden_pad + f) =
+        *reinterpret_cast<u32x4*>(g.out[part] + ((n0 + row) * g.hidden_pad + f) * kHalves<X>) =
             *reinterpret_cast<const u32x4*>(lds + staged<kChunks>(row, chunk) * 8);
       }
     }
@@ -283,8 +298,8 @@ __global__ void __launch_bounds__(Shape<SHAPE>::kAllThreads, Shape<SHAPE>::kGrou
   };
   load_pairs(0);
   // A round: 16 rows of every wavefront, of three planes in LDS: dg, du and a; of FP32 one of them in its three parts.
-  constexpr int kRows = 16 * (S::kWavesOf / 2), kChunks = TILE / 8;
-  constexpr int kPlane = kRows * TILE;
+  constexpr int kRows = 16 * (S::kWavesOf / 2), kChunks = TILE / 8 * kHalves<X>;
+  constexpr int kPlane = kRows * TILE * kHalves<X>;
   static_assert(3 * kPlane <= S::kLds, "three planes");
   constexpr int kTurns = kParts<X>;
   const auto round = [&](auto number, auto turn_number) {
@@ -323,10 +338,14 @@ __global__ void __launch_bounds__(Shape<SHAPE>::kAllThreads, Shape<SHAPE>::kGrou
 #pragma unroll
           for (int e = 0; e < 4; ++e) x[turn][e] = __uint_as_float(turn == 1 ? pair.high[e] : pair.rest[e]);
         }
-        const int chunk = (wave % 2) * (2 * kDown) + i * 2 + lane / 32;
-        uint16_t* to = lds + staged<kChunks>(row, chunk) * 8 + (lane / 16 % 2) * 4;
+        const int chunk = kHalves<X> == 2 ? (wave % 2) * (4 * kDown) + i * 4 + lane / 16 : (wave % 2) * (2 * kDown) + i * 2 + lane / 32;
+        uint16_t* to = lds + staged<kChunks>(row, chunk) * 8 + (kHalves<X> == 2 ? 0 : lane / 16 % 2 * 4);
 #pragma unroll
         for (int plane = 0; plane < 3; ++plane) {
+          if constexpr (kHalves<X> == 2) {
+            *reinterpret_cast<f32x4*>(to + plane * kPlane) = f32x4{x[plane][0], x[plane][1], x[plane][2], x[plane][3]};
+            continue;
+          }
           float* value = x[kTurns == 1 ? plane : turn];
           const uint32_t packed[2] = {pack2<T>(value[0], value[1]), pack2<T>(value[2], value[3])};
           *reinterpret_cast<uint64_t*>(to + plane * kPlane) = static_cast<uint64_t>(packed[1]) << 32 | packed[0];
@@ -349,9 +368,9 @@ __global__ void __launch_bounds__(Shape<SHAPE>::kAllThreads, Shape<SHAPE>::kGrou
       for (int k = threadIdx.x; k < kRows * kChunks; k += S::kThreadsOf) {
         const int r = k / kChunks, chunk = k % kChunks;
         const int64_t n = n0 + r / 16 * (16 * kAcross) + j * 16 + r % 16;
-        const int f = f0 + chunk * 8;
+        const int f = f0 + chunk * (8 / kHalves<X>);
         if (n < g.rows_pad && f < g.hidden_pad) {
-          *reinterpret_cast<u32x4*>(out + n * ld + first + f) =
+          *reinterpret_cast<u32x4*>(out + (n * ld + first + f) * kHalves<X>) =
               *reinterpret_cast<const u32x4*>(lds + plane * kPlane + staged<kChunks>(r, chunk) * 8);
         }
       }
@@ -480,8 +499,8 @@ __global__ void __launch_bounds__(Shape<SHAPE>::kAllThreads, Shape<SHAPE>::kGrou
   } else {
     if (!multiply_tile<SHAPE, Part<X>, kSegments<X>, false, false>(g.product, tile, stages, lds, acc)) return;
   }
-  if (std::is_same_v<X, float> || args.wide[which]) store_tile<float, SHAPE>(g, tile, acc, lds);
-  else store_tile<X, SHAPE>(g, tile, acc, lds);
+  if (kFp32<X> || args.wide[which]) store_tile<float, SHAPE>(g, tile, acc, lds);
+  else store_tile<Value<X>, SHAPE>(g, tile, acc, lds);
 }
 
 // Passes over rows of chunks of kVec, several tensors in one launch: a workgroup takes whole rows, kChunksOfGroup chunks or one row.
@@ -541,7 +560,7 @@ __global__ void __launch_bounds__(kBlock) attnres_ffn_join_kernel(JoinArgs<X> g)
 template <class X>
 struct PackArgs {
   Rows rows;  // of the operand
-  const X* x;
+  const Value<X>* x;
   int64_t stride, half, half_pad;
   int width;
   uint16_t* to[3];
@@ -567,6 +586,12 @@ __global__ void __launch_bounds__(kBlock) attnres_ffn_pack_kernel(PacksArgs<X> a
     const int64_t at = (r * g.rows.chunks + chunk) * kVec;
 #pragma unroll
     for (int part = 0; part < kParts<X>; ++part) {
+      if constexpr (kHalves<X> == 2) {
+        auto* to = reinterpret_cast<f32x4*>(g.to[0] + at * 2);
+        to[0] = f32x4{v[0], v[1], v[2], v[3]};
+        to[1] = f32x4{v[4], v[5], v[6], v[7]};
+        continue;
+      }
       uint32_t packed[kVec / 2];
 #pragma unroll
       for (int e = 0; e < kVec / 2; ++e) packed[e] = pack2<T>(v[2 * e], v[2 * e + 1]);
@@ -731,13 +756,16 @@ __global__ void __launch_bounds__(64 * WAVES) attnres_ffn_few_out_kernel(FewOutA
 constexpr int64_t kMaxRows = int64_t{1} << 24;
 constexpr int64_t kMaxHidden = int64_t{1} << 16;
 constexpr int64_t kMaxStride = int64_t{1} << 22;  // of operands multiplied in place: 256 rows stay within 32-bit offsets
-constexpr int64_t kMaxSecond = int64_t{1} << 30;  // from the gate's rows to the up's
+constexpr int64_t kMaxSecond = int64_t{1} << 30;  // from the gate's rows to the up's, of 16 bits
 constexpr int64_t kMaxTiles = int64_t{1} << 22;   // a launch takes fewer than 2^32 threads
 // Rounds of the chip up to which the gradients' products go in one launch: one product's last round is filled by the next
 // one's first, which counts less the more rounds there are, and each then finds less of its operands in the caches.
 // Three launches against one, rows x width x hidden, BF16: 4096 x 1024 x 2816 0.309 ms to 0.144, 4096 x 2048 x 5632
 // 0.603 to 0.496, 8192 x 2048 x 5632 0.990 to 0.943; 4096 x 4096 x 8192 1.21 to 1.20; 16384 x 4096 x 11264 6.17 to 6.23.
 constexpr uint32_t kTogether = 8;
+// Rows up to which FP32 inputs are multiplied as they are, on tiles of 64.
+constexpr int64_t kSingleRows = 512;
+constexpr double kSingleCost = 3.0;  // of their products, in 16-bit products of twice the depth
 
 enum Pass { kForward = 0, kBackward = 1, kBackwardAgain = 2 };  // the last: without saved g and u
 
@@ -758,7 +786,8 @@ struct Outputs {
 
 struct FfnPlan {
   int parts, segments;
-  bool few;
+  bool few, single;  // FP32 by matrix instructions of its own
+  int halves;         // of a product's element
   int64_t rows_pad, width_pad, hidden_pad, out_pad;
   bool pack_x, pack_gate_up, pack_down, pack_grad;
   int64_t x[3], gate_up[3], down[3], grad[3], a[3], both[3];  // offsets
@@ -810,10 +839,12 @@ class Schedule {
 
 // The cut that takes the least time: the schedule of all tiles at a unit's rate for them, and the partial sums' way to memory and
 // back.  Rates as measured on a full chip.
-Cut choose_cut(const Outputs* outputs, int count, int segments, bool whole) {
+Cut choose_cut(const Outputs* outputs, int count, const FfnPlan& plan, bool whole) {
+  const double segments = plan.single ? kSingleCost : plan.segments;
   Cut best{256, {1, 1, 1}, 0};
   double least = 0.0;
   for (const int tile : {256, 128, 64}) {
+    if (plan.single && tile > 64) continue;
     // a workgroup alone on a unit that has room for more reaches two thirds of its rate
     const double alone = tile == 256 ? 1.0 : 1.5;
     const double rate = (tile == 256 ? 1.25e15 : tile == 128 ? 0.87e15 : 0.6e15) / kUnits;
@@ -863,9 +894,12 @@ int64_t saved_bytes(const Sizes& s) {
 
 FfnPlan make_plan(const Sizes& s, int pass) {
   FfnPlan p{};
-  const bool split = s.dtype == ATTNRES_F32, backward = pass != kForward;
+  p.single = s.dtype == ATTNRES_F32 && s.rows <= kSingleRows;
+  const bool split = s.dtype == ATTNRES_F32 && !p.single, backward = pass != kForward;
   p.parts = split ? 3 : 1;
   p.segments = split ? 6 : 1;
+  p.halves = p.single ? 2 : 1;
+  const int64_t size = 2 * p.halves;
   p.rows_pad = round_up(s.rows, kDepth);
   p.width_pad = round_up(s.width, kDepth);
   p.hidden_pad = round_up(s.hidden, kDepth);
@@ -885,20 +919,20 @@ FfnPlan make_plan(const Sizes& s, int pass) {
     return from;
   };
   for (int k = 0; k < p.parts; ++k) {
-    if (p.pack_x) p.x[k] = take(2 * p.rows_pad * p.width_pad);
-    if (p.pack_gate_up) p.gate_up[k] = take(4 * p.hidden_pad * p.width_pad);
-    if (p.pack_down) p.down[k] = take(2 * p.out_pad * p.hidden_pad);
-    if (p.pack_grad) p.grad[k] = take(2 * p.rows_pad * p.out_pad);
-    if (tiles) p.a[k] = take(2 * p.rows_pad * p.hidden_pad);
-    if (backward) p.both[k] = take(4 * p.rows_pad * p.hidden_pad);
+    if (p.pack_x) p.x[k] = take(size * p.rows_pad * p.width_pad);
+    if (p.pack_gate_up) p.gate_up[k] = take(2 * size * p.hidden_pad * p.width_pad);
+    if (p.pack_down) p.down[k] = take(size * p.out_pad * p.hidden_pad);
+    if (p.pack_grad) p.grad[k] = take(size * p.rows_pad * p.out_pad);
+    if (tiles) p.a[k] = take(size * p.rows_pad * p.hidden_pad);
+    if (backward) p.both[k] = take(2 * size * p.rows_pad * p.hidden_pad);
   }
   if (!tiles) p.a[0] = take(s.rows * p.hidden_pad * dtype_size(s.dtype));
   if (pass == kBackwardAgain) p.saved = take(p.saved_bytes);
   int64_t partial = 0;
   // what the sums of g, u and da go into needs them whole
   const auto one = [&](int64_t a, int64_t b, int64_t depth, bool whole) {
-    const Outputs o{a, b, depth};
-    return choose_cut(&o, 1, p.segments, whole);
+    const Outputs o{a, b, depth * p.halves};
+    return choose_cut(&o, 1, p, whole);
   };
   if (tiles) p.gate = one(2 * p.hidden_pad, s.rows, p.width_pad, true);
   if (!backward && tiles) {
@@ -907,8 +941,10 @@ FfnPlan make_plan(const Sizes& s, int pass) {
   }
   if (backward) {
     p.slope = one(p.hidden_pad, p.rows_pad, p.out_pad, true);
-    const Outputs o[3] = {{s.width, s.rows, 2 * p.hidden_pad}, {s.width, 2 * p.hidden_pad, p.rows_pad}, {s.hidden, s.out_width, p.rows_pad}};
-    p.gradients = choose_cut(o, 3, p.segments, false);
+    const Outputs o[3] = {{s.width, s.rows, 2 * p.hidden_pad * p.halves},
+                          {s.width, 2 * p.hidden_pad, p.rows_pad * p.halves},
+                          {s.hidden, s.out_width, p.rows_pad * p.halves}};
+    p.gradients = choose_cut(o, 3, p, false);
     for (int i = 0; i < 3; ++i) {
       p.partials[i] = partial;
       if (p.gradients.splits[i] > 1) partial += round_up(4 * p.gradients.splits[i] * o[i].b * round_up(o[i].a, kVec), 256);
@@ -955,11 +991,13 @@ struct Call {
   uint16_t* operand(int64_t offset) const { return reinterpret_cast<uint16_t*>(workspace + offset); }
 };
 
-template <class F>
+template <class X, class F>
 void with_shape(const Cut& cut, F f) {
+  if constexpr (!std::is_same_v<X, Single>) {
+    if (cut.tile == 256) return f(std::integral_constant<int, 256>{});
+    if (cut.tile == 128) return f(std::integral_constant<int, 128>{});
+  }
   switch (cut.shape()) {
-    case 256: return f(std::integral_constant<int, 256>{});
-    case 128: return f(std::integral_constant<int, 128>{});
     case 65: return f(std::integral_constant<int, 65>{});
     case 66: return f(std::integral_constant<int, 66>{});
     default: return f(std::integral_constant<int, 64>{});
@@ -994,7 +1032,7 @@ class Operands {
                 int64_t width_pad) {
     if (!pack) return {{static_cast<const uint16_t*>(x), nullptr, nullptr}, stride, 0, 0, 0};
     PackArgs<X>& g = args_.of[count_++];
-    g = {{halves * half_pad, static_cast<int>(width_pad / kVec), groups_}, static_cast<const X*>(x), stride, half, half_pad,
+    g = {{halves * half_pad, static_cast<int>(width_pad / kVec), groups_}, static_cast<const Value<X>*>(x), stride, half, half_pad,
          static_cast<int>(width), {}};
     groups_ += g.rows.groups();
     Operand o{{nullptr, nullptr, nullptr}, width_pad, 0, 0, 0};
@@ -1017,7 +1055,7 @@ void launch_gate(const Call& c, const Operand& x, const Operand& gate_up, char* 
   w.second = w.entries * w.ld;
   rows.entries = c.s.rows;
   const int tile = p.gate.tile;
-  g.product = {w, rows, nullptr, p.width_pad, 0, static_cast<int>(tiles_of(p.hidden_pad, tile / 2)),
+  g.product = {w, rows, nullptr, p.width_pad * p.halves, 0, static_cast<int>(tiles_of(p.hidden_pad, tile / 2)),
                static_cast<int>(tiles_of(c.s.rows, tile)), 1};
   g.rows = c.s.rows;
   g.hidden = c.s.hidden;
@@ -1025,7 +1063,7 @@ void launch_gate(const Call& c, const Operand& x, const Operand& gate_up, char* 
   g.activation = c.activation;
   g.saved = saved;
   for (int k = 0; a != nullptr && k < kParts<X>; ++k) g.out[k] = c.operand(a[k]);
-  with_shape(p.gate, [&](auto size) {
+  with_shape<X>(p.gate, [&](auto size) {
     constexpr int SHAPE = decltype(size)::value;
     hipLaunchKernelGGL((attnres_ffn_gate_kernel<X, SHAPE>), dim3(g.product.tiles_a * g.product.tiles_b), dim3(Shape<SHAPE>::kAllThreads), 0,
                        c.stream, g);
@@ -1062,7 +1100,7 @@ void few_forward(const Call& c, void* out, char* saved) {
 OutArgs out_args(const Call& c, const Operand& a, const Operand& b, int64_t depth, int64_t entries_a, int64_t half, int64_t half_pad,
                  int64_t entries_b, int tile, int splits, int64_t partial, void* out) {
   OutArgs g{};
-  g.product = {a, b, nullptr, depth, 0, static_cast<int>(tiles_of(entries_a, tile)), static_cast<int>(tiles_of(entries_b, tile)), splits};
+  g.product = {a, b, nullptr, depth * c.plan.halves, 0, static_cast<int>(tiles_of(entries_a, tile)), static_cast<int>(tiles_of(entries_b, tile)), splits};
   g.entries_a = entries_a;
   g.half = half;
   g.half_pad = half_pad;
@@ -1102,7 +1140,7 @@ void join_parts(const Call& c, const OutArgs (&of)[3], void* const (&results)[3]
 template <class X>
 void ffn_forward(const Call& c, void* out, char* saved) {
   const FfnPlan& p = c.plan;
-  if (p.few) return few_forward<X>(c, out, saved);
+  if (p.few) return few_forward<Value<X>>(c, out, saved);
   Operands<X> operands(c);
   const Operand x = operands.x(), gate_up = operands.gate_up();
   Operand down = operands.down(), a{};
@@ -1114,12 +1152,12 @@ void ffn_forward(const Call& c, void* out, char* saved) {
   a.entries = c.s.rows;
   const int splits = p.out.splits[0];
   const OutArgs g = out_args(c, down, a, p.hidden_pad, c.s.out_width, c.s.rows, c.s.rows, c.s.rows, p.out.tile, splits, 0, out);
-  with_shape(p.out, [&](auto size) {
+  with_shape<X>(p.out, [&](auto size) {
     constexpr int SHAPE = decltype(size)::value;
-    const auto kernel = splits > 1 ? attnres_ffn_out_kernel<X, float, SHAPE> : attnres_ffn_out_kernel<X, X, SHAPE>;
+    const auto kernel = splits > 1 ? attnres_ffn_out_kernel<X, float, SHAPE> : attnres_ffn_out_kernel<X, Value<X>, SHAPE>;
     hipLaunchKernelGGL(kernel, dim3(workgroups(g)), dim3(Shape<SHAPE>::kAllThreads), 0, c.stream, g);
   });
-  join_parts<X>(c, {g, OutArgs{}, OutArgs{}}, {out, nullptr, nullptr});
+  join_parts<Value<X>>(c, {g, OutArgs{}, OutArgs{}}, {out, nullptr, nullptr});
 }
 
 template <class X>
@@ -1135,7 +1173,7 @@ void ffn_backward(const Call& c, const void* grad_out, const char* saved, void* 
   operands.pack();
   if (saved == nullptr) {
     char* formed = c.workspace + p.saved;
-    if (p.few) launch_few_gate<X>(c, formed, nullptr);
+    if (p.few) launch_few_gate<Value<X>>(c, formed, nullptr);
     else launch_gate<X>(c, x, gate_up, formed, nullptr);
     saved = formed;
   }
@@ -1146,7 +1184,7 @@ void ffn_backward(const Call& c, const void* grad_out, const char* saved, void* 
     down.depth = p.out_pad;
     rows.entries = c.s.rows;
     const int tile = p.slope.tile;
-    g.product = {down, rows, nullptr, p.out_pad, 0, static_cast<int>(tiles_of(p.hidden_pad, tile)),
+    g.product = {down, rows, nullptr, p.out_pad * p.halves, 0, static_cast<int>(tiles_of(p.hidden_pad, tile)),
                  static_cast<int>(tiles_of(p.rows_pad, tile)), 1};
     g.rows = c.s.rows;
     g.rows_pad = p.rows_pad;
@@ -1158,7 +1196,7 @@ void ffn_backward(const Call& c, const void* grad_out, const char* saved, void* 
       if (grad_x != nullptr || grad_gate_up != nullptr) g.both[k] = c.operand(p.both[k]);
       if (grad_down != nullptr) g.out[k] = c.operand(p.a[k]);
     }
-    with_shape(p.slope, [&](auto size) {
+    with_shape<X>(p.slope, [&](auto size) {
       constexpr int SHAPE = decltype(size)::value;
       hipLaunchKernelGGL((attnres_ffn_slope_kernel<X, SHAPE>), dim3(g.product.tiles_a * g.product.tiles_b), dim3(Shape<SHAPE>::kAllThreads), 0,
                          c.stream, g);
@@ -1209,7 +1247,7 @@ void ffn_backward(const Call& c, const void* grad_out, const char* saved, void* 
   const auto launch = [&] {
     if (count == 0) return;
     for (int k = count; k < 3; ++k) g.first[k] = UINT32_MAX;
-    with_shape(p.gradients, [&](auto size) {
+    with_shape<X>(p.gradients, [&](auto size) {
       constexpr int SHAPE = decltype(size)::value;
       hipLaunchKernelGGL((attnres_ffn_gradients_kernel<X, SHAPE>), dim3(grid), dim3(Shape<SHAPE>::kAllThreads), 0, c.stream, g);
     });
@@ -1226,7 +1264,7 @@ void ffn_backward(const Call& c, const void* grad_out, const char* saved, void* 
     if (!together) launch();
   }
   launch();
-  join_parts<X>(c, of, results);
+  join_parts<Value<X>>(c, of, results);
 }
 
 bool known_sizes(const Sizes& s) {
@@ -1261,14 +1299,13 @@ int check_rows(const char* name, const void* x, int64_t stride, bool in_place, i
 
 int check_call(const Call& c, const void* saved, int64_t workspace_bytes) {
   const FfnPlan& p = c.plan;
-  const bool half = c.s.dtype != ATTNRES_F32, even = c.s.hidden == p.hidden_pad;
-  const bool wide = half && c.s.width == p.width_pad;
+  const bool even = c.s.hidden == p.hidden_pad, wide = c.s.width == p.width_pad;
   if (const int status = check_rows("x", c.x, c.x_stride, wide, 0, kMaxStride)) return status;
   if (const int status = check_rows("gate_up", c.gate_up, c.gate_up_stride, wide && even, c.s.width,
-                                    std::min(kMaxStride, kMaxSecond / c.s.hidden))) {
+                                    std::min(kMaxStride, kMaxSecond * 2 / dtype_size(c.s.dtype) / c.s.hidden))) {
     return status;
   }
-  if (const int status = check_rows("down", c.down, c.down_stride, half && even, c.s.hidden, kMaxStride)) return status;
+  if (const int status = check_rows("down", c.down, c.down_stride, even, c.s.hidden, kMaxStride)) return status;
   if (c.workspace == nullptr || workspace_bytes < p.bytes) {
     return layer_error(ATTNRES_ERR_WORKSPACE, "workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)p.bytes);
   }
@@ -1309,6 +1346,7 @@ int attnres_hip_gated_ffn_forward(const void* x, int64_t x_stride, const void* g
   if (out == nullptr) return layer_error(ATTNRES_ERR_NULL_POINTER, "out is NULL");
   if (dtype == ATTNRES_BF16) ffn_forward<Bf16>(c, out, static_cast<char*>(saved));
   else if (dtype == ATTNRES_F16) ffn_forward<F16>(c, out, static_cast<char*>(saved));
+  else if (c.plan.single) ffn_forward<Single>(c, out, static_cast<char*>(saved));
   else ffn_forward<float>(c, out, static_cast<char*>(saved));
   return layer_launch_status("gated feed-forward forward");
 }
@@ -1329,6 +1367,7 @@ int attnres_hip_gated_ffn_backward(const void* grad_out, const void* x, int64_t 
   const char* kept = static_cast<const char*>(saved);
   if (dtype == ATTNRES_BF16) ffn_backward<Bf16>(c, grad_out, kept, grad_x, grad_gate_up, grad_down);
   else if (dtype == ATTNRES_F16) ffn_backward<F16>(c, grad_out, kept, grad_x, grad_gate_up, grad_down);
+  else if (c.plan.single) ffn_backward<Single>(c, grad_out, kept, grad_x, grad_gate_up, grad_down);
   else ffn_backward<float>(c, grad_out, kept, grad_x, grad_gate_up, grad_down);
   return layer_launch_status("gated feed-forward backward");
 }

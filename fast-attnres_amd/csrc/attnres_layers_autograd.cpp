@@ -348,7 +348,7 @@ Tensor linear_cross_entropy(const Tensor& hidden, const Tensor& weight, const Te
 
 // ----------------------------------------------------- gated feed-forward
 
-// Rows as the products take them: 16-bit rows of whole 32-element steps are multiplied where they lie and have to
+// Rows as the products take them: rows of whole 32-element steps are multiplied where they lie and have to
 // start at multiples of 16 bytes, `least` to `most` elements apart; a copy does.
 Rows product_rows(const Tensor& tensor, bool in_place, int64_t least, int64_t most) {
   Rows rows = rows_view(tensor);
@@ -369,11 +369,12 @@ struct FeedForward {
   FeedForward(const Tensor& input, const Tensor& weights, const Tensor& last)
       : rows(input.numel() / input.size(-1)), width(weights.size(1)), hidden(last.size(1)), out_width(last.size(0)),
         dtype(dtype_of(input.scalar_type())) {
-    const bool half = dtype != ATTNRES_F32, even = hidden % 32 == 0;
+    const bool even = hidden % 32 == 0;
     constexpr int64_t kMost = int64_t{1} << 22;
-    x = product_rows(input, half && width % 32 == 0, 0, kMost);
-    gate_up = product_rows(weights, half && width % 32 == 0 && even, width, std::min(kMost, (int64_t{1} << 30) / hidden));
-    down = product_rows(last, half && even, hidden, kMost);
+    const int64_t second = int64_t{1} << (dtype == ATTNRES_F32 ? 29 : 30);
+    x = product_rows(input, width % 32 == 0, 0, kMost);
+    gate_up = product_rows(weights, width % 32 == 0 && even, width, std::min(kMost, second / hidden));
+    down = product_rows(last, even, hidden, kMost);
   }
   Tensor workspace(const Tensor& like, int backward) const {
     const int64_t bytes = attnres_hip_gated_ffn_workspace_bytes(rows, width, hidden, out_width, dtype, backward);

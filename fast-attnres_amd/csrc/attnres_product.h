@@ -139,9 +139,15 @@ struct Reader {
   }
 };
 
+// FP32: 16 bytes are 4 k's, and the order of the k's is of no account, as both operands share it.
 template <class T>
 __device__ __forceinline__ f32x4 mfma(s16x8 a, s16x8 b, f32x4 c) {
-  if constexpr (std::is_same_v<T, Bf16>) {
+  if constexpr (std::is_same_v<T, float>) {
+    const f32x4 x = __builtin_bit_cast(f32x4, a), y = __builtin_bit_cast(f32x4, b);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_16x16x4f32(x[e], y[e], c, 0, 0, 0);
+    return c;
+  } else if constexpr (std::is_same_v<T, Bf16>) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
   } else {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
@@ -391,16 +397,18 @@ static_assert(Shape<256>::kDownOf == kDown && Shape<256>::kPairedOf == kPaired, 
 
 // 16-byte slots within an LDS row.  Rows of k (128 bytes) and columns of 64 alternate between the banks' halves by themselves.
 __device__ __forceinline__ int small_row_swizzle(int row) { return row >> 1 & 7; }
-template <int TILE>
+template <int TILE, int HALVES>
 __device__ __forceinline__ int small_column_swizzle(int k) {
+  if constexpr (HALVES == 2) return (k >> 2 & 3) << 2;  // four k's to a lane: each group of lanes has its 64 of 256 bytes
   return TILE == 64 ? (k >> 1 & 1) << 1 | (k >> 3 & 1) << 2 : column_swizzle(k);
 }
 
-template <int TILE, int DEPTH, bool ROWS, bool PAIRED>
+// HALVES: of an element, 2 for FP32.  Depths here and in a Product, but not an operand's own, count halves.
+template <int TILE, int DEPTH, bool ROWS, bool PAIRED, int HALVES>
 struct SmallLoader {
   using S = Shape<TILE>;  // its tile and wavefronts are all that is used
   static constexpr int kLoadsOf = TILE * DEPTH / 512 / S::kWavesOf;  // of 1 KB per wavefront and stage
-  static constexpr int kRowsOfLoad = ROWS ? 8 : 512 / TILE, kLanesOfRow = 64 / kRowsOfLoad;
+  static constexpr int kRowsOfLoad = ROWS ? 8 : 512 / TILE / HALVES, kLanesOfRow = 64 / kRowsOfLoad;
   uint32_t offset[kLoadsOf];  // bytes from the stage's origin; columns: of the chunk alone
   int row;                    // of the first load
   __device__ __forceinline__ void init(const Operand& o, int64_t entry0, int wave, int lane) {
@@ -413,12 +421,13 @@ struct SmallLoader {
         const int64_t left = o.entries - 1 - entry0;
         const int64_t at = entry < left ? entry : left;
         const int64_t from = at * o.ld + (PAIRED && r / S::kPairedOf % 2 == 1 ? o.second : 0);
-        offset[j] = static_cast<uint32_t>((from + ((lane % 8) ^ small_row_swizzle(r)) * 8) * 2);
+        offset[j] = static_cast<uint32_t>((from * HALVES + ((lane % 8) ^ small_row_swizzle(r)) * 8) * 2);
       } else {
-        const int chunk = (lane % kLanesOfRow) ^ small_column_swizzle<TILE>(r);
-        const int64_t left = o.entries - 8 - entry0;
-        const int64_t at = chunk * 8 < left ? chunk * 8 : left;
-        offset[j] = static_cast<uint32_t>(at * 2);
+        constexpr int kChunk = 8 / HALVES;  // entries of 16 bytes
+        const int chunk = (lane % kLanesOfRow) ^ small_column_swizzle<TILE, HALVES>(r);
+        const int64_t left = o.entries - kChunk - entry0;
+        const int64_t at = chunk * kChunk < left ? chunk * kChunk : left;
+        offset[j] = static_cast<uint32_t>(at * 2 * HALVES);
       }
     }
   }
@@ -428,13 +437,13 @@ struct SmallLoader {
       const bool upper = (((lane % 8) ^ small_row_swizzle(row + j * kRowsOfLoad)) & 4) != 0;
       return half && upper ? offset[j] - 64 : offset[j];
     } else {
-      return offset[j] + static_cast<uint32_t>(min(row + j * kRowsOfLoad, left)) * static_cast<uint32_t>(o.ld * 2);
+      return offset[j] + static_cast<uint32_t>(min(row + j * kRowsOfLoad, left)) * static_cast<uint32_t>(o.ld * 2 * HALVES);
     }
   }
 };
 
-// Fragments of 16 entries and a step's 32 k's, as Reader's.
-template <int TILE, bool ROWS>
+// Fragments of 16 entries and a step's 32 k's (FP32: 16), as Reader's.
+template <int TILE, bool ROWS, int HALVES>
 struct SmallReader {
   uint32_t at, column;
   __device__ __forceinline__ void init(int entry, int lane) {
@@ -442,15 +451,24 @@ struct SmallReader {
     if constexpr (ROWS) {
       at = static_cast<uint32_t>((entry + j) * 128);
       column = static_cast<uint32_t>((group ^ small_row_swizzle(j)) * 16);
+    } else if constexpr (HALVES == 2) {
+      at = static_cast<uint32_t>(group * 4 * TILE + j % 4) * 4;
+      column = static_cast<uint32_t>(((entry + j) / 4) ^ small_column_swizzle<TILE, HALVES>(group * 4)) * 16;
     } else {
       const int k = group * 8 + j / 4;
       at = static_cast<uint32_t>(k * TILE) * 2;
-      column = static_cast<uint32_t>(((entry / 8 + j % 4 / 2) ^ small_column_swizzle<TILE>(k)) * 8 + j % 2 * 4) * 2;
+      column = static_cast<uint32_t>(((entry / 8 + j % 4 / 2) ^ small_column_swizzle<TILE, HALVES>(k)) * 8 + j % 2 * 4) * 2;
     }
   }
   __device__ __forceinline__ s16x8 read(uint32_t stage, int step, int f) const {
     if constexpr (ROWS) {
       return *(ATTNRES_LDS const s16x8*)(stage + at + (column ^ (step * 64u)) + f * 16 * 128);
+    } else if constexpr (HALVES == 2) {
+      const uint32_t from = stage + step * 32 * TILE * 2 + at + (column ^ (f * 64u));
+      f32x4 x;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] = *(ATTNRES_LDS const float*)(from + e * TILE * 4);
+      return __builtin_bit_cast(s16x8, x);
     } else {
       const uint32_t from = stage + step * 32 * TILE * 2 + at + (column ^ (f * 32u));
       const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((ATTNRES_LDS s16x4*)(from));
@@ -467,6 +485,7 @@ __device__ __forceinline__ bool small_multiply(const Product& p, const TileAt& t
                                                typename Shape<SHAPE>::Sums& acc) {
   using S = Shape<SHAPE>;
   constexpr int TILE = S::kTileOf, kDownOf = S::kDownOf, kAcrossOf = S::kAcrossOf, kSharers = S::kSharers;
+  constexpr int kHalves = sizeof(T) / 2;
   constexpr int kSteps = A_ROWS || B_ROWS || TILE == 64 ? 2 : 1, kDepthOf = kSteps * kDepth, kStagesOf = kStages / kSteps;
   const int wave = wave_index() % S::kWavesOf, sharer = wave_index() / S::kWavesOf, lane = threadIdx.x % 64;
   // a sharer's stages, at least one; by pairs of 32 k's, so that lines stay whole
@@ -483,12 +502,12 @@ __device__ __forceinline__ bool small_multiply(const Product& p, const TileAt& t
   const int first = range.first, stages = (range.count + kSteps - 1) / kSteps, total = stages * SEGMENTS;
   const bool odd = range.count % kSteps != 0;  // the last stage is one step
   const int64_t a0 = static_cast<int64_t>(tile.a) * (PAIRED ? TILE / 2 : TILE), b0 = static_cast<int64_t>(tile.b) * TILE;
-  SmallLoader<TILE, kDepthOf, A_ROWS, PAIRED> load_a;
-  SmallLoader<TILE, kDepthOf, B_ROWS, false> load_b;
+  SmallLoader<TILE, kDepthOf, A_ROWS, PAIRED, kHalves> load_a;
+  SmallLoader<TILE, kDepthOf, B_ROWS, false, kHalves> load_b;
   constexpr int kLoadsOf = decltype(load_a)::kLoadsOf;
   load_a.init(p.a, a0, wave, lane);
   load_b.init(p.b, b0, wave, lane);
-  const int64_t origin_a = (A_ROWS ? a0 * p.a.ld : a0) * 2, origin_b = (B_ROWS ? b0 * p.b.ld : b0) * 2;
+  const int64_t origin_a = (A_ROWS ? a0 * p.a.ld : a0) * 2 * kHalves, origin_b = (B_ROWS ? b0 * p.b.ld : b0) * 2 * kHalves;
   const int64_t next_a = (A_ROWS ? 1 : p.a.ld) * kDepthOf * 2, next_b = (B_ROWS ? 1 : p.b.ld) * kDepthOf * 2;
   const int64_t from_a = origin_a + first * (next_a / kSteps), from_b = origin_b + first * (next_b / kSteps);
   const uint32_t lds0 = lds_byte(lds + sharer * S::kRing);
@@ -498,7 +517,7 @@ __device__ __forceinline__ bool small_multiply(const Product& p, const TileAt& t
   const auto load = [&](uint32_t buffer) {
     const char* a = scalar(reinterpret_cast<const char*>(p.a.part[part_of_a<SEGMENTS>(segment)]) + from_a + stage * next_a);
     const char* b = scalar(reinterpret_cast<const char*>(p.b.part[part_of_b<SEGMENTS>(segment)]) + from_b + stage * next_b);
-    const int64_t k = (first + static_cast<int64_t>(stage) * kSteps) * kDepth;
+    const int64_t k = (first + static_cast<int64_t>(stage) * kSteps) * (kDepth / kHalves);
     const int left_a = __builtin_amdgcn_readfirstlane(static_cast<int>(p.a.depth - 1 - k));
     const int left_b = __builtin_amdgcn_readfirstlane(static_cast<int>(p.b.depth - 1 - k));
     const bool half = odd && stage + 1 == stages;
@@ -508,8 +527,8 @@ __device__ __forceinline__ bool small_multiply(const Product& p, const TileAt& t
     for (int j = 0; j < kLoadsOf; ++j) load_lds(b, load_b.at(p.b, left_b, half, lane, j), buffer + kB + slot + j * 1024);
     if (++stage == stages) stage = 0, ++segment;
   };
-  SmallReader<TILE, A_ROWS> read_a;
-  SmallReader<TILE, B_ROWS> read_b;
+  SmallReader<TILE, A_ROWS, kHalves> read_a;
+  SmallReader<TILE, B_ROWS, kHalves> read_b;
   read_a.init((wave % 2) * (16 * kDownOf), lane);
   read_b.init((wave / 2) * (16 * kAcrossOf), lane);
   struct Fragments {
