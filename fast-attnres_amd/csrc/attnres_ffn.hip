@@ -17,9 +17,9 @@
 // BF16, g and u would each bring an error of the size of the gradients' own rounding (0.0017, root mean square); as it is the gradients
 // are off by 0.0024.  With `saved` NULL the backward forms them again, which adds a third to its products.
 //
-// 16-bit operands are multiplied as they are; a, dg and du are rounded to their type.  FP32 values are written as the
-// sum of three BF16 numbers, 24 bits over FP32's whole range, and a product is the six products of parts that are
-// not below 2^-26 of it: FP32 matrix instructions run at a sixteenth of the BF16 rate.
+// 16-bit operands are multiplied as they are; a, dg and du are rounded to their type.  FP32 values of larger calls (kSingleRows) are written
+// as the sum of three BF16 numbers, 24 bits over FP32's whole range, and a product is the six products of parts that are
+// not below 2^-26 of it: FP32 matrix instructions run at a sixteenth of the BF16 rate.  Smaller calls (Single) take those, and pack nothing.
 
 #include "attnres_product.h"
 
@@ -602,11 +602,12 @@ __global__ void __launch_bounds__(kBlock) attnres_ffn_pack_kernel(PacksArgs<X> a
 }
 
 // ------------------------------------------------------------------- few rows
-// The forward of up to 16 rows, or of kFewRows where tiles need packed weights, reads the weights once and is bound by that: wavefronts
+// The forward of up to 16 rows, 32 of FP32, or kFewRows where tiles need packed weights, reads the weights once and is bound by that: wavefronts
 // share the depth of 16 entries of A (of a gate's 8 and the up projection's 8 that belong to them), so that all of a workgroup's weights
 // are asked for at once, and nothing is packed.  FP32 inputs by FP32 matrix instructions, which so few rows have time for.
 // A lane's 16 bytes are of a row of its own, which the caches serve slowly: BF16, 2048 x 5632, by tiles in brackets, 1 row 19.2 (31) us, 16
-// 26.2 (25.8), 48 46.6 (26.8); 1024 x 2816, 1 row 10.7 (20), 32 15.9 (18.4).
+// 26.2 (25.8), 48 46.6 (26.8); 1024 x 2816, 1 row 10.7 (20), 32 15.9 (18.4); FP32, 4096 x 11264, 17 rows 184 (241), 32 211 (229);
+// packed, 4001 x 4000, 64 rows 117 (157).
 constexpr int64_t kFewRows = 64;
 
 // The wavefronts' sums over their shares of the depth, in LDS; ROWS of a's tiles by TILES of the rows'.
@@ -758,14 +759,18 @@ constexpr int64_t kMaxHidden = int64_t{1} << 16;
 constexpr int64_t kMaxStride = int64_t{1} << 22;  // of operands multiplied in place: 256 rows stay within 32-bit offsets
 constexpr int64_t kMaxSecond = int64_t{1} << 30;  // from the gate's rows to the up's, of 16 bits
 constexpr int64_t kMaxTiles = int64_t{1} << 22;   // a launch takes fewer than 2^32 threads
-// Rounds of the chip up to which the gradients' products go in one launch: one product's last round is filled by the next
+// Rounds of the chip up to which the gradients' products go in one launch of tiles of 256 (smaller ones always do): one product's last round is filled by the next
 // one's first, which counts less the more rounds there are, and each then finds less of its operands in the caches.
 // Three launches against one, rows x width x hidden, BF16: 4096 x 1024 x 2816 0.309 ms to 0.144, 4096 x 2048 x 5632
-// 0.603 to 0.496, 8192 x 2048 x 5632 0.990 to 0.943; 4096 x 4096 x 8192 1.21 to 1.20; 16384 x 4096 x 11264 6.17 to 6.23.
+// 0.603 to 0.496, 8192 x 2048 x 5632 0.990 to 0.943; 4096 x 4096 x 8192 1.21 to 1.20; 16384 x 4096 x 11264 6.17 to 6.23.  Tiles of 128,
+// 2048 x 2048 x 5632: 0.374 to 0.327; FP32 on tiles of 64, 200 x 4096 x 11264: 1.24 to 1.09.
 constexpr uint32_t kTogether = 8;
-// Rows up to which FP32 inputs are multiplied as they are, on tiles of 64.
-constexpr int64_t kSingleRows = 512;
-constexpr double kSingleCost = 3.0;  // of their products, in 16-bit products of twice the depth
+// Rows, and rows times widths, up to which FP32 inputs are multiplied as they are: FP32 instructions reach 100-115 TFLOP/s, the six products
+// of parts 170 once their operands are packed (22 bytes moved per element of a weight and tile of rows, not 4).  Forward and
+// backward in kernels, by parts in brackets: 512 x 2048 x 4096 0.66 (0.84) ms, 1024 x 1024 x 2816 0.58 (0.62), 2048 x 512 x 512
+// 0.13 (0.19), 4000 x 256 x 1024 0.23 (0.26), 1024 x 4096 x 4096 2.52 (2.52); 1500 x 1024 x 2816 0.82 (0.74).
+constexpr int64_t kSingleRows = 1024;
+constexpr int64_t kSingleProducts = int64_t{1} << 31;
 
 enum Pass { kForward = 0, kBackward = 1, kBackwardAgain = 2 };  // the last: without saved g and u
 
@@ -840,14 +845,15 @@ class Schedule {
 // The cut that takes the least time: the schedule of all tiles at a unit's rate for them, and the partial sums' way to memory and
 // back.  Rates as measured on a full chip.
 Cut choose_cut(const Outputs* outputs, int count, const FfnPlan& plan, bool whole) {
-  const double segments = plan.single ? kSingleCost : plan.segments;
+  const int segments = plan.segments;
   Cut best{256, {1, 1, 1}, 0};
   double least = 0.0;
   for (const int tile : {256, 128, 64}) {
-    if (plan.single && tile > 64) continue;
+    if (plan.single && tile > 128) continue;
     // a workgroup alone on a unit that has room for more reaches two thirds of its rate
     const double alone = tile == 256 ? 1.0 : 1.5;
-    const double rate = (tile == 256 ? 1.25e15 : tile == 128 ? 0.87e15 : 0.6e15) / kUnits;
+    // FP32 operands: their depth counts twice
+    const double rate = (plan.single ? (tile == 128 ? 0.23e15 : 0.2e15) : tile == 256 ? 1.25e15 : tile == 128 ? 0.87e15 : 0.6e15) / kUnits;
     const double ends = tile == 256 ? 5e-6 : tile == 128 ? 2e-6 : 1e-6;  // of a tile: its first loads and its epilogue
     int64_t tiles[3] = {};
     bool fits = true;
@@ -894,18 +900,19 @@ int64_t saved_bytes(const Sizes& s) {
 
 FfnPlan make_plan(const Sizes& s, int pass) {
   FfnPlan p{};
-  p.single = s.dtype == ATTNRES_F32 && s.rows <= kSingleRows;
+  p.rows_pad = round_up(s.rows, kDepth);
+  p.width_pad = round_up(s.width, kDepth);
+  p.hidden_pad = round_up(s.hidden, kDepth);
+  p.out_pad = round_up(s.out_width, kDepth);
+  p.single = s.dtype == ATTNRES_F32 &&
+             (s.rows <= kSingleRows || p.rows_pad * std::max(p.width_pad, p.out_pad) * p.hidden_pad <= kSingleProducts);
   const bool split = s.dtype == ATTNRES_F32 && !p.single, backward = pass != kForward;
   p.parts = split ? 3 : 1;
   p.segments = split ? 6 : 1;
   p.halves = p.single ? 2 : 1;
   const int64_t size = 2 * p.halves;
-  p.rows_pad = round_up(s.rows, kDepth);
-  p.width_pad = round_up(s.width, kDepth);
-  p.hidden_pad = round_up(s.hidden, kDepth);
-  p.out_pad = round_up(s.out_width, kDepth);
   // the depth of a product is a whole number of stages, the rest of the last one zeros
-  p.few = s.rows <= (split || s.width != p.width_pad || s.hidden != p.hidden_pad ? kFewRows : kFewRows / 4);
+  p.few = s.rows <= (s.width != p.width_pad || s.hidden != p.hidden_pad ? kFewRows : p.single ? kFewRows / 2 : kFewRows / 4);
   const bool tiles = backward || !p.few;
   p.pack_x = tiles && (split || s.width != p.width_pad || (backward && s.rows != p.rows_pad));
   p.pack_gate_up = tiles && (split || s.width != p.width_pad || s.hidden != p.hidden_pad);
@@ -995,8 +1002,8 @@ template <class X, class F>
 void with_shape(const Cut& cut, F f) {
   if constexpr (!std::is_same_v<X, Single>) {
     if (cut.tile == 256) return f(std::integral_constant<int, 256>{});
-    if (cut.tile == 128) return f(std::integral_constant<int, 128>{});
   }
+  if (cut.tile == 128) return f(std::integral_constant<int, 128>{});
   switch (cut.shape()) {
     case 65: return f(std::integral_constant<int, 65>{});
     case 66: return f(std::integral_constant<int, 66>{});
@@ -1240,7 +1247,7 @@ void ffn_backward(const Call& c, const void* grad_out, const char* saved, void* 
   std::sort(order, order + 3, [&](int i, int j) { return of[i].product.depth * splits[j] > of[j].product.depth * splits[i]; });
   uint32_t all = 0;
   for (const int i : order) all += results[i] != nullptr ? workgroups(of[i]) : 0;
-  const bool together = all <= kTogether * kUnits;
+  const bool together = tile < 256 || all <= kTogether * kUnits;
   GradientsArgs g{};
   int count = 0;
   uint32_t grid = 0;

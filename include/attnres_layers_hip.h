@@ -111,9 +111,9 @@ int attnres_hip_loss_backward(const void* hidden, int64_t hidden_stride, const v
  * out = (act(x Wg^T) * (x Wu^T)) Wd^T.  x [rows, width] (rows x_stride apart), gate_up [2 hidden, width]: Wg's
  * rows, then Wu's (gate_up_stride apart), down [out_width, hidden] (down_stride apart), out [rows, out_width]
  * contiguous, all of one dtype; 1 <= width, out_width <= ATTNRES_MAX_WIDTH, 1 <= hidden <= 2^16, rows up to 2^24 and
- * rows and hidden up to 2^22 tiles of 256 x 128 together.  Operands of 16 bits whose widths are multiples of 32 are
- * multiplied where they lie: their rows start at multiples of 16 bytes, at most 2^22 elements apart, and hidden *
- * gate_up_stride is at most 2^30 (else ATTNRES_ERR_STRIDE).
+ * rows and hidden up to 2^22 tiles of 256 x 128 together.  Operands whose widths are multiples of 32 are
+ * multiplied where they lie: their rows start at multiples of 16 bytes, multiples of 8 and at most 2^22 elements apart,
+ * and hidden * gate_up_stride is at most 2^30, of FP32 2^29 (else ATTNRES_ERR_STRIDE).
  * saved: NULL, or what the backward reads (g = x Wg^T and u = x Wu^T in FP32, of 16-bit inputs cut to 24 bits).
  * workspace: backward 0 for the forward's, 1 for the backward's, 2 for that of a backward without saved, which forms
  * g and u again.  saved and workspace start at multiples of 16 bytes (else ATTNRES_ERR_WORKSPACE). */

@@ -127,3 +127,10 @@ def test_workspaces_are_of_the_shape_alone():
     assert size(*shape, 0, 3) == -1
     for short in (forward - 1, 0):
         assert _forward(rows=300, bytes=short, out_width=64) == _native.ERR_WORKSPACE
+
+
+@pytest.mark.parametrize("call", [_forward, _backward])
+@pytest.mark.parametrize("overrides", [dict(x=4100), dict(x_stride=68), dict(down=4104), dict(gate_up=4104),
+                                       dict(hidden=192, gate_up_stride=2**22, down_stride=192)])
+def test_fp32_operands_in_place_are_checked(call, overrides):
+    assert call(dtype=2, **overrides) == _native.ERR_STRIDE
