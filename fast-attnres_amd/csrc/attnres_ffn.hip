@@ -10,7 +10,7 @@
 // in one each (kTogether).  Tiles are of 256, 128 or 64 by a model of when the chip's last unit is done (choose_cut); products whose
 // tiles do not fill the chip are cut along their depth, and the parts' FP32 sums added up in order.
 // 16384 x 4096 x 11264, BF16: forward 3.7 ms (1.22 PFLOP/s), backward 7.9 (1.15); power sets the clock there, and the library's
-// products of these sizes reach 1.40.  2048 x 1024 x 2816 in 162 us of kernels, 0.65.
+// products of these sizes reach 1.40.  2048 x 1024 x 2816 in 160 us of kernels, 0.66.
 //
 // What goes from the forward to the backward is g and u, in the order in which a lane holds them, so both sides
 // move them 16 bytes per lane with no detour over LDS: FP32 for FP32 inputs, else FP32 cut to 24 bits (2^-17).  Rounded to
@@ -170,8 +170,8 @@ __device__ __forceinline__ void take_part(float* x, const uint32_t* packed, int 
 }
 
 // ------------------------------------------------------------------ g, u and a
-// 16384 x 4096 x 11264, BF16, 2.40-2.43 ms with g and u saved (1.25 PFLOP/s); 4096 x 2048 x 8192, FP16, 0.26-0.29 without, of
-// which about 9 us for each of a unit's four tiles go to filling the ring and to the epilogue; 48 x 2048 x 5632 14 us, reading W at 3.3 TB/s.
+// 16384 x 4096 x 11264, BF16, 2.40-2.43 ms with g and u saved (1.25 PFLOP/s); 4096 x 2048 x 8192, FP16, 0.25-0.28 without, of
+// which about 8 us for each of a unit's four tiles go to filling the ring and to the epilogue; 48 x 2048 x 5632 14 us, reading W at 3.3 TB/s.
 
 struct GateArgs {
   Product product;  // A: gate's and up's rows, paired; B: X
@@ -462,7 +462,7 @@ __device__ __forceinline__ void store_tile(const OutArgs& g, const TileAt& tile,
   }
 }
 
-// Y (A: Wd by rows, B: a by rows).  16384 x 4096 x 11264, BF16, 1.25-1.33 ms (1.1-1.2 PFLOP/s); 48 x 2048 x 5632 in 8 parts 9.4 us, reading
+// Y (A: Wd by rows, B: a by rows).  16384 x 4096 x 11264, BF16, 1.25-1.33 ms (1.1-1.2 PFLOP/s); 48 x 2048 x 5632 in 8 parts 9.2 us, reading
 // Wd at 2.5 TB/s.
 template <class X, class OUT, int SHAPE>
 __global__ void __launch_bounds__(Shape<SHAPE>::kAllThreads, Shape<SHAPE>::kGroupsOf) attnres_ffn_out_kernel(OutArgs g) {
@@ -602,8 +602,8 @@ __global__ void __launch_bounds__(kBlock) attnres_ffn_pack_kernel(PacksArgs<X> a
 }
 
 // ------------------------------------------------------------------- few rows
-// The forward of up to 16 rows, 32 of FP32, or kFewRows where tiles need packed weights, reads the weights once and is bound by that: wavefronts
-// share the depth of 16 entries of A (of a gate's 8 and the up projection's 8 that belong to them), so that all of a workgroup's weights
+// The forward of up to 16 rows, 32 of FP32, or kFewRows where tiles need packed weights, reads the weights once and is bound by that:
+// wavefronts share the depth of 16 entries of A (of a gate's 8 and the up projection's 8 that belong to them), so that all of a workgroup's weights
 // are asked for at once, and nothing is packed.  FP32 inputs by FP32 matrix instructions, which so few rows have time for.
 // A lane's 16 bytes are of a row of its own, which the caches serve slowly: BF16, 2048 x 5632, by tiles in brackets, 1 row 19.2 (31) us, 16
 // 26.2 (25.8), 48 46.6 (26.8); 1024 x 2816, 1 row 10.7 (20), 32 15.9 (18.4); FP32, 4096 x 11264, 17 rows 184 (241), 32 211 (229);
@@ -759,9 +759,9 @@ constexpr int64_t kMaxHidden = int64_t{1} << 16;
 constexpr int64_t kMaxStride = int64_t{1} << 22;  // of operands multiplied in place: 256 rows stay within 32-bit offsets
 constexpr int64_t kMaxSecond = int64_t{1} << 30;  // from the gate's rows to the up's, of 16 bits
 constexpr int64_t kMaxTiles = int64_t{1} << 22;   // a launch takes fewer than 2^32 threads
-// Rounds of the chip up to which the gradients' products go in one launch of tiles of 256 (smaller ones always do): one product's last round is filled by the next
-// one's first, which counts less the more rounds there are, and each then finds less of its operands in the caches.
-// Three launches against one, rows x width x hidden, BF16: 4096 x 1024 x 2816 0.309 ms to 0.144, 4096 x 2048 x 5632
+// Rounds of the chip up to which the gradients' products go in one launch of tiles of 256 (smaller ones always do): one product's last
+// round is filled by the next one's first, which counts less the more rounds there are, and each then finds less of its operands in the
+// caches.  Three launches against one, rows x width x hidden, BF16: 4096 x 1024 x 2816 0.309 ms to 0.144, 4096 x 2048 x 5632
 // 0.603 to 0.496, 8192 x 2048 x 5632 0.990 to 0.943; 4096 x 4096 x 8192 1.21 to 1.20; 16384 x 4096 x 11264 6.17 to 6.23.  Tiles of 128,
 // 2048 x 2048 x 5632: 0.374 to 0.327; FP32 on tiles of 64, 200 x 4096 x 11264: 1.24 to 1.09.
 constexpr uint32_t kTogether = 8;
@@ -885,7 +885,10 @@ Cut choose_cut(const Outputs* outputs, int count, const FfnPlan& plan, bool whol
       if (least == 0.0 || time < least) {
         least = time;
         best = cut;
-        best.shared = tile != 64 || least_depth / kDepth < 16 ? 0 : workgroups <= kUnits ? 2 : workgroups <= 2 * kUnits && least_depth / kDepth >= 32 ? 1 : 0;
+        const int64_t steps = least_depth / kDepth;
+        best.shared = 0;
+        if (tile == 64 && workgroups <= kUnits && steps >= 16) best.shared = 2;
+        else if (tile == 64 && workgroups > kUnits && workgroups <= 2 * kUnits && steps >= 32) best.shared = 1;
       }
       if (whole || worse == 4 || cut.splits[longest] >= 32 || outputs[longest].depth / kDepth / (cut.splits[longest] + 1) < 4) break;
       ++cut.splits[longest];
@@ -1107,7 +1110,8 @@ void few_forward(const Call& c, void* out, char* saved) {
 OutArgs out_args(const Call& c, const Operand& a, const Operand& b, int64_t depth, int64_t entries_a, int64_t half, int64_t half_pad,
                  int64_t entries_b, int tile, int splits, int64_t partial, void* out) {
   OutArgs g{};
-  g.product = {a, b, nullptr, depth * c.plan.halves, 0, static_cast<int>(tiles_of(entries_a, tile)), static_cast<int>(tiles_of(entries_b, tile)), splits};
+  g.product = {a, b, nullptr, depth * c.plan.halves, 0, static_cast<int>(tiles_of(entries_a, tile)),
+               static_cast<int>(tiles_of(entries_b, tile)), splits};
   g.entries_a = entries_a;
   g.half = half;
   g.half_pad = half_pad;

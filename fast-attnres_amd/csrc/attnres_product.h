@@ -374,10 +374,10 @@ __device__ __forceinline__ void multiply(const Product& p, const TileAt& tile, c
 // they are read by whole lines of 128 bytes (4096 x 16384 x 4096, both as rows, tiles of 128: 710 -> 614 us), else 32, twice as many stages ahead
 // (both as columns: 610 -> 592; tiles of 64 are faster with 64, 55 -> 47 us for 1024 x 5632 x 2048).  A step is 32 k's, and the next
 // one's fragments are read meanwhile.
-// SHAPE: the tile's size, or 65 and 66: tiles of 64 by two and by four times as many wavefronts, which share the depth and have a ring of stages
-// each.  For launches of one or two workgroups to a unit, which has nothing else to do while a step's reads and the barrier are waited
-// for (four times: 64 x 11264 x 2048 19.6 -> 13.0 us, 1024 x 1024 x 2816 24.6 -> 16.4, more stages ahead change nothing; twice:
-// 32 x 22528 x 4096 51 -> 37 us, 128 x 11264 x 2048 19.6 -> 18.1; from a depth of 1024 on, 300 x 4096 x 768 10.6 -> 11.8).
+// SHAPE: the tile's size, or 65 and 66: tiles of 64 by two and by four times as many wavefronts, which share the depth and have a ring
+// of stages each.  For launches of two workgroups or one to a unit, which has nothing else to do while a step's reads and the barrier
+// are waited for (four times: 64 x 11264 x 2048 19.6 -> 13.0 us, 1024 x 1024 x 2816 24.6 -> 16.4, more stages ahead change nothing;
+// twice: 32 x 22528 x 4096 51 -> 37 us, 128 x 11264 x 2048 19.6 -> 18.1; but 300 x 4096 x 768 10.6 -> 11.8, so from a depth of 1024 on).
 template <int SHAPE>
 struct Shape {
   static constexpr int kTileOf = SHAPE - SHAPE % 4, TILE = kTileOf;
