@@ -208,8 +208,24 @@ class AdamW(torch.optim.Optimizer):
                        masters=[s["master"] for s in states] if has_master else None, grad_scale=grad_scale)
 
     def load_state_dict(self, state_dict: dict) -> None:
-        """As in ``torch.optim.Optimizer``, but that the states keep the dtypes they were saved in."""
-        super().load_state_dict(state_dict)
+        """As in ``torch.optim.Optimizer``, hooks included, but that the states keep the dtypes they were saved in."""
+        loaded = {}
+
+        def before(_optimizer: Any, state_dict: dict) -> None:  # after the caller's hooks, so as they leave it
+            loaded.update(state_dict)
+
+        def after(_optimizer: Any) -> None:  # before the caller's
+            self._take_state(loaded)
+
+        hooks = (self.register_load_state_dict_pre_hook(before), self.register_load_state_dict_post_hook(after, prepend=True))
+        try:
+            super().load_state_dict(state_dict)
+        finally:
+            for hook in hooks:
+                hook.remove()
+
+    def _take_state(self, state_dict: dict) -> None:
+        """The saved states in the dtypes they were saved in, in place of those that ``torch.optim.Optimizer`` has cast."""
         for group in self.param_groups:
             for name in self.defaults:
                 group.setdefault(name, self.defaults[name])

@@ -1,0 +1,51 @@
+"""State dicts of attnres.optim.AdamW on the CPU: what is loaded, what is kept and what is refused.
+Nothing launches."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from attnres import optim
+
+BF16, FP32, FP8 = torch.bfloat16, torch.float32, torch.float8_e4m3fn
+
+
+def _parameter(dtype=FP32, shape=(96, 64)):
+    return torch.nn.Parameter(torch.linspace(-1.0, 1.0, 96 * 64).reshape(shape).to(dtype))
+
+
+def _torch_dict(dtype=FP32, kind=torch.optim.AdamW, **options):
+    """Of torch's optimizer after a step."""
+    p = _parameter(dtype)
+    optimizer = kind([p], **options)
+    p.grad = torch.full_like(p, 0.5)
+    optimizer.step()
+    return optimizer.state_dict()
+
+
+def test_hooks_of_a_load_see_and_make_what_is_loaded():
+    p = _parameter()
+    optimizer = optim.AdamW([p])
+    seen = []
+
+    def before(_optimizer, state_dict):
+        state = {index: {**state, "exp_avg": state["exp_avg"] + 7.0} for index, state in state_dict["state"].items()}
+        return {**state_dict, "state": state, "param_groups": [{**group, "lr": 0.25} for group in state_dict["param_groups"]]}
+
+    def after(optimizer):
+        seen.append((optimizer.state[p]["exp_avg"].dtype, optimizer.state[p]["step"]))
+        optimizer.state[p]["exp_avg_sq"].fill_(3.0)
+
+    optimizer.register_load_state_dict_pre_hook(before)
+    optimizer.register_load_state_dict_post_hook(after)
+    saved = _torch_dict()
+    for _ in range(2):  # a load leaves no hooks of its own
+        optimizer.load_state_dict(saved)
+        assert torch.equal(optimizer.state[p]["exp_avg"], saved["state"][0]["exp_avg"] + 7.0)
+        assert bool((optimizer.state[p]["exp_avg_sq"] == 3.0).all()) and optimizer.param_groups[0]["lr"] == 0.25
+    assert seen == [(FP32, 1)] * 2
+    with pytest.raises(ValueError):  # another number of groups
+        optimizer.load_state_dict({**saved, "param_groups": saved["param_groups"] * 2})
+    optimizer.load_state_dict(saved)
+    assert len(seen) == 3
