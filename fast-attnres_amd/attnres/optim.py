@@ -101,7 +101,9 @@ class AdamW(torch.optim.Optimizer):
     GPU, for steps in a HIP graph (take one step before capturing); ``lr`` may be an FP32
     tensor of one element on the GPU, to change it between replays.
 
-    State dicts keep the states' dtypes, and those of ``torch.optim.AdamW`` load as 32-bit states.
+    State dicts keep the states' dtypes, and those of ``torch.optim.AdamW`` load as 32-bit states.  Options that this
+    step does not have (``amsgrad``, ``maximize``, ``differentiable``, a decay that is not decoupled) are refused, in a state
+    dict too.
     """
 
     def __init__(self, params: Iterable, lr: float | Tensor = 1e-3, betas: tuple[float, float] = (0.9, 0.999), eps: float = 1e-8,
@@ -123,6 +125,11 @@ class AdamW(torch.optim.Optimizer):
         for name in ("masters", "capturable"):
             if not isinstance(options[name], bool):
                 raise TypeError(f"{name} must be a bool")
+        for name in ("amsgrad", "maximize", "differentiable"):
+            if options.get(name):
+                raise ValueError(f"AdamW has no {name}")
+        if not options.get("decoupled_weight_decay", True) and options["weight_decay"] != 0.0:
+            raise ValueError("AdamW's weight decay is decoupled")
 
     def add_param_group(self, param_group: dict) -> None:
         """As in ``torch.optim.Optimizer``, with the group's options checked."""
@@ -212,6 +219,8 @@ class AdamW(torch.optim.Optimizer):
         loaded = {}
 
         def before(_optimizer: Any, state_dict: dict) -> None:  # after the caller's hooks, so as they leave it
+            for group in state_dict["param_groups"]:
+                self._check_options({**self.defaults, **group})
             loaded.update(state_dict)
 
         def after(_optimizer: Any) -> None:  # before the caller's

@@ -49,3 +49,34 @@ def test_hooks_of_a_load_see_and_make_what_is_loaded():
         optimizer.load_state_dict({**saved, "param_groups": saved["param_groups"] * 2})
     optimizer.load_state_dict(saved)
     assert len(seen) == 3
+
+
+@pytest.mark.parametrize("options,match", [(dict(maximize=True), "maximize"), (dict(amsgrad=True), "amsgrad"),
+                                           (dict(differentiable=True), "differentiable"),
+                                           (dict(decoupled_weight_decay=False, weight_decay=0.1), "decoupled")])
+def test_options_that_the_step_does_not_have_are_refused(options, match):
+    """From a state dict (which then leaves the optimizer as it was) and from a group."""
+    p = _parameter()
+    optimizer = optim.AdamW([p], lr=0.5)
+    saved = _torch_dict()
+    for make in (lambda: optimizer.load_state_dict({**saved, "param_groups": [{**saved["param_groups"][0], **options}]}),
+                 lambda: optimizer.add_param_group({"params": [_parameter()], **options}),
+                 lambda: optim.AdamW([{"params": [p], **options}])):
+        with pytest.raises(ValueError, match=match):
+            make()
+    assert not optimizer.state and optimizer.param_groups[0]["lr"] == 0.5 and len(optimizer.param_groups) == 1
+    with pytest.raises(ValueError, match="decoupled"):
+        optimizer.load_state_dict(_torch_dict(kind=torch.optim.Adam, weight_decay=0.1))
+    optimizer.load_state_dict(_torch_dict())
+    optimizer.load_state_dict(_torch_dict(kind=torch.optim.Adam))  # no decay, so the same step
+    assert optimizer.state[p]["step"] == 1
+
+
+@pytest.mark.parametrize("options,error", [(dict(betas=(0.9, 1.5)), ValueError), (dict(state_bits=4), ValueError), (dict(masters=1), TypeError),
+                                           (dict(lr=-1.0), ValueError)])
+def test_options_of_loaded_groups_are_checked(options, error):
+    optimizer = optim.AdamW([_parameter()], lr=0.5)
+    saved = _torch_dict()
+    with pytest.raises(error, match=next(iter(options))):
+        optimizer.load_state_dict({**saved, "param_groups": [{**saved["param_groups"][0], **options}]})
+    assert not optimizer.state and optimizer.param_groups[0]["lr"] == 0.5
