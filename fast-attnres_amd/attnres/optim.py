@@ -215,8 +215,10 @@ class AdamW(torch.optim.Optimizer):
                        masters=[s["master"] for s in states] if has_master else None, grad_scale=grad_scale)
 
     def load_state_dict(self, state_dict: dict) -> None:
-        """As in ``torch.optim.Optimizer``, hooks included, but that the states keep the dtypes they were saved in."""
+        """As in ``torch.optim.Optimizer``, hooks included, but that the states keep the dtypes they were saved in,
+        and options that the saved groups do not name (those of torch's) stay as they are."""
         loaded = {}
+        own = [{name: group[name] for name in self.defaults} for group in self.param_groups]
 
         def before(_optimizer: Any, state_dict: dict) -> None:  # after the caller's hooks, so as they leave it
             for group in state_dict["param_groups"]:
@@ -224,6 +226,10 @@ class AdamW(torch.optim.Optimizer):
             loaded.update(state_dict)
 
         def after(_optimizer: Any) -> None:  # before the caller's
+            for group, options in zip(self.param_groups, own):
+                for name, value in options.items():
+                    group.setdefault(name, value)
+                group["fused"] = True
             self._take_state(loaded)
 
         hooks = (self.register_load_state_dict_pre_hook(before), self.register_load_state_dict_post_hook(after, prepend=True))
@@ -235,10 +241,6 @@ class AdamW(torch.optim.Optimizer):
 
     def _take_state(self, state_dict: dict) -> None:
         """The saved states in the dtypes they were saved in, in place of those that ``torch.optim.Optimizer`` has cast."""
-        for group in self.param_groups:
-            for name in self.defaults:
-                group.setdefault(name, self.defaults[name])
-            group["fused"] = True
         saved_ids = [i for group in state_dict["param_groups"] for i in group["params"]]
         params = [(p, group) for group in self.param_groups for p in group["params"]]
         shared: dict[tuple, Tensor] = {}

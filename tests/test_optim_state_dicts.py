@@ -80,3 +80,14 @@ def test_options_of_loaded_groups_are_checked(options, error):
     with pytest.raises(error, match=next(iter(options))):
         optimizer.load_state_dict({**saved, "param_groups": [{**saved["param_groups"][0], **options}]})
     assert not optimizer.state and optimizer.param_groups[0]["lr"] == 0.5
+
+
+def test_options_that_a_state_dict_does_not_name_stay_as_they_are():
+    first, second = _parameter(), _parameter()
+    optimizer = optim.AdamW([{"params": [first], "state_bits": 8, "masters": True}, {"params": [second]}], lr=0.5)
+    theirs = torch.optim.AdamW([{"params": [_parameter()], "lr": 0.25}, {"params": [_parameter()]}], lr=0.125)
+    optimizer.load_state_dict(theirs.state_dict())
+    assert [(g["lr"], g["state_bits"], g["masters"]) for g in optimizer.param_groups] == [(0.25, 8, True), (0.125, 32, False)]
+    mine = optim.AdamW([{"params": [first]}, {"params": [second], "state_bits": 8}], lr=0.75)
+    optimizer.load_state_dict(mine.state_dict())  # what it names is loaded
+    assert [(g["lr"], g["state_bits"], g["masters"]) for g in optimizer.param_groups] == [(0.75, 32, False), (0.75, 8, False)]
