@@ -97,7 +97,7 @@ class AdamW(torch.optim.Optimizer):
 
     ``state_bits=8`` keeps the moments of parameters of at least 4096 elements in 8 bits (smaller ones in
     32); ``masters=True`` keeps FP32 weights of BF16 and FP16 parameters, made from the
-    parameters at their first step.  ``capturable=True`` keeps the step count on the
+    parameters at their first step, or at the first one after a state dict without them.  ``capturable=True`` keeps the step count on the
     GPU, for steps in a HIP graph (take one step before capturing); ``lr`` may be an FP32
     tensor of one element on the GPU, to change it between replays.
 
@@ -139,24 +139,26 @@ class AdamW(torch.optim.Optimizer):
     def _own_state(self, p: Tensor, group: dict, shared: dict) -> dict:
         """The parameter's state, made at its first step; `shared`: device step counts made in this call."""
         state = self.state[p]
-        if state:
+        lacks_master = group["masters"] and p.dtype != torch.float32 and "master" not in state  # a loaded state may, too
+        if state and not lacks_master:
             return state
-        if not p.is_cuda:
-            raise RuntimeError("AdamW requires CUDA (ROCm/HIP) device parameters")
-        if torch.cuda.is_current_stream_capturing():
+        if p.is_cuda and torch.cuda.is_current_stream_capturing():
             raise RuntimeError("AdamW's state must exist before a step is captured: take one step first")
-        if group["capturable"]:
-            if p.device not in shared:
-                shared[p.device] = torch.zeros((), dtype=torch.int64, device=p.device)
-            state["step"] = shared[p.device]
-        else:
-            state["step"] = 0
-        eighth = group["state_bits"] == 8 and p.numel() >= _LEAST_OF_8_BITS
-        for name in ("exp_avg", "exp_avg_sq"):
-            state[name] = torch.zeros_like(p, dtype=torch.float8_e4m3fn if eighth else torch.float32)
-            if eighth:
-                state[name + "_scale"] = torch.zeros(-(-p.numel() // BLOCK), dtype=torch.float32, device=p.device)
-        if group["masters"] and p.dtype != torch.float32:
+        if not state:
+            if not p.is_cuda:
+                raise RuntimeError("AdamW requires CUDA (ROCm/HIP) device parameters")
+            if group["capturable"]:
+                if p.device not in shared:
+                    shared[p.device] = torch.zeros((), dtype=torch.int64, device=p.device)
+                state["step"] = shared[p.device]
+            else:
+                state["step"] = 0
+            eighth = group["state_bits"] == 8 and p.numel() >= _LEAST_OF_8_BITS
+            for name in ("exp_avg", "exp_avg_sq"):
+                state[name] = torch.zeros_like(p, dtype=torch.float8_e4m3fn if eighth else torch.float32)
+                if eighth:
+                    state[name + "_scale"] = torch.zeros(-(-p.numel() // BLOCK), dtype=torch.float32, device=p.device)
+        if lacks_master:
             state["master"] = p.detach().to(torch.float32, copy=True)
         return state
 

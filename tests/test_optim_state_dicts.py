@@ -91,3 +91,19 @@ def test_options_that_a_state_dict_does_not_name_stay_as_they_are():
     mine = optim.AdamW([{"params": [first]}, {"params": [second], "state_bits": 8}], lr=0.75)
     optimizer.load_state_dict(mine.state_dict())  # what it names is loaded
     assert [(g["lr"], g["state_bits"], g["masters"]) for g in optimizer.param_groups] == [(0.75, 32, False), (0.75, 8, False)]
+
+
+@pytest.mark.parametrize("dtype", [BF16, torch.float16, FP32])
+def test_masters_that_a_state_dict_lacks_are_made_from_the_parameters_at_the_next_step(dtype):
+    p = _parameter(dtype)
+    optimizer = optim.AdamW([p], masters=True)
+    optimizer.load_state_dict(_torch_dict(dtype))
+    with torch.no_grad():
+        p.copy_(torch.linspace(3.0, 4.0, p.numel()).reshape(p.shape))  # weights that are loaded after the optimizer
+    p.grad = torch.zeros_like(p)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        optimizer.step()
+    state = optimizer.state[p]
+    assert ("master" in state) == (dtype != FP32) and state["exp_avg"].dtype == FP32
+    if dtype != FP32:
+        assert state["master"].dtype == FP32 and torch.equal(state["master"], p.detach().float())
