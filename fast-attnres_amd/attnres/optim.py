@@ -16,7 +16,7 @@ a HIP graph.  Without the built library every call raises.
 
 from __future__ import annotations
 
-from typing import Any, Callable, Iterable, Sequence
+from typing import Any, Callable, Iterable, Iterator, Sequence
 
 import torch
 from torch import Tensor
@@ -42,6 +42,11 @@ def _check_betas(betas: Any) -> tuple[float, float]:
     if not all(0.0 <= beta < 1.0 for beta in pair):
         raise ValueError("betas must be in [0, 1)")
     return pair
+
+
+def _same_order(a: Tensor, b: Tensor) -> bool:
+    """Whether the elements of both, of one shape, lie in one order."""
+    return a.stride() == b.stride() or (a.is_contiguous() and b.is_contiguous())
 
 
 def adamw_step(params: Sequence[Tensor], grads: Sequence[Tensor], exp_avgs: Sequence[Tensor], exp_avg_sqs: Sequence[Tensor], *,
@@ -103,7 +108,7 @@ class AdamW(torch.optim.Optimizer):
 
     State dicts keep the states' dtypes, and those of ``torch.optim.AdamW`` load as 32-bit states.  Options that this
     step does not have (``amsgrad``, ``maximize``, ``differentiable``, a decay that is not decoupled) are refused, in a state
-    dict too.
+    dict too, and so are 8-bit states whose elements lie in another order than their parameter's.
     """
 
     def __init__(self, params: Iterable, lr: float | Tensor = 1e-3, betas: tuple[float, float] = (0.9, 0.999), eps: float = 1e-8,
@@ -225,6 +230,7 @@ class AdamW(torch.optim.Optimizer):
         def before(_optimizer: Any, state_dict: dict) -> None:  # after the caller's hooks, so as they leave it
             for group in state_dict["param_groups"]:
                 self._check_options({**self.defaults, **group})
+            self._check_state(state_dict)
             loaded.update(state_dict)
 
         def after(_optimizer: Any) -> None:  # before the caller's
@@ -241,15 +247,25 @@ class AdamW(torch.optim.Optimizer):
             for hook in hooks:
                 hook.remove()
 
+    def _saved_states(self, state_dict: dict) -> Iterator[tuple[Tensor, dict, dict]]:
+        """(parameter, its group, its saved state) of the parameters that have one."""
+        saved_ids = [i for group in state_dict["param_groups"] for i in group["params"]]
+        for index, (p, group) in zip(saved_ids, [(p, group) for group in self.param_groups for p in group["params"]]):
+            if state_dict["state"].get(index):
+                yield p, group, state_dict["state"][index]
+
+    def _check_state(self, state_dict: dict) -> None:
+        for p, _group, saved in self._saved_states(state_dict):
+            for name in ("exp_avg", "exp_avg_sq"):
+                value = saved.get(name)
+                # a scale is of 256 elements as they lie
+                if value is not None and value.dtype == torch.float8_e4m3fn and not _same_order(value, p):
+                    raise ValueError(f"an 8-bit {name} lies in another order of elements than its parameter")
+
     def _take_state(self, state_dict: dict) -> None:
         """The saved states in the dtypes they were saved in, in place of those that ``torch.optim.Optimizer`` has cast."""
-        saved_ids = [i for group in state_dict["param_groups"] for i in group["params"]]
-        params = [(p, group) for group in self.param_groups for p in group["params"]]
         shared: dict[tuple, Tensor] = {}
-        for index, (p, group) in zip(saved_ids, params):
-            saved = state_dict["state"].get(index)
-            if not saved:
-                continue
+        for p, group, saved in self._saved_states(state_dict):
             state = self.state[p] = {}
             for name in ("exp_avg", "exp_avg_sq", "master"):
                 if name in saved:

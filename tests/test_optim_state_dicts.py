@@ -107,3 +107,34 @@ def test_masters_that_a_state_dict_lacks_are_made_from_the_parameters_at_the_nex
     assert ("master" in state) == (dtype != FP32) and state["exp_avg"].dtype == FP32
     if dtype != FP32:
         assert state["master"].dtype == FP32 and torch.equal(state["master"], p.detach().float())
+
+
+def _eighth_dict(p):
+    """Of this optimizer with 8-bit states, made by hand: numbers as the parameter's elements lie, a scale per 256."""
+    optimizer = optim.AdamW([p], state_bits=8)
+    state = {"step": 3}
+    for name in ("exp_avg", "exp_avg_sq"):
+        state[name] = torch.empty_like(p, dtype=FP32).copy_(torch.arange(p.numel()).reshape(p.shape) % 400).to(FP8)
+        state[name + "_scale"] = torch.arange(1.0, -(-p.numel() // 256) + 1)
+    return {"state": {0: state}, "param_groups": optimizer.state_dict()["param_groups"]}
+
+
+def test_8_bit_states_of_another_order_of_elements_are_refused():
+    """Their scales are of 256 elements as they lie: in another order numbers would meet other blocks' scales."""
+    rows, columns = _parameter(), torch.nn.Parameter(_parameter().detach().T.contiguous().T)
+    assert rows.shape == columns.shape and rows.stride() != columns.stride()
+    for saved, loaded in ((rows, columns), (columns, rows)):
+        optimizer = optim.AdamW([loaded], lr=0.5)
+        with pytest.raises(ValueError, match="order"):
+            optimizer.load_state_dict(_eighth_dict(saved))
+        assert not optimizer.state and optimizer.param_groups[0]["lr"] == 0.5
+    for p in (rows, columns, torch.nn.Parameter(torch.zeros(1, 5000).as_strided((1, 5000), (7, 1)))):
+        saved = _eighth_dict(p)
+        optimizer = optim.AdamW([p])
+        optimizer.load_state_dict(saved)
+        for name, value in saved["state"][0].items():
+            mine = optimizer.state[p][name]
+            assert mine == value if name == "step" else torch.equal(mine.float(), value.float()) and mine.dtype == value.dtype
+    wide = optim.AdamW([columns])
+    wide.load_state_dict(_torch_dict())  # 32-bit states have no blocks
+    assert wide.state[columns]["exp_avg"].stride() == columns.stride()
