@@ -256,10 +256,14 @@ class AdamW(torch.optim.Optimizer):
 
     def _check_state(self, state_dict: dict) -> None:
         for p, _group, saved in self._saved_states(state_dict):
-            for name in ("exp_avg", "exp_avg_sq"):
+            for name in ("exp_avg", "exp_avg_sq", "master"):
                 value = saved.get(name)
+                if value is None:
+                    continue
+                if value.shape != p.shape:
+                    raise ValueError(f"{name} must have the shape of its parameter")
                 # a scale is of 256 elements as they lie
-                if value is not None and value.dtype == torch.float8_e4m3fn and not _same_order(value, p):
+                if value.dtype == torch.float8_e4m3fn and not _same_order(value, p):
                     raise ValueError(f"an 8-bit {name} lies in another order of elements than its parameter")
 
     def _take_state(self, state_dict: dict) -> None:

@@ -138,3 +138,15 @@ def test_8_bit_states_of_another_order_of_elements_are_refused():
     wide = optim.AdamW([columns])
     wide.load_state_dict(_torch_dict())  # 32-bit states have no blocks
     assert wide.state[columns]["exp_avg"].stride() == columns.stride()
+
+
+@pytest.mark.parametrize("name,shape", [("exp_avg", (64,)), ("exp_avg_sq", (1, 64)), ("exp_avg", ()), ("master", (96, 1))])
+def test_states_of_another_shape_are_refused(name, shape):
+    """Also shapes that a copy would broadcast."""
+    p = _parameter(BF16)
+    saved = _torch_dict(BF16)
+    saved["state"][0][name] = torch.ones(shape)
+    optimizer = optim.AdamW([p], lr=0.5, masters=True)
+    with pytest.raises(ValueError, match="shape"):
+        optimizer.load_state_dict(saved)
+    assert not optimizer.state and optimizer.param_groups[0]["lr"] == 0.5
