@@ -120,6 +120,7 @@ LAYER_SIGNATURES = {
         _c_void_p, _c_void_p, _c_void_p, _i64, _c_void_p]),
     "attnres_hip_gated_ffn_saved_bytes": (_i64, [_i64, _i64, _i64, _i64, ctypes.c_int]),
     "attnres_hip_gated_ffn_workspace_bytes": (_i64, [_i64, _i64, _i64, _i64, ctypes.c_int, ctypes.c_int]),
+    "attnres_hip_gated_ffn_plan": (_i64, [_i64, _i64, _i64, _i64, ctypes.c_int, ctypes.c_int, ctypes.c_int]),
     "attnres_hip_gated_ffn_forward": (ctypes.c_int, [
         _c_void_p, _i64, _c_void_p, _i64, _c_void_p, _i64, _i64, _i64, _i64, _i64, ctypes.c_int, ctypes.c_int, _c_void_p,
         _c_void_p, _c_void_p, _i64, _c_void_p]),

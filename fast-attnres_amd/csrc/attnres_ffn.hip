@@ -503,24 +503,33 @@ __global__ void __launch_bounds__(Shape<SHAPE>::kAllThreads, Shape<SHAPE>::kGrou
   else store_tile<Value<X>, SHAPE>(g, tile, acc, lds);
 }
 
-// Passes over rows of chunks of kVec, several tensors in one launch: a workgroup takes whole rows, kChunksOfGroup chunks or one row.
+// Passes over rows of chunks of kVec, several tensors in one launch: a workgroup takes whole rows, kChunksOfGroup chunks or one row,
+// and of a tensor of more than kMaxGroups times that the next ones in turn.
 constexpr int kChunksOfGroup = kBlock;
+constexpr int64_t kMaxGroups = int64_t{1} << 20;  // a launch of four tensors takes 2^30 threads
 
 struct Rows {
   int64_t rows;
-  int chunks;      // of a row
-  uint32_t first;  // workgroup; UINT32_MAX: not there
+  int chunks;       // of a row
+  uint32_t first;   // workgroup; UINT32_MAX: not there
+  uint32_t groups;
   __host__ __device__ int of_group() const { return chunks >= kChunksOfGroup ? 1 : kChunksOfGroup / chunks; }
-  uint32_t groups() const { return static_cast<uint32_t>((rows + of_group() - 1) / of_group()); }
 };
+Rows rows_of(int64_t rows, int64_t chunks, uint32_t first) {
+  Rows r{rows, static_cast<int>(chunks), first, 0};
+  r.groups = static_cast<uint32_t>(std::min((rows + r.of_group() - 1) / r.of_group(), kMaxGroups));
+  return r;
+}
 
 // f(row, chunk) for the workgroup's rows.
 template <class F>
 __device__ __forceinline__ void for_chunks(const Rows& r, F f) {
   const int of_group = r.of_group();
-  const int64_t row0 = static_cast<int64_t>(blockIdx.x - r.first) * of_group;
-  const int here = static_cast<int>(min(static_cast<int64_t>(of_group), r.rows - row0)) * r.chunks;
-  for (int i = threadIdx.x; i < here; i += kBlock) f(row0 + i / r.chunks, i % r.chunks);
+  const int64_t step = static_cast<int64_t>(r.groups) * of_group;
+  for (int64_t row0 = static_cast<int64_t>(blockIdx.x - r.first) * of_group; row0 < r.rows; row0 += step) {
+    const int here = static_cast<int>(min(static_cast<int64_t>(of_group), r.rows - row0)) * r.chunks;
+    for (int i = threadIdx.x; i < here; i += kBlock) f(row0 + i / r.chunks, i % r.chunks);
+  }
 }
 
 // out[r] = the sum of the parts' rows, in order.  Bound by memory: 4096 x 2048 of two parts 13.7 us (6.1 TB/s).
@@ -765,6 +774,7 @@ constexpr int64_t kMaxTiles = int64_t{1} << 22;   // a launch takes fewer than 2
 // 0.603 to 0.496, 8192 x 2048 x 5632 0.990 to 0.943; 4096 x 4096 x 8192 1.21 to 1.20; 16384 x 4096 x 11264 6.17 to 6.23.  Tiles of 128,
 // 2048 x 2048 x 5632: 0.374 to 0.327; FP32 on tiles of 64, 200 x 4096 x 11264: 1.24 to 1.09.
 constexpr uint32_t kTogether = 8;
+inline bool together(int tile, int64_t workgroups) { return tile < 256 || workgroups <= kTogether * kUnits; }
 // Rows, and rows times widths, up to which FP32 inputs are multiplied as they are: FP32 instructions reach 100-115 TFLOP/s, the six products
 // of parts 170 once their operands are packed (22 bytes moved per element of a weight and tile of rows, not 4).  Forward and
 // backward in kernels, by parts in brackets: 512 x 2048 x 4096 0.66 (0.84) ms, 1024 x 1024 x 2816 0.58 (0.62), 2048 x 512 x 512
@@ -1042,9 +1052,9 @@ class Operands {
                 int64_t width_pad) {
     if (!pack) return {{static_cast<const uint16_t*>(x), nullptr, nullptr}, stride, 0, 0, 0};
     PackArgs<X>& g = args_.of[count_++];
-    g = {{halves * half_pad, static_cast<int>(width_pad / kVec), groups_}, static_cast<const Value<X>*>(x), stride, half, half_pad,
+    g = {rows_of(halves * half_pad, width_pad / kVec, groups_), static_cast<const Value<X>*>(x), stride, half, half_pad,
          static_cast<int>(width), {}};
-    groups_ += g.rows.groups();
+    groups_ += g.rows.groups;
     Operand o{{nullptr, nullptr, nullptr}, width_pad, 0, 0, 0};
     for (int k = 0; k < kParts<X>; ++k) o.part[k] = g.to[k] = c_.operand(offsets[k]);
     return o;
@@ -1136,13 +1146,13 @@ void join_parts(const Call& c, const OutArgs (&of)[3], void* const (&results)[3]
   uint32_t groups = 0;
   for (int i = 0; i < 3; ++i) {
     if (results[i] == nullptr || of[i].product.splits == 1) continue;
-    g.rows[count] = {of[i].split_stride / of[i].ld, static_cast<int>(of[i].ld / kVec), groups};
+    g.rows[count] = rows_of(of[i].split_stride / of[i].ld, of[i].ld / kVec, groups);
     g.partial[count] = static_cast<const float*>(of[i].out);
     g.splits[count] = of[i].product.splits;
     g.width[count] = static_cast<int>(of[i].entries_a);
     g.split_stride[count] = of[i].split_stride;
     g.out[count] = static_cast<X*>(results[i]);
-    groups += g.rows[count++].groups();
+    groups += g.rows[count++].groups;
   }
   for (int k = count; k < 3; ++k) g.rows[k].first = UINT32_MAX;
   if (count > 0) hipLaunchKernelGGL((attnres_ffn_join_kernel<X>), dim3(groups), dim3(kBlock), 0, c.stream, g);
@@ -1251,7 +1261,7 @@ void ffn_backward(const Call& c, const void* grad_out, const char* saved, void* 
   std::sort(order, order + 3, [&](int i, int j) { return of[i].product.depth * splits[j] > of[j].product.depth * splits[i]; });
   uint32_t all = 0;
   for (const int i : order) all += results[i] != nullptr ? workgroups(of[i]) : 0;
-  const bool together = tile < 256 || all <= kTogether * kUnits;
+  const bool one_launch = together(tile, all);
   GradientsArgs g{};
   int count = 0;
   uint32_t grid = 0;
@@ -1272,10 +1282,57 @@ void ffn_backward(const Call& c, const void* grad_out, const char* saved, void* 
     g.wide[count] = splits[i] > 1;
     g.first[count++] = grid;
     grid += static_cast<uint32_t>(round_up(workgroups(of[i]), 8));  // whole rounds of the XCDs
-    if (!together) launch();
+    if (!one_launch) launch();
   }
   launch();
   join_parts<Value<X>>(c, of, results);
+}
+
+// What attnres_hip_gated_ffn_plan tells, every gradient being wanted.
+int64_t plan_entry(const Sizes& s, const FfnPlan& p, int pass, int entry) {
+  const bool backward = pass != kForward;
+  const int64_t outputs[3][2] = {{s.width, s.rows}, {s.width, 2 * p.hidden_pad}, {s.hidden, s.out_width}};
+  const Cut& cut = backward ? p.gradients : p.out;
+  const int shape = cut.shape();
+  int64_t products[3] = {}, all = 0, joined = 0;  // workgroups
+  const int count = backward ? 3 : p.few ? 0 : 1;
+  for (int i = 0; i < count; ++i) {
+    const int64_t a = backward ? outputs[i][0] : s.out_width, b = backward ? outputs[i][1] : s.rows;
+    products[i] = tiles_of(a, cut.tile) * tiles_of(b, cut.tile) * cut.splits[i];
+    all += products[i];
+    if (cut.splits[i] > 1) joined += rows_of(backward && i == 1 ? 2 * s.hidden : b, tiles_of(a, kVec), 0).groups;
+  }
+  const bool one_launch = count == 1 || together(cut.tile, all);
+  switch (entry) {
+    case ATTNRES_FFN_GATE_TILE: return p.few || pass == kBackward ? 0 : p.gate.shape();
+    case ATTNRES_FFN_SLOPE_TILE: return backward ? p.slope.shape() : 0;
+    case ATTNRES_FFN_PRODUCT_TILE: return count == 0 ? 0 : shape;
+    case ATTNRES_FFN_PRODUCT_LAUNCHES: return count == 0 ? 0 : one_launch ? 1 : 3;
+    case ATTNRES_FFN_PRODUCT_PARTS: return count == 0 ? 0 : *std::max_element(cut.splits, cut.splits + count);
+    case ATTNRES_FFN_OPERAND_PARTS: return p.single ? 0 : p.parts;
+    default: break;
+  }
+  const auto threads = [](const Cut& of) {
+    const auto shape_threads = [](auto known) { return static_cast<int64_t>(Shape<decltype(known)::value>::kAllThreads); };
+    int64_t result = 0;
+    if (of.tile == 256) return shape_threads(std::integral_constant<int, 256>{});
+    with_shape<Single>(of, [&](auto known) { result = shape_threads(known); });
+    return result;
+  };
+  int64_t packed = 0;
+  const auto pack = [&](bool needed, int64_t rows, int64_t width) {
+    if (needed) packed += rows_of(rows, width / kVec, 0).groups;
+  };
+  pack(p.pack_x, p.rows_pad, p.width_pad);
+  pack(p.pack_gate_up, 2 * p.hidden_pad, p.width_pad);
+  pack(p.pack_down, p.out_pad, p.hidden_pad);
+  pack(p.pack_grad, p.rows_pad, p.out_pad);
+  int64_t most = std::max(packed, joined) * kBlock;
+  const auto product = [&](const Cut& of, int64_t workgroups) { most = std::max(most, workgroups * threads(of)); };
+  if (!p.few && pass != kBackward) product(p.gate, tiles_of(p.hidden_pad, p.gate.tile / 2) * tiles_of(s.rows, p.gate.tile));
+  if (backward) product(p.slope, tiles_of(p.hidden_pad, p.slope.tile) * tiles_of(p.rows_pad, p.slope.tile));
+  for (int i = 0; i < count; ++i) product(cut, one_launch ? all + 3 * 8 : products[i] + 8);
+  return most;
 }
 
 bool known_sizes(const Sizes& s) {
@@ -1343,6 +1400,12 @@ int64_t attnres_hip_gated_ffn_saved_bytes(int64_t rows, int64_t width, int64_t h
 int64_t attnres_hip_gated_ffn_workspace_bytes(int64_t rows, int64_t width, int64_t hidden, int64_t out_width, int dtype, int backward) {
   const Sizes s{rows, width, hidden, out_width, dtype};
   return known_sizes(s) && backward >= kForward && backward <= kBackwardAgain ? ffn_plan(s, backward).bytes : -1;
+}
+
+int64_t attnres_hip_gated_ffn_plan(int64_t rows, int64_t width, int64_t hidden, int64_t out_width, int dtype, int backward, int entry) {
+  const Sizes s{rows, width, hidden, out_width, dtype};
+  if (!known_sizes(s) || rows == 0 || backward < kForward || backward > kBackwardAgain || entry < 0 || entry > ATTNRES_FFN_THREADS) return -1;
+  return plan_entry(s, ffn_plan(s, backward), backward, entry);
 }
 
 int attnres_hip_gated_ffn_forward(const void* x, int64_t x_stride, const void* gate_up, int64_t gate_up_stride, const void* down,

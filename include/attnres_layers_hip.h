@@ -123,6 +123,21 @@ int64_t attnres_hip_gated_ffn_saved_bytes(int64_t rows, int64_t width, int64_t h
 int64_t attnres_hip_gated_ffn_workspace_bytes(int64_t rows, int64_t width, int64_t hidden, int64_t out_width, int dtype,
                                               int backward);
 
+/* Which kernels a call of these sizes takes (backward as above, every gradient wanted), for tests and tuning; -1 for
+ * sizes outside the envelope.  Tiles are 256, 128 or 64 outputs wide, 65 and 66 those of 64 whose depth two and four
+ * times as many wavefronts share, 0: not by tiles, or not in this pass. */
+enum attnres_ffn_plan {
+  ATTNRES_FFN_GATE_TILE = 0,        /* g, u and a */
+  ATTNRES_FFN_SLOPE_TILE = 1,       /* da, dg, du and a */
+  ATTNRES_FFN_PRODUCT_TILE = 2,     /* out, or the three gradients */
+  ATTNRES_FFN_PRODUCT_LAUNCHES = 3, /* for those */
+  ATTNRES_FFN_PRODUCT_PARTS = 4,    /* that a depth is cut into, at most */
+  ATTNRES_FFN_OPERAND_PARTS = 5,    /* 16-bit numbers of an element; 0: FP32 instructions */
+  ATTNRES_FFN_THREADS = 6           /* of the largest launch */
+};
+int64_t attnres_hip_gated_ffn_plan(int64_t rows, int64_t width, int64_t hidden, int64_t out_width, int dtype, int backward,
+                                   int entry);
+
 int attnres_hip_gated_ffn_forward(const void* x, int64_t x_stride, const void* gate_up, int64_t gate_up_stride,
                                   const void* down, int64_t down_stride, int64_t rows, int64_t width, int64_t hidden,
                                   int64_t out_width, int dtype, int activation, void* out, void* saved, void* workspace,
