@@ -391,8 +391,10 @@ def gated_feed_forward(x: Tensor, gate_up: Tensor, down: Tensor, *, activation: 
 
     Sums are FP32, and so are the projections that the activation is formed from.  What the
     second product multiplies, and in the backward the gradients of both projections, is
-    rounded to 16-bit inputs' type.  FP32 inputs are multiplied in FP32, or in large
-    calls as sums of three BF16 numbers, with FP32's 24 bits; infinities may count as NaN.
+    rounded to 16-bit inputs' type; FP16's, where upstream gradients are below 1/4, times a power
+    of two that keeps its 11 bits, and infinite beyond 2^17 times the largest of those (else 65504).
+    FP32 inputs are multiplied in FP32, or in large calls as sums of three BF16 numbers, with
+    FP32's 24 bits; infinities may count as NaN.
 
     Gradients flow to all three.  For them the forward keeps both projections, 6 bytes per
     row and hidden entry each pair (FP32: 8), in every live graph; with ``recompute=True``
