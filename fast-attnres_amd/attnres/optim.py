@@ -184,7 +184,8 @@ class AdamW(torch.optim.Optimizer):
             raise RuntimeError("AdamW must be built with capturable=True for a step that is captured")
         buckets: dict[tuple, list] = {}
         shared: dict = {}
-        counts: dict[int, Tensor] = {}
+        counts: dict[int, Tensor] = {}  # on the device, by id
+        taken: set[int] = set()         # counts whose step was made; a step that is refused is not counted
         for p in group["params"]:
             if p.grad is None:
                 continue
@@ -196,7 +197,7 @@ class AdamW(torch.optim.Optimizer):
                 counts[id(count)] = count
                 key = id(count)
             else:
-                key = state["step"] = count + 1
+                key = count + 1
             buckets.setdefault((p.device, p.dtype, p.grad.dtype, state["exp_avg"].dtype, "master" in state, key), []).append((p, state))
         if counts:
             # parameters without a gradient that share a count with others keep theirs
@@ -211,15 +212,26 @@ class AdamW(torch.optim.Optimizer):
                     self.state[p]["step"] = left[id(count)]
             for count in counts.values():
                 count.add_(1)
-        for (_device, _dtype, _grad, kind, has_master, _key), members in buckets.items():
-            states = [state for _, state in members]
-            eighth = kind == torch.float8_e4m3fn
-            adamw_step([p for p, _ in members], [p.grad for p, _ in members], [s["exp_avg"] for s in states],
-                       [s["exp_avg_sq"] for s in states], step=states[0]["step"], lr=group["lr"], betas=group["betas"],
-                       eps=group["eps"], weight_decay=group["weight_decay"],
-                       exp_avg_scales=[s["exp_avg_scale"] for s in states] if eighth else None,
-                       exp_avg_sq_scales=[s["exp_avg_sq_scale"] for s in states] if eighth else None,
-                       masters=[s["master"] for s in states] if has_master else None, grad_scale=grad_scale)
+        try:
+            for (_device, _dtype, _grad, kind, has_master, key), members in buckets.items():
+                states = [state for _, state in members]
+                count = counts.get(key)
+                eighth = kind == torch.float8_e4m3fn
+                adamw_step([p for p, _ in members], [p.grad for p, _ in members], [s["exp_avg"] for s in states],
+                           [s["exp_avg_sq"] for s in states], step=key if count is None else count, lr=group["lr"], betas=group["betas"],
+                           eps=group["eps"], weight_decay=group["weight_decay"],
+                           exp_avg_scales=[s["exp_avg_scale"] for s in states] if eighth else None,
+                           exp_avg_sq_scales=[s["exp_avg_sq_scale"] for s in states] if eighth else None,
+                           masters=[s["master"] for s in states] if has_master else None, grad_scale=grad_scale)
+                taken.add(key)
+                if count is None:
+                    for state in states:
+                        state["step"] = key
+        except Exception:
+            for key, count in counts.items():
+                if key not in taken:
+                    count.sub_(1)
+            raise
 
     def load_state_dict(self, state_dict: dict) -> None:
         """As in ``torch.optim.Optimizer``, hooks included, but that the states keep the dtypes they were saved in,

@@ -46,3 +46,38 @@ def test_masters_of_a_loaded_state_without_them(dtype, capturable):
     assert int(state["step"]) == 4
     assert torch.equal(p, param) and torch.equal(state["exp_avg"], mean) and torch.equal(state["exp_avg_sq"], square)
     assert torch.equal(state["master"], master) and not torch.equal(master, param.float())
+
+
+@pytest.mark.parametrize("capturable", [False, True])
+def test_steps_that_are_refused_are_not_counted(capturable):
+    """Of two groups the second one's parameter and state overlap: the first is stepped and counted, the second neither."""
+    first, second = (torch.nn.Parameter(torch.ones(40, device="cuda").to(dtype)) for dtype in (BF16, FP32))
+    optimizer = optim.AdamW([{"params": [first]}, {"params": [second]}], capturable=capturable)
+    for p in (first, second):
+        p.grad = torch.ones_like(p)
+    optimizer.step()
+    held = optimizer.state[second]["exp_avg"]
+    optimizer.state[second]["exp_avg"] = second.detach()
+    before = second.detach().clone()
+    with pytest.raises(ValueError, match="overlap"):
+        optimizer.step()
+    assert [int(optimizer.state[p]["step"]) for p in (first, second)] == [2, 1]
+    optimizer.state[second]["exp_avg"] = held
+    assert torch.equal(second, before)
+    optimizer.step()
+    assert [int(optimizer.state[p]["step"]) for p in (first, second)] == [3, 2]
+
+
+def test_a_refused_step_of_a_shared_count():
+    """Parameters of two types share a count on the device; it is taken back where none of them was stepped."""
+    first, second = (torch.nn.Parameter(torch.ones(40, device="cuda").to(dtype)) for dtype in (BF16, FP32))
+    optimizer = optim.AdamW([first, second], capturable=True)
+    for p in (first, second):
+        p.grad = torch.ones_like(p)
+    optimizer.step()
+    assert optimizer.state[first]["step"] is optimizer.state[second]["step"]
+    with pytest.raises(TypeError, match="grad_scale"):
+        optimizer.step(grad_scale=torch.ones(1, device="cuda", dtype=BF16))
+    assert int(optimizer.state[first]["step"]) == 1
+    optimizer.step()
+    assert int(optimizer.state[first]["step"]) == 2

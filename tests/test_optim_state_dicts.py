@@ -150,3 +150,21 @@ def test_states_of_another_shape_are_refused(name, shape):
     with pytest.raises(ValueError, match="shape"):
         optimizer.load_state_dict(saved)
     assert not optimizer.state and optimizer.param_groups[0]["lr"] == 0.5
+
+
+def test_steps_that_are_refused_are_not_counted():
+    """On the CPU every step is; so is one that meets a sparse gradient after others."""
+    first, second = _parameter(), _parameter()
+    optimizer = optim.AdamW([first, second])
+    theirs = torch.optim.AdamW([_parameter(), _parameter()])
+    for p in theirs.param_groups[0]["params"]:
+        p.grad = torch.ones_like(p)
+    theirs.step()
+    optimizer.load_state_dict(theirs.state_dict())
+    first.grad = second.grad = torch.ones_like(first)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        optimizer.step()
+    second.grad = torch.ones_like(second).to_sparse()
+    with pytest.raises(RuntimeError, match="dense"):
+        optimizer.step()
+    assert [optimizer.state[p]["step"] for p in (first, second)] == [1, 1]
