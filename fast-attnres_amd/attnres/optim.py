@@ -73,7 +73,7 @@ def adamw_step(params: Sequence[Tensor], grads: Sequence[Tensor], exp_avgs: Sequ
     the same way.  They are rounded to nearest, relative to the block's largest magnitude over 448 (3 bits of
     mantissa, half of the least number at 2^-19 of the largest); a root above zero is never
     rounded to zero.  A gradient that is not finite makes its element NaN or infinite, and the
-    8-bit moments of its block NaN.
+    8-bit moments of its block NaN; one whose square leaves FP32, the block's second moment.
 
     ``masters`` are FP32 weights of 16-bit parameters: w above, of which the parameters get the
     rounded values.  Without them 16-bit parameters are read, and the new ones rounded to nearest.

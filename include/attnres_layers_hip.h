@@ -144,7 +144,9 @@ int attnres_hip_gated_ffn_forward(const void* x, int64_t x_stride, const void* g
                                   int64_t workspace_bytes, void* stream);
 
 /* grad_out [rows, out_width] contiguous; grad_x [rows, width], grad_gate_up [2 hidden, width] and grad_down
- * [out_width, hidden] contiguous, of dtype; each may be NULL when it is not wanted.  rows >= 1. */
+ * [out_width, hidden] contiguous, of dtype; each may be NULL when it is not wanted.  rows >= 1.  The gradients of g and
+ * u are rounded to 16-bit inputs' type, of FP16 times a power of two where grad_out's largest finite magnitude is below 1/4
+ * (which takes it to between 1/4 and 1/2). */
 int attnres_hip_gated_ffn_backward(const void* grad_out, const void* x, int64_t x_stride, const void* gate_up,
                                    int64_t gate_up_stride, const void* down, int64_t down_stride, int64_t rows,
                                    int64_t width, int64_t hidden, int64_t out_width, int dtype, int activation,

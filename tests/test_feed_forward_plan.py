@@ -52,3 +52,19 @@ def test_sizes_of_the_gpu_tests_launch_every_kernel(sizes, dtype):
                 assert ("out", operand, tile, cut) in reached, (tile, cut)
                 assert ("gradients", operand, tile, cut) in reached or (operand, tile) == (3, 66), (tile, cut)
         assert {("launches", operand, n) for n in ((1, 3) if operand else (1,))} <= reached
+
+
+@pytest.mark.parametrize("sizes,dtype,backward,entry", [
+    ((0, 8, 8, 8), BF16, FORWARD, THREADS), ((4, 8193, 8, 8), BF16, FORWARD, THREADS), ((4, 8, 8, 0), BF16, FORWARD, THREADS),
+    ((2**24 + 1, 8, 8, 8), BF16, FORWARD, THREADS), ((4, 8, 8, 8), 3, FORWARD, THREADS), ((4, 8, 8, 8), BF16, 3, THREADS),
+    ((4, 8, 8, 8), BF16, -1, THREADS), ((4, 8, 8, 8), BF16, FORWARD, THREADS + 1), ((4, 8, 8, 8), BF16, FORWARD, -1)])
+def test_plans_outside_the_envelope(sizes, dtype, backward, entry):
+    assert plan(sizes, dtype, backward, entry) == -1
+
+
+def test_plans_of_few_rows():
+    """By kernels that take no tiles, forwards alone."""
+    sizes = (1, 1024, 2816, 1024)
+    assert [plan(sizes, BF16, FORWARD, e) for e in range(OPERAND_PARTS)] == [0] * 5
+    assert plan(sizes, BF16, BACKWARD, GATE_TILE) == 0 and plan(sizes, BF16, BACKWARD, SLOPE_TILE) > 0
+    assert plan(sizes, BF16, BACKWARD, PRODUCT_LAUNCHES) == 1 and plan(sizes, FP32, FORWARD, OPERAND_PARTS) == 0
